@@ -274,6 +274,84 @@ int sc_attn_decode(const float* qkv, int B, int Hq, int Hkv, int hd, const int32
                    void* out, int out_dtype, void* workspace, size_t workspace_bytes,
                    int32_t* tickets, cudaStream_t stream);
 
+/* ------------------------------------------------------------ paged cache --
+ * A KV cache as a pool of pages k_pages / v_pages [n_pages, Hkv, page, hd],
+ * shared by requests of any lengths.  Request b's token i lies in page
+ * block_table[b * max_blocks + i / page] at offset i % page; that page id
+ * times page plus the offset is the token's slot.  Pages that no request
+ * holds lie on a stack, free_pages[0 .. *free_count).  A prefix that the
+ * whole batch shares lies in pages of its own (prefix_table), ahead of every
+ * request's tokens; its last page need not be full.  All lengths, tables and
+ * counts are int32 in device memory, so that a captured step follows them.
+ * No counterpart in the reference, whose cache grows by concatenation
+ * (parallel/attention.py:427-436).
+ *
+ * sc_paged_reserve: room for new_lens[b] more tokens after the lens[b] of
+ * each request (1..16384 requests).  Pages are taken from the stack's top in
+ * the order of requests and blocks and written into block_table.  Writes
+ *   kv_lens[B]      lens + new_lens (may be lens itself)
+ *   q_start[B + 1]  the requests' rows: request b has rows q_start[b] .. q_start[b + 1)
+ *   slots, positions [max_tokens]: per row its slot and its position, which
+ *                   is *prefix_len (0 if NULL) + its place in the request;
+ *                   rows from q_start[B] on are left as they were
+ *   free_count_out  pages left (may be free_count itself)
+ *   status          0, or the sum of 1 (not enough pages), 2 (a request
+ *                   exceeds max_blocks pages), 4 (more than max_tokens new
+ *                   tokens), 8 (a negative length), 16 (free_count outside
+ *                   0..n_free).  Unless it is 0 nothing is reserved: the
+ *                   table and the count stay, kv_lens = lens, q_start = 0,
+ *                   slots and positions are left as they were.
+ * free_pages holds n_free entries. */
+int sc_paged_reserve(const int32_t* lens, const int32_t* new_lens, int B, const int32_t* prefix_len,
+                     int32_t* block_table, int max_blocks, const int32_t* free_pages, int n_free,
+                     const int32_t* free_count, int page_size, int max_tokens, int32_t* kv_lens, int32_t* q_start,
+                     int32_t* slots, int32_t* positions, int32_t* free_count_out, int32_t* status,
+                     cudaStream_t stream);
+/* Cuts request b to its first keep[b] tokens (0: it has ended; rejected
+ * drafts: its accepted length; clamped to 0..lens[b]).  Pages that hold no
+ * token any more go onto the stack in the order of requests and blocks; the
+ * table's entries behind a request's length are not cleared and never read.
+ * lens_out may be lens, free_count_out may be free_count.  status as above,
+ * 1: the stack has no room for them (a page given back twice); unless it is 0
+ * nothing changes. */
+int sc_paged_truncate(const int32_t* lens, const int32_t* keep, int B, const int32_t* block_table, int max_blocks,
+                      int32_t* free_pages, int n_free, const int32_t* free_count, int page_size, int32_t* lens_out,
+                      int32_t* free_count_out, int32_t* status, cudaStream_t stream);
+/* sc_rope_append for a paged cache: rotates q and k of each row at its
+ * position and writes k and v to its slot.  qkv [rows, (Hq + 2 Hkv) * hd],
+ * fp32 or fp16; q_out [rows, Hq * hd] and the pools in cache_dtype (fp32 or
+ * fp16), rounded once.  Rows from *rows_end on (q_start + B) are left as they
+ * were.  A slot outside the pool or a position outside 0..max_pos-1 is not
+ * written to (at such a position q is not rotated).  The slots of one call
+ * differ.  hd a multiple of 8; all tensors on 16-byte boundaries. */
+int sc_paged_rope_append(const void* qkv, int qkv_dtype, int rows, const int32_t* rows_end, const int32_t* slots,
+                         const int32_t* positions, const float* cos_tab, const float* sin_tab, int max_pos, int Hq,
+                         int Hkv, int hd, void* q_out, void* k_pages, void* v_pages, int cache_dtype, int n_pages,
+                         int page_size, cudaStream_t stream);
+/* Attention behind a shared prefix, causal over each request's own tokens:
+ * row q_start[b] + i of request b (n rows) sees the *prefix_len tokens of
+ * prefix_table and its own tokens 0 .. kv_lens[b] - n + i.  Decoding (n = 1),
+ * drafts and prompt chunks alike; query head j reads kv head j / (Hq / Hkv).
+ *   q, out [T, Hq * hd], k_pages, v_pages: all fp16 or all fp32 (dtype);
+ *   hd 64 or 128; page_size a power of two, 16 or more; scale > 0.
+ *   prefix_len NULL: no prefix.  Rows from q_start[B] on are left as they
+ *   were; a row that sees no token is zero.  Pages whose id is outside
+ *   0..n_pages-1 count as absent: their tokens are not seen.  What lies in a
+ *   page behind a request's last token has no influence, whatever it is.
+ * Softmax statistics and sums are fp32; with fp16 the weights are rounded to
+ * fp16 before their product with v. */
+size_t sc_prefix_attn_workspace_bytes(int T, int B, int Hq, int Hkv, int hd, int max_blocks, int max_prefix_blocks,
+                                      int page_size, int dtype);
+int sc_prefix_attn(const void* q, const void* k_pages, const void* v_pages, int dtype, int T, const int32_t* q_start,
+                   const int32_t* kv_lens, const int32_t* block_table, int B, int max_blocks,
+                   const int32_t* prefix_table, const int32_t* prefix_len, int max_prefix_blocks, int Hq, int Hkv,
+                   int hd, int n_pages, int page_size, float scale, void* out, void* workspace, size_t workspace_bytes,
+                   cudaStream_t stream);
+/* Device-side error word of sc_prefix_attn: nonzero after a CTA gave up a
+ * bounded wait for its tiles (its rows are then undefined).  Synchronises
+ * with the device; reset != 0 clears it. */
+int sc_prefix_attn_device_error(int reset);
+
 /* ------------------------------------------------------------------ K5 --
  * RMSNorm (parallel/transformer.py:46-61): y = x / sqrt(mean(x^2)+eps) * w. */
 int sc_rmsnorm(const void* x, int x_dtype, int M, int H, const uint16_t* w, float eps,

@@ -55,6 +55,13 @@ SIGNATURES = {
     "sc_attn_device_error": (_i, [_i]),
     "sc_attn_decode": (_i, [_vp, _i, _i, _i, _i, _vp, _vp, _vp, _i, _vp, _vp, _i, _f, _i, _vp, _i, _vp, _sz, _vp,
                             _vp]),
+    "sc_paged_reserve": (_i, [_vp, _vp, _i, _vp, _vp, _i, _vp, _i, _vp, _i, _i, _vp, _vp, _vp, _vp, _vp, _vp, _vp]),
+    "sc_paged_truncate": (_i, [_vp, _vp, _i, _vp, _i, _vp, _i, _vp, _i, _vp, _vp, _vp, _vp]),
+    "sc_paged_rope_append": (_i, [_vp, _i, _i, _vp, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _vp, _vp, _vp, _i, _i, _i, _vp]),
+    "sc_prefix_attn_workspace_bytes": (_sz, [_i, _i, _i, _i, _i, _i, _i, _i, _i]),
+    "sc_prefix_attn": (_i, [_vp, _vp, _vp, _i, _i, _vp, _vp, _vp, _i, _i, _vp, _vp, _i, _i, _i, _i, _i, _i, _f, _vp,
+                            _vp, _sz, _vp]),
+    "sc_prefix_attn_device_error": (_i, [_i]),
     "sc_rmsnorm": (_i, [_vp, _i, _i, _i, _vp, _f, _vp, _i, _vp]),
     "sc_silu_mul": (_i, [_vp, _vp, _i, _sz, _vp, _i, _vp]),
     "sc_add": (_i, [_vp, _i, _vp, _i, _sz, _vp, _i, _vp]),

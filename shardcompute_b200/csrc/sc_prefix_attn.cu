@@ -1,0 +1,644 @@
+// Attention of a ragged batch over a paged cache whose requests share a
+// prefix: row i of request b (n new tokens, len tokens with them) sees the
+// prefix's keys [0, P) and its own tokens [0, len - n + i].
+//
+//   o = sum_j exp(scale q.k_j - m) v_j / sum_j exp(scale q.k_j - m)
+//
+// over the keys it sees; m is any bound of the exponents, so a key range can
+// be summed apart (o, l, m) and joined later.  A row that sees no key is zero.
+#include <algorithm>
+
+#include <cuda.h>
+#include <cudaTypedefs.h>
+
+#include "sc_common.cuh"
+
+namespace sc {
+
+constexpr uint64_t PA_WAIT_NS = 2000000000ull;
+
+// Raised by a kernel whose bounded wait ran out; read by
+// sc_prefix_attn_device_error.
+__device__ int g_prefix_attn_error = 0;
+
+struct PrefixAttnParams {
+  const void* q;       // [T, Hq * HD] in the cache's type
+  void* out;           // [T, Hq * HD] in the cache's type
+  float* part_o;       // [nslots, T * Hq, HD]: sum of 2^(c (s - m)) v
+  float2* part_ml;     // [nslots, T * Hq]: (c m, sum of 2^(c (s - m))); (-inf, 0) where the slot saw no key
+  const int32_t *q_start, *kv_lens, *block_table, *prefix_table, *prefix_len;
+  int T, B, max_blocks, max_prefix_blocks, n_pages, lg_page, Hq, Hkv, G;
+  int pool_rows;       // n_pages * Hkv * page: one past the last row of the pools' tensor maps
+  float c;             // scale * log2(e)
+  int nslots;          // partial results per row, all kernels of the call together
+};
+
+struct PoolMaps {
+  CUtensorMap k, v;
+};
+
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+// The request's rows [lo, hi) in q, clamped so that no device value leads out of bounds.
+__device__ __forceinline__ void request_rows(const PrefixAttnParams& p, int b, int& lo, int& hi) {
+  lo = min(max(p.q_start[b], 0), p.T);
+  hi = min(max(p.q_start[b + 1], lo), p.T);
+}
+__device__ __forceinline__ int request_len(const PrefixAttnParams& p, int b) {
+  const long long cap = (long long)p.max_blocks << p.lg_page;
+  return (int)min((long long)max(p.kv_lens[b], 0), cap);
+}
+__device__ __forceinline__ int prefix_keys(const PrefixAttnParams& p) {
+  if (!p.prefix_len) return 0;
+  const long long cap = (long long)p.max_prefix_blocks << p.lg_page;
+  return (int)min((long long)max(*p.prefix_len, 0), cap);
+}
+
+// 3-D copy of `rows` pool rows (all 128-byte column chunks) into shared memory, completing on `bar`.
+__device__ __forceinline__ void tma3d(void* dst, const CUtensorMap* map, int row, uint64_t* bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::
+          "r"(smem_u32(dst)),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(0), "r"(row), "r"(0), "r"(smem_u32(bar))
+      : "memory");
+}
+
+// ---------------------------------------------------------------- few rows
+
+// Kernel for few rows per request.  A CTA takes a request, a kv head, a share
+// of the keys and every row_groups-th tile of rows; its warps take 16-key tiles in turn, each with its own
+// ring of tiles in shared memory (one TMA copy of K and one of V per tile, a
+// tile never straddles a page) and its own running (m, l, o), so no barrier
+// stands in the loop.  The warps' results are joined at the end.
+//
+// fp16: mma m16n8k16 over up to 16 rows (the request's tokens x the group's
+// heads).  P is rounded to fp16 for the second product: 2^-11 relative per
+// weight at most, on the order of the output's own rounding.
+// fp32: every operand is split into two tf32 parts (split_tf32); up to 8 rows
+// lie in the 16-row fragment as [hi; lo], so two tf32 products (with K's hi
+// and its lo) give all four terms.  A value that is not finite gives NaN.
+constexpr int FR_WARPS = 4;
+constexpr int FR_KT = 16;  // keys per tile
+
+template <typename T, int HD>
+struct FewRows {
+  static constexpr bool F16 = sizeof(T) == 2;
+  static constexpr int RT = F16 ? 16 : 8;                   // rows per tile
+  static constexpr int NB = HD * (int)sizeof(T) / 128;      // 128-byte chunks per key
+  static constexpr int TILE = NB * FR_KT * 128;             // bytes of a K or V tile
+  static constexpr int STAGE = 2 * TILE;
+  static constexpr int NST = F16 ? (HD == 128 ? 3 : 6) : 3; // stages per warp
+  static constexpr int SMEM = FR_WARPS * NST * STAGE + 1024;
+};
+
+__device__ __forceinline__ void ldsm4(uint32_t a, uint32_t (&r)[4]) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(a));
+}
+__device__ __forceinline__ void ldsm4_t(uint32_t a, uint32_t (&r)[4]) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(a));
+}
+// D(16x8, fp32) += A(16x8, tf32) * B(8x8, tf32); the operands' low 13 bits are not used.
+__device__ __forceinline__ void mma_1688(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+// x = hi + lo: hi is x rounded to tf32's 11 bits, lo the exact rest, of which the products use 11 bits too (what
+// they drop is below 2^-21 of x, on either side of zero).  An x that is not finite has a lo that is NaN.
+__device__ __forceinline__ void split_tf32(float x, uint32_t& hi, uint32_t& lo) {
+  hi = (__float_as_uint(x) + 0x1000u) & 0xffffe000u;
+  lo = __float_as_uint(x - __uint_as_float(hi));
+}
+
+template <typename T, int HD>
+__global__ void __launch_bounds__(FR_WARPS * 32)
+few_rows_kernel(const PrefixAttnParams p, const __grid_constant__ PoolMaps maps, int with_prefix, int splits, int row_groups,
+                int slot0) {
+  using C = FewRows<T, HD>;
+  constexpr int RT = C::RT, NST = C::NST;
+  extern __shared__ __align__(1024) unsigned char fr_smem[];
+  __shared__ __align__(8) uint64_t full[FR_WARPS][NST];
+  __shared__ float s_m[FR_WARPS][RT], s_l[FR_WARPS][RT];
+  __shared__ int s_abort;
+  unsigned char* base = fr_smem + ((1024 - (smem_u32(fr_smem) & 1023)) & 1023);
+  const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
+  const int q4 = lane & 3, r8 = lane >> 2;
+  const int split = blockIdx.x % splits, group = blockIdx.x / splits, h = blockIdx.y, b = blockIdx.z;
+  if (threadIdx.x == 0) {
+    for (int w = 0; w < FR_WARPS; ++w)
+      for (int s = 0; s < NST; ++s) mbar_init(&full[w][s], 1);
+    s_abort = 0;
+    fence_mbar_init();
+  }
+  __syncthreads();
+  pdl_trigger();
+  pdl_wait();
+  int row_lo, row_hi;
+  request_rows(p, b, row_lo, row_hi);
+  const int n = row_hi - row_lo, len = request_len(p, b), P = with_prefix ? prefix_keys(p) : 0;
+  const int np = (P + FR_KT - 1) / FR_KT;
+  unsigned char* ring = base + (size_t)warp * NST * C::STAGE;
+  const uint32_t ring_u = smem_u32(ring);
+  uint32_t issued = 0, used = 0;  // tiles of this warp's ring, over all row tiles
+
+  for (int r0 = group * RT; r0 < n * p.G; r0 += row_groups * RT) {
+    const int nr = min(RT, n * p.G - r0);
+    // own keys that the tile's last row sees
+    const int own = max(0, min(len, len - n + (r0 + nr - 1) / p.G + 1));
+    const int nt = np + (own + FR_KT - 1) / FR_KT;
+    const int per = (nt + splits - 1) / splits;
+    const int t_lo = min(nt, split * per), t_hi = min(nt, t_lo + per);
+    const int cnt = max(0, (t_hi - t_lo - warp + FR_WARPS - 1) / FR_WARPS);  // tiles t_lo + warp + 4 i
+
+    // the pool rows of this warp's tiles i = base .. base + 31, one per lane; -1: no such page
+    auto rows_of = [&](int first) {
+      const int t = t_lo + warp + FR_WARPS * (first + lane);
+      if (t >= t_hi) return -1;
+      const bool pre = t < np;
+      const int key = (pre ? t : t - np) * FR_KT;
+      const int blk = key >> p.lg_page;
+      const int id = pre ? p.prefix_table[blk] : p.block_table[(size_t)b * p.max_blocks + blk];
+      if (id < 0 || id >= p.n_pages) return -1;
+      return ((id * p.Hkv + h) << p.lg_page) + (key & ((1 << p.lg_page) - 1));
+    };
+    int rows = rows_of(0);
+    uint32_t absent = 0;  // stages whose tile has no page
+    auto issue = [&](int i) {
+      if (i && (i & 31) == 0) rows = rows_of(i);
+      const int r = __shfl_sync(0xffffffffu, rows, i & 31);
+      const int s = issued % NST;
+      absent = (absent & ~(1u << s)) | ((r < 0 ? 1u : 0u) << s);
+      if (lane == 0) {
+        mbar_arrive_expect_tx(&full[warp][s], C::STAGE);
+        const int at = r < 0 ? p.pool_rows : r;  // past the end: zeros
+        tma3d(ring + s * C::STAGE, &maps.k, at, &full[warp][s]);
+        tma3d(ring + s * C::STAGE + C::TILE, &maps.v, at, &full[warp][s]);
+      }
+      ++issued;
+    };
+    for (int i = 0; i < min(NST, cnt); ++i) issue(i);
+
+    // ---- q fragments
+    uint32_t qa[C::F16 ? HD / 16 : HD / 8][4];
+    auto q_row = [&](int r) {  // tile row -> its q, null past the last
+      if (r >= nr) return (const T*)nullptr;
+      const int tok = row_lo + (r0 + r) / p.G, g = (r0 + r) % p.G;
+      return reinterpret_cast<const T*>(p.q) + ((size_t)tok * p.Hq + h * p.G + g) * HD;
+    };
+    if constexpr (C::F16) {
+      const T *qx = q_row(r8), *qy = q_row(r8 + 8);
+#pragma unroll
+      for (int ks = 0; ks < HD / 16; ++ks) {
+        const int d = ks * 16 + q4 * 2;
+        qa[ks][0] = qx ? *reinterpret_cast<const uint32_t*>(qx + d) : 0u;
+        qa[ks][1] = qy ? *reinterpret_cast<const uint32_t*>(qy + d) : 0u;
+        qa[ks][2] = qx ? *reinterpret_cast<const uint32_t*>(qx + d + 8) : 0u;
+        qa[ks][3] = qy ? *reinterpret_cast<const uint32_t*>(qy + d + 8) : 0u;
+      }
+    } else {
+      const T* qx = q_row(r8);
+#pragma unroll
+      for (int dd = 0; dd < HD / 32; ++dd)
+#pragma unroll
+        for (int s = 0; s < 2; ++s) {  // chunk 2 q4 + s of the 32 values: two steps of k
+          float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+          if (qx) v = *reinterpret_cast<const float4*>(qx + dd * 32 + (2 * q4 + s) * 4);
+          const int ks = dd * 4 + s * 2;
+          split_tf32(v.x, qa[ks][0], qa[ks][1]);
+          split_tf32(v.y, qa[ks][2], qa[ks][3]);
+          split_tf32(v.z, qa[ks + 1][0], qa[ks + 1][1]);
+          split_tf32(v.w, qa[ks + 1][2], qa[ks + 1][3]);
+        }
+    }
+    // own keys each of this thread's rows sees (rows past the last: as the last, so they ask for no mask)
+    const int see0 = r8 < nr ? max(0, len - n + (r0 + r8) / p.G + 1) : own;
+    const int see1 = r8 + 8 < nr ? max(0, len - n + (r0 + r8 + 8) / p.G + 1) : own;
+
+    constexpr int NO = HD / 8;
+    float o[NO][4];
+#pragma unroll
+    for (int i = 0; i < NO; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
+    float m0 = -INFINITY, m1 = -INFINITY, l0 = 0.f, l1 = 0.f;
+
+    for (int i = 0; i < cnt; ++i, ++used) {
+      const int s = used % NST;
+      if (!mbar_wait_warp(&full[warp][s], (used / NST) & 1u, &s_abort, PA_WAIT_NS)) break;
+      const uint32_t ks_u = ring_u + s * C::STAGE, vs_u = ks_u + C::TILE;
+      const int t = t_lo + warp + FR_WARPS * i;
+      const bool gone = (absent >> s) & 1u;
+      // keys of this tile that each row sees, and that any row sees
+      const int first = (t < np ? t : t - np) * FR_KT;
+      const int lim0 = gone ? 0 : (t < np ? P : see0) - first, lim1 = gone ? 0 : (t < np ? P : see1) - first;
+      const int lim = gone ? 0 : (t < np ? P : own) - first;
+      const bool part = __any_sync(0xffffffffu, lim0 < FR_KT || (C::F16 && lim1 < FR_KT));
+
+      float sc[2][4];
+#pragma unroll
+      for (int j = 0; j < 2; ++j) sc[j][0] = sc[j][1] = sc[j][2] = sc[j][3] = 0.f;
+      if constexpr (C::F16) {
+        const int row = ((lane >> 4) << 3) + (lane & 7);
+        const uint32_t ra = ks_u + row * 128;
+#pragma unroll
+        for (int ks = 0; ks < HD / 16; ++ks) {
+          const int ch = ks * 2 + ((lane >> 3) & 1);
+          uint32_t kb[4];
+          ldsm4(ra + (ch >> 3) * (FR_KT * 128) + (((ch & 7) ^ (row & 7)) << 4), kb);
+          mma_16816(sc[0], qa[ks][0], qa[ks][1], qa[ks][2], qa[ks][3], kb[0], kb[1]);
+          mma_16816(sc[1], qa[ks][0], qa[ks][1], qa[ks][2], qa[ks][3], kb[2], kb[3]);
+        }
+      } else {
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          const int key = j * 8 + r8;
+          const uint32_t ra = ks_u + key * 128;
+#pragma unroll
+          for (int dd = 0; dd < HD / 32; ++dd)
+#pragma unroll
+            for (int c2 = 0; c2 < 2; ++c2) {
+              const float4 v = lds_f4(ra + dd * (FR_KT * 128) + (((2 * q4 + c2) ^ (key & 7)) << 4));
+              uint32_t hi[4], lo[4];
+              split_tf32(v.x, hi[0], lo[0]);
+              split_tf32(v.y, hi[1], lo[1]);
+              split_tf32(v.z, hi[2], lo[2]);
+              split_tf32(v.w, hi[3], lo[3]);
+              const int ks = dd * 4 + c2 * 2;
+              mma_1688(sc[j], qa[ks], lo[0], lo[1]);
+              mma_1688(sc[j], qa[ks], hi[0], hi[1]);
+              mma_1688(sc[j], qa[ks + 1], lo[2], lo[3]);
+              mma_1688(sc[j], qa[ks + 1], hi[2], hi[3]);
+            }
+          sc[j][0] += sc[j][2];  // rows 8..15 of the fragment: q's low parts
+          sc[j][1] += sc[j][3];
+        }
+      }
+      if (part) {
+#pragma unroll
+        for (int j = 0; j < 2; ++j)
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            const int key = j * 8 + q4 * 2 + e;
+            if (key >= lim0) sc[j][e] = -INFINITY;
+            if (C::F16 && key >= lim1) sc[j][2 + e] = -INFINITY;
+          }
+      }
+      // ---- running softmax
+      float x0 = fmaxf(fmaxf(sc[0][0], sc[0][1]), fmaxf(sc[1][0], sc[1][1]));
+      float x1 = fmaxf(fmaxf(sc[0][2], sc[0][3]), fmaxf(sc[1][2], sc[1][3]));
+#pragma unroll
+      for (int d = 1; d <= 2; d <<= 1) {
+        x0 = fmaxf(x0, __shfl_xor_sync(0xffffffffu, x0, d));
+        if (C::F16) x1 = fmaxf(x1, __shfl_xor_sync(0xffffffffu, x1, d));
+      }
+      x0 = fmaxf(m0, x0 * p.c);
+      x1 = C::F16 ? fmaxf(m1, x1 * p.c) : m1;
+      if (__any_sync(0xffffffffu, x0 > m0 || x1 > m1)) {
+        const float f0 = m0 == -INFINITY ? 0.f : ex2(m0 - x0), f1 = m1 == -INFINITY ? 0.f : ex2(m1 - x1);
+        l0 *= f0;
+        l1 *= f1;
+#pragma unroll
+        for (int k = 0; k < NO; ++k) {
+          o[k][0] *= f0;
+          o[k][1] *= f0;
+          o[k][2] *= C::F16 ? f1 : f0;
+          o[k][3] *= C::F16 ? f1 : f0;
+        }
+        m0 = x0;
+        m1 = x1;
+      }
+      const float n0 = m0 == -INFINITY ? 0.f : m0, n1 = m1 == -INFINITY ? 0.f : m1;
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        sc[j][0] = ex2(fmaf(sc[j][0], p.c, -n0));
+        sc[j][1] = ex2(fmaf(sc[j][1], p.c, -n0));
+        l0 += sc[j][0] + sc[j][1];
+        if (C::F16) {
+          sc[j][2] = ex2(fmaf(sc[j][2], p.c, -n1));
+          sc[j][3] = ex2(fmaf(sc[j][3], p.c, -n1));
+          l1 += sc[j][2] + sc[j][3];
+        }
+      }
+      // ---- o += P V.  Slots behind the last key may hold anything: their V counts as zero.
+      if constexpr (C::F16) {
+        const uint32_t a0 = h2_as_u32(__floats2half2_rn(sc[0][0], sc[0][1])), a1 = h2_as_u32(__floats2half2_rn(sc[0][2], sc[0][3]));
+        const uint32_t a2 = h2_as_u32(__floats2half2_rn(sc[1][0], sc[1][1])), a3 = h2_as_u32(__floats2half2_rn(sc[1][2], sc[1][3]));
+        uint32_t k0 = 0xffffffffu, k1 = 0xffffffffu;
+        if (part) {
+          const int key = q4 * 2;
+          k0 = (key < lim ? 0xffffu : 0u) | (key + 1 < lim ? 0xffff0000u : 0u);
+          k1 = (key + 8 < lim ? 0xffffu : 0u) | (key + 9 < lim ? 0xffff0000u : 0u);
+        }
+        const int row = (((lane >> 3) & 1) << 3) + (lane & 7);
+        const uint32_t ra = vs_u + row * 128;
+#pragma unroll
+        for (int nb = 0; nb < HD / 16; ++nb) {
+          const int ch = nb * 2 + (lane >> 4);
+          uint32_t vb[4];
+          ldsm4_t(ra + (ch >> 3) * (FR_KT * 128) + (((ch & 7) ^ (row & 7)) << 4), vb);
+          mma_16816(o[2 * nb], a0, a1, a2, a3, vb[0] & k0, vb[1] & k1);
+          mma_16816(o[2 * nb + 1], a0, a1, a2, a3, vb[2] & k0, vb[3] & k1);
+        }
+      } else {
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          uint32_t pa[4];
+          split_tf32(sc[j][0], pa[0], pa[1]);
+          split_tf32(sc[j][1], pa[2], pa[3]);
+          const int key = j * 8 + 2 * q4;  // slots q4 and q4 + 4 of k: keys 2 q4 and 2 q4 + 1
+          const bool u0 = !part || key < lim, u1 = !part || key + 1 < lim;
+#pragma unroll
+          for (int dd = 0; dd < HD / 32; ++dd) {
+            const uint32_t sub = vs_u + dd * (FR_KT * 128);
+            float4 va = lds_f4(sub + key * 128 + ((r8 ^ (key & 7)) << 4));
+            float4 vb = lds_f4(sub + (key + 1) * 128 + ((r8 ^ ((key + 1) & 7)) << 4));
+            if (!u0) va = make_float4(0.f, 0.f, 0.f, 0.f);
+            if (!u1) vb = make_float4(0.f, 0.f, 0.f, 0.f);
+            const float xa[4] = {va.x, va.y, va.z, va.w}, xb[4] = {vb.x, vb.y, vb.z, vb.w};
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              uint32_t h0, e0, h1, e1;
+              split_tf32(xa[e], h0, e0);
+              split_tf32(xb[e], h1, e1);
+              mma_1688(o[dd * 4 + e], pa, e0, e1);
+              mma_1688(o[dd * 4 + e], pa, h0, h1);
+            }
+          }
+        }
+      }
+      __syncwarp();
+      if (i + NST < cnt) issue(i + NST);
+    }
+    // ---- join the warps
+    const bool failed = __syncthreads_or(issued != used);  // a wait ran out (also: every ring is free)
+    if (failed) break;
+#pragma unroll
+    for (int d = 1; d <= 2; d <<= 1) {
+      l0 += __shfl_xor_sync(0xffffffffu, l0, d);
+      l1 += __shfl_xor_sync(0xffffffffu, l1, d);
+    }
+    float* so = reinterpret_cast<float*>(ring);  // [RT][HD], this warp's ring
+    if (q4 == 0) {
+      s_m[warp][r8] = m0;
+      s_l[warp][r8] = l0;
+      if (C::F16) {
+        s_m[warp][(r8 + 8) % RT] = m1;
+        s_l[warp][(r8 + 8) % RT] = l1;
+      }
+    }
+    if constexpr (C::F16) {
+#pragma unroll
+      for (int k = 0; k < NO; ++k) {
+        *reinterpret_cast<float2*>(so + r8 * HD + k * 8 + q4 * 2) = make_float2(o[k][0], o[k][1]);
+        *reinterpret_cast<float2*>(so + (r8 + 8) * HD + k * 8 + q4 * 2) = make_float2(o[k][2], o[k][3]);
+      }
+    } else {
+#pragma unroll
+      for (int dd = 0; dd < HD / 32; ++dd) {  // block e's columns 2 q4 and 2 q4 + 1 are values 8 q4 + e and 8 q4 + 4 + e
+        float* dst = so + r8 * HD + dd * 32 + q4 * 8;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          dst[e] = o[dd * 4 + e][0] + o[dd * 4 + e][2];
+          dst[4 + e] = o[dd * 4 + e][1] + o[dd * 4 + e][3];
+        }
+      }
+    }
+    __syncthreads();
+    for (int e = threadIdx.x; e < nr * (HD / 4); e += FR_WARPS * 32) {
+      const int r = e / (HD / 4), d = (e % (HD / 4)) * 4;
+      float M = -INFINITY;
+#pragma unroll
+      for (int w = 0; w < FR_WARPS; ++w) M = fmaxf(M, s_m[w][r]);
+      float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+      float L = 0.f;
+#pragma unroll
+      for (int w = 0; w < FR_WARPS; ++w) {
+        if (s_m[w][r] == -INFINITY && s_l[w][r] == 0.f) continue;
+        const float f = ex2(s_m[w][r] - M);
+        const float4 v = *reinterpret_cast<const float4*>(base + (size_t)w * NST * C::STAGE + ((size_t)r * HD + d) * 4);
+        acc.x += f * v.x;
+        acc.y += f * v.y;
+        acc.z += f * v.z;
+        acc.w += f * v.w;
+        L += f * s_l[w][r];
+      }
+      const int tok = row_lo + (r0 + r) / p.G, g = (r0 + r) % p.G;
+      const size_t row = (size_t)tok * p.Hq + h * p.G + g;
+      if (p.nslots == 1) {
+        const float inv = L == 0.f ? 0.f : 1.f / L;
+        T* dst = reinterpret_cast<T*>(p.out) + row * HD + d;
+        if constexpr (C::F16)
+          *reinterpret_cast<uint2*>(dst) = make_uint2(h2_as_u32(__floats2half2_rn(acc.x * inv, acc.y * inv)),
+                                                      h2_as_u32(__floats2half2_rn(acc.z * inv, acc.w * inv)));
+        else
+          *reinterpret_cast<float4*>(dst) = make_float4(acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv);
+      } else {
+        const size_t at = (size_t)(slot0 + split) * p.T * p.Hq + row;
+        *reinterpret_cast<float4*>(p.part_o + at * HD + d) = acc;
+        if (d == 0) p.part_ml[at] = make_float2(M, L);
+      }
+    }
+    // the rings hold the joined results: written by threads, next by copies
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+    __syncthreads();
+  }
+  // copies in flight land before the CTA may exit (after a wait that ran out)
+  if (lane == 0)
+    for (; used < issued; ++used) {
+      int ignore = 0;
+      mbar_wait_bounded(&full[warp][used % NST], (used / NST) & 1u, &ignore, PA_WAIT_NS);
+    }
+  if (threadIdx.x == 0 && s_abort) atomicExch(&g_prefix_attn_error, 1);
+}
+
+// ---------------------------------------------------------------- join
+
+// One warp per (row, head): the slots' (m, l) first, one slot a lane, then
+// their sums, weighted.  Reads each partial result once; bound by L2.
+template <typename T, int HD>
+__global__ void __launch_bounds__(256) join_slots_kernel(const PrefixAttnParams p) {
+  pdl_trigger();
+  pdl_wait();
+  const int rows = min(max(p.q_start[p.B], 0), p.T) * p.Hq;
+  const int row = blockIdx.x * (blockDim.x / 32) + (threadIdx.x >> 5), lane = threadIdx.x & 31;
+  if (row >= rows) return;
+  const size_t stride = (size_t)p.T * p.Hq;
+  constexpr int V = HD / 32;
+  float M = -INFINITY;
+  for (int s0 = 0; s0 < p.nslots; s0 += 32)
+    if (s0 + lane < p.nslots) M = fmaxf(M, p.part_ml[(s0 + lane) * stride + row].x);
+#pragma unroll
+  for (int d = 16; d; d >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, d));
+  float acc[V], L = 0.f;
+#pragma unroll
+  for (int i = 0; i < V; ++i) acc[i] = 0.f;
+  for (int s = 0; s < p.nslots; ++s) {
+    const float2 ml = p.part_ml[s * stride + row];
+    if (ml.x == -INFINITY && ml.y == 0.f) continue;
+    const float f = ex2(ml.x - M);
+    L += f * ml.y;
+    const float* src = p.part_o + (s * stride + row) * HD + lane * V;
+    if constexpr (V == 4) {
+      const float4 v = *reinterpret_cast<const float4*>(src);
+      acc[0] += f * v.x; acc[1] += f * v.y; acc[2] += f * v.z; acc[3] += f * v.w;
+    } else {
+      const float2 v = *reinterpret_cast<const float2*>(src);
+      acc[0] += f * v.x; acc[1] += f * v.y;
+    }
+  }
+  const float inv = L == 0.f ? 0.f : 1.f / L;
+  T* dst = reinterpret_cast<T*>(p.out) + (size_t)row * HD + lane * V;
+#pragma unroll
+  for (int i = 0; i < V; ++i) acc[i] *= inv;
+  if constexpr (sizeof(T) == 2) {
+#pragma unroll
+    for (int i = 0; i < V; i += 2) *reinterpret_cast<__half2*>(dst + i) = __floats2half2_rn(acc[i], acc[i + 1]);
+  } else if constexpr (V == 4) {
+    *reinterpret_cast<float4*>(dst) = make_float4(acc[0], acc[1], acc[2], acc[3]);
+  } else {
+    *reinterpret_cast<float2*>(dst) = make_float2(acc[0], acc[1]);
+  }
+}
+
+// ---------------------------------------------------------------- host side
+
+// A pool [rows, hd] as (128-byte chunk, row, chunk index), box (chunk, box_rows, all chunks), 128-byte swizzle: a
+// tile lies in shared memory as hd * es / 128 sub-tiles of box_rows rows of 128 bytes.
+static bool pool_map(CUtensorMap* m, const void* pool, size_t rows, int hd, bool f16, int box_rows) {
+  static const PFN_cuTensorMapEncodeTiled_v12000 fn = [] {
+    void* ptr = nullptr;
+    cudaDriverEntryPointQueryResult q;
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &ptr, cudaEnableDefault, &q) != cudaSuccess ||
+        q != cudaDriverEntryPointSuccess)
+      ptr = nullptr;
+    return reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(ptr);
+  }();
+  if (!fn) return false;
+  const int es = f16 ? 2 : 4, chunk = 128 / es;
+  cuuint64_t dims[3] = {(cuuint64_t)chunk, (cuuint64_t)rows, (cuuint64_t)(hd / chunk)};
+  cuuint64_t strides[2] = {(cuuint64_t)hd * es, 128};
+  cuuint32_t box[3] = {(cuuint32_t)chunk, (cuuint32_t)box_rows, (cuuint32_t)(hd / chunk)}, step[3] = {1, 1, 1};
+  return fn(m, f16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 3, const_cast<void*>(pool), dims,
+            strides, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+            CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+// How a call is cut.  The host knows the rows T and the requests B, not which request has how many.
+struct AttnPlan {
+  int splits, row_groups, nslots;
+};
+
+static AttnPlan plan_attn(int T, int B, int Hkv, int G, int rt, long long max_keys, int sms) {
+  AttnPlan a;
+  // four CTAs per SM over all requests and heads: first from tiles of rows, then from the keys (at least a 16-key
+  // tile for each of a CTA's 4 warps)
+  const long long want = (4ll * sms + (long long)B * Hkv - 1) / ((long long)B * Hkv);
+  const long long tiles = ((long long)T * G + (long long)B * rt - 1) / ((long long)B * rt);
+  a.row_groups = (int)std::max(1ll, std::min(want, tiles));
+  const long long most = std::max(1ll, (max_keys + 63) / 64);
+  a.splits = (int)std::max(1ll, std::min({(want + a.row_groups - 1) / a.row_groups, most, 64ll}));
+  a.nslots = a.splits;
+  return a;
+}
+
+template <typename T, int HD>
+static int run_attn(PrefixAttnParams p, const void* k, const void* v, const AttnPlan& a, cudaStream_t stream) {
+  using C = FewRows<T, HD>;
+  PoolMaps maps;
+  SC_REQUIRE(pool_map(&maps.k, k, p.pool_rows, HD, C::F16, FR_KT) && pool_map(&maps.v, v, p.pool_rows, HD, C::F16, FR_KT),
+             SC_ERR_CUDA, "prefix_attn: tensor map of the pages refused");
+  auto kern = few_rows_kernel<T, HD>;
+  const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM);
+  if (e != cudaSuccess) return check_launch("prefix_attn", e);
+  launch(kern, dim3(a.splits * a.row_groups, p.Hkv, p.B), dim3(FR_WARPS * 32), C::SMEM, stream, p, maps, 1, a.splits,
+         a.row_groups, 0);
+  const int st = check_launch("prefix_attn");
+  if (st != SC_OK || p.nslots == 1) return st;
+  launch(join_slots_kernel<T, HD>, dim3((unsigned)(((size_t)p.T * p.Hq + 7) / 8)), dim3(256), 0, stream, p);
+  return check_launch("prefix_attn_join");
+}
+
+}  // namespace sc
+
+extern "C" {
+
+int sc_prefix_attn_device_error(int reset) {
+  int v = 0;
+  cudaMemcpyFromSymbol(&v, sc::g_prefix_attn_error, sizeof(int));
+  if (reset) {
+    const int z = 0;
+    cudaMemcpyToSymbol(sc::g_prefix_attn_error, &z, sizeof(int));
+  }
+  return v;
+}
+
+size_t sc_prefix_attn_workspace_bytes(int T, int B, int Hq, int Hkv, int hd, int max_blocks, int max_prefix_blocks,
+                                      int page_size, int dtype) {
+  if (T < 1 || B < 1 || Hq < 1 || Hkv < 1 || hd < 1 || max_blocks < 0 || max_prefix_blocks < 0 || page_size < 1) return 0;
+  if (Hq % Hkv) return 0;
+  const sc::AttnPlan a = sc::plan_attn(T, B, Hkv, Hq / Hkv, dtype == SC_F16 ? 16 : 8,
+                                       ((long long)max_blocks + max_prefix_blocks) * page_size, sc::sm_count());
+  return a.nslots <= 1 ? 0 : (size_t)a.nslots * T * Hq * (hd + 2) * sizeof(float);
+}
+
+int sc_prefix_attn(const void* q, const void* k_pages, const void* v_pages, int dtype, int T, const int32_t* q_start,
+                   const int32_t* kv_lens, const int32_t* block_table, int B, int max_blocks,
+                   const int32_t* prefix_table, const int32_t* prefix_len, int max_prefix_blocks, int Hq, int Hkv,
+                   int hd, int n_pages, int page_size, float scale, void* out, void* workspace, size_t workspace_bytes,
+                   cudaStream_t stream) {
+  using namespace sc;
+  SC_REQUIRE(q && k_pages && v_pages && q_start && kv_lens && block_table && out, SC_ERR_ARG, "prefix_attn: null pointer");
+  SC_REQUIRE(!prefix_len || (prefix_table && max_prefix_blocks >= 1), SC_ERR_ARG, "prefix_attn: a prefix needs its table");
+  SC_REQUIRE(dtype == SC_F16 || dtype == SC_F32, SC_ERR_ARG, "prefix_attn: dtype");
+  SC_REQUIRE(hd == 64 || hd == 128, SC_ERR_UNSUPPORTED, "prefix_attn: head_dim %d unsupported (64, 128)", hd);
+  SC_REQUIRE(page_size >= 16 && page_size <= 32768 && (page_size & (page_size - 1)) == 0, SC_ERR_UNSUPPORTED,
+             "prefix_attn: page size %d unsupported (a power of two from 16)", page_size);
+  SC_REQUIRE(T >= 1 && B >= 1 && B <= 65535 && max_blocks >= 1 && n_pages >= 1, SC_ERR_SHAPE, "prefix_attn: bad T/B/max_blocks");
+  SC_REQUIRE(Hkv >= 1 && Hkv <= 65535 && Hq >= Hkv && Hq % Hkv == 0, SC_ERR_SHAPE, "prefix_attn: Hq=%d not a multiple of Hkv=%d", Hq, Hkv);
+  SC_REQUIRE((long long)n_pages * Hkv * page_size < INT32_MAX && (long long)T * Hq <= INT32_MAX &&
+                 (long long)max_blocks * page_size <= INT32_MAX && (long long)max_prefix_blocks * page_size <= INT32_MAX,
+             SC_ERR_SHAPE, "prefix_attn: rows past 32 bits");
+  SC_REQUIRE(scale > 0.f && scale < INFINITY, SC_ERR_ARG, "prefix_attn: scale must be positive and finite");
+  SC_REQUIRE((((uintptr_t)q | (uintptr_t)k_pages | (uintptr_t)v_pages | (uintptr_t)out) & 15) == 0, SC_ERR_ARG,
+             "prefix_attn: tensors must start on 16-byte boundaries");
+  if (!prefix_len) max_prefix_blocks = 0;
+  const AttnPlan a = plan_attn(T, B, Hkv, Hq / Hkv, dtype == SC_F16 ? 16 : 8,
+                               ((long long)max_blocks + max_prefix_blocks) * page_size, sm_count());
+  const size_t need = sc_prefix_attn_workspace_bytes(T, B, Hq, Hkv, hd, max_blocks, max_prefix_blocks, page_size, dtype);
+  SC_REQUIRE(workspace_bytes >= need && (need == 0 || workspace), SC_ERR_WORKSPACE,
+             "prefix_attn: workspace of %zu bytes needed (got %zu)", need, workspace_bytes);
+  SC_REQUIRE(((uintptr_t)workspace & 15) == 0, SC_ERR_ARG, "prefix_attn: the workspace must start on a 16-byte boundary");
+  PrefixAttnParams p{};
+  p.q = q;
+  p.out = out;
+  p.part_o = static_cast<float*>(workspace);
+  p.part_ml = reinterpret_cast<float2*>(p.part_o + (size_t)a.nslots * T * Hq * hd);
+  p.q_start = q_start;
+  p.kv_lens = kv_lens;
+  p.block_table = block_table;
+  p.prefix_table = prefix_table;
+  p.prefix_len = prefix_len;
+  p.T = T;
+  p.B = B;
+  p.max_blocks = max_blocks;
+  p.max_prefix_blocks = max_prefix_blocks;
+  p.n_pages = n_pages;
+  p.lg_page = __builtin_ctz(page_size);
+  p.Hq = Hq;
+  p.Hkv = Hkv;
+  p.G = Hq / Hkv;
+  p.pool_rows = n_pages * Hkv * page_size;
+  p.c = scale * 1.4426950408889634f;
+  p.nslots = a.nslots;
+  if (dtype == SC_F16)
+    return hd == 128 ? run_attn<__half, 128>(p, k_pages, v_pages, a, stream) : run_attn<__half, 64>(p, k_pages, v_pages, a, stream);
+  return hd == 128 ? run_attn<float, 128>(p, k_pages, v_pages, a, stream) : run_attn<float, 64>(p, k_pages, v_pages, a, stream);
+}
+
+}  // extern "C"

@@ -10,7 +10,7 @@ from __future__ import annotations
 
 import ctypes as C
 import math
-from typing import Optional, Sequence
+from typing import NamedTuple, Optional, Sequence
 
 import torch
 
@@ -245,6 +245,217 @@ def attn_decode(qkv: torch.Tensor, B: int, Hq: int, Hkv: int, hd: int, pos: torc
     L.call("sc_attn_decode", _p(qkv), B, Hq, Hkv, hd, _p(pos), _p(cos_tab), _p(sin_tab), cos_tab.shape[0],
            _p(k_cache), _p(v_cache), k_cache.shape[2], float(sc), splits, _p(out), _dt(out), _p(workspace),
            nbytes if workspace is not None else 0, _p(tickets), stream_handle(qkv.device))
+    return out
+
+
+# ---------------------------------------------------------------- paged cache
+
+class PagedStep(NamedTuple):
+    """What ``paged_reserve`` wrote (all int32 on the device)."""
+
+    kv_lens: torch.Tensor      # [B] tokens of each request, the new ones among them
+    q_start: torch.Tensor      # [B + 1] rows of each request
+    slots: torch.Tensor        # [max_tokens] each row's slot in the cache
+    positions: torch.Tensor    # [max_tokens] each row's position
+    free_count: torch.Tensor   # [1] pages left
+    status: torch.Tensor       # [1] 0, or why nothing was reserved
+
+
+def _on_one_device(what: str, first: torch.Tensor, *rest: Optional[torch.Tensor]) -> torch.device:
+    """The device of the tensors, which are CUDA tensors of one device and contiguous."""
+    dev = first.device
+    for t in (first, *rest):
+        if t is None:
+            continue
+        if not t.is_cuda:
+            raise RuntimeError("libsc_b200 ops take CUDA tensors only (no CPU path)")
+        if t.device != dev:
+            raise ValueError(f"{what}: tensors on {dev} and {t.device}")
+        if not t.is_contiguous():
+            raise ValueError(f"{what}: tensors must be contiguous")
+    return dev
+
+
+def _int32(what: str, **named: Optional[torch.Tensor]) -> None:
+    for name, t in named.items():
+        if t is not None and t.dtype != torch.int32:
+            raise ValueError(f"{what}: {name} must be int32, got {t.dtype}")
+
+
+def _sized(what: str, n: int, **named: Optional[torch.Tensor]) -> None:
+    for name, t in named.items():
+        if t is not None and t.numel() != n:
+            raise ValueError(f"{what}: {name} holds {t.numel()} values, {n} are needed")
+
+
+def _call_on(dev: torch.device, name: str, *args) -> None:
+    """The call with ``dev`` as the current device, on its current stream."""
+    if dev.index == torch.cuda.current_device():
+        L.call(name, *args, torch.cuda.current_stream(dev).cuda_stream)
+    else:
+        with torch.cuda.device(dev):
+            L.call(name, *args, torch.cuda.current_stream(dev).cuda_stream)
+
+
+def paged_reserve(lens: torch.Tensor, new_lens: torch.Tensor, block_table: torch.Tensor, free_pages: torch.Tensor,
+                  free_count: torch.Tensor, page_size: int, max_tokens: Optional[int] = None,
+                  prefix_len: Optional[torch.Tensor] = None, kv_lens: Optional[torch.Tensor] = None,
+                  q_start: Optional[torch.Tensor] = None, slots: Optional[torch.Tensor] = None,
+                  positions: Optional[torch.Tensor] = None, free_count_out: Optional[torch.Tensor] = None,
+                  status: Optional[torch.Tensor] = None) -> PagedStep:
+    """Pages, slots and row offsets for ``new_lens[b]`` more tokens of every request.
+
+    ``block_table`` [B, max_blocks] gets the new pages, taken from the top of the stack ``free_pages`` [:free_count].
+    Outputs not passed are allocated (``slots`` and ``positions`` of ``max_tokens`` rows, -1 behind the last one);
+    ``kv_lens`` may be ``lens`` and ``free_count_out`` may be ``free_count``.  If ``status`` is not 0 nothing was
+    reserved and ``q_start`` is all zeros: 1 not enough pages, 2 a request exceeds ``max_blocks`` pages, 4 more than
+    ``max_tokens`` new tokens, 8 a negative length, 16 ``free_count`` outside the stack (the sum of those that hold)."""
+    B = lens.numel()
+    dev = _on_one_device("paged_reserve", lens, new_lens, block_table, free_pages, free_count, prefix_len, kv_lens, q_start,
+                         slots, positions, free_count_out, status)
+    if slots is None:
+        if max_tokens is None:
+            raise ValueError("paged_reserve: max_tokens or slots is needed")
+        slots = torch.full((max_tokens,), -1, dtype=torch.int32, device=dev)
+    rows = slots.numel() if max_tokens is None else max_tokens
+    if positions is None:
+        positions = torch.full((rows,), -1, dtype=torch.int32, device=dev)
+    new = lambda n: torch.empty(n, dtype=torch.int32, device=dev)  # noqa: E731
+    kv_lens = new(B) if kv_lens is None else kv_lens
+    q_start = new(B + 1) if q_start is None else q_start
+    free_count_out = new(1) if free_count_out is None else free_count_out
+    status = new(1) if status is None else status
+    _int32("paged_reserve", lens=lens, new_lens=new_lens, block_table=block_table, free_pages=free_pages, free_count=free_count,
+           prefix_len=prefix_len, kv_lens=kv_lens, q_start=q_start, slots=slots, positions=positions,
+           free_count_out=free_count_out, status=status)
+    if block_table.dim() != 2 or block_table.shape[0] != B:
+        raise ValueError(f"paged_reserve: block_table {tuple(block_table.shape)} is not [{B}, max_blocks]")
+    _sized("paged_reserve", B, new_lens=new_lens, kv_lens=kv_lens)
+    _sized("paged_reserve", B + 1, q_start=q_start)
+    _sized("paged_reserve", 1, free_count=free_count, prefix_len=prefix_len, free_count_out=free_count_out, status=status)
+    if slots.numel() < rows or positions.numel() < rows:
+        raise ValueError(f"paged_reserve: slots and positions hold {slots.numel()} and {positions.numel()} rows, {rows} are needed")
+    _call_on(dev, "sc_paged_reserve", lens.data_ptr(), new_lens.data_ptr(), B, _p(prefix_len), block_table.data_ptr(),
+             block_table.shape[1], free_pages.data_ptr(), free_pages.numel(), free_count.data_ptr(), page_size, rows,
+             kv_lens.data_ptr(), q_start.data_ptr(), slots.data_ptr(), positions.data_ptr(), free_count_out.data_ptr(),
+             status.data_ptr())
+    return PagedStep(kv_lens, q_start, slots, positions, free_count_out, status)
+
+
+def paged_truncate(lens: torch.Tensor, keep: torch.Tensor, block_table: torch.Tensor, free_pages: torch.Tensor,
+                   free_count: torch.Tensor, page_size: int, lens_out: Optional[torch.Tensor] = None,
+                   free_count_out: Optional[torch.Tensor] = None, status: Optional[torch.Tensor] = None):
+    """Cut every request to its first ``keep[b]`` tokens (0: it has ended) and put the pages that it no longer needs
+    back on the stack.  ``lens_out`` may be ``lens``, ``free_count_out`` may be ``free_count``.  Returns ``(lens_out,
+    free_count_out, status)``; unless ``status`` is 0 nothing changed (1: the stack has no room, as when a page is given
+    back twice; 2, 8, 16 as for ``paged_reserve``)."""
+    B = lens.numel()
+    dev = _on_one_device("paged_truncate", lens, keep, block_table, free_pages, free_count, lens_out, free_count_out, status)
+    lens_out = torch.empty_like(lens) if lens_out is None else lens_out
+    free_count_out = torch.empty_like(free_count) if free_count_out is None else free_count_out
+    status = torch.empty(1, dtype=torch.int32, device=dev) if status is None else status
+    _int32("paged_truncate", lens=lens, keep=keep, block_table=block_table, free_pages=free_pages, free_count=free_count,
+           lens_out=lens_out, free_count_out=free_count_out, status=status)
+    if block_table.dim() != 2 or block_table.shape[0] != B:
+        raise ValueError(f"paged_truncate: block_table {tuple(block_table.shape)} is not [{B}, max_blocks]")
+    _sized("paged_truncate", B, keep=keep, lens_out=lens_out)
+    _sized("paged_truncate", 1, free_count=free_count, free_count_out=free_count_out, status=status)
+    _call_on(dev, "sc_paged_truncate", lens.data_ptr(), keep.data_ptr(), B, block_table.data_ptr(), block_table.shape[1],
+             free_pages.data_ptr(), free_pages.numel(), free_count.data_ptr(), page_size, lens_out.data_ptr(),
+             free_count_out.data_ptr(), status.data_ptr())
+    return lens_out, free_count_out, status
+
+
+def _pools(what: str, k_pages: torch.Tensor, v_pages: torch.Tensor):
+    if k_pages.dim() != 4 or k_pages.shape != v_pages.shape:
+        raise ValueError(f"{what}: k_pages {tuple(k_pages.shape)} and v_pages {tuple(v_pages.shape)} must be one "
+                         "[n_pages, Hkv, page, hd]")
+    if k_pages.dtype != v_pages.dtype or k_pages.dtype not in (_F16, _F32):
+        raise ValueError(f"{what}: pages must both be float16 or float32, got {k_pages.dtype} and {v_pages.dtype}")
+    return k_pages.shape
+
+
+def paged_rope_append(qkv: torch.Tensor, q_start: torch.Tensor, slots: torch.Tensor, positions: torch.Tensor,
+                      cos_tab: torch.Tensor, sin_tab: torch.Tensor, q_out: torch.Tensor, k_pages: torch.Tensor,
+                      v_pages: torch.Tensor) -> torch.Tensor:
+    """``rope_append`` for a paged cache: q and k of each row (``qkv`` [T, (Hq + 2 Hkv) hd], float16 or float32) rotated
+    at ``positions``, k and v written to ``slots`` of the pools, q to ``q_out`` [T, Hq hd] in the pools' type.  Rows from
+    ``q_start[-1]`` on are left as they were; a slot outside the pool or a position past the tables is not written."""
+    dev = _on_one_device("paged_rope_append", qkv, q_start, slots, positions, cos_tab, sin_tab, q_out, k_pages, v_pages)
+    n_pages, Hkv, page, hd = _pools("paged_rope_append", k_pages, v_pages)
+    if qkv.dim() != 2 or qkv.dtype not in (_F16, _F32):
+        raise ValueError(f"paged_rope_append: qkv must be a float16 or float32 [T, (Hq + 2 Hkv) hd], got {qkv.dtype} {tuple(qkv.shape)}")
+    T, width = qkv.shape
+    Hq = width // hd - 2 * Hkv
+    if width % hd or Hq < 1:
+        raise ValueError(f"paged_rope_append: qkv rows of {width} do not hold q beside {Hkv} heads of {hd}")
+    if q_out.dtype != k_pages.dtype or q_out.numel() != T * Hq * hd:
+        raise ValueError(f"paged_rope_append: q_out must be a {k_pages.dtype} [{T}, {Hq * hd}], got {q_out.dtype} {tuple(q_out.shape)}")
+    if slots.numel() < T or positions.numel() < T:
+        raise ValueError(f"paged_rope_append: {slots.numel()} slots and {positions.numel()} positions for {T} rows")
+    if cos_tab.dtype != _F32 or sin_tab.dtype != _F32 or cos_tab.dim() != 2 or cos_tab.shape[1] * 2 != hd or cos_tab.shape != sin_tab.shape:
+        raise ValueError(f"paged_rope_append: cos_tab and sin_tab must be float32 [max_pos, {hd // 2}]")
+    _int32("paged_rope_append", q_start=q_start, slots=slots, positions=positions)
+    if q_start.numel() < 1:
+        raise ValueError("paged_rope_append: q_start is empty")
+    if T:
+        _call_on(dev, "sc_paged_rope_append", qkv.data_ptr(), _dt(qkv), T, q_start.data_ptr() + 4 * (q_start.numel() - 1),
+                 slots.data_ptr(), positions.data_ptr(), cos_tab.data_ptr(), sin_tab.data_ptr(), cos_tab.shape[0], Hq, Hkv, hd,
+                 q_out.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), _dt(k_pages), n_pages, page)
+    return q_out
+
+
+def prefix_attn_workspace_bytes(T: int, B: int, Hq: int, Hkv: int, hd: int, max_blocks: int, max_prefix_blocks: int,
+                                page_size: int, dtype: torch.dtype) -> int:
+    return int(L.load().sc_prefix_attn_workspace_bytes(T, B, Hq, Hkv, hd, max_blocks, max_prefix_blocks, page_size,
+                                                       L.SC_F16 if dtype == _F16 else L.SC_F32))
+
+
+def prefix_attn(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, q_start: torch.Tensor, kv_lens: torch.Tensor,
+                block_table: torch.Tensor, prefix_table: Optional[torch.Tensor] = None,
+                prefix_len: Optional[torch.Tensor] = None, out: Optional[torch.Tensor] = None,
+                scale: Optional[float] = None, workspace: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Attention of a ragged batch behind a prefix that all its requests share.
+
+    Row ``q_start[b] + i`` of request b (n rows) sees the ``prefix_len`` tokens in the pages ``prefix_table`` and its own
+    tokens ``0 .. kv_lens[b] - n + i`` in the pages ``block_table[b]``; GQA by heads.  ``q`` and ``out`` [T, Hq hd] have
+    the pools' type.  Rows from ``q_start[-1]`` on are left as they were (an ``out`` that is allocated here is zero
+    there); a row that sees no token is zero; pages outside the pool count as absent.  ``workspace``: uint8, at least
+    ``prefix_attn_workspace_bytes``; without it scratch is allocated per call, so calls on two streams do not meet."""
+    n_pages, Hkv, page, hd = _pools("prefix_attn", k_pages, v_pages)
+    T = q.shape[0] if q.dim() else 0
+    if out is None:
+        out = torch.zeros_like(q)
+    dev = _on_one_device("prefix_attn", q, k_pages, v_pages, q_start, kv_lens, block_table, prefix_table, prefix_len, out, workspace)
+    B = kv_lens.numel()
+    if q.dtype != k_pages.dtype or out.dtype != q.dtype or out.numel() != q.numel():
+        raise ValueError(f"prefix_attn: q and out must have the pages' type {k_pages.dtype} and one size, got {q.dtype} "
+                         f"{tuple(q.shape)} and {out.dtype} {tuple(out.shape)}")
+    Hq = q.numel() // (T * hd) if T else Hkv
+    if T and Hq * T * hd != q.numel():
+        raise ValueError(f"prefix_attn: q rows of {q.numel() // T} are no multiple of head_dim {hd}")
+    _int32("prefix_attn", q_start=q_start, kv_lens=kv_lens, block_table=block_table, prefix_table=prefix_table, prefix_len=prefix_len)
+    if block_table.dim() != 2 or block_table.shape[0] != B:
+        raise ValueError(f"prefix_attn: block_table {tuple(block_table.shape)} is not [{B}, max_blocks]")
+    _sized("prefix_attn", B + 1, q_start=q_start)
+    if (prefix_len is None) != (prefix_table is None):
+        raise ValueError("prefix_attn: prefix_table and prefix_len go together")
+    nbp = 0
+    if prefix_len is not None:
+        _sized("prefix_attn", 1, prefix_len=prefix_len)
+        nbp = prefix_table.numel()
+    if not T or not B:
+        return out
+    sc = (1.0 / math.sqrt(hd)) if scale is None else float(scale)
+    nbytes = prefix_attn_workspace_bytes(T, B, Hq, Hkv, hd, block_table.shape[1], nbp, page, q.dtype)
+    if workspace is None:
+        if nbytes:
+            workspace = torch.empty(nbytes, dtype=torch.uint8, device=dev)
+    elif workspace.dtype != torch.uint8:
+        raise ValueError(f"prefix_attn: workspace must be uint8, got {workspace.dtype}")
+    _call_on(dev, "sc_prefix_attn", q.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), _dt(q), T, q_start.data_ptr(),
+             kv_lens.data_ptr(), block_table.data_ptr(), B, block_table.shape[1], _p(prefix_table), _p(prefix_len), nbp, Hq, Hkv,
+             hd, n_pages, page, sc, out.data_ptr(), _p(workspace), workspace.numel() if workspace is not None else 0)
     return out
 
 
