@@ -11,7 +11,7 @@
 #include <cuda.h>
 #include <cudaTypedefs.h>
 
-#include "sc_common.cuh"
+#include "sc_tc.cuh"
 
 namespace sc {
 
@@ -457,6 +457,420 @@ few_rows_kernel(const PrefixAttnParams p, const __grid_constant__ PoolMaps maps,
   if (threadIdx.x == 0 && s_abort) atomicExch(&g_prefix_attn_error, 1);
 }
 
+// ---------------------------------------------------------------- many rows, fp16
+
+// Kernel for many rows of queries over the same keys, on the tensor cores
+// (tcgen05): the shared prefix under the rows of all requests, or one
+// request's prompt chunk.  A CTA takes two tiles of 128 rows (a row: a token
+// and a head of the group), a kv head and a share of the keys:
+//   warp 0     TMA producer: K and V tiles of 128 keys through one ring, a
+//              copy per page and 64-wide column, issued by a lane each
+//   warp 1     MMA issuer: S = Q K^T into TMEM, then O += P V with P read
+//              from TMEM; V's slots behind the last key are zeroed here first,
+//              for they may hold anything (0 x NaN is NaN)
+//   warps 2-5, 6-9: softmax of tile 0 and of tile 1, a thread per row: the
+//              row's maximum, P = exp2(c s - m) in fp16 over S's own columns,
+//              its sum in fp32, and in the end O / l or a partial result
+// The tiles take turns: while one is in the softmax, the other is in the
+// tensor cores.  The maximum a row is scaled by is raised, and O rescaled,
+// only when a score passes it by 2^8 (P then stays below 2^8 and l in fp32).
+// TMEM: S0 | S1 (128 columns each, P in the first 64), O0 | O1 (HD each).
+constexpr int TC_M = 128, TC_N = 128;   // rows and keys of a tile
+constexpr int TC_THREADS = 10 * 32;
+constexpr float TC_RAISE = 8.f;
+
+template <int HD>
+struct ManyRows {
+  static constexpr int NCH = HD / 64;               // 64-wide columns
+  static constexpr int TILE = TC_N * HD * 2;        // bytes of a Q, K or V tile
+  static constexpr int NBUF = HD == 128 ? 5 : 8;    // K and V tiles in the ring
+  static constexpr int SMEM = 2 * TILE + NBUF * TILE + 1024;
+};
+
+__device__ __forceinline__ bool pa_wait(uint64_t* bar, uint32_t parity, volatile int* abort) {
+  return mbar_wait_bounded(bar, parity, abort, PA_WAIT_NS);
+}
+
+__device__ __forceinline__ void tma3d_at(uint32_t dst, const CUtensorMap* map, int row, int chunk, uint64_t* bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::
+          "r"(dst),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(0), "r"(row), "r"(chunk), "r"(smem_u32(bar))
+      : "memory");
+}
+
+__device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(taddr),
+      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
+      "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+      : "memory");
+}
+__device__ __forceinline__ void tmem_st32(uint32_t taddr, const float (&v)[32]) {
+  uint32_t a[16], b[16];
+#pragma unroll
+  for (int i = 0; i < 16; ++i) {
+    a[i] = __float_as_uint(v[i]);
+    b[i] = __float_as_uint(v[16 + i]);
+  }
+  tmem_st16(taddr, a);
+  tmem_st16(taddr + 16, b);
+}
+__device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+// PACKED: rows of all requests, keys of the prefix.  Otherwise: rows of one
+// request, keys of the prefix and its own.
+template <int HD, bool PACKED>
+__global__ void __launch_bounds__(TC_THREADS, 1)
+many_rows_kernel(const PrefixAttnParams p, const __grid_constant__ PoolMaps maps, int splits, int slot0) {
+  using C = ManyRows<HD>;
+  constexpr int NBUF = C::NBUF;
+  extern __shared__ __align__(1024) unsigned char mr_smem[];
+  __shared__ __align__(8) uint64_t full[NBUF], empty[NBUF], q_full[2], s_full[2], p_full[2], o_full[2], drained;
+  __shared__ uint32_t s_tmem, s_absent[16];
+  __shared__ int s_abort, s_req, s_row0, s_sum[TC_THREADS / 32];
+  unsigned char* base = mr_smem + ((1024 - (smem_u32(mr_smem) & 1023)) & 1023);
+  const uint32_t q_u = smem_u32(base), ring_u = q_u + 2 * C::TILE;
+  const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
+  const int split = blockIdx.x % splits, item = blockIdx.x / splits, h = blockIdx.y;
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < NBUF; ++i) {
+      mbar_init(&full[i], 1);
+      mbar_init(&empty[i], 1);
+    }
+    for (int x = 0; x < 2; ++x) {
+      mbar_init(&q_full[x], TC_M);
+      mbar_init(&s_full[x], 1);
+      mbar_init(&p_full[x], TC_M);
+      mbar_init(&o_full[x], 1);
+    }
+    mbar_init(&drained, 1);
+    s_abort = 0;
+    s_req = -1;
+    fence_mbar_init();
+  }
+  if (warp == 1) tmem_alloc_cols(&s_tmem, 512);
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  pdl_trigger();
+  pdl_wait();
+  volatile int* abort = &s_abort;
+  const uint32_t tmem = s_tmem;
+
+  // ---- which rows
+  int b = 0, row_lo, row_hi;
+  int r0;  // first row of tile 0, counted in the request (or in the batch)
+  if (PACKED) {
+    row_lo = 0;
+    row_hi = min(max(p.q_start[p.B], 0), p.T);
+    r0 = item * 2 * TC_M;
+  } else {
+    // item -> request: items of the requests before it
+    int before = 0;
+    for (int b0 = 0; b0 < p.B; b0 += TC_THREADS) {
+      const int bb = b0 + threadIdx.x;
+      int lo, hi, cnt = 0;
+      if (bb < p.B) {
+        request_rows(p, bb, lo, hi);
+        cnt = (int)(((long long)(hi - lo) * p.G + 2 * TC_M - 1) / (2 * TC_M));
+      }
+      int sum = cnt;
+#pragma unroll
+      for (int d = 1; d < 32; d <<= 1) {
+        const int u = __shfl_up_sync(0xffffffffu, sum, d);
+        if (lane >= d) sum += u;
+      }
+      if (lane == 31) s_sum[warp] = sum;
+      __syncthreads();
+      int at = before;
+      for (int w = 0; w < TC_THREADS / 32; ++w) {
+        if (w < warp) at += s_sum[w];
+        before += s_sum[w];
+      }
+      at += sum - cnt;
+      if (item >= at && item < at + cnt) {
+        s_req = bb;
+        s_row0 = (item - at) * 2 * TC_M;
+      }
+      __syncthreads();
+      if (s_req >= 0) break;
+    }
+    b = max(s_req, 0);
+    r0 = s_row0;
+    request_rows(p, b, row_lo, row_hi);
+    if (s_req < 0) row_hi = row_lo;
+  }
+  const int rows = (row_hi - row_lo) * p.G;  // fits: T * Hq does
+  const bool work = r0 < rows && (PACKED || s_req >= 0);
+  const int n = row_hi - row_lo, len = PACKED ? 0 : request_len(p, b), P = prefix_keys(p);
+  const int np = (P + TC_N - 1) / TC_N;
+  const int last = min(r0 + 2 * TC_M, rows) - 1;  // the CTA's last row: sees the most own keys
+  const int own = PACKED || !work ? 0 : max(0, min(len, len - n + last / p.G + 1));
+  const int nt = np + (own + TC_N - 1) / TC_N;
+  const int per = (nt + splits - 1) / splits;
+  const int t_lo = min(nt, split * per), t_hi = min(nt, t_lo + per);
+  const int cnt = work ? t_hi - t_lo : 0;
+  const int nx = work && r0 + TC_M < rows ? 2 : 1;  // row tiles in use
+  // keys of tile t that exist
+  auto keys_of = [&](int t) { return t < np ? P - t * TC_N : own - (t - np) * TC_N; };
+
+  if (warp == 0) {
+    // ================================ TMA producer ================================
+    const int lg = min(p.lg_page, 7), rpb = 1 << lg;  // rows per copy
+    const int boxes = (TC_N >> lg) * C::NCH;
+    const int sub = lane / C::NCH, ch = lane % C::NCH;
+    uint32_t it = 0;
+    bool ok = true;
+    for (int i = 0; i < cnt && ok; ++i) {
+      const int t = t_lo + i, k0 = (t < np ? t : t - np) * TC_N;
+      int row = -1;
+      if (lane < boxes && sub * rpb < keys_of(t)) {
+        const int key = k0 + sub * rpb, blk = key >> p.lg_page;
+        const int id = t < np ? p.prefix_table[blk] : p.block_table[(size_t)b * p.max_blocks + blk];
+        if (id >= 0 && id < p.n_pages) row = ((id * p.Hkv + h) << p.lg_page) + (key & ((1 << p.lg_page) - 1));
+      }
+      uint32_t gone = 0;  // pages of this tile that do not exist, a bit per copy's rows
+      for (int k = 0; k < (TC_N >> lg); ++k) gone |= (__shfl_sync(0xffffffffu, row, k * C::NCH) < 0 ? 1u : 0u) << k;
+      if (lane == 0) s_absent[i & 15] = gone;
+#pragma unroll
+      for (int kv = 0; kv < 2; ++kv, ++it) {
+        const int s = it % NBUF;
+        ok = __all_sync(0xffffffffu, pa_wait(&empty[s], ((it / NBUF) & 1u) ^ 1u, abort));
+        if (!ok) break;
+        if (lane == 0) mbar_arrive_expect_tx(&full[s], C::TILE);
+        __syncwarp();
+        if (lane < boxes)
+          tma3d_at(ring_u + s * C::TILE + ch * (TC_N * 128) + sub * rpb * 128, kv ? &maps.v : &maps.k,
+                   row < 0 ? p.pool_rows : row, ch, &full[s]);
+      }
+    }
+    // copies in flight land before the CTA may exit
+    if (lane == 0) {
+      int ignore = 0;
+      for (uint32_t k = it > NBUF ? it - NBUF : 0; k < it; ++k) pa_wait(&full[k % NBUF], (k / NBUF) & 1u, &ignore);
+    }
+  } else if (warp == 1) {
+    // ================================ MMA issuer ================================
+    const uint32_t idesc_s = (1u << 4) | ((TC_N >> 3) << 17) | ((TC_M >> 4) << 24);
+    const uint32_t idesc_o = (1u << 4) | (1u << 16) | ((HD >> 3) << 17) | ((TC_M >> 4) << 24);  // V: contiguous along N
+    auto buf = [&](uint32_t it) { return ring_u + (it % NBUF) * C::TILE; };
+    auto wait_full = [&](uint32_t it) {
+      return __all_sync(0xffffffffu, pa_wait(&full[it % NBUF], (it / NBUF) & 1u, abort));
+    };
+    auto issue_s = [&](int x, uint32_t it) {  // S_x = Q_x K^T
+      if (lane == 0) {
+#pragma unroll
+        for (int kk = 0; kk < HD / 16; ++kk) {
+          const uint32_t off = (kk >> 2) * (TC_N * 128) + (kk & 3) * 32;
+          umma_f16(tmem + x * TC_N, umma_desc_sw128(q_u + x * C::TILE + off), umma_desc_sw128(buf(it) + off), idesc_s, kk != 0);
+        }
+        tc_commit(&s_full[x]);
+      }
+    };
+    bool ok = true;
+    if (cnt > 0) {
+      for (int x = 0; x < nx && ok; ++x) ok = __all_sync(0xffffffffu, pa_wait(&q_full[x], 0, abort));
+      ok = ok && wait_full(0);
+      tc_fence_after();
+      if (ok) {
+        for (int x = 0; x < nx; ++x) issue_s(x, 0);
+        if (lane == 0) tc_commit(&empty[0]);
+      }
+    }
+    for (int i = 0; i < cnt && ok; ++i) {
+      const uint32_t vi = 2 * i + 1, ki = 2 * i + 2;
+      if (!(ok = wait_full(vi))) break;
+      const int keys = keys_of(t_lo + i);
+      if (keys < TC_N) {  // zero the slots behind the last key
+        const uint32_t v = buf(vi);
+        for (int e = lane; e < (TC_N - keys) * 8 * C::NCH; e += 32) {
+          const int r = keys + e / (8 * C::NCH), c = e % (8 * C::NCH);
+          asm volatile("st.shared.v4.u32 [%0], {%1, %1, %1, %1};" ::"r"(v + (c >> 3) * (TC_N * 128) + r * 128 + ((c & 7) << 4)), "r"(0)
+                       : "memory");
+        }
+        fence_async_smem();
+        __syncwarp();
+      }
+      for (int x = 0; x < nx && ok; ++x) {
+        ok = __all_sync(0xffffffffu, pa_wait(&p_full[x], i & 1, abort));
+        if (!ok) break;
+        tc_fence_after();
+        if (lane == 0) {
+#pragma unroll
+          for (int kk = 0; kk < TC_N / 16; ++kk)
+            umma_f16_ta(tmem + 2 * TC_N + x * HD, tmem + x * TC_N + kk * 8, umma_desc_sw128_mn(buf(vi) + kk * 2048, TC_N * 128), idesc_o,
+                        (i | kk) != 0);
+          if (i + 1 == cnt) tc_commit(&o_full[x]);
+        }
+        if (i + 1 < cnt) {
+          if (x == 0 && !(ok = wait_full(ki))) break;
+          tc_fence_after();
+          issue_s(x, ki);
+        }
+      }
+      if (ok && lane == 0) {
+        tc_commit(&empty[vi % NBUF]);
+        if (i + 1 < cnt) tc_commit(&empty[ki % NBUF]);
+      }
+    }
+  } else {
+    // ================================ softmax ================================
+    const int x = (warp - 2) >> 2;               // row tile
+    const int lanes = (warp & 3) * 32;           // TMEM lanes this warp may access
+    const int r = r0 + x * TC_M + lanes + lane;  // this thread's row
+    const uint32_t st = tmem + ((uint32_t)lanes << 16) + x * TC_N, ot = tmem + ((uint32_t)lanes << 16) + 2 * TC_N + x * HD;
+    const bool valid = r < rows;
+    const int see = PACKED ? 0 : (valid ? max(0, min(len, len - n + r / p.G + 1)) : own);
+    const float c = p.c;
+    float m = -INFINITY, l = 0.f;
+    if (x < nx && cnt > 0) {
+      // ---- Q: this warp's 32 rows, 16 bytes a lane, into the K-major swizzled tile
+      constexpr int LPR = HD / 8;  // 16-byte pieces of a row
+      const uint32_t qt = q_u + x * C::TILE;
+#pragma unroll 4
+      for (int e = lane; e < 32 * LPR; e += 32) {
+        const int rr = lanes + e / LPR, pc = e % LPR;
+        const int gr = r0 + x * TC_M + rr;
+        uint4 v = make_uint4(0u, 0u, 0u, 0u);
+        if (gr < rows) {
+          const size_t at = ((size_t)(row_lo + gr / p.G) * p.Hq + h * p.G + gr % p.G) * HD + pc * 8;
+          v = *reinterpret_cast<const uint4*>(reinterpret_cast<const __half*>(p.q) + at);
+        }
+        asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(qt + (pc >> 3) * (TC_M * 128) + sw128(rr, pc & 7)), "r"(v.x),
+                     "r"(v.y), "r"(v.z), "r"(v.w)
+                     : "memory");
+      }
+      fence_async_smem();
+      mbar_arrive(&q_full[x]);
+
+      bool ok = true;
+      for (int i = 0; i < cnt; ++i) {
+        ok = __all_sync(0xffffffffu, pa_wait(&s_full[x], i & 1, abort));
+        if (!ok) break;
+        tc_fence_after();
+        const int t = t_lo + i;
+        const uint32_t gone = s_absent[i & 15];
+        const int lim = (t < np ? P : see) - (t < np ? t : t - np) * TC_N;  // keys of the tile this row sees
+        const int lg = min(p.lg_page, 7);
+        const bool part = __any_sync(0xffffffffu, lim < TC_N) || gone != 0;
+        auto seen = [&](int k) { return k < lim && !((gone >> (k >> lg)) & 1u); };
+        // the row's maximum
+        float mx = -INFINITY;
+#pragma unroll
+        for (int q = 0; q < TC_N / 32; ++q) {
+          float v[32];
+          tmem_ld32(st + q * 32, v);
+          if (part) {
+#pragma unroll
+            for (int k = 0; k < 32; ++k) v[k] = seen(q * 32 + k) ? v[k] : -INFINITY;
+          }
+          float a0 = -INFINITY, a1 = -INFINITY;
+#pragma unroll
+          for (int k = 0; k < 32; k += 2) {
+            a0 = fmaxf(a0, v[k]);
+            a1 = fmaxf(a1, v[k + 1]);
+          }
+          mx = fmaxf(mx, fmaxf(a0, a1));
+        }
+        mx *= c;
+        if (__any_sync(0xffffffffu, mx > m + TC_RAISE)) {  // also from -inf
+          const float mn = fmaxf(m, mx);
+          const float f = m == -INFINITY ? 0.f : ex2(m - mn);
+          m = mn;
+          l *= f;
+          if (i > 0) {  // S is there: so is the last product into O
+#pragma unroll
+            for (int q = 0; q < HD / 32; ++q) {
+              float v[32];
+              tmem_ld32(ot + q * 32, v);
+#pragma unroll
+              for (int k = 0; k < 32; ++k) v[k] *= f;
+              tmem_st32(ot + q * 32, v);
+            }
+          }
+        }
+        const float mm = m == -INFINITY ? 0.f : m;
+        float l0 = 0.f, l1 = 0.f;
+#pragma unroll
+        for (int q = 0; q < TC_N / 32; ++q) {
+          float v[32];
+          tmem_ld32(st + q * 32, v);
+          if (part) {
+#pragma unroll
+            for (int k = 0; k < 32; ++k) v[k] = seen(q * 32 + k) ? v[k] : -INFINITY;
+          }
+          uint32_t w[16];
+#pragma unroll
+          for (int k = 0; k < 32; k += 2) {
+            const float e0 = ex2(fmaf(v[k], c, -mm)), e1 = ex2(fmaf(v[k + 1], c, -mm));
+            l0 += e0;
+            l1 += e1;
+            w[k / 2] = h2_as_u32(__floats2half2_rn(e0, e1));
+          }
+          tmem_st16(st + q * 16, w);  // over columns of S that have been read
+        }
+        l += l0 + l1;
+        tmem_wait_st();
+        tc_fence_before();
+        mbar_arrive(&p_full[x]);
+      }
+      // ---- O / l, or the partial result
+      ok = ok && __all_sync(0xffffffffu, pa_wait(&o_full[x], 0, abort));
+      tc_fence_after();
+      if (ok) {
+        const size_t row = valid ? (size_t)(row_lo + r / p.G) * p.Hq + h * p.G + r % p.G : 0;
+        const size_t at = (size_t)(slot0 + split) * p.T * p.Hq + row;
+        const float inv = l == 0.f ? 0.f : 1.f / l;
+        if (valid && p.nslots > 1) p.part_ml[at] = make_float2(m, l);
+#pragma unroll
+        for (int q = 0; q < HD / 32; ++q) {
+          float v[32];
+          tmem_ld32(ot + q * 32, v);
+          if (!valid) continue;
+          if (p.nslots > 1) {
+            float* dst = p.part_o + at * HD + q * 32;
+#pragma unroll
+            for (int k = 0; k < 32; k += 4) *reinterpret_cast<float4*>(dst + k) = make_float4(v[k], v[k + 1], v[k + 2], v[k + 3]);
+          } else {
+            __half* dst = reinterpret_cast<__half*>(p.out) + row * HD + q * 32;
+#pragma unroll
+            for (int k = 0; k < 32; k += 8) {
+              uint32_t w[4];
+#pragma unroll
+              for (int j = 0; j < 4; ++j) w[j] = h2_as_u32(__floats2half2_rn(v[k + 2 * j] * inv, v[k + 2 * j + 1] * inv));
+              *reinterpret_cast<uint4*>(dst + k) = make_uint4(w[0], w[1], w[2], w[3]);
+            }
+          }
+        }
+      }
+    } else if (x < nx && work && valid) {  // no keys in this share
+      const size_t row = (size_t)(row_lo + r / p.G) * p.Hq + h * p.G + r % p.G;
+      if (p.nslots > 1) {
+        p.part_ml[(size_t)(slot0 + split) * p.T * p.Hq + row] = make_float2(-INFINITY, 0.f);
+      } else {
+        for (int d = 0; d < HD; d += 8)
+          *reinterpret_cast<uint4*>(reinterpret_cast<__half*>(p.out) + row * HD + d) = make_uint4(0u, 0u, 0u, 0u);
+      }
+    }
+  }
+  // after a wait that ran out: the products in flight have ended before the TMEM is freed
+  tc_fence_before();
+  const bool failed = __syncthreads_or(*abort);
+  tc_fence_after();
+  if (failed && threadIdx.x == 32) {
+    int ignore = 0;
+    tc_commit(&drained);
+    pa_wait(&drained, 0, &ignore);
+  }
+  __syncthreads();
+  if (warp == 1) {
+    tmem_dealloc_cols(tmem, 512);
+    tmem_relinquish();
+  }
+  if (threadIdx.x == 0 && failed) atomicExch(&g_prefix_attn_error, 1);
+}
+
 // ---------------------------------------------------------------- join
 
 // One warp per (row, head): the slots' (m, l) first, one slot a lane, then
@@ -508,9 +922,9 @@ __global__ void __launch_bounds__(256) join_slots_kernel(const PrefixAttnParams 
 
 // ---------------------------------------------------------------- host side
 
-// A pool [rows, hd] as (128-byte chunk, row, chunk index), box (chunk, box_rows, all chunks), 128-byte swizzle: a
-// tile lies in shared memory as hd * es / 128 sub-tiles of box_rows rows of 128 bytes.
-static bool pool_map(CUtensorMap* m, const void* pool, size_t rows, int hd, bool f16, int box_rows) {
+// A pool [rows, hd] as (128-byte chunk, row, chunk index), box (chunk, box_rows, box_chunks), 128-byte swizzle: a
+// copy lies in shared memory as box_chunks sub-tiles of box_rows rows of 128 bytes.
+static bool pool_map(CUtensorMap* m, const void* pool, size_t rows, int hd, bool f16, int box_rows, int box_chunks) {
   static const PFN_cuTensorMapEncodeTiled_v12000 fn = [] {
     void* ptr = nullptr;
     cudaDriverEntryPointQueryResult q;
@@ -523,43 +937,85 @@ static bool pool_map(CUtensorMap* m, const void* pool, size_t rows, int hd, bool
   const int es = f16 ? 2 : 4, chunk = 128 / es;
   cuuint64_t dims[3] = {(cuuint64_t)chunk, (cuuint64_t)rows, (cuuint64_t)(hd / chunk)};
   cuuint64_t strides[2] = {(cuuint64_t)hd * es, 128};
-  cuuint32_t box[3] = {(cuuint32_t)chunk, (cuuint32_t)box_rows, (cuuint32_t)(hd / chunk)}, step[3] = {1, 1, 1};
+  cuuint32_t box[3] = {(cuuint32_t)chunk, (cuuint32_t)box_rows, (cuuint32_t)box_chunks}, step[3] = {1, 1, 1};
   return fn(m, f16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 3, const_cast<void*>(pool), dims,
             strides, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
             CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-// How a call is cut.  The host knows the rows T and the requests B, not which request has how many.
+// How a call is cut.  The host knows the rows T and the requests B, not which request has how many, nor how many
+// keys there are, only how many the tables hold.
+//   few rows      few_rows_kernel over the prefix and the requests' own keys
+//   shared        many_rows_kernel<PACKED> over the prefix (fp16), few_rows_kernel over the own keys
+//   chunks        many_rows_kernel over both (fp16)
 struct AttnPlan {
-  int splits, row_groups, nslots;
+  enum Kind { FEW, SHARED, CHUNKS } kind;
+  int splits, row_groups;       // few_rows_kernel
+  int tc_splits, tc_items;      // many_rows_kernel
+  int nslots;
 };
 
-static AttnPlan plan_attn(int T, int B, int Hkv, int G, int rt, long long max_keys, int sms) {
-  AttnPlan a;
-  // four CTAs per SM over all requests and heads: first from tiles of rows, then from the keys (at least a 16-key
-  // tile for each of a CTA's 4 warps)
-  const long long want = (4ll * sms + (long long)B * Hkv - 1) / ((long long)B * Hkv);
-  const long long tiles = ((long long)T * G + (long long)B * rt - 1) / ((long long)B * rt);
-  a.row_groups = (int)std::max(1ll, std::min(want, tiles));
-  const long long most = std::max(1ll, (max_keys + 63) / 64);
-  a.splits = (int)std::max(1ll, std::min({(want + a.row_groups - 1) / a.row_groups, most, 64ll}));
-  a.nslots = a.splits;
+static AttnPlan plan_attn(int T, int B, int Hkv, int G, bool f16, long long own_keys, long long prefix_keys, int sms) {
+  AttnPlan a{};
+  const long long rows = (long long)T * G, pairs = (rows + 2 * TC_M - 1) / (2 * TC_M);
+  const auto ceil_div = [](long long x, long long y) { return (x + y - 1) / y; };
+  a.kind = !f16 ? AttnPlan::FEW : rows >= 64ll * B ? AttnPlan::CHUNKS : prefix_keys > 0 && B > 1 ? AttnPlan::SHARED : AttnPlan::FEW;
+  if (a.kind != AttnPlan::FEW) {
+    // one CTA per SM holds two row tiles; shares of the keys until there is one CTA for every SM
+    const long long keys = prefix_keys + (a.kind == AttnPlan::CHUNKS ? own_keys : 0);
+    a.tc_items = (int)(a.kind == AttnPlan::CHUNKS ? pairs + B : pairs);
+    a.tc_splits = (int)std::max(1ll, std::min({(long long)sms / (pairs * Hkv), ceil_div(keys, TC_N), 32ll}));
+    a.nslots = a.tc_splits;
+  }
+  if (a.kind != AttnPlan::CHUNKS) {
+    // four CTAs per SM over all requests and heads: first from tiles of rows, then from the keys (at least a 16-key
+    // tile for each of a CTA's 4 warps)
+    const int rt = f16 ? 16 : 8;
+    const long long keys = own_keys + (a.kind == AttnPlan::FEW ? prefix_keys : 0);
+    const long long want = ceil_div(4ll * sms, (long long)B * Hkv), tiles = ceil_div(rows, (long long)B * rt);
+    a.row_groups = (int)std::max(1ll, std::min(want, tiles));
+    a.splits = (int)std::max(1ll, std::min({ceil_div(want, a.row_groups), ceil_div(keys, 64), 64ll}));
+    a.nslots += a.splits;
+  }
   return a;
 }
 
-template <typename T, int HD>
-static int run_attn(PrefixAttnParams p, const void* k, const void* v, const AttnPlan& a, cudaStream_t stream) {
-  using C = FewRows<T, HD>;
-  PoolMaps maps;
-  SC_REQUIRE(pool_map(&maps.k, k, p.pool_rows, HD, C::F16, FR_KT) && pool_map(&maps.v, v, p.pool_rows, HD, C::F16, FR_KT),
-             SC_ERR_CUDA, "prefix_attn: tensor map of the pages refused");
-  auto kern = few_rows_kernel<T, HD>;
-  const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM);
+template <int HD, bool PACKED>
+static int run_many_rows(const PrefixAttnParams& p, const PoolMaps& maps, const AttnPlan& a, cudaStream_t stream) {
+  auto kern = many_rows_kernel<HD, PACKED>;
+  const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, ManyRows<HD>::SMEM);
   if (e != cudaSuccess) return check_launch("prefix_attn", e);
-  launch(kern, dim3(a.splits * a.row_groups, p.Hkv, p.B), dim3(FR_WARPS * 32), C::SMEM, stream, p, maps, 1, a.splits,
-         a.row_groups, 0);
-  const int st = check_launch("prefix_attn");
-  if (st != SC_OK || p.nslots == 1) return st;
+  launch(kern, dim3((unsigned)(a.tc_splits * a.tc_items), p.Hkv), dim3(TC_THREADS), ManyRows<HD>::SMEM, stream, p, maps, a.tc_splits, 0);
+  return check_launch("prefix_attn_many_rows");
+}
+
+template <typename T, int HD>
+static int run_attn(const PrefixAttnParams& p, const void* k, const void* v, const AttnPlan& a, cudaStream_t stream) {
+  using C = FewRows<T, HD>;
+  int st = SC_OK;
+  if constexpr (C::F16) {
+    if (a.kind != AttnPlan::FEW) {
+      PoolMaps maps;
+      const int box = std::min(TC_N, 1 << p.lg_page);
+      SC_REQUIRE(pool_map(&maps.k, k, p.pool_rows, HD, true, box, 1) && pool_map(&maps.v, v, p.pool_rows, HD, true, box, 1),
+                 SC_ERR_CUDA, "prefix_attn: tensor map of the pages refused");
+      st = a.kind == AttnPlan::SHARED ? run_many_rows<HD, true>(p, maps, a, stream) : run_many_rows<HD, false>(p, maps, a, stream);
+      if (st != SC_OK) return st;
+    }
+  }
+  if (a.kind != AttnPlan::CHUNKS) {
+    PoolMaps maps;
+    SC_REQUIRE(pool_map(&maps.k, k, p.pool_rows, HD, C::F16, FR_KT, C::NB) && pool_map(&maps.v, v, p.pool_rows, HD, C::F16, FR_KT, C::NB),
+               SC_ERR_CUDA, "prefix_attn: tensor map of the pages refused");
+    auto kern = few_rows_kernel<T, HD>;
+    const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM);
+    if (e != cudaSuccess) return check_launch("prefix_attn", e);
+    launch(kern, dim3(a.splits * a.row_groups, p.Hkv, p.B), dim3(FR_WARPS * 32), C::SMEM, stream, p, maps,
+           a.kind == AttnPlan::FEW ? 1 : 0, a.splits, a.row_groups, a.kind == AttnPlan::SHARED ? a.tc_splits : 0);
+    st = check_launch("prefix_attn_few_rows");
+    if (st != SC_OK) return st;
+  }
+  if (p.nslots == 1) return SC_OK;
   launch(join_slots_kernel<T, HD>, dim3((unsigned)(((size_t)p.T * p.Hq + 7) / 8)), dim3(256), 0, stream, p);
   return check_launch("prefix_attn_join");
 }
@@ -582,8 +1038,8 @@ size_t sc_prefix_attn_workspace_bytes(int T, int B, int Hq, int Hkv, int hd, int
                                       int page_size, int dtype) {
   if (T < 1 || B < 1 || Hq < 1 || Hkv < 1 || hd < 1 || max_blocks < 0 || max_prefix_blocks < 0 || page_size < 1) return 0;
   if (Hq % Hkv) return 0;
-  const sc::AttnPlan a = sc::plan_attn(T, B, Hkv, Hq / Hkv, dtype == SC_F16 ? 16 : 8,
-                                       ((long long)max_blocks + max_prefix_blocks) * page_size, sc::sm_count());
+  const sc::AttnPlan a = sc::plan_attn(T, B, Hkv, Hq / Hkv, dtype == SC_F16, (long long)max_blocks * page_size,
+                                       (long long)max_prefix_blocks * page_size, sc::sm_count());
   return a.nslots <= 1 ? 0 : (size_t)a.nslots * T * Hq * (hd + 2) * sizeof(float);
 }
 
@@ -601,15 +1057,15 @@ int sc_prefix_attn(const void* q, const void* k_pages, const void* v_pages, int 
              "prefix_attn: page size %d unsupported (a power of two from 16)", page_size);
   SC_REQUIRE(T >= 1 && B >= 1 && B <= 65535 && max_blocks >= 1 && n_pages >= 1, SC_ERR_SHAPE, "prefix_attn: bad T/B/max_blocks");
   SC_REQUIRE(Hkv >= 1 && Hkv <= 65535 && Hq >= Hkv && Hq % Hkv == 0, SC_ERR_SHAPE, "prefix_attn: Hq=%d not a multiple of Hkv=%d", Hq, Hkv);
-  SC_REQUIRE((long long)n_pages * Hkv * page_size < INT32_MAX && (long long)T * Hq <= INT32_MAX &&
+  SC_REQUIRE((long long)n_pages * Hkv * page_size < INT32_MAX && (long long)T * Hq <= (1 << 30) &&
                  (long long)max_blocks * page_size <= INT32_MAX && (long long)max_prefix_blocks * page_size <= INT32_MAX,
              SC_ERR_SHAPE, "prefix_attn: rows past 32 bits");
   SC_REQUIRE(scale > 0.f && scale < INFINITY, SC_ERR_ARG, "prefix_attn: scale must be positive and finite");
   SC_REQUIRE((((uintptr_t)q | (uintptr_t)k_pages | (uintptr_t)v_pages | (uintptr_t)out) & 15) == 0, SC_ERR_ARG,
              "prefix_attn: tensors must start on 16-byte boundaries");
   if (!prefix_len) max_prefix_blocks = 0;
-  const AttnPlan a = plan_attn(T, B, Hkv, Hq / Hkv, dtype == SC_F16 ? 16 : 8,
-                               ((long long)max_blocks + max_prefix_blocks) * page_size, sm_count());
+  const AttnPlan a = plan_attn(T, B, Hkv, Hq / Hkv, dtype == SC_F16, (long long)max_blocks * page_size,
+                               (long long)max_prefix_blocks * page_size, sm_count());
   const size_t need = sc_prefix_attn_workspace_bytes(T, B, Hq, Hkv, hd, max_blocks, max_prefix_blocks, page_size, dtype);
   SC_REQUIRE(workspace_bytes >= need && (need == 0 || workspace), SC_ERR_WORKSPACE,
              "prefix_attn: workspace of %zu bytes needed (got %zu)", need, workspace_bytes);
