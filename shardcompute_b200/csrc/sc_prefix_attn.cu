@@ -140,7 +140,10 @@ few_rows_kernel(const PrefixAttnParams p, const __grid_constant__ PoolMaps maps,
   }
   __syncthreads();
   pdl_trigger();
-  pdl_wait();
+  // Without the prefix this kernel follows many_rows_kernel, whose CTAs all are past their own wait by the time
+  // this one starts: what both read is there, and they run side by side.  It waits for that kernel before it ends,
+  // so that the join, which waits for this one, has both results.
+  if (with_prefix) pdl_wait();
   int row_lo, row_hi;
   request_rows(p, b, row_lo, row_hi);
   const int n = row_hi - row_lo, len = request_len(p, b), P = with_prefix ? prefix_keys(p) : 0;
@@ -455,6 +458,7 @@ few_rows_kernel(const PrefixAttnParams p, const __grid_constant__ PoolMaps maps,
       mbar_wait_bounded(&full[warp][used % NST], (used / NST) & 1u, &ignore, PA_WAIT_NS);
     }
   if (threadIdx.x == 0 && s_abort) atomicExch(&g_prefix_attn_error, 1);
+  if (!with_prefix) pdl_wait();
 }
 
 // ---------------------------------------------------------------- many rows, fp16
@@ -468,15 +472,16 @@ few_rows_kernel(const PrefixAttnParams p, const __grid_constant__ PoolMaps maps,
 //   warp 1     MMA issuer: S = Q K^T into TMEM, then O += P V with P read
 //              from TMEM; V's slots behind the last key are zeroed here first,
 //              for they may hold anything (0 x NaN is NaN)
-//   warps 2-5, 6-9: softmax of tile 0 and of tile 1, a thread per row: the
-//              row's maximum, P = exp2(c s - m) in fp16 over S's own columns,
-//              its sum in fp32, and in the end O / l or a partial result
+//   warps 4-7, 8-11: softmax of tile 0 and of tile 1, a thread per row, which
+//              holds its 128 scores in registers: their maximum, P = exp2(c s
+//              - m) in fp16 over S's own columns, its sum in fp32, and in the
+//              end O / l or a partial result
 // The tiles take turns: while one is in the softmax, the other is in the
 // tensor cores.  The maximum a row is scaled by is raised, and O rescaled,
 // only when a score passes it by 2^8 (P then stays below 2^8 and l in fp32).
 // TMEM: S0 | S1 (128 columns each, P in the first 64), O0 | O1 (HD each).
 constexpr int TC_M = 128, TC_N = 128;   // rows and keys of a tile
-constexpr int TC_THREADS = 10 * 32;
+constexpr int TC_THREADS = 12 * 32;
 constexpr float TC_RAISE = 8.f;
 
 template <int HD>
@@ -517,6 +522,47 @@ __device__ __forceinline__ void tmem_st32(uint32_t taddr, const float (&v)[32]) 
   tmem_st16(taddr + 16, b);
 }
 __device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+// 32 columns, not waited for: tmem_wait_ld, then tmem_ready of each block before its values are used.
+__device__ __forceinline__ void tmem_ld32_async(uint32_t taddr, float* v) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,"
+      "%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+      : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]), "=f"(v[4]), "=f"(v[5]), "=f"(v[6]), "=f"(v[7]), "=f"(v[8]),
+        "=f"(v[9]), "=f"(v[10]), "=f"(v[11]), "=f"(v[12]), "=f"(v[13]), "=f"(v[14]), "=f"(v[15]), "=f"(v[16]),
+        "=f"(v[17]), "=f"(v[18]), "=f"(v[19]), "=f"(v[20]), "=f"(v[21]), "=f"(v[22]), "=f"(v[23]), "=f"(v[24]),
+        "=f"(v[25]), "=f"(v[26]), "=f"(v[27]), "=f"(v[28]), "=f"(v[29]), "=f"(v[30]), "=f"(v[31])
+      : "r"(taddr));
+}
+__device__ __forceinline__ void tmem_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void tmem_ready(float* v) {  // no use of v[0..31] moves above this
+#pragma unroll
+  for (int i = 0; i < 32; i += 8)
+    asm volatile("" : "+f"(v[i]), "+f"(v[i + 1]), "+f"(v[i + 2]), "+f"(v[i + 3]), "+f"(v[i + 4]), "+f"(v[i + 5]), "+f"(v[i + 6]), "+f"(v[i + 7]));
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float d;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
+// two fp32 in one instruction
+__device__ __forceinline__ uint64_t pack2(float x, float y) {
+  uint64_t d;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(d) : "f"(x), "f"(y));
+  return d;
+}
+__device__ __forceinline__ void unpack2(uint64_t d, float& x, float& y) {
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(x), "=f"(y) : "l"(d));
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+  return d;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t d;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
 
 // PACKED: rows of all requests, keys of the prefix.  Otherwise: rows of one
 // request, keys of the prefix and its own.
@@ -553,8 +599,8 @@ many_rows_kernel(const PrefixAttnParams p, const __grid_constant__ PoolMaps maps
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  pdl_trigger();
   pdl_wait();
+  pdl_trigger();  // after the wait: few_rows_kernel relies on it
   volatile int* abort = &s_abort;
   const uint32_t tmem = s_tmem;
 
@@ -630,8 +676,9 @@ many_rows_kernel(const PrefixAttnParams p, const __grid_constant__ PoolMaps maps
         const int id = t < np ? p.prefix_table[blk] : p.block_table[(size_t)b * p.max_blocks + blk];
         if (id >= 0 && id < p.n_pages) row = ((id * p.Hkv + h) << p.lg_page) + (key & ((1 << p.lg_page) - 1));
       }
-      uint32_t gone = 0;  // pages of this tile that do not exist, a bit per copy's rows
-      for (int k = 0; k < (TC_N >> lg); ++k) gone |= (__shfl_sync(0xffffffffu, row, k * C::NCH) < 0 ? 1u : 0u) << k;
+      uint32_t gone = 0;  // keys of this tile that have no page, a bit per 16
+      for (int k = 0; k < TC_N / 16; ++k)
+        gone |= (__shfl_sync(0xffffffffu, row, ((k * 16) >> lg) * C::NCH) < 0 ? 1u : 0u) << k;
       if (lane == 0) s_absent[i & 15] = gone;
 #pragma unroll
       for (int kv = 0; kv < 2; ++kv, ++it) {
@@ -714,9 +761,9 @@ many_rows_kernel(const PrefixAttnParams p, const __grid_constant__ PoolMaps maps
         if (i + 1 < cnt) tc_commit(&empty[ki % NBUF]);
       }
     }
-  } else {
+  } else if (warp >= 4) {
     // ================================ softmax ================================
-    const int x = (warp - 2) >> 2;               // row tile
+    const int x = (warp - 4) >> 2;               // row tile
     const int lanes = (warp & 3) * 32;           // TMEM lanes this warp may access
     const int r = r0 + x * TC_M + lanes + lane;  // this thread's row
     const uint32_t st = tmem + ((uint32_t)lanes << 16) + x * TC_N, ot = tmem + ((uint32_t)lanes << 16) + 2 * TC_N + x * HD;
@@ -752,27 +799,27 @@ many_rows_kernel(const PrefixAttnParams p, const __grid_constant__ PoolMaps maps
         const int t = t_lo + i;
         const uint32_t gone = s_absent[i & 15];
         const int lim = (t < np ? P : see) - (t < np ? t : t - np) * TC_N;  // keys of the tile this row sees
-        const int lg = min(p.lg_page, 7);
         const bool part = __any_sync(0xffffffffu, lim < TC_N) || gone != 0;
-        auto seen = [&](int k) { return k < lim && !((gone >> (k >> lg)) & 1u); };
-        // the row's maximum
-        float mx = -INFINITY;
+        auto seen = [&](int k) { return k < lim && !((gone >> (k / 16)) & 1u); };
+        float v[TC_N];
 #pragma unroll
-        for (int q = 0; q < TC_N / 32; ++q) {
-          float v[32];
-          tmem_ld32(st + q * 32, v);
-          if (part) {
+        for (int q = 0; q < TC_N; q += 32) tmem_ld32_async(st + q, v + q);
+        tmem_wait_ld();
 #pragma unroll
-            for (int k = 0; k < 32; ++k) v[k] = seen(q * 32 + k) ? v[k] : -INFINITY;
-          }
-          float a0 = -INFINITY, a1 = -INFINITY;
+        for (int q = 0; q < TC_N; q += 32) tmem_ready(v + q);
+        if (part) {
 #pragma unroll
-          for (int k = 0; k < 32; k += 2) {
-            a0 = fmaxf(a0, v[k]);
-            a1 = fmaxf(a1, v[k + 1]);
-          }
-          mx = fmaxf(mx, fmaxf(a0, a1));
+          for (int k = 0; k < TC_N; ++k) v[k] = seen(k) ? v[k] : -INFINITY;
         }
+        float a0 = fmaxf(v[0], v[1]), a1 = fmaxf(v[2], v[3]), a2 = fmaxf(v[4], v[5]), a3 = fmaxf(v[6], v[7]);
+#pragma unroll
+        for (int k = 8; k < TC_N; k += 8) {
+          a0 = max3(a0, v[k], v[k + 1]);
+          a1 = max3(a1, v[k + 2], v[k + 3]);
+          a2 = max3(a2, v[k + 4], v[k + 5]);
+          a3 = max3(a3, v[k + 6], v[k + 7]);
+        }
+        float mx = fmaxf(fmaxf(a0, a1), fmaxf(a2, a3));
         mx *= c;
         if (__any_sync(0xffffffffu, mx > m + TC_RAISE)) {  // also from -inf
           const float mn = fmaxf(m, mx);
@@ -782,34 +829,33 @@ many_rows_kernel(const PrefixAttnParams p, const __grid_constant__ PoolMaps maps
           if (i > 0) {  // S is there: so is the last product into O
 #pragma unroll
             for (int q = 0; q < HD / 32; ++q) {
-              float v[32];
-              tmem_ld32(ot + q * 32, v);
+              float u[32];
+              tmem_ld32(ot + q * 32, u);
 #pragma unroll
-              for (int k = 0; k < 32; ++k) v[k] *= f;
-              tmem_st32(ot + q * 32, v);
+              for (int k = 0; k < 32; ++k) u[k] *= f;
+              tmem_st32(ot + q * 32, u);
             }
           }
         }
         const float mm = m == -INFINITY ? 0.f : m;
-        float l0 = 0.f, l1 = 0.f;
+        const uint64_t c2 = pack2(c, c), m2 = pack2(-mm, -mm);
+        uint64_t l2[2] = {pack2(0.f, 0.f), pack2(0.f, 0.f)};
 #pragma unroll
         for (int q = 0; q < TC_N / 32; ++q) {
-          float v[32];
-          tmem_ld32(st + q * 32, v);
-          if (part) {
-#pragma unroll
-            for (int k = 0; k < 32; ++k) v[k] = seen(q * 32 + k) ? v[k] : -INFINITY;
-          }
           uint32_t w[16];
 #pragma unroll
           for (int k = 0; k < 32; k += 2) {
-            const float e0 = ex2(fmaf(v[k], c, -mm)), e1 = ex2(fmaf(v[k + 1], c, -mm));
-            l0 += e0;
-            l1 += e1;
+            float e0, e1;
+            unpack2(fma2(pack2(v[q * 32 + k], v[q * 32 + k + 1]), c2, m2), e0, e1);
+            e0 = ex2(e0);
+            e1 = ex2(e1);
+            l2[(k >> 1) & 1] = add2(l2[(k >> 1) & 1], pack2(e0, e1));
             w[k / 2] = h2_as_u32(__floats2half2_rn(e0, e1));
           }
           tmem_st16(st + q * 16, w);  // over columns of S that have been read
         }
+        float l0, l1;
+        unpack2(add2(l2[0], l2[1]), l0, l1);
         l += l0 + l1;
         tmem_wait_st();
         tc_fence_before();
