@@ -469,9 +469,10 @@ few_rows_kernel(const PrefixAttnParams p, const __grid_constant__ PoolMaps maps,
 // and a head of the group), a kv head and a share of the keys:
 //   warp 0     TMA producer: K and V tiles of 128 keys through one ring, a
 //              copy per page and 64-wide column, issued by a lane each
-//   warp 1     MMA issuer: S = Q K^T into TMEM, then O += P V with P read
-//              from TMEM; V's slots behind the last key are zeroed here first,
-//              for they may hold anything (0 x NaN is NaN)
+//   warps 1, 2 MMA issuers of tile 0 and of tile 1: S = Q K^T into TMEM, then
+//              O += P V with P read from TMEM, each half of P as it is ready
+//   warp 3     zeroes V's slots behind the last key, which may hold anything
+//              (0 x NaN is NaN), before the MMA issuers use the tile
 //   warps 4-7, 8-11: softmax of tile 0 and of tile 1, a thread per row, which
 //              holds its 128 scores in registers: their maximum, P = exp2(c s
 //              - m) in fp16 over S's own columns, its sum in fp32, and in the
@@ -494,6 +495,13 @@ struct ManyRows {
 
 __device__ __forceinline__ bool pa_wait(uint64_t* bar, uint32_t parity, volatile int* abort) {
   return mbar_wait_bounded(bar, parity, abort, PA_WAIT_NS);
+}
+
+// The same for one thread on the critical path: polls, and looks at the clock now and then.
+__device__ __forceinline__ bool pa_spin(uint64_t* bar, uint32_t parity, volatile int* abort) {
+  for (int i = 0; i < 64; ++i)
+    if (mbar_test_wait(bar, parity)) return true;
+  return pa_wait(bar, parity, abort);
 }
 
 __device__ __forceinline__ void tma3d_at(uint32_t dst, const CUtensorMap* map, int row, int chunk, uint64_t* bar) {
@@ -572,7 +580,7 @@ many_rows_kernel(const PrefixAttnParams p, const __grid_constant__ PoolMaps maps
   using C = ManyRows<HD>;
   constexpr int NBUF = C::NBUF;
   extern __shared__ __align__(1024) unsigned char mr_smem[];
-  __shared__ __align__(8) uint64_t full[NBUF], empty[NBUF], q_full[2], s_full[2], p_full[2], o_full[2], drained;
+  __shared__ __align__(8) uint64_t full[NBUF], empty[NBUF], q_full[2], s_full[2], p_full[2][2], o_full[2], v_clean[2], drained[2], turn[2][4];
   __shared__ uint32_t s_tmem, s_absent[16];
   __shared__ int s_abort, s_req, s_row0, s_sum[TC_THREADS / 32];
   unsigned char* base = mr_smem + ((1024 - (smem_u32(mr_smem) & 1023)) & 1023);
@@ -580,20 +588,8 @@ many_rows_kernel(const PrefixAttnParams p, const __grid_constant__ PoolMaps maps
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   const int split = blockIdx.x % splits, item = blockIdx.x / splits, h = blockIdx.y;
   if (threadIdx.x == 0) {
-    for (int i = 0; i < NBUF; ++i) {
-      mbar_init(&full[i], 1);
-      mbar_init(&empty[i], 1);
-    }
-    for (int x = 0; x < 2; ++x) {
-      mbar_init(&q_full[x], TC_M);
-      mbar_init(&s_full[x], 1);
-      mbar_init(&p_full[x], TC_M);
-      mbar_init(&o_full[x], 1);
-    }
-    mbar_init(&drained, 1);
     s_abort = 0;
     s_req = -1;
-    fence_mbar_init();
   }
   if (warp == 1) tmem_alloc_cols(&s_tmem, 512);
   tc_fence_before();
@@ -660,6 +656,28 @@ many_rows_kernel(const PrefixAttnParams p, const __grid_constant__ PoolMaps maps
   const int nx = work && r0 + TC_M < rows ? 2 : 1;  // row tiles in use
   // keys of tile t that exist
   auto keys_of = [&](int t) { return t < np ? P - t * TC_N : own - (t - np) * TC_N; };
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < NBUF; ++i) {
+      mbar_init(&full[i], 1);
+      mbar_init(&empty[i], nx);
+    }
+    for (int x = 0; x < 2; ++x) {
+      mbar_init(&q_full[x], TC_M);
+      mbar_init(&s_full[x], 1);
+      mbar_init(&p_full[x][0], 4);
+      mbar_init(&p_full[x][1], 4);
+      mbar_init(&o_full[x], 1);
+      mbar_init(&drained[x], 1);
+    }
+    for (int w = 0; w < 4; ++w) {
+      mbar_init(&turn[0][w], 1);
+      mbar_init(&turn[1][w], 1);
+    }
+    mbar_init(&v_clean[0], 1);  // the prefix's last tile
+    mbar_init(&v_clean[1], 1);  // the request's
+    fence_mbar_init();
+  }
+  __syncthreads();
 
   if (warp == 0) {
     // ================================ TMA producer ================================
@@ -697,69 +715,70 @@ many_rows_kernel(const PrefixAttnParams p, const __grid_constant__ PoolMaps maps
       int ignore = 0;
       for (uint32_t k = it > NBUF ? it - NBUF : 0; k < it; ++k) pa_wait(&full[k % NBUF], (k / NBUF) & 1u, &ignore);
     }
-  } else if (warp == 1) {
-    // ================================ MMA issuer ================================
-    const uint32_t idesc_s = (1u << 4) | ((TC_N >> 3) << 17) | ((TC_M >> 4) << 24);
-    const uint32_t idesc_o = (1u << 4) | (1u << 16) | ((HD >> 3) << 17) | ((TC_M >> 4) << 24);  // V: contiguous along N
-    auto buf = [&](uint32_t it) { return ring_u + (it % NBUF) * C::TILE; };
-    auto wait_full = [&](uint32_t it) {
-      return __all_sync(0xffffffffu, pa_wait(&full[it % NBUF], (it / NBUF) & 1u, abort));
-    };
-    auto issue_s = [&](int x, uint32_t it) {  // S_x = Q_x K^T
-      if (lane == 0) {
+  } else if (warp <= 2) {
+    // ================================ MMA issuers ================================
+    const int x = warp - 1;
+    if (lane == 0 && x < nx && cnt > 0) {
+      constexpr uint32_t idesc_s = (1u << 4) | ((TC_N >> 3) << 17) | ((TC_M >> 4) << 24);
+      constexpr uint32_t idesc_o = (1u << 4) | (1u << 16) | ((HD >> 3) << 17) | ((TC_M >> 4) << 24);  // V: contiguous along N
+      const uint32_t ts = tmem + x * TC_N, to = tmem + 2 * TC_N + x * HD;
+      const uint64_t dq = umma_desc_sw128(q_u + x * C::TILE), dk = umma_desc_sw128(ring_u), dv = umma_desc_sw128_mn(ring_u, TC_N * 128);
+      auto at = [](uint32_t it) { return (uint64_t)((it % NBUF) * (C::TILE >> 4)); };  // a ring tile, in descriptor units
+      auto wait_full = [&](uint32_t it) { return pa_spin(&full[it % NBUF], (it / NBUF) & 1u, abort); };
+      auto issue_s = [&](uint32_t it) {  // S = Q K^T
+        const uint64_t k = dk + at(it);
 #pragma unroll
         for (int kk = 0; kk < HD / 16; ++kk) {
-          const uint32_t off = (kk >> 2) * (TC_N * 128) + (kk & 3) * 32;
-          umma_f16(tmem + x * TC_N, umma_desc_sw128(q_u + x * C::TILE + off), umma_desc_sw128(buf(it) + off), idesc_s, kk != 0);
+          const uint32_t off = ((kk >> 2) * (TC_N * 128) + (kk & 3) * 32) >> 4;
+          umma_f16(ts, dq + off, k + off, idesc_s, kk != 0);
         }
         tc_commit(&s_full[x]);
-      }
-    };
-    bool ok = true;
-    if (cnt > 0) {
-      for (int x = 0; x < nx && ok; ++x) ok = __all_sync(0xffffffffu, pa_wait(&q_full[x], 0, abort));
-      ok = ok && wait_full(0);
-      tc_fence_after();
+        tc_commit(&empty[it % NBUF]);
+      };
+      bool ok = pa_spin(&q_full[x], 0, abort) && wait_full(0);
       if (ok) {
-        for (int x = 0; x < nx; ++x) issue_s(x, 0);
-        if (lane == 0) tc_commit(&empty[0]);
+        tc_fence_after();
+        issue_s(0);
+      }
+      for (int i = 0; i < cnt && ok; ++i) {
+        const uint32_t vi = 2 * i + 1, ki = 2 * i + 2;
+        ok = wait_full(vi);
+        if (ok && keys_of(t_lo + i) < TC_N) ok = pa_spin(&v_clean[t_lo + i >= np], 0, abort);
+        const uint64_t v = dv + at(vi);
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+          ok = ok && pa_spin(&p_full[x][half], i & 1, abort);
+          if (!ok) break;
+          tc_fence_after();
+#pragma unroll
+          for (int kk = half * (TC_N / 32); kk < (half + 1) * (TC_N / 32); ++kk)
+            umma_f16_ta(to, ts + kk * 8, v + kk * (2048 >> 4), idesc_o, (i | kk) != 0);
+        }
+        if (!ok) break;
+        tc_commit(&empty[vi % NBUF]);
+        if (i + 1 == cnt) {
+          tc_commit(&o_full[x]);
+        } else {
+          ok = wait_full(ki);
+          if (ok) issue_s(ki);
+        }
       }
     }
-    for (int i = 0; i < cnt && ok; ++i) {
-      const uint32_t vi = 2 * i + 1, ki = 2 * i + 2;
-      if (!(ok = wait_full(vi))) break;
+  } else if (warp == 3) {
+    // ================================ V's tail ================================
+    for (int i = 0; i < cnt; ++i) {
       const int keys = keys_of(t_lo + i);
-      if (keys < TC_N) {  // zero the slots behind the last key
-        const uint32_t v = buf(vi);
-        for (int e = lane; e < (TC_N - keys) * 8 * C::NCH; e += 32) {
-          const int r = keys + e / (8 * C::NCH), c = e % (8 * C::NCH);
-          asm volatile("st.shared.v4.u32 [%0], {%1, %1, %1, %1};" ::"r"(v + (c >> 3) * (TC_N * 128) + r * 128 + ((c & 7) << 4)), "r"(0)
-                       : "memory");
-        }
-        fence_async_smem();
-        __syncwarp();
+      if (keys >= TC_N) continue;
+      const uint32_t vi = 2 * i + 1, v = ring_u + (vi % NBUF) * C::TILE;
+      if (!__all_sync(0xffffffffu, pa_wait(&full[vi % NBUF], (vi / NBUF) & 1u, abort))) break;
+      for (int e = lane; e < (TC_N - keys) * 8 * C::NCH; e += 32) {
+        const int r = keys + e / (8 * C::NCH), c = e % (8 * C::NCH);
+        asm volatile("st.shared.v4.u32 [%0], {%1, %1, %1, %1};" ::"r"(v + (c >> 3) * (TC_N * 128) + r * 128 + ((c & 7) << 4)), "r"(0)
+                     : "memory");
       }
-      for (int x = 0; x < nx && ok; ++x) {
-        ok = __all_sync(0xffffffffu, pa_wait(&p_full[x], i & 1, abort));
-        if (!ok) break;
-        tc_fence_after();
-        if (lane == 0) {
-#pragma unroll
-          for (int kk = 0; kk < TC_N / 16; ++kk)
-            umma_f16_ta(tmem + 2 * TC_N + x * HD, tmem + x * TC_N + kk * 8, umma_desc_sw128_mn(buf(vi) + kk * 2048, TC_N * 128), idesc_o,
-                        (i | kk) != 0);
-          if (i + 1 == cnt) tc_commit(&o_full[x]);
-        }
-        if (i + 1 < cnt) {
-          if (x == 0 && !(ok = wait_full(ki))) break;
-          tc_fence_after();
-          issue_s(x, ki);
-        }
-      }
-      if (ok && lane == 0) {
-        tc_commit(&empty[vi % NBUF]);
-        if (i + 1 < cnt) tc_commit(&empty[ki % NBUF]);
-      }
+      fence_async_smem();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&v_clean[t_lo + i >= np]);
     }
   } else if (warp >= 4) {
     // ================================ softmax ================================
@@ -838,6 +857,12 @@ many_rows_kernel(const PrefixAttnParams p, const __grid_constant__ PoolMaps maps
           }
         }
         const float mm = m == -INFINITY ? 0.f : m;
+        // The two warps of a scheduler take turns here, or both tiles fall into step: both in the softmax, then both
+        // in the tensor cores.
+        if (nx == 2 && (x == 1 || i > 0)) {
+          ok = __all_sync(0xffffffffu, pa_wait(&turn[x][warp & 3], (x == 1 ? i : i - 1) & 1, abort));
+          if (!ok) break;
+        }
         const uint64_t c2 = pack2(c, c), m2 = pack2(-mm, -mm);
         uint64_t l2[2] = {pack2(0.f, 0.f), pack2(0.f, 0.f)};
 #pragma unroll
@@ -853,13 +878,17 @@ many_rows_kernel(const PrefixAttnParams p, const __grid_constant__ PoolMaps maps
             w[k / 2] = h2_as_u32(__floats2half2_rn(e0, e1));
           }
           tmem_st16(st + q * 16, w);  // over columns of S that have been read
+          if (q & 1) {
+            tmem_wait_st();
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&p_full[x][q >> 1]);
+          }
         }
+        if (nx == 2 && lane == 0) mbar_arrive(&turn[x ^ 1][warp & 3]);
         float l0, l1;
         unpack2(add2(l2[0], l2[1]), l0, l1);
         l += l0 + l1;
-        tmem_wait_st();
-        tc_fence_before();
-        mbar_arrive(&p_full[x]);
       }
       // ---- O / l, or the partial result
       ok = ok && __all_sync(0xffffffffu, pa_wait(&o_full[x], 0, abort));
@@ -904,10 +933,10 @@ many_rows_kernel(const PrefixAttnParams p, const __grid_constant__ PoolMaps maps
   tc_fence_before();
   const bool failed = __syncthreads_or(*abort);
   tc_fence_after();
-  if (failed && threadIdx.x == 32) {
+  if (failed && (warp == 1 || warp == 2) && lane == 0) {
     int ignore = 0;
-    tc_commit(&drained);
-    pa_wait(&drained, 0, &ignore);
+    tc_commit(&drained[warp - 1]);
+    pa_wait(&drained[warp - 1], 0, &ignore);
   }
   __syncthreads();
   if (warp == 1) {
