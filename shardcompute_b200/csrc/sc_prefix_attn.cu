@@ -483,6 +483,8 @@ few_rows_kernel(const PrefixAttnParams p, const __grid_constant__ PoolMaps maps,
 // TMEM: S0 | S1 (128 columns each, P in the first 64), O0 | O1 (HD each).
 constexpr int TC_M = 128, TC_N = 128;   // rows and keys of a tile
 constexpr int TC_THREADS = 12 * 32;
+constexpr int TC_REGS_CTL = 88, TC_REGS_SM = 208;  // 128 x 88 + 256 x 208: what the block starts with, 384 x 168
+constexpr int TC_HAND = 3;  // quarter of a tile before which its softmax lets the other one start
 constexpr float TC_RAISE = 8.f;
 
 template <int HD>
@@ -572,6 +574,78 @@ __device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
   return d;
 }
 
+// The rows and keys of a CTA of the many-rows kernels: `item`-th block of ROWS rows (of the whole batch where PACKED,
+// else of one request, items counted over the requests), the split-th share of its tiles of KEYS keys.
+struct RowShare {
+  int b, r0;               // request; first row, counted in the request (in the batch where PACKED)
+  int row_lo, rows;        // the request's first token in q, its rows
+  int n, len, P, np, own;  // its new tokens, its tokens; prefix keys, prefix tiles; own keys that the last row sees
+  int t_lo, cnt;           // tiles
+  bool work;
+};
+
+template <bool PACKED, int ROWS, int KEYS, int THREADS>
+__device__ __forceinline__ RowShare row_share(const PrefixAttnParams& p, int item, int split, int splits, int& s_req, int& s_row0,
+                                              int* s_sum) {
+  RowShare w;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  int row_hi;
+  if (PACKED) {
+    w.b = 0;
+    w.row_lo = 0;
+    row_hi = min(max(p.q_start[p.B], 0), p.T);
+    w.r0 = item * ROWS;
+    w.work = true;
+  } else {
+    // s_req, s_row0: the request that holds the item, found by a scan of the requests' items
+    int before = 0;
+    for (int b0 = 0; b0 < p.B; b0 += THREADS) {
+      const int bb = b0 + threadIdx.x;
+      int lo, hi, cnt = 0;
+      if (bb < p.B) {
+        request_rows(p, bb, lo, hi);
+        cnt = (int)(((long long)(hi - lo) * p.G + ROWS - 1) / ROWS);
+      }
+      int sum = cnt;
+#pragma unroll
+      for (int d = 1; d < 32; d <<= 1) {
+        const int u = __shfl_up_sync(0xffffffffu, sum, d);
+        if (lane >= d) sum += u;
+      }
+      if (lane == 31) s_sum[warp] = sum;
+      __syncthreads();
+      int at = before;
+      for (int i = 0; i < THREADS / 32; ++i) {
+        if (i < warp) at += s_sum[i];
+        before += s_sum[i];
+      }
+      at += sum - cnt;
+      if (item >= at && item < at + cnt) {
+        s_req = bb;
+        s_row0 = (item - at) * ROWS;
+      }
+      __syncthreads();
+      if (s_req >= 0) break;
+    }
+    w.work = s_req >= 0;
+    w.b = max(s_req, 0);
+    w.r0 = s_row0;
+    request_rows(p, w.b, w.row_lo, row_hi);
+  }
+  w.n = row_hi - w.row_lo;
+  w.rows = w.n * p.G;  // fits: T * Hq does
+  w.work = w.work && w.r0 < w.rows;
+  w.len = PACKED ? 0 : request_len(p, w.b);
+  w.P = prefix_keys(p);
+  w.np = (w.P + KEYS - 1) / KEYS;
+  const int last = min(w.r0 + ROWS, w.rows) - 1;
+  w.own = PACKED || !w.work ? 0 : max(0, min(w.len, w.len - w.n + last / p.G + 1));
+  const int nt = w.np + (w.own + KEYS - 1) / KEYS, per = (nt + splits - 1) / splits;
+  w.t_lo = min(nt, split * per);
+  w.cnt = w.work ? min(nt, w.t_lo + per) - w.t_lo : 0;
+  return w;
+}
+
 // PACKED: rows of all requests, keys of the prefix.  Otherwise: rows of one
 // request, keys of the prefix and its own.
 template <int HD, bool PACKED>
@@ -590,6 +664,7 @@ many_rows_kernel(const PrefixAttnParams p, const __grid_constant__ PoolMaps maps
   if (threadIdx.x == 0) {
     s_abort = 0;
     s_req = -1;
+    s_row0 = 0;
   }
   if (warp == 1) tmem_alloc_cols(&s_tmem, 512);
   tc_fence_before();
@@ -600,59 +675,10 @@ many_rows_kernel(const PrefixAttnParams p, const __grid_constant__ PoolMaps maps
   volatile int* abort = &s_abort;
   const uint32_t tmem = s_tmem;
 
-  // ---- which rows
-  int b = 0, row_lo, row_hi;
-  int r0;  // first row of tile 0, counted in the request (or in the batch)
-  if (PACKED) {
-    row_lo = 0;
-    row_hi = min(max(p.q_start[p.B], 0), p.T);
-    r0 = item * 2 * TC_M;
-  } else {
-    // item -> request: items of the requests before it
-    int before = 0;
-    for (int b0 = 0; b0 < p.B; b0 += TC_THREADS) {
-      const int bb = b0 + threadIdx.x;
-      int lo, hi, cnt = 0;
-      if (bb < p.B) {
-        request_rows(p, bb, lo, hi);
-        cnt = (int)(((long long)(hi - lo) * p.G + 2 * TC_M - 1) / (2 * TC_M));
-      }
-      int sum = cnt;
-#pragma unroll
-      for (int d = 1; d < 32; d <<= 1) {
-        const int u = __shfl_up_sync(0xffffffffu, sum, d);
-        if (lane >= d) sum += u;
-      }
-      if (lane == 31) s_sum[warp] = sum;
-      __syncthreads();
-      int at = before;
-      for (int w = 0; w < TC_THREADS / 32; ++w) {
-        if (w < warp) at += s_sum[w];
-        before += s_sum[w];
-      }
-      at += sum - cnt;
-      if (item >= at && item < at + cnt) {
-        s_req = bb;
-        s_row0 = (item - at) * 2 * TC_M;
-      }
-      __syncthreads();
-      if (s_req >= 0) break;
-    }
-    b = max(s_req, 0);
-    r0 = s_row0;
-    request_rows(p, b, row_lo, row_hi);
-    if (s_req < 0) row_hi = row_lo;
-  }
-  const int rows = (row_hi - row_lo) * p.G;  // fits: T * Hq does
-  const bool work = r0 < rows && (PACKED || s_req >= 0);
-  const int n = row_hi - row_lo, len = PACKED ? 0 : request_len(p, b), P = prefix_keys(p);
-  const int np = (P + TC_N - 1) / TC_N;
-  const int last = min(r0 + 2 * TC_M, rows) - 1;  // the CTA's last row: sees the most own keys
-  const int own = PACKED || !work ? 0 : max(0, min(len, len - n + last / p.G + 1));
-  const int nt = np + (own + TC_N - 1) / TC_N;
-  const int per = (nt + splits - 1) / splits;
-  const int t_lo = min(nt, split * per), t_hi = min(nt, t_lo + per);
-  const int cnt = work ? t_hi - t_lo : 0;
+  const RowShare w = row_share<PACKED, 2 * TC_M, TC_N, TC_THREADS>(p, item, split, splits, s_req, s_row0, s_sum);
+  const int b = w.b, r0 = w.r0, row_lo = w.row_lo, rows = w.rows, n = w.n, len = w.len, P = w.P, np = w.np, own = w.own;
+  const int t_lo = w.t_lo, cnt = w.cnt;
+  const bool work = w.work;
   const int nx = work && r0 + TC_M < rows ? 2 : 1;  // row tiles in use
   // keys of tile t that exist
   auto keys_of = [&](int t) { return t < np ? P - t * TC_N : own - (t - np) * TC_N; };
@@ -679,6 +705,10 @@ many_rows_kernel(const PrefixAttnParams p, const __grid_constant__ PoolMaps maps
   }
   __syncthreads();
 
+  if (warp < 4)
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(TC_REGS_CTL));
+  else
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(TC_REGS_SM));
   if (warp == 0) {
     // ================================ TMA producer ================================
     const int lg = min(p.lg_page, 7), rpb = 1 << lg;  // rows per copy
@@ -794,17 +824,21 @@ many_rows_kernel(const PrefixAttnParams p, const __grid_constant__ PoolMaps maps
       // ---- Q: this warp's 32 rows, 16 bytes a lane, into the K-major swizzled tile
       constexpr int LPR = HD / 8;  // 16-byte pieces of a row
       const uint32_t qt = q_u + x * C::TILE;
-#pragma unroll 4
-      for (int e = lane; e < 32 * LPR; e += 32) {
-        const int rr = lanes + e / LPR, pc = e % LPR;
-        const int gr = r0 + x * TC_M + rr;
-        uint4 v = make_uint4(0u, 0u, 0u, 0u);
+      uint4 qv[LPR];
+#pragma unroll
+      for (int e = 0; e < LPR; ++e) {
+        const int gr = r0 + x * TC_M + lanes + (e * 32 + lane) / LPR, pc = (e * 32 + lane) % LPR;
+        qv[e] = make_uint4(0u, 0u, 0u, 0u);
         if (gr < rows) {
           const size_t at = ((size_t)(row_lo + gr / p.G) * p.Hq + h * p.G + gr % p.G) * HD + pc * 8;
-          v = *reinterpret_cast<const uint4*>(reinterpret_cast<const __half*>(p.q) + at);
+          qv[e] = *reinterpret_cast<const uint4*>(reinterpret_cast<const __half*>(p.q) + at);
         }
-        asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(qt + (pc >> 3) * (TC_M * 128) + sw128(rr, pc & 7)), "r"(v.x),
-                     "r"(v.y), "r"(v.z), "r"(v.w)
+      }
+#pragma unroll
+      for (int e = 0; e < LPR; ++e) {
+        const int rr = lanes + (e * 32 + lane) / LPR, pc = (e * 32 + lane) % LPR;
+        asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(qt + (pc >> 3) * (TC_M * 128) + sw128(rr, pc & 7)), "r"(qv[e].x),
+                     "r"(qv[e].y), "r"(qv[e].z), "r"(qv[e].w)
                      : "memory");
       }
       fence_async_smem();
@@ -830,17 +864,18 @@ many_rows_kernel(const PrefixAttnParams p, const __grid_constant__ PoolMaps maps
 #pragma unroll
           for (int k = 0; k < TC_N; ++k) v[k] = seen(k) ? v[k] : -INFINITY;
         }
-        float a0 = fmaxf(v[0], v[1]), a1 = fmaxf(v[2], v[3]), a2 = fmaxf(v[4], v[5]), a3 = fmaxf(v[6], v[7]);
+        auto row_max = [&]() {
+          float a0 = fmaxf(v[0], v[1]), a1 = fmaxf(v[2], v[3]), a2 = fmaxf(v[4], v[5]), a3 = fmaxf(v[6], v[7]);
 #pragma unroll
-        for (int k = 8; k < TC_N; k += 8) {
-          a0 = max3(a0, v[k], v[k + 1]);
-          a1 = max3(a1, v[k + 2], v[k + 3]);
-          a2 = max3(a2, v[k + 4], v[k + 5]);
-          a3 = max3(a3, v[k + 6], v[k + 7]);
-        }
-        float mx = fmaxf(fmaxf(a0, a1), fmaxf(a2, a3));
-        mx *= c;
-        if (__any_sync(0xffffffffu, mx > m + TC_RAISE)) {  // also from -inf
+          for (int k = 8; k < TC_N; k += 8) {
+            a0 = max3(a0, v[k], v[k + 1]);
+            a1 = max3(a1, v[k + 2], v[k + 3]);
+            a2 = max3(a2, v[k + 4], v[k + 5]);
+            a3 = max3(a3, v[k + 6], v[k + 7]);
+          }
+          return fmaxf(fmaxf(a0, a1), fmaxf(a2, a3)) * c;
+        };
+        auto raise = [&](float mx) {
           const float mn = fmaxf(m, mx);
           const float f = m == -INFINITY ? 0.f : ex2(m - mn);
           m = mn;
@@ -855,29 +890,49 @@ many_rows_kernel(const PrefixAttnParams p, const __grid_constant__ PoolMaps maps
               tmem_st32(ot + q * 32, u);
             }
           }
-        }
-        const float mm = m == -INFINITY ? 0.f : m;
+        };
+        uint64_t l2[2];
+        uint32_t pw[16];
+        const uint64_t c2 = pack2(c, c);
+        auto quarter = [&](int q) {  // P of 32 keys
+          const float mm = m == -INFINITY ? 0.f : m;
+          const uint64_t m2 = pack2(-mm, -mm);
+#pragma unroll
+          for (int k = 0; k < 32; k += 2) {
+            const uint64_t y = fma2(pack2(v[q * 32 + k], v[q * 32 + k + 1]), c2, m2);
+            float e0, e1;
+            unpack2(y, e0, e1);
+            e0 = ex2(e0);
+            e1 = ex2(e1);
+            l2[(k >> 1) & 1] = add2(l2[(k >> 1) & 1], pack2(e0, e1));
+            pw[k / 2] = h2_as_u32(__floats2half2_rn(e0, e1));
+          }
+        };
+        bool known = __any_sync(0xffffffffu, m == -INFINITY);  // the tile's maximum has been looked at
+        if (known) raise(row_max());
         // The two warps of a scheduler take turns here, or both tiles fall into step: both in the softmax, then both
         // in the tensor cores.
         if (nx == 2 && (x == 1 || i > 0)) {
           ok = __all_sync(0xffffffffu, pa_wait(&turn[x][warp & 3], (x == 1 ? i : i - 1) & 1, abort));
           if (!ok) break;
         }
-        const uint64_t c2 = pack2(c, c), m2 = pack2(-mm, -mm);
-        uint64_t l2[2] = {pack2(0.f, 0.f), pack2(0.f, 0.f)};
+        // The first quarter's P is taken with the maximum so far while the tile's is found, which the MUFU's pace
+        // leaves room for; it seldom has to be taken again.
+        for (;;) {
+          l2[0] = l2[1] = pack2(0.f, 0.f);
+          quarter(0);
+          if (known) break;
+          const float mx = row_max();
+          if (!__any_sync(0xffffffffu, mx > m + TC_RAISE)) break;
+          raise(mx);
+          known = true;
+        }
+        tmem_st16(st, pw);  // over columns of S that have been read
 #pragma unroll
-        for (int q = 0; q < TC_N / 32; ++q) {
-          uint32_t w[16];
-#pragma unroll
-          for (int k = 0; k < 32; k += 2) {
-            float e0, e1;
-            unpack2(fma2(pack2(v[q * 32 + k], v[q * 32 + k + 1]), c2, m2), e0, e1);
-            e0 = ex2(e0);
-            e1 = ex2(e1);
-            l2[(k >> 1) & 1] = add2(l2[(k >> 1) & 1], pack2(e0, e1));
-            w[k / 2] = h2_as_u32(__floats2half2_rn(e0, e1));
-          }
-          tmem_st16(st + q * 16, w);  // over columns of S that have been read
+        for (int q = 1; q < TC_N / 32; ++q) {
+          if (q == TC_HAND && nx == 2 && lane == 0) mbar_arrive(&turn[x ^ 1][warp & 3]);
+          quarter(q);
+          tmem_st16(st + q * 16, pw);
           if (q & 1) {
             tmem_wait_st();
             tc_fence_before();
@@ -885,7 +940,6 @@ many_rows_kernel(const PrefixAttnParams p, const __grid_constant__ PoolMaps maps
             if (lane == 0) mbar_arrive(&p_full[x][q >> 1]);
           }
         }
-        if (nx == 2 && lane == 0) mbar_arrive(&turn[x ^ 1][warp & 3]);
         float l0, l1;
         unpack2(add2(l2[0], l2[1]), l0, l1);
         l += l0 + l1;
@@ -911,10 +965,10 @@ many_rows_kernel(const PrefixAttnParams p, const __grid_constant__ PoolMaps maps
             __half* dst = reinterpret_cast<__half*>(p.out) + row * HD + q * 32;
 #pragma unroll
             for (int k = 0; k < 32; k += 8) {
-              uint32_t w[4];
+              uint32_t ow[4];
 #pragma unroll
-              for (int j = 0; j < 4; ++j) w[j] = h2_as_u32(__floats2half2_rn(v[k + 2 * j] * inv, v[k + 2 * j + 1] * inv));
-              *reinterpret_cast<uint4*>(dst + k) = make_uint4(w[0], w[1], w[2], w[3]);
+              for (int j = 0; j < 4; ++j) ow[j] = h2_as_u32(__floats2half2_rn(v[k + 2 * j] * inv, v[k + 2 * j + 1] * inv));
+              *reinterpret_cast<uint4*>(dst + k) = make_uint4(ow[0], ow[1], ow[2], ow[3]);
             }
           }
         }
@@ -937,6 +991,380 @@ many_rows_kernel(const PrefixAttnParams p, const __grid_constant__ PoolMaps maps
     int ignore = 0;
     tc_commit(&drained[warp - 1]);
     pa_wait(&drained[warp - 1], 0, &ignore);
+  }
+  __syncthreads();
+  if (warp == 1) {
+    tmem_dealloc_cols(tmem, 512);
+    tmem_relinquish();
+  }
+  if (threadIdx.x == 0 && failed) atomicExch(&g_prefix_attn_error, 1);
+}
+
+// ---------------------------------------------------------------- many rows, fp32
+
+// The many-rows kernel for fp32.  Every operand x is carried as two fp16 parts,
+// hi = fp16(x) and lo = fp16(2^11 (x - hi)) -- 2^-22 of x is lost, whatever its
+// size down to 2^-24 -- and each product of two operands is three fp16
+// products in two fp32 accumulators, hi.hi and hi.lo + lo.hi, joined as the
+// first plus 2^-11 of the second.  The parts' range is fp16's: a value beyond
+// 65504 gives NaN.  One tile of 128 rows, tiles of 64 keys:
+//   warp 0       TMA producer: raw fp32 K and V tiles through a ring
+//   warp 1       MMA issuer; S of the next tile goes ahead of O += P V of this one
+//   warps 4-7    softmax, a thread per row (P's own two parts over S's columns)
+//   warps 8-15   split a raw tile into its two fp16 tiles; V's slots behind the
+//                last key, which may hold anything, become zero
+// TMEM: two buffers of S (hi.hi | cross, 64 columns each), O (hi.hi | cross).
+constexpr int TF_N = 64;              // keys of a tile
+constexpr int TF_THREADS = 16 * 32;
+constexpr int TF_CONV = 8;            // warps that split
+
+template <int HD>
+struct ManyRowsF32 {
+  static constexpr int NCH = HD / 64;               // 64-wide fp16 columns
+  static constexpr int QT = TC_M * HD * 2;          // bytes of one part of Q
+  static constexpr int PT = TF_N * HD * 2;          // bytes of one part of a K or V tile
+  static constexpr int RAW = TF_N * HD * 4;         // bytes of a raw tile
+  static constexpr int BOX = FR_KT * HD * 4;        // bytes of one copy: 16 keys
+  static constexpr int NRAW = HD == 128 ? 3 : 6;
+  static constexpr int SMEM = 2 * QT + 4 * PT + NRAW * RAW + 1024;
+};
+
+// two fp32 -> their fp16 parts, packed
+__device__ __forceinline__ void split_f16(float x, float y, uint32_t& hi, uint32_t& lo) {
+  const __half2 h = __floats2half2_rn(x, y);
+  const float2 f = __half22float2(h);
+  hi = h2_as_u32(h);
+  lo = h2_as_u32(__floats2half2_rn((x - f.x) * 2048.f, (y - f.y) * 2048.f));
+}
+
+template <int HD, bool PACKED>
+__global__ void __launch_bounds__(TF_THREADS, 1)
+many_rows_f32_kernel(const PrefixAttnParams p, const __grid_constant__ PoolMaps maps, int splits, int slot0) {
+  using C = ManyRowsF32<HD>;
+  constexpr int NRAW = C::NRAW, NCH = C::NCH;
+  extern __shared__ __align__(1024) unsigned char mf_smem[];
+  __shared__ __align__(8) uint64_t raw_full[NRAW], raw_empty[NRAW], q_full, k_full, v_full, s_full[2], p_full, pv_done, drained;
+  __shared__ uint32_t s_tmem, s_absent[16];
+  __shared__ int s_abort, s_req, s_row0, s_sum[TF_THREADS / 32];
+  unsigned char* base = mf_smem + ((1024 - (smem_u32(mf_smem) & 1023)) & 1023);
+  const uint32_t q_u = smem_u32(base), k_u = q_u + 2 * C::QT, v_u = k_u + 2 * C::PT, raw_u = v_u + 2 * C::PT;
+  const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
+  const int split = blockIdx.x % splits, item = blockIdx.x / splits, h = blockIdx.y;
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < NRAW; ++i) {
+      mbar_init(&raw_full[i], 1);
+      mbar_init(&raw_empty[i], TF_CONV);
+    }
+    mbar_init(&q_full, 4);
+    mbar_init(&k_full, TF_CONV);
+    mbar_init(&v_full, TF_CONV);
+    mbar_init(&s_full[0], 1);
+    mbar_init(&s_full[1], 1);
+    mbar_init(&p_full, 4);
+    mbar_init(&pv_done, 1);
+    mbar_init(&drained, 1);
+    s_abort = 0;
+    s_req = -1;
+    s_row0 = 0;
+    fence_mbar_init();
+  }
+  if (warp == 1) tmem_alloc_cols(&s_tmem, 512);
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  pdl_wait();
+  pdl_trigger();  // after the wait: few_rows_kernel relies on it
+  volatile int* abort = &s_abort;
+  const uint32_t tmem = s_tmem;  // S: buffer j at 128 j, its cross part 64 further; O at 256, its cross part HD further
+  const RowShare w = row_share<PACKED, TC_M, TF_N, TF_THREADS>(p, item, split, splits, s_req, s_row0, s_sum);
+  const int np = w.np, cnt = w.cnt;
+  auto keys_of = [&](int t) { return t < np ? w.P - t * TF_N : w.own - (t - np) * TF_N; };
+  // K tiles run one ahead of V tiles through the ring: K0 K1 V0 K2 V1 ...; the place of tile i's K and V
+  auto k_at = [&](int i) { return (uint32_t)(i == 0 ? 0 : 2 * i - 1); };
+  auto v_at = [&](int i) { return (uint32_t)(i + 1 < cnt ? 2 * i + 2 : 2 * i + 1); };
+
+  if (warp == 0) {
+    // ================================ TMA producer ================================
+    int row[2] = {-1, -1};  // pool rows of the tile whose K goes next and of the one before, one per copy
+    auto rows_of = [&](int i) {
+      const int t = w.t_lo + i;
+      int at = -1;
+      if (lane < TF_N / FR_KT && lane * FR_KT < keys_of(t)) {
+        const int key = (t < np ? t : t - np) * TF_N + lane * FR_KT, blk = key >> p.lg_page;
+        const int id = t < np ? p.prefix_table[blk] : p.block_table[(size_t)w.b * p.max_blocks + blk];
+        if (id >= 0 && id < p.n_pages) at = ((id * p.Hkv + h) << p.lg_page) + (key & ((1 << p.lg_page) - 1));
+      }
+      const uint32_t gone = __ballot_sync(0xffffffffu, at < 0) & ((1u << (TF_N / FR_KT)) - 1);
+      if (lane == 0) s_absent[i & 15] = gone;  // a bit per 16 keys
+      return at;
+    };
+    auto copy = [&](const CUtensorMap* map, int at, uint32_t it) {
+      const int s = it % NRAW;
+      if (!__all_sync(0xffffffffu, pa_wait(&raw_empty[s], ((it / NRAW) & 1u) ^ 1u, abort))) return false;
+      if (lane == 0) mbar_arrive_expect_tx(&raw_full[s], C::RAW);
+      __syncwarp();
+      if (lane < TF_N / FR_KT) tma3d_at(raw_u + s * C::RAW + lane * C::BOX, map, at < 0 ? p.pool_rows : at, 0, &raw_full[s]);
+      return true;
+    };
+    uint32_t it = 0;
+    bool ok = true;
+    for (int i = 0; i <= cnt && ok && cnt; ++i) {  // K of tile i, then V of tile i - 1
+      if (i < cnt) {
+        row[i & 1] = rows_of(i);
+        if ((ok = copy(&maps.k, i & 1 ? row[1] : row[0], it))) ++it;
+      }
+      if (i > 0 && ok && (ok = copy(&maps.v, i & 1 ? row[0] : row[1], it))) ++it;
+    }
+    if (lane == 0) {  // copies in flight land before the CTA may exit
+      int ignore = 0;
+      for (uint32_t k = it > NRAW ? it - NRAW : 0; k < it; ++k) pa_wait(&raw_full[k % NRAW], (k / NRAW) & 1u, &ignore);
+    }
+  } else if (warp == 1) {
+    // ================================ MMA issuer ================================
+    if (lane == 0 && cnt > 0) {
+      constexpr uint32_t idesc_s = (1u << 4) | ((TF_N >> 3) << 17) | ((TC_M >> 4) << 24);
+      constexpr uint32_t idesc_o = (1u << 4) | (1u << 16) | ((HD >> 3) << 17) | ((TC_M >> 4) << 24);
+      const uint64_t qh = umma_desc_sw128(q_u), ql = umma_desc_sw128(q_u + C::QT);
+      const uint64_t kh = umma_desc_sw128(k_u), kl = umma_desc_sw128(k_u + C::PT);
+      const uint64_t vh = umma_desc_sw128_mn(v_u, TF_N * 128), vl = umma_desc_sw128_mn(v_u + C::PT, TF_N * 128);
+      const uint32_t to = tmem + 256;
+      auto issue_s = [&](int i) {
+        const uint32_t ts = tmem + (i & 1) * 128;
+#pragma unroll
+        for (int kk = 0; kk < HD / 16; ++kk) {
+          const uint32_t qo = ((kk >> 2) * (TC_M * 128) + (kk & 3) * 32) >> 4, ko = ((kk >> 2) * (TF_N * 128) + (kk & 3) * 32) >> 4;
+          umma_f16(ts + 64, ql + qo, kh + ko, idesc_s, kk != 0);
+          umma_f16(ts + 64, qh + qo, kl + ko, idesc_s, 1u);
+          umma_f16(ts, qh + qo, kh + ko, idesc_s, kk != 0);
+        }
+        tc_commit(&s_full[i & 1]);
+      };
+      bool ok = pa_spin(&q_full, 0, abort) && pa_spin(&k_full, 0, abort);
+      if (ok) {
+        tc_fence_after();
+        issue_s(0);
+      }
+      for (int i = 0; i < cnt && ok; ++i) {
+        if (i + 1 < cnt) {  // its buffer held P of tile i - 1, whose product comes before this one
+          if (!(ok = pa_spin(&k_full, (i + 1) & 1, abort))) break;
+          tc_fence_after();
+          issue_s(i + 1);
+        }
+        ok = pa_spin(&v_full, i & 1, abort) && pa_spin(&p_full, i & 1, abort);
+        if (!ok) break;
+        tc_fence_after();
+        const uint32_t ph = tmem + (i & 1) * 128, pl = ph + 64;
+#pragma unroll
+        for (int kk = 0; kk < TF_N / 16; ++kk) {
+          umma_f16_ta(to + HD, pl + kk * 8, vh + kk * (2048 >> 4), idesc_o, (i | kk) != 0);
+          umma_f16_ta(to + HD, ph + kk * 8, vl + kk * (2048 >> 4), idesc_o, 1u);
+          umma_f16_ta(to, ph + kk * 8, vh + kk * (2048 >> 4), idesc_o, (i | kk) != 0);
+        }
+        tc_commit(&pv_done);
+      }
+    }
+  } else if (warp >= 8) {
+    // ================================ split K and V ================================
+    constexpr int LPK = HD / 8, KPW = 32 / LPK;  // lanes per key (8 values each), keys per warp and step
+    const int g = lane % LPK, sub = lane / LPK;
+    auto convert = [&](uint32_t it, uint32_t dst, int keys) {  // slots from `keys` on become zero
+      const int s = it % NRAW;
+      if (!__all_sync(0xffffffffu, pa_wait(&raw_full[s], (it / NRAW) & 1u, abort))) return false;
+      const uint32_t src = raw_u + s * C::RAW;
+#pragma unroll 4
+      for (int k0 = 0; k0 < TF_N; k0 += TF_CONV * KPW) {
+        const int key = k0 + (warp - 8) * KPW + sub, r = key % FR_KT;
+        // 8 values: pieces 2 (g % 4) and 2 (g % 4) + 1 of 128-byte chunk g / 4; odd chunks in the other order, so that
+        // eight lanes read eight banks' worth
+        const uint32_t at = src + (key / FR_KT) * C::BOX + (g >> 2) * (FR_KT * 128) + r * 128;
+        const int p0 = 2 * (g & 3) + ((g >> 2) & 1);
+        float4 a = lds_f4(at + ((p0 ^ (r & 7)) << 4)), b = lds_f4(at + (((p0 ^ 1) ^ (r & 7)) << 4));
+        if ((g >> 2) & 1) {
+          const float4 x = a;
+          a = b;
+          b = x;
+        }
+        if (key >= keys) a = b = make_float4(0.f, 0.f, 0.f, 0.f);
+        uint32_t hi[4], lo[4];
+        split_f16(a.x, a.y, hi[0], lo[0]);
+        split_f16(a.z, a.w, hi[1], lo[1]);
+        split_f16(b.x, b.y, hi[2], lo[2]);
+        split_f16(b.z, b.w, hi[3], lo[3]);
+        const uint32_t d = dst + (g >> 3) * (TF_N * 128) + sw128(key, g & 7);
+        asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(d), "r"(hi[0]), "r"(hi[1]), "r"(hi[2]), "r"(hi[3]) : "memory");
+        asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(d + C::PT), "r"(lo[0]), "r"(lo[1]), "r"(lo[2]), "r"(lo[3]) : "memory");
+      }
+      fence_async_smem();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&raw_empty[s]);
+      return true;
+    };
+    bool ok = true;
+    for (int i = 0; i <= cnt && ok && cnt; ++i) {
+      if (i < cnt) {  // K of tile i, once S of tile i - 1 is done with the buffer
+        if (i > 0) ok = __all_sync(0xffffffffu, pa_wait(&s_full[(i - 1) & 1], ((i - 1) >> 1) & 1, abort));
+        ok = ok && convert(k_at(i), k_u, TF_N);
+        if (ok && lane == 0) mbar_arrive(&k_full);
+      }
+      if (i > 0 && ok) {  // V of tile i - 1, once the product of tile i - 2 is
+        if (i > 1) ok = __all_sync(0xffffffffu, pa_wait(&pv_done, (i - 2) & 1, abort));
+        ok = ok && convert(v_at(i - 1), v_u, keys_of(w.t_lo + i - 1));
+        if (ok && lane == 0) mbar_arrive(&v_full);
+      }
+    }
+  } else if (warp >= 4) {
+    // ================================ softmax ================================
+    const int lanes = (warp & 3) * 32;
+    const int r = w.r0 + lanes + lane;  // this thread's row
+    const uint32_t tl = tmem + ((uint32_t)lanes << 16), ot = tl + 256;
+    const bool valid = w.work && r < w.rows;
+    const int see = PACKED ? 0 : (valid ? max(0, min(w.len, w.len - w.n + r / p.G + 1)) : w.own);
+    const float c = p.c;
+    float m = -INFINITY, l = 0.f;
+    const size_t row = valid ? (size_t)(w.row_lo + r / p.G) * p.Hq + h * p.G + r % p.G : 0;
+    const size_t at = (size_t)(slot0 + split) * p.T * p.Hq + row;
+    if (cnt > 0) {
+      // ---- Q's parts: this warp's 32 rows, 8 values a lane
+      constexpr int LPR = HD / 8;
+#pragma unroll
+      for (int e0 = 0; e0 < LPR; e0 += 4) {
+        float4 x[4][2];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const int rr = lanes + ((e0 + j) * 32 + lane) / LPR, pc = ((e0 + j) * 32 + lane) % LPR, gr = w.r0 + rr;
+          x[j][0] = x[j][1] = make_float4(0.f, 0.f, 0.f, 0.f);
+          if (gr < w.rows) {
+            const float4* src = reinterpret_cast<const float4*>(reinterpret_cast<const float*>(p.q) +
+                                                                ((size_t)(w.row_lo + gr / p.G) * p.Hq + h * p.G + gr % p.G) * HD + pc * 8);
+            x[j][0] = src[0];
+            x[j][1] = src[1];
+          }
+        }
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const int rr = lanes + ((e0 + j) * 32 + lane) / LPR, pc = ((e0 + j) * 32 + lane) % LPR;
+          uint32_t hi[4], lo[4];
+          split_f16(x[j][0].x, x[j][0].y, hi[0], lo[0]);
+          split_f16(x[j][0].z, x[j][0].w, hi[1], lo[1]);
+          split_f16(x[j][1].x, x[j][1].y, hi[2], lo[2]);
+          split_f16(x[j][1].z, x[j][1].w, hi[3], lo[3]);
+          const uint32_t d = q_u + (pc >> 3) * (TC_M * 128) + sw128(rr, pc & 7);
+          asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(d), "r"(hi[0]), "r"(hi[1]), "r"(hi[2]), "r"(hi[3]) : "memory");
+          asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(d + C::QT), "r"(lo[0]), "r"(lo[1]), "r"(lo[2]), "r"(lo[3]) : "memory");
+        }
+      }
+      fence_async_smem();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&q_full);
+
+      bool ok = true;
+      for (int i = 0; i < cnt; ++i) {
+        ok = __all_sync(0xffffffffu, pa_wait(&s_full[i & 1], (i >> 1) & 1, abort));
+        if (!ok) break;
+        tc_fence_after();
+        const uint32_t st = tl + (i & 1) * 128;
+        const int t = w.t_lo + i;
+        const uint32_t gone = s_absent[i & 15];
+        const int lim = (t < np ? w.P : see) - (t < np ? t : t - np) * TF_N;  // keys of the tile this row sees
+        float v[TF_N];
+#pragma unroll
+        for (int q = 0; q < TF_N; q += 32) {
+          float x[32];
+          tmem_ld32_async(st + q, v + q);
+          tmem_ld32_async(st + 64 + q, x);
+          tmem_wait_ld();
+          tmem_ready(v + q);
+          tmem_ready(x);
+#pragma unroll
+          for (int k = 0; k < 32; ++k) v[q + k] = fmaf(x[k], 1.f / 2048.f, v[q + k]);
+        }
+        if (__any_sync(0xffffffffu, lim < TF_N) || gone != 0) {
+#pragma unroll
+          for (int k = 0; k < TF_N; ++k) v[k] = k < lim && !((gone >> (k / 16)) & 1u) ? v[k] : -INFINITY;
+        }
+        float a0 = fmaxf(v[0], v[1]), a1 = fmaxf(v[2], v[3]);
+#pragma unroll
+        for (int k = 4; k < TF_N; k += 4) {
+          a0 = max3(a0, v[k], v[k + 1]);
+          a1 = max3(a1, v[k + 2], v[k + 3]);
+        }
+        const float mx = fmaxf(a0, a1) * c;
+        if (__any_sync(0xffffffffu, mx > m + TC_RAISE)) {  // also from -inf
+          const float mn = fmaxf(m, mx);
+          const float f = m == -INFINITY ? 0.f : ex2(m - mn);
+          m = mn;
+          l *= f;
+          if (i > 0) {
+            ok = __all_sync(0xffffffffu, pa_wait(&pv_done, (i - 1) & 1, abort));
+            if (!ok) break;
+            tc_fence_after();
+#pragma unroll
+            for (int q = 0; q < 2 * HD; q += 32) {
+              float u[32];
+              tmem_ld32(ot + q, u);
+#pragma unroll
+              for (int k = 0; k < 32; ++k) u[k] *= f;
+              tmem_st32(ot + q, u);
+            }
+          }
+        }
+        const float mm = m == -INFINITY ? 0.f : m;
+        float l0 = 0.f, l1 = 0.f;
+#pragma unroll
+        for (int q = 0; q < TF_N; q += 32) {
+          uint32_t hi[16], lo[16];
+#pragma unroll
+          for (int k = 0; k < 32; k += 2) {
+            const float e0 = ex2(fmaf(v[q + k], c, -mm)), e1 = ex2(fmaf(v[q + k + 1], c, -mm));
+            l0 += e0;
+            l1 += e1;
+            split_f16(e0, e1, hi[k / 2], lo[k / 2]);
+          }
+          tmem_st16(st + q / 2, hi);  // over S, which has been read
+          tmem_st16(st + 64 + q / 2, lo);
+        }
+        l += l0 + l1;
+        tmem_wait_st();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&p_full);
+      }
+      ok = ok && __all_sync(0xffffffffu, pa_wait(&pv_done, (cnt - 1) & 1, abort));
+      tc_fence_after();
+      if (ok) {
+        const float inv = l == 0.f ? 0.f : 1.f / l;
+        if (valid && p.nslots > 1) p.part_ml[at] = make_float2(m, l);
+        float* dst = p.nslots > 1 ? p.part_o + at * HD : reinterpret_cast<float*>(p.out) + row * HD;
+        const float f = p.nslots > 1 ? 1.f : inv;
+#pragma unroll
+        for (int q = 0; q < HD; q += 32) {
+          float v[32], x[32];
+          tmem_ld32(ot + q, v);
+          tmem_ld32(ot + HD + q, x);
+          if (!valid) continue;
+#pragma unroll
+          for (int k = 0; k < 32; ++k) v[k] = fmaf(x[k], 1.f / 2048.f, v[k]) * f;
+#pragma unroll
+          for (int k = 0; k < 32; k += 4) *reinterpret_cast<float4*>(dst + q + k) = make_float4(v[k], v[k + 1], v[k + 2], v[k + 3]);
+        }
+      }
+    } else if (valid) {  // no keys in this share
+      if (p.nslots > 1) {
+        p.part_ml[at] = make_float2(-INFINITY, 0.f);
+      } else {
+        for (int d = 0; d < HD; d += 4)
+          *reinterpret_cast<float4*>(reinterpret_cast<float*>(p.out) + row * HD + d) = make_float4(0.f, 0.f, 0.f, 0.f);
+      }
+    }
+  }
+  // after a wait that ran out: the products in flight have ended before the TMEM is freed
+  tc_fence_before();
+  const bool failed = __syncthreads_or(*abort);
+  tc_fence_after();
+  if (failed && threadIdx.x == 32) {
+    int ignore = 0;
+    tc_commit(&drained);
+    pa_wait(&drained, 0, &ignore);
   }
   __syncthreads();
   if (warp == 1) {
@@ -1021,25 +1449,26 @@ static bool pool_map(CUtensorMap* m, const void* pool, size_t rows, int hd, bool
 // How a call is cut.  The host knows the rows T and the requests B, not which request has how many, nor how many
 // keys there are, only how many the tables hold.
 //   few rows      few_rows_kernel over the prefix and the requests' own keys
-//   shared        many_rows_kernel<PACKED> over the prefix (fp16), few_rows_kernel over the own keys
-//   chunks        many_rows_kernel over both (fp16)
+//   shared        a many-rows kernel, PACKED, over the prefix, few_rows_kernel over the own keys
+//   chunks        a many-rows kernel over both
 struct AttnPlan {
   enum Kind { FEW, SHARED, CHUNKS } kind;
   int splits, row_groups;       // few_rows_kernel
-  int tc_splits, tc_items;      // many_rows_kernel
+  int tc_splits, tc_items;      // many_rows_kernel, many_rows_f32_kernel
   int nslots;
 };
 
 static AttnPlan plan_attn(int T, int B, int Hkv, int G, bool f16, long long own_keys, long long prefix_keys, int sms) {
   AttnPlan a{};
-  const long long rows = (long long)T * G, pairs = (rows + 2 * TC_M - 1) / (2 * TC_M);
+  const int per_cta = f16 ? 2 * TC_M : TC_M;  // rows
+  const long long rows = (long long)T * G, items = (rows + per_cta - 1) / per_cta;
   const auto ceil_div = [](long long x, long long y) { return (x + y - 1) / y; };
-  a.kind = !f16 ? AttnPlan::FEW : rows >= 64ll * B ? AttnPlan::CHUNKS : prefix_keys > 0 && B > 1 ? AttnPlan::SHARED : AttnPlan::FEW;
+  a.kind = rows >= 64ll * B ? AttnPlan::CHUNKS : prefix_keys > 0 && B > 1 ? AttnPlan::SHARED : AttnPlan::FEW;
   if (a.kind != AttnPlan::FEW) {
-    // one CTA per SM holds two row tiles; shares of the keys until there is one CTA for every SM
+    // shares of the keys until there is a CTA for every SM
     const long long keys = prefix_keys + (a.kind == AttnPlan::CHUNKS ? own_keys : 0);
-    a.tc_items = (int)(a.kind == AttnPlan::CHUNKS ? pairs + B : pairs);
-    a.tc_splits = (int)std::max(1ll, std::min({(long long)sms / (pairs * Hkv), ceil_div(keys, TC_N), 32ll}));
+    a.tc_items = (int)(a.kind == AttnPlan::CHUNKS ? items + B : items);
+    a.tc_splits = (int)std::max(1ll, std::min({(long long)sms / (items * Hkv), ceil_div(keys, f16 ? TC_N : TF_N), 32ll}));
     a.nslots = a.tc_splits;
   }
   if (a.kind != AttnPlan::CHUNKS) {
@@ -1055,12 +1484,12 @@ static AttnPlan plan_attn(int T, int B, int Hkv, int G, bool f16, long long own_
   return a;
 }
 
-template <int HD, bool PACKED>
-static int run_many_rows(const PrefixAttnParams& p, const PoolMaps& maps, const AttnPlan& a, cudaStream_t stream) {
-  auto kern = many_rows_kernel<HD, PACKED>;
-  const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, ManyRows<HD>::SMEM);
+template <typename K>
+static int run_many_rows(K kern, int smem, int threads, const PrefixAttnParams& p, const PoolMaps& maps, const AttnPlan& a,
+                         cudaStream_t stream) {
+  const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
   if (e != cudaSuccess) return check_launch("prefix_attn", e);
-  launch(kern, dim3((unsigned)(a.tc_splits * a.tc_items), p.Hkv), dim3(TC_THREADS), ManyRows<HD>::SMEM, stream, p, maps, a.tc_splits, 0);
+  launch(kern, dim3((unsigned)(a.tc_splits * a.tc_items), p.Hkv), dim3(threads), smem, stream, p, maps, a.tc_splits, 0);
   return check_launch("prefix_attn_many_rows");
 }
 
@@ -1068,15 +1497,18 @@ template <typename T, int HD>
 static int run_attn(const PrefixAttnParams& p, const void* k, const void* v, const AttnPlan& a, cudaStream_t stream) {
   using C = FewRows<T, HD>;
   int st = SC_OK;
-  if constexpr (C::F16) {
-    if (a.kind != AttnPlan::FEW) {
-      PoolMaps maps;
-      const int box = std::min(TC_N, 1 << p.lg_page);
-      SC_REQUIRE(pool_map(&maps.k, k, p.pool_rows, HD, true, box, 1) && pool_map(&maps.v, v, p.pool_rows, HD, true, box, 1),
-                 SC_ERR_CUDA, "prefix_attn: tensor map of the pages refused");
-      st = a.kind == AttnPlan::SHARED ? run_many_rows<HD, true>(p, maps, a, stream) : run_many_rows<HD, false>(p, maps, a, stream);
-      if (st != SC_OK) return st;
-    }
+  if (a.kind != AttnPlan::FEW) {
+    PoolMaps maps;
+    const int box = C::F16 ? std::min(TC_N, 1 << p.lg_page) : FR_KT, chunks = C::F16 ? 1 : C::NB;
+    SC_REQUIRE(pool_map(&maps.k, k, p.pool_rows, HD, C::F16, box, chunks) && pool_map(&maps.v, v, p.pool_rows, HD, C::F16, box, chunks),
+               SC_ERR_CUDA, "prefix_attn: tensor map of the pages refused");
+    const bool packed = a.kind == AttnPlan::SHARED;
+    if constexpr (C::F16)
+      st = run_many_rows(packed ? many_rows_kernel<HD, true> : many_rows_kernel<HD, false>, ManyRows<HD>::SMEM, TC_THREADS, p, maps, a, stream);
+    else
+      st = run_many_rows(packed ? many_rows_f32_kernel<HD, true> : many_rows_f32_kernel<HD, false>, ManyRowsF32<HD>::SMEM, TF_THREADS, p,
+                         maps, a, stream);
+    if (st != SC_OK) return st;
   }
   if (a.kind != AttnPlan::CHUNKS) {
     PoolMaps maps;
