@@ -1043,7 +1043,7 @@ many_rows_f32_kernel(const PrefixAttnParams p, const __grid_constant__ PoolMaps 
   using C = ManyRowsF32<HD>;
   constexpr int NRAW = C::NRAW, NCH = C::NCH;
   extern __shared__ __align__(1024) unsigned char mf_smem[];
-  __shared__ __align__(8) uint64_t raw_full[NRAW], raw_empty[NRAW], q_full, k_full, v_full, s_full[2], p_full, pv_done, drained;
+  __shared__ __align__(8) uint64_t raw_full[NRAW], raw_empty[NRAW], q_full, k_full, v_full, s_full[2], p_full, pv_done, o_full, drained;
   __shared__ uint32_t s_tmem, s_absent[16];
   __shared__ int s_abort, s_req, s_row0, s_sum[TF_THREADS / 32];
   unsigned char* base = mf_smem + ((1024 - (smem_u32(mf_smem) & 1023)) & 1023);
@@ -1062,6 +1062,7 @@ many_rows_f32_kernel(const PrefixAttnParams p, const __grid_constant__ PoolMaps 
     mbar_init(&s_full[1], 1);
     mbar_init(&p_full, 4);
     mbar_init(&pv_done, 1);
+    mbar_init(&o_full, 1);
     mbar_init(&drained, 1);
     s_abort = 0;
     s_req = -1;
@@ -1161,6 +1162,7 @@ many_rows_f32_kernel(const PrefixAttnParams p, const __grid_constant__ PoolMaps 
           umma_f16_ta(to, ph + kk * 8, vh + kk * (2048 >> 4), idesc_o, (i | kk) != 0);
         }
         tc_commit(&pv_done);
+        if (i + 1 == cnt) tc_commit(&o_full);
       }
     }
   } else if (warp >= 8) {
@@ -1294,7 +1296,7 @@ many_rows_f32_kernel(const PrefixAttnParams p, const __grid_constant__ PoolMaps 
           const float f = m == -INFINITY ? 0.f : ex2(m - mn);
           m = mn;
           l *= f;
-          if (i > 0) {
+          if (i > 0) {  // the last product into O; the one before it precedes this tile's S
             ok = __all_sync(0xffffffffu, pa_wait(&pv_done, (i - 1) & 1, abort));
             if (!ok) break;
             tc_fence_after();
@@ -1329,7 +1331,7 @@ many_rows_f32_kernel(const PrefixAttnParams p, const __grid_constant__ PoolMaps 
         __syncwarp();
         if (lane == 0) mbar_arrive(&p_full);
       }
-      ok = ok && __all_sync(0xffffffffu, pa_wait(&pv_done, (cnt - 1) & 1, abort));
+      ok = ok && __all_sync(0xffffffffu, pa_wait(&o_full, 0, abort));
       tc_fence_after();
       if (ok) {
         const float inv = l == 0.f ? 0.f : 1.f / l;

@@ -306,6 +306,20 @@ def test_attn_lengths(cuda, rng, dtype, B, prefix, longest):
 
 
 @pytest.mark.parametrize("dtype", ["f16", "f32"])
+@pytest.mark.parametrize("hq,hkv,hd", [(32, 4, 64), (64, 8, 128)])
+@pytest.mark.parametrize("prefix,longest", [(1000, 60), (2900, 5)])
+def test_attn_many_rows_many_tiles(cuda, rng, dtype, hq, hkv, hd, prefix, longest):
+    """Several tiles of rows, each with several tiles of keys in one CTA, over and over: what one run leaves unordered
+    shows in another."""
+    new = [int(x) for x in rng.integers(1, 6, 16)]
+    lens = [n + int(rng.integers(0, longest)) for n in new]
+    d = make_attn(cuda, rng, dtype, hq, hkv, hd, 32, prefix, lens, new)
+    out = check_attn(cuda, dtype, d, hq)
+    for _ in range(8):
+        assert torch.equal(out, run_attn(cuda, d))
+
+
+@pytest.mark.parametrize("dtype", ["f16", "f32"])
 @pytest.mark.parametrize("new", [[1, 1, 1], [9, 40, 150]])
 def test_attn_no_prefix_and_scale(cuda, rng, dtype, new):
     d = make_attn(cuda, rng, dtype, 8, 2, 64, 16, 0, [30, 200, 151], new)
