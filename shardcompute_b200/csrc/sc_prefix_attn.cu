@@ -1043,7 +1043,7 @@ many_rows_f32_kernel(const PrefixAttnParams p, const __grid_constant__ PoolMaps 
   using C = ManyRowsF32<HD>;
   constexpr int NRAW = C::NRAW, NCH = C::NCH;
   extern __shared__ __align__(1024) unsigned char mf_smem[];
-  __shared__ __align__(8) uint64_t raw_full[NRAW], raw_empty[NRAW], q_full, k_full, v_full, s_full[2], p_full, pv_done, o_full, drained;
+  __shared__ __align__(8) uint64_t raw_full[NRAW], raw_empty[NRAW], q_full, k_full, v_full, s_full[2], p_full[2], pv_done, o_full, drained;
   __shared__ uint32_t s_tmem, s_absent[16];
   __shared__ int s_abort, s_req, s_row0, s_sum[TF_THREADS / 32];
   unsigned char* base = mf_smem + ((1024 - (smem_u32(mf_smem) & 1023)) & 1023);
@@ -1060,7 +1060,8 @@ many_rows_f32_kernel(const PrefixAttnParams p, const __grid_constant__ PoolMaps 
     mbar_init(&v_full, TF_CONV);
     mbar_init(&s_full[0], 1);
     mbar_init(&s_full[1], 1);
-    mbar_init(&p_full, 4);
+    mbar_init(&p_full[0], 4);  // by buffer of S: P of the next tile may be there before this one's is taken
+    mbar_init(&p_full[1], 4);
     mbar_init(&pv_done, 1);
     mbar_init(&o_full, 1);
     mbar_init(&drained, 1);
@@ -1151,7 +1152,7 @@ many_rows_f32_kernel(const PrefixAttnParams p, const __grid_constant__ PoolMaps 
           tc_fence_after();
           issue_s(i + 1);
         }
-        ok = pa_spin(&v_full, i & 1, abort) && pa_spin(&p_full, i & 1, abort);
+        ok = pa_spin(&v_full, i & 1, abort) && pa_spin(&p_full[i & 1], (i >> 1) & 1, abort);
         if (!ok) break;
         tc_fence_after();
         const uint32_t ph = tmem + (i & 1) * 128, pl = ph + 64;
@@ -1329,7 +1330,7 @@ many_rows_f32_kernel(const PrefixAttnParams p, const __grid_constant__ PoolMaps 
         tmem_wait_st();
         tc_fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive(&p_full);
+        if (lane == 0) mbar_arrive(&p_full[i & 1]);
       }
       ok = ok && __all_sync(0xffffffffu, pa_wait(&o_full, 0, abort));
       tc_fence_after();
