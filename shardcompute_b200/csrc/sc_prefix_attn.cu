@@ -141,8 +141,8 @@ few_rows_kernel(const PrefixAttnParams p, const __grid_constant__ PoolMaps maps,
   __syncthreads();
   pdl_trigger();
   // Without the prefix this kernel follows many_rows_kernel, whose CTAs all are past their own wait by the time
-  // this one starts: what both read is there, and they run side by side.  It waits for that kernel before it ends,
-  // so that the join, which waits for this one, has both results.
+  // this one starts: what both read is there, and they run side by side.  One CTA, the last to be placed, waits for
+  // that kernel before it ends, so that the join, which waits for this one, has both results.
   if (with_prefix) pdl_wait();
   int row_lo, row_hi;
   request_rows(p, b, row_lo, row_hi);
@@ -458,7 +458,7 @@ few_rows_kernel(const PrefixAttnParams p, const __grid_constant__ PoolMaps maps,
       mbar_wait_bounded(&full[warp][used % NST], (used / NST) & 1u, &ignore, PA_WAIT_NS);
     }
   if (threadIdx.x == 0 && s_abort) atomicExch(&g_prefix_attn_error, 1);
-  if (!with_prefix) pdl_wait();
+  if (!with_prefix && blockIdx.x == gridDim.x - 1 && blockIdx.y == gridDim.y - 1 && blockIdx.z == gridDim.z - 1) pdl_wait();
 }
 
 // ---------------------------------------------------------------- many rows, fp16
@@ -1041,7 +1041,7 @@ template <int HD, bool PACKED>
 __global__ void __launch_bounds__(TF_THREADS, 1)
 many_rows_f32_kernel(const PrefixAttnParams p, const __grid_constant__ PoolMaps maps, int splits, int slot0) {
   using C = ManyRowsF32<HD>;
-  constexpr int NRAW = C::NRAW, NCH = C::NCH;
+  constexpr int NRAW = C::NRAW;
   extern __shared__ __align__(1024) unsigned char mf_smem[];
   __shared__ __align__(8) uint64_t raw_full[NRAW], raw_empty[NRAW], q_full, k_full, v_full, s_full[2], p_full[2], pv_done, o_full, drained;
   __shared__ uint32_t s_tmem, s_absent[16];
@@ -1471,7 +1471,7 @@ static AttnPlan plan_attn(int T, int B, int Hkv, int G, bool f16, long long own_
     // shares of the keys until there is a CTA for every SM
     const long long keys = prefix_keys + (a.kind == AttnPlan::CHUNKS ? own_keys : 0);
     a.tc_items = (int)(a.kind == AttnPlan::CHUNKS ? items + B : items);
-    a.tc_splits = (int)std::max(1ll, std::min({(long long)sms / (items * Hkv), ceil_div(keys, f16 ? TC_N : TF_N), 32ll}));
+    a.tc_splits = (int)std::max(1ll, std::min({(long long)sms * 4 / 5 / (items * Hkv), ceil_div(keys, f16 ? TC_N : TF_N), 32ll}));
     a.nslots = a.tc_splits;
   }
   if (a.kind != AttnPlan::CHUNKS) {
