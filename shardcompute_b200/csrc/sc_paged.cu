@@ -12,7 +12,8 @@
 
 namespace sc {
 
-constexpr int PG_THREADS = 512;
+constexpr int PG_THREADS = 1024;
+constexpr int PG_BATCH = 4;  // rows or pages a thread has under way
 constexpr int PG_MAX_BATCH = 16384;  // a request's scan state is 12 bytes of shared memory: 192 KB
 
 __device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
@@ -137,21 +138,39 @@ __global__ void __launch_bounds__(PG_THREADS) paged_reserve_kernel(const Reserve
   cluster_arrive();
   const int nthr = (int)cluster_size() * PG_THREADS, tid = (int)cluster_rank() * PG_THREADS + threadIdx.x;
   if (st == 0) {
-    for (int n = tid; n < (int)take0; n += nthr) {
-      const int b = first_above(s_take, p.B, n);
-      const int j = (s_len[b] + p.page - 1) / p.page + n - (b ? s_take[b - 1] : 0);
-      p.block_table[(size_t)b * p.max_blocks + j] = p.free_pages[count - 1 - n];
+    for (int n0 = tid; n0 < (int)take0; n0 += PG_BATCH * nthr) {
+      int id[PG_BATCH];
+#pragma unroll
+      for (int i = 0; i < PG_BATCH; ++i) id[i] = n0 + i * nthr < (int)take0 ? p.free_pages[count - 1 - (n0 + i * nthr)] : 0;
+#pragma unroll
+      for (int i = 0; i < PG_BATCH; ++i) {
+        const int n = n0 + i * nthr;
+        if (n >= (int)take0) break;
+        const int b = first_above(s_take, p.B, n);
+        const int j = (s_len[b] + p.page - 1) / p.page + n - (b ? s_take[b - 1] : 0);
+        p.block_table[(size_t)b * p.max_blocks + j] = id[i];
+      }
     }
-    for (int t = tid; t < (int)end0; t += nthr) {
-      const int b = first_above(s_end, p.B, t);
-      const int len = s_len[b];
-      const int at = len + t - (b ? s_end[b - 1] : 0);
-      const int j = at / p.page, have = (len + p.page - 1) / p.page;
-      // a block of this step's is on the stack still, an older one in the table
-      const int id = j < have ? p.block_table[(size_t)b * p.max_blocks + j]
-                              : p.free_pages[count - 1 - (b ? s_take[b - 1] : 0) - (j - have)];
-      p.slots[t] = id * p.page + at % p.page;
-      p.positions[t] = prefix + at;
+    for (int t0 = tid; t0 < (int)end0; t0 += PG_BATCH * nthr) {
+      int at[PG_BATCH], id[PG_BATCH];
+#pragma unroll
+      for (int i = 0; i < PG_BATCH; ++i) {
+        const int t = min(t0 + i * nthr, (int)end0 - 1);
+        const int b = first_above(s_end, p.B, t);
+        const int len = s_len[b];
+        at[i] = len + t - (b ? s_end[b - 1] : 0);
+        const int j = at[i] / p.page, have = (len + p.page - 1) / p.page;
+        // a block of this step's is on the stack still, an older one in the table
+        id[i] = j < have ? p.block_table[(size_t)b * p.max_blocks + j]
+                         : p.free_pages[count - 1 - (b ? s_take[b - 1] : 0) - (j - have)];
+      }
+#pragma unroll
+      for (int i = 0; i < PG_BATCH; ++i) {
+        const int t = t0 + i * nthr;
+        if (t >= (int)end0) break;
+        p.slots[t] = id[i] * p.page + at[i] % p.page;
+        p.positions[t] = prefix + at[i];
+      }
     }
   }
   cluster_wait();
@@ -223,10 +242,18 @@ __global__ void __launch_bounds__(PG_THREADS) paged_truncate_kernel(const Trunca
   cluster_arrive();
   const int nthr = (int)cluster_size() * PG_THREADS, tid = (int)cluster_rank() * PG_THREADS + threadIdx.x;
   if (st == 0) {
-    for (int n = tid; n < (int)give0; n += nthr) {
-      const int b = first_above(s_give, p.B, n);
-      const int j = (s_keep[b] + p.page - 1) / p.page + n - (b ? s_give[b - 1] : 0);
-      p.free_pages[count + n] = p.block_table[(size_t)b * p.max_blocks + j];
+    for (int n0 = tid; n0 < (int)give0; n0 += PG_BATCH * nthr) {
+      int id[PG_BATCH];
+#pragma unroll
+      for (int i = 0; i < PG_BATCH; ++i) {
+        const int n = min(n0 + i * nthr, (int)give0 - 1);
+        const int b = first_above(s_give, p.B, n);
+        const int j = (s_keep[b] + p.page - 1) / p.page + n - (b ? s_give[b - 1] : 0);
+        id[i] = p.block_table[(size_t)b * p.max_blocks + j];
+      }
+#pragma unroll
+      for (int i = 0; i < PG_BATCH; ++i)
+        if (n0 + i * nthr < (int)give0) p.free_pages[count + n0 + i * nthr] = id[i];
     }
   }
   cluster_wait();
@@ -260,8 +287,8 @@ static int launch_cluster(void (*kern)(const P), int ctas, size_t smem, cudaStre
   return check_launch(what, cudaLaunchKernelEx(&cfg, kern, p));
 }
 
-// CTAs of the cluster: one per 2048 rows or requests, at most the portable 8.
-static int cluster_ctas(int rows, int B) { return std::max(1, std::min(8, (std::max(rows, B) + 2047) / 2048)); }
+// CTAs of the cluster: one per batch of rows a CTA has under way, at most the portable 8.
+static int cluster_ctas(int rows) { return std::max(1, std::min(8, (rows + PG_THREADS * PG_BATCH - 1) / (PG_THREADS * PG_BATCH))); }
 
 // ---------------------------------------------------------------- append
 
@@ -362,7 +389,7 @@ int sc_paged_reserve(const int32_t* lens, const int32_t* new_lens, int B, const 
              SC_ERR_SHAPE, "paged_reserve: slots past 32 bits (%d pages of %d, %d blocks)", n_free, page_size, max_blocks);
   const ReserveParams p = {lens,        new_lens, prefix_len, free_pages, free_count, block_table, kv_lens, q_start, slots,
                            positions,   free_count_out, status, B, max_blocks, page_size, n_free, max_tokens};
-  return launch_cluster(paged_reserve_kernel, cluster_ctas(max_tokens, B), (size_t)B * 12, stream, p, "paged_reserve");
+  return launch_cluster(paged_reserve_kernel, cluster_ctas(std::max(max_tokens, B)), (size_t)B * 12, stream, p, "paged_reserve");
 }
 
 int sc_paged_truncate(const int32_t* lens, const int32_t* keep, int B, const int32_t* block_table, int max_blocks,
@@ -377,7 +404,7 @@ int sc_paged_truncate(const int32_t* lens, const int32_t* keep, int B, const int
              SC_ERR_SHAPE, "paged_truncate: slots past 32 bits (%d pages of %d, %d blocks)", n_free, page_size, max_blocks);
   const TruncateParams p = {lens, keep, block_table, free_count, free_pages, lens_out, free_count_out, status, B,
                             max_blocks, page_size, n_free};
-  return launch_cluster(paged_truncate_kernel, cluster_ctas(std::min(n_free, 16 * B), B), (size_t)B * 12, stream, p,
+  return launch_cluster(paged_truncate_kernel, cluster_ctas(std::min(n_free, 16 * B)), (size_t)B * 12, stream, p,
                         "paged_truncate");
 }
 

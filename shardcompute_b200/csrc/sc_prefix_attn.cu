@@ -7,6 +7,7 @@
 // over the keys it sees; m is any bound of the exponents, so a key range can
 // be summed apart (o, l, m) and joined later.  A row that sees no key is zero.
 #include <algorithm>
+#include <atomic>
 
 #include <cuda.h>
 #include <cudaTypedefs.h>
@@ -70,7 +71,7 @@ __device__ __forceinline__ void tma3d(void* dst, const CUtensorMap* map, int row
 // ---------------------------------------------------------------- few rows
 
 // Kernel for few rows per request.  A CTA takes a request, a kv head, a share
-// of the keys and every row_groups-th tile of rows; its warps take 16-key tiles in turn, each with its own
+// of the keys and every row_groups-th tile of rows; its warps take tiles of 16 (fp32: 8) keys in turn, each with its own
 // ring of tiles in shared memory (one TMA copy of K and one of V per tile, a
 // tile never straddles a page) and its own running (m, l, o), so no barrier
 // stands in the loop.  The warps' results are joined at the end.
@@ -82,16 +83,19 @@ __device__ __forceinline__ void tma3d(void* dst, const CUtensorMap* map, int row
 // lie in the 16-row fragment as [hi; lo], so two tf32 products (with K's hi
 // and its lo) give all four terms.  A value that is not finite gives NaN.
 constexpr int FR_WARPS = 4;
-constexpr int FR_KT = 16;  // keys per tile
+constexpr float FR_RAISE = 8.f;
 
 template <typename T, int HD>
 struct FewRows {
   static constexpr bool F16 = sizeof(T) == 2;
-  static constexpr int RT = F16 ? 16 : 8;                   // rows per tile
-  static constexpr int NB = HD * (int)sizeof(T) / 128;      // 128-byte chunks per key
-  static constexpr int TILE = NB * FR_KT * 128;             // bytes of a K or V tile
+  static constexpr int RT = F16 ? 16 : 8;               // rows per tile
+  static constexpr int KT = F16 ? 16 : 8;               // keys per tile
+  static constexpr int NJ = KT / 8;                     // 8-key blocks of the product
+  static constexpr int NB = HD * (int)sizeof(T) / 128;  // 128-byte chunks per key
+  static constexpr int SUB = KT * 128;                  // bytes of a chunk of a tile
+  static constexpr int TILE = NB * SUB;                 // bytes of a K or V tile
   static constexpr int STAGE = 2 * TILE;
-  static constexpr int NST = F16 ? (HD == 128 ? 3 : 6) : 3; // stages per warp
+  static constexpr int NST = HD == 128 ? 3 : 6;         // stages per warp: 96 KB a CTA, two CTAs an SM
   static constexpr int SMEM = FR_WARPS * NST * STAGE + 1024;
 };
 
@@ -123,7 +127,7 @@ __global__ void __launch_bounds__(FR_WARPS * 32)
 few_rows_kernel(const PrefixAttnParams p, const __grid_constant__ PoolMaps maps, int with_prefix, int splits, int row_groups,
                 int slot0) {
   using C = FewRows<T, HD>;
-  constexpr int RT = C::RT, NST = C::NST;
+  constexpr int RT = C::RT, NST = C::NST, KT = C::KT, NJ = C::NJ, SUB = C::SUB;
   extern __shared__ __align__(1024) unsigned char fr_smem[];
   __shared__ __align__(8) uint64_t full[FR_WARPS][NST];
   __shared__ float s_m[FR_WARPS][RT], s_l[FR_WARPS][RT];
@@ -147,7 +151,7 @@ few_rows_kernel(const PrefixAttnParams p, const __grid_constant__ PoolMaps maps,
   int row_lo, row_hi;
   request_rows(p, b, row_lo, row_hi);
   const int n = row_hi - row_lo, len = request_len(p, b), P = with_prefix ? prefix_keys(p) : 0;
-  const int np = (P + FR_KT - 1) / FR_KT;
+  const int np = (P + KT - 1) / KT;
   unsigned char* ring = base + (size_t)warp * NST * C::STAGE;
   const uint32_t ring_u = smem_u32(ring);
   uint32_t issued = 0, used = 0;  // tiles of this warp's ring, over all row tiles
@@ -156,7 +160,7 @@ few_rows_kernel(const PrefixAttnParams p, const __grid_constant__ PoolMaps maps,
     const int nr = min(RT, n * p.G - r0);
     // own keys that the tile's last row sees
     const int own = max(0, min(len, len - n + (r0 + nr - 1) / p.G + 1));
-    const int nt = np + (own + FR_KT - 1) / FR_KT;
+    const int nt = np + (own + KT - 1) / KT;
     const int per = (nt + splits - 1) / splits;
     const int t_lo = min(nt, split * per), t_hi = min(nt, t_lo + per);
     const int cnt = max(0, (t_hi - t_lo - warp + FR_WARPS - 1) / FR_WARPS);  // tiles t_lo + warp + 4 i
@@ -166,7 +170,7 @@ few_rows_kernel(const PrefixAttnParams p, const __grid_constant__ PoolMaps maps,
       const int t = t_lo + warp + FR_WARPS * (first + lane);
       if (t >= t_hi) return -1;
       const bool pre = t < np;
-      const int key = (pre ? t : t - np) * FR_KT;
+      const int key = (pre ? t : t - np) * KT;
       const int blk = key >> p.lg_page;
       const int id = pre ? p.prefix_table[blk] : p.block_table[(size_t)b * p.max_blocks + blk];
       if (id < 0 || id >= p.n_pages) return -1;
@@ -221,10 +225,13 @@ few_rows_kernel(const PrefixAttnParams p, const __grid_constant__ PoolMaps maps,
           split_tf32(v.w, qa[ks + 1][2], qa[ks + 1][3]);
         }
     }
-    // own keys each of this thread's rows sees (rows past the last: as the last, so they ask for no mask)
+    // own keys that the first row sees, and each of this thread's rows (rows past the last: as the last)
+    const int see_first = max(0, min(len, len - n + r0 / p.G + 1));
     const int see0 = r8 < nr ? max(0, len - n + (r0 + r8) / p.G + 1) : own;
     const int see1 = r8 + 8 < nr ? max(0, len - n + (r0 + r8 + 8) / p.G + 1) : own;
 
+    const uint32_t k_lane = (((lane >> 4) << 3) + (lane & 7)) * 128 + ((((lane >> 3) & 1) ^ (lane & 7)) << 4);
+    const uint32_t v_lane = ((((lane >> 3) & 1) << 3) + (lane & 7)) * 128 + (((lane >> 4) ^ (lane & 7)) << 4);
     constexpr int NO = HD / 8;
     float o[NO][4];
 #pragma unroll
@@ -237,54 +244,48 @@ few_rows_kernel(const PrefixAttnParams p, const __grid_constant__ PoolMaps maps,
       const uint32_t ks_u = ring_u + s * C::STAGE, vs_u = ks_u + C::TILE;
       const int t = t_lo + warp + FR_WARPS * i;
       const bool gone = (absent >> s) & 1u;
-      // keys of this tile that each row sees, and that any row sees
-      const int first = (t < np ? t : t - np) * FR_KT;
-      const int lim0 = gone ? 0 : (t < np ? P : see0) - first, lim1 = gone ? 0 : (t < np ? P : see1) - first;
-      const int lim = gone ? 0 : (t < np ? P : own) - first;
-      const bool part = __any_sync(0xffffffffu, lim0 < FR_KT || (C::F16 && lim1 < FR_KT));
-
-      float sc[2][4];
+      const int first = (t < np ? t : t - np) * KT;
+      const bool part = gone || (t < np ? P : see_first) - first < KT;  // not every row sees every key
+      float sc[NJ][4];
 #pragma unroll
-      for (int j = 0; j < 2; ++j) sc[j][0] = sc[j][1] = sc[j][2] = sc[j][3] = 0.f;
+      for (int j = 0; j < NJ; ++j) sc[j][0] = sc[j][1] = sc[j][2] = sc[j][3] = 0.f;
       if constexpr (C::F16) {
-        const int row = ((lane >> 4) << 3) + (lane & 7);
-        const uint32_t ra = ks_u + row * 128;
+        // lane l: row l & 7 of key block l >> 4, 16-byte piece 2 ks + (l >> 3 & 1), swizzled by its row
+        const uint32_t ra = ks_u + k_lane;
 #pragma unroll
         for (int ks = 0; ks < HD / 16; ++ks) {
-          const int ch = ks * 2 + ((lane >> 3) & 1);
           uint32_t kb[4];
-          ldsm4(ra + (ch >> 3) * (FR_KT * 128) + (((ch & 7) ^ (row & 7)) << 4), kb);
+          ldsm4((ra ^ ((2 * ks & 7) << 4)) + (ks >> 2) * SUB, kb);
           mma_16816(sc[0], qa[ks][0], qa[ks][1], qa[ks][2], qa[ks][3], kb[0], kb[1]);
-          mma_16816(sc[1], qa[ks][0], qa[ks][1], qa[ks][2], qa[ks][3], kb[2], kb[3]);
+          mma_16816(sc[NJ - 1], qa[ks][0], qa[ks][1], qa[ks][2], qa[ks][3], kb[2], kb[3]);
         }
       } else {
+        const uint32_t ra = ks_u + r8 * 128;
+        float cr[4] = {0.f, 0.f, 0.f, 0.f};  // K's low parts, apart: a shorter chain of sums
 #pragma unroll
-        for (int j = 0; j < 2; ++j) {
-          const int key = j * 8 + r8;
-          const uint32_t ra = ks_u + key * 128;
+        for (int dd = 0; dd < HD / 32; ++dd)
 #pragma unroll
-          for (int dd = 0; dd < HD / 32; ++dd)
-#pragma unroll
-            for (int c2 = 0; c2 < 2; ++c2) {
-              const float4 v = lds_f4(ra + dd * (FR_KT * 128) + (((2 * q4 + c2) ^ (key & 7)) << 4));
-              uint32_t hi[4], lo[4];
-              split_tf32(v.x, hi[0], lo[0]);
-              split_tf32(v.y, hi[1], lo[1]);
-              split_tf32(v.z, hi[2], lo[2]);
-              split_tf32(v.w, hi[3], lo[3]);
-              const int ks = dd * 4 + c2 * 2;
-              mma_1688(sc[j], qa[ks], lo[0], lo[1]);
-              mma_1688(sc[j], qa[ks], hi[0], hi[1]);
-              mma_1688(sc[j], qa[ks + 1], lo[2], lo[3]);
-              mma_1688(sc[j], qa[ks + 1], hi[2], hi[3]);
-            }
-          sc[j][0] += sc[j][2];  // rows 8..15 of the fragment: q's low parts
-          sc[j][1] += sc[j][3];
-        }
+          for (int c2 = 0; c2 < 2; ++c2) {
+            const float4 v = lds_f4(ra + dd * SUB + (((2 * q4 + c2) ^ r8) << 4));
+            uint32_t hi[4], lo[4];
+            split_tf32(v.x, hi[0], lo[0]);
+            split_tf32(v.y, hi[1], lo[1]);
+            split_tf32(v.z, hi[2], lo[2]);
+            split_tf32(v.w, hi[3], lo[3]);
+            const int ks = dd * 4 + c2 * 2;
+            mma_1688(cr, qa[ks], lo[0], lo[1]);
+            mma_1688(sc[0], qa[ks], hi[0], hi[1]);
+            mma_1688(cr, qa[ks + 1], lo[2], lo[3]);
+            mma_1688(sc[0], qa[ks + 1], hi[2], hi[3]);
+          }
+        // rows 8..15 of the fragment: q's low parts
+        sc[0][0] += (sc[0][2] + cr[0]) + cr[2];
+        sc[0][1] += (sc[0][3] + cr[1]) + cr[3];
       }
       if (part) {
+        const int lim0 = gone ? 0 : (t < np ? P : see0) - first, lim1 = gone ? 0 : (t < np ? P : see1) - first;
 #pragma unroll
-        for (int j = 0; j < 2; ++j)
+        for (int j = 0; j < NJ; ++j)
 #pragma unroll
           for (int e = 0; e < 2; ++e) {
             const int key = j * 8 + q4 * 2 + e;
@@ -292,17 +293,23 @@ few_rows_kernel(const PrefixAttnParams p, const __grid_constant__ PoolMaps maps,
             if (C::F16 && key >= lim1) sc[j][2 + e] = -INFINITY;
           }
       }
-      // ---- running softmax
-      float x0 = fmaxf(fmaxf(sc[0][0], sc[0][1]), fmaxf(sc[1][0], sc[1][1]));
-      float x1 = fmaxf(fmaxf(sc[0][2], sc[0][3]), fmaxf(sc[1][2], sc[1][3]));
-#pragma unroll
-      for (int d = 1; d <= 2; d <<= 1) {
-        x0 = fmaxf(x0, __shfl_xor_sync(0xffffffffu, x0, d));
-        if (C::F16) x1 = fmaxf(x1, __shfl_xor_sync(0xffffffffu, x1, d));
+      // ---- running softmax.  A row's m, the same in its four lanes, is raised (and o rescaled) only when a score
+      // passes it by 2^8: weights stay below 2^8, and the lanes seldom have to agree on a maximum.
+      float x0 = fmaxf(sc[0][0], sc[0][1]), x1 = fmaxf(sc[0][2], sc[0][3]);
+      if (NJ == 2) {
+        x0 = fmaxf(x0, fmaxf(sc[NJ - 1][0], sc[NJ - 1][1]));
+        x1 = fmaxf(x1, fmaxf(sc[NJ - 1][2], sc[NJ - 1][3]));
       }
-      x0 = fmaxf(m0, x0 * p.c);
-      x1 = C::F16 ? fmaxf(m1, x1 * p.c) : m1;
-      if (__any_sync(0xffffffffu, x0 > m0 || x1 > m1)) {
+      x0 *= p.c;
+      x1 = C::F16 ? x1 * p.c : -INFINITY;
+      if (__any_sync(0xffffffffu, x0 > m0 + FR_RAISE || x1 > m1 + FR_RAISE)) {
+#pragma unroll
+        for (int d = 1; d <= 2; d <<= 1) {
+          x0 = fmaxf(x0, __shfl_xor_sync(0xffffffffu, x0, d));
+          x1 = fmaxf(x1, __shfl_xor_sync(0xffffffffu, x1, d));
+        }
+        x0 = fmaxf(m0, x0);
+        x1 = fmaxf(m1, x1);
         const float f0 = m0 == -INFINITY ? 0.f : ex2(m0 - x0), f1 = m1 == -INFINITY ? 0.f : ex2(m1 - x1);
         l0 *= f0;
         l1 *= f1;
@@ -318,7 +325,7 @@ few_rows_kernel(const PrefixAttnParams p, const __grid_constant__ PoolMaps maps,
       }
       const float n0 = m0 == -INFINITY ? 0.f : m0, n1 = m1 == -INFINITY ? 0.f : m1;
 #pragma unroll
-      for (int j = 0; j < 2; ++j) {
+      for (int j = 0; j < NJ; ++j) {
         sc[j][0] = ex2(fmaf(sc[j][0], p.c, -n0));
         sc[j][1] = ex2(fmaf(sc[j][1], p.c, -n0));
         l0 += sc[j][0] + sc[j][1];
@@ -329,49 +336,49 @@ few_rows_kernel(const PrefixAttnParams p, const __grid_constant__ PoolMaps maps,
         }
       }
       // ---- o += P V.  Slots behind the last key may hold anything: their V counts as zero.
+      const int lim = gone ? 0 : (t < np ? P : own) - first;  // keys that any row sees
       if constexpr (C::F16) {
         const uint32_t a0 = h2_as_u32(__floats2half2_rn(sc[0][0], sc[0][1])), a1 = h2_as_u32(__floats2half2_rn(sc[0][2], sc[0][3]));
-        const uint32_t a2 = h2_as_u32(__floats2half2_rn(sc[1][0], sc[1][1])), a3 = h2_as_u32(__floats2half2_rn(sc[1][2], sc[1][3]));
-        uint32_t k0 = 0xffffffffu, k1 = 0xffffffffu;
-        if (part) {
-          const int key = q4 * 2;
-          k0 = (key < lim ? 0xffffu : 0u) | (key + 1 < lim ? 0xffff0000u : 0u);
-          k1 = (key + 8 < lim ? 0xffffu : 0u) | (key + 9 < lim ? 0xffff0000u : 0u);
-        }
-        const int row = (((lane >> 3) & 1) << 3) + (lane & 7);
-        const uint32_t ra = vs_u + row * 128;
+        const uint32_t a2 = h2_as_u32(__floats2half2_rn(sc[NJ - 1][0], sc[NJ - 1][1])),
+                       a3 = h2_as_u32(__floats2half2_rn(sc[NJ - 1][2], sc[NJ - 1][3]));
+        const uint32_t ra = vs_u + v_lane;
+        auto product = [&](uint32_t k0, uint32_t k1) {
 #pragma unroll
-        for (int nb = 0; nb < HD / 16; ++nb) {
-          const int ch = nb * 2 + (lane >> 4);
-          uint32_t vb[4];
-          ldsm4_t(ra + (ch >> 3) * (FR_KT * 128) + (((ch & 7) ^ (row & 7)) << 4), vb);
-          mma_16816(o[2 * nb], a0, a1, a2, a3, vb[0] & k0, vb[1] & k1);
-          mma_16816(o[2 * nb + 1], a0, a1, a2, a3, vb[2] & k0, vb[3] & k1);
+          for (int nb = 0; nb < HD / 16; ++nb) {
+            uint32_t vb[4];
+            ldsm4_t((ra ^ ((2 * nb & 7) << 4)) + (nb >> 2) * SUB, vb);
+            mma_16816(o[2 * nb], a0, a1, a2, a3, vb[0] & k0, vb[1] & k1);
+            mma_16816(o[2 * nb + 1], a0, a1, a2, a3, vb[2] & k0, vb[3] & k1);
+          }
+        };
+        if (!part) {
+          product(0xffffffffu, 0xffffffffu);
+        } else {
+          const int key = q4 * 2;
+          product((key < lim ? 0xffffu : 0u) | (key + 1 < lim ? 0xffff0000u : 0u),
+                  (key + 8 < lim ? 0xffffu : 0u) | (key + 9 < lim ? 0xffff0000u : 0u));
         }
       } else {
+        uint32_t pa[4];
+        split_tf32(sc[0][0], pa[0], pa[1]);
+        split_tf32(sc[0][1], pa[2], pa[3]);
+        const int key = 2 * q4;  // slots q4 and q4 + 4 of k: keys 2 q4 and 2 q4 + 1
+        const bool u0 = !part || key < lim, u1 = !part || key + 1 < lim;
 #pragma unroll
-        for (int j = 0; j < 2; ++j) {
-          uint32_t pa[4];
-          split_tf32(sc[j][0], pa[0], pa[1]);
-          split_tf32(sc[j][1], pa[2], pa[3]);
-          const int key = j * 8 + 2 * q4;  // slots q4 and q4 + 4 of k: keys 2 q4 and 2 q4 + 1
-          const bool u0 = !part || key < lim, u1 = !part || key + 1 < lim;
+        for (int dd = 0; dd < HD / 32; ++dd) {
+          const uint32_t sub = vs_u + dd * SUB;
+          float4 va = lds_f4(sub + key * 128 + ((r8 ^ key) << 4));
+          float4 vb = lds_f4(sub + (key + 1) * 128 + ((r8 ^ (key + 1)) << 4));
+          if (!u0) va = make_float4(0.f, 0.f, 0.f, 0.f);
+          if (!u1) vb = make_float4(0.f, 0.f, 0.f, 0.f);
+          const float xa[4] = {va.x, va.y, va.z, va.w}, xb[4] = {vb.x, vb.y, vb.z, vb.w};
 #pragma unroll
-          for (int dd = 0; dd < HD / 32; ++dd) {
-            const uint32_t sub = vs_u + dd * (FR_KT * 128);
-            float4 va = lds_f4(sub + key * 128 + ((r8 ^ (key & 7)) << 4));
-            float4 vb = lds_f4(sub + (key + 1) * 128 + ((r8 ^ ((key + 1) & 7)) << 4));
-            if (!u0) va = make_float4(0.f, 0.f, 0.f, 0.f);
-            if (!u1) vb = make_float4(0.f, 0.f, 0.f, 0.f);
-            const float xa[4] = {va.x, va.y, va.z, va.w}, xb[4] = {vb.x, vb.y, vb.z, vb.w};
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              uint32_t h0, e0, h1, e1;
-              split_tf32(xa[e], h0, e0);
-              split_tf32(xb[e], h1, e1);
-              mma_1688(o[dd * 4 + e], pa, e0, e1);
-              mma_1688(o[dd * 4 + e], pa, h0, h1);
-            }
+          for (int e = 0; e < 4; ++e) {
+            uint32_t h0, e0, h1, e1;
+            split_tf32(xa[e], h0, e0);
+            split_tf32(xb[e], h1, e1);
+            mma_1688(o[dd * 4 + e], pa, e0, e1);
+            mma_1688(o[dd * 4 + e], pa, h0, h1);
           }
         }
       }
@@ -685,7 +692,7 @@ many_rows_kernel(const PrefixAttnParams p, const __grid_constant__ PoolMaps maps
   if (threadIdx.x == 0) {
     for (int i = 0; i < NBUF; ++i) {
       mbar_init(&full[i], 1);
-      mbar_init(&empty[i], nx);
+      mbar_init(&empty[i], nx + 1);  // the MMA issuers, and warp 3
     }
     for (int x = 0; x < 2; ++x) {
       mbar_init(&q_full[x], TC_M);
@@ -796,19 +803,24 @@ many_rows_kernel(const PrefixAttnParams p, const __grid_constant__ PoolMaps maps
     }
   } else if (warp == 3) {
     // ================================ V's tail ================================
-    for (int i = 0; i < cnt; ++i) {
+    // It follows every tile of the ring and frees it as the MMA issuers do: a barrier's parity says which of two
+    // phases is over, not which of many.
+    for (uint32_t it = 0; it < 2u * cnt; ++it) {
+      const int s = it % NBUF, i = it / 2;
+      if (!__all_sync(0xffffffffu, pa_wait(&full[s], (it / NBUF) & 1u, abort))) break;
       const int keys = keys_of(t_lo + i);
-      if (keys >= TC_N) continue;
-      const uint32_t vi = 2 * i + 1, v = ring_u + (vi % NBUF) * C::TILE;
-      if (!__all_sync(0xffffffffu, pa_wait(&full[vi % NBUF], (vi / NBUF) & 1u, abort))) break;
-      for (int e = lane; e < (TC_N - keys) * 8 * C::NCH; e += 32) {
-        const int r = keys + e / (8 * C::NCH), c = e % (8 * C::NCH);
-        asm volatile("st.shared.v4.u32 [%0], {%1, %1, %1, %1};" ::"r"(v + (c >> 3) * (TC_N * 128) + r * 128 + ((c & 7) << 4)), "r"(0)
-                     : "memory");
+      if ((it & 1) && keys < TC_N) {
+        const uint32_t v = ring_u + s * C::TILE;
+        for (int e = lane; e < (TC_N - keys) * 8 * C::NCH; e += 32) {
+          const int r = keys + e / (8 * C::NCH), c = e % (8 * C::NCH);
+          asm volatile("st.shared.v4.u32 [%0], {%1, %1, %1, %1};" ::"r"(v + (c >> 3) * (TC_N * 128) + r * 128 + ((c & 7) << 4)), "r"(0)
+                       : "memory");
+        }
+        fence_async_smem();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&v_clean[t_lo + i >= np]);
       }
-      fence_async_smem();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&v_clean[t_lo + i >= np]);
+      if (lane == 0) mbar_arrive(&empty[s]);
     }
   } else if (warp >= 4) {
     // ================================ softmax ================================
@@ -1015,6 +1027,7 @@ many_rows_kernel(const PrefixAttnParams p, const __grid_constant__ PoolMaps maps
 //                last key, which may hold anything, become zero
 // TMEM: two buffers of S (hi.hi | cross, 64 columns each), O (hi.hi | cross).
 constexpr int TF_N = 64;              // keys of a tile
+constexpr int TF_BOX = 16;            // keys of a copy
 constexpr int TF_THREADS = 16 * 32;
 constexpr int TF_CONV = 8;            // warps that split
 
@@ -1024,7 +1037,7 @@ struct ManyRowsF32 {
   static constexpr int QT = TC_M * HD * 2;          // bytes of one part of Q
   static constexpr int PT = TF_N * HD * 2;          // bytes of one part of a K or V tile
   static constexpr int RAW = TF_N * HD * 4;         // bytes of a raw tile
-  static constexpr int BOX = FR_KT * HD * 4;        // bytes of one copy: 16 keys
+  static constexpr int BOX = TF_BOX * HD * 4;        // bytes of one copy: 16 keys
   static constexpr int NRAW = HD == 128 ? 3 : 6;
   static constexpr int SMEM = 2 * QT + 4 * PT + NRAW * RAW + 1024;
 };
@@ -1091,12 +1104,12 @@ many_rows_f32_kernel(const PrefixAttnParams p, const __grid_constant__ PoolMaps 
     auto rows_of = [&](int i) {
       const int t = w.t_lo + i;
       int at = -1;
-      if (lane < TF_N / FR_KT && lane * FR_KT < keys_of(t)) {
-        const int key = (t < np ? t : t - np) * TF_N + lane * FR_KT, blk = key >> p.lg_page;
+      if (lane < TF_N / TF_BOX && lane * TF_BOX < keys_of(t)) {
+        const int key = (t < np ? t : t - np) * TF_N + lane * TF_BOX, blk = key >> p.lg_page;
         const int id = t < np ? p.prefix_table[blk] : p.block_table[(size_t)w.b * p.max_blocks + blk];
         if (id >= 0 && id < p.n_pages) at = ((id * p.Hkv + h) << p.lg_page) + (key & ((1 << p.lg_page) - 1));
       }
-      const uint32_t gone = __ballot_sync(0xffffffffu, at < 0) & ((1u << (TF_N / FR_KT)) - 1);
+      const uint32_t gone = __ballot_sync(0xffffffffu, at < 0) & ((1u << (TF_N / TF_BOX)) - 1);
       if (lane == 0) s_absent[i & 15] = gone;  // a bit per 16 keys
       return at;
     };
@@ -1105,7 +1118,7 @@ many_rows_f32_kernel(const PrefixAttnParams p, const __grid_constant__ PoolMaps 
       if (!__all_sync(0xffffffffu, pa_wait(&raw_empty[s], ((it / NRAW) & 1u) ^ 1u, abort))) return false;
       if (lane == 0) mbar_arrive_expect_tx(&raw_full[s], C::RAW);
       __syncwarp();
-      if (lane < TF_N / FR_KT) tma3d_at(raw_u + s * C::RAW + lane * C::BOX, map, at < 0 ? p.pool_rows : at, 0, &raw_full[s]);
+      if (lane < TF_N / TF_BOX) tma3d_at(raw_u + s * C::RAW + lane * C::BOX, map, at < 0 ? p.pool_rows : at, 0, &raw_full[s]);
       return true;
     };
     uint32_t it = 0;
@@ -1176,10 +1189,10 @@ many_rows_f32_kernel(const PrefixAttnParams p, const __grid_constant__ PoolMaps 
       const uint32_t src = raw_u + s * C::RAW;
 #pragma unroll 4
       for (int k0 = 0; k0 < TF_N; k0 += TF_CONV * KPW) {
-        const int key = k0 + (warp - 8) * KPW + sub, r = key % FR_KT;
+        const int key = k0 + (warp - 8) * KPW + sub, r = key % TF_BOX;
         // 8 values: pieces 2 (g % 4) and 2 (g % 4) + 1 of 128-byte chunk g / 4; odd chunks in the other order, so that
         // eight lanes read eight banks' worth
-        const uint32_t at = src + (key / FR_KT) * C::BOX + (g >> 2) * (FR_KT * 128) + r * 128;
+        const uint32_t at = src + (key / TF_BOX) * C::BOX + (g >> 2) * (TF_BOX * 128) + r * 128;
         const int p0 = 2 * (g & 3) + ((g >> 2) & 1);
         float4 a = lds_f4(at + ((p0 ^ (r & 7)) << 4)), b = lds_f4(at + (((p0 ^ 1) ^ (r & 7)) << 4));
         if ((g >> 2) & 1) {
@@ -1449,6 +1462,19 @@ static bool pool_map(CUtensorMap* m, const void* pool, size_t rows, int hd, bool
             CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
+// Shared-memory opt-in of a kernel, once per device.
+template <auto KERN>
+static cudaError_t opt_in(int smem) {
+  static std::atomic<uint64_t> done{0};
+  int dev = 0;
+  cudaGetDevice(&dev);
+  const uint64_t bit = dev < 64 ? 1ull << dev : 0;
+  if (done.load(std::memory_order_acquire) & bit) return cudaSuccess;
+  const cudaError_t e = cudaFuncSetAttribute(KERN, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  if (e == cudaSuccess) done.fetch_or(bit, std::memory_order_release);
+  return e;
+}
+
 // How a call is cut.  The host knows the rows T and the requests B, not which request has how many, nor how many
 // keys there are, only how many the tables hold.
 //   few rows      few_rows_kernel over the prefix and the requests' own keys
@@ -1475,8 +1501,7 @@ static AttnPlan plan_attn(int T, int B, int Hkv, int G, bool f16, long long own_
     a.nslots = a.tc_splits;
   }
   if (a.kind != AttnPlan::CHUNKS) {
-    // four CTAs per SM over all requests and heads: first from tiles of rows, then from the keys (at least a 16-key
-    // tile for each of a CTA's 4 warps)
+    // four CTAs per SM over all requests and heads: first from tiles of rows, then from the keys (64 of them at least)
     const int rt = f16 ? 16 : 8;
     const long long keys = own_keys + (a.kind == AttnPlan::FEW ? prefix_keys : 0);
     const long long want = ceil_div(4ll * sms, (long long)B * Hkv), tiles = ceil_div(rows, (long long)B * rt);
@@ -1487,12 +1512,11 @@ static AttnPlan plan_attn(int T, int B, int Hkv, int G, bool f16, long long own_
   return a;
 }
 
-template <typename K>
-static int run_many_rows(K kern, int smem, int threads, const PrefixAttnParams& p, const PoolMaps& maps, const AttnPlan& a,
-                         cudaStream_t stream) {
-  const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+template <auto KERN>
+static int run_many_rows(int smem, int threads, const PrefixAttnParams& p, const PoolMaps& maps, const AttnPlan& a, cudaStream_t stream) {
+  const cudaError_t e = opt_in<KERN>(smem);
   if (e != cudaSuccess) return check_launch("prefix_attn", e);
-  launch(kern, dim3((unsigned)(a.tc_splits * a.tc_items), p.Hkv), dim3(threads), smem, stream, p, maps, a.tc_splits, 0);
+  launch(KERN, dim3((unsigned)(a.tc_splits * a.tc_items), p.Hkv), dim3(threads), smem, stream, p, maps, a.tc_splits, 0);
   return check_launch("prefix_attn_many_rows");
 }
 
@@ -1502,25 +1526,25 @@ static int run_attn(const PrefixAttnParams& p, const void* k, const void* v, con
   int st = SC_OK;
   if (a.kind != AttnPlan::FEW) {
     PoolMaps maps;
-    const int box = C::F16 ? std::min(TC_N, 1 << p.lg_page) : FR_KT, chunks = C::F16 ? 1 : C::NB;
+    const int box = C::F16 ? std::min(TC_N, 1 << p.lg_page) : TF_BOX, chunks = C::F16 ? 1 : C::NB;
     SC_REQUIRE(pool_map(&maps.k, k, p.pool_rows, HD, C::F16, box, chunks) && pool_map(&maps.v, v, p.pool_rows, HD, C::F16, box, chunks),
                SC_ERR_CUDA, "prefix_attn: tensor map of the pages refused");
     const bool packed = a.kind == AttnPlan::SHARED;
     if constexpr (C::F16)
-      st = run_many_rows(packed ? many_rows_kernel<HD, true> : many_rows_kernel<HD, false>, ManyRows<HD>::SMEM, TC_THREADS, p, maps, a, stream);
+      st = packed ? run_many_rows<many_rows_kernel<HD, true>>(ManyRows<HD>::SMEM, TC_THREADS, p, maps, a, stream)
+                  : run_many_rows<many_rows_kernel<HD, false>>(ManyRows<HD>::SMEM, TC_THREADS, p, maps, a, stream);
     else
-      st = run_many_rows(packed ? many_rows_f32_kernel<HD, true> : many_rows_f32_kernel<HD, false>, ManyRowsF32<HD>::SMEM, TF_THREADS, p,
-                         maps, a, stream);
+      st = packed ? run_many_rows<many_rows_f32_kernel<HD, true>>(ManyRowsF32<HD>::SMEM, TF_THREADS, p, maps, a, stream)
+                  : run_many_rows<many_rows_f32_kernel<HD, false>>(ManyRowsF32<HD>::SMEM, TF_THREADS, p, maps, a, stream);
     if (st != SC_OK) return st;
   }
   if (a.kind != AttnPlan::CHUNKS) {
     PoolMaps maps;
-    SC_REQUIRE(pool_map(&maps.k, k, p.pool_rows, HD, C::F16, FR_KT, C::NB) && pool_map(&maps.v, v, p.pool_rows, HD, C::F16, FR_KT, C::NB),
+    SC_REQUIRE(pool_map(&maps.k, k, p.pool_rows, HD, C::F16, C::KT, C::NB) && pool_map(&maps.v, v, p.pool_rows, HD, C::F16, C::KT, C::NB),
                SC_ERR_CUDA, "prefix_attn: tensor map of the pages refused");
-    auto kern = few_rows_kernel<T, HD>;
-    const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM);
+    const cudaError_t e = opt_in<few_rows_kernel<T, HD>>(C::SMEM);
     if (e != cudaSuccess) return check_launch("prefix_attn", e);
-    launch(kern, dim3(a.splits * a.row_groups, p.Hkv, p.B), dim3(FR_WARPS * 32), C::SMEM, stream, p, maps,
+    launch(few_rows_kernel<T, HD>, dim3(a.splits * a.row_groups, p.Hkv, p.B), dim3(FR_WARPS * 32), C::SMEM, stream, p, maps,
            a.kind == AttnPlan::FEW ? 1 : 0, a.splits, a.row_groups, a.kind == AttnPlan::SHARED ? a.tc_splits : 0);
     st = check_launch("prefix_attn_few_rows");
     if (st != SC_OK) return st;

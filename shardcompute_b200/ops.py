@@ -9,6 +9,7 @@ device; there is no CPU path.
 from __future__ import annotations
 
 import ctypes as C
+import functools
 import math
 from typing import NamedTuple, Optional, Sequence
 
@@ -261,25 +262,30 @@ class PagedStep(NamedTuple):
     status: torch.Tensor       # [1] 0, or why nothing was reserved
 
 
-def _on_one_device(what: str, first: torch.Tensor, *rest: Optional[torch.Tensor]) -> torch.device:
-    """The device of the tensors, which are CUDA tensors of one device and contiguous."""
-    dev = first.device
-    for t in (first, *rest):
-        if t is None:
-            continue
+_I32 = torch.int32
+
+
+def _refuse(what: str, dev: int, ts: Sequence[torch.Tensor], dtype: Optional[torch.dtype]) -> None:
+    """Raises for the first of the tensors that is not a contiguous CUDA tensor of device ``dev`` and type ``dtype``."""
+    for t in ts:
         if not t.is_cuda:
             raise RuntimeError("libsc_b200 ops take CUDA tensors only (no CPU path)")
-        if t.device != dev:
-            raise ValueError(f"{what}: tensors on {dev} and {t.device}")
+        if t.get_device() != dev:
+            raise ValueError(f"{what}: tensors on cuda:{dev} and {t.device}")
+        if dtype is not None and t.dtype is not dtype:
+            raise ValueError(f"{what}: lengths, tables, slots and counts must be int32, got {t.dtype}")
         if not t.is_contiguous():
             raise ValueError(f"{what}: tensors must be contiguous")
-    return dev
+    raise ValueError(f"{what}: unsupported tensors")
 
 
-def _int32(what: str, **named: Optional[torch.Tensor]) -> None:
-    for name, t in named.items():
-        if t is not None and t.dtype != torch.int32:
-            raise ValueError(f"{what}: {name} must be int32, got {t.dtype}")
+def _check(what: str, dev: int, ts: Sequence[torch.Tensor], dtype: Optional[torch.dtype] = None) -> None:
+    """One pass over the tensors of a call, which a serving loop makes for every layer and token."""
+    if dev < 0:
+        _refuse(what, dev, ts, dtype)
+    for t in ts:
+        if t.get_device() != dev or (dtype is not None and t.dtype is not dtype) or not t.is_contiguous():
+            _refuse(what, dev, ts, dtype)
 
 
 def _sized(what: str, n: int, **named: Optional[torch.Tensor]) -> None:
@@ -288,13 +294,13 @@ def _sized(what: str, n: int, **named: Optional[torch.Tensor]) -> None:
             raise ValueError(f"{what}: {name} holds {t.numel()} values, {n} are needed")
 
 
-def _call_on(dev: torch.device, name: str, *args) -> None:
-    """The call with ``dev`` as the current device, on its current stream."""
-    if dev.index == torch.cuda.current_device():
-        L.call(name, *args, torch.cuda.current_stream(dev).cuda_stream)
+def _call_on(dev: int, name: str, *args) -> None:
+    """The call with device ``dev`` as the current one, on its current stream."""
+    if dev == torch._C._cuda_getDevice():
+        L.call(name, *args, torch._C._cuda_getCurrentRawStream(dev))
     else:
         with torch.cuda.device(dev):
-            L.call(name, *args, torch.cuda.current_stream(dev).cuda_stream)
+            L.call(name, *args, torch._C._cuda_getCurrentRawStream(dev))
 
 
 def paged_reserve(lens: torch.Tensor, new_lens: torch.Tensor, block_table: torch.Tensor, free_pages: torch.Tensor,
@@ -310,24 +316,21 @@ def paged_reserve(lens: torch.Tensor, new_lens: torch.Tensor, block_table: torch
     ``kv_lens`` may be ``lens`` and ``free_count_out`` may be ``free_count``.  If ``status`` is not 0 nothing was
     reserved and ``q_start`` is all zeros: 1 not enough pages, 2 a request exceeds ``max_blocks`` pages, 4 more than
     ``max_tokens`` new tokens, 8 a negative length, 16 ``free_count`` outside the stack (the sum of those that hold)."""
-    B = lens.numel()
-    dev = _on_one_device("paged_reserve", lens, new_lens, block_table, free_pages, free_count, prefix_len, kv_lens, q_start,
-                         slots, positions, free_count_out, status)
+    B, dev = lens.numel(), lens.get_device()
     if slots is None:
         if max_tokens is None:
             raise ValueError("paged_reserve: max_tokens or slots is needed")
-        slots = torch.full((max_tokens,), -1, dtype=torch.int32, device=dev)
+        slots = torch.full((max_tokens,), -1, dtype=_I32, device=lens.device)
     rows = slots.numel() if max_tokens is None else max_tokens
     if positions is None:
-        positions = torch.full((rows,), -1, dtype=torch.int32, device=dev)
-    new = lambda n: torch.empty(n, dtype=torch.int32, device=dev)  # noqa: E731
+        positions = torch.full((rows,), -1, dtype=_I32, device=lens.device)
+    new = lambda n: torch.empty(n, dtype=_I32, device=lens.device)  # noqa: E731
     kv_lens = new(B) if kv_lens is None else kv_lens
     q_start = new(B + 1) if q_start is None else q_start
     free_count_out = new(1) if free_count_out is None else free_count_out
     status = new(1) if status is None else status
-    _int32("paged_reserve", lens=lens, new_lens=new_lens, block_table=block_table, free_pages=free_pages, free_count=free_count,
-           prefix_len=prefix_len, kv_lens=kv_lens, q_start=q_start, slots=slots, positions=positions,
-           free_count_out=free_count_out, status=status)
+    ts = (lens, new_lens, block_table, free_pages, free_count, kv_lens, q_start, slots, positions, free_count_out, status)
+    _check("paged_reserve", dev, ts if prefix_len is None else (*ts, prefix_len), _I32)
     if block_table.dim() != 2 or block_table.shape[0] != B:
         raise ValueError(f"paged_reserve: block_table {tuple(block_table.shape)} is not [{B}, max_blocks]")
     _sized("paged_reserve", B, new_lens=new_lens, kv_lens=kv_lens)
@@ -349,13 +352,11 @@ def paged_truncate(lens: torch.Tensor, keep: torch.Tensor, block_table: torch.Te
     back on the stack.  ``lens_out`` may be ``lens``, ``free_count_out`` may be ``free_count``.  Returns ``(lens_out,
     free_count_out, status)``; unless ``status`` is 0 nothing changed (1: the stack has no room, as when a page is given
     back twice; 2, 8, 16 as for ``paged_reserve``)."""
-    B = lens.numel()
-    dev = _on_one_device("paged_truncate", lens, keep, block_table, free_pages, free_count, lens_out, free_count_out, status)
+    B, dev = lens.numel(), lens.get_device()
     lens_out = torch.empty_like(lens) if lens_out is None else lens_out
     free_count_out = torch.empty_like(free_count) if free_count_out is None else free_count_out
-    status = torch.empty(1, dtype=torch.int32, device=dev) if status is None else status
-    _int32("paged_truncate", lens=lens, keep=keep, block_table=block_table, free_pages=free_pages, free_count=free_count,
-           lens_out=lens_out, free_count_out=free_count_out, status=status)
+    status = torch.empty(1, dtype=_I32, device=lens.device) if status is None else status
+    _check("paged_truncate", dev, (lens, keep, block_table, free_pages, free_count, lens_out, free_count_out, status), _I32)
     if block_table.dim() != 2 or block_table.shape[0] != B:
         raise ValueError(f"paged_truncate: block_table {tuple(block_table.shape)} is not [{B}, max_blocks]")
     _sized("paged_truncate", B, keep=keep, lens_out=lens_out)
@@ -381,7 +382,9 @@ def paged_rope_append(qkv: torch.Tensor, q_start: torch.Tensor, slots: torch.Ten
     """``rope_append`` for a paged cache: q and k of each row (``qkv`` [T, (Hq + 2 Hkv) hd], float16 or float32) rotated
     at ``positions``, k and v written to ``slots`` of the pools, q to ``q_out`` [T, Hq hd] in the pools' type.  Rows from
     ``q_start[-1]`` on are left as they were; a slot outside the pool or a position past the tables is not written."""
-    dev = _on_one_device("paged_rope_append", qkv, q_start, slots, positions, cos_tab, sin_tab, q_out, k_pages, v_pages)
+    dev = qkv.get_device()
+    _check("paged_rope_append", dev, (qkv, cos_tab, sin_tab, q_out, k_pages, v_pages))
+    _check("paged_rope_append", dev, (q_start, slots, positions), _I32)
     n_pages, Hkv, page, hd = _pools("paged_rope_append", k_pages, v_pages)
     if qkv.dim() != 2 or qkv.dtype not in (_F16, _F32):
         raise ValueError(f"paged_rope_append: qkv must be a float16 or float32 [T, (Hq + 2 Hkv) hd], got {qkv.dtype} {tuple(qkv.shape)}")
@@ -395,7 +398,6 @@ def paged_rope_append(qkv: torch.Tensor, q_start: torch.Tensor, slots: torch.Ten
         raise ValueError(f"paged_rope_append: {slots.numel()} slots and {positions.numel()} positions for {T} rows")
     if cos_tab.dtype != _F32 or sin_tab.dtype != _F32 or cos_tab.dim() != 2 or cos_tab.shape[1] * 2 != hd or cos_tab.shape != sin_tab.shape:
         raise ValueError(f"paged_rope_append: cos_tab and sin_tab must be float32 [max_pos, {hd // 2}]")
-    _int32("paged_rope_append", q_start=q_start, slots=slots, positions=positions)
     if q_start.numel() < 1:
         raise ValueError("paged_rope_append: q_start is empty")
     if T:
@@ -405,10 +407,14 @@ def paged_rope_append(qkv: torch.Tensor, q_start: torch.Tensor, slots: torch.Ten
     return q_out
 
 
+@functools.lru_cache(maxsize=1024)
+def _prefix_attn_bytes(*args: int) -> int:
+    return int(L.load().sc_prefix_attn_workspace_bytes(*args))
+
+
 def prefix_attn_workspace_bytes(T: int, B: int, Hq: int, Hkv: int, hd: int, max_blocks: int, max_prefix_blocks: int,
                                 page_size: int, dtype: torch.dtype) -> int:
-    return int(L.load().sc_prefix_attn_workspace_bytes(T, B, Hq, Hkv, hd, max_blocks, max_prefix_blocks, page_size,
-                                                       L.SC_F16 if dtype == _F16 else L.SC_F32))
+    return _prefix_attn_bytes(T, B, Hq, Hkv, hd, max_blocks, max_prefix_blocks, page_size, L.SC_F16 if dtype == _F16 else L.SC_F32)
 
 
 def prefix_attn(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, q_start: torch.Tensor, kv_lens: torch.Tensor,
@@ -426,7 +432,12 @@ def prefix_attn(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, q
     T = q.shape[0] if q.dim() else 0
     if out is None:
         out = torch.zeros_like(q)
-    dev = _on_one_device("prefix_attn", q, k_pages, v_pages, q_start, kv_lens, block_table, prefix_table, prefix_len, out, workspace)
+    dev = q.get_device()
+    _check("prefix_attn", dev, (q, k_pages, v_pages, out))
+    ints = (q_start, kv_lens, block_table)
+    if prefix_len is not None and prefix_table is not None:
+        ints = (q_start, kv_lens, block_table, prefix_table, prefix_len)
+    _check("prefix_attn", dev, ints, _I32)
     B = kv_lens.numel()
     if q.dtype != k_pages.dtype or out.dtype != q.dtype or out.numel() != q.numel():
         raise ValueError(f"prefix_attn: q and out must have the pages' type {k_pages.dtype} and one size, got {q.dtype} "
@@ -434,7 +445,6 @@ def prefix_attn(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, q
     Hq = q.numel() // (T * hd) if T else Hkv
     if T and Hq * T * hd != q.numel():
         raise ValueError(f"prefix_attn: q rows of {q.numel() // T} are no multiple of head_dim {hd}")
-    _int32("prefix_attn", q_start=q_start, kv_lens=kv_lens, block_table=block_table, prefix_table=prefix_table, prefix_len=prefix_len)
     if block_table.dim() != 2 or block_table.shape[0] != B:
         raise ValueError(f"prefix_attn: block_table {tuple(block_table.shape)} is not [{B}, max_blocks]")
     _sized("prefix_attn", B + 1, q_start=q_start)
@@ -450,9 +460,11 @@ def prefix_attn(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, q
     nbytes = prefix_attn_workspace_bytes(T, B, Hq, Hkv, hd, block_table.shape[1], nbp, page, q.dtype)
     if workspace is None:
         if nbytes:
-            workspace = torch.empty(nbytes, dtype=torch.uint8, device=dev)
-    elif workspace.dtype != torch.uint8:
-        raise ValueError(f"prefix_attn: workspace must be uint8, got {workspace.dtype}")
+            workspace = torch.empty(nbytes, dtype=torch.uint8, device=q.device)
+    else:
+        _check("prefix_attn", dev, (workspace,))
+        if workspace.dtype != torch.uint8:
+            raise ValueError(f"prefix_attn: workspace must be uint8, got {workspace.dtype}")
     _call_on(dev, "sc_prefix_attn", q.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), _dt(q), T, q_start.data_ptr(),
              kv_lens.data_ptr(), block_table.data_ptr(), B, block_table.shape[1], _p(prefix_table), _p(prefix_len), nbp, Hq, Hkv,
              hd, n_pages, page, sc, out.data_ptr(), _p(workspace), workspace.numel() if workspace is not None else 0)
