@@ -13,7 +13,7 @@
 namespace sc {
 
 constexpr int PG_THREADS = 1024;
-constexpr int PG_BATCH = 4;  // rows or pages a thread has under way
+constexpr int PG_RUN = 4;        // consecutive rows or pages of a thread
 constexpr int PG_MAX_BATCH = 16384;  // a request's scan state is 12 bytes of shared memory: 192 KB
 
 __device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
@@ -46,14 +46,29 @@ __device__ __forceinline__ void block_scan2(long long& a, long long& b, long lon
     s_w[warp][1] = b;
   }
   __syncthreads();
-  long long pa = 0, pb = 0;
-  for (int w = 0; w < warp; ++w) {
-    pa += s_w[w][0];
-    pb += s_w[w][1];
+  long long pa = lane < warp ? s_w[lane][0] : 0, pb = lane < warp ? s_w[lane][1] : 0;
+#pragma unroll
+  for (int o = 16; o; o >>= 1) {
+    pa += __shfl_xor_sync(0xffffffffu, pa, o);
+    pb += __shfl_xor_sync(0xffffffffu, pb, o);
   }
   a += pa;
   b += pb;
   __syncthreads();
+}
+
+// x / d for 0 <= x < 2^31 by a product: m = floor(2^(31 + l) / d) + 1 with l = ceil(log2 d) is off by less than
+// 2^-(31 + l) relative to 1 / d, too little to reach the next whole number.
+struct PageDiv {
+  unsigned long long m;
+  int d, sh;
+  __device__ __forceinline__ int div(int x) const { return (int)(((unsigned long long)(unsigned)x * m) >> sh); }
+  __device__ __forceinline__ int up(int x) const { return x > 0 ? div(x - 1) + 1 : 0; }
+};
+static PageDiv page_div(int d) {
+  int l = 0;
+  while ((1ll << l) < d) ++l;
+  return {(1ull << (31 + l)) / (unsigned)d + 1, d, 31 + l};
 }
 
 // First index i in [0, n) with a[i] > x (a is non-decreasing, a[n - 1] > x).
@@ -72,14 +87,15 @@ __device__ __forceinline__ int first_above(const int* a, int n, int x) {
 struct ReserveParams {
   const int32_t *lens, *new_lens, *prefix_len, *free_pages, *free_count;
   int32_t *block_table, *kv_lens, *q_start, *slots, *positions, *free_out, *status;
-  int B, max_blocks, page, n_free, max_tokens;
+  int B, max_blocks, n_free, max_tokens;
+  PageDiv page;
 };
 
 // One cluster.  Every CTA scans all requests (new tokens, new pages) into its
 // own shared memory, so each knows every offset and the status without a
 // message; then the rows, the pages and the requests are spread over the
-// cluster's threads, a row or page finding its request by binary search in
-// shared memory.  The one cluster barrier separates the reads of lens and
+// cluster's threads, four consecutive rows or pages a thread, which finds the
+// first one's request by binary search in shared memory and walks on.  The one cluster barrier separates the reads of lens and
 // free_count from the writes of kv_lens and free_out, which may be the same
 // arrays.  Bound by latency: launch, one round trip for the lengths, one for
 // the pages.
@@ -96,9 +112,9 @@ __global__ void __launch_bounds__(PG_THREADS) paged_reserve_kernel(const Reserve
   if (threadIdx.x == 0) s_bad = 0;
   __syncthreads();
   const int count = *p.free_count;
-  const long long cap = (long long)p.max_blocks * p.page;
+  const long long cap = (long long)p.max_blocks * p.page.d;
   long long end0 = 0, take0 = 0;
-  for (int b0 = 0; b0 < p.B; b0 += PG_THREADS) {
+  for (int b0 = 0; b0 < p.B; b0 += blockDim.x) {
     const int b = b0 + threadIdx.x;
     long long a = 0, t = 0;
     if (b < p.B) {
@@ -110,7 +126,8 @@ __global__ void __launch_bounds__(PG_THREADS) paged_reserve_kernel(const Reserve
       if (bad) atomicOr(&s_bad, bad);
       if (!(bad & 8)) {
         a = add;
-        t = (kv + p.page - 1) / p.page - ((long long)len + p.page - 1) / p.page;
+        // past 32 bits only where it does not fit the table either
+        t = kv <= INT32_MAX ? p.page.up((int)kv) - p.page.up(len) : (kv - len) / p.page.d;
       }
       s_len[b] = len;
     }
@@ -121,7 +138,7 @@ __global__ void __launch_bounds__(PG_THREADS) paged_reserve_kernel(const Reserve
       s_end[b] = (int)min(a, (long long)INT32_MAX);
       s_take[b] = (int)min(t, (long long)INT32_MAX);
     }
-    if (threadIdx.x == PG_THREADS - 1) {
+    if (threadIdx.x == blockDim.x - 1) {
       s_tot[0] = a;
       s_tot[1] = t;
     }
@@ -136,40 +153,46 @@ __global__ void __launch_bounds__(PG_THREADS) paged_reserve_kernel(const Reserve
   if (end0 > p.max_tokens) st |= 4;
   if (count < 0 || count > p.n_free) st |= 16;
   cluster_arrive();
-  const int nthr = (int)cluster_size() * PG_THREADS, tid = (int)cluster_rank() * PG_THREADS + threadIdx.x;
+  const int nthr = (int)cluster_size() * blockDim.x, tid = (int)cluster_rank() * blockDim.x + threadIdx.x;
+  const bool wide = (((uintptr_t)p.slots | (uintptr_t)p.positions) & 15) == 0;
   if (st == 0) {
-    for (int n0 = tid; n0 < (int)take0; n0 += PG_BATCH * nthr) {
-      int id[PG_BATCH];
+    for (int n0 = tid * PG_RUN; n0 < (int)take0; n0 += PG_RUN * nthr) {
+      int b = first_above(s_take, p.B, n0);
 #pragma unroll
-      for (int i = 0; i < PG_BATCH; ++i) id[i] = n0 + i * nthr < (int)take0 ? p.free_pages[count - 1 - (n0 + i * nthr)] : 0;
-#pragma unroll
-      for (int i = 0; i < PG_BATCH; ++i) {
-        const int n = n0 + i * nthr;
+      for (int i = 0; i < PG_RUN; ++i) {
+        const int n = n0 + i;
         if (n >= (int)take0) break;
-        const int b = first_above(s_take, p.B, n);
-        const int j = (s_len[b] + p.page - 1) / p.page + n - (b ? s_take[b - 1] : 0);
-        p.block_table[(size_t)b * p.max_blocks + j] = id[i];
+        while (s_take[b] <= n) ++b;
+        const int j = p.page.up(s_len[b]) + n - (b ? s_take[b - 1] : 0);
+        p.block_table[(size_t)b * p.max_blocks + j] = p.free_pages[count - 1 - n];
       }
     }
-    for (int t0 = tid; t0 < (int)end0; t0 += PG_BATCH * nthr) {
-      int at[PG_BATCH], id[PG_BATCH];
+    for (int t0 = tid * PG_RUN; t0 < (int)end0; t0 += PG_RUN * nthr) {
+      int b = first_above(s_end, p.B, t0);
+      int at[PG_RUN], off[PG_RUN], id[PG_RUN];
 #pragma unroll
-      for (int i = 0; i < PG_BATCH; ++i) {
-        const int t = min(t0 + i * nthr, (int)end0 - 1);
-        const int b = first_above(s_end, p.B, t);
+      for (int i = 0; i < PG_RUN; ++i) {
+        const int t = min(t0 + i, (int)end0 - 1);
+        while (s_end[b] <= t) ++b;
         const int len = s_len[b];
         at[i] = len + t - (b ? s_end[b - 1] : 0);
-        const int j = at[i] / p.page, have = (len + p.page - 1) / p.page;
+        const int j = p.page.div(at[i]), have = p.page.up(len);
+        off[i] = at[i] - j * p.page.d;
         // a block of this step's is on the stack still, an older one in the table
         id[i] = j < have ? p.block_table[(size_t)b * p.max_blocks + j]
                          : p.free_pages[count - 1 - (b ? s_take[b - 1] : 0) - (j - have)];
       }
+      if (wide && t0 + PG_RUN <= (int)end0) {
+        *reinterpret_cast<int4*>(p.slots + t0) = make_int4(id[0] * p.page.d + off[0], id[1] * p.page.d + off[1],
+                                                           id[2] * p.page.d + off[2], id[3] * p.page.d + off[3]);
+        *reinterpret_cast<int4*>(p.positions + t0) = make_int4(prefix + at[0], prefix + at[1], prefix + at[2], prefix + at[3]);
+      } else {
 #pragma unroll
-      for (int i = 0; i < PG_BATCH; ++i) {
-        const int t = t0 + i * nthr;
-        if (t >= (int)end0) break;
-        p.slots[t] = id[i] * p.page + at[i] % p.page;
-        p.positions[t] = prefix + at[i];
+        for (int i = 0; i < PG_RUN; ++i) {
+          if (t0 + i >= (int)end0) break;
+          p.slots[t0 + i] = id[i] * p.page.d + off[i];
+          p.positions[t0 + i] = prefix + at[i];
+        }
       }
     }
   }
@@ -189,7 +212,8 @@ __global__ void __launch_bounds__(PG_THREADS) paged_reserve_kernel(const Reserve
 struct TruncateParams {
   const int32_t *lens, *keep, *block_table, *free_count;
   int32_t *free_pages, *lens_out, *free_out, *status;
-  int B, max_blocks, page, n_free;
+  int B, max_blocks, n_free;
+  PageDiv page;
 };
 
 // The same shape as the reservation: every CTA scans how many pages each
@@ -208,9 +232,9 @@ __global__ void __launch_bounds__(PG_THREADS) paged_truncate_kernel(const Trunca
   if (threadIdx.x == 0) s_bad = 0;
   __syncthreads();
   const int count = *p.free_count;
-  const long long cap = (long long)p.max_blocks * p.page;
+  const long long cap = (long long)p.max_blocks * p.page.d;
   long long give0 = 0;
-  for (int b0 = 0; b0 < p.B; b0 += PG_THREADS) {
+  for (int b0 = 0; b0 < p.B; b0 += blockDim.x) {
     const int b = b0 + threadIdx.x;
     long long g = 0, unused = 0;
     if (b < p.B) {
@@ -222,14 +246,14 @@ __global__ void __launch_bounds__(PG_THREADS) paged_truncate_kernel(const Trunca
       if (bad)
         atomicOr(&s_bad, bad);
       else
-        g = ((long long)len + p.page - 1) / p.page - ((long long)kp + p.page - 1) / p.page;
+        g = p.page.up(len) - p.page.up(kp);
       s_len[b] = len;
       s_keep[b] = kp;
     }
     block_scan2(g, unused, s_w);
     g += give0;
     if (b < p.B) s_give[b] = (int)min(g, (long long)INT32_MAX);
-    if (threadIdx.x == PG_THREADS - 1) s_tot = g;
+    if (threadIdx.x == blockDim.x - 1) s_tot = g;
     __syncthreads();
     give0 = s_tot;
     __syncthreads();
@@ -240,20 +264,19 @@ __global__ void __launch_bounds__(PG_THREADS) paged_truncate_kernel(const Trunca
   else if (count + give0 > p.n_free)
     st |= 1;
   cluster_arrive();
-  const int nthr = (int)cluster_size() * PG_THREADS, tid = (int)cluster_rank() * PG_THREADS + threadIdx.x;
+  const int nthr = (int)cluster_size() * blockDim.x, tid = (int)cluster_rank() * blockDim.x + threadIdx.x;
   if (st == 0) {
-    for (int n0 = tid; n0 < (int)give0; n0 += PG_BATCH * nthr) {
-      int id[PG_BATCH];
+    for (int n0 = tid * PG_RUN; n0 < (int)give0; n0 += PG_RUN * nthr) {
+      int b = first_above(s_give, p.B, n0), id[PG_RUN];
 #pragma unroll
-      for (int i = 0; i < PG_BATCH; ++i) {
-        const int n = min(n0 + i * nthr, (int)give0 - 1);
-        const int b = first_above(s_give, p.B, n);
-        const int j = (s_keep[b] + p.page - 1) / p.page + n - (b ? s_give[b - 1] : 0);
-        id[i] = p.block_table[(size_t)b * p.max_blocks + j];
+      for (int i = 0; i < PG_RUN; ++i) {
+        const int n = min(n0 + i, (int)give0 - 1);
+        while (s_give[b] <= n) ++b;
+        id[i] = p.block_table[(size_t)b * p.max_blocks + p.page.up(s_keep[b]) + n - (b ? s_give[b - 1] : 0)];
       }
 #pragma unroll
-      for (int i = 0; i < PG_BATCH; ++i)
-        if (n0 + i * nthr < (int)give0) p.free_pages[count + n0 + i * nthr] = id[i];
+      for (int i = 0; i < PG_RUN; ++i)
+        if (n0 + i < (int)give0) p.free_pages[count + n0 + i] = id[i];
     }
   }
   cluster_wait();
@@ -264,16 +287,19 @@ __global__ void __launch_bounds__(PG_THREADS) paged_truncate_kernel(const Trunca
   }
 }
 
-// Launches one cluster of `ctas` CTAs with programmatic stream serialisation.
+// Launches one cluster with programmatic stream serialisation, for `items` rows or pages at most: CTAs of up to 1024
+// threads, up to the portable 8.
 template <typename P>
-static int launch_cluster(void (*kern)(const P), int ctas, size_t smem, cudaStream_t stream, const P& p, const char* what) {
+static int launch_cluster(void (*kern)(const P), int items, size_t smem, cudaStream_t stream, const P& p, const char* what) {
   if (smem > (48u << 10)) {
     const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
     if (e != cudaSuccess) return check_launch(what, e);
   }
+  const long long threads = ((long long)items + PG_RUN - 1) / PG_RUN;
+  const int ctas = (int)std::max(1ll, std::min(8ll, (threads + PG_THREADS - 1) / PG_THREADS));
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(ctas);
-  cfg.blockDim = dim3(PG_THREADS);
+  cfg.blockDim = dim3((unsigned)std::max(128ll, std::min((long long)PG_THREADS, (std::max(threads, (long long)p.B) + 31) / 32 * 32)));
   cfg.dynamicSmemBytes = smem;
   cfg.stream = stream;
   cudaLaunchAttribute attr[2];
@@ -286,9 +312,6 @@ static int launch_cluster(void (*kern)(const P), int ctas, size_t smem, cudaStre
   cfg.numAttrs = pdl_enabled() ? 2 : 1;
   return check_launch(what, cudaLaunchKernelEx(&cfg, kern, p));
 }
-
-// CTAs of the cluster: one per batch of rows a CTA has under way, at most the portable 8.
-static int cluster_ctas(int rows) { return std::max(1, std::min(8, (rows + PG_THREADS * PG_BATCH - 1) / (PG_THREADS * PG_BATCH))); }
 
 // ---------------------------------------------------------------- append
 
@@ -318,10 +341,13 @@ struct AppendParams {
   const int32_t *rows_end, *slots, *positions;  // rows_end: one past the last row that is used
   const float *cos_tab, *sin_tab;
   void *q_out, *k_pages, *v_pages;
-  int rows, Hq, Hkv, hd, max_pos, n_pages, page;
+  int row0, items, Hq, Hkv, hd, max_pos, n_pages;
+  PageDiv page, per_row, per_head;  // items of a row, of a head
 };
 
-// A thread takes eight values of a row: four pairs (d, d + hd/2) of a q or k
+constexpr int AP_ITEMS = 2;  // of a thread
+
+// An item is eight values of a row: four pairs (d, d + hd/2) of a q or k
 // head, rotated, or eight values of a v head.  q, k and v are rounded once, to
 // the cache's type; the products of the rotation are not fused, as in
 // rope_append_kernel.  Moves its bytes once; bound by HBM for many rows, by
@@ -330,44 +356,65 @@ template <typename ST, typename CT>
 __global__ void __launch_bounds__(256) paged_append_kernel(const AppendParams p) {
   pdl_trigger();
   pdl_wait();
-  const int per_row = (p.Hq + 2 * p.Hkv) * (p.hd / 8);
-  const size_t it = (size_t)blockIdx.x * blockDim.x + threadIdx.x;
-  const int row = (int)(it / per_row), e = (int)(it % per_row);
-  if (row >= min(p.rows, *p.rows_end)) return;
-  const int per_head = p.hd / 8, half = p.hd / 2;
-  const int h = e / per_head, d = (e % per_head) * 4;
-  const ST* src = reinterpret_cast<const ST*>(p.qkv) + ((size_t)row * (p.Hq + 2 * p.Hkv) + h) * p.hd;
-  const int pos = p.positions[row], slot = p.slots[row];
-  const bool pos_ok = pos >= 0 && pos < p.max_pos;
-  const bool ok = pos_ok && slot >= 0 && slot / p.page < p.n_pages;
-  const int id = slot / p.page, off = slot % p.page;
-  float a[4], b[4];
-  if (h >= p.Hq + p.Hkv) {
-    if (!ok) return;
-    ld4<ST>(src + 2 * d, a);
-    ld4<ST>(src + 2 * d + 4, b);
-    CT* dst = reinterpret_cast<CT*>(p.v_pages) + (((size_t)id * p.Hkv + (h - p.Hq - p.Hkv)) * p.page + off) * p.hd;
-    st4(dst + 2 * d, a);
-    st4(dst + 2 * d + 4, b);
-    return;
-  }
-  if (h >= p.Hq && !ok) return;
-  ld4<ST>(src + d, a);
-  ld4<ST>(src + d + half, b);
-  float c[4] = {1.f, 1.f, 1.f, 1.f}, s[4] = {0.f, 0.f, 0.f, 0.f}, x[4], y[4];
-  if (pos_ok) {
-    ld4<float>(p.cos_tab + (size_t)pos * half + d, c);
-    ld4<float>(p.sin_tab + (size_t)pos * half + d, s);
+  const int end = *p.rows_end;
+  const int half = p.hd / 2;
+  int row[AP_ITEMS], h[AP_ITEMS], d[AP_ITEMS], pos[AP_ITEMS], slot[AP_ITEMS];
+  bool live[AP_ITEMS];
+  float a[AP_ITEMS][4], b[AP_ITEMS][4], c[AP_ITEMS][4], s[AP_ITEMS][4];
+#pragma unroll
+  for (int i = 0; i < AP_ITEMS; ++i) {
+    const int it = (blockIdx.x * AP_ITEMS + i) * 256 + threadIdx.x;
+    live[i] = it < p.items;
+    const int r = live[i] ? p.per_row.div(it) : 0, e = it - r * p.per_row.d;
+    row[i] = p.row0 + r;
+    live[i] = live[i] && row[i] < end;
+    h[i] = live[i] ? p.per_head.div(e) : 0;
+    d[i] = (e - h[i] * p.per_head.d) * 4;
+    pos[i] = slot[i] = -1;
+    if (live[i]) {
+      pos[i] = p.positions[row[i]];
+      slot[i] = p.slots[row[i]];
+      const ST* src = reinterpret_cast<const ST*>(p.qkv) + ((size_t)row[i] * (p.Hq + 2 * p.Hkv) + h[i]) * p.hd;
+      const bool v = h[i] >= p.Hq + p.Hkv;  // a v head: eight values in a row, from 2 d
+      ld4<ST>(src + (v ? 2 * d[i] : d[i]), a[i]);
+      ld4<ST>(src + (v ? 2 * d[i] + 4 : d[i] + half), b[i]);
+    }
   }
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    x[i] = __fadd_rn(__fmul_rn(a[i], c[i]), __fmul_rn(-b[i], s[i]));
-    y[i] = __fadd_rn(__fmul_rn(b[i], c[i]), __fmul_rn(a[i], s[i]));
+  for (int i = 0; i < AP_ITEMS; ++i) {
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      c[i][k] = 1.f;
+      s[i][k] = 0.f;
+    }
+    if (live[i] && h[i] < p.Hq + p.Hkv && pos[i] >= 0 && pos[i] < p.max_pos) {
+      ld4<float>(p.cos_tab + (size_t)pos[i] * half + d[i], c[i]);
+      ld4<float>(p.sin_tab + (size_t)pos[i] * half + d[i], s[i]);
+    }
   }
-  CT* dst = h < p.Hq ? reinterpret_cast<CT*>(p.q_out) + ((size_t)row * p.Hq + h) * p.hd
-                     : reinterpret_cast<CT*>(p.k_pages) + (((size_t)id * p.Hkv + (h - p.Hq)) * p.page + off) * p.hd;
-  st4(dst + d, x);
-  st4(dst + d + half, y);
+#pragma unroll
+  for (int i = 0; i < AP_ITEMS; ++i) {
+    if (!live[i]) continue;
+    const int id = slot[i] >= 0 ? p.page.div(slot[i]) : p.n_pages, off = slot[i] - id * p.page.d;
+    const bool ok = pos[i] >= 0 && pos[i] < p.max_pos && id < p.n_pages;
+    if (h[i] >= p.Hq && !ok) continue;
+    if (h[i] >= p.Hq + p.Hkv) {
+      CT* dst = reinterpret_cast<CT*>(p.v_pages) + (((size_t)id * p.Hkv + (h[i] - p.Hq - p.Hkv)) * p.page.d + off) * p.hd;
+      st4(dst + 2 * d[i], a[i]);
+      st4(dst + 2 * d[i] + 4, b[i]);
+      continue;
+    }
+    float x[4], y[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      x[k] = __fadd_rn(__fmul_rn(a[i][k], c[i][k]), __fmul_rn(-b[i][k], s[i][k]));
+      y[k] = __fadd_rn(__fmul_rn(b[i][k], c[i][k]), __fmul_rn(a[i][k], s[i][k]));
+    }
+    CT* dst = h[i] < p.Hq ? reinterpret_cast<CT*>(p.q_out) + ((size_t)row[i] * p.Hq + h[i]) * p.hd
+                          : reinterpret_cast<CT*>(p.k_pages) + (((size_t)id * p.Hkv + (h[i] - p.Hq)) * p.page.d + off) * p.hd;
+    st4(dst + d[i], x);
+    st4(dst + d[i] + half, y);
+  }
 }
 
 }  // namespace sc
@@ -388,8 +435,8 @@ int sc_paged_reserve(const int32_t* lens, const int32_t* new_lens, int B, const 
   SC_REQUIRE(page_size >= 1 && (long long)n_free * page_size <= INT32_MAX && (long long)max_blocks * page_size <= INT32_MAX,
              SC_ERR_SHAPE, "paged_reserve: slots past 32 bits (%d pages of %d, %d blocks)", n_free, page_size, max_blocks);
   const ReserveParams p = {lens,        new_lens, prefix_len, free_pages, free_count, block_table, kv_lens, q_start, slots,
-                           positions,   free_count_out, status, B, max_blocks, page_size, n_free, max_tokens};
-  return launch_cluster(paged_reserve_kernel, cluster_ctas(std::max(max_tokens, B)), (size_t)B * 12, stream, p, "paged_reserve");
+                           positions,   free_count_out, status, B, max_blocks, n_free, max_tokens, page_div(page_size)};
+  return launch_cluster(paged_reserve_kernel, max_tokens, (size_t)B * 12, stream, p, "paged_reserve");
 }
 
 int sc_paged_truncate(const int32_t* lens, const int32_t* keep, int B, const int32_t* block_table, int max_blocks,
@@ -403,8 +450,8 @@ int sc_paged_truncate(const int32_t* lens, const int32_t* keep, int B, const int
   SC_REQUIRE(page_size >= 1 && (long long)n_free * page_size <= INT32_MAX && (long long)max_blocks * page_size <= INT32_MAX,
              SC_ERR_SHAPE, "paged_truncate: slots past 32 bits (%d pages of %d, %d blocks)", n_free, page_size, max_blocks);
   const TruncateParams p = {lens, keep, block_table, free_count, free_pages, lens_out, free_count_out, status, B,
-                            max_blocks, page_size, n_free};
-  return launch_cluster(paged_truncate_kernel, cluster_ctas(std::min(n_free, 16 * B)), (size_t)B * 12, stream, p,
+                            max_blocks, n_free, page_div(page_size)};
+  return launch_cluster(paged_truncate_kernel, std::min(n_free, 16 * B), (size_t)B * 12, stream, p,
                         "paged_truncate");
 }
 
@@ -424,14 +471,20 @@ int sc_paged_rope_append(const void* qkv, int qkv_dtype, int rows, const int32_t
   SC_REQUIRE((((uintptr_t)qkv | (uintptr_t)q_out | (uintptr_t)k_pages | (uintptr_t)v_pages | (uintptr_t)cos_tab |
                (uintptr_t)sin_tab) & 15) == 0,
              SC_ERR_ARG, "paged_rope_append: tensors must start on 16-byte boundaries");
-  const size_t blocks = ((size_t)rows * (Hq + 2 * Hkv) * (hd / 8) + 255) / 256;
-  SC_REQUIRE(blocks <= INT32_MAX, SC_ERR_SHAPE, "paged_rope_append: %d rows are too many for one launch", rows);
-  const AppendParams p = {qkv, rows_end, slots, positions, cos_tab, sin_tab, q_out, k_pages, v_pages,
-                          rows, Hq, Hkv, hd, max_pos, n_pages, page_size};
-  auto kern = qkv_dtype == SC_F32 ? (cache_dtype == SC_F32 ? paged_append_kernel<float, float> : paged_append_kernel<float, __half>)
-                                  : (cache_dtype == SC_F32 ? paged_append_kernel<__half, float> : paged_append_kernel<__half, __half>);
-  ::sc::launch(kern, dim3((unsigned)blocks), dim3(256), 0, stream, p);
-  return check_launch("paged_rope_append");
+  SC_REQUIRE(((long long)Hq + 2 * Hkv) * (hd / 8) <= (1 << 24), SC_ERR_SHAPE, "paged_rope_append: rows of %d heads are too wide", Hq + 2 * Hkv);
+  const int per_row = (Hq + 2 * Hkv) * (hd / 8), most = (1 << 30) / per_row;  // rows of a launch: items stay below 2^30
+  for (int row0 = 0; row0 < rows; row0 += std::min(most, rows - row0)) {
+    const int n = std::min(most, rows - row0);
+    const AppendParams p = {qkv,   rows_end,    slots, positions, cos_tab, sin_tab, q_out,   k_pages,
+                            v_pages, row0, n * per_row, Hq,    Hkv,       hd,      max_pos, n_pages, page_div(page_size),
+                            page_div(per_row), page_div(hd / 8)};
+    auto kern = qkv_dtype == SC_F32 ? (cache_dtype == SC_F32 ? paged_append_kernel<float, float> : paged_append_kernel<float, __half>)
+                                    : (cache_dtype == SC_F32 ? paged_append_kernel<__half, float> : paged_append_kernel<__half, __half>);
+    ::sc::launch(kern, dim3((unsigned)((p.items + 256 * AP_ITEMS - 1) / (256 * AP_ITEMS))), dim3(256), 0, stream, p);
+    const int st = check_launch("paged_rope_append");
+    if (st != SC_OK) return st;
+  }
+  return SC_OK;
 }
 
 }  // extern "C"

@@ -58,7 +58,7 @@ def append(**kw):
 
 @pytest.mark.parametrize("kw,code", [(dict(rows=0), L.SC_ERR_SHAPE), (dict(hq=0), L.SC_ERR_SHAPE), (dict(hd=12), L.SC_ERR_SHAPE),
                                      (dict(hd=0), L.SC_ERR_SHAPE), (dict(max_pos=0), L.SC_ERR_SHAPE), (dict(pages=I31), L.SC_ERR_SHAPE),
-                                     (dict(rows=I31, hq=4096), L.SC_ERR_SHAPE), (dict(dt=L.SC_I32), L.SC_ERR_ARG), (dict(cdt=L.SC_U8), L.SC_ERR_ARG),
+                                     (dict(hq=1 << 22), L.SC_ERR_SHAPE), (dict(dt=L.SC_I32), L.SC_ERR_ARG), (dict(cdt=L.SC_U8), L.SC_ERR_ARG),
                                      (dict(qkv=A + 4), L.SC_ERR_ARG), (dict(k=A + 8), L.SC_ERR_ARG), (dict(cos=A + 4), L.SC_ERR_ARG),
                                      (dict(v=None), L.SC_ERR_ARG), (dict(end=None), L.SC_ERR_ARG), (dict(pos=None), L.SC_ERR_ARG)])
 def test_append_refuses(kw, code):
