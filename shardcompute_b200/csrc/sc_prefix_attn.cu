@@ -1019,27 +1019,32 @@ many_rows_kernel(const PrefixAttnParams p, const __grid_constant__ PoolMaps maps
 // size down to 2^-24 -- and each product of two operands is three fp16
 // products in two fp32 accumulators, hi.hi and hi.lo + lo.hi, joined as the
 // first plus 2^-11 of the second.  The parts' range is fp16's: a value beyond
-// 65504 gives NaN.  One tile of 128 rows, tiles of 64 keys:
+// 65504 gives NaN.  The parts of K and of V lie side by side, so that hi.hi
+// and hi.lo are one product of twice the width.  One tile of 128 rows, tiles of
+// 64 keys:
 //   warp 0       TMA producer: raw fp32 K and V tiles through a ring
 //   warp 1       MMA issuer; S of the next tile goes ahead of O += P V of this one
-//   warps 4-7    softmax, a thread per row (P's own two parts over S's columns)
-//   warps 8-15   split a raw tile into its two fp16 tiles; V's slots behind the
-//                last key, which may hold anything, become zero
+//   warps 4-11   softmax, two threads per row with half the tile's keys each,
+//                which tell each other the maxima they find (P's own two parts
+//                over S's columns)
+//   warps 12-19  split Q, then each raw tile, into the fp16 parts; V's slots
+//                behind the last key, which may hold anything, become zero
 // TMEM: two buffers of S (hi.hi | cross, 64 columns each), O (hi.hi | cross).
 constexpr int TF_N = 64;              // keys of a tile
 constexpr int TF_BOX = 16;            // keys of a copy
-constexpr int TF_THREADS = 16 * 32;
+constexpr int TF_THREADS = 20 * 32;
 constexpr int TF_CONV = 8;            // warps that split
 
 template <int HD>
 struct ManyRowsF32 {
   static constexpr int NCH = HD / 64;               // 64-wide fp16 columns
   static constexpr int QT = TC_M * HD * 2;          // bytes of one part of Q
-  static constexpr int PT = TF_N * HD * 2;          // bytes of one part of a K or V tile
+  static constexpr int CH = TF_N * 128;             // bytes of a 64-wide column of one part of a tile
+  static constexpr int PT = NCH * CH;               // bytes of one part of a K or V tile
   static constexpr int RAW = TF_N * HD * 4;         // bytes of a raw tile
-  static constexpr int BOX = TF_BOX * HD * 4;        // bytes of one copy: 16 keys
+  static constexpr int BOX = TF_BOX * HD * 4;       // bytes of one copy
   static constexpr int NRAW = HD == 128 ? 3 : 6;
-  static constexpr int SMEM = 2 * QT + 4 * PT + NRAW * RAW + 1024;
+  static constexpr int SMEM = 2 * QT + 4 * PT + NRAW * RAW;  // to the last byte of 227 KB with the static part
 };
 
 // two fp32 -> their fp16 parts, packed
@@ -1049,32 +1054,47 @@ __device__ __forceinline__ void split_f16(float x, float y, uint32_t& hi, uint32
   hi = h2_as_u32(h);
   lo = h2_as_u32(__floats2half2_rn((x - f.x) * 2048.f, (y - f.y) * 2048.f));
 }
+// eight fp32 -> 16 bytes of each part, at shared addresses h and l
+__device__ __forceinline__ void split_f16x8(const float4& a, const float4& b, uint32_t h, uint32_t l) {
+  uint32_t hi[4], lo[4];
+  split_f16(a.x, a.y, hi[0], lo[0]);
+  split_f16(a.z, a.w, hi[1], lo[1]);
+  split_f16(b.x, b.y, hi[2], lo[2]);
+  split_f16(b.z, b.w, hi[3], lo[3]);
+  asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(h), "r"(hi[0]), "r"(hi[1]), "r"(hi[2]), "r"(hi[3]) : "memory");
+  asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(l), "r"(lo[0]), "r"(lo[1]), "r"(lo[2]), "r"(lo[3]) : "memory");
+}
 
 template <int HD, bool PACKED>
 __global__ void __launch_bounds__(TF_THREADS, 1)
 many_rows_f32_kernel(const PrefixAttnParams p, const __grid_constant__ PoolMaps maps, int splits, int slot0) {
   using C = ManyRowsF32<HD>;
-  constexpr int NRAW = C::NRAW;
+  constexpr int NRAW = C::NRAW, CH = C::CH;
   extern __shared__ __align__(1024) unsigned char mf_smem[];
-  __shared__ __align__(8) uint64_t raw_full[NRAW], raw_empty[NRAW], q_full, k_full, v_full, s_full[2], p_full[2], pv_done, o_full, drained;
+  __shared__ __align__(8) uint64_t raw_full[NRAW], raw_empty[NRAW], q_full, k_full, v_full, s_full[2], p_full[2], max_full[4], pv_done, o_full, drained;
   __shared__ uint32_t s_tmem, s_absent[16];
   __shared__ int s_abort, s_req, s_row0, s_sum[TF_THREADS / 32];
-  unsigned char* base = mf_smem + ((1024 - (smem_u32(mf_smem) & 1023)) & 1023);
-  const uint32_t q_u = smem_u32(base), k_u = q_u + 2 * C::QT, v_u = k_u + 2 * C::PT, raw_u = v_u + 2 * C::PT;
+  __shared__ float s_max[2][2][TC_M];  // by tile's parity, by half
+  const uint32_t q_u = smem_u32(mf_smem), k_u = q_u + 2 * C::QT, v_u = k_u + 2 * C::PT, raw_u = v_u + 2 * C::PT;
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   const int split = blockIdx.x % splits, item = blockIdx.x / splits, h = blockIdx.y;
+  if (q_u & 1023) {  // the tiles' swizzle counts on the declared alignment
+    if (threadIdx.x == 0) atomicExch(&g_prefix_attn_error, 1);
+    return;
+  }
   if (threadIdx.x == 0) {
     for (int i = 0; i < NRAW; ++i) {
       mbar_init(&raw_full[i], 1);
       mbar_init(&raw_empty[i], TF_CONV);
     }
-    mbar_init(&q_full, 4);
+    mbar_init(&q_full, TF_CONV);
     mbar_init(&k_full, TF_CONV);
     mbar_init(&v_full, TF_CONV);
     mbar_init(&s_full[0], 1);
     mbar_init(&s_full[1], 1);
-    mbar_init(&p_full[0], 4);  // by buffer of S: P of the next tile may be there before this one's is taken
-    mbar_init(&p_full[1], 4);
+    mbar_init(&p_full[0], 8);  // by buffer of S: P of the next tile may be there before this one's is taken
+    mbar_init(&p_full[1], 8);
+    for (int i = 0; i < 4; ++i) mbar_init(&max_full[i], 2);  // the two warps of 32 rows
     mbar_init(&pv_done, 1);
     mbar_init(&o_full, 1);
     mbar_init(&drained, 1);
@@ -1100,8 +1120,7 @@ many_rows_f32_kernel(const PrefixAttnParams p, const __grid_constant__ PoolMaps 
 
   if (warp == 0) {
     // ================================ TMA producer ================================
-    int row[2] = {-1, -1};  // pool rows of the tile whose K goes next and of the one before, one per copy
-    auto rows_of = [&](int i) {
+    auto rows_of = [&](int i) {  // the pool rows of tile i, one per copy
       const int t = w.t_lo + i;
       int at = -1;
       if (lane < TF_N / TF_BOX && lane * TF_BOX < keys_of(t)) {
@@ -1123,12 +1142,14 @@ many_rows_f32_kernel(const PrefixAttnParams p, const __grid_constant__ PoolMaps 
     };
     uint32_t it = 0;
     bool ok = true;
+    int row = -1, before = -1;
     for (int i = 0; i <= cnt && ok && cnt; ++i) {  // K of tile i, then V of tile i - 1
+      before = row;
       if (i < cnt) {
-        row[i & 1] = rows_of(i);
-        if ((ok = copy(&maps.k, i & 1 ? row[1] : row[0], it))) ++it;
+        row = rows_of(i);
+        if ((ok = copy(&maps.k, row, it))) ++it;
       }
-      if (i > 0 && ok && (ok = copy(&maps.v, i & 1 ? row[0] : row[1], it))) ++it;
+      if (i > 0 && ok && (ok = copy(&maps.v, before, it))) ++it;
     }
     if (lane == 0) {  // copies in flight land before the CTA may exit
       int ignore = 0;
@@ -1137,20 +1158,20 @@ many_rows_f32_kernel(const PrefixAttnParams p, const __grid_constant__ PoolMaps 
   } else if (warp == 1) {
     // ================================ MMA issuer ================================
     if (lane == 0 && cnt > 0) {
-      constexpr uint32_t idesc_s = (1u << 4) | ((TF_N >> 3) << 17) | ((TC_M >> 4) << 24);
-      constexpr uint32_t idesc_o = (1u << 4) | (1u << 16) | ((HD >> 3) << 17) | ((TC_M >> 4) << 24);
-      const uint64_t qh = umma_desc_sw128(q_u), ql = umma_desc_sw128(q_u + C::QT);
-      const uint64_t kh = umma_desc_sw128(k_u), kl = umma_desc_sw128(k_u + C::PT);
-      const uint64_t vh = umma_desc_sw128_mn(v_u, TF_N * 128), vl = umma_desc_sw128_mn(v_u + C::PT, TF_N * 128);
+      constexpr uint32_t mn = (1u << 4) | ((TC_M >> 4) << 24);
+      constexpr uint32_t idesc_s2 = mn | ((2 * TF_N >> 3) << 17), idesc_s = mn | ((TF_N >> 3) << 17);
+      constexpr uint32_t idesc_o2 = mn | (1u << 16) | ((2 * HD >> 3) << 17), idesc_o = mn | (1u << 16) | ((HD >> 3) << 17);
+      const uint64_t qh = umma_desc_sw128(q_u), ql = umma_desc_sw128(q_u + C::QT), kd = umma_desc_sw128(k_u);
+      const uint64_t vd = umma_desc_sw128_mn(v_u, CH);
       const uint32_t to = tmem + 256;
       auto issue_s = [&](int i) {
         const uint32_t ts = tmem + (i & 1) * 128;
 #pragma unroll
         for (int kk = 0; kk < HD / 16; ++kk) {
-          const uint32_t qo = ((kk >> 2) * (TC_M * 128) + (kk & 3) * 32) >> 4, ko = ((kk >> 2) * (TF_N * 128) + (kk & 3) * 32) >> 4;
-          umma_f16(ts + 64, ql + qo, kh + ko, idesc_s, kk != 0);
-          umma_f16(ts + 64, qh + qo, kl + ko, idesc_s, 1u);
-          umma_f16(ts, qh + qo, kh + ko, idesc_s, kk != 0);
+          // K: 64-wide column, in it the 64 rows of hi, then those of lo
+          const uint32_t qo = ((kk >> 2) * (TC_M * 128) + (kk & 3) * 32) >> 4, ko = ((kk >> 2) * 2 * CH + (kk & 3) * 32) >> 4;
+          umma_f16(ts, qh + qo, kd + ko, idesc_s2, kk != 0);
+          umma_f16(ts + 64, ql + qo, kd + ko, idesc_s, 1u);
         }
         tc_commit(&s_full[i & 1]);
       };
@@ -1171,68 +1192,92 @@ many_rows_f32_kernel(const PrefixAttnParams p, const __grid_constant__ PoolMaps 
         const uint32_t ph = tmem + (i & 1) * 128, pl = ph + 64;
 #pragma unroll
         for (int kk = 0; kk < TF_N / 16; ++kk) {
-          umma_f16_ta(to + HD, pl + kk * 8, vh + kk * (2048 >> 4), idesc_o, (i | kk) != 0);
-          umma_f16_ta(to + HD, ph + kk * 8, vl + kk * (2048 >> 4), idesc_o, 1u);
-          umma_f16_ta(to, ph + kk * 8, vh + kk * (2048 >> 4), idesc_o, (i | kk) != 0);
+          umma_f16_ta(to, ph + kk * 8, vd + kk * (2048 >> 4), idesc_o2, (i | kk) != 0);
+          umma_f16_ta(to + HD, pl + kk * 8, vd + kk * (2048 >> 4), idesc_o, 1u);
         }
         tc_commit(&pv_done);
         if (i + 1 == cnt) tc_commit(&o_full);
       }
     }
-  } else if (warp >= 8) {
-    // ================================ split K and V ================================
+  } else if (warp >= 12) {
+    // ================================ split Q, K and V ================================
     constexpr int LPK = HD / 8, KPW = 32 / LPK;  // lanes per key (8 values each), keys per warp and step
-    const int g = lane % LPK, sub = lane / LPK;
-    auto convert = [&](uint32_t it, uint32_t dst, int keys) {  // slots from `keys` on become zero
+    constexpr int STEPS = TF_N / (TF_CONV * KPW);
+    const int cw = warp - 12, g = lane % LPK, sub = lane / LPK;
+    const bool odd = (g >> 2) & 1;
+    auto convert = [&](uint32_t it, bool is_v, int keys) {  // slots from `keys` on become zero
       const int s = it % NRAW;
       if (!__all_sync(0xffffffffu, pa_wait(&raw_full[s], (it / NRAW) & 1u, abort))) return false;
       const uint32_t src = raw_u + s * C::RAW;
-#pragma unroll 4
-      for (int k0 = 0; k0 < TF_N; k0 += TF_CONV * KPW) {
-        const int key = k0 + (warp - 8) * KPW + sub, r = key % TF_BOX;
+      float4 a[STEPS], b[STEPS];
+#pragma unroll
+      for (int j = 0; j < STEPS; ++j) {
+        const int key = (j * TF_CONV + cw) * KPW + sub, r = key % TF_BOX;
         // 8 values: pieces 2 (g % 4) and 2 (g % 4) + 1 of 128-byte chunk g / 4; odd chunks in the other order, so that
-        // eight lanes read eight banks' worth
+        // eight lanes read all the banks
         const uint32_t at = src + (key / TF_BOX) * C::BOX + (g >> 2) * (TF_BOX * 128) + r * 128;
-        const int p0 = 2 * (g & 3) + ((g >> 2) & 1);
-        float4 a = lds_f4(at + ((p0 ^ (r & 7)) << 4)), b = lds_f4(at + (((p0 ^ 1) ^ (r & 7)) << 4));
-        if ((g >> 2) & 1) {
-          const float4 x = a;
-          a = b;
-          b = x;
-        }
-        if (key >= keys) a = b = make_float4(0.f, 0.f, 0.f, 0.f);
-        uint32_t hi[4], lo[4];
-        split_f16(a.x, a.y, hi[0], lo[0]);
-        split_f16(a.z, a.w, hi[1], lo[1]);
-        split_f16(b.x, b.y, hi[2], lo[2]);
-        split_f16(b.z, b.w, hi[3], lo[3]);
-        const uint32_t d = dst + (g >> 3) * (TF_N * 128) + sw128(key, g & 7);
-        asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(d), "r"(hi[0]), "r"(hi[1]), "r"(hi[2]), "r"(hi[3]) : "memory");
-        asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(d + C::PT), "r"(lo[0]), "r"(lo[1]), "r"(lo[2]), "r"(lo[3]) : "memory");
+        const int p0 = 2 * (g & 3) + odd;
+        a[j] = lds_f4(at + ((p0 ^ (r & 7)) << 4));
+        b[j] = lds_f4(at + (((p0 ^ 1) ^ (r & 7)) << 4));
+      }
+#pragma unroll
+      for (int j = 0; j < STEPS; ++j) {
+        const int key = (j * TF_CONV + cw) * KPW + sub;
+        if (key >= keys) a[j] = b[j] = make_float4(0.f, 0.f, 0.f, 0.f);
+        const uint32_t c = sw128(key, g & 7);
+        const uint32_t d = is_v ? v_u + (g >> 3) * CH + c : k_u + (g >> 3) * 2 * CH + c;
+        split_f16x8(odd ? b[j] : a[j], odd ? a[j] : b[j], d, d + (is_v ? C::PT : CH));
       }
       fence_async_smem();
       __syncwarp();
       if (lane == 0) mbar_arrive(&raw_empty[s]);
       return true;
     };
+    if (cnt > 0) {
+      constexpr int QS = TC_M / (TF_CONV * KPW);  // this warp's share of Q's rows
+#pragma unroll
+      for (int j0 = 0; j0 < QS; j0 += 4) {
+        float4 a[4], b[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const int gr = w.r0 + ((j0 + j) * TF_CONV + cw) * KPW + sub;
+          a[j] = b[j] = make_float4(0.f, 0.f, 0.f, 0.f);
+          if (gr < w.rows) {
+            const float4* src = reinterpret_cast<const float4*>(reinterpret_cast<const float*>(p.q) +
+                                                                ((size_t)(w.row_lo + gr / p.G) * p.Hq + h * p.G + gr % p.G) * HD + g * 8);
+            a[j] = src[0];
+            b[j] = src[1];
+          }
+        }
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const uint32_t d = q_u + (g >> 3) * (TC_M * 128) + sw128(((j0 + j) * TF_CONV + cw) * KPW + sub, g & 7);
+          split_f16x8(a[j], b[j], d, d + C::QT);
+        }
+      }
+      fence_async_smem();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&q_full);
+    }
     bool ok = true;
     for (int i = 0; i <= cnt && ok && cnt; ++i) {
       if (i < cnt) {  // K of tile i, once S of tile i - 1 is done with the buffer
         if (i > 0) ok = __all_sync(0xffffffffu, pa_wait(&s_full[(i - 1) & 1], ((i - 1) >> 1) & 1, abort));
-        ok = ok && convert(k_at(i), k_u, TF_N);
+        ok = ok && convert(k_at(i), false, TF_N);
         if (ok && lane == 0) mbar_arrive(&k_full);
       }
       if (i > 0 && ok) {  // V of tile i - 1, once the product of tile i - 2 is
         if (i > 1) ok = __all_sync(0xffffffffu, pa_wait(&pv_done, (i - 2) & 1, abort));
-        ok = ok && convert(v_at(i - 1), v_u, keys_of(w.t_lo + i - 1));
+        ok = ok && convert(v_at(i - 1), true, keys_of(w.t_lo + i - 1));
         if (ok && lane == 0) mbar_arrive(&v_full);
       }
     }
   } else if (warp >= 4) {
     // ================================ softmax ================================
+    const int half = (warp - 4) >> 2;  // keys 32 half .. 32 half + 31 of every tile; columns HD / 2 of both parts of O
     const int lanes = (warp & 3) * 32;
     const int r = w.r0 + lanes + lane;  // this thread's row
-    const uint32_t tl = tmem + ((uint32_t)lanes << 16), ot = tl + 256;
+    const uint32_t tl = tmem + ((uint32_t)lanes << 16), ot = tl + 256 + half * (HD / 2);
     const bool valid = w.work && r < w.rows;
     const int see = PACKED ? 0 : (valid ? max(0, min(w.len, w.len - w.n + r / p.G + 1)) : w.own);
     const float c = p.c;
@@ -1240,72 +1285,44 @@ many_rows_f32_kernel(const PrefixAttnParams p, const __grid_constant__ PoolMaps 
     const size_t row = valid ? (size_t)(w.row_lo + r / p.G) * p.Hq + h * p.G + r % p.G : 0;
     const size_t at = (size_t)(slot0 + split) * p.T * p.Hq + row;
     if (cnt > 0) {
-      // ---- Q's parts: this warp's 32 rows, 8 values a lane
-      constexpr int LPR = HD / 8;
-#pragma unroll
-      for (int e0 = 0; e0 < LPR; e0 += 4) {
-        float4 x[4][2];
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const int rr = lanes + ((e0 + j) * 32 + lane) / LPR, pc = ((e0 + j) * 32 + lane) % LPR, gr = w.r0 + rr;
-          x[j][0] = x[j][1] = make_float4(0.f, 0.f, 0.f, 0.f);
-          if (gr < w.rows) {
-            const float4* src = reinterpret_cast<const float4*>(reinterpret_cast<const float*>(p.q) +
-                                                                ((size_t)(w.row_lo + gr / p.G) * p.Hq + h * p.G + gr % p.G) * HD + pc * 8);
-            x[j][0] = src[0];
-            x[j][1] = src[1];
-          }
-        }
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const int rr = lanes + ((e0 + j) * 32 + lane) / LPR, pc = ((e0 + j) * 32 + lane) % LPR;
-          uint32_t hi[4], lo[4];
-          split_f16(x[j][0].x, x[j][0].y, hi[0], lo[0]);
-          split_f16(x[j][0].z, x[j][0].w, hi[1], lo[1]);
-          split_f16(x[j][1].x, x[j][1].y, hi[2], lo[2]);
-          split_f16(x[j][1].z, x[j][1].w, hi[3], lo[3]);
-          const uint32_t d = q_u + (pc >> 3) * (TC_M * 128) + sw128(rr, pc & 7);
-          asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(d), "r"(hi[0]), "r"(hi[1]), "r"(hi[2]), "r"(hi[3]) : "memory");
-          asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(d + C::QT), "r"(lo[0]), "r"(lo[1]), "r"(lo[2]), "r"(lo[3]) : "memory");
-        }
-      }
-      fence_async_smem();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&q_full);
-
       bool ok = true;
       for (int i = 0; i < cnt; ++i) {
         ok = __all_sync(0xffffffffu, pa_wait(&s_full[i & 1], (i >> 1) & 1, abort));
         if (!ok) break;
         tc_fence_after();
-        const uint32_t st = tl + (i & 1) * 128;
+        const uint32_t st = tl + (i & 1) * 128 + half * 32;
         const int t = w.t_lo + i;
-        const uint32_t gone = s_absent[i & 15];
-        const int lim = (t < np ? w.P : see) - (t < np ? t : t - np) * TF_N;  // keys of the tile this row sees
-        float v[TF_N];
+        const uint32_t gone = s_absent[i & 15] >> (half * 2);
+        // of this thread's keys, those that its row sees
+        const int lim = (t < np ? w.P : see) - (t < np ? t : t - np) * TF_N - half * 32;
+        float v[32], x[32];
+        tmem_ld32_async(st, v);
+        tmem_ld32_async(st + 64, x);
+        tmem_wait_ld();
+        tmem_ready(v);
+        tmem_ready(x);
 #pragma unroll
-        for (int q = 0; q < TF_N; q += 32) {
-          float x[32];
-          tmem_ld32_async(st + q, v + q);
-          tmem_ld32_async(st + 64 + q, x);
-          tmem_wait_ld();
-          tmem_ready(v + q);
-          tmem_ready(x);
+        for (int k = 0; k < 32; ++k) v[k] = fmaf(x[k], 1.f / 2048.f, v[k]);
+        if (__any_sync(0xffffffffu, lim < 32) || (gone & 3u) != 0) {
 #pragma unroll
-          for (int k = 0; k < 32; ++k) v[q + k] = fmaf(x[k], 1.f / 2048.f, v[q + k]);
-        }
-        if (__any_sync(0xffffffffu, lim < TF_N) || gone != 0) {
-#pragma unroll
-          for (int k = 0; k < TF_N; ++k) v[k] = k < lim && !((gone >> (k / 16)) & 1u) ? v[k] : -INFINITY;
+          for (int k = 0; k < 32; ++k) v[k] = k < lim && !((gone >> (k / 16)) & 1u) ? v[k] : -INFINITY;
         }
         float a0 = fmaxf(v[0], v[1]), a1 = fmaxf(v[2], v[3]);
 #pragma unroll
-        for (int k = 4; k < TF_N; k += 4) {
+        for (int k = 4; k < 32; k += 4) {
           a0 = max3(a0, v[k], v[k + 1]);
           a1 = max3(a1, v[k + 2], v[k + 3]);
         }
-        const float mx = fmaxf(a0, a1) * c;
-        if (__any_sync(0xffffffffu, mx > m + TC_RAISE)) {  // also from -inf
+        float mx = fmaxf(a0, a1) * c;
+        s_max[i & 1][half][lanes + lane] = mx;
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&max_full[warp & 3]);
+        ok = __all_sync(0xffffffffu, pa_wait(&max_full[warp & 3], i & 1, abort));  // both have read S, too: P goes over it
+        if (!ok) break;
+        tc_fence_after();
+        mx = fmaxf(mx, s_max[i & 1][half ^ 1][lanes + lane]);
+        if (__any_sync(0xffffffffu, mx > m + TC_RAISE)) {  // also from -inf; the other half comes to the same
           const float mn = fmaxf(m, mx);
           const float f = m == -INFINITY ? 0.f : ex2(m - mn);
           m = mn;
@@ -1315,30 +1332,29 @@ many_rows_f32_kernel(const PrefixAttnParams p, const __grid_constant__ PoolMaps 
             if (!ok) break;
             tc_fence_after();
 #pragma unroll
-            for (int q = 0; q < 2 * HD; q += 32) {
+            for (int q = 0; q < HD; q += 32) {  // HD / 2 columns of each part
+              const uint32_t ad = ot + (q < HD / 2 ? q : HD / 2 + q);
               float u[32];
-              tmem_ld32(ot + q, u);
+              tmem_ld32(ad, u);
 #pragma unroll
               for (int k = 0; k < 32; ++k) u[k] *= f;
-              tmem_st32(ot + q, u);
+              tmem_st32(ad, u);
             }
           }
         }
         const float mm = m == -INFINITY ? 0.f : m;
         float l0 = 0.f, l1 = 0.f;
+        uint32_t hi[16], lo[16];
 #pragma unroll
-        for (int q = 0; q < TF_N; q += 32) {
-          uint32_t hi[16], lo[16];
-#pragma unroll
-          for (int k = 0; k < 32; k += 2) {
-            const float e0 = ex2(fmaf(v[q + k], c, -mm)), e1 = ex2(fmaf(v[q + k + 1], c, -mm));
-            l0 += e0;
-            l1 += e1;
-            split_f16(e0, e1, hi[k / 2], lo[k / 2]);
-          }
-          tmem_st16(st + q / 2, hi);  // over S, which has been read
-          tmem_st16(st + 64 + q / 2, lo);
+        for (int k = 0; k < 32; k += 2) {
+          const float e0 = ex2(fmaf(v[k], c, -mm)), e1 = ex2(fmaf(v[k + 1], c, -mm));
+          l0 += e0;
+          l1 += e1;
+          split_f16(e0, e1, hi[k / 2], lo[k / 2]);
         }
+        const uint32_t pt = tl + (i & 1) * 128 + half * 16;
+        tmem_st16(pt, hi);
+        tmem_st16(pt + 64, lo);
         l += l0 + l1;
         tmem_wait_st();
         tc_fence_before();
@@ -1348,12 +1364,17 @@ many_rows_f32_kernel(const PrefixAttnParams p, const __grid_constant__ PoolMaps 
       ok = ok && __all_sync(0xffffffffu, pa_wait(&o_full, 0, abort));
       tc_fence_after();
       if (ok) {
+        s_max[cnt & 1][half][lanes + lane] = l;
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&max_full[warp & 3]);
+        ok = __all_sync(0xffffffffu, pa_wait(&max_full[warp & 3], cnt & 1, abort));
+        l += s_max[cnt & 1][half ^ 1][lanes + lane];
         const float inv = l == 0.f ? 0.f : 1.f / l;
-        if (valid && p.nslots > 1) p.part_ml[at] = make_float2(m, l);
-        float* dst = p.nslots > 1 ? p.part_o + at * HD : reinterpret_cast<float*>(p.out) + row * HD;
+        if (valid && p.nslots > 1 && half == 0) p.part_ml[at] = make_float2(m, l);
+        float* dst = (p.nslots > 1 ? p.part_o + at * HD : reinterpret_cast<float*>(p.out) + row * HD) + half * (HD / 2);
         const float f = p.nslots > 1 ? 1.f : inv;
 #pragma unroll
-        for (int q = 0; q < HD; q += 32) {
+        for (int q = 0; q < HD / 2; q += 32) {
           float v[32], x[32];
           tmem_ld32(ot + q, v);
           tmem_ld32(ot + HD + q, x);
@@ -1364,7 +1385,7 @@ many_rows_f32_kernel(const PrefixAttnParams p, const __grid_constant__ PoolMaps 
           for (int k = 0; k < 32; k += 4) *reinterpret_cast<float4*>(dst + q + k) = make_float4(v[k], v[k + 1], v[k + 2], v[k + 3]);
         }
       }
-    } else if (valid) {  // no keys in this share
+    } else if (valid && half == 0) {  // no keys in this share
       if (p.nslots > 1) {
         p.part_ml[at] = make_float2(-INFINITY, 0.f);
       } else {
