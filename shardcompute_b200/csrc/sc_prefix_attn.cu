@@ -59,12 +59,12 @@ __device__ __forceinline__ int prefix_keys(const PrefixAttnParams& p) {
   return (int)min((long long)max(*p.prefix_len, 0), cap);
 }
 
-// 3-D copy of `rows` pool rows (all 128-byte column chunks) into shared memory, completing on `bar`.
-__device__ __forceinline__ void tma3d(void* dst, const CUtensorMap* map, int row, uint64_t* bar) {
+// Copy of a box of pool rows, from 128-byte column `chunk` on, into shared memory, completing on `bar`.
+__device__ __forceinline__ void tma3d_at(uint32_t dst, const CUtensorMap* map, int row, int chunk, uint64_t* bar) {
   asm volatile(
       "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::
-          "r"(smem_u32(dst)),
-      "l"(reinterpret_cast<uint64_t>(map)), "r"(0), "r"(row), "r"(0), "r"(smem_u32(bar))
+          "r"(dst),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(0), "r"(row), "r"(chunk), "r"(smem_u32(bar))
       : "memory");
 }
 
@@ -72,8 +72,8 @@ __device__ __forceinline__ void tma3d(void* dst, const CUtensorMap* map, int row
 
 // Kernel for few rows per request.  A CTA takes a request, a kv head, a share
 // of the keys and every row_groups-th tile of rows; its warps take tiles of 16 (fp32: 8) keys in turn, each with its own
-// ring of tiles in shared memory (one TMA copy of K and one of V per tile, a
-// tile never straddles a page) and its own running (m, l, o), so no barrier
+// ring of tiles in shared memory (a TMA copy per 16 or 8 keys, which never
+// straddle a page) and its own running (m, l, o), so no barrier
 // stands in the loop.  The warps' results are joined at the end.
 //
 // fp16: mma m16n8k16 over up to 16 rows (the request's tokens x the group's
@@ -95,6 +95,7 @@ struct FewRows {
   static constexpr int SUB = KT * 128;                  // bytes of a chunk of a tile
   static constexpr int TILE = NB * SUB;                 // bytes of a K or V tile
   static constexpr int STAGE = 2 * TILE;
+  static constexpr int COPIES = F16 ? NB : 1;           // of a tile: fp16, one per 128-byte chunk, as many_rows_kernel's
   static constexpr int NST = HD == 128 ? 3 : 6;         // stages per warp: 96 KB a CTA, two CTAs an SM
   static constexpr int SMEM = FR_WARPS * NST * STAGE + 1024;
 };
@@ -183,11 +184,13 @@ few_rows_kernel(const PrefixAttnParams p, const __grid_constant__ PoolMaps maps,
       const int r = __shfl_sync(0xffffffffu, rows, i & 31);
       const int s = issued % NST;
       absent = (absent & ~(1u << s)) | ((r < 0 ? 1u : 0u) << s);
-      if (lane == 0) {
-        mbar_arrive_expect_tx(&full[warp][s], C::STAGE);
-        const int at = r < 0 ? p.pool_rows : r;  // past the end: zeros
-        tma3d(ring + s * C::STAGE, &maps.k, at, &full[warp][s]);
-        tma3d(ring + s * C::STAGE + C::TILE, &maps.v, at, &full[warp][s]);
+      if (lane == 0) mbar_arrive_expect_tx(&full[warp][s], C::STAGE);
+      __syncwarp();
+      if (lane < 2 * C::COPIES) {
+        const bool v = lane >= C::COPIES;
+        const int ch = lane % C::COPIES;
+        tma3d_at(ring_u + s * C::STAGE + (v ? C::TILE : 0) + ch * SUB, v ? &maps.v : &maps.k, r < 0 ? p.pool_rows : r, ch,
+                 &full[warp][s]);  // past the end: zeros
       }
       ++issued;
     };
@@ -489,6 +492,7 @@ few_rows_kernel(const PrefixAttnParams p, const __grid_constant__ PoolMaps maps,
 // only when a score passes it by 2^8 (P then stays below 2^8 and l in fp32).
 // TMEM: S0 | S1 (128 columns each, P in the first 64), O0 | O1 (HD each).
 constexpr int TC_M = 128, TC_N = 128;   // rows and keys of a tile
+constexpr int TC_BOX = 16;              // keys of a copy
 constexpr int TC_THREADS = 12 * 32;
 constexpr int TC_REGS_CTL = 88, TC_REGS_SM = 208;  // 128 x 88 + 256 x 208: what the block starts with, 384 x 168
 constexpr int TC_HAND = 3;  // quarter of a tile before which its softmax lets the other one start
@@ -511,14 +515,6 @@ __device__ __forceinline__ bool pa_spin(uint64_t* bar, uint32_t parity, volatile
   for (int i = 0; i < 64; ++i)
     if (mbar_test_wait(bar, parity)) return true;
   return pa_wait(bar, parity, abort);
-}
-
-__device__ __forceinline__ void tma3d_at(uint32_t dst, const CUtensorMap* map, int row, int chunk, uint64_t* bar) {
-  asm volatile(
-      "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::
-          "r"(dst),
-      "l"(reinterpret_cast<uint64_t>(map)), "r"(0), "r"(row), "r"(chunk), "r"(smem_u32(bar))
-      : "memory");
 }
 
 __device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&r)[16]) {
@@ -556,6 +552,11 @@ __device__ __forceinline__ void tmem_ready(float* v) {  // no use of v[0..31] mo
   for (int i = 0; i < 32; i += 8)
     asm volatile("" : "+f"(v[i]), "+f"(v[i + 1]), "+f"(v[i + 2]), "+f"(v[i + 3]), "+f"(v[i + 4]), "+f"(v[i + 5]), "+f"(v[i + 6]), "+f"(v[i + 7]));
 }
+__device__ __forceinline__ void tmem_ld32_wait(uint32_t taddr, float* v) {
+  tmem_ld32_async(taddr, v);
+  tmem_wait_ld();
+  tmem_ready(v);
+}
 __device__ __forceinline__ float max3(float a, float b, float c) {
   float d;
   asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
@@ -579,6 +580,36 @@ __device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
   uint64_t d;
   asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
   return d;
+}
+
+// A warp's 32 rows of RB bytes, a row in each lane's registers (`get(c)`: its c-th 16 bytes), to global rows of `stride`
+// bytes: through shared memory (`sm`, 32 RB bytes of this warp's own), so that a row's lanes write next to each other.
+// Written straight from the registers, the 128 rows of a tile took 4300 clocks.
+template <int RB, typename F>
+__device__ __forceinline__ void flush_rows(uint32_t sm, F get, char* dst, size_t stride, size_t row, bool valid) {
+  constexpr int LPR = RB / 16, RPI = 32 / LPR;  // lanes per row, rows per store
+  const int lane = threadIdx.x & 31;
+#pragma unroll
+  for (int c = 0; c < LPR; ++c) {
+    const uint4 v = get(c);
+    asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(sm + lane * RB + ((c ^ (lane & (LPR - 1))) << 4)), "r"(v.x), "r"(v.y),
+                 "r"(v.z), "r"(v.w)
+                 : "memory");
+  }
+  __syncwarp();
+  const int c = lane % LPR;
+#pragma unroll
+  for (int j = 0; j < 32 / RPI; ++j) {
+    const int r = j * RPI + lane / LPR;
+    const size_t to = __shfl_sync(0xffffffffu, (unsigned long long)row, r);
+    const bool ok = __shfl_sync(0xffffffffu, (int)valid, r);
+    const uint4 v = lds_v4(sm + r * RB + ((c ^ (r & (LPR - 1))) << 4));
+    if (ok) *reinterpret_cast<uint4*>(dst + to * stride + c * 16) = v;
+  }
+  __syncwarp();
+}
+__device__ __forceinline__ uint4 f4_as_u4(const float* v) {
+  return make_uint4(__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]), __float_as_uint(v[3]));
 }
 
 // The rows and keys of a CTA of the many-rows kernels: `item`-th block of ROWS rows (of the whole batch where PACKED,
@@ -718,22 +749,24 @@ many_rows_kernel(const PrefixAttnParams p, const __grid_constant__ PoolMaps maps
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(TC_REGS_SM));
   if (warp == 0) {
     // ================================ TMA producer ================================
-    const int lg = min(p.lg_page, 7), rpb = 1 << lg;  // rows per copy
-    const int boxes = (TC_N >> lg) * C::NCH;
+    constexpr int COPIES = TC_N / TC_BOX * C::NCH;
     const int sub = lane / C::NCH, ch = lane % C::NCH;
+    auto rows_of = [&](int i) {  // the pool rows of tile i, one per copy; -1: no such page
+      const int t = t_lo + i;
+      if (i >= cnt || lane >= COPIES || sub * TC_BOX >= keys_of(t)) return -1;
+      const int key = (t < np ? t : t - np) * TC_N + sub * TC_BOX, blk = key >> p.lg_page;
+      const int id = t < np ? p.prefix_table[blk] : p.block_table[(size_t)b * p.max_blocks + blk];
+      return id >= 0 && id < p.n_pages ? ((id * p.Hkv + h) << p.lg_page) + (key & ((1 << p.lg_page) - 1)) : -1;
+    };
     uint32_t it = 0;
     bool ok = true;
+    int next = rows_of(0);
     for (int i = 0; i < cnt && ok; ++i) {
-      const int t = t_lo + i, k0 = (t < np ? t : t - np) * TC_N;
-      int row = -1;
-      if (lane < boxes && sub * rpb < keys_of(t)) {
-        const int key = k0 + sub * rpb, blk = key >> p.lg_page;
-        const int id = t < np ? p.prefix_table[blk] : p.block_table[(size_t)b * p.max_blocks + blk];
-        if (id >= 0 && id < p.n_pages) row = ((id * p.Hkv + h) << p.lg_page) + (key & ((1 << p.lg_page) - 1));
-      }
-      uint32_t gone = 0;  // keys of this tile that have no page, a bit per 16
-      for (int k = 0; k < TC_N / 16; ++k)
-        gone |= (__shfl_sync(0xffffffffu, row, ((k * 16) >> lg) * C::NCH) < 0 ? 1u : 0u) << k;
+      const int row = next;
+      next = rows_of(i + 1);
+      uint32_t gone = 0;  // keys of this tile that have no page, a bit per copy's
+#pragma unroll
+      for (int k = 0; k < TC_N / TC_BOX; ++k) gone |= (__shfl_sync(0xffffffffu, row, k * C::NCH) < 0 ? 1u : 0u) << k;
       if (lane == 0) s_absent[i & 15] = gone;
 #pragma unroll
       for (int kv = 0; kv < 2; ++kv, ++it) {
@@ -742,8 +775,8 @@ many_rows_kernel(const PrefixAttnParams p, const __grid_constant__ PoolMaps maps
         if (!ok) break;
         if (lane == 0) mbar_arrive_expect_tx(&full[s], C::TILE);
         __syncwarp();
-        if (lane < boxes)
-          tma3d_at(ring_u + s * C::TILE + ch * (TC_N * 128) + sub * rpb * 128, kv ? &maps.v : &maps.k,
+        if (lane < COPIES)
+          tma3d_at(ring_u + s * C::TILE + ch * (TC_N * 128) + sub * TC_BOX * 128, kv ? &maps.v : &maps.k,
                    row < 0 ? p.pool_rows : row, ch, &full[s]);
       }
     }
@@ -865,7 +898,7 @@ many_rows_kernel(const PrefixAttnParams p, const __grid_constant__ PoolMaps maps
         const uint32_t gone = s_absent[i & 15];
         const int lim = (t < np ? P : see) - (t < np ? t : t - np) * TC_N;  // keys of the tile this row sees
         const bool part = __any_sync(0xffffffffu, lim < TC_N) || gone != 0;
-        auto seen = [&](int k) { return k < lim && !((gone >> (k / 16)) & 1u); };
+        auto seen = [&](int k) { return k < lim && !((gone >> (k / TC_BOX)) & 1u); };
         float v[TC_N];
 #pragma unroll
         for (int q = 0; q < TC_N; q += 32) tmem_ld32_async(st + q, v + q);
@@ -896,7 +929,7 @@ many_rows_kernel(const PrefixAttnParams p, const __grid_constant__ PoolMaps maps
 #pragma unroll
             for (int q = 0; q < HD / 32; ++q) {
               float u[32];
-              tmem_ld32(ot + q * 32, u);
+              tmem_ld32_wait(ot + q * 32, u);
 #pragma unroll
               for (int k = 0; k < 32; ++k) u[k] *= f;
               tmem_st32(ot + q * 32, u);
@@ -964,25 +997,27 @@ many_rows_kernel(const PrefixAttnParams p, const __grid_constant__ PoolMaps maps
         const size_t at = (size_t)(slot0 + split) * p.T * p.Hq + row;
         const float inv = l == 0.f ? 0.f : 1.f / l;
         if (valid && p.nslots > 1) p.part_ml[at] = make_float2(m, l);
+        const uint32_t sm = q_u + x * C::TILE + lanes * (HD * 2);  // in the tile's Q, which is done with
+        if (p.nslots > 1) {
 #pragma unroll
-        for (int q = 0; q < HD / 32; ++q) {
-          float v[32];
-          tmem_ld32(ot + q * 32, v);
-          if (!valid) continue;
-          if (p.nslots > 1) {
-            float* dst = p.part_o + at * HD + q * 32;
+          for (int q = 0; q < HD; q += HD / 2) {
+            float v[HD / 2];
 #pragma unroll
-            for (int k = 0; k < 32; k += 4) *reinterpret_cast<float4*>(dst + k) = make_float4(v[k], v[k + 1], v[k + 2], v[k + 3]);
-          } else {
-            __half* dst = reinterpret_cast<__half*>(p.out) + row * HD + q * 32;
-#pragma unroll
-            for (int k = 0; k < 32; k += 8) {
-              uint32_t ow[4];
-#pragma unroll
-              for (int j = 0; j < 4; ++j) ow[j] = h2_as_u32(__floats2half2_rn(v[k + 2 * j] * inv, v[k + 2 * j + 1] * inv));
-              *reinterpret_cast<uint4*>(dst + k) = make_uint4(ow[0], ow[1], ow[2], ow[3]);
-            }
+            for (int k = 0; k < HD / 2; k += 32) tmem_ld32_wait(ot + q + k, v + k);
+            flush_rows<HD * 2>(sm, [&](int c) { return f4_as_u4(v + c * 4); }, reinterpret_cast<char*>(p.part_o + (at - row) * HD + q),
+                               HD * sizeof(float), row, valid);
           }
+        } else {
+          uint32_t o2[HD / 2];
+#pragma unroll
+          for (int k = 0; k < HD; k += 32) {
+            float v[32];
+            tmem_ld32_wait(ot + k, v);
+#pragma unroll
+            for (int j = 0; j < 16; ++j) o2[k / 2 + j] = h2_as_u32(__floats2half2_rn(v[2 * j] * inv, v[2 * j + 1] * inv));
+          }
+          flush_rows<HD * 2>(sm, [&](int c) { return make_uint4(o2[4 * c], o2[4 * c + 1], o2[4 * c + 2], o2[4 * c + 3]); },
+                             reinterpret_cast<char*>(p.out), HD * sizeof(__half), row, valid);
         }
       }
     } else if (x < nx && work && valid) {  // no keys in this share
@@ -1031,7 +1066,7 @@ many_rows_kernel(const PrefixAttnParams p, const __grid_constant__ PoolMaps maps
 //                behind the last key, which may hold anything, become zero
 // TMEM: two buffers of S (hi.hi | cross, 64 columns each), O (hi.hi | cross).
 constexpr int TF_N = 64;              // keys of a tile
-constexpr int TF_BOX = 16;            // keys of a copy
+constexpr int TF_BOX = 8;             // keys of a copy
 constexpr int TF_THREADS = 20 * 32;
 constexpr int TF_CONV = 8;            // warps that split
 
@@ -1129,7 +1164,7 @@ many_rows_f32_kernel(const PrefixAttnParams p, const __grid_constant__ PoolMaps 
         if (id >= 0 && id < p.n_pages) at = ((id * p.Hkv + h) << p.lg_page) + (key & ((1 << p.lg_page) - 1));
       }
       const uint32_t gone = __ballot_sync(0xffffffffu, at < 0) & ((1u << (TF_N / TF_BOX)) - 1);
-      if (lane == 0) s_absent[i & 15] = gone;  // a bit per 16 keys
+      if (lane == 0) s_absent[i & 15] = gone;  // a bit per copy
       return at;
     };
     auto copy = [&](const CUtensorMap* map, int at, uint32_t it) {
@@ -1292,7 +1327,7 @@ many_rows_f32_kernel(const PrefixAttnParams p, const __grid_constant__ PoolMaps 
         tc_fence_after();
         const uint32_t st = tl + (i & 1) * 128 + half * 32;
         const int t = w.t_lo + i;
-        const uint32_t gone = s_absent[i & 15] >> (half * 2);
+        const uint32_t gone = (s_absent[i & 15] >> (half * (32 / TF_BOX))) & ((1u << (32 / TF_BOX)) - 1);
         // of this thread's keys, those that its row sees
         const int lim = (t < np ? w.P : see) - (t < np ? t : t - np) * TF_N - half * 32;
         float v[32], x[32];
@@ -1303,9 +1338,9 @@ many_rows_f32_kernel(const PrefixAttnParams p, const __grid_constant__ PoolMaps 
         tmem_ready(x);
 #pragma unroll
         for (int k = 0; k < 32; ++k) v[k] = fmaf(x[k], 1.f / 2048.f, v[k]);
-        if (__any_sync(0xffffffffu, lim < 32) || (gone & 3u) != 0) {
+        if (__any_sync(0xffffffffu, lim < 32) || gone != 0) {
 #pragma unroll
-          for (int k = 0; k < 32; ++k) v[k] = k < lim && !((gone >> (k / 16)) & 1u) ? v[k] : -INFINITY;
+          for (int k = 0; k < 32; ++k) v[k] = k < lim && !((gone >> (k / TF_BOX)) & 1u) ? v[k] : -INFINITY;
         }
         float a0 = fmaxf(v[0], v[1]), a1 = fmaxf(v[2], v[3]);
 #pragma unroll
@@ -1335,7 +1370,7 @@ many_rows_f32_kernel(const PrefixAttnParams p, const __grid_constant__ PoolMaps 
             for (int q = 0; q < HD; q += 32) {  // HD / 2 columns of each part
               const uint32_t ad = ot + (q < HD / 2 ? q : HD / 2 + q);
               float u[32];
-              tmem_ld32(ad, u);
+              tmem_ld32_wait(ad, u);
 #pragma unroll
               for (int k = 0; k < 32; ++k) u[k] *= f;
               tmem_st32(ad, u);
@@ -1371,19 +1406,20 @@ many_rows_f32_kernel(const PrefixAttnParams p, const __grid_constant__ PoolMaps 
         l += s_max[cnt & 1][half ^ 1][lanes + lane];
         const float inv = l == 0.f ? 0.f : 1.f / l;
         if (valid && p.nslots > 1 && half == 0) p.part_ml[at] = make_float2(m, l);
-        float* dst = (p.nslots > 1 ? p.part_o + at * HD : reinterpret_cast<float*>(p.out) + row * HD) + half * (HD / 2);
+        float* dst = (p.nslots > 1 ? p.part_o + (at - row) * HD : reinterpret_cast<float*>(p.out)) + half * (HD / 2);
         const float f = p.nslots > 1 ? 1.f : inv;
+        float v[HD / 2];
 #pragma unroll
         for (int q = 0; q < HD / 2; q += 32) {
-          float v[32], x[32];
-          tmem_ld32(ot + q, v);
-          tmem_ld32(ot + HD + q, x);
-          if (!valid) continue;
+          float x[32];
+          tmem_ld32_wait(ot + q, v + q);
+          tmem_ld32_wait(ot + HD + q, x);
 #pragma unroll
-          for (int k = 0; k < 32; ++k) v[k] = fmaf(x[k], 1.f / 2048.f, v[k]) * f;
-#pragma unroll
-          for (int k = 0; k < 32; k += 4) *reinterpret_cast<float4*>(dst + q + k) = make_float4(v[k], v[k + 1], v[k + 2], v[k + 3]);
+          for (int k = 0; k < 32; ++k) v[q + k] = fmaf(x[k], 1.f / 2048.f, v[q + k]) * f;
         }
+        // through Q's tiles, which are done with
+        flush_rows<HD * 2>(q_u + (warp - 4) * 32 * HD * 2, [&](int c) { return f4_as_u4(v + c * 4); }, reinterpret_cast<char*>(dst),
+                           HD * sizeof(float), row, valid);
       }
     } else if (valid && half == 0) {  // no keys in this share
       if (p.nslots > 1) {
@@ -1413,8 +1449,8 @@ many_rows_f32_kernel(const PrefixAttnParams p, const __grid_constant__ PoolMaps 
 
 // ---------------------------------------------------------------- join
 
-// One warp per (row, head): the slots' (m, l) first, one slot a lane, then
-// their sums, weighted.  Reads each partial result once; bound by L2.
+// One warp per (row, head).  Lane s holds slot s's weight 2^(m_s - M), so the slots' sums are read without waiting for
+// one another.  Reads each partial result once; bound by L2.
 template <typename T, int HD>
 __global__ void __launch_bounds__(256) join_slots_kernel(const PrefixAttnParams p) {
   pdl_trigger();
@@ -1423,29 +1459,40 @@ __global__ void __launch_bounds__(256) join_slots_kernel(const PrefixAttnParams 
   const int row = blockIdx.x * (blockDim.x / 32) + (threadIdx.x >> 5), lane = threadIdx.x & 31;
   if (row >= rows) return;
   const size_t stride = (size_t)p.T * p.Hq;
-  constexpr int V = HD / 32;
+  constexpr int V = HD / 32, SETS = 3;  // at most 96 slots
+  float2 ml[SETS];
   float M = -INFINITY;
-  for (int s0 = 0; s0 < p.nslots; s0 += 32)
-    if (s0 + lane < p.nslots) M = fmaxf(M, p.part_ml[(s0 + lane) * stride + row].x);
+#pragma unroll
+  for (int k = 0; k < SETS; ++k) {
+    ml[k] = k * 32 + lane < p.nslots ? p.part_ml[(k * 32 + lane) * stride + row] : make_float2(-INFINITY, 0.f);
+    M = fmaxf(M, ml[k].x);
+  }
 #pragma unroll
   for (int d = 16; d; d >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, d));
   float acc[V], L = 0.f;
 #pragma unroll
   for (int i = 0; i < V; ++i) acc[i] = 0.f;
-  for (int s = 0; s < p.nslots; ++s) {
-    const float2 ml = p.part_ml[s * stride + row];
-    if (ml.x == -INFINITY && ml.y == 0.f) continue;
-    const float f = ex2(ml.x - M);
-    L += f * ml.y;
-    const float* src = p.part_o + (s * stride + row) * HD + lane * V;
-    if constexpr (V == 4) {
-      const float4 v = *reinterpret_cast<const float4*>(src);
-      acc[0] += f * v.x; acc[1] += f * v.y; acc[2] += f * v.z; acc[3] += f * v.w;
-    } else {
-      const float2 v = *reinterpret_cast<const float2*>(src);
-      acc[0] += f * v.x; acc[1] += f * v.y;
+#pragma unroll
+  for (int k = 0; k < SETS; ++k) {
+    const float f = ml[k].x == -INFINITY && ml[k].y == 0.f ? 0.f : ex2(ml[k].x - M);  // 0: no key, nothing was written
+    L += f * ml[k].y;
+    const int n = min(32, p.nslots - k * 32);
+#pragma unroll 4
+    for (int s = 0; s < n; ++s) {
+      const float fs = __shfl_sync(0xffffffffu, f, s);
+      if (fs == 0.f) continue;
+      const float* src = p.part_o + ((k * 32 + s) * stride + row) * HD + lane * V;
+      if constexpr (V == 4) {
+        const float4 v = *reinterpret_cast<const float4*>(src);
+        acc[0] += fs * v.x; acc[1] += fs * v.y; acc[2] += fs * v.z; acc[3] += fs * v.w;
+      } else {
+        const float2 v = *reinterpret_cast<const float2*>(src);
+        acc[0] += fs * v.x; acc[1] += fs * v.y;
+      }
     }
   }
+#pragma unroll
+  for (int d = 16; d; d >>= 1) L += __shfl_xor_sync(0xffffffffu, L, d);
   const float inv = L == 0.f ? 0.f : 1.f / L;
   T* dst = reinterpret_cast<T*>(p.out) + (size_t)row * HD + lane * V;
 #pragma unroll
@@ -1545,11 +1592,13 @@ template <typename T, int HD>
 static int run_attn(const PrefixAttnParams& p, const void* k, const void* v, const AttnPlan& a, cudaStream_t stream) {
   using C = FewRows<T, HD>;
   int st = SC_OK;
+  // one pair of maps for all kernels of the type: 16 keys of a 128-byte column, or 8 keys of all columns
+  PoolMaps maps;
+  const int box = C::F16 ? TC_BOX : TF_BOX, chunks = C::F16 ? 1 : C::NB;
+  static_assert(C::KT == (C::F16 ? TC_BOX : TF_BOX), "a tile of the few-rows kernel is one box high");
+  SC_REQUIRE(pool_map(&maps.k, k, p.pool_rows, HD, C::F16, box, chunks) && pool_map(&maps.v, v, p.pool_rows, HD, C::F16, box, chunks),
+             SC_ERR_CUDA, "prefix_attn: tensor map of the pages refused");
   if (a.kind != AttnPlan::FEW) {
-    PoolMaps maps;
-    const int box = C::F16 ? std::min(TC_N, 1 << p.lg_page) : TF_BOX, chunks = C::F16 ? 1 : C::NB;
-    SC_REQUIRE(pool_map(&maps.k, k, p.pool_rows, HD, C::F16, box, chunks) && pool_map(&maps.v, v, p.pool_rows, HD, C::F16, box, chunks),
-               SC_ERR_CUDA, "prefix_attn: tensor map of the pages refused");
     const bool packed = a.kind == AttnPlan::SHARED;
     if constexpr (C::F16)
       st = packed ? run_many_rows<many_rows_kernel<HD, true>>(ManyRows<HD>::SMEM, TC_THREADS, p, maps, a, stream)
@@ -1560,9 +1609,6 @@ static int run_attn(const PrefixAttnParams& p, const void* k, const void* v, con
     if (st != SC_OK) return st;
   }
   if (a.kind != AttnPlan::CHUNKS) {
-    PoolMaps maps;
-    SC_REQUIRE(pool_map(&maps.k, k, p.pool_rows, HD, C::F16, C::KT, C::NB) && pool_map(&maps.v, v, p.pool_rows, HD, C::F16, C::KT, C::NB),
-               SC_ERR_CUDA, "prefix_attn: tensor map of the pages refused");
     const cudaError_t e = opt_in<few_rows_kernel<T, HD>>(C::SMEM);
     if (e != cudaSuccess) return check_launch("prefix_attn", e);
     launch(few_rows_kernel<T, HD>, dim3(a.splits * a.row_groups, p.Hkv, p.B), dim3(FR_WARPS * 32), C::SMEM, stream, p, maps,

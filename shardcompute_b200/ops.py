@@ -297,7 +297,9 @@ def _sized(what: str, n: int, **named: Optional[torch.Tensor]) -> None:
 def _call_on(dev: int, name: str, *args) -> None:
     """The call with device ``dev`` as the current one, on its current stream."""
     if dev == torch._C._cuda_getDevice():
-        L.call(name, *args, torch._C._cuda_getCurrentRawStream(dev))
+        st = getattr(L.load(), name)(*args, torch._C._cuda_getCurrentRawStream(dev))
+        if st:
+            L.check(st, name)
     else:
         with torch.cuda.device(dev):
             L.call(name, *args, torch._C._cuda_getCurrentRawStream(dev))
@@ -333,9 +335,11 @@ def paged_reserve(lens: torch.Tensor, new_lens: torch.Tensor, block_table: torch
     _check("paged_reserve", dev, ts if prefix_len is None else (*ts, prefix_len), _I32)
     if block_table.dim() != 2 or block_table.shape[0] != B:
         raise ValueError(f"paged_reserve: block_table {tuple(block_table.shape)} is not [{B}, max_blocks]")
-    _sized("paged_reserve", B, new_lens=new_lens, kv_lens=kv_lens)
-    _sized("paged_reserve", B + 1, q_start=q_start)
-    _sized("paged_reserve", 1, free_count=free_count, prefix_len=prefix_len, free_count_out=free_count_out, status=status)
+    if (new_lens.numel() != B or kv_lens.numel() != B or q_start.numel() != B + 1 or free_count.numel() != 1
+            or free_count_out.numel() != 1 or status.numel() != 1 or (prefix_len is not None and prefix_len.numel() != 1)):
+        _sized("paged_reserve", B, new_lens=new_lens, kv_lens=kv_lens)
+        _sized("paged_reserve", B + 1, q_start=q_start)
+        _sized("paged_reserve", 1, free_count=free_count, prefix_len=prefix_len, free_count_out=free_count_out, status=status)
     if slots.numel() < rows or positions.numel() < rows:
         raise ValueError(f"paged_reserve: slots and positions hold {slots.numel()} and {positions.numel()} rows, {rows} are needed")
     _call_on(dev, "sc_paged_reserve", lens.data_ptr(), new_lens.data_ptr(), B, _p(prefix_len), block_table.data_ptr(),
@@ -359,8 +363,9 @@ def paged_truncate(lens: torch.Tensor, keep: torch.Tensor, block_table: torch.Te
     _check("paged_truncate", dev, (lens, keep, block_table, free_pages, free_count, lens_out, free_count_out, status), _I32)
     if block_table.dim() != 2 or block_table.shape[0] != B:
         raise ValueError(f"paged_truncate: block_table {tuple(block_table.shape)} is not [{B}, max_blocks]")
-    _sized("paged_truncate", B, keep=keep, lens_out=lens_out)
-    _sized("paged_truncate", 1, free_count=free_count, free_count_out=free_count_out, status=status)
+    if keep.numel() != B or lens_out.numel() != B or free_count.numel() != 1 or free_count_out.numel() != 1 or status.numel() != 1:
+        _sized("paged_truncate", B, keep=keep, lens_out=lens_out)
+        _sized("paged_truncate", 1, free_count=free_count, free_count_out=free_count_out, status=status)
     _call_on(dev, "sc_paged_truncate", lens.data_ptr(), keep.data_ptr(), B, block_table.data_ptr(), block_table.shape[1],
              free_pages.data_ptr(), free_pages.numel(), free_count.data_ptr(), page_size, lens_out.data_ptr(),
              free_count_out.data_ptr(), status.data_ptr())
