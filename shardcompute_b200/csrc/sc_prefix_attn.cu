@@ -1555,25 +1555,35 @@ struct AttnPlan {
   int nslots;
 };
 
-static AttnPlan plan_attn(int T, int B, int Hkv, int G, bool f16, long long own_keys, long long prefix_keys, int sms) {
+static AttnPlan plan_attn(int T, int B, int Hkv, int G, int hd, bool f16, long long own_keys, long long prefix_keys, int sms) {
   AttnPlan a{};
-  const int per_cta = f16 ? 2 * TC_M : TC_M;  // rows
+  const int per_cta = f16 ? 2 * TC_M : TC_M, tile = f16 ? TC_N : TF_N;
   const long long rows = (long long)T * G, items = (rows + per_cta - 1) / per_cta;
   const auto ceil_div = [](long long x, long long y) { return (x + y - 1) / y; };
   a.kind = rows >= 64ll * B ? AttnPlan::CHUNKS : prefix_keys > 0 && B > 1 ? AttnPlan::SHARED : AttnPlan::FEW;
   if (a.kind != AttnPlan::FEW) {
-    // shares of the keys until there is a CTA for every SM
-    const long long keys = prefix_keys + (a.kind == AttnPlan::CHUNKS ? own_keys : 0);
+    // Shares of the keys until there is a CTA for every SM; with the own keys' kernel beside it, for this kernel's part
+    // of the SMs only.  That part goes by the two kernels' work, as far as the host knows it: a tile takes an SM 2.1 us
+    // (256 rows, 128 keys, fp16) or 1.9 us (128 rows, 64 keys, fp32), and own keys, taken for half of what the tables
+    // hold, stream at 44 KB a us and SM.  Measured over the splits 3, 4, 6, 8, 10, 14: 64 requests behind 8197 tokens,
+    // fp16, 61, 53, 55, 58, 60, 64 us (the rule takes 4); 32 behind 4099, fp32, 68, 56, 44, 41, 44, 47 us (it takes 7).
+    long long part = 1000;
+    const long long tiles = ceil_div(prefix_keys + (a.kind == AttnPlan::CHUNKS ? own_keys : 0), tile);
+    if (a.kind == AttnPlan::SHARED) {
+      const double many = (double)items * Hkv * tiles * (f16 ? 2.1 : 1.9);
+      const double few = (double)B * own_keys / 2 * Hkv * hd * (f16 ? 4 : 8) / 44e3;
+      part = (long long)(1000 * many / (many + few));
+    }
     a.tc_items = (int)(a.kind == AttnPlan::CHUNKS ? items + B : items);
-    a.tc_splits = (int)std::max(1ll, std::min({(long long)sms * 4 / 5 / (items * Hkv), ceil_div(keys, f16 ? TC_N : TF_N), 32ll}));
+    a.tc_splits = (int)std::max(1ll, std::min({(sms * part / 1000 + items * Hkv / 2) / (items * Hkv), sms / (items * Hkv), tiles, 32ll}));
     a.nslots = a.tc_splits;
   }
   if (a.kind != AttnPlan::CHUNKS) {
     // four CTAs per SM over all requests and heads: first from tiles of rows, then from the keys (64 of them at least)
     const int rt = f16 ? 16 : 8;
     const long long keys = own_keys + (a.kind == AttnPlan::FEW ? prefix_keys : 0);
-    const long long want = ceil_div(4ll * sms, (long long)B * Hkv), tiles = ceil_div(rows, (long long)B * rt);
-    a.row_groups = (int)std::max(1ll, std::min(want, tiles));
+    const long long want = ceil_div(4ll * sms, (long long)B * Hkv), groups = ceil_div(rows, (long long)B * rt);
+    a.row_groups = (int)std::max(1ll, std::min(want, groups));
     a.splits = (int)std::max(1ll, std::min({ceil_div(want, a.row_groups), ceil_div(keys, 64), 64ll}));
     a.nslots += a.splits;
   }
@@ -1639,7 +1649,7 @@ size_t sc_prefix_attn_workspace_bytes(int T, int B, int Hq, int Hkv, int hd, int
                                       int page_size, int dtype) {
   if (T < 1 || B < 1 || Hq < 1 || Hkv < 1 || hd < 1 || max_blocks < 0 || max_prefix_blocks < 0 || page_size < 1) return 0;
   if (Hq % Hkv) return 0;
-  const sc::AttnPlan a = sc::plan_attn(T, B, Hkv, Hq / Hkv, dtype == SC_F16, (long long)max_blocks * page_size,
+  const sc::AttnPlan a = sc::plan_attn(T, B, Hkv, Hq / Hkv, hd, dtype == SC_F16, (long long)max_blocks * page_size,
                                        (long long)max_prefix_blocks * page_size, sc::sm_count());
   return a.nslots <= 1 ? 0 : (size_t)a.nslots * T * Hq * (hd + 2) * sizeof(float);
 }
@@ -1665,7 +1675,7 @@ int sc_prefix_attn(const void* q, const void* k_pages, const void* v_pages, int 
   SC_REQUIRE((((uintptr_t)q | (uintptr_t)k_pages | (uintptr_t)v_pages | (uintptr_t)out) & 15) == 0, SC_ERR_ARG,
              "prefix_attn: tensors must start on 16-byte boundaries");
   if (!prefix_len) max_prefix_blocks = 0;
-  const AttnPlan a = plan_attn(T, B, Hkv, Hq / Hkv, dtype == SC_F16, (long long)max_blocks * page_size,
+  const AttnPlan a = plan_attn(T, B, Hkv, Hq / Hkv, hd, dtype == SC_F16, (long long)max_blocks * page_size,
                                (long long)max_prefix_blocks * page_size, sm_count());
   const size_t need = sc_prefix_attn_workspace_bytes(T, B, Hq, Hkv, hd, max_blocks, max_prefix_blocks, page_size, dtype);
   SC_REQUIRE(workspace_bytes >= need && (need == 0 || workspace), SC_ERR_WORKSPACE,
