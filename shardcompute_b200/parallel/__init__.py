@@ -6,11 +6,12 @@ from .decode_engine import DecodeEngine
 from .embedding import ParallelEmbedding, QuantizedParallelEmbedding, VocabParallelEmbedding
 from .linear import ColumnParallelLinear, RowParallelLinear
 from .mlp import ParallelMLP
+from .paged import PagedKVCache, PagedLayer
 from .quantized_linear import QuantizedColumnParallelLinear, QuantizedRowParallelLinear
 from .transformer import ParallelTransformer, ParallelTransformerBlock, RMSNorm
 from .weights import LayerWeights, RankWeights
 
 __all__ = ["KVCache", "ParallelAttention", "RoPE", "DecodeEngine", "ParallelEmbedding", "QuantizedParallelEmbedding",
-           "VocabParallelEmbedding", "ColumnParallelLinear", "RowParallelLinear", "ParallelMLP",
+           "VocabParallelEmbedding", "ColumnParallelLinear", "RowParallelLinear", "ParallelMLP", "PagedKVCache", "PagedLayer",
            "QuantizedColumnParallelLinear", "QuantizedRowParallelLinear", "ParallelTransformer",
            "ParallelTransformerBlock", "RMSNorm", "LayerWeights", "RankWeights"]

@@ -17,6 +17,11 @@ fp32 buffers (the reference caches fp32: RoPE's fp32 tables promote k) with
 the position kept on the device; ``cache[0]`` / ``cache[1]``
 return the filled ``[B, Hkv/TP, L, hd]`` views, so code that reads
 ``past_key_value[0].shape[2]`` as the cached length keeps working.
+
+With a ``PagedLayer`` as ``past_key_value`` (one layer of a ``PagedKVCache``)
+``hidden_states`` ``[1, T, H]`` holds the new tokens of a ragged batch in a
+row, as the cache's last ``reserve`` placed them: ``sc_paged_rope_append``
+and ``sc_prefix_attn`` take the place of the two cache kernels.
 """
 
 from __future__ import annotations
@@ -29,6 +34,7 @@ import torch
 
 from .. import ops
 from .linear import ColumnParallelLinear, RowParallelLinear
+from .paged import PagedLayer
 from .quantized_linear import QuantizedColumnParallelLinear, QuantizedRowParallelLinear
 
 
@@ -186,6 +192,8 @@ class ParallelAttention:
         B, S, _ = hidden_states.shape
         dev = hidden_states.device
         cache = past_key_value
+        if isinstance(cache, PagedLayer):
+            return self._paged_partial(hidden_states, cache), (cache if use_cache else None)
         if cache is None:
             cache = self.new_cache(B, max(S, self.max_position_embeddings), dev)
         elif not isinstance(cache, KVCache):
@@ -207,6 +215,20 @@ class ParallelAttention:
         attn = attn.view(B, S, self.local_hidden)
         part = self.o_proj.forward_partial(attn)
         return part, (cache if use_cache else None)
+
+    def _paged_partial(self, hidden_states: torch.Tensor, layer: PagedLayer) -> torch.Tensor:
+        """The same for the new tokens of a ragged batch, ``[1, T, H]``, over one layer of a paged cache."""
+        B, T, _ = hidden_states.shape
+        cache, step = layer.cache, layer.cache.step
+        if B != 1 or T > cache.max_tokens:
+            raise ValueError(f"a paged step takes [1, T, H] with T <= {cache.max_tokens}, got {tuple(hidden_states.shape)}")
+        cos, sin = self.rope.tables(cache.max_positions, hidden_states.device)
+        q = torch.zeros(T, self.local_hidden, dtype=layer.k.dtype, device=hidden_states.device)
+        ops.paged_rope_append(self._qkv(hidden_states.reshape(T, -1)).contiguous(), step.q_start, step.slots, step.positions,
+                              cos, sin, q, layer.k, layer.v)
+        attn = ops.prefix_attn(q, layer.k, layer.v, step.q_start, step.kv_lens, cache.block_table, cache.prefix_table,
+                               cache.prefix_len, scale=self.scale)
+        return self.o_proj.forward_partial(attn.view(1, T, self.local_hidden))
 
     async def forward(self, hidden_states: torch.Tensor, attention_mask: Optional[torch.Tensor] = None,
                       position_ids: Optional[torch.Tensor] = None, past_key_value: Optional[KVCache] = None,

@@ -510,6 +510,85 @@ def test_serving_run_in_one_graph(cuda, rng):
         assert sorted(live + free[: int(count)].tolist()) == list(range(n_pages))  # every page held once or free
 
 
+@pytest.mark.parametrize("dtype,tol", [("f32", 4e-4), ("f16", 4e-3)])
+def test_model_over_a_paged_cache(cuda, dtype, tol):
+    """A quantized model over the paged cache -- a shared prefix, ragged prompts, single tokens, drafts that are cut, a
+    request that ends and one that takes its place -- against the same model over the contiguous cache, a request at a
+    time.  fp32: the two attentions differ by d = 2^-19 (two operands and two weights split to 2^-21 each).  The layers round
+    the MLP's inner values to fp16, where values that differ by d fall to different sides with probability d / 2^-11 and
+    are then 2^-10 apart: 2^-10 sqrt(2^11 d) = 6e-5 after the first layer, and with that as d, 2^-10 sqrt(2^11 6e-5) = 3.4e-4
+    after the second, the last.  fp16: keys, values, q, weights and outputs of the attention are rounded by up to 2^-11 each,
+    five of them in two layers: 10 2^-11 = 4.9e-3 at most, and seldom all one way."""
+    import asyncio
+
+    from oracle import sharder as osh
+    from oracle import synth
+    from shardcompute_b200.model.config import ModelConfig
+    from shardcompute_b200.parallel import PagedKVCache, ParallelTransformer, RankWeights
+
+    shape = synth.tiny_shape()
+    full = synth.checkpoint(shape, seed=0)
+    cfg = ModelConfig.from_dict(synth.model_config_dict(shape))
+    model = ParallelTransformer.from_config(cfg, 1, 0, None)
+    model.load_rank_weights(RankWeights.from_shard(cfg, osh.shard_weights(full, 1, 0), 1, 0, shape.bits, shape.group_size, cuda))
+    run = lambda ids, past: asyncio.run(model.forward(ids, past_key_values=past))[0][0]  # noqa: E731
+    gen = np.random.default_rng(5)
+    words = lambda n: gen.integers(0, shape.vocab_size, n).tolist()  # noqa: E731
+    cache = PagedKVCache(cfg.num_layers, cfg.kv_heads, cfg.head_dim, 24, 3, 64, page_size=16, max_prefix=64, max_tokens=48, dtype=DT[dtype],
+                         device=cuda)
+    prefix = words(21)
+
+    def step(tokens):
+        """The new tokens of each request in, their logits out."""
+        cache.reserve([len(t) for t in tokens])
+        cache.check()
+        ids = sum(tokens, [])
+        out = run(torch.tensor([ids], device=cuda), cache.layers())
+        return torch.split(out, [len(t) for t in tokens])
+
+    def want(text):
+        return run(torch.tensor([text], device=cuda), model.new_cache(1, 128))
+
+    got = step([prefix, [], []])[0]
+    assert rel(got, want(prefix)) <= tol
+    cache.share_prefix(0)
+    held = [[], [], []]
+    for new_n, kept in [((5, 1, 9), None), ((1, 1, 1), None), ((4, 0, 3), (2, None, 0)), ((1, 1, 1), (None, "end", None)), ((2, 17, 1), None)]:
+        tokens = [words(n) for n in new_n]
+        outs = step(tokens)
+        for b in range(3):
+            if tokens[b]:
+                ref = want(prefix + held[b] + tokens[b])[-len(tokens[b]):]
+                assert rel(outs[b], ref) <= tol, (b, rel(outs[b], ref))
+        keep = []
+        for b in range(3):
+            k = None if kept is None else kept[b]
+            held[b] = [] if k == "end" else held[b] + (tokens[b] if k is None else tokens[b][:k])
+            keep.append(len(held[b]))
+        cache.truncate(keep)
+        cache.check()
+        assert cache.lens.tolist() == keep
+    with pytest.raises(ValueError):
+        cache.share_prefix(1)
+    with pytest.raises(ValueError):
+        cache.release_prefix()
+    cache.truncate([0, 0, 0])
+    cache.release_prefix()
+    cache.check()
+    assert int(cache.free_count) == 24 and sorted(cache.free_pages.tolist()) == list(range(24))
+    cache.reserve([64, 64, 64])
+    assert int(cache.status) == 4  # more rows than the cache was made for
+    with pytest.raises(ValueError, match="rows"):
+        cache.check()
+    assert cache.lens.tolist() == [0, 0, 0]
+    with pytest.raises(ValueError):
+        run(torch.zeros(1, 49, dtype=torch.long, device=cuda), cache.layers())
+
+
+def rel(a, b):
+    return float((a.double() - b.double()).norm() / b.double().norm())
+
+
 def test_on_another_stream(cuda, rng):
     d = make_attn(cuda, rng, "f16", 8, 2, 128, 16, 500, [40, 90, 33], [1, 1, 1])
     first = run_attn(cuda, d)
