@@ -1560,7 +1560,11 @@ static AttnPlan plan_attn(int T, int B, int Hkv, int G, int hd, bool f16, long l
   const int per_cta = f16 ? 2 * TC_M : TC_M, tile = f16 ? TC_N : TF_N;
   const long long rows = (long long)T * G, items = (rows + per_cta - 1) / per_cta;
   const auto ceil_div = [](long long x, long long y) { return (x + y - 1) / y; };
-  a.kind = rows >= 64ll * B ? AttnPlan::CHUNKS : prefix_keys > 0 && B > 1 ? AttnPlan::SHARED : AttnPlan::FEW;
+  // The few-rows kernel streams the prefix once per request.  While that is little it beats a kernel more (us in a graph,
+  // 8 kv heads of 128, fp16, few | shared: 2 requests behind 500 tokens 8.7 | 12.0, 1000 12.4 | 13.1, 2000 17.3 | 15.4;
+  // 8 behind 128 12.5 | 13.1, 500 16.2 | 13.3; fp32: 2 behind 1000 14.6 | 17.6, 2000 19.3 | 18.8).
+  a.kind = rows >= 64ll * B ? AttnPlan::CHUNKS : prefix_keys > 0 && B * prefix_keys > 2048 ? AttnPlan::SHARED : AttnPlan::FEW;
+  if (B == 1 && a.kind == AttnPlan::SHARED) a.kind = AttnPlan::FEW;  // nothing to share
   if (a.kind != AttnPlan::FEW) {
     // Shares of the keys until there is a CTA for every SM; with the own keys' kernel beside it, for this kernel's part
     // of the SMs only.  That part goes by the two kernels' work, as far as the host knows it: a tile takes an SM 2.1 us
@@ -1583,7 +1587,8 @@ static AttnPlan plan_attn(int T, int B, int Hkv, int G, int hd, bool f16, long l
     const int rt = f16 ? 16 : 8;
     const long long keys = own_keys + (a.kind == AttnPlan::FEW ? prefix_keys : 0);
     const long long want = ceil_div(4ll * sms, (long long)B * Hkv), groups = ceil_div(rows, (long long)B * rt);
-    a.row_groups = (int)std::max(1ll, std::min(want, groups));
+    // (row tiles are counted for the mean request: twice as many CTAs, so that one of twice the rows does not take twice as long)
+    a.row_groups = (int)std::max(1ll, std::min(want, groups > 1 ? 2 * groups : 1));
     a.splits = (int)std::max(1ll, std::min({ceil_div(want, a.row_groups), ceil_div(keys, 64), 64ll}));
     a.nslots += a.splits;
   }
