@@ -283,9 +283,14 @@ def _check(what: str, dev: int, ts: Sequence[torch.Tensor], dtype: Optional[torc
     """One pass over the tensors of a call, which a serving loop makes for every layer and token."""
     if dev < 0:
         _refuse(what, dev, ts, dtype)
-    for t in ts:
-        if t.get_device() != dev or (dtype is not None and t.dtype is not dtype) or not t.is_contiguous():
-            _refuse(what, dev, ts, dtype)
+    if dtype is None:
+        for t in ts:
+            if t.get_device() != dev or not t.is_contiguous():
+                _refuse(what, dev, ts, dtype)
+    else:
+        for t in ts:
+            if t.dtype is not dtype or t.get_device() != dev or not t.is_contiguous():
+                _refuse(what, dev, ts, dtype)
 
 
 def _sized(what: str, n: int, **named: Optional[torch.Tensor]) -> None:
@@ -333,8 +338,9 @@ def paged_reserve(lens: torch.Tensor, new_lens: torch.Tensor, block_table: torch
     status = new(1) if status is None else status
     ts = (lens, new_lens, block_table, free_pages, free_count, kv_lens, q_start, slots, positions, free_count_out, status)
     _check("paged_reserve", dev, ts if prefix_len is None else (*ts, prefix_len), _I32)
-    if block_table.dim() != 2 or block_table.shape[0] != B:
-        raise ValueError(f"paged_reserve: block_table {tuple(block_table.shape)} is not [{B}, max_blocks]")
+    tab = block_table.shape
+    if len(tab) != 2 or tab[0] != B:
+        raise ValueError(f"paged_reserve: block_table {tuple(tab)} is not [{B}, max_blocks]")
     if (new_lens.numel() != B or kv_lens.numel() != B or q_start.numel() != B + 1 or free_count.numel() != 1
             or free_count_out.numel() != 1 or status.numel() != 1 or (prefix_len is not None and prefix_len.numel() != 1)):
         _sized("paged_reserve", B, new_lens=new_lens, kv_lens=kv_lens)
@@ -343,7 +349,7 @@ def paged_reserve(lens: torch.Tensor, new_lens: torch.Tensor, block_table: torch
     if slots.numel() < rows or positions.numel() < rows:
         raise ValueError(f"paged_reserve: slots and positions hold {slots.numel()} and {positions.numel()} rows, {rows} are needed")
     _call_on(dev, "sc_paged_reserve", lens.data_ptr(), new_lens.data_ptr(), B, _p(prefix_len), block_table.data_ptr(),
-             block_table.shape[1], free_pages.data_ptr(), free_pages.numel(), free_count.data_ptr(), page_size, rows,
+             tab[1], free_pages.data_ptr(), free_pages.numel(), free_count.data_ptr(), page_size, rows,
              kv_lens.data_ptr(), q_start.data_ptr(), slots.data_ptr(), positions.data_ptr(), free_count_out.data_ptr(),
              status.data_ptr())
     return PagedStep(kv_lens, q_start, slots, positions, free_count_out, status)
@@ -361,24 +367,25 @@ def paged_truncate(lens: torch.Tensor, keep: torch.Tensor, block_table: torch.Te
     free_count_out = torch.empty_like(free_count) if free_count_out is None else free_count_out
     status = torch.empty(1, dtype=_I32, device=lens.device) if status is None else status
     _check("paged_truncate", dev, (lens, keep, block_table, free_pages, free_count, lens_out, free_count_out, status), _I32)
-    if block_table.dim() != 2 or block_table.shape[0] != B:
-        raise ValueError(f"paged_truncate: block_table {tuple(block_table.shape)} is not [{B}, max_blocks]")
+    tab = block_table.shape
+    if len(tab) != 2 or tab[0] != B:
+        raise ValueError(f"paged_truncate: block_table {tuple(tab)} is not [{B}, max_blocks]")
     if keep.numel() != B or lens_out.numel() != B or free_count.numel() != 1 or free_count_out.numel() != 1 or status.numel() != 1:
         _sized("paged_truncate", B, keep=keep, lens_out=lens_out)
         _sized("paged_truncate", 1, free_count=free_count, free_count_out=free_count_out, status=status)
-    _call_on(dev, "sc_paged_truncate", lens.data_ptr(), keep.data_ptr(), B, block_table.data_ptr(), block_table.shape[1],
+    _call_on(dev, "sc_paged_truncate", lens.data_ptr(), keep.data_ptr(), B, block_table.data_ptr(), tab[1],
              free_pages.data_ptr(), free_pages.numel(), free_count.data_ptr(), page_size, lens_out.data_ptr(),
              free_count_out.data_ptr(), status.data_ptr())
     return lens_out, free_count_out, status
 
 
 def _pools(what: str, k_pages: torch.Tensor, v_pages: torch.Tensor):
-    if k_pages.dim() != 4 or k_pages.shape != v_pages.shape:
-        raise ValueError(f"{what}: k_pages {tuple(k_pages.shape)} and v_pages {tuple(v_pages.shape)} must be one "
-                         "[n_pages, Hkv, page, hd]")
-    if k_pages.dtype != v_pages.dtype or k_pages.dtype not in (_F16, _F32):
-        raise ValueError(f"{what}: pages must both be float16 or float32, got {k_pages.dtype} and {v_pages.dtype}")
-    return k_pages.shape
+    shape, dt = k_pages.shape, k_pages.dtype
+    if len(shape) != 4 or shape != v_pages.shape:
+        raise ValueError(f"{what}: k_pages {tuple(shape)} and v_pages {tuple(v_pages.shape)} must be one [n_pages, Hkv, page, hd]")
+    if dt is not v_pages.dtype or (dt is not _F16 and dt is not _F32):
+        raise ValueError(f"{what}: pages must both be float16 or float32, got {dt} and {v_pages.dtype}")
+    return shape
 
 
 def paged_rope_append(qkv: torch.Tensor, q_start: torch.Tensor, slots: torch.Tensor, positions: torch.Tensor,
@@ -434,45 +441,50 @@ def prefix_attn(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, q
     there); a row that sees no token is zero; pages outside the pool count as absent.  ``workspace``: uint8, at least
     ``prefix_attn_workspace_bytes``; without it scratch is allocated per call, so calls on two streams do not meet."""
     n_pages, Hkv, page, hd = _pools("prefix_attn", k_pages, v_pages)
-    T = q.shape[0] if q.dim() else 0
     if out is None:
         out = torch.zeros_like(q)
-    dev = q.get_device()
+    dev, dt = q.get_device(), k_pages.dtype
     _check("prefix_attn", dev, (q, k_pages, v_pages, out))
-    ints = (q_start, kv_lens, block_table)
+    nbp, pt, pl = 0, None, None
     if prefix_len is not None and prefix_table is not None:
-        ints = (q_start, kv_lens, block_table, prefix_table, prefix_len)
-    _check("prefix_attn", dev, ints, _I32)
-    B = kv_lens.numel()
-    if q.dtype != k_pages.dtype or out.dtype != q.dtype or out.numel() != q.numel():
-        raise ValueError(f"prefix_attn: q and out must have the pages' type {k_pages.dtype} and one size, got {q.dtype} "
-                         f"{tuple(q.shape)} and {out.dtype} {tuple(out.shape)}")
-    Hq = q.numel() // (T * hd) if T else Hkv
-    if T and Hq * T * hd != q.numel():
-        raise ValueError(f"prefix_attn: q rows of {q.numel() // T} are no multiple of head_dim {hd}")
-    if block_table.dim() != 2 or block_table.shape[0] != B:
-        raise ValueError(f"prefix_attn: block_table {tuple(block_table.shape)} is not [{B}, max_blocks]")
-    _sized("prefix_attn", B + 1, q_start=q_start)
-    if (prefix_len is None) != (prefix_table is None):
+        _check("prefix_attn", dev, (q_start, kv_lens, block_table, prefix_table, prefix_len), _I32)
+        if prefix_len.numel() != 1:
+            _sized("prefix_attn", 1, prefix_len=prefix_len)
+        nbp, pt, pl = prefix_table.numel(), prefix_table.data_ptr(), prefix_len.data_ptr()
+    elif prefix_len is None and prefix_table is None:
+        _check("prefix_attn", dev, (q_start, kv_lens, block_table), _I32)
+    else:
         raise ValueError("prefix_attn: prefix_table and prefix_len go together")
-    nbp = 0
-    if prefix_len is not None:
-        _sized("prefix_attn", 1, prefix_len=prefix_len)
-        nbp = prefix_table.numel()
+    B, nq = kv_lens.numel(), q.numel()
+    T = q.shape[0] if q.dim() else 0
+    if q.dtype is not dt or out.dtype is not dt or out.numel() != nq:
+        raise ValueError(f"prefix_attn: q and out must have the pages' type {dt} and one size, got {q.dtype} "
+                         f"{tuple(q.shape)} and {out.dtype} {tuple(out.shape)}")
+    Hq = nq // (T * hd) if T else Hkv
+    if T and Hq * T * hd != nq:
+        raise ValueError(f"prefix_attn: q rows of {nq // T} are no multiple of head_dim {hd}")
+    tab = block_table.shape
+    if len(tab) != 2 or tab[0] != B:
+        raise ValueError(f"prefix_attn: block_table {tuple(tab)} is not [{B}, max_blocks]")
+    if q_start.numel() != B + 1:
+        _sized("prefix_attn", B + 1, q_start=q_start)
     if not T or not B:
         return out
-    sc = (1.0 / math.sqrt(hd)) if scale is None else float(scale)
-    nbytes = prefix_attn_workspace_bytes(T, B, Hq, Hkv, hd, block_table.shape[1], nbp, page, q.dtype)
-    if workspace is None:
-        if nbytes:
-            workspace = torch.empty(nbytes, dtype=torch.uint8, device=q.device)
-    else:
+    code = L.SC_F16 if dt is _F16 else L.SC_F32
+    mb = tab[1]
+    nbytes = _prefix_attn_bytes(T, B, Hq, Hkv, hd, mb, nbp, page, code)
+    wp, wb = None, 0
+    if workspace is not None:
         _check("prefix_attn", dev, (workspace,))
         if workspace.dtype != torch.uint8:
             raise ValueError(f"prefix_attn: workspace must be uint8, got {workspace.dtype}")
-    _call_on(dev, "sc_prefix_attn", q.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), _dt(q), T, q_start.data_ptr(),
-             kv_lens.data_ptr(), block_table.data_ptr(), B, block_table.shape[1], _p(prefix_table), _p(prefix_len), nbp, Hq, Hkv,
-             hd, n_pages, page, sc, out.data_ptr(), _p(workspace), workspace.numel() if workspace is not None else 0)
+        wp, wb = workspace.data_ptr(), workspace.numel()
+    elif nbytes:
+        workspace = torch.empty(nbytes, dtype=torch.uint8, device=dev)
+        wp, wb = workspace.data_ptr(), nbytes
+    _call_on(dev, "sc_prefix_attn", q.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), code, T, q_start.data_ptr(),
+             kv_lens.data_ptr(), block_table.data_ptr(), B, mb, pt, pl, nbp, Hq, Hkv, hd, n_pages, page,
+             1.0 / math.sqrt(hd) if scale is None else float(scale), out.data_ptr(), wp, wb)
     return out
 
 
