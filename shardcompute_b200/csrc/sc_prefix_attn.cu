@@ -149,10 +149,23 @@ few_rows_kernel(const PrefixAttnParams p, const __grid_constant__ PoolMaps maps,
   // this one starts: what both read is there, and they run side by side.  One CTA, the last to be placed, waits for
   // that kernel before it ends, so that the join, which waits for this one, has both results.
   if (with_prefix) pdl_wait();
+  const int P = with_prefix ? prefix_keys(p) : 0, np = (P + KT - 1) / KT;
+  const int t0 = split * FR_WARPS + warp, step = splits * FR_WARPS;
+  // the pool rows of this warp's tiles first .. first + 31, one per lane; -1: no such page
+  auto rows_of = [&](int first) {
+    const long long t = t0 + (long long)step * (first + lane);
+    const bool pre = t < np;
+    const long long key = (pre ? t : t - np) * KT;
+    const int blk = (int)min(key >> p.lg_page, (long long)INT32_MAX);
+    if (blk >= (pre ? p.max_prefix_blocks : p.max_blocks)) return -1;
+    const int id = pre ? p.prefix_table[blk] : p.block_table[(size_t)b * p.max_blocks + blk];
+    if (id < 0 || id >= p.n_pages) return -1;
+    return ((id * p.Hkv + h) << p.lg_page) + ((int)key & ((1 << p.lg_page) - 1));
+  };
+  const int rows0 = rows_of(0);
   int row_lo, row_hi;
   request_rows(p, b, row_lo, row_hi);
-  const int n = row_hi - row_lo, len = request_len(p, b), P = with_prefix ? prefix_keys(p) : 0;
-  const int np = (P + KT - 1) / KT;
+  const int n = row_hi - row_lo, len = request_len(p, b);
   unsigned char* ring = base + (size_t)warp * NST * C::STAGE;
   const uint32_t ring_u = smem_u32(ring);
   uint32_t issued = 0, used = 0;  // tiles of this warp's ring, over all row tiles
@@ -162,22 +175,11 @@ few_rows_kernel(const PrefixAttnParams p, const __grid_constant__ PoolMaps maps,
     // own keys that the tile's last row sees
     const int own = max(0, min(len, len - n + (r0 + nr - 1) / p.G + 1));
     const int nt = np + (own + KT - 1) / KT;
-    const int per = (nt + splits - 1) / splits;
-    const int t_lo = min(nt, split * per), t_hi = min(nt, t_lo + per);
-    const int cnt = max(0, (t_hi - t_lo - warp + FR_WARPS - 1) / FR_WARPS);  // tiles t_lo + warp + 4 i
+    // This warp's tiles are t0 + step i, whatever the lengths are: without a prefix the first page ids are asked for
+    // before the lengths are there.
+    const int cnt = max(0, (nt - t0 + step - 1) / step);
 
-    // the pool rows of this warp's tiles i = base .. base + 31, one per lane; -1: no such page
-    auto rows_of = [&](int first) {
-      const int t = t_lo + warp + FR_WARPS * (first + lane);
-      if (t >= t_hi) return -1;
-      const bool pre = t < np;
-      const int key = (pre ? t : t - np) * KT;
-      const int blk = key >> p.lg_page;
-      const int id = pre ? p.prefix_table[blk] : p.block_table[(size_t)b * p.max_blocks + blk];
-      if (id < 0 || id >= p.n_pages) return -1;
-      return ((id * p.Hkv + h) << p.lg_page) + (key & ((1 << p.lg_page) - 1));
-    };
-    int rows = rows_of(0);
+    int rows = rows0;
     uint32_t absent = 0;  // stages whose tile has no page
     auto issue = [&](int i) {
       if (i && (i & 31) == 0) rows = rows_of(i);
@@ -245,7 +247,7 @@ few_rows_kernel(const PrefixAttnParams p, const __grid_constant__ PoolMaps maps,
       const int s = used % NST;
       if (!mbar_wait_warp(&full[warp][s], (used / NST) & 1u, &s_abort, PA_WAIT_NS)) break;
       const uint32_t ks_u = ring_u + s * C::STAGE, vs_u = ks_u + C::TILE;
-      const int t = t_lo + warp + FR_WARPS * i;
+      const int t = t0 + step * i;
       const bool gone = (absent >> s) & 1u;
       const int first = (t < np ? t : t - np) * KT;
       const bool part = gone || (t < np ? P : see_first) - first < KT;  // not every row sees every key
@@ -953,25 +955,16 @@ many_rows_kernel(const PrefixAttnParams p, const __grid_constant__ PoolMaps maps
             pw[k / 2] = h2_as_u32(__floats2half2_rn(e0, e1));
           }
         };
-        bool known = __any_sync(0xffffffffu, m == -INFINITY);  // the tile's maximum has been looked at
-        if (known) raise(row_max());
+        const float mx = row_max();
+        if (__any_sync(0xffffffffu, mx > m + TC_RAISE)) raise(mx);  // also from -inf
         // The two warps of a scheduler take turns here, or both tiles fall into step: both in the softmax, then both
         // in the tensor cores.
         if (nx == 2 && (x == 1 || i > 0)) {
           ok = __all_sync(0xffffffffu, pa_wait(&turn[x][warp & 3], (x == 1 ? i : i - 1) & 1, abort));
           if (!ok) break;
         }
-        // The first quarter's P is taken with the maximum so far while the tile's is found, which the MUFU's pace
-        // leaves room for; it seldom has to be taken again.
-        for (;;) {
-          l2[0] = l2[1] = pack2(0.f, 0.f);
-          quarter(0);
-          if (known) break;
-          const float mx = row_max();
-          if (!__any_sync(0xffffffffu, mx > m + TC_RAISE)) break;
-          raise(mx);
-          known = true;
-        }
+        l2[0] = l2[1] = pack2(0.f, 0.f);
+        quarter(0);
         tmem_st16(st, pw);  // over columns of S that have been read
 #pragma unroll
         for (int q = 1; q < TC_N / 32; ++q) {
@@ -1455,9 +1448,9 @@ template <typename T, int HD>
 __global__ void __launch_bounds__(256) join_slots_kernel(const PrefixAttnParams p) {
   pdl_trigger();
   pdl_wait();
-  const int rows = min(max(p.q_start[p.B], 0), p.T) * p.Hq;
   const int row = blockIdx.x * (blockDim.x / 32) + (threadIdx.x >> 5), lane = threadIdx.x & 31;
-  if (row >= rows) return;
+  if (row >= p.T * p.Hq) return;
+  const int end = p.q_start[p.B];  // on its way together with the weights
   const size_t stride = (size_t)p.T * p.Hq;
   constexpr int V = HD / 32, SETS = 3;  // at most 96 slots
   float2 ml[SETS];
@@ -1467,6 +1460,7 @@ __global__ void __launch_bounds__(256) join_slots_kernel(const PrefixAttnParams 
     ml[k] = k * 32 + lane < p.nslots ? p.part_ml[(k * 32 + lane) * stride + row] : make_float2(-INFINITY, 0.f);
     M = fmaxf(M, ml[k].x);
   }
+  if (row >= min(max(end, 0), p.T) * p.Hq) return;
 #pragma unroll
   for (int d = 16; d; d >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, d));
   float acc[V], L = 0.f;
