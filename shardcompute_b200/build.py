@@ -2,7 +2,9 @@
 
 ``python -m shardcompute_b200.build`` compiles every ``csrc/*.cu`` with nvcc
 for ``sm_100a`` only and links them, with NCCL, into
-``shardcompute_b200/libsc_b200.so``.  Object files go to
+``shardcompute_b200/libsc_b200.so``, and builds the Python binding
+``csrc/sc_binding.cpp`` against torch's headers into
+``shardcompute_b200/_native.so``.  Object files go to
 ``shardcompute_b200/_build/``; a source is recompiled when it or a header is
 newer than its object.  No GPU is needed (nvcc cross-compiles).
 """
@@ -22,6 +24,8 @@ CSRC = os.path.join(PKG, "csrc")
 INCLUDE = os.path.join(ROOT, "include")
 BUILD = os.path.join(PKG, "_build")
 LIB = os.path.join(PKG, "libsc_b200.so")
+BINDING = os.path.join(CSRC, "sc_binding.cpp")
+NATIVE = os.path.join(PKG, "_native.so")
 
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 CFLAGS = ["-O3", "-lineinfo", "-std=c++17", "-Xcompiler", "-fPIC", "--expt-relaxed-constexpr"]
@@ -45,6 +49,28 @@ def nccl_dirs():
         if os.path.exists(os.path.join(inc, "nccl.h")) and glob.glob(os.path.join(lib, "libnccl.so*")):
             return inc, lib
     raise RuntimeError("NCCL headers/library (nvidia-nccl wheel) not found")
+
+
+def build_binding(force: bool = False) -> str:
+    """The extension module that calls the paged operators from torch tensors (host code, linked with libsc_b200.so)."""
+    import importlib.util
+    import sysconfig
+
+    if not force and os.path.exists(NATIVE) and os.path.getmtime(NATIVE) >= _newest([BINDING, os.path.join(INCLUDE, "sc_b200.h")]):
+        return NATIVE
+    torch_dir = list(importlib.util.find_spec("torch").submodule_search_locations)[0]
+    inc = [sysconfig.get_paths()["include"], os.path.join(torch_dir, "include"), os.path.join(torch_dir, "include", "torch", "csrc", "api", "include"),
+           os.path.join(os.path.dirname(os.path.dirname(_nvcc())), "include"), INCLUDE]
+    lib = os.path.join(torch_dir, "lib")
+    cxx = shutil.which("g++") or shutil.which("c++")
+    if not cxx:
+        raise RuntimeError("a C++ compiler is required to build _native.so")
+    cmd = [cxx, "-O2", "-std=c++17", "-fPIC", "-shared", "-o", NATIVE, BINDING, *[f"-I{d}" for d in inc if os.path.isdir(d)], f"-L{PKG}",
+           "-l:libsc_b200.so", f"-L{lib}", "-ltorch_python", "-ltorch_cpu", "-lc10", "-lc10_cuda", "-Wl,-rpath,$ORIGIN", f"-Wl,-rpath,{lib}"]
+    res = subprocess.run(cmd, capture_output=True, text=True)
+    if res.returncode != 0:
+        raise RuntimeError(f"building _native.so failed:\n{res.stdout}\n{res.stderr}")
+    return NATIVE
 
 
 def _newest(paths):
@@ -83,6 +109,7 @@ def build(verbose: bool = False, force: bool = False) -> str:
         res = subprocess.run(cmd, capture_output=True, text=True)
         if res.returncode != 0:
             raise RuntimeError(f"link failed:\n{res.stdout}\n{res.stderr}")
+    build_binding(force)
     return LIB
 
 

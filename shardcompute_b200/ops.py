@@ -299,6 +299,23 @@ def _sized(what: str, n: int, **named: Optional[torch.Tensor]) -> None:
             raise ValueError(f"{what}: {name} holds {t.numel()} values, {n} are needed")
 
 
+_bound = None
+
+
+def _native():
+    """The binding of the paged operators (csrc/sc_binding.cpp): each of its functions checks the tensors and makes the call in
+    one go, and returns the status, or -1 where the checks below have to say what is wrong or the device has to be changed."""
+    global _bound
+    if _bound is None:
+        L.load()
+        try:
+            from . import _native as m
+        except ImportError as e:
+            raise RuntimeError(f"_native.so is missing or does not load ({e}); build it with `python -m shardcompute_b200.build`") from e
+        _bound = m
+    return _bound
+
+
 def _call_on(dev: int, name: str, *args) -> None:
     """The call with device ``dev`` as the current one, on its current stream."""
     if dev == torch._C._cuda_getDevice():
@@ -323,7 +340,6 @@ def paged_reserve(lens: torch.Tensor, new_lens: torch.Tensor, block_table: torch
     ``kv_lens`` may be ``lens`` and ``free_count_out`` may be ``free_count``.  If ``status`` is not 0 nothing was
     reserved and ``q_start`` is all zeros: 1 not enough pages, 2 a request exceeds ``max_blocks`` pages, 4 more than
     ``max_tokens`` new tokens, 8 a negative length, 16 ``free_count`` outside the stack (the sum of those that hold)."""
-    B, dev = lens.numel(), lens.get_device()
     if slots is None:
         if max_tokens is None:
             raise ValueError("paged_reserve: max_tokens or slots is needed")
@@ -332,10 +348,15 @@ def paged_reserve(lens: torch.Tensor, new_lens: torch.Tensor, block_table: torch
     if positions is None:
         positions = torch.full((rows,), -1, dtype=_I32, device=lens.device)
     new = lambda n: torch.empty(n, dtype=_I32, device=lens.device)  # noqa: E731
-    kv_lens = new(B) if kv_lens is None else kv_lens
-    q_start = new(B + 1) if q_start is None else q_start
+    kv_lens = new(lens.numel()) if kv_lens is None else kv_lens
+    q_start = new(lens.numel() + 1) if q_start is None else q_start
     free_count_out = new(1) if free_count_out is None else free_count_out
     status = new(1) if status is None else status
+    st = _native().paged_reserve(lens, new_lens, block_table, free_pages, free_count, page_size, rows, prefix_len, kv_lens, q_start, slots,
+                                 positions, free_count_out, status)
+    if st == 0:
+        return PagedStep(kv_lens, q_start, slots, positions, free_count_out, status)
+    B, dev = lens.numel(), lens.get_device()
     ts = (lens, new_lens, block_table, free_pages, free_count, kv_lens, q_start, slots, positions, free_count_out, status)
     _check("paged_reserve", dev, ts if prefix_len is None else (*ts, prefix_len), _I32)
     tab = block_table.shape
@@ -362,10 +383,13 @@ def paged_truncate(lens: torch.Tensor, keep: torch.Tensor, block_table: torch.Te
     back on the stack.  ``lens_out`` may be ``lens``, ``free_count_out`` may be ``free_count``.  Returns ``(lens_out,
     free_count_out, status)``; unless ``status`` is 0 nothing changed (1: the stack has no room, as when a page is given
     back twice; 2, 8, 16 as for ``paged_reserve``)."""
-    B, dev = lens.numel(), lens.get_device()
     lens_out = torch.empty_like(lens) if lens_out is None else lens_out
     free_count_out = torch.empty_like(free_count) if free_count_out is None else free_count_out
     status = torch.empty(1, dtype=_I32, device=lens.device) if status is None else status
+    st = _native().paged_truncate(lens, keep, block_table, free_pages, free_count, page_size, lens_out, free_count_out, status)
+    if st == 0:
+        return lens_out, free_count_out, status
+    B, dev = lens.numel(), lens.get_device()
     _check("paged_truncate", dev, (lens, keep, block_table, free_pages, free_count, lens_out, free_count_out, status), _I32)
     tab = block_table.shape
     if len(tab) != 2 or tab[0] != B:
@@ -394,6 +418,9 @@ def paged_rope_append(qkv: torch.Tensor, q_start: torch.Tensor, slots: torch.Ten
     """``rope_append`` for a paged cache: q and k of each row (``qkv`` [T, (Hq + 2 Hkv) hd], float16 or float32) rotated
     at ``positions``, k and v written to ``slots`` of the pools, q to ``q_out`` [T, Hq hd] in the pools' type.  Rows from
     ``q_start[-1]`` on are left as they were; a slot outside the pool or a position past the tables is not written."""
+    st = _native().paged_rope_append(qkv, q_start, slots, positions, cos_tab, sin_tab, q_out, k_pages, v_pages)
+    if st == 0:
+        return q_out
     dev = qkv.get_device()
     _check("paged_rope_append", dev, (qkv, cos_tab, sin_tab, q_out, k_pages, v_pages))
     _check("paged_rope_append", dev, (q_start, slots, positions), _I32)
@@ -440,9 +467,12 @@ def prefix_attn(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, q
     the pools' type.  Rows from ``q_start[-1]`` on are left as they were (an ``out`` that is allocated here is zero
     there); a row that sees no token is zero; pages outside the pool count as absent.  ``workspace``: uint8, at least
     ``prefix_attn_workspace_bytes``; without it scratch is allocated per call, so calls on two streams do not meet."""
-    n_pages, Hkv, page, hd = _pools("prefix_attn", k_pages, v_pages)
     if out is None:
         out = torch.zeros_like(q)
+    st = _native().prefix_attn(q, k_pages, v_pages, q_start, kv_lens, block_table, prefix_table, prefix_len, out, scale, workspace)
+    if st == 0:
+        return out
+    n_pages, Hkv, page, hd = _pools("prefix_attn", k_pages, v_pages)
     dev, dt = q.get_device(), k_pages.dtype
     _check("prefix_attn", dev, (q, k_pages, v_pages, out))
     nbp, pt, pl = 0, None, None
