@@ -13,7 +13,10 @@
 namespace sc {
 
 constexpr int PG_THREADS = 1024;
-constexpr int PG_RUN = 4;        // consecutive rows or pages of a thread
+// Consecutive rows or pages of a thread.  Reservation: one while the cluster's threads last (8 requests, 8 rows: 8 4.3 us,
+// 1 3.0 us), else eight (1500 requests, 38000 rows: 4 11.4 us, 8 9.4 us).  Truncation, whose pages lie in many requests'
+// tables (1024 requests, 7000 pages): 8 8.8 us, 4 5.4 us, 2 5.1 us.
+constexpr int PG_RUN = 8, PG_RUN_BACK = 2;
 constexpr int PG_MAX_BATCH = 16384;  // a request's scan state is 12 bytes of shared memory: 192 KB
 
 __device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
@@ -94,11 +97,12 @@ struct ReserveParams {
 // One cluster.  Every CTA scans all requests (new tokens, new pages) into its
 // own shared memory, so each knows every offset and the status without a
 // message; then the rows, the pages and the requests are spread over the
-// cluster's threads, four consecutive rows or pages a thread, which finds the
+// cluster's threads, a run of rows or pages a thread, which finds the
 // first one's request by binary search in shared memory and walks on.  The one cluster barrier separates the reads of lens and
 // free_count from the writes of kv_lens and free_out, which may be the same
 // arrays.  Bound by latency: launch, one round trip for the lengths, one for
 // the pages.
+template <int RUN>
 __global__ void __launch_bounds__(PG_THREADS) paged_reserve_kernel(const ReserveParams p) {
   extern __shared__ int pg_smem[];
   int* s_end = pg_smem;            // new tokens of requests 0..b
@@ -111,43 +115,48 @@ __global__ void __launch_bounds__(PG_THREADS) paged_reserve_kernel(const Reserve
   pdl_wait();
   if (threadIdx.x == 0) s_bad = 0;
   __syncthreads();
-  const int count = *p.free_count;
+  const int count = *p.free_count, prefix = p.prefix_len ? *p.prefix_len : 0;
   const long long cap = (long long)p.max_blocks * p.page.d;
+  // a thread takes consecutive requests: its own sums, one scan of those, then the sums up to each request
+  const int each = (p.B + blockDim.x - 1) / blockDim.x, b_lo = min(p.B, (int)threadIdx.x * each), b_hi = min(p.B, b_lo + each);
   long long end0 = 0, take0 = 0;
-  for (int b0 = 0; b0 < p.B; b0 += blockDim.x) {
-    const int b = b0 + threadIdx.x;
-    long long a = 0, t = 0;
-    if (b < p.B) {
-      const int len = p.lens[b], add = p.new_lens[b];
-      const long long kv = (long long)len + add;
-      int bad = 0;
-      if (len < 0 || add < 0) bad |= 8;
-      if (kv > cap) bad |= 2;
-      if (bad) atomicOr(&s_bad, bad);
-      if (!(bad & 8)) {
-        a = add;
-        // past 32 bits only where it does not fit the table either
-        t = kv <= INT32_MAX ? p.page.up((int)kv) - p.page.up(len) : (kv - len) / p.page.d;
-      }
-      s_len[b] = len;
+  int bad = 0;
+  for (int b = b_lo; b < b_hi; ++b) {
+    const int len = p.lens[b], add = p.new_lens[b];
+    const long long kv = (long long)len + add;
+    int a = 0, t = 0;
+    if (len < 0 || add < 0) {
+      bad |= 8;
+    } else {
+      a = add;
+      // past 32 bits only where it does not fit the table either
+      t = kv <= INT32_MAX ? p.page.up((int)kv) - p.page.up(len) : (int)((kv - len) / p.page.d);
     }
-    block_scan2(a, t, s_w);
-    a += end0;
-    t += take0;
-    if (b < p.B) {
-      s_end[b] = (int)min(a, (long long)INT32_MAX);
-      s_take[b] = (int)min(t, (long long)INT32_MAX);
-    }
-    if (threadIdx.x == blockDim.x - 1) {
-      s_tot[0] = a;
-      s_tot[1] = t;
-    }
-    __syncthreads();
-    end0 = s_tot[0];
-    take0 = s_tot[1];
-    __syncthreads();
+    if (kv > cap) bad |= 2;
+    s_len[b] = len;
+    s_end[b] = a;
+    s_take[b] = t;
+    end0 += a;
+    take0 += t;
   }
-  const int prefix = p.prefix_len ? *p.prefix_len : 0;
+  if (bad) atomicOr(&s_bad, bad);
+  long long ea = end0, ta = take0;
+  block_scan2(ea, ta, s_w);
+  if (threadIdx.x == blockDim.x - 1) {
+    s_tot[0] = ea;
+    s_tot[1] = ta;
+  }
+  ea -= end0;
+  ta -= take0;
+  for (int b = b_lo; b < b_hi; ++b) {
+    ea += s_end[b];
+    ta += s_take[b];
+    s_end[b] = (int)min(ea, (long long)INT32_MAX);
+    s_take[b] = (int)min(ta, (long long)INT32_MAX);
+  }
+  __syncthreads();
+  end0 = s_tot[0];
+  take0 = s_tot[1];
   int st = s_bad;
   if (take0 > count) st |= 1;
   if (end0 > p.max_tokens) st |= 4;
@@ -156,10 +165,11 @@ __global__ void __launch_bounds__(PG_THREADS) paged_reserve_kernel(const Reserve
   const int nthr = (int)cluster_size() * blockDim.x, tid = (int)cluster_rank() * blockDim.x + threadIdx.x;
   const bool wide = (((uintptr_t)p.slots | (uintptr_t)p.positions) & 15) == 0;
   if (st == 0) {
-    for (int n0 = tid * PG_RUN; n0 < (int)take0; n0 += PG_RUN * nthr) {
+    // the pages by the threads from the cluster's other end: few are needed, and the rows' are busy
+    for (int n0 = (nthr - 1 - tid) * RUN; n0 < (int)take0; n0 += RUN * nthr) {
       int b = first_above(s_take, p.B, n0);
 #pragma unroll
-      for (int i = 0; i < PG_RUN; ++i) {
+      for (int i = 0; i < RUN; ++i) {
         const int n = n0 + i;
         if (n >= (int)take0) break;
         while (s_take[b] <= n) ++b;
@@ -167,11 +177,11 @@ __global__ void __launch_bounds__(PG_THREADS) paged_reserve_kernel(const Reserve
         p.block_table[(size_t)b * p.max_blocks + j] = p.free_pages[count - 1 - n];
       }
     }
-    for (int t0 = tid * PG_RUN; t0 < (int)end0; t0 += PG_RUN * nthr) {
+    for (int t0 = tid * RUN; t0 < (int)end0; t0 += RUN * nthr) {
       int b = first_above(s_end, p.B, t0);
-      int at[PG_RUN], off[PG_RUN], id[PG_RUN];
+      int at[RUN], off[RUN], id[RUN];
 #pragma unroll
-      for (int i = 0; i < PG_RUN; ++i) {
+      for (int i = 0; i < RUN; ++i) {
         const int t = min(t0 + i, (int)end0 - 1);
         while (s_end[b] <= t) ++b;
         const int len = s_len[b];
@@ -182,13 +192,17 @@ __global__ void __launch_bounds__(PG_THREADS) paged_reserve_kernel(const Reserve
         id[i] = j < have ? p.block_table[(size_t)b * p.max_blocks + j]
                          : p.free_pages[count - 1 - (b ? s_take[b - 1] : 0) - (j - have)];
       }
-      if (wide && t0 + PG_RUN <= (int)end0) {
-        *reinterpret_cast<int4*>(p.slots + t0) = make_int4(id[0] * p.page.d + off[0], id[1] * p.page.d + off[1],
-                                                           id[2] * p.page.d + off[2], id[3] * p.page.d + off[3]);
-        *reinterpret_cast<int4*>(p.positions + t0) = make_int4(prefix + at[0], prefix + at[1], prefix + at[2], prefix + at[3]);
+      if (RUN >= 4 && wide && t0 + RUN <= (int)end0) {
+#pragma unroll
+        for (int i = 0; i + 3 < RUN; i += 4) {
+          *reinterpret_cast<int4*>(p.slots + t0 + i) = make_int4(id[i] * p.page.d + off[i], id[i + 1] * p.page.d + off[i + 1],
+                                                                 id[i + 2] * p.page.d + off[i + 2], id[i + 3] * p.page.d + off[i + 3]);
+          *reinterpret_cast<int4*>(p.positions + t0 + i) =
+              make_int4(prefix + at[i], prefix + at[i + 1], prefix + at[i + 2], prefix + at[i + 3]);
+        }
       } else {
 #pragma unroll
-        for (int i = 0; i < PG_RUN; ++i) {
+        for (int i = 0; i < RUN; ++i) {
           if (t0 + i >= (int)end0) break;
           p.slots[t0 + i] = id[i] * p.page.d + off[i];
           p.positions[t0 + i] = prefix + at[i];
@@ -233,31 +247,35 @@ __global__ void __launch_bounds__(PG_THREADS) paged_truncate_kernel(const Trunca
   __syncthreads();
   const int count = *p.free_count;
   const long long cap = (long long)p.max_blocks * p.page.d;
-  long long give0 = 0;
-  for (int b0 = 0; b0 < p.B; b0 += blockDim.x) {
-    const int b = b0 + threadIdx.x;
-    long long g = 0, unused = 0;
-    if (b < p.B) {
-      const int len = p.lens[b];
-      const int kp = min(max(p.keep[b], 0), max(len, 0));
-      int bad = 0;
-      if (len < 0) bad |= 8;
-      if (len > cap) bad |= 2;
-      if (bad)
-        atomicOr(&s_bad, bad);
-      else
-        g = p.page.up(len) - p.page.up(kp);
-      s_len[b] = len;
-      s_keep[b] = kp;
-    }
-    block_scan2(g, unused, s_w);
-    g += give0;
-    if (b < p.B) s_give[b] = (int)min(g, (long long)INT32_MAX);
-    if (threadIdx.x == blockDim.x - 1) s_tot = g;
-    __syncthreads();
-    give0 = s_tot;
-    __syncthreads();
+  const int each = (p.B + blockDim.x - 1) / blockDim.x, b_lo = min(p.B, (int)threadIdx.x * each), b_hi = min(p.B, b_lo + each);
+  long long give0 = 0, unused = 0;
+  int bad = 0;
+  for (int b = b_lo; b < b_hi; ++b) {
+    const int len = p.lens[b];
+    const int kp = min(max(p.keep[b], 0), max(len, 0));
+    int g = 0;
+    if (len < 0)
+      bad |= 8;
+    else if (len > cap)
+      bad |= 2;
+    else
+      g = p.page.up(len) - p.page.up(kp);
+    s_len[b] = len;
+    s_keep[b] = kp;
+    s_give[b] = g;
+    give0 += g;
   }
+  if (bad) atomicOr(&s_bad, bad);
+  long long ga = give0;
+  block_scan2(ga, unused, s_w);
+  if (threadIdx.x == blockDim.x - 1) s_tot = ga;
+  ga -= give0;
+  for (int b = b_lo; b < b_hi; ++b) {
+    ga += s_give[b];
+    s_give[b] = (int)min(ga, (long long)INT32_MAX);
+  }
+  __syncthreads();
+  give0 = s_tot;
   int st = s_bad;
   if (count < 0 || count > p.n_free)
     st |= 16;
@@ -266,16 +284,16 @@ __global__ void __launch_bounds__(PG_THREADS) paged_truncate_kernel(const Trunca
   cluster_arrive();
   const int nthr = (int)cluster_size() * blockDim.x, tid = (int)cluster_rank() * blockDim.x + threadIdx.x;
   if (st == 0) {
-    for (int n0 = tid * PG_RUN; n0 < (int)give0; n0 += PG_RUN * nthr) {
-      int b = first_above(s_give, p.B, n0), id[PG_RUN];
+    for (int n0 = tid * PG_RUN_BACK; n0 < (int)give0; n0 += PG_RUN_BACK * nthr) {
+      int b = first_above(s_give, p.B, n0), id[PG_RUN_BACK];
 #pragma unroll
-      for (int i = 0; i < PG_RUN; ++i) {
+      for (int i = 0; i < PG_RUN_BACK; ++i) {
         const int n = min(n0 + i, (int)give0 - 1);
         while (s_give[b] <= n) ++b;
         id[i] = p.block_table[(size_t)b * p.max_blocks + p.page.up(s_keep[b]) + n - (b ? s_give[b - 1] : 0)];
       }
 #pragma unroll
-      for (int i = 0; i < PG_RUN; ++i)
+      for (int i = 0; i < PG_RUN_BACK; ++i)
         if (n0 + i < (int)give0) p.free_pages[count + n0 + i] = id[i];
     }
   }
@@ -290,12 +308,12 @@ __global__ void __launch_bounds__(PG_THREADS) paged_truncate_kernel(const Trunca
 // Launches one cluster with programmatic stream serialisation, for `items` rows or pages at most: CTAs of up to 1024
 // threads, up to the portable 8.
 template <typename P>
-static int launch_cluster(void (*kern)(const P), int items, size_t smem, cudaStream_t stream, const P& p, const char* what) {
+static int launch_cluster(void (*kern)(const P), int items, int run, size_t smem, cudaStream_t stream, const P& p, const char* what) {
   if (smem > (48u << 10)) {
     const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
     if (e != cudaSuccess) return check_launch(what, e);
   }
-  const long long threads = ((long long)items + PG_RUN - 1) / PG_RUN;
+  const long long threads = ((long long)items + run - 1) / run;
   const int ctas = (int)std::max(1ll, std::min(8ll, (threads + PG_THREADS - 1) / PG_THREADS));
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(ctas);
@@ -303,13 +321,14 @@ static int launch_cluster(void (*kern)(const P), int items, size_t smem, cudaStr
   cfg.dynamicSmemBytes = smem;
   cfg.stream = stream;
   cudaLaunchAttribute attr[2];
-  attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = ctas;
-  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
-  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[1].val.programmaticStreamSerializationAllowed = 1;
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchAttribute& cl = attr[pdl_enabled() ? 1 : 0];
+  cl.id = cudaLaunchAttributeClusterDimension;
+  cl.val.clusterDim.x = ctas;
+  cl.val.clusterDim.y = cl.val.clusterDim.z = 1;
   cfg.attrs = attr;
-  cfg.numAttrs = pdl_enabled() ? 2 : 1;
+  cfg.numAttrs = (pdl_enabled() ? 1 : 0) + (ctas > 1 ? 1 : 0);  // a CTA alone is a cluster without being told
   return check_launch(what, cudaLaunchKernelEx(&cfg, kern, p));
 }
 
@@ -436,7 +455,9 @@ int sc_paged_reserve(const int32_t* lens, const int32_t* new_lens, int B, const 
              SC_ERR_SHAPE, "paged_reserve: slots past 32 bits (%d pages of %d, %d blocks)", n_free, page_size, max_blocks);
   const ReserveParams p = {lens,        new_lens, prefix_len, free_pages, free_count, block_table, kv_lens, q_start, slots,
                            positions,   free_count_out, status, B, max_blocks, n_free, max_tokens, page_div(page_size)};
-  return launch_cluster(paged_reserve_kernel, max_tokens, (size_t)B * 12, stream, p, "paged_reserve");
+  const bool thin = max_tokens <= 8 * PG_THREADS;
+  return launch_cluster(thin ? paged_reserve_kernel<1> : paged_reserve_kernel<PG_RUN>, max_tokens, thin ? 1 : PG_RUN, (size_t)B * 12, stream,
+                        p, "paged_reserve");
 }
 
 int sc_paged_truncate(const int32_t* lens, const int32_t* keep, int B, const int32_t* block_table, int max_blocks,
@@ -451,7 +472,7 @@ int sc_paged_truncate(const int32_t* lens, const int32_t* keep, int B, const int
              SC_ERR_SHAPE, "paged_truncate: slots past 32 bits (%d pages of %d, %d blocks)", n_free, page_size, max_blocks);
   const TruncateParams p = {lens, keep, block_table, free_count, free_pages, lens_out, free_count_out, status, B,
                             max_blocks, n_free, page_div(page_size)};
-  return launch_cluster(paged_truncate_kernel, std::min(n_free, 16 * B), (size_t)B * 12, stream, p,
+  return launch_cluster(paged_truncate_kernel, std::min(n_free, 16 * B), PG_RUN_BACK, (size_t)B * 12, stream, p,
                         "paged_truncate");
 }
 
