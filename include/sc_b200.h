@@ -336,10 +336,12 @@ int sc_paged_rope_append(const void* qkv, int qkv_dtype, int rows, const int32_t
  *   hd 64 or 128; page_size a power of two, 16 or more; scale > 0.
  *   prefix_len NULL: no prefix.  Rows from q_start[B] on are left as they
  *   were; a row that sees no token is zero.  Pages whose id is outside
- *   0..n_pages-1 count as absent: their tokens are not seen.  What lies in a
- *   page behind a request's last token has no influence, whatever it is.
+ *   0..n_pages-1 count as absent: their tokens are not seen.  What a row does
+ *   not see has no influence on it, whatever it is (infinities and NaN too).
  * Softmax statistics and sums are fp32; with fp16 the weights are rounded to
- * fp16 before their product with v. */
+ * fp16 before their product with v.  With fp32, q, k and v are taken to 2^-21
+ * of each value; values that are not finite, or of 65520 or more in size (the
+ * range of the parts that the tensor cores take), make what sees them NaN. */
 size_t sc_prefix_attn_workspace_bytes(int T, int B, int Hq, int Hkv, int hd, int max_blocks, int max_prefix_blocks,
                                       int page_size, int dtype);
 int sc_prefix_attn(const void* q, const void* k_pages, const void* v_pages, int dtype, int T, const int32_t* q_start,

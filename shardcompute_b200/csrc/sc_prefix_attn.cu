@@ -123,6 +123,14 @@ __device__ __forceinline__ void split_tf32(float x, uint32_t& hi, uint32_t& lo) 
   lo = __float_as_uint(x - __uint_as_float(hi));
 }
 
+// Whether one of 16 bytes' values (fp16 or fp32) has all bits of its exponent set.
+template <typename T>
+__device__ __forceinline__ bool not_finite(const uint4& v) {
+  constexpr uint32_t mask = sizeof(T) == 2 ? 0x7c007c00u : 0x7f800000u, one = sizeof(T) == 2 ? 0x04000400u : 0x00800000u,
+                     top = sizeof(T) == 2 ? 0x80008000u : 0x80000000u;
+  return ((((v.x & mask) + one) | ((v.y & mask) + one) | ((v.z & mask) + one) | ((v.w & mask) + one)) & top) != 0;
+}
+
 template <typename T, int HD>
 __global__ void __launch_bounds__(FR_WARPS * 32)
 few_rows_kernel(const PrefixAttnParams p, const __grid_constant__ PoolMaps maps, int with_prefix, int splits, int row_groups,
@@ -341,7 +349,17 @@ few_rows_kernel(const PrefixAttnParams p, const __grid_constant__ PoolMaps maps,
         }
       }
       // ---- o += P V.  Slots behind the last key may hold anything: their V counts as zero.
-      const int lim = gone ? 0 : (t < np ? P : own) - first;  // keys that any row sees
+      const int lim = gone ? 0 : min(KT, (t < np ? P : own) - first);  // keys that any row sees
+      // whether V holds an infinity or NaN at a key that some of the rows see and some do not
+      auto hidden_not_finite = [&](uint32_t v, int end) {
+        const int from = t < np ? end : max(0, see_first - first);
+        bool bad = false;
+        for (int e = lane; e < (end - from) * C::NB * 8; e += 32) {
+          const int k = from + e / (C::NB * 8), c = e % (C::NB * 8);
+          bad |= not_finite<T>(lds_v4(v + (c >> 3) * SUB + k * 128 + ((c & 7) << 4)));
+        }
+        return __any_sync(0xffffffffu, bad) != 0;
+      };
       if constexpr (C::F16) {
         const uint32_t a0 = h2_as_u32(__floats2half2_rn(sc[0][0], sc[0][1])), a1 = h2_as_u32(__floats2half2_rn(sc[0][2], sc[0][3]));
         const uint32_t a2 = h2_as_u32(__floats2half2_rn(sc[NJ - 1][0], sc[NJ - 1][1])),
@@ -358,10 +376,50 @@ few_rows_kernel(const PrefixAttnParams p, const __grid_constant__ PoolMaps maps,
         };
         if (!part) {
           product(0xffffffffu, 0xffffffffu);
+        } else if (hidden_not_finite(vs_u, lim)) {
+          // a row's weight of zero must not meet the infinity or NaN of a token that it does not see
+          const int lim0 = see0 - first, lim1 = see1 - first;
+#pragma unroll 1
+          for (int k = 0; k < lim; ++k) {
+            const float y0 = k & 1 ? (k & 8 ? sc[NJ - 1][1] : sc[0][1]) : (k & 8 ? sc[NJ - 1][0] : sc[0][0]);
+            const float y1 = k & 1 ? (k & 8 ? sc[NJ - 1][3] : sc[0][3]) : (k & 8 ? sc[NJ - 1][2] : sc[0][2]);
+            const int from = (lane & ~3) | ((k & 7) >> 1);
+            const float p0 = __shfl_sync(0xffffffffu, y0, from), p1 = __shfl_sync(0xffffffffu, y1, from);
+#pragma unroll
+            for (int nb = 0; nb < NO; ++nb) {
+              const float2 v = __half22float2(u32_as_h2(lds_u32(vs_u + (nb >> 3) * SUB + k * 128 + (((nb & 7) ^ (k & 7)) << 4) + q4 * 4)));
+              if (k < lim0) {
+                o[nb][0] += p0 * v.x;
+                o[nb][1] += p0 * v.y;
+              }
+              if (k < lim1) {
+                o[nb][2] += p1 * v.x;
+                o[nb][3] += p1 * v.y;
+              }
+            }
+          }
         } else {
           const int key = q4 * 2;
           product((key < lim ? 0xffffu : 0u) | (key + 1 < lim ? 0xffff0000u : 0u),
                   (key + 8 < lim ? 0xffffu : 0u) | (key + 9 < lim ? 0xffff0000u : 0u));
+        }
+      } else if (part && hidden_not_finite(vs_u, lim)) {
+        const int lim0 = see0 - first;
+#pragma unroll 1
+        for (int k = 0; k < lim; ++k) {
+          const float p0 = __shfl_sync(0xffffffffu, k & 1 ? sc[0][1] : sc[0][0], (lane & ~3) | (k >> 1));
+          if (k >= lim0) continue;
+#pragma unroll
+          for (int dd = 0; dd < HD / 32; ++dd) {
+            const float4 va = lds_f4(vs_u + dd * SUB + k * 128 + (((2 * q4) ^ (k & 7)) << 4));
+            const float4 vb = lds_f4(vs_u + dd * SUB + k * 128 + (((2 * q4 + 1) ^ (k & 7)) << 4));
+            const float xa[4] = {va.x, va.y, va.z, va.w}, xb[4] = {vb.x, vb.y, vb.z, vb.w};
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              o[dd * 4 + e][0] += p0 * xa[e];
+              o[dd * 4 + e][1] += p0 * xb[e];
+            }
+          }
         }
       } else {
         uint32_t pa[4];
@@ -620,6 +678,7 @@ struct RowShare {
   int b, r0;               // request; first row, counted in the request (in the batch where PACKED)
   int row_lo, rows;        // the request's first token in q, its rows
   int n, len, P, np, own;  // its new tokens, its tokens; prefix keys, prefix tiles; own keys that the last row sees
+  int all;                 // own keys that every row sees
   int t_lo, cnt;           // tiles
   bool work;
 };
@@ -680,6 +739,7 @@ __device__ __forceinline__ RowShare row_share(const PrefixAttnParams& p, int ite
   w.np = (w.P + KEYS - 1) / KEYS;
   const int last = min(w.r0 + ROWS, w.rows) - 1;
   w.own = PACKED || !w.work ? 0 : max(0, min(w.len, w.len - w.n + last / p.G + 1));
+  w.all = PACKED || !w.work ? 0 : max(0, min(w.len, w.len - w.n + w.r0 / p.G + 1));
   const int nt = w.np + (w.own + KEYS - 1) / KEYS, per = (nt + splits - 1) / splits;
   w.t_lo = min(nt, split * per);
   w.cnt = w.work ? min(nt, w.t_lo + per) - w.t_lo : 0;
@@ -694,9 +754,10 @@ many_rows_kernel(const PrefixAttnParams p, const __grid_constant__ PoolMaps maps
   using C = ManyRows<HD>;
   constexpr int NBUF = C::NBUF;
   extern __shared__ __align__(1024) unsigned char mr_smem[];
-  __shared__ __align__(8) uint64_t full[NBUF], empty[NBUF], q_full[2], s_full[2], p_full[2][2], o_full[2], v_clean[2], drained[2], turn[2][4];
+  __shared__ __align__(8) uint64_t full[NBUF], empty[NBUF], q_full[2], s_full[2], p_full[2][2], o_full[2], v_clean[NBUF], drained[2], turn[2][4];
   __shared__ uint32_t s_tmem, s_absent[16];
   __shared__ int s_abort, s_req, s_row0, s_sum[TC_THREADS / 32];
+  __shared__ int s_any_bad, s_bad[3][PACKED ? 1 : HD];  // per column the first hidden key with inf, -inf, NaN
   unsigned char* base = mr_smem + ((1024 - (smem_u32(mr_smem) & 1023)) & 1023);
   const uint32_t q_u = smem_u32(base), ring_u = q_u + 2 * C::TILE;
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
@@ -705,7 +766,10 @@ many_rows_kernel(const PrefixAttnParams p, const __grid_constant__ PoolMaps maps
     s_abort = 0;
     s_req = -1;
     s_row0 = 0;
+    s_any_bad = 0;
   }
+  if (!PACKED)
+    for (int i = threadIdx.x; i < 3 * HD; i += TC_THREADS) s_bad[i / HD][PACKED ? 0 : i % HD] = INT32_MAX;
   if (warp == 1) tmem_alloc_cols(&s_tmem, 512);
   tc_fence_before();
   __syncthreads();
@@ -739,8 +803,7 @@ many_rows_kernel(const PrefixAttnParams p, const __grid_constant__ PoolMaps maps
       mbar_init(&turn[0][w], 1);
       mbar_init(&turn[1][w], 1);
     }
-    mbar_init(&v_clean[0], 1);  // the prefix's last tile
-    mbar_init(&v_clean[1], 1);  // the request's
+    for (int i = 0; i < NBUF; ++i) mbar_init(&v_clean[i], 1);
     fence_mbar_init();
   }
   __syncthreads();
@@ -814,8 +877,7 @@ many_rows_kernel(const PrefixAttnParams p, const __grid_constant__ PoolMaps maps
       }
       for (int i = 0; i < cnt && ok; ++i) {
         const uint32_t vi = 2 * i + 1, ki = 2 * i + 2;
-        ok = wait_full(vi);
-        if (ok && keys_of(t_lo + i) < TC_N) ok = pa_spin(&v_clean[t_lo + i >= np], 0, abort);
+        ok = pa_spin(&v_clean[vi % NBUF], (vi / NBUF) & 1u, abort);
         const uint64_t v = dv + at(vi);
 #pragma unroll
         for (int half = 0; half < 2; ++half) {
@@ -837,25 +899,47 @@ many_rows_kernel(const PrefixAttnParams p, const __grid_constant__ PoolMaps maps
       }
     }
   } else if (warp == 3) {
-    // ================================ V's tail ================================
-    // It follows every tile of the ring and frees it as the MMA issuers do: a barrier's parity says which of two
-    // phases is over, not which of many.
+    // ================================ V looked over ================================
+    // Every tile passes here before the MMA issuers take it, and is freed as by them: a barrier's parity says which of
+    // two phases is over, not which of many.
     for (uint32_t it = 0; it < 2u * cnt; ++it) {
-      const int s = it % NBUF, i = it / 2;
+      const int s = it % NBUF, t = t_lo + (int)(it / 2), keys = min(TC_N, keys_of(t));
       if (!__all_sync(0xffffffffu, pa_wait(&full[s], (it / NBUF) & 1u, abort))) break;
-      const int keys = keys_of(t_lo + i);
-      if ((it & 1) && keys < TC_N) {
-        const uint32_t v = ring_u + s * C::TILE;
+      const uint32_t v = ring_u + s * C::TILE;
+      // keys from here on are hidden from some row
+      const int shown = PACKED || t < np ? keys : max(0, min(keys, w.all - (t - np) * TC_N));
+      if ((it & 1) && shown < TC_N) {
+        for (int e = lane; e < (keys - shown) * 8 * C::NCH; e += 32) {
+          const int r = shown + e / (8 * C::NCH), c = e % (8 * C::NCH);
+          const uint32_t at = v + (c >> 3) * (TC_N * 128) + r * 128 + ((c & 7) << 4);
+          const uint4 u = lds_v4(at);
+          if (!not_finite<__half>(u)) continue;
+          // it is zero for the products; at the end the rows that see it become what it makes of them
+          uint32_t y[4] = {u.x, u.y, u.z, u.w};
+          for (int k = 0; k < 8; ++k) {
+            const uint32_t half = (y[k >> 1] >> ((k & 1) * 16)) & 0xffffu;
+            if ((half & 0x7c00u) != 0x7c00u) continue;
+            const int col = (c >> 3) * 64 + ((c & 7) ^ (r & 7)) * 8 + k;
+            atomicMin(&s_bad[half == 0x7c00u ? 0 : half == 0xfc00u ? 1 : 2][col], (t - np) * TC_N + r);
+            y[k >> 1] &= k & 1 ? 0x0000ffffu : 0xffff0000u;
+            s_any_bad = 1;
+          }
+          asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(y[0]), "r"(y[1]), "r"(y[2]), "r"(y[3]) : "memory");
+        }
+        // the slots behind the last key may hold anything
         for (int e = lane; e < (TC_N - keys) * 8 * C::NCH; e += 32) {
           const int r = keys + e / (8 * C::NCH), c = e % (8 * C::NCH);
           asm volatile("st.shared.v4.u32 [%0], {%1, %1, %1, %1};" ::"r"(v + (c >> 3) * (TC_N * 128) + r * 128 + ((c & 7) << 4)), "r"(0)
                        : "memory");
         }
         fence_async_smem();
+        __threadfence_block();
         __syncwarp();
-        if (lane == 0) mbar_arrive(&v_clean[t_lo + i >= np]);
       }
-      if (lane == 0) mbar_arrive(&empty[s]);
+      if (lane == 0) {
+        mbar_arrive(&v_clean[s]);
+        mbar_arrive(&empty[s]);
+      }
     }
   } else if (warp >= 4) {
     // ================================ softmax ================================
@@ -991,12 +1075,28 @@ many_rows_kernel(const PrefixAttnParams p, const __grid_constant__ PoolMaps maps
         const float inv = l == 0.f ? 0.f : 1.f / l;
         if (valid && p.nslots > 1) p.part_ml[at] = make_float2(m, l);
         const uint32_t sm = q_u + x * C::TILE + lanes * (HD * 2);  // in the tile's Q, which is done with
+        auto unhide = [&](float* v, int col, int count) {  // what is not finite, for the rows that see it
+          if constexpr (!PACKED) {
+            if (!s_any_bad) return;
+#pragma unroll
+            for (int k = 0; k < count; ++k) {
+              const bool up = see > s_bad[0][col + k], down = see > s_bad[1][col + k];
+              if (see > s_bad[2][col + k] || (up && down))
+                v[k] = NAN;
+              else if (up || down)
+                v[k] += up ? INFINITY : -INFINITY;
+            }
+          }
+        };
         if (p.nslots > 1) {
 #pragma unroll
           for (int q = 0; q < HD; q += HD / 2) {
             float v[HD / 2];
 #pragma unroll
-            for (int k = 0; k < HD / 2; k += 32) tmem_ld32_wait(ot + q + k, v + k);
+            for (int k = 0; k < HD / 2; k += 32) {
+              tmem_ld32_wait(ot + q + k, v + k);
+              unhide(v + k, q + k, 32);
+            }
             flush_rows<HD * 2>(sm, [&](int c) { return f4_as_u4(v + c * 4); }, reinterpret_cast<char*>(p.part_o + (at - row) * HD + q),
                                HD * sizeof(float), row, valid);
           }
@@ -1006,6 +1106,7 @@ many_rows_kernel(const PrefixAttnParams p, const __grid_constant__ PoolMaps maps
           for (int k = 0; k < HD; k += 32) {
             float v[32];
             tmem_ld32_wait(ot + k, v);
+            unhide(v, k, 32);
 #pragma unroll
             for (int j = 0; j < 16; ++j) o2[k / 2 + j] = h2_as_u32(__floats2half2_rn(v[2 * j] * inv, v[2 * j + 1] * inv));
           }
@@ -1046,8 +1147,8 @@ many_rows_kernel(const PrefixAttnParams p, const __grid_constant__ PoolMaps maps
 // hi = fp16(x) and lo = fp16(2^11 (x - hi)) -- 2^-22 of x is lost, whatever its
 // size down to 2^-24 -- and each product of two operands is three fp16
 // products in two fp32 accumulators, hi.hi and hi.lo + lo.hi, joined as the
-// first plus 2^-11 of the second.  The parts' range is fp16's: a value beyond
-// 65504 gives NaN.  The parts of K and of V lie side by side, so that hi.hi
+// first plus 2^-11 of the second.  The parts' range is fp16's: a value of
+// 65520 or more gives NaN.  The parts of K and of V lie side by side, so that hi.hi
 // and hi.lo are one product of twice the width.  One tile of 128 rows, tiles of
 // 64 keys:
 //   warp 0       TMA producer: raw fp32 K and V tiles through a ring
@@ -1103,6 +1204,7 @@ many_rows_f32_kernel(const PrefixAttnParams p, const __grid_constant__ PoolMaps 
   __shared__ uint32_t s_tmem, s_absent[16];
   __shared__ int s_abort, s_req, s_row0, s_sum[TF_THREADS / 32];
   __shared__ float s_max[2][2][TC_M];  // by tile's parity, by half
+  __shared__ int s_any_bad, s_bad[PACKED ? 1 : HD];  // per column the first hidden key with an infinity or NaN
   const uint32_t q_u = smem_u32(mf_smem), k_u = q_u + 2 * C::QT, v_u = k_u + 2 * C::PT, raw_u = v_u + 2 * C::PT;
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   const int split = blockIdx.x % splits, item = blockIdx.x / splits, h = blockIdx.y;
@@ -1129,8 +1231,10 @@ many_rows_f32_kernel(const PrefixAttnParams p, const __grid_constant__ PoolMaps 
     s_abort = 0;
     s_req = -1;
     s_row0 = 0;
+    s_any_bad = 0;
     fence_mbar_init();
   }
+  if (!PACKED && threadIdx.x < HD) s_bad[PACKED ? 0 : threadIdx.x] = INT32_MAX;
   if (warp == 1) tmem_alloc_cols(&s_tmem, 512);
   tc_fence_before();
   __syncthreads();
@@ -1233,7 +1337,9 @@ many_rows_f32_kernel(const PrefixAttnParams p, const __grid_constant__ PoolMaps 
     constexpr int STEPS = TF_N / (TF_CONV * KPW);
     const int cw = warp - 12, g = lane % LPK, sub = lane / LPK;
     const bool odd = (g >> 2) & 1;
-    auto convert = [&](uint32_t it, bool is_v, int keys) {  // slots from `keys` on become zero
+    // Slots from `keys` on become zero, and what is not finite (or not in the parts' range) from `shown` on: rows that do not
+    // see those keys have weights of zero for them, the others become NaN at the end.  key0: the tile's first own key.
+    auto convert = [&](uint32_t it, bool is_v, int keys, int shown, int key0) {
       const int s = it % NRAW;
       if (!__all_sync(0xffffffffu, pa_wait(&raw_full[s], (it / NRAW) & 1u, abort))) return false;
       const uint32_t src = raw_u + s * C::RAW;
@@ -1252,11 +1358,22 @@ many_rows_f32_kernel(const PrefixAttnParams p, const __grid_constant__ PoolMaps 
       for (int j = 0; j < STEPS; ++j) {
         const int key = (j * TF_CONV + cw) * KPW + sub;
         if (key >= keys) a[j] = b[j] = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (!PACKED && key >= shown) {
+          float* y[8] = {&a[j].x, &a[j].y, &a[j].z, &a[j].w, &b[j].x, &b[j].y, &b[j].z, &b[j].w};
+#pragma unroll
+          for (int k = 0; k < 8; ++k) {
+            if (fabsf(*y[k]) < 65520.f) continue;  // what fp16 rounds to a number
+            *y[k] = 0.f;
+            atomicMin(&s_bad[PACKED ? 0 : g * 8 + ((k < 4) != odd ? k & 3 : 4 + (k & 3))], key0 + key);
+            s_any_bad = 1;
+          }
+        }
         const uint32_t c = sw128(key, g & 7);
         const uint32_t d = is_v ? v_u + (g >> 3) * CH + c : k_u + (g >> 3) * 2 * CH + c;
         split_f16x8(odd ? b[j] : a[j], odd ? a[j] : b[j], d, d + (is_v ? C::PT : CH));
       }
       fence_async_smem();
+      if (!PACKED) __threadfence_block();
       __syncwarp();
       if (lane == 0) mbar_arrive(&raw_empty[s]);
       return true;
@@ -1291,12 +1408,13 @@ many_rows_f32_kernel(const PrefixAttnParams p, const __grid_constant__ PoolMaps 
     for (int i = 0; i <= cnt && ok && cnt; ++i) {
       if (i < cnt) {  // K of tile i, once S of tile i - 1 is done with the buffer
         if (i > 0) ok = __all_sync(0xffffffffu, pa_wait(&s_full[(i - 1) & 1], ((i - 1) >> 1) & 1, abort));
-        ok = ok && convert(k_at(i), false, TF_N);
+        ok = ok && convert(k_at(i), false, TF_N, TF_N, 0);
         if (ok && lane == 0) mbar_arrive(&k_full);
       }
       if (i > 0 && ok) {  // V of tile i - 1, once the product of tile i - 2 is
         if (i > 1) ok = __all_sync(0xffffffffu, pa_wait(&pv_done, (i - 2) & 1, abort));
-        ok = ok && convert(v_at(i - 1), true, keys_of(w.t_lo + i - 1));
+        const int t = w.t_lo + i - 1, key0 = (t - np) * TF_N;
+        ok = ok && convert(v_at(i - 1), true, keys_of(t), PACKED || t < np ? TF_N : w.all - key0, key0);
         if (ok && lane == 0) mbar_arrive(&v_full);
       }
     }
@@ -1409,6 +1527,11 @@ many_rows_f32_kernel(const PrefixAttnParams p, const __grid_constant__ PoolMaps 
           tmem_ld32_wait(ot + HD + q, x);
 #pragma unroll
           for (int k = 0; k < 32; ++k) v[q + k] = fmaf(x[k], 1.f / 2048.f, v[q + k]) * f;
+          if (!PACKED && s_any_bad) {
+#pragma unroll
+            for (int k = 0; k < 32; ++k)
+              if (see > s_bad[PACKED ? 0 : half * (HD / 2) + q + k]) v[q + k] = NAN;
+          }
         }
         // through Q's tiles, which are done with
         flush_rows<HD * 2>(q_u + (warp - 4) * 32 * HD * 2, [&](int c) { return f4_as_u4(v + c * 4); }, reinterpret_cast<char*>(dst),

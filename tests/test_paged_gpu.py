@@ -387,6 +387,46 @@ def test_attn_not_finite_where_it_is_seen(cuda, rng, dtype):
     assert torch.isnan(out[1, : 2 * 64]).all() and torch.equal(out[1, 2 * 64:], clean[1, 2 * 64:])
 
 
+@pytest.mark.parametrize("dtype", ["f16", "f32"])
+@pytest.mark.parametrize("hq,hkv,hd", [(4, 2, 64), (12, 2, 128)])
+@pytest.mark.parametrize("new", [[3, 1, 5], [9, 150, 70]])
+def test_attn_not_finite_where_it_is_hidden(cuda, rng, dtype, hq, hkv, hd, new):
+    """Infinities and NaN in the keys and values of a chunk's later tokens: the rows before them are as without, the rows
+    that see them are what the formula makes of it (fp32: not a number)."""
+    lens = [n + 20 for n in new]
+    d = make_attn(cuda, rng, dtype, hq, hkv, hd, 16, 40, lens, new, scale_q=0.3)
+    v, k = d["v"], d["k"]
+
+    def put(pool, b, back, h, col, what):  # the request's token `back` from its end
+        i = lens[b] - back
+        pool[d["table"][b, i // 16], h, i % 16, col] = what
+
+    for b in range(3):
+        if new[b] > 1:
+            put(v, b, 1, 0, 3, float("nan"))
+            put(v, b, 2, 1, 7, float("inf"))
+            put(v, b, 1, 1, hd - 1, float("-inf"))
+            put(v, b, new[b] - 1, 0, 11, float("-inf"))
+            put(v, b, 1, 0, 11, float("inf"))
+        if new[b] > 4:
+            put(k, b, 1, 1, 5, float("nan"))
+            put(v, b, new[b] // 2, 0, 40, float("nan"))
+    out = run_attn(cuda, d)
+    with np.errstate(invalid="ignore"):
+        want, mass, dot, keys, tail = op.attention(d["q"].double().numpy(), k.double().numpy(), v.double().numpy(), d["start"], d["lens"],
+                                                   d["table"], d["ptab"], d["prefix"], hq, 1 / math.sqrt(hd))
+    got = out[: sum(new)].double().cpu().numpy().reshape(want.shape)
+    fine = np.isfinite(want)
+    assert 0 < (~fine).sum() < fine.size / 2
+    if dtype == "f16":
+        assert np.array_equal(np.isnan(got), np.isnan(want)) and np.array_equal(got[np.isinf(want)], want[np.isinf(want)])
+    else:
+        assert np.array_equal(np.isfinite(got), fine)
+    bound = attn_bound(dtype, want, np.where(fine, mass, 0), np.where(np.isfinite(dot), dot, 0), keys, np.where(fine, tail, 0), hd)
+    assert (np.abs(got[fine] - want[fine]) <= bound[fine]).all()
+    assert L.load().sc_prefix_attn_device_error(1) == 0
+
+
 def test_attn_large_offsets(cuda):
     """Pages beyond 2^31 elements from the pool's start."""
     hkv, hd, page = 8, 128, 128
