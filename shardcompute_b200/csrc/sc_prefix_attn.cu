@@ -95,7 +95,6 @@ struct FewRows {
   static constexpr int SUB = KT * 128;                  // bytes of a chunk of a tile
   static constexpr int TILE = NB * SUB;                 // bytes of a K or V tile
   static constexpr int STAGE = 2 * TILE;
-  static constexpr int COPIES = F16 ? NB : 1;           // of a tile: fp16, one per 128-byte chunk, as many_rows_kernel's
   static constexpr int NST = HD == 128 ? 3 : 6;         // stages per warp: 96 KB a CTA, two CTAs an SM
   static constexpr int SMEM = FR_WARPS * NST * STAGE + 1024;
 };
@@ -196,12 +195,9 @@ few_rows_kernel(const PrefixAttnParams p, const __grid_constant__ PoolMaps maps,
       absent = (absent & ~(1u << s)) | ((r < 0 ? 1u : 0u) << s);
       if (lane == 0) mbar_arrive_expect_tx(&full[warp][s], C::STAGE);
       __syncwarp();
-      if (lane < 2 * C::COPIES) {
-        const bool v = lane >= C::COPIES;
-        const int ch = lane % C::COPIES;
-        tma3d_at(ring_u + s * C::STAGE + (v ? C::TILE : 0) + ch * SUB, v ? &maps.v : &maps.k, r < 0 ? p.pool_rows : r, ch,
+      if (lane < 2)
+        tma3d_at(ring_u + s * C::STAGE + lane * C::TILE, lane ? &maps.v : &maps.k, r < 0 ? p.pool_rows : r, 0,
                  &full[warp][s]);  // past the end: zeros
-      }
       ++issued;
     };
     for (int i = 0; i < min(NST, cnt); ++i) issue(i);
@@ -552,7 +548,6 @@ few_rows_kernel(const PrefixAttnParams p, const __grid_constant__ PoolMaps maps,
 // only when a score passes it by 2^8 (P then stays below 2^8 and l in fp32).
 // TMEM: S0 | S1 (128 columns each, P in the first 64), O0 | O1 (HD each).
 constexpr int TC_M = 128, TC_N = 128;   // rows and keys of a tile
-constexpr int TC_BOX = 16;              // keys of a copy
 constexpr int TC_THREADS = 12 * 32;
 constexpr int TC_REGS_CTL = 88, TC_REGS_SM = 208;  // 128 x 88 + 256 x 208: what the block starts with, 384 x 168
 constexpr int TC_HAND = 3;  // quarter of a tile before which its softmax lets the other one start
@@ -673,13 +668,13 @@ __device__ __forceinline__ uint4 f4_as_u4(const float* v) {
 }
 
 // The rows and keys of a CTA of the many-rows kernels: `item`-th block of ROWS rows (of the whole batch where PACKED,
-// else of one request, items counted over the requests), the split-th share of its tiles of KEYS keys.
+// else of one request, items counted over the requests), every splits-th of its tiles of KEYS keys.
 struct RowShare {
   int b, r0;               // request; first row, counted in the request (in the batch where PACKED)
   int row_lo, rows;        // the request's first token in q, its rows
   int n, len, P, np, own;  // its new tokens, its tokens; prefix keys, prefix tiles; own keys that the last row sees
   int all;                 // own keys that every row sees
-  int t_lo, cnt;           // tiles
+  int t0, step, cnt;       // tiles: t0 + step i
   bool work;
 };
 
@@ -740,9 +735,10 @@ __device__ __forceinline__ RowShare row_share(const PrefixAttnParams& p, int ite
   const int last = min(w.r0 + ROWS, w.rows) - 1;
   w.own = PACKED || !w.work ? 0 : max(0, min(w.len, w.len - w.n + last / p.G + 1));
   w.all = PACKED || !w.work ? 0 : max(0, min(w.len, w.len - w.n + w.r0 / p.G + 1));
-  const int nt = w.np + (w.own + KEYS - 1) / KEYS, per = (nt + splits - 1) / splits;
-  w.t_lo = min(nt, split * per);
-  w.cnt = w.work ? min(nt, w.t_lo + per) - w.t_lo : 0;
+  // every splits-th tile, so that the first one does not depend on the lengths
+  w.t0 = split;
+  w.step = splits;
+  w.cnt = w.work ? max(0, (w.np + (w.own + KEYS - 1) / KEYS - split + splits - 1) / splits) : 0;
   return w;
 }
 
@@ -763,10 +759,25 @@ many_rows_kernel(const PrefixAttnParams p, const __grid_constant__ PoolMaps maps
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   const int split = blockIdx.x % splits, item = blockIdx.x / splits, h = blockIdx.y;
   if (threadIdx.x == 0) {
+    for (int i = 0; i < NBUF; ++i) {
+      mbar_init(&full[i], 1);
+      mbar_init(&empty[i], 3);  // the MMA issuers (warp 3 for the second where it has no rows), and warp 3
+      mbar_init(&v_clean[i], 1);
+    }
+    for (int x = 0; x < 2; ++x) {
+      mbar_init(&q_full[x], TC_M);
+      mbar_init(&s_full[x], 1);
+      mbar_init(&p_full[x][0], 4);
+      mbar_init(&p_full[x][1], 4);
+      mbar_init(&o_full[x], 1);
+      mbar_init(&drained[x], 1);
+      for (int i = 0; i < 4; ++i) mbar_init(&turn[x][i], 1);
+    }
     s_abort = 0;
     s_req = -1;
     s_row0 = 0;
     s_any_bad = 0;
+    fence_mbar_init();
   }
   if (!PACKED)
     for (int i = threadIdx.x; i < 3 * HD; i += TC_THREADS) s_bad[i / HD][PACKED ? 0 : i % HD] = INT32_MAX;
@@ -781,57 +792,39 @@ many_rows_kernel(const PrefixAttnParams p, const __grid_constant__ PoolMaps maps
 
   const RowShare w = row_share<PACKED, 2 * TC_M, TC_N, TC_THREADS>(p, item, split, splits, s_req, s_row0, s_sum);
   const int b = w.b, r0 = w.r0, row_lo = w.row_lo, rows = w.rows, n = w.n, len = w.len, P = w.P, np = w.np, own = w.own;
-  const int t_lo = w.t_lo, cnt = w.cnt;
+  const int cnt = w.cnt;
   const bool work = w.work;
   const int nx = work && r0 + TC_M < rows ? 2 : 1;  // row tiles in use
+  auto tile_of = [&](int i) { return w.t0 + w.step * i; };
   // keys of tile t that exist
   auto keys_of = [&](int t) { return t < np ? P - t * TC_N : own - (t - np) * TC_N; };
-  if (threadIdx.x == 0) {
-    for (int i = 0; i < NBUF; ++i) {
-      mbar_init(&full[i], 1);
-      mbar_init(&empty[i], nx + 1);  // the MMA issuers, and warp 3
-    }
-    for (int x = 0; x < 2; ++x) {
-      mbar_init(&q_full[x], TC_M);
-      mbar_init(&s_full[x], 1);
-      mbar_init(&p_full[x][0], 4);
-      mbar_init(&p_full[x][1], 4);
-      mbar_init(&o_full[x], 1);
-      mbar_init(&drained[x], 1);
-    }
-    for (int w = 0; w < 4; ++w) {
-      mbar_init(&turn[0][w], 1);
-      mbar_init(&turn[1][w], 1);
-    }
-    for (int i = 0; i < NBUF; ++i) mbar_init(&v_clean[i], 1);
-    fence_mbar_init();
-  }
-  __syncthreads();
-
   if (warp < 4)
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(TC_REGS_CTL));
   else
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(TC_REGS_SM));
   if (warp == 0) {
     // ================================ TMA producer ================================
-    constexpr int COPIES = TC_N / TC_BOX * C::NCH;
-    const int sub = lane / C::NCH, ch = lane % C::NCH;
-    auto rows_of = [&](int i) {  // the pool rows of tile i, one per copy; -1: no such page
-      const int t = t_lo + i;
-      if (i >= cnt || lane >= COPIES || sub * TC_BOX >= keys_of(t)) return -1;
-      const int key = (t < np ? t : t - np) * TC_N + sub * TC_BOX, blk = key >> p.lg_page;
-      const int id = t < np ? p.prefix_table[blk] : p.block_table[(size_t)b * p.max_blocks + blk];
-      return id >= 0 && id < p.n_pages ? ((id * p.Hkv + h) << p.lg_page) + (key & ((1 << p.lg_page) - 1)) : -1;
+    // copies: a page's rows (128 at most) of a 64-wide column, one per lane
+    const int lg_box = min(p.lg_page, 7), sub = lane / C::NCH, ch = lane % C::NCH;
+    auto pool_row = [&](int t) {  // this lane's first row of tile t in the pools; -1: no such page
+      const bool pre = PACKED || t < np;
+      const long long key = (long long)(pre ? t : t - np) * TC_N + (sub << lg_box);
+      const int blk = (int)min(key >> p.lg_page, (long long)INT32_MAX);
+      if (blk >= (pre ? p.max_prefix_blocks : p.max_blocks)) return -1;
+      const int id = pre ? p.prefix_table[blk] : p.block_table[(size_t)b * p.max_blocks + blk];
+      return id >= 0 && id < p.n_pages ? ((id * p.Hkv + h) << p.lg_page) + (int)(key & ((1 << p.lg_page) - 1)) : -1;
     };
+    const int copies = (TC_N >> lg_box) * C::NCH;
     uint32_t it = 0;
     bool ok = true;
-    int next = rows_of(0);
+    int next = pool_row(tile_of(0));
     for (int i = 0; i < cnt && ok; ++i) {
-      const int row = next;
-      next = rows_of(i + 1);
-      uint32_t gone = 0;  // keys of this tile that have no page, a bit per copy's
+      const int keys = keys_of(tile_of(i));
+      const int row = sub << lg_box < keys ? next : -1;
+      if (i + 1 < cnt) next = pool_row(tile_of(i + 1));
+      uint32_t gone = 0;  // keys of this tile that have no page, a bit per 16
 #pragma unroll
-      for (int k = 0; k < TC_N / TC_BOX; ++k) gone |= (__shfl_sync(0xffffffffu, row, k * C::NCH) < 0 ? 1u : 0u) << k;
+      for (int k = 0; k < TC_N / 16; ++k) gone |= (__shfl_sync(0xffffffffu, row, ((k * 16) >> lg_box) * C::NCH) < 0 ? 1u : 0u) << k;
       if (lane == 0) s_absent[i & 15] = gone;
 #pragma unroll
       for (int kv = 0; kv < 2; ++kv, ++it) {
@@ -840,8 +833,8 @@ many_rows_kernel(const PrefixAttnParams p, const __grid_constant__ PoolMaps maps
         if (!ok) break;
         if (lane == 0) mbar_arrive_expect_tx(&full[s], C::TILE);
         __syncwarp();
-        if (lane < COPIES)
-          tma3d_at(ring_u + s * C::TILE + ch * (TC_N * 128) + sub * TC_BOX * 128, kv ? &maps.v : &maps.k,
+        if (lane < copies)
+          tma3d_at(ring_u + s * C::TILE + ch * (TC_N * 128) + (sub << lg_box) * 128, kv ? &maps.v : &maps.k,
                    row < 0 ? p.pool_rows : row, ch, &full[s]);
       }
     }
@@ -903,7 +896,7 @@ many_rows_kernel(const PrefixAttnParams p, const __grid_constant__ PoolMaps maps
     // Every tile passes here before the MMA issuers take it, and is freed as by them: a barrier's parity says which of
     // two phases is over, not which of many.
     for (uint32_t it = 0; it < 2u * cnt; ++it) {
-      const int s = it % NBUF, t = t_lo + (int)(it / 2), keys = min(TC_N, keys_of(t));
+      const int s = it % NBUF, t = tile_of((int)(it / 2)), keys = min(TC_N, keys_of(t));
       if (!__all_sync(0xffffffffu, pa_wait(&full[s], (it / NBUF) & 1u, abort))) break;
       const uint32_t v = ring_u + s * C::TILE;
       // keys from here on are hidden from some row
@@ -939,6 +932,7 @@ many_rows_kernel(const PrefixAttnParams p, const __grid_constant__ PoolMaps maps
       if (lane == 0) {
         mbar_arrive(&v_clean[s]);
         mbar_arrive(&empty[s]);
+        if (nx == 1) mbar_arrive(&empty[s]);
       }
     }
   } else if (warp >= 4) {
@@ -980,11 +974,11 @@ many_rows_kernel(const PrefixAttnParams p, const __grid_constant__ PoolMaps maps
         ok = __all_sync(0xffffffffu, pa_wait(&s_full[x], i & 1, abort));
         if (!ok) break;
         tc_fence_after();
-        const int t = t_lo + i;
+        const int t = tile_of(i);
         const uint32_t gone = s_absent[i & 15];
         const int lim = (t < np ? P : see) - (t < np ? t : t - np) * TC_N;  // keys of the tile this row sees
         const bool part = __any_sync(0xffffffffu, lim < TC_N) || gone != 0;
-        auto seen = [&](int k) { return k < lim && !((gone >> (k / TC_BOX)) & 1u); };
+        auto seen = [&](int k) { return k < lim && !((gone >> (k / 16)) & 1u); };
         float v[TC_N];
 #pragma unroll
         for (int q = 0; q < TC_N; q += 32) tmem_ld32_async(st + q, v + q);
@@ -1088,7 +1082,9 @@ many_rows_kernel(const PrefixAttnParams p, const __grid_constant__ PoolMaps maps
             }
           }
         };
-        if (p.nslots > 1) {
+        if (!__any_sync(0xffffffffu, valid)) {
+          // rows behind the last
+        } else if (p.nslots > 1) {
 #pragma unroll
           for (int q = 0; q < HD; q += HD / 2) {
             float v[HD / 2];
@@ -1253,7 +1249,7 @@ many_rows_f32_kernel(const PrefixAttnParams p, const __grid_constant__ PoolMaps 
   if (warp == 0) {
     // ================================ TMA producer ================================
     auto rows_of = [&](int i) {  // the pool rows of tile i, one per copy
-      const int t = w.t_lo + i;
+      const int t = w.t0 + w.step * i;
       int at = -1;
       if (lane < TF_N / TF_BOX && lane * TF_BOX < keys_of(t)) {
         const int key = (t < np ? t : t - np) * TF_N + lane * TF_BOX, blk = key >> p.lg_page;
@@ -1413,7 +1409,7 @@ many_rows_f32_kernel(const PrefixAttnParams p, const __grid_constant__ PoolMaps 
       }
       if (i > 0 && ok) {  // V of tile i - 1, once the product of tile i - 2 is
         if (i > 1) ok = __all_sync(0xffffffffu, pa_wait(&pv_done, (i - 2) & 1, abort));
-        const int t = w.t_lo + i - 1, key0 = (t - np) * TF_N;
+        const int t = w.t0 + w.step * (i - 1), key0 = (t - np) * TF_N;
         ok = ok && convert(v_at(i - 1), true, keys_of(t), PACKED || t < np ? TF_N : w.all - key0, key0);
         if (ok && lane == 0) mbar_arrive(&v_full);
       }
@@ -1437,7 +1433,7 @@ many_rows_f32_kernel(const PrefixAttnParams p, const __grid_constant__ PoolMaps 
         if (!ok) break;
         tc_fence_after();
         const uint32_t st = tl + (i & 1) * 128 + half * 32;
-        const int t = w.t_lo + i;
+        const int t = w.t0 + w.step * i;
         const uint32_t gone = (s_absent[i & 15] >> (half * (32 / TF_BOX))) & ((1u << (32 / TF_BOX)) - 1);
         // of this thread's keys, those that its row sees
         const int lim = (t < np ? w.P : see) - (t < np ? t : t - np) * TF_N - half * 32;
@@ -1724,12 +1720,14 @@ template <typename T, int HD>
 static int run_attn(const PrefixAttnParams& p, const void* k, const void* v, const AttnPlan& a, cudaStream_t stream) {
   using C = FewRows<T, HD>;
   int st = SC_OK;
-  // one pair of maps for all kernels of the type: 16 keys of a 128-byte column, or 8 keys of all columns
+  static_assert(C::F16 || C::KT == TF_BOX, "both fp32 kernels copy boxes of eight keys");
   PoolMaps maps;
-  const int box = C::F16 ? TC_BOX : TF_BOX, chunks = C::F16 ? 1 : C::NB;
-  static_assert(C::KT == (C::F16 ? TC_BOX : TF_BOX), "a tile of the few-rows kernel is one box high");
-  SC_REQUIRE(pool_map(&maps.k, k, p.pool_rows, HD, C::F16, box, chunks) && pool_map(&maps.v, v, p.pool_rows, HD, C::F16, box, chunks),
-             SC_ERR_CUDA, "prefix_attn: tensor map of the pages refused");
+  const auto encode = [&](int box, int chunks) {
+    return pool_map(&maps.k, k, p.pool_rows, HD, C::F16, box, chunks) && pool_map(&maps.v, v, p.pool_rows, HD, C::F16, box, chunks);
+  };
+  const bool tiles = C::F16 && a.kind != AttnPlan::FEW;  // many_rows_kernel: a page's rows of a 64-wide column at a time
+  SC_REQUIRE(tiles ? encode(std::min(TC_N, 1 << p.lg_page), 1) : encode(C::KT, C::NB), SC_ERR_CUDA,
+             "prefix_attn: tensor map of the pages refused");
   if (a.kind != AttnPlan::FEW) {
     const bool packed = a.kind == AttnPlan::SHARED;
     if constexpr (C::F16)
@@ -1741,6 +1739,7 @@ static int run_attn(const PrefixAttnParams& p, const void* k, const void* v, con
     if (st != SC_OK) return st;
   }
   if (a.kind != AttnPlan::CHUNKS) {
+    SC_REQUIRE(!tiles || encode(C::KT, C::NB), SC_ERR_CUDA, "prefix_attn: tensor map of the pages refused");
     const cudaError_t e = opt_in<few_rows_kernel<T, HD>>(C::SMEM);
     if (e != cudaSuccess) return check_launch("prefix_attn", e);
     launch(few_rows_kernel<T, HD>, dim3(a.splits * a.row_groups, p.Hkv, p.B), dim3(FR_WARPS * 32), C::SMEM, stream, p, maps,
