@@ -81,7 +81,9 @@ __device__ __forceinline__ void tma3d_at(uint32_t dst, const CUtensorMap* map, i
 // weight at most, on the order of the output's own rounding.
 // fp32: every operand is split into two tf32 parts (split_tf32); up to 8 rows
 // lie in the 16-row fragment as [hi; lo], so two tf32 products (with K's hi
-// and its lo) give all four terms.  A value that is not finite gives NaN.
+// and its lo) give all four terms.  The tensor cores cut their sums off, always
+// towards zero, so a tile's products are added to o outside of them (in them,
+// 16000 keys left out 2.4e-6 of o).  A value that is not finite gives NaN.
 constexpr int FR_WARPS = 4;
 constexpr float FR_RAISE = 8.f;
 
@@ -436,8 +438,11 @@ few_rows_kernel(const PrefixAttnParams p, const __grid_constant__ PoolMaps maps,
             uint32_t h0, e0, h1, e1;
             split_tf32(xa[e], h0, e0);
             split_tf32(xb[e], h1, e1);
-            mma_1688(o[dd * 4 + e], pa, e0, e1);
-            mma_1688(o[dd * 4 + e], pa, h0, h1);
+            float y[4] = {0.f, 0.f, 0.f, 0.f};
+            mma_1688(y, pa, e0, e1);
+            mma_1688(y, pa, h0, h1);
+#pragma unroll
+            for (int k = 0; k < 4; ++k) o[dd * 4 + e][k] += y[k];
           }
         }
       }
@@ -1142,11 +1147,19 @@ many_rows_kernel(const PrefixAttnParams p, const __grid_constant__ PoolMaps maps
 // The many-rows kernel for fp32.  Every operand x is carried as two fp16 parts,
 // hi = fp16(x) and lo = fp16(2^11 (x - hi)) -- 2^-22 of x is lost, whatever its
 // size down to 2^-24 -- and each product of two operands is three fp16
-// products in two fp32 accumulators, hi.hi and hi.lo + lo.hi, joined as the
-// first plus 2^-11 of the second.  The parts' range is fp16's: a value of
-// 65520 or more gives NaN.  The parts of K and of V lie side by side, so that hi.hi
-// and hi.lo are one product of twice the width.  One tile of 128 rows, tiles of
-// 64 keys:
+// products.
+//   S = Q K^T: in two fp32 accumulators, hi.hi and hi.lo + lo.hi, joined as the
+//     first plus 2^-11 of the second; K's parts lie side by side, so that hi.hi
+//     and hi.lo are one product of twice the width.
+//   O = P V: in one, for P has a largest value of 1 or more in every row and
+//     what is lost below 2^-24 of that does not count: lo(P) as it is times
+//     hi(V), and 2^-11 hi(P) times lo(V), then hi.hi.
+// The tensor cores cut their fp32 sums off, always towards zero.  Over a long
+// row that adds up (3.5e-8 of O per 16 keys, 3.6e-5 after 16500), so every
+// second tile the products so far are added to a sum of their own, in fp32 and
+// rounded to nearest, and begin anew: 4e-7 of O at any length.
+// The parts' range is fp16's: a value of 65520 or more gives NaN.  One tile of
+// 128 rows, tiles of 64 keys:
 //   warp 0       TMA producer: raw fp32 K and V tiles through a ring
 //   warp 1       MMA issuer; S of the next tile goes ahead of O += P V of this one
 //   warps 4-11   softmax, two threads per row with half the tile's keys each,
@@ -1154,11 +1167,12 @@ many_rows_kernel(const PrefixAttnParams p, const __grid_constant__ PoolMaps maps
 //                over S's columns)
 //   warps 12-19  split Q, then each raw tile, into the fp16 parts; V's slots
 //                behind the last key, which may hold anything, become zero
-// TMEM: two buffers of S (hi.hi | cross, 64 columns each), O (hi.hi | cross).
+// TMEM: two buffers of S (hi.hi | cross, 64 columns each), the products, their sum.
 constexpr int TF_N = 64;              // keys of a tile
 constexpr int TF_BOX = 8;             // keys of a copy
 constexpr int TF_THREADS = 20 * 32;
 constexpr int TF_CONV = 8;            // warps that split
+constexpr int TF_FOLD = 2;            // tiles after which the products go to the sum
 
 template <int HD>
 struct ManyRowsF32 {
@@ -1178,6 +1192,14 @@ __device__ __forceinline__ void split_f16(float x, float y, uint32_t& hi, uint32
   const float2 f = __half22float2(h);
   hi = h2_as_u32(h);
   lo = h2_as_u32(__floats2half2_rn((x - f.x) * 2048.f, (y - f.y) * 2048.f));
+}
+// two weights -> hi, lo as it is, 2^-11 hi
+__device__ __forceinline__ void split_weight(float x, float y, uint32_t& hi, uint32_t& lo, uint32_t& low_hi) {
+  const __half2 h = __floats2half2_rn(x, y);
+  const float2 f = __half22float2(h);
+  hi = h2_as_u32(h);
+  lo = h2_as_u32(__floats2half2_rn(x - f.x, y - f.y));
+  low_hi = h2_as_u32(__hmul2(h, __float2half2_rn(1.f / 2048.f)));
 }
 // eight fp32 -> 16 bytes of each part, at shared addresses h and l
 __device__ __forceinline__ void split_f16x8(const float4& a, const float4& b, uint32_t h, uint32_t l) {
@@ -1238,7 +1260,7 @@ many_rows_f32_kernel(const PrefixAttnParams p, const __grid_constant__ PoolMaps 
   pdl_wait();
   pdl_trigger();  // after the wait: few_rows_kernel relies on it
   volatile int* abort = &s_abort;
-  const uint32_t tmem = s_tmem;  // S: buffer j at 128 j, its cross part 64 further; O at 256, its cross part HD further
+  const uint32_t tmem = s_tmem;  // S: buffer j at 128 j, its cross part 64 further; the products at 256, their sum at 384
   const RowShare w = row_share<PACKED, TC_M, TF_N, TF_THREADS>(p, item, split, splits, s_req, s_row0, s_sum);
   const int np = w.np, cnt = w.cnt;
   auto keys_of = [&](int t) { return t < np ? w.P - t * TF_N : w.own - (t - np) * TF_N; };
@@ -1288,7 +1310,7 @@ many_rows_f32_kernel(const PrefixAttnParams p, const __grid_constant__ PoolMaps 
     if (lane == 0 && cnt > 0) {
       constexpr uint32_t mn = (1u << 4) | ((TC_M >> 4) << 24);
       constexpr uint32_t idesc_s2 = mn | ((2 * TF_N >> 3) << 17), idesc_s = mn | ((TF_N >> 3) << 17);
-      constexpr uint32_t idesc_o2 = mn | (1u << 16) | ((2 * HD >> 3) << 17), idesc_o = mn | (1u << 16) | ((HD >> 3) << 17);
+      constexpr uint32_t idesc_o = mn | (1u << 16) | ((HD >> 3) << 17);
       const uint64_t qh = umma_desc_sw128(q_u), ql = umma_desc_sw128(q_u + C::QT), kd = umma_desc_sw128(k_u);
       const uint64_t vd = umma_desc_sw128_mn(v_u, CH);
       const uint32_t to = tmem + 256;
@@ -1317,12 +1339,14 @@ many_rows_f32_kernel(const PrefixAttnParams p, const __grid_constant__ PoolMaps 
         ok = pa_spin(&v_full, i & 1, abort) && pa_spin(&p_full[i & 1], (i >> 1) & 1, abort);
         if (!ok) break;
         tc_fence_after();
-        const uint32_t ph = tmem + (i & 1) * 128, pl = ph + 64;
+        const uint32_t ph = tmem + (i & 1) * 128;  // hi, lo, 2^-11 hi
 #pragma unroll
         for (int kk = 0; kk < TF_N / 16; ++kk) {
-          umma_f16_ta(to, ph + kk * 8, vd + kk * (2048 >> 4), idesc_o2, (i | kk) != 0);
-          umma_f16_ta(to + HD, pl + kk * 8, vd + kk * (2048 >> 4), idesc_o, 1u);
+          umma_f16_ta(to, ph + 32 + kk * 8, vd + kk * (2048 >> 4), idesc_o, (i % TF_FOLD | kk) != 0);
+          umma_f16_ta(to, ph + 64 + kk * 8, vd + ((C::PT + kk * 2048) >> 4), idesc_o, 1u);
         }
+#pragma unroll
+        for (int kk = 0; kk < TF_N / 16; ++kk) umma_f16_ta(to, ph + kk * 8, vd + kk * (2048 >> 4), idesc_o, 1u);
         tc_commit(&pv_done);
         if (i + 1 == cnt) tc_commit(&o_full);
       }
@@ -1416,10 +1440,10 @@ many_rows_f32_kernel(const PrefixAttnParams p, const __grid_constant__ PoolMaps 
     }
   } else if (warp >= 4) {
     // ================================ softmax ================================
-    const int half = (warp - 4) >> 2;  // keys 32 half .. 32 half + 31 of every tile; columns HD / 2 of both parts of O
+    const int half = (warp - 4) >> 2;  // keys 32 half .. 32 half + 31 of every tile; half of O's columns
     const int lanes = (warp & 3) * 32;
     const int r = w.r0 + lanes + lane;  // this thread's row
-    const uint32_t tl = tmem + ((uint32_t)lanes << 16), ot = tl + 256 + half * (HD / 2);
+    const uint32_t tl = tmem + ((uint32_t)lanes << 16), ot = tl + 256 + half * (HD / 2), sum = ot + 128;
     const bool valid = w.work && r < w.rows;
     const int see = PACKED ? 0 : (valid ? max(0, min(w.len, w.len - w.n + r / p.G + 1)) : w.own);
     const float c = p.c;
@@ -1464,39 +1488,60 @@ many_rows_f32_kernel(const PrefixAttnParams p, const __grid_constant__ PoolMaps 
         if (!ok) break;
         tc_fence_after();
         mx = fmaxf(mx, s_max[i & 1][half ^ 1][lanes + lane]);
-        if (__any_sync(0xffffffffu, mx > m + TC_RAISE)) {  // also from -inf; the other half comes to the same
+        const bool up = __any_sync(0xffffffffu, mx > m + TC_RAISE);  // also from -inf; the other half comes to the same
+        const bool fold = i > 0 && i % TF_FOLD == 0;
+        float f = 1.f;
+        if (up) {
           const float mn = fmaxf(m, mx);
-          const float f = m == -INFINITY ? 0.f : ex2(m - mn);
+          f = m == -INFINITY ? 0.f : ex2(m - mn);
           m = mn;
           l *= f;
-          if (i > 0) {  // the last product into O; the one before it precedes this tile's S
-            ok = __all_sync(0xffffffffu, pa_wait(&pv_done, (i - 1) & 1, abort));
-            if (!ok) break;
-            tc_fence_after();
+        }
+        if (fold || (up && i > 0)) {  // the last product; the one before it precedes this tile's S
+          ok = __all_sync(0xffffffffu, pa_wait(&pv_done, (i - 1) & 1, abort));
+          if (!ok) break;
+          tc_fence_after();
 #pragma unroll
-            for (int q = 0; q < HD; q += 32) {  // HD / 2 columns of each part
-              const uint32_t ad = ot + (q < HD / 2 ? q : HD / 2 + q);
-              float u[32];
-              tmem_ld32_wait(ad, u);
+          for (int q = 0; q < HD / 2; q += 32) {
+            float u[32];
+            tmem_ld32_wait(ot + q, u);
+            if (fold) {
+              if (i > TF_FOLD) {
+                float y[32];
+                tmem_ld32_wait(sum + q, y);
+#pragma unroll
+                for (int k = 0; k < 32; ++k) u[k] += y[k];
+              }
 #pragma unroll
               for (int k = 0; k < 32; ++k) u[k] *= f;
-              tmem_st32(ad, u);
+              tmem_st32(sum + q, u);
+            } else {
+#pragma unroll
+              for (int k = 0; k < 32; ++k) u[k] *= f;
+              tmem_st32(ot + q, u);
+              if (i > TF_FOLD) {
+                tmem_ld32_wait(sum + q, u);
+#pragma unroll
+                for (int k = 0; k < 32; ++k) u[k] *= f;
+                tmem_st32(sum + q, u);
+              }
             }
           }
         }
         const float mm = m == -INFINITY ? 0.f : m;
         float l0 = 0.f, l1 = 0.f;
-        uint32_t hi[16], lo[16];
+        uint32_t hi[16], lo[16], low_hi[16];
 #pragma unroll
         for (int k = 0; k < 32; k += 2) {
           const float e0 = ex2(fmaf(v[k], c, -mm)), e1 = ex2(fmaf(v[k + 1], c, -mm));
           l0 += e0;
           l1 += e1;
-          split_f16(e0, e1, hi[k / 2], lo[k / 2]);
+          split_weight(e0, e1, hi[k / 2], lo[k / 2], low_hi[k / 2]);
         }
         const uint32_t pt = tl + (i & 1) * 128 + half * 16;
         tmem_st16(pt, hi);
-        tmem_st16(pt + 64, lo);
+        tmem_st16(pt + 32, lo);
+        tmem_st16(pt + 64, low_hi);
         l += l0 + l1;
         tmem_wait_st();
         tc_fence_before();
@@ -1518,11 +1563,15 @@ many_rows_f32_kernel(const PrefixAttnParams p, const __grid_constant__ PoolMaps 
         float v[HD / 2];
 #pragma unroll
         for (int q = 0; q < HD / 2; q += 32) {
-          float x[32];
           tmem_ld32_wait(ot + q, v + q);
-          tmem_ld32_wait(ot + HD + q, x);
+          if (cnt > TF_FOLD) {
+            float x[32];
+            tmem_ld32_wait(sum + q, x);
 #pragma unroll
-          for (int k = 0; k < 32; ++k) v[q + k] = fmaf(x[k], 1.f / 2048.f, v[q + k]) * f;
+            for (int k = 0; k < 32; ++k) v[q + k] += x[k];
+          }
+#pragma unroll
+          for (int k = 0; k < 32; ++k) v[q + k] *= f;
           if (!PACKED && s_any_bad) {
 #pragma unroll
             for (int k = 0; k < 32; ++k)

@@ -319,6 +319,38 @@ def test_attn_many_rows_many_tiles(cuda, rng, dtype, hq, hkv, hd, prefix, longes
         assert torch.equal(out, run_attn(cuda, d))
 
 
+@pytest.mark.parametrize("hkv,hd,new,prefix,own,cut", [(4, 64, [1] * 48, 0, 16000, 2), (8, 128, [600], 16000, 600, 24), (8, 64, [600], 0, 16000, 24),
+                                                       (4, 64, [1] * 128, 16000, 10, 24)])
+def test_attn_long_rows_do_not_shrink(cuda, hkv, hd, new, prefix, own, cut):
+    """fp32: the tensor cores cut their sums off towards zero, which must not add up over the keys.  With values above zero
+    all of that is on one side, and the mean of out / exact - 1 shows it: at most 2^-23 for each of the `cut` sums that
+    follow one another in the tensor cores.  The rest is rounded to nearest: 2^-24 for each of up to 1000 additions to a
+    row's sum and to its weights', as a walk 2^-24 sqrt(1000) for a row, a fourteenth of that for the mean of 192 rows (the
+    fewest here, 48 requests of 4 heads); four times it."""
+    g = torch.Generator(device=cuda).manual_seed(7)
+    B, page, G = len(new), 32, 4 if len(new) == 1 else 1 if prefix == 0 else 8
+    per, pre = -(-own // page), -(-prefix // page)
+    n_pages = B * per + pre
+    k = torch.randn(n_pages, hkv, page, hd, device=cuda, generator=g)
+    v = torch.rand(n_pages, hkv, page, hd, device=cuda, generator=g) + 0.5
+    q = torch.randn(sum(new), hkv * G * hd, device=cuda, generator=g) * 0.25
+    table = torch.arange(B * per, dtype=torch.int32, device=cuda).view(B, per)
+    ptab = torch.arange(B * per, n_pages, dtype=torch.int32, device=cuda)
+    start = np.concatenate([[0], np.cumsum(new)])
+    kw = dict(prefix_table=ptab, prefix_len=i32([prefix], cuda)) if prefix else {}
+    out = ops.prefix_attn(q, k, v, i32(start, cuda), i32([own] * B, cuda), table, **kw).view(-1, hkv, G, hd)
+    total = 0.0
+    for b in range(B):
+        lo, hi = int(start[b]), int(start[b + 1])
+        pos = torch.arange(own - (hi - lo), own, device=cuda)
+        for h in range(hkv):
+            flat = lambda x: torch.cat([x[ptab.long(), h].reshape(-1, hd)[:prefix], x[table[b].long(), h].reshape(-1, hd)[:own]]).double()
+            s = q[lo:hi].view(-1, hkv, G, hd)[:, h].double() @ flat(k).T / math.sqrt(hd)
+            s[..., prefix:].masked_fill_(torch.arange(own, device=cuda) > pos[:, None, None], float("-inf"))
+            total += float((out[lo:hi, h].double() / (torch.softmax(s, -1) @ flat(v)) - 1).sum())
+    assert abs(total / out.numel()) <= cut * 2.0**-23 + 4 * 2.0**-24 * math.sqrt(1000 / 192)
+
+
 @pytest.mark.parametrize("dtype", ["f16", "f32"])
 @pytest.mark.parametrize("new", [[1, 1, 1], [9, 40, 150]])
 def test_attn_no_prefix_and_scale(cuda, rng, dtype, new):
