@@ -50,22 +50,35 @@ int run_qgemm(const void* x, int x_dtype, int M, int K, int ldx, const uint16_t*
 // Records a failed launch for the next check_launch() on this thread.
 void note_launch_status(cudaError_t e);
 
+// In clusters of `cluster` CTAs along x (1: none).
 template <typename... KArgs, typename... Args>
-inline cudaError_t launch(void (*kern)(KArgs...), dim3 grid, dim3 block, size_t smem, cudaStream_t stream,
-                          Args&&... args) {
+inline cudaError_t launch_clusters(int cluster, void (*kern)(KArgs...), dim3 grid, dim3 block, size_t smem, cudaStream_t stream,
+                                   Args&&... args) {
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = grid;
   cfg.blockDim = block;
   cfg.dynamicSmemBytes = smem;
   cfg.stream = stream;
-  cudaLaunchAttribute attr[1];
+  cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
+  if (cluster > 1) {
+    cudaLaunchAttribute& cl = attr[pdl_enabled() ? 1 : 0];
+    cl.id = cudaLaunchAttributeClusterDimension;
+    cl.val.clusterDim.x = cluster;
+    cl.val.clusterDim.y = cl.val.clusterDim.z = 1;
+  }
   cfg.attrs = attr;
-  cfg.numAttrs = pdl_enabled() ? 1 : 0;
+  cfg.numAttrs = (pdl_enabled() ? 1 : 0) + (cluster > 1 ? 1 : 0);
   const cudaError_t e = cudaLaunchKernelEx(&cfg, kern, std::forward<Args>(args)...);
   note_launch_status(e);
   return e;
+}
+
+template <typename... KArgs, typename... Args>
+inline cudaError_t launch(void (*kern)(KArgs...), dim3 grid, dim3 block, size_t smem, cudaStream_t stream,
+                          Args&&... args) {
+  return launch_clusters(1, kern, grid, block, smem, stream, std::forward<Args>(args)...);
 }
 
 #define SC_REQUIRE(cond, code, ...)          \

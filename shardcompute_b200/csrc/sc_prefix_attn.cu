@@ -74,7 +74,10 @@ __device__ __forceinline__ void tma3d_at(uint32_t dst, const CUtensorMap* map, i
 // of the keys and every row_groups-th tile of rows; its warps take tiles of 16 (fp32: 8) keys in turn, each with its own
 // ring of tiles in shared memory (a TMA copy per 16 or 8 keys, which never
 // straddle a page) and its own running (m, l, o), so no barrier
-// stands in the loop.  The warps' results are joined at the end.
+// stands in the loop.  The warps' results are joined at the end, and with
+// CLUSTER those of the CTAs that share a request's keys, each CTA a part of the
+// outputs from all the CTAs' shared memory: no partial results in memory, no
+// kernel after this one (four requests behind 500 tokens 12.3 -> 7.4 us).
 //
 // fp16: mma m16n8k16 over up to 16 rows (the request's tokens x the group's
 // heads).  P is rounded to fp16 for the second product: 2^-11 relative per
@@ -86,6 +89,23 @@ __device__ __forceinline__ void tma3d_at(uint32_t dst, const CUtensorMap* map, i
 // 16000 keys left out 2.4e-6 of o).  A value that is not finite gives NaN.
 constexpr int FR_WARPS = 4;
 constexpr float FR_RAISE = 8.f;
+constexpr int FR_CLUSTER = 8;  // shares of the keys that a cluster joins, at most
+
+__device__ __forceinline__ void cluster_sync() {
+  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+// A value at shared address `a` of the cluster's CTA `rank`.
+template <typename V>
+__device__ __forceinline__ V ld_peer(uint32_t a, int rank) {
+  V v;
+  uint32_t at;
+  asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(a), "r"(rank));
+  if constexpr (sizeof(V) == 16)
+    asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(at) : "memory");
+  else
+    asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(at) : "memory");
+  return v;
+}
 
 template <typename T, int HD>
 struct FewRows {
@@ -132,7 +152,53 @@ __device__ __forceinline__ bool not_finite(const uint4& v) {
   return ((((v.x & mask) + one) | ((v.y & mask) + one) | ((v.z & mask) + one) | ((v.w & mask) + one)) & top) != 0;
 }
 
+// Four outputs: the sums over their weights'.
+template <typename T>
+__device__ __forceinline__ void store_out(T* dst, const float4& acc, float L) {
+  const float inv = L == 0.f ? 0.f : 1.f / L;
+  if constexpr (sizeof(T) == 2)
+    *reinterpret_cast<uint2*>(dst) = make_uint2(h2_as_u32(__floats2half2_rn(acc.x * inv, acc.y * inv)),
+                                                h2_as_u32(__floats2half2_rn(acc.z * inv, acc.w * inv)));
+  else
+    *reinterpret_cast<float4*>(dst) = make_float4(acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv);
+}
+
+// CTA `rank` of a cluster of `size`: its part of the outputs of a tile of nr rows from the CTAs' results, (m, l) at
+// shared address ml_u and o at o_u of each.
 template <typename T, int HD>
+__device__ __forceinline__ void join_cluster(const PrefixAttnParams& p, uint32_t ml_u, uint32_t o_u, int rank, int size, int nr, int row_lo,
+                                             int r0, int h) {
+  for (int e = rank * FR_WARPS * 32 + threadIdx.x; e < nr * (HD / 4); e += size * FR_WARPS * 32) {
+    const int r = e / (HD / 4), d = (e % (HD / 4)) * 4;
+    float2 ml[FR_CLUSTER];
+    float4 v[FR_CLUSTER];
+    float M = -INFINITY, L = 0.f;
+#pragma unroll
+    for (int w = 0; w < FR_CLUSTER; ++w) {
+      ml[w] = make_float2(-INFINITY, 0.f);
+      if (w < size) {
+        ml[w] = ld_peer<float2>(ml_u + r * 8, w);
+        v[w] = ld_peer<float4>(o_u + (r * HD + d) * 4, w);
+      }
+      M = fmaxf(M, ml[w].x);
+    }
+    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+    for (int w = 0; w < FR_CLUSTER; ++w) {
+      if (ml[w].x == -INFINITY && ml[w].y == 0.f) continue;
+      const float f = ex2(ml[w].x - M);
+      acc.x += f * v[w].x;
+      acc.y += f * v[w].y;
+      acc.z += f * v[w].z;
+      acc.w += f * v[w].w;
+      L += f * ml[w].y;
+    }
+    const size_t row = (size_t)(row_lo + (r0 + r) / p.G) * p.Hq + h * p.G + (r0 + r) % p.G;
+    store_out(reinterpret_cast<T*>(p.out) + row * HD + d, acc, L);
+  }
+}
+
+template <typename T, int HD, bool CLUSTER>
 __global__ void __launch_bounds__(FR_WARPS * 32)
 few_rows_kernel(const PrefixAttnParams p, const __grid_constant__ PoolMaps maps, int with_prefix, int splits, int row_groups,
                 int slot0) {
@@ -141,6 +207,7 @@ few_rows_kernel(const PrefixAttnParams p, const __grid_constant__ PoolMaps maps,
   extern __shared__ __align__(1024) unsigned char fr_smem[];
   __shared__ __align__(8) uint64_t full[FR_WARPS][NST];
   __shared__ float s_m[FR_WARPS][RT], s_l[FR_WARPS][RT];
+  __shared__ float2 s_ml[CLUSTER ? RT : 1];
   __shared__ int s_abort;
   unsigned char* base = fr_smem + ((1024 - (smem_u32(fr_smem) & 1023)) & 1023);
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
@@ -451,7 +518,14 @@ few_rows_kernel(const PrefixAttnParams p, const __grid_constant__ PoolMaps maps,
     }
     // ---- join the warps
     const bool failed = __syncthreads_or(issued != used);  // a wait ran out (also: every ring is free)
-    if (failed) break;
+    if (failed) {
+      if (CLUSTER)  // the others' barriers: two for this tile of rows and for each that follows
+        for (int r = r0; r < n * p.G; r += row_groups * RT) {
+          cluster_sync();
+          cluster_sync();
+        }
+      break;
+    }
 #pragma unroll
     for (int d = 1; d <= 2; d <<= 1) {
       l0 += __shfl_xor_sync(0xffffffffu, l0, d);
@@ -504,19 +578,23 @@ few_rows_kernel(const PrefixAttnParams p, const __grid_constant__ PoolMaps maps,
       }
       const int tok = row_lo + (r0 + r) / p.G, g = (r0 + r) % p.G;
       const size_t row = (size_t)tok * p.Hq + h * p.G + g;
-      if (p.nslots == 1) {
-        const float inv = L == 0.f ? 0.f : 1.f / L;
-        T* dst = reinterpret_cast<T*>(p.out) + row * HD + d;
-        if constexpr (C::F16)
-          *reinterpret_cast<uint2*>(dst) = make_uint2(h2_as_u32(__floats2half2_rn(acc.x * inv, acc.y * inv)),
-                                                      h2_as_u32(__floats2half2_rn(acc.z * inv, acc.w * inv)));
-        else
-          *reinterpret_cast<float4*>(dst) = make_float4(acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv);
+      if (CLUSTER) {
+        *reinterpret_cast<float4*>(base + ((size_t)(RT + r) * HD + d) * 4) = acc;  // behind warp 0's result
+        if (d == 0) s_ml[CLUSTER ? r : 0] = make_float2(M, L);
+      } else if (p.nslots == 1) {
+        store_out<T>(reinterpret_cast<T*>(p.out) + row * HD + d, acc, L);
       } else {
         const size_t at = (size_t)(slot0 + split) * p.T * p.Hq + row;
         *reinterpret_cast<float4*>(p.part_o + at * HD + d) = acc;
         if (d == 0) p.part_ml[at] = make_float2(M, L);
       }
+    }
+    if (CLUSTER) {  // join the CTAs, each a part of the outputs
+      __syncthreads();
+      cluster_sync();
+      join_cluster<T, HD>(p, smem_u32(s_ml), smem_u32(base) + RT * HD * 4, split, splits, nr, row_lo, r0, h);
+      __syncthreads();
+      cluster_sync();  // before a result is written over, or its CTA exits
     }
     // the rings hold the joined results: written by threads, next by copies
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
@@ -1707,12 +1785,13 @@ static cudaError_t opt_in(int smem) {
 
 // How a call is cut.  The host knows the rows T and the requests B, not which request has how many, nor how many
 // keys there are, only how many the tables hold.
-//   few rows      few_rows_kernel over the prefix and the requests' own keys
+//   few rows      few_rows_kernel over the prefix and the requests' own keys, its shares joined in a cluster if they are short
 //   shared        a many-rows kernel, PACKED, over the prefix, few_rows_kernel over the own keys
 //   chunks        a many-rows kernel over both
 struct AttnPlan {
   enum Kind { FEW, SHARED, CHUNKS } kind;
   int splits, row_groups;       // few_rows_kernel
+  bool cluster;                 // its shares are joined in a cluster
   int tc_splits, tc_items;      // many_rows_kernel, many_rows_f32_kernel
   int nslots;
 };
@@ -1722,11 +1801,17 @@ static AttnPlan plan_attn(int T, int B, int Hkv, int G, int hd, bool f16, long l
   const int per_cta = f16 ? 2 * TC_M : TC_M, tile = f16 ? TC_N : TF_N;
   const long long rows = (long long)T * G, items = (rows + per_cta - 1) / per_cta;
   const auto ceil_div = [](long long x, long long y) { return (x + y - 1) / y; };
-  // The few-rows kernel streams the prefix once per request.  While that is little it beats a kernel more (us in a graph,
-  // 8 kv heads of 128, fp16, few | shared: 2 requests behind 500 tokens 8.7 | 12.0, 1000 12.4 | 13.1, 2000 17.3 | 15.4;
-  // 8 behind 128 12.5 | 13.1, 500 16.2 | 13.3; fp32: 2 behind 1000 14.6 | 17.6, 2000 19.3 | 18.8).
-  a.kind = rows >= 64ll * B ? AttnPlan::CHUNKS : prefix_keys > 0 && B * prefix_keys > 2048 ? AttnPlan::SHARED : AttnPlan::FEW;
-  if (B == 1 && a.kind == AttnPlan::SHARED) a.kind = AttnPlan::FEW;  // nothing to share
+  const int rt = f16 ? 16 : 8;
+  const long long groups = ceil_div(rows, (long long)B * rt), slots = 2ll * sms;  // few_rows_kernel: two CTAs an SM
+  a.kind = rows >= 64ll * B ? AttnPlan::CHUNKS : AttnPlan::FEW;
+  if (a.kind == AttnPlan::FEW && prefix_keys > 0 && B > 1) {
+    // The few-rows kernel streams the prefix once per request.  While that is little it beats two kernels and the join:
+    // up to so many keys a CTA slot, in clusters of eight at most (us in a graph, few | shared, fp16: 8 kv heads of 128,
+    // 1050 keys a slot 17.6 | 21.2 and 17.6 | 20.2, 1300 19.1 | 19.7, 2100 28.1 | 23.8; 4 of 64, 1050 13.8 | 16.1, 2050
+    // 21.2 | 18.8; fp32: 160 13.0 | 17.5, 290 16.0 | 19.1, 325 18.9 | 18.6, 540 26.8 | 23.6).
+    const long long load = (own_keys + prefix_keys) * std::max(slots / FR_CLUSTER, (long long)B * Hkv * groups) / slots;
+    if (load > (f16 ? 1100 : 320)) a.kind = AttnPlan::SHARED;
+  }
   if (a.kind != AttnPlan::FEW) {
     // Shares of the keys until there is a CTA for every SM; with the own keys' kernel beside it, for this kernel's part
     // of the SMs only.  That part goes by the two kernels' work, as far as the host knows it: a tile takes an SM 2.1 us
@@ -1745,14 +1830,22 @@ static AttnPlan plan_attn(int T, int B, int Hkv, int G, int hd, bool f16, long l
     a.nslots = a.tc_splits;
   }
   if (a.kind != AttnPlan::CHUNKS) {
-    // four CTAs per SM over all requests and heads: first from tiles of rows, then from the keys (64 of them at least)
-    const int rt = f16 ? 16 : 8;
     const long long keys = own_keys + (a.kind == AttnPlan::FEW ? prefix_keys : 0);
-    const long long want = ceil_div(4ll * sms, (long long)B * Hkv), groups = ceil_div(rows, (long long)B * rt);
     // (row tiles are counted for the mean request: twice as many CTAs, so that one of twice the rows does not take twice as long)
+    const long long want = ceil_div(4ll * sms, (long long)B * Hkv);
     a.row_groups = (int)std::max(1ll, std::min(want, groups > 1 ? 2 * groups : 1));
-    a.splits = (int)std::max(1ll, std::min({ceil_div(want, a.row_groups), ceil_div(keys, 64), 64ll}));
-    a.nslots += a.splits;
+    // Shares of 64 keys or more.  Of as many as all run at once, while there are few keys for each place of a CTA; what the
+    // few-rows kernel alone computes is then joined within a cluster.  Past that four CTAs per SM, which even out requests of
+    // different lengths, or for one request use the whole machine, and their results are joined by a kernel more.
+    // Measured with lengths spread evenly up to the longest (us in a graph, all at once | four, no prefix; fp16: 64 requests,
+    // 8 kv heads of 128, 870 keys a place 19.1 | 23.5, 2600 40.9 | 40.4, 6900 99.7 | 94.1; 16, 4 of 64, 1000 12.6 | 17.8, 3000
+    // 28.2 | 26.9; fp32: 4, 8 of 128, 500 25.8 | 29.8, 1500 54.8 | 46.1; 64, 860 37.2 | 38.0, 2600 87.0 | 74.3).
+    const long long most = ceil_div(keys, 64);
+    const long long once = std::max(1ll, std::min({slots / ((long long)B * Hkv * a.row_groups), most, a.kind == AttnPlan::FEW ? (long long)FR_CLUSTER : 64ll}));
+    const bool few_keys = keys * std::max(ceil_div(slots, once), (long long)B * Hkv * a.row_groups) <= slots * (f16 ? 1536 : 512);
+    a.splits = (int)(few_keys ? once : std::max(1ll, std::min({ceil_div(want, a.row_groups), most, 64ll})));
+    a.cluster = few_keys && a.kind == AttnPlan::FEW && a.splits > 1;
+    a.nslots += a.cluster ? 1 : a.splits;
   }
   return a;
 }
@@ -1763,6 +1856,17 @@ static int run_many_rows(int smem, int threads, const PrefixAttnParams& p, const
   if (e != cudaSuccess) return check_launch("prefix_attn", e);
   launch(KERN, dim3((unsigned)(a.tc_splits * a.tc_items), p.Hkv), dim3(threads), smem, stream, p, maps, a.tc_splits, 0);
   return check_launch("prefix_attn_many_rows");
+}
+
+template <typename T, int HD, bool CLUSTER>
+static int run_few_rows(const PrefixAttnParams& p, const PoolMaps& maps, const AttnPlan& a, cudaStream_t stream) {
+  constexpr auto kern = few_rows_kernel<T, HD, CLUSTER>;
+  constexpr int smem = FewRows<T, HD>::SMEM;
+  const cudaError_t e = opt_in<kern>(smem);
+  if (e != cudaSuccess) return check_launch("prefix_attn", e);
+  launch_clusters(CLUSTER ? a.splits : 1, kern, dim3(a.splits * a.row_groups, p.Hkv, p.B), dim3(FR_WARPS * 32), smem, stream, p, maps,
+                  a.kind == AttnPlan::FEW ? 1 : 0, a.splits, a.row_groups, a.kind == AttnPlan::SHARED ? a.tc_splits : 0);
+  return check_launch("prefix_attn_few_rows");
 }
 
 template <typename T, int HD>
@@ -1789,11 +1893,7 @@ static int run_attn(const PrefixAttnParams& p, const void* k, const void* v, con
   }
   if (a.kind != AttnPlan::CHUNKS) {
     SC_REQUIRE(!tiles || encode(C::KT, C::NB), SC_ERR_CUDA, "prefix_attn: tensor map of the pages refused");
-    const cudaError_t e = opt_in<few_rows_kernel<T, HD>>(C::SMEM);
-    if (e != cudaSuccess) return check_launch("prefix_attn", e);
-    launch(few_rows_kernel<T, HD>, dim3(a.splits * a.row_groups, p.Hkv, p.B), dim3(FR_WARPS * 32), C::SMEM, stream, p, maps,
-           a.kind == AttnPlan::FEW ? 1 : 0, a.splits, a.row_groups, a.kind == AttnPlan::SHARED ? a.tc_splits : 0);
-    st = check_launch("prefix_attn_few_rows");
+    st = a.cluster ? run_few_rows<T, HD, true>(p, maps, a, stream) : run_few_rows<T, HD, false>(p, maps, a, stream);
     if (st != SC_OK) return st;
   }
   if (p.nslots == 1) return SC_OK;

@@ -83,8 +83,8 @@ def attn(**kw):
                                      (dict(scale=0.0), L.SC_ERR_ARG), (dict(scale=-1.0), L.SC_ERR_ARG), (dict(scale=float("nan")), L.SC_ERR_ARG),
                                      (dict(scale=float("inf")), L.SC_ERR_ARG), (dict(ptab=None), L.SC_ERR_ARG), (dict(pblocks=0), L.SC_ERR_ARG),
                                      (dict(q=None), L.SC_ERR_ARG), (dict(out=None), L.SC_ERR_ARG), (dict(q=A + 2), L.SC_ERR_ARG),
-                                     (dict(v=A + 8), L.SC_ERR_ARG), (dict(ws=A + 4), L.SC_ERR_ARG), (dict(wb=16), L.SC_ERR_WORKSPACE),
-                                     (dict(ws=None), L.SC_ERR_WORKSPACE)])
+                                     (dict(v=A + 8), L.SC_ERR_ARG), (dict(ws=A + 4), L.SC_ERR_ARG), (dict(blocks=4096, wb=16), L.SC_ERR_WORKSPACE),
+                                     (dict(blocks=4096, ws=None), L.SC_ERR_WORKSPACE)])
 def test_attn_refuses(kw, code):
     assert attn(**kw) == code
     assert L.last_error()

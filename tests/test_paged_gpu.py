@@ -319,6 +319,37 @@ def test_attn_many_rows_many_tiles(cuda, rng, dtype, hq, hkv, hd, prefix, longes
         assert torch.equal(out, run_attn(cuda, d))
 
 
+@pytest.mark.parametrize("dtype", ["f16", "f32"])
+@pytest.mark.parametrize("hq,hkv,hd,page", [(32, 4, 64, 32), (24, 8, 128, 16)])
+@pytest.mark.parametrize("prefix,longest", [(2900, 40), (1111, 700)])
+def test_attn_shared_by_many_requests(cuda, rng, dtype, hq, hkv, hd, page, prefix, longest):
+    """Batches large enough for the prefix to be taken once for all, with absent pages in it and in a request."""
+    new = [int(x) for x in rng.integers(0, 6, 64)]
+    lens = [n + int(rng.integers(0, longest)) for n in new]
+    d = make_attn(cuda, rng, dtype, hq, hkv, hd, page, prefix, lens, new)
+    check_attn(cuda, dtype, d, hq)
+    d["ptab"][[0, len(d["ptab"]) - 1]] = [-1, len(d["k"]) + 5]
+    d["table"][7, 0] = -3
+    out = check_attn(cuda, dtype, d, hq)
+    for _ in range(8):
+        assert torch.equal(out, run_attn(cuda, d))
+
+
+@pytest.mark.parametrize("dtype", ["f16", "f32"])
+@pytest.mark.parametrize("B,hq,hkv,hd", [(1, 8, 8, 128), (2, 6, 2, 64), (5, 8, 8, 128), (9, 16, 4, 64), (17, 8, 8, 128), (23, 5, 5, 64)])
+@pytest.mark.parametrize("drafts", [False, True])
+def test_attn_shares_joined(cuda, rng, dtype, B, hq, hkv, hd, drafts):
+    """Few requests, whose keys several CTAs share: from two shares to eight, some without a key."""
+    new = [int(x) for x in rng.integers(0, 8, B)] if drafts else [1] * B
+    lens = [n + int(rng.integers(0, 2)) * int(rng.integers(0, 900)) for n in new]
+    lens[0] = new[0] + 900
+    for prefix in (0, 130):
+        d = make_attn(cuda, rng, dtype, hq, hkv, hd, 16, prefix, lens, new)
+        out = check_attn(cuda, dtype, d, hq)
+        for _ in range(4):
+            assert torch.equal(out, run_attn(cuda, d))
+
+
 @pytest.mark.parametrize("hkv,hd,new,prefix,own,cut", [(4, 64, [1] * 48, 0, 16000, 2), (8, 128, [600], 16000, 600, 24), (8, 64, [600], 0, 16000, 24),
                                                        (4, 64, [1] * 128, 16000, 10, 24)])
 def test_attn_long_rows_do_not_shrink(cuda, hkv, hd, new, prefix, own, cut):
