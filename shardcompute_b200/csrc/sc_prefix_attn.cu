@@ -78,6 +78,9 @@ __device__ __forceinline__ void tma3d_at(uint32_t dst, const CUtensorMap* map, i
 // CLUSTER those of the CTAs that share a request's keys, each CTA a part of the
 // outputs from all the CTAs' shared memory: no partial results in memory, no
 // kernel after this one (four requests behind 500 tokens 12.3 -> 7.4 us).
+// Few keys: bound by latency, three dependent loads before the first tile and
+// the joins.  Many: by the stream of keys, 64 requests of up to 1500 tokens, 8 kv
+// heads of 128, 40 us in fp16 and 74 us in fp32 (4.9 and 5.3 TB/s).
 //
 // fp16: mma m16n8k16 over up to 16 rows (the request's tokens x the group's
 // heads).  P is rounded to fp16 for the second product: 2^-11 relative per
@@ -630,6 +633,8 @@ few_rows_kernel(const PrefixAttnParams p, const __grid_constant__ PoolMaps maps,
 // tensor cores.  The maximum a row is scaled by is raised, and O rescaled,
 // only when a score passes it by 2^8 (P then stays below 2^8 and l in fp32).
 // TMEM: S0 | S1 (128 columns each, P in the first 64), O0 | O1 (HD each).
+// Bound by the softmax's chain: 12 chunks of 120 to 700 tokens behind a prefix of
+// 2050, 32 heads of 128, 292 us, 731 TFLOP/s, 44 % of the tensor cores' cycles.
 constexpr int TC_M = 128, TC_N = 128;   // rows and keys of a tile
 constexpr int TC_THREADS = 12 * 32;
 constexpr int TC_REGS_CTL = 88, TC_REGS_SM = 208;  // 128 x 88 + 256 x 208: what the block starts with, 384 x 168
@@ -1246,6 +1251,8 @@ many_rows_kernel(const PrefixAttnParams p, const __grid_constant__ PoolMaps maps
 //   warps 12-19  split Q, then each raw tile, into the fp16 parts; V's slots
 //                behind the last key, which may hold anything, become zero
 // TMEM: two buffers of S (hi.hi | cross, 64 columns each), the products, their sum.
+// Bound by the chain from a raw tile to its product, which the 227 KB leave no
+// room to double: the chunks above 1117 us, 191 TFLOP/s (574 of fp16 products).
 constexpr int TF_N = 64;              // keys of a tile
 constexpr int TF_BOX = 8;             // keys of a copy
 constexpr int TF_THREADS = 20 * 32;
@@ -1809,7 +1816,7 @@ static AttnPlan plan_attn(int T, int B, int Hkv, int G, int hd, bool f16, long l
     // up to so many keys a CTA slot, in clusters of eight at most (us in a graph, few | shared, fp16: 8 kv heads of 128,
     // 1050 keys a slot 17.6 | 21.2 and 17.6 | 20.2, 1300 19.1 | 19.7, 2100 28.1 | 23.8; 4 of 64, 1050 13.8 | 16.1, 2050
     // 21.2 | 18.8; fp32: 160 13.0 | 17.5, 290 16.0 | 19.1, 325 18.9 | 18.6, 540 26.8 | 23.6).
-    const long long load = (own_keys + prefix_keys) * std::max(slots / FR_CLUSTER, (long long)B * Hkv * groups) / slots;
+    const double load = (double)(own_keys + prefix_keys) * std::max(slots / FR_CLUSTER, (long long)B * Hkv * groups) / slots;
     if (load > (f16 ? 1100 : 320)) a.kind = AttnPlan::SHARED;
   }
   if (a.kind != AttnPlan::FEW) {
@@ -1827,6 +1834,9 @@ static AttnPlan plan_attn(int T, int B, int Hkv, int G, int hd, bool f16, long l
     }
     a.tc_items = (int)(a.kind == AttnPlan::CHUNKS ? items + B : items);
     a.tc_splits = (int)std::max(1ll, std::min({(sms * part / 1000 + items * Hkv / 2) / (items * Hkv), sms / (items * Hkv), tiles, 32ll}));
+    // The tensor cores' cut-off sums lose 1.1e-9 of O per key; with fp16 that is left, up to 131072 keys a share (1.4e-4, the
+    // output's own error is 1.8e-4).  A table with room for more is cut.
+    if (f16) a.tc_splits = std::max(a.tc_splits, (int)std::min(32ll, ceil_div(tiles, 131072 / TC_N)));
     a.nslots = a.tc_splits;
   }
   if (a.kind != AttnPlan::CHUNKS) {
@@ -1842,7 +1852,7 @@ static AttnPlan plan_attn(int T, int B, int Hkv, int G, int hd, bool f16, long l
     // 28.2 | 26.9; fp32: 4, 8 of 128, 500 25.8 | 29.8, 1500 54.8 | 46.1; 64, 860 37.2 | 38.0, 2600 87.0 | 74.3).
     const long long most = ceil_div(keys, 64);
     const long long once = std::max(1ll, std::min({slots / ((long long)B * Hkv * a.row_groups), most, a.kind == AttnPlan::FEW ? (long long)FR_CLUSTER : 64ll}));
-    const bool few_keys = keys * std::max(ceil_div(slots, once), (long long)B * Hkv * a.row_groups) <= slots * (f16 ? 1536 : 512);
+    const bool few_keys = (double)keys * std::max(ceil_div(slots, once), (long long)B * Hkv * a.row_groups) <= slots * (f16 ? 1536 : 512);
     a.splits = (int)(few_keys ? once : std::max(1ll, std::min({ceil_div(want, a.row_groups), most, 64ll})));
     a.cluster = few_keys && a.kind == AttnPlan::FEW && a.splits > 1;
     a.nslots += a.cluster ? 1 : a.splits;

@@ -99,6 +99,15 @@ def test_workspace_is_bounded():
     assert L.load().sc_prefix_attn_workspace_bytes(4, 4, 7, 2, 128, 8, 8, 16, 0) == 0
 
 
+def test_workspace_of_long_chunks():
+    """Chunks that fill the machine need none, until a share of the keys would pass 131072: then one result more per row."""
+    bytes_of = lambda blocks, dt: ops.prefix_attn_workspace_bytes(16384, 1, 32, 8, 128, blocks, 16, 16, dt)  # noqa: E731
+    for dt in (torch.float16, torch.float32):
+        assert bytes_of(1000, dt) == 0
+    assert bytes_of(8192 - 16, torch.float16) == 0
+    assert bytes_of(8192, torch.float16) == 2 * 16384 * 32 * 130 * 4
+
+
 def test_cpu_tensors_are_refused():
     z = torch.zeros(4, dtype=torch.int32)
     t = torch.zeros(4, 2, dtype=torch.int32)
