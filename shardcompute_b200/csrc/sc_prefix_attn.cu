@@ -1794,7 +1794,7 @@ static cudaError_t opt_in(int smem) {
 // keys there are, only how many the tables hold.
 //   few rows      few_rows_kernel over the prefix and the requests' own keys, its shares joined in a cluster if they are short
 //   shared        a many-rows kernel, PACKED, over the prefix, few_rows_kernel over the own keys
-//   chunks        a many-rows kernel over both
+//   chunks        a many-rows kernel over both, a request's rows at a time
 struct AttnPlan {
   enum Kind { FEW, SHARED, CHUNKS } kind;
   int splits, row_groups;       // few_rows_kernel
@@ -1810,15 +1810,23 @@ static AttnPlan plan_attn(int T, int B, int Hkv, int G, int hd, bool f16, long l
   const auto ceil_div = [](long long x, long long y) { return (x + y - 1) / y; };
   const int rt = f16 ? 16 : 8;
   const long long groups = ceil_div(rows, (long long)B * rt), slots = 2ll * sms;  // few_rows_kernel: two CTAs an SM
-  a.kind = rows >= 64ll * B ? AttnPlan::CHUNKS : AttnPlan::FEW;
-  if (a.kind == AttnPlan::FEW && prefix_keys > 0 && B > 1) {
-    // The few-rows kernel streams the prefix once per request.  While that is little it beats two kernels and the join:
-    // up to so many keys a CTA slot, in clusters of eight at most (us in a graph, few | shared, fp16: 8 kv heads of 128,
-    // 1050 keys a slot 17.6 | 21.2 and 17.6 | 20.2, 1300 19.1 | 19.7, 2100 28.1 | 23.8; 4 of 64, 1050 13.8 | 16.1, 2050
-    // 21.2 | 18.8; fp32: 160 13.0 | 17.5, 290 16.0 | 19.1, 325 18.9 | 18.6, 540 26.8 | 23.6).
-    const double load = (double)(own_keys + prefix_keys) * std::max(slots / FR_CLUSTER, (long long)B * Hkv * groups) / slots;
-    if (load > (f16 ? 1100 : 320)) a.kind = AttnPlan::SHARED;
-  }
+  // The few-rows kernel streams a request's keys, the prefix's too, once per tile of 16 (8) rows.  While that is little it
+  // beats the others: up to so many keys a CTA slot, in clusters of eight at most.  us in a graph, fp16, few | shared: 8 kv
+  // heads of 128, 1050 keys a slot 17.6 | 21.2 and 17.6 | 20.2, 1300 19.1 | 19.7, 2100 28.1 | 23.8; 4 of 64, 1050 13.8 |
+  // 16.1, 2050 21.2 | 18.8; few | chunks: 210 13.3 | 16.5, 410 13.4 | 21.3 and 18.6 | 24.8, 520 19.0 | 17.9 and 14.0 | 13.6,
+  // 1250 31.2 | 20.9.  fp32, few | shared: 160 13.0 | 17.5, 290 16.0 | 19.1, 325 18.9 | 18.6, 540 26.8 | 23.6; few | chunks:
+  // 64 7.8 | 12.0, 106 12.2 | 13.1, 118 12.2 | 10.8, 250 24.3 | 14.5.
+  const double load = (double)(own_keys + prefix_keys) * std::max(slots / FR_CLUSTER, (long long)B * Hkv * groups) / slots;
+  const bool many = rows >= 64ll * B, shares = prefix_keys > 0 && B > 1;
+  if (load <= (many ? (f16 ? 450 : 110) : (f16 ? 1100 : 320)) || !(many || shares))
+    a.kind = AttnPlan::FEW;
+  // A chunk fills its last tile of rows for itself alone, where SHARED packs all requests' rows: worth a second kernel while
+  // a request has less than a tile and the prefix is most of what it sees (behind 2000 tokens, shared | chunks: 8 requests of
+  // 80 rows 29.3 | 43.9, of 160 21.1 | 27.6, of 240 55.8 | 40.1; behind 300 with 200 own, fp32, of 150 51.7 | 32.4).
+  else if (!many || (shares && rows < 192ll * B && prefix_keys >= 4 * own_keys))
+    a.kind = AttnPlan::SHARED;
+  else
+    a.kind = AttnPlan::CHUNKS;
   if (a.kind != AttnPlan::FEW) {
     // Shares of the keys until there is a CTA for every SM; with the own keys' kernel beside it, for this kernel's part
     // of the SMs only.  That part goes by the two kernels' work, as far as the host knows it: a tile takes an SM 2.1 us

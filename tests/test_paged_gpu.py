@@ -490,6 +490,32 @@ def test_attn_not_finite_where_it_is_hidden(cuda, rng, dtype, hq, hkv, hd, new):
     assert L.load().sc_prefix_attn_device_error(1) == 0
 
 
+WIDE = ([(test_attn_ragged_chunks, (hq, hkv, hd, prefix)) for hq, hkv, hd in LAYOUTS for prefix in (0, 1, 333)]
+        + [(test_attn_lengths, a) for a in [(1, 2000, 700), (3, 5000, 40), (2, 0, 3001), (40, 129, 300)]]
+        + [(test_attn_no_prefix_and_scale, ([1, 1, 1],)), (test_attn_no_prefix_and_scale, ([9, 40, 150],)), (test_attn_rows_that_see_nothing, (0,)),
+           (test_attn_rows_that_see_nothing, (50,)), (test_attn_absent_pages, ([1, 1, 1],)), (test_attn_absent_pages, ([5, 70, 33],)),
+           (test_attn_all_pages_absent, ()), (test_attn_shared_page_and_same_request_twice, ()), (test_attn_not_finite_where_it_is_seen, ())]
+        + [(test_attn_not_finite_where_it_is_hidden, (4, 2, 64, new)) for new in ([3, 1, 5], [9, 150, 70])]
+        + [(test_attn_not_finite_where_it_is_hidden, (12, 2, 128, new)) for new in ([3, 1, 5], [9, 150, 70])])
+
+
+@pytest.mark.parametrize("dtype", ["f16", "f32"])
+@pytest.mark.parametrize("which", ["table", "ptab"])
+@pytest.mark.parametrize("case", range(len(WIDE)))
+def test_attn_tables_with_room(cuda, rng, monkeypatch, dtype, which, case):
+    """The same with tables that have room for 65536 more tokens: the call is cut for those, into other kernels and more
+    shares, most of them without a key."""
+    def roomy(*args, make=make_attn, **kw):
+        d = make(*args, **kw)
+        wide = 65536 // d["k"].shape[2]
+        d[which] = np.concatenate([d[which], np.full(d[which].shape[:-1] + (wide,), -1, np.int32)], -1)
+        return d
+
+    monkeypatch.setitem(globals(), "make_attn", roomy)
+    test, args = WIDE[case]
+    test(cuda, rng, dtype, *args)
+
+
 def test_attn_large_offsets(cuda):
     """Pages beyond 2^31 elements from the pool's start."""
     hkv, hd, page = 8, 128, 128
