@@ -1842,6 +1842,12 @@ static AttnPlan plan_attn(int T, int B, int Hkv, int G, int hd, bool f16, long l
     }
     a.tc_items = (int)(a.kind == AttnPlan::CHUNKS ? items + B : items);
     a.tc_splits = (int)std::max(1ll, std::min({(sms * part / 1000 + items * Hkv / 2) / (items * Hkv), sms / (items * Hkv), tiles, 32ll}));
+    // No more shares than their longest one needs: eight tiles in five shares take two each, as in four.  A second share
+    // brings the join: not for less than three tiles (us, chunks, one share | as many as there are SMs for; fp16: 3 requests
+    // of 150 tokens, 2 tiles 14.3 | 21.6; 8 of 60 behind 300, 4 tiles in two shares 18.5 | 25.9; one of 150 behind 300, 4 in
+    // four 20.4 | 17.9; fp32: 8 of 20, 2 tiles 10.2 | 15.2).
+    a.tc_splits = (int)ceil_div(tiles, ceil_div(tiles, a.tc_splits));
+    if (a.kind == AttnPlan::CHUNKS && tiles - ceil_div(tiles, a.tc_splits) < 3) a.tc_splits = 1;
     // The tensor cores' cut-off sums lose 1.1e-9 of O per key; with fp16 that is left, up to 131072 keys a share (1.4e-4, the
     // output's own error is 1.8e-4).  A table with room for more is cut.
     if (f16) a.tc_splits = std::max(a.tc_splits, (int)std::min(32ll, ceil_div(tiles, 131072 / TC_N)));
