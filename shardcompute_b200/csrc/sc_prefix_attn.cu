@@ -1696,7 +1696,8 @@ many_rows_f32_kernel(const PrefixAttnParams p, const __grid_constant__ PoolMaps 
 // ---------------------------------------------------------------- join
 
 // One warp per (row, head).  Lane s holds slot s's weight 2^(m_s - M), so the slots' sums are read without waiting for
-// one another.  Reads each partial result once; bound by L2.
+// one another.  Reads each partial result once, from L2; bound by latency (64 rows, 32 heads of 128, 6 slots: 6.3 MB in
+// 5.2 us).
 template <typename T, int HD>
 __global__ void __launch_bounds__(256) join_slots_kernel(const PrefixAttnParams p) {
   pdl_trigger();
