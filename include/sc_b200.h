@@ -338,8 +338,9 @@ int sc_paged_rope_append(const void* qkv, int qkv_dtype, int rows, const int32_t
  *   were; a row that sees no token is zero.  Pages whose id is outside
  *   0..n_pages-1 count as absent: their tokens are not seen.  What a row does
  *   not see has no influence on it, whatever it is (infinities and NaN too).
- * Softmax statistics and sums are fp32; with fp16 the weights are rounded to
- * fp16 before their product with v.  With fp32, q, k and v are taken to 2^-21
+ * Softmax statistics and sums are fp32; with fp16 the weights are rounded
+ * before their product with v: 2^-11 of each, down to 2^-25 of the row's
+ * largest weight, and in steps of 2^-35 of that below.  With fp32, q, k and v are taken to 2^-21
  * of each value; values that are not finite, or of 65520 or more in size (the
  * range of the parts that the tensor cores take), make what sees them NaN. */
 size_t sc_prefix_attn_workspace_bytes(int T, int B, int Hq, int Hkv, int hd, int max_blocks, int max_prefix_blocks,

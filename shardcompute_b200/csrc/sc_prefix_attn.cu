@@ -18,6 +18,13 @@ namespace sc {
 
 constexpr uint64_t PA_WAIT_NS = 2000000000ull;
 
+// Weights on their way through fp16: a row's reference m lies PA_LIFT below a score that was its largest, in powers of
+// two, and is raised when one comes to lie PA_LIFT + PA_RAISE above it.  Its weights 2^(c s - m) then reach 2^11 to
+// 2^15, half of fp16's range, and keep their 11 bits down to 2^-14.  With a largest weight of 1 to 2^8 in place of that
+// thousands of keys 2^-25 below it vanished from the output, though not from the sum that divides it: 16384 keys behind
+// one that takes most of the weight and has a value of zero came out 8.6e-2 off, now 1.8e-4 (the output's own rounding).
+constexpr float PA_LIFT = 11.f, PA_RAISE = 4.f;
+
 // Raised by a kernel whose bounded wait ran out; read by
 // sc_prefix_attn_device_error.
 __device__ int g_prefix_attn_error = 0;
@@ -83,15 +90,16 @@ __device__ __forceinline__ void tma3d_at(uint32_t dst, const CUtensorMap* map, i
 // heads of 128, 40 us in fp16 and 74 us in fp32 (4.9 and 5.3 TB/s).
 //
 // fp16: mma m16n8k16 over up to 16 rows (the request's tokens x the group's
-// heads).  P is rounded to fp16 for the second product: 2^-11 relative per
-// weight at most, on the order of the output's own rounding.
+// heads).  P is rounded to fp16 for the second product, 2^11 to 2^15 high
+// (PA_LIFT): 2^-11 of each weight, on the order of the output's own rounding,
+// down to weights of 2^-25 of the row's largest, and steps of 2^-35 of that
+// below, where fp16 has no more bits.
 // fp32: every operand is split into two tf32 parts (split_tf32); up to 8 rows
 // lie in the 16-row fragment as [hi; lo], so two tf32 products (with K's hi
 // and its lo) give all four terms.  The tensor cores cut their sums off, always
 // towards zero, so a tile's products are added to o outside of them (in them,
 // 16000 keys left out 2.4e-6 of o).  A value that is not finite gives NaN.
 constexpr int FR_WARPS = 4;
-constexpr float FR_RAISE = 8.f;
 constexpr int FR_CLUSTER = 8;  // shares of the keys that a cluster joins, at most
 
 __device__ __forceinline__ void cluster_sync() {
@@ -122,6 +130,7 @@ struct FewRows {
   static constexpr int STAGE = 2 * TILE;
   static constexpr int NST = HD == 128 ? 3 : 6;         // stages per warp: 96 KB a CTA, two CTAs an SM
   static constexpr int SMEM = FR_WARPS * NST * STAGE + 1024;
+  static constexpr float LIFT = F16 ? PA_LIFT : 0.f, RAISE = F16 ? PA_RAISE : 8.f;  // tf32 has fp32's range
 };
 
 __device__ __forceinline__ void ldsm4(uint32_t a, uint32_t (&r)[4]) {
@@ -374,16 +383,16 @@ few_rows_kernel(const PrefixAttnParams p, const __grid_constant__ PoolMaps maps,
             if (C::F16 && key >= lim1) sc[j][2 + e] = -INFINITY;
           }
       }
-      // ---- running softmax.  A row's m, the same in its four lanes, is raised (and o rescaled) only when a score
-      // passes it by 2^8: weights stay below 2^8, and the lanes seldom have to agree on a maximum.
+      // ---- running softmax.  A row's m, the same in its four lanes, is raised (and o rescaled) only when a weight
+      // passes 2^(LIFT + RAISE): the lanes seldom have to agree on a maximum.
       float x0 = fmaxf(sc[0][0], sc[0][1]), x1 = fmaxf(sc[0][2], sc[0][3]);
       if (NJ == 2) {
         x0 = fmaxf(x0, fmaxf(sc[NJ - 1][0], sc[NJ - 1][1]));
         x1 = fmaxf(x1, fmaxf(sc[NJ - 1][2], sc[NJ - 1][3]));
       }
-      x0 *= p.c;
-      x1 = C::F16 ? x1 * p.c : -INFINITY;
-      if (__any_sync(0xffffffffu, x0 > m0 + FR_RAISE || x1 > m1 + FR_RAISE)) {
+      x0 = fmaf(x0, p.c, -C::LIFT);
+      x1 = C::F16 ? fmaf(x1, p.c, -C::LIFT) : -INFINITY;
+      if (__any_sync(0xffffffffu, x0 > m0 + C::RAISE || x1 > m1 + C::RAISE)) {
 #pragma unroll
         for (int d = 1; d <= 2; d <<= 1) {
           x0 = fmaxf(x0, __shfl_xor_sync(0xffffffffu, x0, d));
@@ -630,8 +639,8 @@ few_rows_kernel(const PrefixAttnParams p, const __grid_constant__ PoolMaps maps,
 //              - m) in fp16 over S's own columns, its sum in fp32, and in the
 //              end O / l or a partial result
 // The tiles take turns: while one is in the softmax, the other is in the
-// tensor cores.  The maximum a row is scaled by is raised, and O rescaled,
-// only when a score passes it by 2^8 (P then stays below 2^8 and l in fp32).
+// tensor cores.  The reference a row is scaled by is raised, and O rescaled,
+// only when a weight passes 2^15 (PA_LIFT); l is summed in fp32.
 // TMEM: S0 | S1 (128 columns each, P in the first 64), O0 | O1 (HD each).
 // Bound by the softmax's chain: 12 chunks of 120 to 700 tokens behind a prefix of
 // 2050, 32 heads of 128, 292 us, 731 TFLOP/s, 44 % of the tensor cores' cycles.
@@ -639,7 +648,6 @@ constexpr int TC_M = 128, TC_N = 128;   // rows and keys of a tile
 constexpr int TC_THREADS = 12 * 32;
 constexpr int TC_REGS_CTL = 88, TC_REGS_SM = 208;  // 128 x 88 + 256 x 208: what the block starts with, 384 x 168
 constexpr int TC_HAND = 3;  // quarter of a tile before which its softmax lets the other one start
-constexpr float TC_RAISE = 8.f;
 
 template <int HD>
 struct ManyRows {
@@ -1086,7 +1094,7 @@ many_rows_kernel(const PrefixAttnParams p, const __grid_constant__ PoolMaps maps
             a2 = max3(a2, v[k + 4], v[k + 5]);
             a3 = max3(a3, v[k + 6], v[k + 7]);
           }
-          return fmaxf(fmaxf(a0, a1), fmaxf(a2, a3)) * c;
+          return fmaf(fmaxf(fmaxf(a0, a1), fmaxf(a2, a3)), c, -PA_LIFT);
         };
         auto raise = [&](float mx) {
           const float mn = fmaxf(m, mx);
@@ -1122,7 +1130,7 @@ many_rows_kernel(const PrefixAttnParams p, const __grid_constant__ PoolMaps maps
           }
         };
         const float mx = row_max();
-        if (__any_sync(0xffffffffu, mx > m + TC_RAISE)) raise(mx);  // also from -inf
+        if (__any_sync(0xffffffffu, mx > m + PA_RAISE)) raise(mx);  // also from -inf
         // The two warps of a scheduler take turns here, or both tiles fall into step: both in the softmax, then both
         // in the tensor cores.
         if (nx == 2 && (x == 1 || i > 0)) {
@@ -1258,6 +1266,7 @@ constexpr int TF_BOX = 8;             // keys of a copy
 constexpr int TF_THREADS = 20 * 32;
 constexpr int TF_CONV = 8;            // warps that split
 constexpr int TF_FOLD = 2;            // tiles after which the products go to the sum
+constexpr float TF_RAISE = 8.f;       // a row's reference is raised when a weight passes 2^8
 
 template <int HD>
 struct ManyRowsF32 {
@@ -1573,7 +1582,7 @@ many_rows_f32_kernel(const PrefixAttnParams p, const __grid_constant__ PoolMaps 
         if (!ok) break;
         tc_fence_after();
         mx = fmaxf(mx, s_max[i & 1][half ^ 1][lanes + lane]);
-        const bool up = __any_sync(0xffffffffu, mx > m + TC_RAISE);  // also from -inf; the other half comes to the same
+        const bool up = __any_sync(0xffffffffu, mx > m + TF_RAISE);  // also from -inf; the other half comes to the same
         const bool fold = i > 0 && i % TF_FOLD == 0;
         float f = 1.f;
         if (up) {
