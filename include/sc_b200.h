@@ -340,9 +340,10 @@ int sc_paged_rope_append(const void* qkv, int qkv_dtype, int rows, const int32_t
  *   not see has no influence on it, whatever it is (infinities and NaN too).
  * Softmax statistics and sums are fp32; with fp16 the weights are rounded
  * before their product with v: 2^-11 of each, down to 2^-25 of the row's
- * largest weight, and in steps of 2^-35 of that below.  With fp32, q, k and v are taken to 2^-21
- * of each value; values that are not finite, or of 65520 or more in size (the
- * range of the parts that the tensor cores take), make what sees them NaN. */
+ * largest weight, and in steps of 2^-35 of that below.
+ * With fp32, q, k, v and the weights are taken to 2^-21 of each value, whatever
+ * its size; values that are not finite, or of 3.39e38 or more in size, make
+ * what sees them NaN. */
 size_t sc_prefix_attn_workspace_bytes(int T, int B, int Hq, int Hkv, int hd, int max_blocks, int max_prefix_blocks,
                                       int page_size, int dtype);
 int sc_prefix_attn(const void* q, const void* k_pages, const void* v_pages, int dtype, int T, const int32_t* q_start,

@@ -74,7 +74,6 @@ __device__ __forceinline__ void tma3d_at(uint32_t dst, const CUtensorMap* map, i
       "l"(reinterpret_cast<uint64_t>(map)), "r"(0), "r"(row), "r"(chunk), "r"(smem_u32(bar))
       : "memory");
 }
-
 // ---------------------------------------------------------------- few rows
 
 // Kernel for few rows per request.  A CTA takes a request, a kv head, a share
@@ -675,6 +674,11 @@ __device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&r)[16
       "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
       : "memory");
 }
+__device__ __forceinline__ void tmem_st8(uint32_t taddr, const uint32_t (&r)[8]) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]),
+               "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
+               : "memory");
+}
 __device__ __forceinline__ void tmem_st32(uint32_t taddr, const float (&v)[32]) {
   uint32_t a[16], b[16];
 #pragma unroll
@@ -1235,37 +1239,41 @@ many_rows_kernel(const PrefixAttnParams p, const __grid_constant__ PoolMaps maps
 
 // ---------------------------------------------------------------- many rows, fp32
 
-// The many-rows kernel for fp32.  Every operand x is carried as two fp16 parts,
-// hi = fp16(x) and lo = fp16(2^11 (x - hi)) -- 2^-22 of x is lost, whatever its
-// size down to 2^-24 -- and each product of two operands is three fp16
-// products.
-//   S = Q K^T: in two fp32 accumulators, hi.hi and hi.lo + lo.hi, joined as the
-//     first plus 2^-11 of the second; K's parts lie side by side, so that hi.hi
-//     and hi.lo are one product of twice the width.
-//   O = P V: in one, for P has a largest value of 1 or more in every row and
-//     what is lost below 2^-24 of that does not count: lo(P) as it is times
-//     hi(V), and 2^-11 hi(P) times lo(V), then hi.hi.
+// The many-rows kernel for fp32.  Every operand x is carried as three bf16
+// parts, x0 = bf16(x), x1 = bf16(x - x0), x2 = bf16(x - x0 - x1): 8 bits each,
+// so that all 24 are there, and bf16 has fp32's range.  A product of two
+// operands is the six products of parts that count: x0 y0, x0 y1, x1 y0, x0 y2,
+// x1 y1, x2 y0; what is left out is 2^-25 of it at most.  (Two fp16 parts and
+// three products carried 22 bits of values from 2^-14 to 65504 only, and of
+// weights down to 2^-14: values of 1e-9 came out 8e-3 off, 1e5 as NaN.)
+//   S = Q K^T: in two fp32 accumulators, (q0 + q1) k0 and the rest, for K's
+//     parts lie one behind the other and [k0 | k1] is one product of twice the
+//     width.
+//   O = P V: in one, small products first.
 // The tensor cores cut their fp32 sums off, always towards zero.  Over a long
 // row that adds up (3.5e-8 of O per 16 keys, 3.6e-5 after 16500), so every
-// second tile the products so far are added to a sum of their own, in fp32 and
-// rounded to nearest, and begin anew: 4e-7 of O at any length.
-// The parts' range is fp16's: a value of 65520 or more gives NaN.  One tile of
-// 128 rows, tiles of 64 keys:
-//   warp 0       TMA producer: raw fp32 K and V tiles through a ring
+// tile's products are added to a sum of their own, in fp32 and rounded to
+// nearest: 3.6e-7 of O at any length.  A value that is not finite, or rounds
+// past bf16's largest, gives NaN.  One tile of 128 rows, tiles of 64 keys:
+//   warp 0       TMA producer: raw fp32 K and V through a ring, 8 KB a stage
 //   warp 1       MMA issuer; S of the next tile goes ahead of O += P V of this one
 //   warps 4-11   softmax, two threads per row with half the tile's keys each,
-//                which tell each other the maxima they find (P's own two parts
-//                over S's columns)
-//   warps 12-19  split Q, then each raw tile, into the fp16 parts; V's slots
+//                which tell each other the maxima they find (P's parts over
+//                S's columns)
+//   warps 12-19  split Q, then each raw stage, into the parts; V's slots
 //                behind the last key, which may hold anything, become zero
-// TMEM: two buffers of S (hi.hi | cross, 64 columns each), the products, their sum.
+// TMEM: two buffers of S (two accumulators of 64 columns each), the products, their sum.
 // Bound by the chain from a raw tile to its product, which the 227 KB leave no
-// room to double: the chunks above 1117 us, 191 TFLOP/s (574 of fp16 products).
+// room to double: 2.9 us a tile where a CTA has a share of its own (the two fp16
+// parts took 2.3), 44 % of the tensor cores' cycles; 12 chunks of 120 to 700
+// tokens behind 2050, 32 heads of 128, 1205 us, 177 TFLOP/s (1060 of bf16
+// products; two fp16 parts 1116 us).  The warps' parts run side by side and
+// share the instruction cache: with the splits and products unrolled at every
+// place, 128 KB of code, the same took 1.7 times as long.
 constexpr int TF_N = 64;              // keys of a tile
 constexpr int TF_BOX = 8;             // keys of a copy
 constexpr int TF_THREADS = 20 * 32;
 constexpr int TF_CONV = 8;            // warps that split
-constexpr int TF_FOLD = 2;            // tiles after which the products go to the sum
 constexpr float TF_RAISE = 8.f;       // a row's reference is raised when a weight passes 2^8
 
 template <int HD>
@@ -1274,36 +1282,46 @@ struct ManyRowsF32 {
   static constexpr int QT = TC_M * HD * 2;          // bytes of one part of Q
   static constexpr int CH = TF_N * 128;             // bytes of a 64-wide column of one part of a tile
   static constexpr int PT = NCH * CH;               // bytes of one part of a K or V tile
-  static constexpr int RAW = TF_N * HD * 4;         // bytes of a raw tile
+  static constexpr int LPK = HD / 8;                // lanes that split a key, 8 values each
+  static constexpr int KPW = 32 / LPK;              // keys of a warp at a time
+  static constexpr int KEYS = TF_CONV * KPW;        // keys of a raw stage: one of each lane's turns
+  static constexpr int STEPS = TF_N / KEYS;         // stages of a tile
   static constexpr int BOX = TF_BOX * HD * 4;       // bytes of one copy
-  static constexpr int NRAW = HD == 128 ? 3 : 6;
-  static constexpr int SMEM = 2 * QT + 4 * PT + NRAW * RAW;  // to the last byte of 227 KB with the static part
+  static constexpr int COPIES = KEYS / TF_BOX;      // copies of a stage
+  static constexpr int RAW = COPIES * BOX;          // bytes of a stage
+  static constexpr int NRAW = HD == 128 ? 4 : 12;
+  static constexpr int SMEM = 3 * QT + 6 * PT + NRAW * RAW;  // to the last byte of 227 KB with the static part
 };
 
-// two fp32 -> their fp16 parts, packed
-__device__ __forceinline__ void split_f16(float x, float y, uint32_t& hi, uint32_t& lo) {
-  const __half2 h = __floats2half2_rn(x, y);
-  const float2 f = __half22float2(h);
-  hi = h2_as_u32(h);
-  lo = h2_as_u32(__floats2half2_rn((x - f.x) * 2048.f, (y - f.y) * 2048.f));
+// two fp32 -> bf16, packed, x in the low half
+__device__ __forceinline__ uint32_t bf16_pair(float x, float y) {
+  uint32_t d;
+  asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(d) : "f"(y), "f"(x));
+  return d;
 }
-// two weights -> hi, lo as it is, 2^-11 hi
-__device__ __forceinline__ void split_weight(float x, float y, uint32_t& hi, uint32_t& lo, uint32_t& low_hi) {
-  const __half2 h = __floats2half2_rn(x, y);
-  const float2 f = __half22float2(h);
-  hi = h2_as_u32(h);
-  lo = h2_as_u32(__floats2half2_rn(x - f.x, y - f.y));
-  low_hi = h2_as_u32(__hmul2(h, __float2half2_rn(1.f / 2048.f)));
+// two fp32 -> their three bf16 parts, packed; the differences are exact
+__device__ __forceinline__ void split_bf16(float x, float y, uint32_t& p0, uint32_t& p1, uint32_t& p2) {
+  const uint64_t minus = pack2(-1.f, -1.f);
+  uint64_t rest = pack2(x, y);
+  p0 = bf16_pair(x, y);
+  rest = fma2(pack2(__uint_as_float(p0 << 16), __uint_as_float(p0 & 0xffff0000u)), minus, rest);
+  unpack2(rest, x, y);
+  p1 = bf16_pair(x, y);
+  rest = fma2(pack2(__uint_as_float(p1 << 16), __uint_as_float(p1 & 0xffff0000u)), minus, rest);
+  unpack2(rest, x, y);
+  p2 = bf16_pair(x, y);
 }
-// eight fp32 -> 16 bytes of each part, at shared addresses h and l
-__device__ __forceinline__ void split_f16x8(const float4& a, const float4& b, uint32_t h, uint32_t l) {
-  uint32_t hi[4], lo[4];
-  split_f16(a.x, a.y, hi[0], lo[0]);
-  split_f16(a.z, a.w, hi[1], lo[1]);
-  split_f16(b.x, b.y, hi[2], lo[2]);
-  split_f16(b.z, b.w, hi[3], lo[3]);
-  asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(h), "r"(hi[0]), "r"(hi[1]), "r"(hi[2]), "r"(hi[3]) : "memory");
-  asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(l), "r"(lo[0]), "r"(lo[1]), "r"(lo[2]), "r"(lo[3]) : "memory");
+// eight fp32 -> 16 bytes of each part, at shared address `at` and `part` bytes further each
+__device__ __forceinline__ void split_bf16x8(const float4& a, const float4& b, uint32_t at, uint32_t part) {
+  uint32_t y[3][4];
+  split_bf16(a.x, a.y, y[0][0], y[1][0], y[2][0]);
+  split_bf16(a.z, a.w, y[0][1], y[1][1], y[2][1]);
+  split_bf16(b.x, b.y, y[0][2], y[1][2], y[2][2]);
+  split_bf16(b.z, b.w, y[0][3], y[1][3], y[2][3]);
+#pragma unroll
+  for (int i = 0; i < 3; ++i)
+    asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(at + i * part), "r"(y[i][0]), "r"(y[i][1]), "r"(y[i][2]), "r"(y[i][3])
+                 : "memory");
 }
 
 template <int HD, bool PACKED>
@@ -1317,7 +1335,7 @@ many_rows_f32_kernel(const PrefixAttnParams p, const __grid_constant__ PoolMaps 
   __shared__ int s_abort, s_req, s_row0, s_sum[TF_THREADS / 32];
   __shared__ float s_max[2][2][TC_M];  // by tile's parity, by half
   __shared__ int s_any_bad, s_bad[PACKED ? 1 : HD];  // per column the first hidden key with an infinity or NaN
-  const uint32_t q_u = smem_u32(mf_smem), k_u = q_u + 2 * C::QT, v_u = k_u + 2 * C::PT, raw_u = v_u + 2 * C::PT;
+  const uint32_t q_u = smem_u32(mf_smem), k_u = q_u + 3 * C::QT, v_u = k_u + 3 * C::PT, raw_u = v_u + 3 * C::PT;
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   const int split = blockIdx.x % splits, item = blockIdx.x / splits, h = blockIdx.y;
   if (q_u & 1023) {  // the tiles' swizzle counts on the declared alignment
@@ -1358,9 +1376,7 @@ many_rows_f32_kernel(const PrefixAttnParams p, const __grid_constant__ PoolMaps 
   const RowShare w = row_share<PACKED, TC_M, TF_N, TF_THREADS>(p, item, split, splits, s_req, s_row0, s_sum);
   const int np = w.np, cnt = w.cnt;
   auto keys_of = [&](int t) { return t < np ? w.P - t * TF_N : w.own - (t - np) * TF_N; };
-  // K tiles run one ahead of V tiles through the ring: K0 K1 V0 K2 V1 ...; the place of tile i's K and V
-  auto k_at = [&](int i) { return (uint32_t)(i == 0 ? 0 : 2 * i - 1); };
-  auto v_at = [&](int i) { return (uint32_t)(i + 1 < cnt ? 2 * i + 2 : 2 * i + 1); };
+  // K tiles run one ahead of V tiles through the ring: K0 K1 V0 K2 V1 ...
 
   if (warp == 0) {
     // ================================ TMA producer ================================
@@ -1376,24 +1392,28 @@ many_rows_f32_kernel(const PrefixAttnParams p, const __grid_constant__ PoolMaps 
       if (lane == 0) s_absent[i & 15] = gone;  // a bit per copy
       return at;
     };
-    auto copy = [&](const CUtensorMap* map, int at, uint32_t it) {
-      const int s = it % NRAW;
-      if (!__all_sync(0xffffffffu, pa_wait(&raw_empty[s], ((it / NRAW) & 1u) ^ 1u, abort))) return false;
-      if (lane == 0) mbar_arrive_expect_tx(&raw_full[s], C::RAW);
-      __syncwarp();
-      if (lane < TF_N / TF_BOX) tma3d_at(raw_u + s * C::RAW + lane * C::BOX, map, at < 0 ? p.pool_rows : at, 0, &raw_full[s]);
+    uint32_t it = 0;
+    auto copy = [&](const CUtensorMap* map, int rows) {
+#pragma unroll
+      for (int j = 0; j < C::STEPS; ++j, ++it) {
+        const int s = it % NRAW, at = __shfl_sync(0xffffffffu, rows, j * C::COPIES + lane % C::COPIES);
+        if (!__all_sync(0xffffffffu, pa_wait(&raw_empty[s], ((it / NRAW) & 1u) ^ 1u, abort))) return false;
+        if (lane == 0) mbar_arrive_expect_tx(&raw_full[s], C::RAW);
+        __syncwarp();
+        if (lane < C::COPIES) tma3d_at(raw_u + s * C::RAW + lane * C::BOX, map, at < 0 ? p.pool_rows : at, 0, &raw_full[s]);
+      }
       return true;
     };
-    uint32_t it = 0;
     bool ok = true;
     int row = -1, before = -1;
+#pragma unroll 1
     for (int i = 0; i <= cnt && ok && cnt; ++i) {  // K of tile i, then V of tile i - 1
       before = row;
       if (i < cnt) {
         row = rows_of(i);
-        if ((ok = copy(&maps.k, row, it))) ++it;
+        ok = copy(&maps.k, row);
       }
-      if (i > 0 && ok && (ok = copy(&maps.v, before, it))) ++it;
+      if (i > 0 && ok) ok = copy(&maps.v, before);
     }
     if (lane == 0) {  // copies in flight land before the CTA may exit
       int ignore = 0;
@@ -1402,99 +1422,96 @@ many_rows_f32_kernel(const PrefixAttnParams p, const __grid_constant__ PoolMaps 
   } else if (warp == 1) {
     // ================================ MMA issuer ================================
     if (lane == 0 && cnt > 0) {
-      constexpr uint32_t mn = (1u << 4) | ((TC_M >> 4) << 24);
+      constexpr uint32_t mn = (1u << 4) | (1u << 7) | (1u << 10) | ((TC_M >> 4) << 24);  // bf16 by bf16 into fp32
       constexpr uint32_t idesc_s2 = mn | ((2 * TF_N >> 3) << 17), idesc_s = mn | ((TF_N >> 3) << 17);
       constexpr uint32_t idesc_o = mn | (1u << 16) | ((HD >> 3) << 17);
-      const uint64_t qh = umma_desc_sw128(q_u), ql = umma_desc_sw128(q_u + C::QT), kd = umma_desc_sw128(k_u);
+      const uint64_t q0 = umma_desc_sw128(q_u), q1 = umma_desc_sw128(q_u + C::QT), q2 = umma_desc_sw128(q_u + 2 * C::QT);
+      const uint64_t kd = umma_desc_sw128(k_u);
       const uint64_t vd = umma_desc_sw128_mn(v_u, CH);
       const uint32_t to = tmem + 256;
-      auto issue_s = [&](int i) {
-        const uint32_t ts = tmem + (i & 1) * 128;
-#pragma unroll
-        for (int kk = 0; kk < HD / 16; ++kk) {
-          // K: 64-wide column, in it the 64 rows of hi, then those of lo
-          const uint32_t qo = ((kk >> 2) * (TC_M * 128) + (kk & 3) * 32) >> 4, ko = ((kk >> 2) * 2 * CH + (kk & 3) * 32) >> 4;
-          umma_f16(ts, qh + qo, kd + ko, idesc_s2, kk != 0);
-          umma_f16(ts + 64, ql + qo, kd + ko, idesc_s, 1u);
-        }
-        tc_commit(&s_full[i & 1]);
-      };
-      bool ok = pa_spin(&q_full, 0, abort) && pa_spin(&k_full, 0, abort);
-      if (ok) {
-        tc_fence_after();
-        issue_s(0);
-      }
-      for (int i = 0; i < cnt && ok; ++i) {
-        if (i + 1 < cnt) {  // its buffer held P of tile i - 1, whose product comes before this one
+      bool ok = pa_spin(&q_full, 0, abort);
+#pragma unroll 1
+      for (int i = -1; i < cnt && ok; ++i) {
+        if (i + 1 < cnt) {  // S of the next tile; its buffer held P of tile i - 1, whose product comes before this one
           if (!(ok = pa_spin(&k_full, (i + 1) & 1, abort))) break;
           tc_fence_after();
-          issue_s(i + 1);
+          const uint32_t ts = tmem + ((i + 1) & 1) * 128;
+#pragma unroll
+          for (int kk = 0; kk < HD / 16; ++kk) {
+            // K: 64-wide column, in it the 64 rows of each part
+            const uint32_t qo = ((kk >> 2) * (TC_M * 128) + (kk & 3) * 32) >> 4, ko = ((kk >> 2) * 3 * CH + (kk & 3) * 32) >> 4;
+            umma_f16(ts, q0 + qo, kd + ko, idesc_s2, kk != 0);  // q0 k0 | q0 k1
+            umma_f16(ts, q1 + qo, kd + ko, idesc_s2, 1u);       // q1 k0 | q1 k1
+            umma_f16(ts + 64, q2 + qo, kd + ko, idesc_s, 1u);   // q2 k0
+            umma_f16(ts + 64, q0 + qo, kd + ko + (2 * CH >> 4), idesc_s, 1u);  // q0 k2
+          }
+          tc_commit(&s_full[(i + 1) & 1]);
         }
+        if (i < 0) continue;
         ok = pa_spin(&v_full, i & 1, abort) && pa_spin(&p_full[i & 1], (i >> 1) & 1, abort);
         if (!ok) break;
         tc_fence_after();
-        const uint32_t ph = tmem + (i & 1) * 128;  // hi, lo, 2^-11 hi
+        const uint32_t pt = tmem + (i & 1) * 128;  // P's parts, 32 columns each
+        auto product = [&](int a, int b, int kk, uint32_t accumulate) {  // part a of P by part b of V
+          umma_f16_ta(to, pt + a * 32 + kk * 8, vd + ((b * C::PT + kk * 2048) >> 4), idesc_o, accumulate);
+        };
 #pragma unroll
         for (int kk = 0; kk < TF_N / 16; ++kk) {
-          umma_f16_ta(to, ph + 32 + kk * 8, vd + kk * (2048 >> 4), idesc_o, (i % TF_FOLD | kk) != 0);
-          umma_f16_ta(to, ph + 64 + kk * 8, vd + ((C::PT + kk * 2048) >> 4), idesc_o, 1u);
+          product(2, 0, kk, kk != 0);
+          product(1, 1, kk, 1u);
+          product(0, 2, kk, 1u);
+          product(1, 0, kk, 1u);
+          product(0, 1, kk, 1u);
         }
 #pragma unroll
-        for (int kk = 0; kk < TF_N / 16; ++kk) umma_f16_ta(to, ph + kk * 8, vd + kk * (2048 >> 4), idesc_o, 1u);
+        for (int kk = 0; kk < TF_N / 16; ++kk) product(0, 0, kk, 1u);
         tc_commit(&pv_done);
         if (i + 1 == cnt) tc_commit(&o_full);
       }
     }
   } else if (warp >= 12) {
     // ================================ split Q, K and V ================================
-    constexpr int LPK = HD / 8, KPW = 32 / LPK;  // lanes per key (8 values each), keys per warp and step
-    constexpr int STEPS = TF_N / (TF_CONV * KPW);
+    constexpr int LPK = C::LPK, KPW = C::KPW, STEPS = C::STEPS;
     const int cw = warp - 12, g = lane % LPK, sub = lane / LPK;
     const bool odd = (g >> 2) & 1;
-    // Slots from `keys` on become zero, and what is not finite (or not in the parts' range) from `shown` on: rows that do not
+    uint32_t it = 0;
+    // Slots from `keys` on become zero, and what is not finite (or not in bf16) from `shown` on: rows that do not
     // see those keys have weights of zero for them, the others become NaN at the end.  key0: the tile's first own key.
-    auto convert = [&](uint32_t it, bool is_v, int keys, int shown, int key0) {
-      const int s = it % NRAW;
-      if (!__all_sync(0xffffffffu, pa_wait(&raw_full[s], (it / NRAW) & 1u, abort))) return false;
-      const uint32_t src = raw_u + s * C::RAW;
-      float4 a[STEPS], b[STEPS];
-#pragma unroll
-      for (int j = 0; j < STEPS; ++j) {
-        const int key = (j * TF_CONV + cw) * KPW + sub, r = key % TF_BOX;
+    auto convert = [&](bool is_v, int keys, int shown, int key0) {
+      const uint32_t to = is_v ? v_u + (g >> 3) * CH : k_u + (g >> 3) * 3 * CH, part = is_v ? C::PT : CH;
+#pragma unroll 1
+      for (int j = 0; j < STEPS; ++j, ++it) {
+        const int s = it % NRAW;
+        if (!__all_sync(0xffffffffu, pa_wait(&raw_full[s], (it / NRAW) & 1u, abort))) return false;
+        const int in = cw * KPW + sub, r = in % TF_BOX, key = j * C::KEYS + in;  // key of the stage, of the tile
         // 8 values: pieces 2 (g % 4) and 2 (g % 4) + 1 of 128-byte chunk g / 4; odd chunks in the other order, so that
         // eight lanes read all the banks
-        const uint32_t at = src + (key / TF_BOX) * C::BOX + (g >> 2) * (TF_BOX * 128) + r * 128;
+        const uint32_t at = raw_u + s * C::RAW + (in / TF_BOX) * C::BOX + (g >> 2) * (TF_BOX * 128) + r * 128;
         const int p0 = 2 * (g & 3) + odd;
-        a[j] = lds_f4(at + ((p0 ^ (r & 7)) << 4));
-        b[j] = lds_f4(at + (((p0 ^ 1) ^ (r & 7)) << 4));
-      }
-#pragma unroll
-      for (int j = 0; j < STEPS; ++j) {
-        const int key = (j * TF_CONV + cw) * KPW + sub;
-        if (key >= keys) a[j] = b[j] = make_float4(0.f, 0.f, 0.f, 0.f);
+        float4 a = lds_f4(at + ((p0 ^ (r & 7)) << 4)), b = lds_f4(at + (((p0 ^ 1) ^ (r & 7)) << 4));
+        if (key >= keys) a = b = make_float4(0.f, 0.f, 0.f, 0.f);
         if (!PACKED && key >= shown) {
-          float* y[8] = {&a[j].x, &a[j].y, &a[j].z, &a[j].w, &b[j].x, &b[j].y, &b[j].z, &b[j].w};
+          float* y[8] = {&a.x, &a.y, &a.z, &a.w, &b.x, &b.y, &b.z, &b.w};
 #pragma unroll
           for (int k = 0; k < 8; ++k) {
-            if (fabsf(*y[k]) < 65520.f) continue;  // what fp16 rounds to a number
+            if (fabsf(*y[k]) < __uint_as_float(0x7f7f8000u)) continue;  // what bf16 rounds to a number
             *y[k] = 0.f;
             atomicMin(&s_bad[PACKED ? 0 : g * 8 + ((k < 4) != odd ? k & 3 : 4 + (k & 3))], key0 + key);
             s_any_bad = 1;
           }
         }
-        const uint32_t c = sw128(key, g & 7);
-        const uint32_t d = is_v ? v_u + (g >> 3) * CH + c : k_u + (g >> 3) * 2 * CH + c;
-        split_f16x8(odd ? b[j] : a[j], odd ? a[j] : b[j], d, d + (is_v ? C::PT : CH));
+        split_bf16x8(odd ? b : a, odd ? a : b, to + sw128(key, g & 7), part);
+        __syncwarp();  // the stage's values are in registers
+        if (lane == 0) mbar_arrive(&raw_empty[s]);
       }
       fence_async_smem();
       if (!PACKED) __threadfence_block();
       __syncwarp();
-      if (lane == 0) mbar_arrive(&raw_empty[s]);
       return true;
     };
     if (cnt > 0) {
       constexpr int QS = TC_M / (TF_CONV * KPW);  // this warp's share of Q's rows
-#pragma unroll
+#pragma unroll 1
       for (int j0 = 0; j0 < QS; j0 += 4) {
         float4 a[4], b[4];
 #pragma unroll
@@ -1510,8 +1527,7 @@ many_rows_f32_kernel(const PrefixAttnParams p, const __grid_constant__ PoolMaps 
         }
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-          const uint32_t d = q_u + (g >> 3) * (TC_M * 128) + sw128(((j0 + j) * TF_CONV + cw) * KPW + sub, g & 7);
-          split_f16x8(a[j], b[j], d, d + C::QT);
+          split_bf16x8(a[j], b[j], q_u + (g >> 3) * (TC_M * 128) + sw128(((j0 + j) * TF_CONV + cw) * KPW + sub, g & 7), C::QT);
         }
       }
       fence_async_smem();
@@ -1519,18 +1535,14 @@ many_rows_f32_kernel(const PrefixAttnParams p, const __grid_constant__ PoolMaps 
       if (lane == 0) mbar_arrive(&q_full);
     }
     bool ok = true;
-    for (int i = 0; i <= cnt && ok && cnt; ++i) {
-      if (i < cnt) {  // K of tile i, once S of tile i - 1 is done with the buffer
-        if (i > 0) ok = __all_sync(0xffffffffu, pa_wait(&s_full[(i - 1) & 1], ((i - 1) >> 1) & 1, abort));
-        ok = ok && convert(k_at(i), false, TF_N, TF_N, 0);
-        if (ok && lane == 0) mbar_arrive(&k_full);
-      }
-      if (i > 0 && ok) {  // V of tile i - 1, once the product of tile i - 2 is
-        if (i > 1) ok = __all_sync(0xffffffffu, pa_wait(&pv_done, (i - 2) & 1, abort));
-        const int t = w.t0 + w.step * (i - 1), key0 = (t - np) * TF_N;
-        ok = ok && convert(v_at(i - 1), true, keys_of(t), PACKED || t < np ? TF_N : w.all - key0, key0);
-        if (ok && lane == 0) mbar_arrive(&v_full);
-      }
+#pragma unroll 1
+    for (int n = 0; n < 2 * cnt && ok; ++n) {  // K0 K1 V0 K2 V1 ...
+      const bool is_v = n == 2 * cnt - 1 || (n > 0 && !(n & 1));
+      const int i = is_v ? (n - 1) >> 1 : (n + 1) >> 1, t = w.t0 + w.step * i, key0 = (t - np) * TF_N;
+      // K goes where S of the tile before is done with, V where the product of the tile before is
+      if (i > 0) ok = __all_sync(0xffffffffu, is_v ? pa_wait(&pv_done, (i - 1) & 1, abort) : pa_wait(&s_full[(i - 1) & 1], ((i - 1) >> 1) & 1, abort));
+      ok = ok && convert(is_v, is_v ? keys_of(t) : TF_N, PACKED || !is_v || t < np ? TF_N : w.all - key0, key0);
+      if (ok && lane == 0) mbar_arrive(is_v ? &v_full : &k_full);
     }
   } else if (warp >= 4) {
     // ================================ softmax ================================
@@ -1562,7 +1574,7 @@ many_rows_f32_kernel(const PrefixAttnParams p, const __grid_constant__ PoolMaps 
         tmem_ready(v);
         tmem_ready(x);
 #pragma unroll
-        for (int k = 0; k < 32; ++k) v[k] = fmaf(x[k], 1.f / 2048.f, v[k]);
+        for (int k = 0; k < 32; k += 2) unpack2(add2(pack2(v[k], v[k + 1]), pack2(x[k], x[k + 1])), v[k], v[k + 1]);
         if (__any_sync(0xffffffffu, lim < 32) || gone != 0) {
 #pragma unroll
           for (int k = 0; k < 32; ++k) v[k] = k < lim && !((gone >> (k / TF_BOX)) & 1u) ? v[k] : -INFINITY;
@@ -1583,7 +1595,6 @@ many_rows_f32_kernel(const PrefixAttnParams p, const __grid_constant__ PoolMaps 
         tc_fence_after();
         mx = fmaxf(mx, s_max[i & 1][half ^ 1][lanes + lane]);
         const bool up = __any_sync(0xffffffffu, mx > m + TF_RAISE);  // also from -inf; the other half comes to the same
-        const bool fold = i > 0 && i % TF_FOLD == 0;
         float f = 1.f;
         if (up) {
           const float mn = fmaxf(m, mx);
@@ -1591,51 +1602,47 @@ many_rows_f32_kernel(const PrefixAttnParams p, const __grid_constant__ PoolMaps 
           m = mn;
           l *= f;
         }
-        if (fold || (up && i > 0)) {  // the last product; the one before it precedes this tile's S
+        const float mm = m == -INFINITY ? 0.f : m;
+        const uint64_t c2 = pack2(c, c), m2 = pack2(-mm, -mm);
+        uint64_t l2 = pack2(0.f, 0.f);
+        const uint32_t pt = tl + (i & 1) * 128 + half * 16;
+#pragma unroll
+        for (int q = 0; q < 32; q += 16) {
+          uint32_t p0[8], p1[8], p2[8];
+#pragma unroll
+          for (int k = 0; k < 16; k += 2) {
+            float e0, e1;
+            unpack2(fma2(pack2(v[q + k], v[q + k + 1]), c2, m2), e0, e1);
+            e0 = ex2(e0);
+            e1 = ex2(e1);
+            l2 = add2(l2, pack2(e0, e1));
+            split_bf16(e0, e1, p0[k / 2], p1[k / 2], p2[k / 2]);
+          }
+          tmem_st8(pt + q / 2, p0);
+          tmem_st8(pt + 32 + q / 2, p1);
+          tmem_st8(pt + 64 + q / 2, p2);
+        }
+        if (i > 0) {  // the last tile's products, made while this tile's P was, go to the sum
           ok = __all_sync(0xffffffffu, pa_wait(&pv_done, (i - 1) & 1, abort));
           if (!ok) break;
           tc_fence_after();
-#pragma unroll
+#pragma unroll 1
           for (int q = 0; q < HD / 2; q += 32) {
             float u[32];
             tmem_ld32_wait(ot + q, u);
-            if (fold) {
-              if (i > TF_FOLD) {
-                float y[32];
-                tmem_ld32_wait(sum + q, y);
+            if (i > 1) {
+              float y[32];
+              tmem_ld32_wait(sum + q, y);
 #pragma unroll
-                for (int k = 0; k < 32; ++k) u[k] += y[k];
-              }
-#pragma unroll
-              for (int k = 0; k < 32; ++k) u[k] *= f;
-              tmem_st32(sum + q, u);
-            } else {
-#pragma unroll
-              for (int k = 0; k < 32; ++k) u[k] *= f;
-              tmem_st32(ot + q, u);
-              if (i > TF_FOLD) {
-                tmem_ld32_wait(sum + q, u);
-#pragma unroll
-                for (int k = 0; k < 32; ++k) u[k] *= f;
-                tmem_st32(sum + q, u);
-              }
+              for (int k = 0; k < 32; ++k) u[k] += y[k];
             }
+#pragma unroll
+            for (int k = 0; k < 32; ++k) u[k] *= f;
+            tmem_st32(sum + q, u);
           }
         }
-        const float mm = m == -INFINITY ? 0.f : m;
-        float l0 = 0.f, l1 = 0.f;
-        uint32_t hi[16], lo[16], low_hi[16];
-#pragma unroll
-        for (int k = 0; k < 32; k += 2) {
-          const float e0 = ex2(fmaf(v[k], c, -mm)), e1 = ex2(fmaf(v[k + 1], c, -mm));
-          l0 += e0;
-          l1 += e1;
-          split_weight(e0, e1, hi[k / 2], lo[k / 2], low_hi[k / 2]);
-        }
-        const uint32_t pt = tl + (i & 1) * 128 + half * 16;
-        tmem_st16(pt, hi);
-        tmem_st16(pt + 32, lo);
-        tmem_st16(pt + 64, low_hi);
+        float l0, l1;
+        unpack2(l2, l0, l1);
         l += l0 + l1;
         tmem_wait_st();
         tc_fence_before();
@@ -1658,7 +1665,7 @@ many_rows_f32_kernel(const PrefixAttnParams p, const __grid_constant__ PoolMaps 
 #pragma unroll
         for (int q = 0; q < HD / 2; q += 32) {
           tmem_ld32_wait(ot + q, v + q);
-          if (cnt > TF_FOLD) {
+          if (cnt > 1) {
             float x[32];
             tmem_ld32_wait(sum + q, x);
 #pragma unroll
@@ -1840,13 +1847,13 @@ static AttnPlan plan_attn(int T, int B, int Hkv, int G, int hd, bool f16, long l
   if (a.kind != AttnPlan::FEW) {
     // Shares of the keys until there is a CTA for every SM; with the own keys' kernel beside it, for this kernel's part
     // of the SMs only.  That part goes by the two kernels' work, as far as the host knows it: a tile takes an SM 2.1 us
-    // (256 rows, 128 keys, fp16) or 1.9 us (128 rows, 64 keys, fp32), and own keys, taken for half of what the tables
+    // (256 rows, 128 keys, fp16) or 2.9 us (128 rows, 64 keys, fp32), and own keys, taken for half of what the tables
     // hold, stream at 44 KB a us and SM.  Measured over the splits 3, 4, 6, 8, 10, 14: 64 requests behind 8197 tokens,
-    // fp16, 61, 53, 55, 58, 60, 64 us (the rule takes 4); 32 behind 4099, fp32, 68, 56, 44, 41, 44, 47 us (it takes 7).
+    // fp16, 61, 53, 55, 58, 60, 64 us (the rule takes 4); 32 behind 4099, fp32, 82, 68, 51, 45, 45, 48 us (it takes 8).
     long long part = 1000;
     const long long tiles = ceil_div(prefix_keys + (a.kind == AttnPlan::CHUNKS ? own_keys : 0), tile);
     if (a.kind == AttnPlan::SHARED) {
-      const double many = (double)items * Hkv * tiles * (f16 ? 2.1 : 1.9);
+      const double many = (double)items * Hkv * tiles * (f16 ? 2.1 : 2.9);
       const double few = (double)B * own_keys / 2 * Hkv * hd * (f16 ? 4 : 8) / 44e3;
       part = (long long)(1000 * many / (many + few));
     }

@@ -1,5 +1,5 @@
-"""The attention over a paged cache where number formats run out: weights far below the row's largest, in every kernel
-that a call may be cut into.  Against float64 on the device."""
+"""The attention over a paged cache where number formats run out: weights far below the row's largest, values of any size,
+in every kernel that a call may be cut into.  Against float64 on the device."""
 
 import math
 
@@ -72,7 +72,7 @@ def check(dtype, out, want, mass, dot, keys, tail):
     assert np.isfinite(out).all() and (err <= bound).all(), (worst, out[worst], want[worst], bound[worst])
 
 
-@pytest.mark.parametrize("dtype", ["f16"])
+@pytest.mark.parametrize("dtype", ["f16", "f32"])
 @pytest.mark.parametrize("kind", KINDS)
 @pytest.mark.parametrize("keys,bits", [(4099, 20.6), (16384, 20.6), (16384, 25.3)])
 @pytest.mark.parametrize("alike,sink", [(True, 0.0), (False, 0.0), (True, 1.0)])
@@ -90,3 +90,54 @@ def test_first_key_takes_most_of_the_weight(cuda, dtype, kind, keys, bits, alike
     d["v"][d["first"], :, 0] = sink
     d["q"] += (u * size).repeat_interleave(HQ // HKV, 0)
     check(dtype, *run(d, dtype, cuda))
+
+
+def normal(d, cuda, seed=5):
+    g = torch.Generator(device=cuda).manual_seed(seed)
+    for n in "kvq":
+        d[n] += torch.randn(d[n].shape, generator=g, device=cuda, dtype=torch.float64)
+    return g
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("what,size", [("v", 1e-6), ("v", 1e-9), ("v", 1e-20), ("v", 1e5), ("v", 1e30), ("kq", 1e-6), ("kq", 1e6), ("kq", 1e-20),
+                                       ("kq", 1e20)])
+def test_fp32_values_of_any_size(cuda, kind, what, size):
+    """v, or k against q, scaled far out of fp16's range: attn_bound is relative to the values, and holds as it is."""
+    d = batch(cuda, kind, "f32", 4099)
+    normal(d, cuda)
+    if what == "v":
+        d["v"] *= size
+    else:
+        d["k"] *= size
+        d["q"] /= size
+    check("f32", *run(d, "f32", cuda))
+
+
+@pytest.mark.parametrize("kind", KINDS)
+def test_fp32_values_of_all_sizes_at_once(cuda, kind):
+    """Every value of v with a power of two of its own, every channel of k with one that q has the inverse of."""
+    d = batch(cuda, kind, "f32", 4099)
+    g = normal(d, cuda)
+    two = lambda *shape: 2.0 ** torch.randint(-40, 41, shape, generator=g, device=cuda).double()  # noqa: E731
+    d["v"] *= two(*d["v"].shape)
+    e = two(HKV, HD)
+    d["k"] *= e[:, None]
+    d["q"] /= e.repeat_interleave(HQ // HKV, 0)
+    check("f32", *run(d, "f32", cuda))
+
+
+@pytest.mark.parametrize("keys", [200, 4099])
+def test_fp32_large_hidden_values(cuda, keys):
+    """Finite values of 1e30 among a chunk's last tokens: the rows before are the same bits as without, those that see them
+    are within the bound."""
+    outs = []
+    for size in (1.0, 1e30):
+        d = batch(cuda, "chunk", "f32", keys)
+        normal(d, cuda)
+        page, off = divmod(keys - 20, PAGE)
+        d["v"][page, :, off] *= size
+        r = run(d, "f32", cuda)
+        check("f32", *r)
+        outs.append(r[0])
+    assert np.array_equal(outs[0][:130], outs[1][:130]) and (outs[0][130:] != outs[1][130:]).any()
