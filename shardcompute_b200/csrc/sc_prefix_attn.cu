@@ -8,6 +8,7 @@
 // be summed apart (o, l, m) and joined later.  A row that sees no key is zero.
 #include <algorithm>
 #include <atomic>
+#include <type_traits>
 
 #include <cuda.h>
 #include <cudaTypedefs.h>
@@ -24,6 +25,15 @@ constexpr uint64_t PA_WAIT_NS = 2000000000ull;
 // thousands of keys 2^-25 below it vanished from the output, though not from the sum that divides it: 16384 keys behind
 // one that takes most of the weight and has a value of zero came out 8.6e-2 off, now 1.8e-4 (the output's own rounding).
 constexpr float PA_LIFT = 11.f, PA_RAISE = 4.f;
+
+// Where a row's reference m is this far from zero, c s - m in one rounding is no longer small at the largest score: m is
+// c s rounded, by up to half of fp32's step there (a weight of 2^16 at m = 2^24, past fp16, and of 2^128 at 2^31).
+// There c s is rounded by itself, as it was for m, so that the largest weight is what m was chosen for.
+constexpr float PA_FAR = 1048576.f;
+__device__ __forceinline__ float far_exponent(float s, float c, float m) {
+  const float d = __fsub_rn(__fmul_rn(s, c), m);
+  return d > PA_LIFT + PA_RAISE ? PA_LIFT + PA_RAISE : d;  // m - PA_LIFT is rounded as well; a NaN stays
+}
 
 // Raised by a kernel whose bounded wait ran out; read by
 // sc_prefix_attn_device_error.
@@ -326,6 +336,7 @@ few_rows_kernel(const PrefixAttnParams p, const __grid_constant__ PoolMaps maps,
 #pragma unroll
     for (int i = 0; i < NO; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
     float m0 = -INFINITY, m1 = -INFINITY, l0 = 0.f, l1 = 0.f;
+    bool far = false;  // of some row of this warp's
 
     for (int i = 0; i < cnt; ++i, ++used) {
       const int s = used % NST;
@@ -389,8 +400,8 @@ few_rows_kernel(const PrefixAttnParams p, const __grid_constant__ PoolMaps maps,
         x0 = fmaxf(x0, fmaxf(sc[NJ - 1][0], sc[NJ - 1][1]));
         x1 = fmaxf(x1, fmaxf(sc[NJ - 1][2], sc[NJ - 1][3]));
       }
-      x0 = fmaf(x0, p.c, -C::LIFT);
-      x1 = C::F16 ? fmaf(x1, p.c, -C::LIFT) : -INFINITY;
+      x0 = __fadd_rn(__fmul_rn(x0, p.c), -C::LIFT);
+      x1 = C::F16 ? __fadd_rn(__fmul_rn(x1, p.c), -C::LIFT) : -INFINITY;
       if (__any_sync(0xffffffffu, x0 > m0 + C::RAISE || x1 > m1 + C::RAISE)) {
 #pragma unroll
         for (int d = 1; d <= 2; d <<= 1) {
@@ -411,16 +422,25 @@ few_rows_kernel(const PrefixAttnParams p, const __grid_constant__ PoolMaps maps,
         }
         m0 = x0;
         m1 = x1;
+        far = __any_sync(0xffffffffu, (fabsf(m0) >= PA_FAR && m0 != -INFINITY) || (fabsf(m1) >= PA_FAR && m1 != -INFINITY));
       }
-      const float n0 = m0 == -INFINITY ? 0.f : m0, n1 = m1 == -INFINITY ? 0.f : m1;
+      float n0 = m0 == -INFINITY ? 0.f : m0, n1 = m1 == -INFINITY ? 0.f : m1, c = p.c;
+      if (far) {
+#pragma unroll
+        for (int j = 0; j < NJ; ++j)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) sc[j][e] = far_exponent(sc[j][e], c, e < 2 ? n0 : n1);
+        n0 = n1 = 0.f;
+        c = 1.f;
+      }
 #pragma unroll
       for (int j = 0; j < NJ; ++j) {
-        sc[j][0] = ex2(fmaf(sc[j][0], p.c, -n0));
-        sc[j][1] = ex2(fmaf(sc[j][1], p.c, -n0));
+        sc[j][0] = ex2(fmaf(sc[j][0], c, -n0));
+        sc[j][1] = ex2(fmaf(sc[j][1], c, -n0));
         l0 += sc[j][0] + sc[j][1];
         if (C::F16) {
-          sc[j][2] = ex2(fmaf(sc[j][2], p.c, -n1));
-          sc[j][3] = ex2(fmaf(sc[j][3], p.c, -n1));
+          sc[j][2] = ex2(fmaf(sc[j][2], c, -n1));
+          sc[j][3] = ex2(fmaf(sc[j][3], c, -n1));
           l1 += sc[j][2] + sc[j][3];
         }
       }
@@ -1045,6 +1065,7 @@ many_rows_kernel(const PrefixAttnParams p, const __grid_constant__ PoolMaps maps
     const int see = PACKED ? 0 : (valid ? max(0, min(len, len - n + r / p.G + 1)) : own);
     const float c = p.c;
     float m = -INFINITY, l = 0.f;
+    bool far = false;
     if (x < nx && cnt > 0) {
       // ---- Q: this warp's 32 rows, 16 bytes a lane, into the K-major swizzled tile
       constexpr int LPR = HD / 8;  // 16-byte pieces of a row
@@ -1098,12 +1119,13 @@ many_rows_kernel(const PrefixAttnParams p, const __grid_constant__ PoolMaps maps
             a2 = max3(a2, v[k + 4], v[k + 5]);
             a3 = max3(a3, v[k + 6], v[k + 7]);
           }
-          return fmaf(fmaxf(fmaxf(a0, a1), fmaxf(a2, a3)), c, -PA_LIFT);
+          return __fadd_rn(__fmul_rn(fmaxf(fmaxf(a0, a1), fmaxf(a2, a3)), c), -PA_LIFT);
         };
         auto raise = [&](float mx) {
           const float mn = fmaxf(m, mx);
           const float f = m == -INFINITY ? 0.f : ex2(m - mn);
           m = mn;
+          far = __any_sync(0xffffffffu, fabsf(m) >= PA_FAR && m != -INFINITY);
           l *= f;
           if (i > 0) {  // S is there: so is the last product into O
 #pragma unroll
@@ -1118,15 +1140,18 @@ many_rows_kernel(const PrefixAttnParams p, const __grid_constant__ PoolMaps maps
         };
         uint64_t l2[2];
         uint32_t pw[16];
-        const uint64_t c2 = pack2(c, c);
-        auto quarter = [&](int q) {  // P of 32 keys
+        auto quarter = [&](int q, auto is_far) {  // P of 32 keys
           const float mm = m == -INFINITY ? 0.f : m;
-          const uint64_t m2 = pack2(-mm, -mm);
+          const uint64_t c2 = pack2(c, c), m2 = pack2(-mm, -mm);
 #pragma unroll
           for (int k = 0; k < 32; k += 2) {
-            const uint64_t y = fma2(pack2(v[q * 32 + k], v[q * 32 + k + 1]), c2, m2);
             float e0, e1;
-            unpack2(y, e0, e1);
+            if constexpr (is_far) {
+              e0 = far_exponent(v[q * 32 + k], c, mm);
+              e1 = far_exponent(v[q * 32 + k + 1], c, mm);
+            } else {
+              unpack2(fma2(pack2(v[q * 32 + k], v[q * 32 + k + 1]), c2, m2), e0, e1);
+            }
             e0 = ex2(e0);
             e1 = ex2(e1);
             l2[(k >> 1) & 1] = add2(l2[(k >> 1) & 1], pack2(e0, e1));
@@ -1142,20 +1167,26 @@ many_rows_kernel(const PrefixAttnParams p, const __grid_constant__ PoolMaps maps
           if (!ok) break;
         }
         l2[0] = l2[1] = pack2(0.f, 0.f);
-        quarter(0);
-        tmem_st16(st, pw);  // over columns of S that have been read
+        auto weights = [&](auto is_far) {
+          quarter(0, is_far);
+          tmem_st16(st, pw);  // over columns of S that have been read
 #pragma unroll
-        for (int q = 1; q < TC_N / 32; ++q) {
-          if (q == TC_HAND && nx == 2 && lane == 0) mbar_arrive(&turn[x ^ 1][warp & 3]);
-          quarter(q);
-          tmem_st16(st + q * 16, pw);
-          if (q & 1) {
-            tmem_wait_st();
-            tc_fence_before();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&p_full[x][q >> 1]);
+          for (int q = 1; q < TC_N / 32; ++q) {
+            if (q == TC_HAND && nx == 2 && lane == 0) mbar_arrive(&turn[x ^ 1][warp & 3]);
+            quarter(q, is_far);
+            tmem_st16(st + q * 16, pw);
+            if (q & 1) {
+              tmem_wait_st();
+              tc_fence_before();
+              __syncwarp();
+              if (lane == 0) mbar_arrive(&p_full[x][q >> 1]);
+            }
           }
-        }
+        };
+        if (far)
+          weights(std::true_type{});
+        else
+          weights(std::false_type{});
         float l0, l1;
         unpack2(add2(l2[0], l2[1]), l0, l1);
         l += l0 + l1;
@@ -1556,6 +1587,7 @@ many_rows_f32_kernel(const PrefixAttnParams p, const __grid_constant__ PoolMaps 
     float m = -INFINITY, l = 0.f;
     const size_t row = valid ? (size_t)(w.row_lo + r / p.G) * p.Hq + h * p.G + r % p.G : 0;
     const size_t at = (size_t)(slot0 + split) * p.T * p.Hq + row;
+    bool far = false;
     if (cnt > 0) {
       bool ok = true;
       for (int i = 0; i < cnt; ++i) {
@@ -1600,28 +1632,40 @@ many_rows_f32_kernel(const PrefixAttnParams p, const __grid_constant__ PoolMaps 
           const float mn = fmaxf(m, mx);
           f = m == -INFINITY ? 0.f : ex2(m - mn);
           m = mn;
+          far = __any_sync(0xffffffffu, fabsf(m) >= PA_FAR && m != -INFINITY);
           l *= f;
         }
         const float mm = m == -INFINITY ? 0.f : m;
-        const uint64_t c2 = pack2(c, c), m2 = pack2(-mm, -mm);
         uint64_t l2 = pack2(0.f, 0.f);
         const uint32_t pt = tl + (i & 1) * 128 + half * 16;
+        auto weights = [&](auto is_far) {
+          const uint64_t c2 = pack2(c, c), m2 = pack2(-mm, -mm);
 #pragma unroll
-        for (int q = 0; q < 32; q += 16) {
-          uint32_t p0[8], p1[8], p2[8];
+          for (int q = 0; q < 32; q += 16) {
+            uint32_t p0[8], p1[8], p2[8];
 #pragma unroll
-          for (int k = 0; k < 16; k += 2) {
-            float e0, e1;
-            unpack2(fma2(pack2(v[q + k], v[q + k + 1]), c2, m2), e0, e1);
-            e0 = ex2(e0);
-            e1 = ex2(e1);
-            l2 = add2(l2, pack2(e0, e1));
-            split_bf16(e0, e1, p0[k / 2], p1[k / 2], p2[k / 2]);
+            for (int k = 0; k < 16; k += 2) {
+              float e0, e1;
+              if constexpr (is_far) {
+                e0 = far_exponent(v[q + k], c, mm);
+                e1 = far_exponent(v[q + k + 1], c, mm);
+              } else {
+                unpack2(fma2(pack2(v[q + k], v[q + k + 1]), c2, m2), e0, e1);
+              }
+              e0 = ex2(e0);
+              e1 = ex2(e1);
+              l2 = add2(l2, pack2(e0, e1));
+              split_bf16(e0, e1, p0[k / 2], p1[k / 2], p2[k / 2]);
+            }
+            tmem_st8(pt + q / 2, p0);
+            tmem_st8(pt + 32 + q / 2, p1);
+            tmem_st8(pt + 64 + q / 2, p2);
           }
-          tmem_st8(pt + q / 2, p0);
-          tmem_st8(pt + 32 + q / 2, p1);
-          tmem_st8(pt + 64 + q / 2, p2);
-        }
+        };
+        if (far)
+          weights(std::true_type{});
+        else
+          weights(std::false_type{});
         if (i > 0) {  // the last tile's products, made while this tile's P was, go to the sum
           ok = __all_sync(0xffffffffu, pa_wait(&pv_done, (i - 1) & 1, abort));
           if (!ok) break;

@@ -1,5 +1,5 @@
-"""The attention over a paged cache where number formats run out: weights far below the row's largest, values of any size,
-in every kernel that a call may be cut into.  Against float64 on the device."""
+"""The attention over a paged cache where number formats run out: weights far below the row's largest, values of any
+size, scores past what fp32 steps finely, in every kernel that a call may be cut into.  Against float64 on the device."""
 
 import math
 
@@ -141,3 +141,31 @@ def test_fp32_large_hidden_values(cuda, keys):
         check("f32", *r)
         outs.append(r[0])
     assert np.array_equal(outs[0][:130], outs[1][:130]) and (outs[0][130:] != outs[1][130:]).any()
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("dtype,size", [("f16", 200.0), ("f16", 1000.0), ("f16", 4000.0), ("f16", 15000.0), ("f32", 1e3), ("f32", 3e4), ("f32", 1e6),
+                                        ("f32", 1e9), ("f32", 1e15)])
+def test_large_scores(cuda, kind, dtype, size):
+    """q and k so large that a row's largest score alone counts: its value comes out, by as much as its own weight (fp16:
+    2^-11) and the output (as much again) are rounded; fp32: three roundings of 2^-24 and a quotient's, below 2^-20.  Rows
+    whose two largest scores differ by less than the products' error, 2^-16 of sum |q| |k|, are only looked at for numbers."""
+    d = batch(cuda, kind, dtype, 4099)
+    normal(d, cuda)
+    for n in "kq":
+        d[n] = d[n].clamp(-4, 4) * size
+    out, want, mass, dot, keys, tail = run(d, dtype, cuda)
+    assert np.isfinite(out).all()
+    q, k = d["q"].to(DT[dtype]).double(), d["k"].to(DT[dtype]).double()
+    G, new, clear = HQ // HKV, d["new"], []
+    for b, n in enumerate(d["lens"]):
+        for h in range(HQ):
+            flat = torch.cat([k[d["ptab"].long(), h // G].reshape(-1, HD)[: d["P"]], k[d["table"][b].long(), h // G].reshape(-1, HD)[:n]])
+            s = q[b * new:(b + 1) * new, h] @ flat.T / math.sqrt(HD)
+            s.masked_fill_(torch.arange(len(flat), device=cuda) > d["P"] + n - new + torch.arange(new, device=cuda)[:, None], -math.inf)
+            two = s.topk(2).values
+            clear.append((two[:, 0] - two[:, 1]).cpu().numpy())
+    clear = np.concatenate([np.stack(clear[i:i + HQ], 1) for i in range(0, len(clear), HQ)])  # [rows, HQ]
+    clear = clear > 20 + dot * 2.0**-16
+    assert clear.mean() > 0.5
+    assert np.abs(out - want)[clear].max() <= (2.0**-10 if dtype == "f16" else 2.0**-20) * 1.01 * np.abs(want).max()
