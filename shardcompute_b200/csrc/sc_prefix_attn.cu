@@ -1370,6 +1370,7 @@ many_rows_f32_kernel(const PrefixAttnParams p, const __grid_constant__ PoolMaps 
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   const int split = blockIdx.x % splits, item = blockIdx.x / splits, h = blockIdx.y;
   if (q_u & 1023) {  // the tiles' swizzle counts on the declared alignment
+    pdl_wait();  // few_rows_kernel relies on it here as well
     if (threadIdx.x == 0) atomicExch(&g_prefix_attn_error, 1);
     return;
   }
