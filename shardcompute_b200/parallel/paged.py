@@ -18,6 +18,7 @@ from .. import ops
 
 _WHY = {1: "not enough free pages", 2: "a request exceeds its block table", 4: "more new tokens than rows",
         8: "a negative length", 16: "the count of free pages is outside the stack"}
+_WHY_BACK = {**_WHY, 1: "no room for the pages given back (a page held twice)"}
 
 
 class PagedLayer(NamedTuple):
@@ -54,7 +55,9 @@ class PagedKVCache:
         self.lens = torch.zeros(max_batch, **i32)
         self.prefix_table = torch.full((blocks,), -1, **i32) if max_prefix else None
         self.prefix_len = torch.zeros(1, **i32) if max_prefix else None
-        self.status = torch.zeros(1, **i32)
+        # of the last reservation, and of the last truncation or release: a step's truncation must not cover its reservation's
+        self._status = torch.zeros(2, **i32)
+        self.status, self.truncate_status = self._status[:1], self._status[1:]
         self._q_start = torch.zeros(max_batch + 1, **i32)
         self._slots = torch.full((self.max_tokens,), -1, **i32)
         self._positions = torch.zeros(self.max_tokens, **i32)
@@ -77,7 +80,7 @@ class PagedKVCache:
     def truncate(self, keep: Union[torch.Tensor, Sequence[int]]) -> None:
         """Cut every request to its first ``keep[b]`` tokens; 0 ends it and gives its pages back."""
         ops.paged_truncate(self.lens, self._per_request("truncate", keep), self.block_table, self.free_pages, self.free_count,
-                           self.page_size, lens_out=self.lens, free_count_out=self.free_count, status=self.status)
+                           self.page_size, lens_out=self.lens, free_count_out=self.free_count, status=self.truncate_status)
 
     def share_prefix(self, request: int) -> None:
         """Make this request's tokens the prefix of the whole batch; the request is empty after it."""
@@ -101,13 +104,15 @@ class PagedKVCache:
             raise ValueError("requests still hold tokens behind the prefix")
         ops.paged_truncate(self.prefix_len, torch.zeros_like(self.prefix_len), self.prefix_table.view(1, -1), self.free_pages,
                            self.free_count, self.page_size, lens_out=self.prefix_len, free_count_out=self.free_count,
-                           status=self.status)
+                           status=self.truncate_status)
 
     def check(self) -> None:
-        """Raise ``ValueError`` if the last ``reserve`` or ``truncate`` was refused (reads the status from the device)."""
-        st = int(self.status)
-        if st:
-            raise ValueError("paged cache: " + ", ".join(why for bit, why in _WHY.items() if st & bit))
+        """Raise ``ValueError`` if the last ``reserve`` was refused, or the last ``truncate`` or ``release_prefix`` (reads both
+        status words from the device)."""
+        why = [f"{what}: " + ", ".join(w for bit, w in names.items() if st & bit)
+               for what, names, st in zip(("reserve", "truncate"), (_WHY, _WHY_BACK), self._status.tolist()) if st]
+        if why:
+            raise ValueError("paged cache, " + "; ".join(why))
 
     def layers(self) -> List[PagedLayer]:
         """``past_key_values`` of ``ParallelTransformer.forward``."""
