@@ -34,11 +34,21 @@ class PagedKVCache:
                  page_size: int = 16, max_prefix: int = 0, max_tokens: Optional[int] = None,
                  dtype: torch.dtype = torch.float32, device: Optional[torch.device] = None):
         """``max_len`` / ``max_prefix``: tokens of a request and of the shared prefix at most (0: none).
-        ``max_tokens``: new tokens of a step at most (default ``max_batch``, one each)."""
+        ``max_tokens``: new tokens of a step at most (default ``max_batch``, one each).  What the operators do not take is
+        refused here, not after pages were reserved and keys written: heads of 64 or 128, pages of a power of two from 16 to
+        32768 tokens, 16384 requests at most, and a pool whose rows (pages x heads x page size) count in 32 bits."""
         if dtype not in (torch.float16, torch.float32):
             raise ValueError(f"pages must be float16 or float32, got {dtype}")
         if min(num_layers, kv_heads, head_dim, n_pages, max_batch, max_len, page_size) < 1 or max_prefix < 0:
             raise ValueError("PagedKVCache: sizes must be positive")
+        if head_dim not in (64, 128):
+            raise ValueError(f"PagedKVCache: head_dim {head_dim} unsupported (64, 128)")
+        if not 16 <= page_size <= 32768 or page_size & (page_size - 1):
+            raise ValueError(f"PagedKVCache: page_size {page_size} unsupported (a power of two from 16 to 32768)")
+        if max_batch > 16384 or (max_tokens is not None and max_tokens < 1):
+            raise ValueError(f"PagedKVCache: 1..16384 requests and at least one new token, got {max_batch} and {max_tokens}")
+        if max(n_pages * kv_heads * page_size, max_len + page_size, max_prefix + page_size) >= 2**31:
+            raise ValueError("PagedKVCache: rows of the pool, or tokens of a request, past 32 bits")
         dev = device or torch.device("cuda", torch.cuda.current_device())
         i32 = dict(dtype=torch.int32, device=dev)
         blocks = -(-max_len // page_size)

@@ -1,0 +1,29 @@
+"""PagedKVCache's refusals, before anything is allocated."""
+
+import pytest
+import torch
+
+from shardcompute_b200.parallel import PagedKVCache
+
+
+def cache(**kw):
+    a = dict(num_layers=1, kv_heads=2, head_dim=64, n_pages=4, max_batch=2, max_len=64, device=torch.device("cpu"))
+    return PagedKVCache(**{**a, **kw})
+
+
+@pytest.mark.parametrize("kw,match", [(dict(head_dim=40), "head_dim"), (dict(head_dim=256), "head_dim"), (dict(page_size=8), "page_size"),
+                                      (dict(page_size=48), "page_size"), (dict(page_size=1 << 16), "page_size"),
+                                      (dict(max_batch=16385), "requests"), (dict(max_tokens=0), "token"), (dict(max_tokens=-4), "token"),
+                                      (dict(n_pages=1 << 26), "32 bits"), (dict(max_len=2**31 - 8), "32 bits"),
+                                      (dict(max_prefix=2**31 - 1), "32 bits"), (dict(n_pages=0), "positive"), (dict(max_prefix=-1), "positive"),
+                                      (dict(dtype=torch.bfloat16), "float16 or float32")])
+def test_refuses_what_the_operators_do_not_take(kw, match):
+    with pytest.raises(ValueError, match=match):
+        cache(**kw)
+
+
+@pytest.mark.parametrize("kw", [dict(), dict(head_dim=128, page_size=128, max_prefix=300), dict(dtype=torch.float16, max_tokens=1)])
+def test_takes_the_rest(kw):
+    c = cache(**kw)
+    assert c.k.shape[2:] == (2, c.page_size, kw.get("head_dim", 64)) and int(c.free_count) == 4
+    c.check()
