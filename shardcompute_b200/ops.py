@@ -518,6 +518,14 @@ def prefix_attn(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, q
     return out
 
 
+def prefix_attn_device_error(device: Optional[torch.device] = None, reset: bool = True) -> int:
+    """Nonzero after a CTA of ``prefix_attn`` on this device gave up a bounded wait: outputs since the last reset are undefined.
+    Waits for the device's current stream."""
+    with torch.cuda.device(device):
+        torch.cuda.current_stream().synchronize()
+        return int(L.load().sc_prefix_attn_device_error(int(reset)))
+
+
 # ---------------------------------------------------------------- K5 / K7
 
 def rmsnorm(x: torch.Tensor, w: torch.Tensor, eps: float, out_dtype: Optional[torch.dtype] = None) -> torch.Tensor:

@@ -118,11 +118,13 @@ class PagedKVCache:
 
     def check(self) -> None:
         """Raise ``ValueError`` if the last ``reserve`` was refused, or the last ``truncate`` or ``release_prefix`` (reads both
-        status words from the device)."""
+        status words from the device), and ``RuntimeError`` if the attention gave up a wait since the last check."""
         why = [f"{what}: " + ", ".join(w for bit, w in names.items() if st & bit)
                for what, names, st in zip(("reserve", "truncate"), (_WHY, _WHY_BACK), self._status.tolist()) if st]
         if why:
             raise ValueError("paged cache, " + "; ".join(why))
+        if self.lens.is_cuda and ops.prefix_attn_device_error(self.lens.device):
+            raise RuntimeError("prefix_attn gave up a bounded wait: the attention's outputs since the last check are undefined")
 
     def layers(self) -> List[PagedLayer]:
         """``past_key_values`` of ``ParallelTransformer.forward``."""
