@@ -335,7 +335,8 @@ int sc_paged_rope_append(const void* qkv, int qkv_dtype, int rows, const int32_t
  *   q, out [T, Hq * hd], k_pages, v_pages: all fp16 or all fp32 (dtype);
  *   hd 64 or 128; page_size a power of two, 16 or more; scale > 0.
  *   prefix_len NULL: no prefix.  Rows from q_start[B] on are left as they
- *   were; a row that sees no token is zero.  Pages whose id is outside
+ *   were; where T is less than q_start[B], the T rows are those of the whole
+ *   call.  A row that sees no token is zero.  Pages whose id is outside
  *   0..n_pages-1 count as absent: their tokens are not seen.  What a row does
  *   not see has no influence on it, whatever it is (infinities and NaN too).
  * Softmax statistics and sums are fp32; with fp16 the weights are rounded

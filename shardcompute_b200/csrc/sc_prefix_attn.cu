@@ -61,10 +61,13 @@ __device__ __forceinline__ float ex2(float x) {
   return y;
 }
 
-// The request's rows [lo, hi) in q, clamped so that no device value leads out of bounds.
-__device__ __forceinline__ void request_rows(const PrefixAttnParams& p, int b, int& lo, int& hi) {
-  lo = min(max(p.q_start[b], 0), p.T);
-  hi = min(max(p.q_start[b + 1], lo), p.T);
+// The request's rows [lo, hi) in q, clamped so that no device value leads out of bounds, and its new tokens, which are
+// more where q ends before them.
+__device__ __forceinline__ void request_rows(const PrefixAttnParams& p, int b, int& lo, int& hi, int& n) {
+  const int from = max(p.q_start[b], 0), to = max(p.q_start[b + 1], from);
+  lo = min(from, p.T);
+  hi = min(to, p.T);
+  n = to - from;
 }
 __device__ __forceinline__ int request_len(const PrefixAttnParams& p, int b) {
   const long long cap = (long long)p.max_blocks << p.lg_page;
@@ -260,15 +263,15 @@ few_rows_kernel(const PrefixAttnParams p, const __grid_constant__ PoolMaps maps,
     return ((id * p.Hkv + h) << p.lg_page) + ((int)key & ((1 << p.lg_page) - 1));
   };
   const int rows0 = rows_of(0);
-  int row_lo, row_hi;
-  request_rows(p, b, row_lo, row_hi);
-  const int n = row_hi - row_lo, len = request_len(p, b);
+  int row_lo, row_hi, n;
+  request_rows(p, b, row_lo, row_hi, n);
+  const int rows_b = (row_hi - row_lo) * p.G, len = request_len(p, b);
   unsigned char* ring = base + (size_t)warp * NST * C::STAGE;
   const uint32_t ring_u = smem_u32(ring);
   uint32_t issued = 0, used = 0;  // tiles of this warp's ring, over all row tiles
 
-  for (int r0 = group * RT; r0 < n * p.G; r0 += row_groups * RT) {
-    const int nr = min(RT, n * p.G - r0);
+  for (int r0 = group * RT; r0 < rows_b; r0 += row_groups * RT) {
+    const int nr = min(RT, rows_b - r0);
     // own keys that the tile's last row sees
     const int own = max(0, min(len, len - n + (r0 + nr - 1) / p.G + 1));
     const int nt = np + (own + KT - 1) / KT;
@@ -551,7 +554,7 @@ few_rows_kernel(const PrefixAttnParams p, const __grid_constant__ PoolMaps maps,
     const bool failed = __syncthreads_or(issued != used);  // a wait ran out (also: every ring is free)
     if (failed) {
       if (CLUSTER)  // the others' barriers: two for this tile of rows and for each that follows
-        for (int r = r0; r < n * p.G; r += row_groups * RT) {
+        for (int r = r0; r < rows_b; r += row_groups * RT) {
           cluster_sync();
           cluster_sync();
         }
@@ -807,7 +810,7 @@ __device__ __forceinline__ RowShare row_share(const PrefixAttnParams& p, int ite
   if (PACKED) {
     w.b = 0;
     w.row_lo = 0;
-    row_hi = min(max(p.q_start[p.B], 0), p.T);
+    w.n = row_hi = min(max(p.q_start[p.B], 0), p.T);
     w.r0 = item * ROWS;
     w.work = true;
   } else {
@@ -815,9 +818,9 @@ __device__ __forceinline__ RowShare row_share(const PrefixAttnParams& p, int ite
     int before = 0;
     for (int b0 = 0; b0 < p.B; b0 += THREADS) {
       const int bb = b0 + threadIdx.x;
-      int lo, hi, cnt = 0;
+      int lo, hi, n, cnt = 0;
       if (bb < p.B) {
-        request_rows(p, bb, lo, hi);
+        request_rows(p, bb, lo, hi, n);
         cnt = (int)(((long long)(hi - lo) * p.G + ROWS - 1) / ROWS);
       }
       int sum = cnt;
@@ -844,10 +847,9 @@ __device__ __forceinline__ RowShare row_share(const PrefixAttnParams& p, int ite
     w.work = s_req >= 0;
     w.b = max(s_req, 0);
     w.r0 = s_row0;
-    request_rows(p, w.b, w.row_lo, row_hi);
+    request_rows(p, w.b, w.row_lo, row_hi, w.n);
   }
-  w.n = row_hi - w.row_lo;
-  w.rows = w.n * p.G;  // fits: T * Hq does
+  w.rows = (row_hi - w.row_lo) * p.G;  // fits: T * Hq does
   w.work = w.work && w.r0 < w.rows;
   w.len = PACKED ? 0 : request_len(p, w.b);
   w.P = prefix_keys(p);
