@@ -27,7 +27,7 @@ and ``sc_prefix_attn`` take the place of the two cache kernels.
 from __future__ import annotations
 
 import math
-from typing import Optional
+from typing import Dict, List, Optional, Tuple
 
 import numpy as np
 import torch
@@ -52,23 +52,27 @@ class RoPE:
         self.device = device
         self.inv_freq = (np.float32(1.0) / (np.float32(base) ** (np.arange(0, head_dim, 2, dtype=np.float32)
                                                                    / np.float32(head_dim)))).astype(np.float32)
-        self._cos: Optional[torch.Tensor] = None
-        self._sin: Optional[torch.Tensor] = None
-        self._cache_seq_len = 0
+        self._tables: Dict[torch.device, Tuple[torch.Tensor, torch.Tensor]] = {}
+        self._outgrown: List[Tuple[torch.Tensor, torch.Tensor]] = []  # a captured step may read them still
 
     def tables(self, seq_len: int, device: torch.device):
         """fp32 cos/sin halves ``[len, hd/2]`` covering ``seq_len`` positions
-        (grown like the reference: max(seq, 2 * old, 256))."""
-        if seq_len > self._cache_seq_len or self._cos is None or self._cos.device != device:
-            n = max(seq_len, self._cache_seq_len * 2, 256)
+        (grown like the reference: max(seq, 2 * old, 256)).  Tables that were
+        given out stay where they are; all outgrown ones together are smaller
+        than the present one."""
+        have = self._tables.get(device)
+        old = 0 if have is None else have[0].shape[0]
+        if seq_len > old:
+            n = max(seq_len, old * 2, 256)
             t = np.arange(n, dtype=np.float32)
             if self.scaling_factor != 1.0:
                 t = (t / np.float32(self.scaling_factor)).astype(np.float32)
             f = np.outer(t, self.inv_freq).astype(np.float32)
-            self._cos = torch.from_numpy(np.cos(f).astype(np.float32)).to(device)
-            self._sin = torch.from_numpy(np.sin(f).astype(np.float32)).to(device)
-            self._cache_seq_len = n
-        return self._cos, self._sin
+            if have is not None:
+                self._outgrown.append(have)
+            have = self._tables[device] = (torch.from_numpy(np.cos(f).astype(np.float32)).to(device),
+                                           torch.from_numpy(np.sin(f).astype(np.float32)).to(device))
+        return have
 
     def __call__(self, q: torch.Tensor, k: torch.Tensor, position_offset: int = 0):
         S = q.shape[2]

@@ -27,3 +27,20 @@ def test_takes_the_rest(kw):
     c = cache(**kw)
     assert c.k.shape[2:] == (2, c.page_size, kw.get("head_dim", 64)) and int(c.free_count) == 4
     c.check()
+
+
+def test_outgrown_rotary_tables_stay():
+    """A captured step reads the tables that it was captured with: growing them must not free those."""
+    import gc
+    import weakref
+
+    from shardcompute_b200.parallel import RoPE
+
+    rope, cpu = RoPE(64), torch.device("cpu")
+    first = weakref.ref(rope.tables(100, cpu)[0])
+    small = rope.tables(100, cpu)[0].clone()
+    big = rope.tables(5000, cpu)
+    gc.collect()
+    assert first() is not None and torch.equal(first(), small) and torch.equal(big[0][: len(small)], small)
+    assert rope.tables(4000, cpu)[0] is big[0] and len(big[0]) == 5000
+    assert sum(len(c) for c, _ in rope._outgrown) < len(big[0])
