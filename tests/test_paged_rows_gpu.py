@@ -26,3 +26,20 @@ def test_q_ends_before_the_last_request(cuda, rng, dtype, prefix, new, rows):
     got = run_attn(cuda, d).double().cpu().numpy().reshape(want.shape)
     assert (np.abs(got - want) <= attn_bound(dtype, want, mass, dot, keys, tail, hd)).all()
     assert L.load().sc_prefix_attn_device_error(1) == 0
+
+
+@pytest.mark.parametrize("dtype", ["f16", "f32"])
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("page,B,hkv", [(128, 40, 4), (256, 40, 4), (4096, 8, 2), (32768, 2, 1)])
+def test_large_pages(cuda, rng, dtype, hd, page, B, hkv):
+    """Pages of a tile of keys and more, up to the largest: a token each behind a prefix that ends inside a page, then a
+    chunk behind it, and alone."""
+    hq = 2 * hkv
+    prefix = 3000
+    lens = [1, page // 2 + 1] + [int(x) for x in rng.integers(1, min(page, 600), B - 2)]
+    check_attn(cuda, dtype, make_attn(cuda, rng, dtype, hq, hkv, hd, page, prefix, lens, [1] * B), hq)
+    for prefix, n, own in ((page + 3 if page < 1000 else 131, 700, 700), (0, 650, 901)):
+        d = make_attn(cuda, rng, dtype, hq, hkv, hd, page, prefix, [own], [n])
+        if page < 1000:  # a page that is not there, in the prefix or among the chunk's own
+            (d["ptab"] if prefix else d["table"][0])[1] = -1
+        check_attn(cuda, dtype, d, hq)
