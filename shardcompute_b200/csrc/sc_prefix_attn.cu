@@ -1878,11 +1878,12 @@ static AttnPlan plan_attn(int T, int B, int Hkv, int G, int hd, bool f16, long l
   // beats the others: up to so many keys a CTA slot, in clusters of eight at most.  us in a graph, fp16, few | shared: 8 kv
   // heads of 128, 1050 keys a slot 17.6 | 21.2 and 17.6 | 20.2, 1300 19.1 | 19.7, 2100 28.1 | 23.8; 4 of 64, 1050 13.8 |
   // 16.1, 2050 21.2 | 18.8; few | chunks: 210 13.3 | 16.5, 410 13.4 | 21.3 and 18.6 | 24.8, 520 19.0 | 17.9 and 14.0 | 13.6,
-  // 1250 31.2 | 20.9.  fp32, few | shared: 160 13.0 | 17.5, 290 16.0 | 19.1, 325 18.9 | 18.6, 540 26.8 | 23.6; few | chunks:
-  // 64 7.8 | 12.0, 106 12.2 | 13.1, 118 12.2 | 10.8, 250 24.3 | 14.5.
+  // 1250 31.2 | 20.9.  fp32, few | shared: 142 12.6 | 16.0 and 8.4 | 11.0, 266 16.4 | 19.2, 277 17.9 | 15.6 and 13.2 | 12.4, 392
+  // 21.5 | 23.8 and 15.1 | 14.6, 490 36.2 | 19.1; few | chunks: 104 9.2 | 11.2, 121 11.1 | 16.1, 182 12.9 | 19.1, 225 18.2 |
+  // 18.2 and 13.3 | 12.1, 242 18.5 | 19.0 and 14.7 | 12.0, 303 19.4 | 17.0 and 15.0 | 12.0.
   const double load = (double)(own_keys + prefix_keys) * std::max(slots / FR_CLUSTER, (long long)B * Hkv * groups) / slots;
   const bool many = rows >= 64ll * B, shares = prefix_keys > 0 && B > 1;
-  if (load <= (many ? (f16 ? 450 : 110) : (f16 ? 1100 : 320)) || !(many || shares))
+  if (load <= (many ? (f16 ? 450 : 220) : (f16 ? 1100 : 320)) || !(many || shares))
     a.kind = AttnPlan::FEW;
   // A chunk fills its last tile of rows for itself alone, where SHARED packs all requests' rows: worth a second kernel while
   // a request has less than a tile and the prefix is most of what it sees (behind 2000 tokens, shared | chunks: 8 requests of
