@@ -1887,7 +1887,7 @@ static AttnPlan plan_attn(int T, int B, int Hkv, int G, int hd, bool f16, long l
     a.kind = AttnPlan::FEW;
   // A chunk fills its last tile of rows for itself alone, where SHARED packs all requests' rows: worth a second kernel while
   // a request has less than a tile and the prefix is most of what it sees (behind 2000 tokens, shared | chunks: 8 requests of
-  // 80 rows 29.3 | 43.9, of 160 21.1 | 27.6, of 240 55.8 | 40.1; behind 300 with 200 own, fp32, of 150 51.7 | 32.4).
+  // 80 rows 29.3 | 43.9, of 160 21.1 | 27.6, of 240 55.8 | 40.1; behind 300 with 200 own, fp32, of 150 57.1 | 37.7).
   else if (!many || (shares && rows < 192ll * B && prefix_keys >= 4 * own_keys))
     a.kind = AttnPlan::SHARED;
   else
@@ -1910,7 +1910,7 @@ static AttnPlan plan_attn(int T, int B, int Hkv, int G, int hd, bool f16, long l
     // No more shares than their longest one needs: eight tiles in five shares take two each, as in four.  A second share
     // brings the join: not for less than three tiles (us, chunks, one share | as many as there are SMs for; fp16: 3 requests
     // of 150 tokens, 2 tiles 14.3 | 21.6; 8 of 60 behind 300, 4 tiles in two shares 18.5 | 25.9; one of 150 behind 300, 4 in
-    // four 20.4 | 17.9; fp32: 8 of 20, 2 tiles 10.2 | 15.2).
+    // four 20.4 | 17.9; fp32: 8 of 20, 2 tiles 15.7 | 19.9).
     a.tc_splits = (int)ceil_div(tiles, ceil_div(tiles, a.tc_splits));
     if (a.kind == AttnPlan::CHUNKS && tiles - ceil_div(tiles, a.tc_splits) < 3) a.tc_splits = 1;
     // The tensor cores' cut-off sums lose 1.1e-9 of O per key; with fp16 that is left, up to 131072 keys a share (1.4e-4, the
@@ -2030,7 +2030,8 @@ int sc_prefix_attn(const void* q, const void* k_pages, const void* v_pages, int 
   SC_REQUIRE((long long)n_pages * Hkv * page_size < INT32_MAX && (long long)T * Hq <= (1 << 30) &&
                  (long long)max_blocks * page_size <= INT32_MAX && (long long)max_prefix_blocks * page_size <= INT32_MAX,
              SC_ERR_SHAPE, "prefix_attn: rows past 32 bits");
-  SC_REQUIRE(scale > 0.f && scale < INFINITY, SC_ERR_ARG, "prefix_attn: scale must be positive and finite");
+  const float c = scale * 1.4426950408889634f;  // log2(e)
+  SC_REQUIRE(scale > 0.f && c < INFINITY, SC_ERR_ARG, "prefix_attn: scale must be positive and below 2.3e38");
   SC_REQUIRE((((uintptr_t)q | (uintptr_t)k_pages | (uintptr_t)v_pages | (uintptr_t)out) & 15) == 0, SC_ERR_ARG,
              "prefix_attn: tensors must start on 16-byte boundaries");
   if (!prefix_len) max_prefix_blocks = 0;
@@ -2060,7 +2061,7 @@ int sc_prefix_attn(const void* q, const void* k_pages, const void* v_pages, int 
   p.Hkv = Hkv;
   p.G = Hq / Hkv;
   p.pool_rows = n_pages * Hkv * page_size;
-  p.c = scale * 1.4426950408889634f;
+  p.c = c;
   p.nslots = a.nslots;
   if (dtype == SC_F16)
     return hd == 128 ? run_attn<__half, 128>(p, k_pages, v_pages, a, stream) : run_attn<__half, 64>(p, k_pages, v_pages, a, stream);

@@ -1,4 +1,4 @@
-"""PagedKVCache's refusals, before anything is allocated."""
+"""What the paged cache refuses and keeps, without a GPU."""
 
 import pytest
 import torch
@@ -44,3 +44,12 @@ def test_outgrown_rotary_tables_stay():
     assert first() is not None and torch.equal(first(), small) and torch.equal(big[0][: len(small)], small)
     assert rope.tables(4000, cpu)[0] is big[0] and len(big[0]) == 5000
     assert sum(len(c) for c, _ in rope._outgrown) < len(big[0])
+
+
+def test_attn_refuses_a_scale_that_overflows_with_log2_e():
+    from shardcompute_b200 import _lib as L
+
+    at = 1 << 20  # an address that no refused call reads
+    call = lambda scale: L.load().sc_prefix_attn(at, at, at, L.SC_F16, 4, at, at, at, 4, 8, None, None, 0, 8, 2, 128, 100, 16, scale, at, at, 16,  # noqa: E731
+                                                 None)
+    assert call(3e38) == L.SC_ERR_ARG and "scale" in L.last_error()
