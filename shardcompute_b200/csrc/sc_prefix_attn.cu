@@ -96,10 +96,10 @@ __device__ __forceinline__ void tma3d_at(uint32_t dst, const CUtensorMap* map, i
 // stands in the loop.  The warps' results are joined at the end, and with
 // CLUSTER those of the CTAs that share a request's keys, each CTA a part of the
 // outputs from all the CTAs' shared memory: no partial results in memory, no
-// kernel after this one (four requests behind 500 tokens 12.3 -> 7.4 us).
+// kernel after this one (four requests behind 500 tokens 12.3 -> 7.6 us).
 // Few keys: bound by latency, three dependent loads before the first tile and
 // the joins.  Many: by the stream of keys, 64 requests of up to 1500 tokens, 8 kv
-// heads of 128, 40 us in fp16 and 74 us in fp32 (4.9 and 5.3 TB/s).
+// heads of 128, with the join 42 us in fp16 and 76 us in fp32 (4.8 and 4.7 TB/s).
 //
 // fp16: mma m16n8k16 over up to 16 rows (the request's tokens x the group's
 // heads).  P is rounded to fp16 for the second product, 2^11 to 2^15 high
@@ -665,7 +665,8 @@ few_rows_kernel(const PrefixAttnParams p, const __grid_constant__ PoolMaps maps,
 // only when a weight passes 2^15 (PA_LIFT); l is summed in fp32.
 // TMEM: S0 | S1 (128 columns each, P in the first 64), O0 | O1 (HD each).
 // Bound by the softmax's chain: 12 chunks of 120 to 700 tokens behind a prefix of
-// 2050, 32 heads of 128, 292 us, 731 TFLOP/s, 44 % of the tensor cores' cycles.
+// 2050, 32 heads of 128, 295 us in a graph, 722 TFLOP/s, 44 % of the tensor
+// cores' cycles (call after call, with the clock down under the power cap, 316 us).
 constexpr int TC_M = 128, TC_N = 128;   // rows and keys of a tile
 constexpr int TC_THREADS = 12 * 32;
 constexpr int TC_REGS_CTL = 88, TC_REGS_SM = 208;  // 128 x 88 + 256 x 208: what the block starts with, 384 x 168
@@ -1297,10 +1298,9 @@ many_rows_kernel(const PrefixAttnParams p, const __grid_constant__ PoolMaps maps
 //                behind the last key, which may hold anything, become zero
 // TMEM: two buffers of S (two accumulators of 64 columns each), the products, their sum.
 // Bound by the chain from a raw tile to its product, which the 227 KB leave no
-// room to double: 2.9 us a tile where a CTA has a share of its own (the two fp16
-// parts took 2.3), 44 % of the tensor cores' cycles; 12 chunks of 120 to 700
-// tokens behind 2050, 32 heads of 128, 1205 us, 177 TFLOP/s (1060 of bf16
-// products; two fp16 parts 1116 us).  The warps' parts run side by side and
+// room to double: 2.9 us a tile (the two fp16 parts took 2.3), 39 % of the tensor
+// cores' cycles; 12 chunks of 120 to 700 tokens behind 2050, 32 heads of 128,
+// 1210 us, 176 TFLOP/s (1060 of bf16 products; two fp16 parts 1116 us).  The warps' parts run side by side and
 // share the instruction cache: with the splits and products unrolled at every
 // place, 128 KB of code, the same took 1.7 times as long.
 constexpr int TF_N = 64;              // keys of a tile

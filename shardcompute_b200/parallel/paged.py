@@ -1,7 +1,8 @@
 """A KV cache of pages for a ragged batch, next to the contiguous ``KVCache``.
 
 ``PagedKVCache`` holds every layer's pool of pages ``[n_pages, Hkv/TP, page, hd]`` and, shared by all layers, the block
-table, the requests' lengths and the stack of free pages -- all on the device, so that a step can be captured.  A step
+table, the requests' lengths and the stack of free pages -- all on the device, so that a step can be captured (with counts
+that are device tensors; the first step runs outside of the capture, for it makes the model's rotary tables).  A step
 is: ``reserve`` room for each request's new tokens, run the model on the new tokens of all requests in a row
 (``input_ids`` ``[1, T]``) with ``past_key_values=cache.layers()``, then ``truncate`` what did not stay (rejected
 drafts, ended requests).  A request can be made the prefix that all others share (``share_prefix``): its keys and values
