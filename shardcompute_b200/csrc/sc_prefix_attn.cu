@@ -1290,7 +1290,7 @@ many_rows_kernel(const PrefixAttnParams p, const __grid_constant__ PoolMaps maps
 // nearest: 3.6e-7 of O at any length.  A value that is not finite, or rounds
 // past bf16's largest, gives NaN.  One tile of 128 rows, tiles of 64 keys:
 //   warp 0       TMA producer: raw fp32 K and V through a ring, 8 KB a stage
-//   warp 1       MMA issuer; S of the next tile goes ahead of O += P V of this one
+//   warp 1       MMA issuer; S of the next tile goes ahead of O = P V of this one
 //   warps 4-11   softmax, two threads per row with half the tile's keys each,
 //                which tell each other the maxima they find (P's parts over
 //                S's columns)
@@ -1298,11 +1298,12 @@ many_rows_kernel(const PrefixAttnParams p, const __grid_constant__ PoolMaps maps
 //                behind the last key, which may hold anything, become zero
 // TMEM: two buffers of S (two accumulators of 64 columns each), the products, their sum.
 // Bound by the chain from a raw tile to its product, which the 227 KB leave no
-// room to double: 2.9 us a tile (the two fp16 parts took 2.3), 39 % of the tensor
+// room to double: 2.9 us a tile (the two fp16 parts took 2.4), 39 % of the tensor
 // cores' cycles; 12 chunks of 120 to 700 tokens behind 2050, 32 heads of 128,
-// 1210 us, 176 TFLOP/s (1060 of bf16 products; two fp16 parts 1116 us).  The warps' parts run side by side and
-// share the instruction cache: with the splits and products unrolled at every
-// place, 128 KB of code, the same took 1.7 times as long.
+// 1210 us, 176 TFLOP/s (1060 of bf16 products; two fp16 parts 1116 us).  The
+// warps' parts run side by side and share the instruction cache: with the splits
+// and products unrolled at every place, 128 KB of code, the same took 1.7 times as
+// long.
 constexpr int TF_N = 64;              // keys of a tile
 constexpr int TF_BOX = 8;             // keys of a copy
 constexpr int TF_THREADS = 20 * 32;
@@ -1311,13 +1312,13 @@ constexpr float TF_RAISE = 8.f;       // a row's reference is raised when a weig
 
 template <int HD>
 struct ManyRowsF32 {
-  static constexpr int NCH = HD / 64;               // 64-wide fp16 columns
+  static constexpr int NCH = HD / 64;               // 64-wide bf16 columns
   static constexpr int QT = TC_M * HD * 2;          // bytes of one part of Q
   static constexpr int CH = TF_N * 128;             // bytes of a 64-wide column of one part of a tile
   static constexpr int PT = NCH * CH;               // bytes of one part of a K or V tile
   static constexpr int LPK = HD / 8;                // lanes that split a key, 8 values each
   static constexpr int KPW = 32 / LPK;              // keys of a warp at a time
-  static constexpr int KEYS = TF_CONV * KPW;        // keys of a raw stage: one of each lane's turns
+  static constexpr int KEYS = TF_CONV * KPW;        // keys of a raw stage, which the warps split in one go
   static constexpr int STEPS = TF_N / KEYS;         // stages of a tile
   static constexpr int BOX = TF_BOX * HD * 4;       // bytes of one copy
   static constexpr int COPIES = KEYS / TF_BOX;      // copies of a stage
