@@ -341,7 +341,9 @@ int sc_paged_rope_append(const void* qkv, int qkv_dtype, int rows, const int32_t
  *   not see has no influence on it, whatever it is (infinities and NaN too).
  * Softmax statistics and sums are fp32; with fp16 the weights are rounded
  * before their product with v: 2^-11 of each, down to 2^-25 of the row's
- * largest weight, and in steps of 2^-35 of that below.
+ * largest weight, and in steps of 2^-35 of that below; an infinity in v makes
+ * its column of the rows that see it infinite or NaN, and a row whose scores
+ * are all -inf counts as one that sees no token.
  * With fp32, q, k, v and the weights are taken to 2^-21 of each value, whatever
  * its size; values that are not finite, or of 3.39e38 or more in size, make
  * what sees them NaN. */
