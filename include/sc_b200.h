@@ -354,7 +354,46 @@ int sc_prefix_attn(const void* q, const void* k_pages, const void* v_pages, int 
                    const int32_t* prefix_table, const int32_t* prefix_len, int max_prefix_blocks, int Hq, int Hkv,
                    int hd, int n_pages, int page_size, float scale, void* out, void* workspace, size_t workspace_bytes,
                    cudaStream_t stream);
-/* Device-side error word of sc_prefix_attn: nonzero after a CTA gave up a
+/* The paged cache in 8 or 4 bits.  A token's k (rotated) and v of a head, in
+ * groups of `group` consecutive dims, are codes c of `bits` bits, a scale s and
+ * a bias b (fp16) that stand for s c + b:
+ *   b = min x rounded down, s = the smallest fp16 value with (2^bits - 1) s >=
+ *   max x - b, c = rint((x - b) / s), 0 where s is 0: at most s / 2 off x.
+ * A group that holds a value that is not finite, below -65504 or too far above
+ * 65504 for s stands for NaN.
+ *   hd 64 or 128; bits 4 or 8; group 32 or 64.
+ * Pages [n_pages, Hkv, sc_quant_page_bytes] of bytes, in blocks of 16 tokens
+ * whose order is the kernels' own (csrc/sc_quant.cuh); sc_paged_reserve and
+ * sc_paged_truncate serve them as they are, page sizes a multiple of 16.  The
+ * page's bytes, 0 for what is unsupported: */
+size_t sc_quant_page_bytes(int page_size, int hd, int bits, int group);
+/* sc_paged_rope_append that quantises k and v as it writes them; q_out fp16.
+ * The same rows, slots and positions are written, and left as they were. */
+int sc_paged_rope_append_q(const void* qkv, int qkv_dtype, int rows, const int32_t* rows_end, const int32_t* slots,
+                           const int32_t* positions, const float* cos_tab, const float* sin_tab, int max_pos, int Hq,
+                           int Hkv, int hd, void* q_out, void* pages, int bits, int group, int n_pages, int page_size,
+                           cudaStream_t stream);
+/* The tokens in `slots`, read back: k_out, v_out [rows, Hkv, hd] in out_dtype
+ * (fp16 or fp32): s c + b in fp32, rounded once.  Zeros for a slot outside the
+ * pool.  Rows from *rows_end on are left as they were (NULL: none).  A slot may
+ * be named more than once. */
+int sc_paged_read_q(const void* pages, int bits, int group, int n_pages, int page_size, int Hkv, int hd,
+                    const int32_t* slots, int rows, const int32_t* rows_end, void* k_out, void* v_out, int out_dtype,
+                    cudaStream_t stream);
+/* sc_prefix_attn over such pages, in all else as above: q, out fp16; page_size a
+ * power of two, 16 to 32768; 0 < scale < 5e28.  The products take the codes
+ * as they are; scores, softmax statistics and sums are fp32; weights times
+ * scales are rounded to fp16 before their product with v's codes: 2^-11 of each,
+ * down to 2^-25 of the row's largest.  A group that stands for NaN makes the
+ * rows that see it NaN (of v: its dims), and no others. */
+size_t sc_prefix_attn_q_workspace_bytes(int T, int B, int Hq, int Hkv, int hd, int max_blocks, int max_prefix_blocks,
+                                        int page_size);
+int sc_prefix_attn_q(const void* q, const void* pages, int bits, int group, int T, const int32_t* q_start,
+                     const int32_t* kv_lens, const int32_t* block_table, int B, int max_blocks,
+                     const int32_t* prefix_table, const int32_t* prefix_len, int max_prefix_blocks, int Hq, int Hkv,
+                     int hd, int n_pages, int page_size, float scale, void* out, void* workspace,
+                     size_t workspace_bytes, cudaStream_t stream);
+/* Device-side error word of sc_prefix_attn and sc_prefix_attn_q: nonzero after a CTA gave up a
  * bounded wait for its tiles (its rows are then undefined).  Synchronises
  * with the device; reset != 0 clears it. */
 int sc_prefix_attn_device_error(int reset);

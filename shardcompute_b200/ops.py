@@ -518,8 +518,174 @@ def prefix_attn(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, q
     return out
 
 
+# ---------------------------------------------------------------- paged cache in 8 or 4 bits
+
+class QuantPages(NamedTuple):
+    """A pool of pages in 8 or 4 bits: uint8 ``[n_pages, Hkv, bytes of a page]``, and what it holds."""
+
+    data: torch.Tensor
+    head_dim: int
+    page_size: int
+    bits: int = 4
+    group_size: int = 64
+
+
+@functools.lru_cache(maxsize=64)
+def quant_page_bytes(page_size: int, head_dim: int, bits: int = 4, group_size: int = 64) -> int:
+    """Bytes of a page of one kv head: a token's codes, and four bytes for each group of k and of v."""
+    n = int(L.load().sc_quant_page_bytes(page_size, head_dim, bits, group_size))
+    if not n:
+        raise ValueError(f"pages of {page_size} tokens, head_dim {head_dim}, {bits} bits, groups of {group_size} unsupported "
+                         "(multiples of 16; 64 or 128; 4 or 8; 32 or 64)")
+    return n
+
+
+def quant_pages(n_pages: int, kv_heads: int, page_size: int, head_dim: int, bits: int = 4, group_size: int = 64,
+                device: Optional[torch.device] = None) -> QuantPages:
+    """An empty pool (every token stands for zeros)."""
+    dev = device or torch.device("cuda", torch.cuda.current_device())
+    data = torch.zeros(n_pages, kv_heads, quant_page_bytes(page_size, head_dim, bits, group_size), dtype=torch.uint8, device=dev)
+    return QuantPages(data, head_dim, page_size, bits, group_size)
+
+
+def _quant_pool(what: str, pages: QuantPages):
+    """(n_pages, Hkv) of a pool whose bytes are those of its kind."""
+    n, t = quant_page_bytes(pages.page_size, pages.head_dim, pages.bits, pages.group_size), pages.data
+    if t.dtype is not torch.uint8 or t.dim() != 3 or t.shape[2] != n:
+        raise ValueError(f"{what}: pages must be uint8 [n_pages, Hkv, {n}], got {t.dtype} {tuple(t.shape)}")
+    return t.shape[0], t.shape[1]
+
+
+def paged_rope_append_q(qkv: torch.Tensor, q_start: torch.Tensor, slots: torch.Tensor, positions: torch.Tensor,
+                        cos_tab: torch.Tensor, sin_tab: torch.Tensor, q_out: torch.Tensor, pages: QuantPages) -> torch.Tensor:
+    """``paged_rope_append`` for a cache in 8 or 4 bits: k and v of each row are quantised as they are written to ``slots`` of
+    ``pages``, by groups of ``pages.group_size`` dims (at most half a step of the group's codes off); q goes to ``q_out``
+    [T, Hq hd], float16.  Rows from ``q_start[-1]`` on are left as they were; a slot outside the pool or a position past the
+    tables is not written; the slots of one call differ."""
+    data, hd, page, bits, group = pages
+    st = _native().paged_rope_append_q(qkv, q_start, slots, positions, cos_tab, sin_tab, q_out, data, hd, page, bits, group)
+    if st == 0:
+        return q_out
+    n_pages, Hkv = _quant_pool("paged_rope_append_q", pages)
+    dev = qkv.get_device()
+    _check("paged_rope_append_q", dev, (qkv, cos_tab, sin_tab, q_out, data))
+    _check("paged_rope_append_q", dev, (q_start, slots, positions), _I32)
+    if qkv.dim() != 2 or qkv.dtype not in (_F16, _F32):
+        raise ValueError(f"paged_rope_append_q: qkv must be a float16 or float32 [T, (Hq + 2 Hkv) hd], got {qkv.dtype} {tuple(qkv.shape)}")
+    T, width = qkv.shape
+    Hq = width // hd - 2 * Hkv
+    if width % hd or Hq < 1:
+        raise ValueError(f"paged_rope_append_q: qkv rows of {width} do not hold q beside {Hkv} heads of {hd}")
+    if q_out.dtype != _F16 or q_out.numel() != T * Hq * hd:
+        raise ValueError(f"paged_rope_append_q: q_out must be a float16 [{T}, {Hq * hd}], got {q_out.dtype} {tuple(q_out.shape)}")
+    if slots.numel() < T or positions.numel() < T:
+        raise ValueError(f"paged_rope_append_q: {slots.numel()} slots and {positions.numel()} positions for {T} rows")
+    if cos_tab.dtype != _F32 or sin_tab.dtype != _F32 or cos_tab.dim() != 2 or cos_tab.shape[1] * 2 != hd or cos_tab.shape != sin_tab.shape:
+        raise ValueError(f"paged_rope_append_q: cos_tab and sin_tab must be float32 [max_pos, {hd // 2}]")
+    if q_start.numel() < 1:
+        raise ValueError("paged_rope_append_q: q_start is empty")
+    if T:
+        _call_on(dev, "sc_paged_rope_append_q", qkv.data_ptr(), _dt(qkv), T, q_start.data_ptr() + 4 * (q_start.numel() - 1),
+                 slots.data_ptr(), positions.data_ptr(), cos_tab.data_ptr(), sin_tab.data_ptr(), cos_tab.shape[0], Hq, Hkv, hd,
+                 q_out.data_ptr(), data.data_ptr(), bits, group, n_pages, page)
+    return q_out
+
+
+def paged_read_q(pages: QuantPages, slots: torch.Tensor, q_start: Optional[torch.Tensor] = None, k_out: Optional[torch.Tensor] = None,
+                 v_out: Optional[torch.Tensor] = None, dtype: torch.dtype = _F16):
+    """The tokens that ``slots`` [T] hold, as ``(k, v)`` [T, Hkv, hd] of ``dtype`` (float16 or float32; that of ``k_out`` and
+    ``v_out`` where they are given): what the cache stands for, rounded once.  Zeros for a slot outside the pool.  With
+    ``q_start`` rows from ``q_start[-1]`` on are left as they were."""
+    n_pages, Hkv = _quant_pool("paged_read_q", pages)
+    data, hd, page, bits, group = pages
+    T, dev = slots.numel(), slots.get_device()
+    if (k_out is None) != (v_out is None):
+        raise ValueError("paged_read_q: k_out and v_out go together")
+    if k_out is None:
+        if dtype not in (_F16, _F32):
+            raise ValueError(f"paged_read_q: float16 or float32, got {dtype}")
+        k_out = torch.zeros(T, Hkv, hd, dtype=dtype, device=slots.device)
+        v_out = torch.zeros_like(k_out)
+    st = _native().paged_read_q(slots, data, hd, page, bits, group, q_start, k_out, v_out)
+    if st == 0:
+        return k_out, v_out
+    _check("paged_read_q", dev, (data, k_out, v_out))
+    _check("paged_read_q", dev, (slots,) if q_start is None else (slots, q_start), _I32)
+    if k_out.dtype not in (_F16, _F32) or v_out.dtype != k_out.dtype or k_out.numel() != T * Hkv * hd or v_out.numel() != k_out.numel():
+        raise ValueError(f"paged_read_q: k_out and v_out must both be float16 or float32 [{T}, {Hkv}, {hd}], got {k_out.dtype} "
+                         f"{tuple(k_out.shape)} and {v_out.dtype} {tuple(v_out.shape)}")
+    if q_start is not None and q_start.numel() < 1:
+        raise ValueError("paged_read_q: q_start is empty")
+    if T:
+        _call_on(dev, "sc_paged_read_q", data.data_ptr(), bits, group, n_pages, page, Hkv, hd, slots.data_ptr(), T,
+                 None if q_start is None else q_start.data_ptr() + 4 * (q_start.numel() - 1), k_out.data_ptr(), v_out.data_ptr(), _dt(k_out))
+    return k_out, v_out
+
+
+@functools.lru_cache(maxsize=1024)
+def prefix_attn_q_workspace_bytes(T: int, B: int, Hq: int, Hkv: int, hd: int, max_blocks: int, max_prefix_blocks: int,
+                                  page_size: int) -> int:
+    return int(L.load().sc_prefix_attn_q_workspace_bytes(T, B, Hq, Hkv, hd, max_blocks, max_prefix_blocks, page_size))
+
+
+def prefix_attn_q(q: torch.Tensor, pages: QuantPages, q_start: torch.Tensor, kv_lens: torch.Tensor, block_table: torch.Tensor,
+                  prefix_table: Optional[torch.Tensor] = None, prefix_len: Optional[torch.Tensor] = None,
+                  out: Optional[torch.Tensor] = None, scale: Optional[float] = None,
+                  workspace: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """``prefix_attn`` over pages in 8 or 4 bits: the same rows, tables and lengths; ``q`` and ``out`` [T, Hq hd] are float16.
+    The attention is that of what the cache stands for (``paged_read_q``); weights are rounded to float16 before the
+    second product, everything else is kept in float32.  ``workspace``: uint8, at least ``prefix_attn_q_workspace_bytes``;
+    without it scratch is allocated per call, so calls on two streams do not meet."""
+    if out is None:
+        out = torch.zeros_like(q)
+    data, hd, page, bits, group = pages
+    st = _native().prefix_attn_q(q, data, hd, page, bits, group, q_start, kv_lens, block_table, prefix_table, prefix_len, out, scale, workspace)
+    if st == 0:
+        return out
+    n_pages, Hkv = _quant_pool("prefix_attn_q", pages)
+    dev = q.get_device()
+    _check("prefix_attn_q", dev, (q, data, out))
+    nbp, pt, pl = 0, None, None
+    if prefix_len is not None and prefix_table is not None:
+        _check("prefix_attn_q", dev, (q_start, kv_lens, block_table, prefix_table, prefix_len), _I32)
+        _sized("prefix_attn_q", 1, prefix_len=prefix_len)
+        nbp, pt, pl = prefix_table.numel(), prefix_table.data_ptr(), prefix_len.data_ptr()
+    elif prefix_len is None and prefix_table is None:
+        _check("prefix_attn_q", dev, (q_start, kv_lens, block_table), _I32)
+    else:
+        raise ValueError("prefix_attn_q: prefix_table and prefix_len go together")
+    B, nq = kv_lens.numel(), q.numel()
+    T = q.shape[0] if q.dim() else 0
+    if q.dtype is not _F16 or out.dtype is not _F16 or out.numel() != nq:
+        raise ValueError(f"prefix_attn_q: q and out must be float16 and of one size, got {q.dtype} {tuple(q.shape)} and {out.dtype} "
+                         f"{tuple(out.shape)}")
+    Hq = nq // (T * hd) if T else Hkv
+    if T and Hq * T * hd != nq:
+        raise ValueError(f"prefix_attn_q: q rows of {nq // T} are no multiple of head_dim {hd}")
+    tab = block_table.shape
+    if len(tab) != 2 or tab[0] != B:
+        raise ValueError(f"prefix_attn_q: block_table {tuple(tab)} is not [{B}, max_blocks]")
+    _sized("prefix_attn_q", B + 1, q_start=q_start)
+    if not T or not B:
+        return out
+    nbytes = prefix_attn_q_workspace_bytes(T, B, Hq, Hkv, hd, tab[1], nbp, page)
+    wp, wb = None, 0
+    if workspace is not None:
+        _check("prefix_attn_q", dev, (workspace,))
+        if workspace.dtype != torch.uint8:
+            raise ValueError(f"prefix_attn_q: workspace must be uint8, got {workspace.dtype}")
+        wp, wb = workspace.data_ptr(), workspace.numel()
+    elif nbytes:
+        workspace = torch.empty(nbytes, dtype=torch.uint8, device=dev)
+        wp, wb = workspace.data_ptr(), nbytes
+    _call_on(dev, "sc_prefix_attn_q", q.data_ptr(), data.data_ptr(), bits, group, T, q_start.data_ptr(), kv_lens.data_ptr(),
+             block_table.data_ptr(), B, tab[1], pt, pl, nbp, Hq, Hkv, hd, n_pages, page,
+             1.0 / math.sqrt(hd) if scale is None else float(scale), out.data_ptr(), wp, wb)
+    return out
+
+
 def prefix_attn_device_error(device: Optional[torch.device] = None, reset: bool = True) -> int:
-    """Nonzero after a CTA of ``prefix_attn`` on this device gave up a bounded wait: outputs since the last reset are undefined.
+    """Nonzero after a CTA of ``prefix_attn`` or ``prefix_attn_q`` on this device gave up a bounded wait: outputs since the last reset are undefined.
     Waits for the device's current stream."""
     with torch.cuda.device(device):
         torch.cuda.current_stream().synchronize()
