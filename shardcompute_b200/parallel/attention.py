@@ -21,7 +21,8 @@ return the filled ``[B, Hkv/TP, L, hd]`` views, so code that reads
 With a ``PagedLayer`` as ``past_key_value`` (one layer of a ``PagedKVCache``)
 ``hidden_states`` ``[1, T, H]`` holds the new tokens of a ragged batch in a
 row, as the cache's last ``reserve`` placed them: ``sc_paged_rope_append``
-and ``sc_prefix_attn`` take the place of the two cache kernels.
+and ``sc_prefix_attn`` (``_q`` where it holds 8 or 4 bits) take the place of
+the two cache kernels.
 """
 
 from __future__ import annotations
@@ -227,9 +228,15 @@ class ParallelAttention:
         if B != 1 or T > cache.max_tokens:
             raise ValueError(f"a paged step takes [1, T, H] with T <= {cache.max_tokens}, got {tuple(hidden_states.shape)}")
         cos, sin = self.rope.tables(cache.max_positions, hidden_states.device)
+        qkv = self._qkv(hidden_states.reshape(T, -1)).contiguous()
+        if layer.pages is not None:
+            q = torch.zeros(T, self.local_hidden, dtype=torch.float16, device=hidden_states.device)
+            ops.paged_rope_append_q(qkv, step.q_start, step.slots, step.positions, cos, sin, q, layer.pages)
+            attn = ops.prefix_attn_q(q, layer.pages, step.q_start, step.kv_lens, cache.block_table, cache.prefix_table,
+                                     cache.prefix_len, scale=self.scale)
+            return self.o_proj.forward_partial(attn.view(1, T, self.local_hidden))
         q = torch.zeros(T, self.local_hidden, dtype=layer.k.dtype, device=hidden_states.device)
-        ops.paged_rope_append(self._qkv(hidden_states.reshape(T, -1)).contiguous(), step.q_start, step.slots, step.positions,
-                              cos, sin, q, layer.k, layer.v)
+        ops.paged_rope_append(qkv, step.q_start, step.slots, step.positions, cos, sin, q, layer.k, layer.v)
         attn = ops.prefix_attn(q, layer.k, layer.v, step.q_start, step.kv_lens, cache.block_table, cache.prefix_table,
                                cache.prefix_len, scale=self.scale)
         return self.o_proj.forward_partial(attn.view(1, T, self.local_hidden))

@@ -7,6 +7,10 @@ is: ``reserve`` room for each request's new tokens, run the model on the new tok
 (``input_ids`` ``[1, T]``) with ``past_key_values=cache.layers()``, then ``truncate`` what did not stay (rejected
 drafts, ended requests).  A request can be made the prefix that all others share (``share_prefix``): its keys and values
 are held once and attended to once for the whole batch.
+
+With ``bits`` 8 or 4 the pages hold codes (``ops.QuantPages``): a quarter to a half of float16's room, 72 bytes in place of
+256 for a token's key or value of a head of 128.  Keys and values are quantised as they are written and attended to as they
+lie; ``read`` gives back what the cache stands for.
 """
 
 from __future__ import annotations
@@ -23,19 +27,24 @@ _WHY_BACK = {**_WHY, 1: "no room for the pages given back (a page held twice)"}
 
 
 class PagedLayer(NamedTuple):
-    """One layer of a ``PagedKVCache``: what ``ParallelAttention`` takes as ``past_key_value``."""
+    """One layer of a ``PagedKVCache``: what ``ParallelAttention`` takes as ``past_key_value``.  ``pages`` in place of ``k``
+    and ``v`` where they are held in 8 or 4 bits."""
 
     cache: "PagedKVCache"
-    k: torch.Tensor
-    v: torch.Tensor
+    k: Optional[torch.Tensor]
+    v: Optional[torch.Tensor]
+    pages: Optional["ops.QuantPages"] = None
 
 
 class PagedKVCache:
     def __init__(self, num_layers: int, kv_heads: int, head_dim: int, n_pages: int, max_batch: int, max_len: int,
                  page_size: int = 16, max_prefix: int = 0, max_tokens: Optional[int] = None,
-                 dtype: torch.dtype = torch.float32, device: Optional[torch.device] = None):
+                 dtype: torch.dtype = torch.float32, device: Optional[torch.device] = None, bits: Optional[int] = None,
+                 group_size: int = 64):
         """``max_len`` / ``max_prefix``: tokens of a request and of the shared prefix at most (0: none).
-        ``max_tokens``: new tokens of a step at most (default ``max_batch``, one each).  What the operators do not take is
+        ``max_tokens``: new tokens of a step at most (default ``max_batch``, one each).  ``bits``: 8 or 4, by groups of
+        ``group_size`` (32 or 64) dims, and queries and outputs of the attention are float16; ``dtype`` is that of pages
+        which are not.  What the operators do not take is
         refused here, not after pages were reserved and keys written: heads of 64 or 128, pages of a power of two from 16 to
         32768 tokens, 16384 requests at most, and a pool whose rows (pages x heads x page size) count in 32 bits."""
         if dtype not in (torch.float16, torch.float32):
@@ -58,8 +67,14 @@ class PagedKVCache:
         self.page_size, self.max_batch = page_size, max_batch
         self.max_tokens = max_batch if max_tokens is None else max_tokens
         self.max_positions = blocks * page_size * (2 if max_prefix else 1)
-        self.k = torch.zeros(num_layers, n_pages, kv_heads, page_size, head_dim, dtype=dtype, device=dev)
-        self.v = torch.zeros_like(self.k)
+        self.k = self.v = self.pages = None
+        if bits is None:
+            self.k = torch.zeros(num_layers, n_pages, kv_heads, page_size, head_dim, dtype=dtype, device=dev)
+            self.v = torch.zeros_like(self.k)
+        else:
+            nbytes = ops.quant_page_bytes(page_size, head_dim, bits, group_size)
+            data = torch.zeros(num_layers, n_pages, kv_heads, nbytes, dtype=torch.uint8, device=dev)
+            self.pages = [ops.QuantPages(d, head_dim, page_size, bits, group_size) for d in data]
         self.free_pages = torch.arange(n_pages - 1, -1, -1, **i32)  # page 0 on top
         self.free_count = torch.full((1,), n_pages, **i32)
         self.block_table = torch.full((max_batch, blocks), -1, **i32)
@@ -129,4 +144,19 @@ class PagedKVCache:
 
     def layers(self) -> List[PagedLayer]:
         """``past_key_values`` of ``ParallelTransformer.forward``."""
+        if self.pages is not None:
+            return [PagedLayer(self, None, None, p) for p in self.pages]
         return [PagedLayer(self, k, v) for k, v in zip(self.k, self.v)]
+
+    def read(self, layer: int, request: int, dtype: torch.dtype = torch.float16):
+        """The request's tokens in one layer, as ``(k, v)`` ``[len, Hkv/TP, hd]``: to look at, or to move to another cache.
+        Waits for the device (a request's length lives there).  The shared prefix is not among them."""
+        if not 0 <= request < self.max_batch:
+            raise IndexError(f"request {request} out of range [0, {self.max_batch})")
+        n = int(self.lens[request])
+        at = torch.arange(n, device=self.lens.device)
+        slots = self.block_table[request, at // self.page_size] * self.page_size + at.int() % self.page_size
+        if self.pages is not None:
+            return ops.paged_read_q(self.pages[layer], slots, dtype=dtype)
+        page, off = slots.long() // self.page_size, slots.long() % self.page_size
+        return self.k[layer][page, :, off].to(dtype), self.v[layer][page, :, off].to(dtype)

@@ -151,3 +151,25 @@ def test_oracle_quantises_within_half_a_step(hd, bits, group):
 def test_floor16():
     x = np.array([0.0, 1e-9, -1e-9, 1.0, 1.0004, -1.0004, 65504.0, 70000.0, -70000.0, 2.0**-24, -(2.0**-24)])
     assert oq.floor16(x).tolist() == [0.0, 0.0, -(2.0**-24), 1.0, 1.0, -1.0009765625, 65504.0, 65504.0, -np.inf, 2.0**-24, -(2.0**-24)]
+
+
+# ------------------------------------------------------------------------------------------------ the cache class
+
+def test_cache_in_codes():
+    from shardcompute_b200.parallel import PagedKVCache
+
+    a = dict(num_layers=2, kv_heads=3, head_dim=64, n_pages=4, max_batch=2, max_len=64, device=torch.device("cpu"))
+    for bits, group in [(4, 32), (8, 64)]:
+        c = PagedKVCache(**a, bits=bits, group_size=group)
+        assert c.k is None and c.v is None and [layer.pages.data.shape for layer in c.layers()] == [(4, 3, oq.block_bytes(64, bits, group))] * 2
+        assert all(layer.pages.bits == bits and layer.pages.group_size == group for layer in c.layers())
+        c.check()
+    for kw in (dict(bits=2), dict(bits=16), dict(bits=4, group_size=128), dict(bits=8, group_size=16)):
+        with pytest.raises(ValueError, match="unsupported"):
+            PagedKVCache(**a, **kw)
+    full = PagedKVCache(**a)
+    assert all(layer.pages is None for layer in full.layers())
+    full.block_table[1, 0], full.lens[1] = 2, 3
+    full.k[1, 2, :, :3] = torch.arange(3.0).view(1, 3, 1)
+    k, v = full.read(1, 1, torch.float32)
+    assert k.shape == (3, 3, 64) and k[:, 0, 0].tolist() == [0.0, 1.0, 2.0] and (v == 0).all()
