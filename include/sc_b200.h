@@ -386,8 +386,8 @@ int sc_paged_read_q(const void* pages, int bits, int group, int n_pages, int pag
  * scales are rounded to fp16 before their product with v's codes: 2^-11 of each,
  * down to 2^-25 of the row's largest.  A group that stands for NaN makes the
  * rows that see it NaN (of v: its dims), and no others. */
-size_t sc_prefix_attn_q_workspace_bytes(int T, int B, int Hq, int Hkv, int hd, int max_blocks, int max_prefix_blocks,
-                                        int page_size);
+size_t sc_prefix_attn_q_workspace_bytes(int T, int B, int Hq, int Hkv, int hd, int bits, int group, int max_blocks,
+                                        int max_prefix_blocks, int page_size);
 int sc_prefix_attn_q(const void* q, const void* pages, int bits, int group, int T, const int32_t* q_start,
                      const int32_t* kv_lens, const int32_t* block_table, int B, int max_blocks,
                      const int32_t* prefix_table, const int32_t* prefix_len, int max_prefix_blocks, int Hq, int Hkv,

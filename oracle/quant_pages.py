@@ -147,19 +147,23 @@ def attention(q, data, q_start, kv_lens, table, prefix_table, prefix_len, Hq, hd
     for b in range(len(kv_lens)):
         lo, hi = int(q_start[b]), int(q_start[b + 1])
         L = int(kv_lens[b])
-        for i in range(hi - lo):
-            own = max(0, min(L, L - (hi - lo) + i + 1))
-            p1, o1, _ = where(table[b], own)
-            pid, off = np.concatenate([pp, p1]), np.concatenate([po, o1])
-            if not len(pid):
-                continue
-            for h in range(Hq):
-                x = {name: pool[pid, h // G, off] for name, pool in pools.items()}
-                sc = scale * (x["k"] @ q[lo + i, h])
-                w = np.exp(sc - sc.max())
-                out[lo + i, h] = w @ x["v"] / w.sum()
-                mass[lo + i, h] = w @ x["va"] / w.sum()
-                tail[lo + i, h] = (w * x["s"].max(-1)).max() * x["c"].sum(0) / w.sum()
-                dot[lo + i, h] = scale * (x["ka"] @ np.abs(q[lo + i, h])).max()
-                keys[lo + i, h] = len(sc)
+        p1, o1, there = where(table[b], L)
+        pid, off = np.concatenate([pp, p1]), np.concatenate([po, o1])
+        place_of = np.concatenate([np.full(len(pp), -1), np.flatnonzero(there)])  # a token's place in the request; -1: the prefix
+        for h in range(Hkv if hi > lo else 0):
+            x = {name: pool[pid, h, off] for name, pool in pools.items()}
+            heads = slice(h * G, (h + 1) * G)
+            for i in range(hi - lo):
+                n = int(np.searchsorted(place_of, max(-1, L - (hi - lo) + i), side="right"))  # tokens that the row sees
+                if n == 0:
+                    continue
+                qs = q[lo + i, heads]
+                sc = scale * (qs @ x["k"][:n].T)
+                w = np.exp(sc - sc.max(-1, keepdims=True))
+                total = w.sum(-1, keepdims=True)
+                out[lo + i, heads] = w @ x["v"][:n] / total
+                mass[lo + i, heads] = w @ x["va"][:n] / total
+                tail[lo + i, heads] = (w * x["s"][:n].max(-1)).max(-1, keepdims=True) * x["c"][:n].sum(0) / total
+                dot[lo + i, heads] = scale * (np.abs(qs) @ x["ka"][:n].T).max(-1)
+                keys[lo + i, heads] = n
     return out, mass, dot, keys, tail

@@ -299,7 +299,7 @@ PyObject* prefix_attn_q(PyObject*, PyObject* const* args, Py_ssize_t n) {
       ws = w->data_ptr();
       bytes = (size_t)w->numel();
     } else {
-      bytes = sc_prefix_attn_q_workspace_bytes((int)T, (int)B, (int)Hq, (int)k.Hkv, k.hd, (int)blocks, (int)pblocks, k.page);
+      bytes = sc_prefix_attn_q_workspace_bytes((int)T, (int)B, (int)Hq, (int)k.Hkv, k.hd, k.bits, k.group, (int)blocks, (int)pblocks, k.page);
       if (bytes) {
         scratch = at::empty({(int64_t)bytes}, q->options().dtype(at::kByte));
         ws = scratch.data_ptr();

@@ -60,20 +60,6 @@ __device__ __forceinline__ void block_scan2(long long& a, long long& b, long lon
   __syncthreads();
 }
 
-// x / d for 0 <= x < 2^31 by a product: m = floor(2^(31 + l) / d) + 1 with l = ceil(log2 d) is off by less than
-// 2^-(31 + l) relative to 1 / d, too little to reach the next whole number.
-struct PageDiv {
-  unsigned long long m;
-  int d, sh;
-  __device__ __forceinline__ int div(int x) const { return (int)(((unsigned long long)(unsigned)x * m) >> sh); }
-  __device__ __forceinline__ int up(int x) const { return x > 0 ? div(x - 1) + 1 : 0; }
-};
-static PageDiv page_div(int d) {
-  int l = 0;
-  while ((1ll << l) < d) ++l;
-  return {(1ull << (31 + l)) / (unsigned)d + 1, d, 31 + l};
-}
-
 // First index i in [0, n) with a[i] > x (a is non-decreasing, a[n - 1] > x).
 __device__ __forceinline__ int first_above(const int* a, int n, int x) {
   int lo = 0, hi = n - 1;

@@ -3,8 +3,7 @@
 // dims (sc_quant.cuh), and the codes c go into the products as they are:
 //   q.k = sum_g s_g (q_g.c_g) + b_g (sum of q over g)
 //   o_g = sum_j (p_j s_jg) c_jg + sum_j p_j b_jg
-#include "sc_prefix_attn.cuh"
-#include "sc_quant.cuh"
+#include "sc_many_rows.cuh"
 
 namespace sc {
 
@@ -33,16 +32,50 @@ struct FewRowsQuant {
   static constexpr int WORDS = QB::KSH / 4;    // of codes in a thread's share of a token
   static constexpr int PER = 32 / QB::BITS;    // codes of a word
   static constexpr int KSTEPS = QB::HD / 16, MT = QB::HD / 16;
-  static constexpr int NST = QB::BYTES > 3000 ? 4 : QB::BYTES > 1600 ? 5 : 8;
+  static constexpr int STAGE = 2 * QB::BYTES;  // two blocks: 32 tokens
+  static constexpr int NST = STAGE > 4000 ? 2 : STAGE > 2400 ? 3 : 4;
   static constexpr int OUT = 2 * RT * QB::HD * 4;  // a warp's result, and the CTA's behind it
-  static constexpr int RING = NST * QB::BYTES > OUT ? NST * QB::BYTES : OUT;
-  static constexpr int SMEM = FR_WARPS * RING + 128;
-  static constexpr int CTAS = NT == 1 ? 4 : 3;  // of an SM
+  static constexpr int RING = NST * STAGE > OUT ? NST * STAGE : OUT;
+  static constexpr int QBYTES = NT * KSTEPS * 256;  // q's fragments
+  static constexpr int SMEM = FR_WARPS * RING + QBYTES;
+  // CTAs of an SM, by shared memory and by the registers that they need without spills
+  static constexpr int CTAS = NT == 1 ? (SMEM > 56000 ? 3 : SMEM > 44000 || QB::NG == 4 ? 4 : 5) : QB::NG == 4 || SMEM > 75000 ? 2 : 3;
+  static constexpr int CTAS_CLUSTER = NT == 1 ? (CTAS < 4 ? CTAS : 4) : 2;
 };
+
+// Work of the CTAs where a grid of requests would leave them uneven: the (request, kv head, tile of rows) follow one another on
+// a line, each as long as its tiles of keys and FQ_UNIT more, and each CTA takes a piece of `quantum`.  What a piece holds of
+// a unit that reaches past it goes to one of the CTA's two places for partial results (first unit, last unit).
+struct StreamArgs {
+  long long* offsets;  // [B + 1]: where each request's units begin, and the quantum behind them: written by CTA 0, for the join
+  float* o;            // [2 CTAs, RT, HD]
+  float2* ml;          // [2 CTAs, RT]
+};
+constexpr int FQ_KEYS = 32;         // of a tile
+constexpr int FQ_UNIT = 4;          // tiles that a unit's start and end are worth
+constexpr int FQ_LEAST = 8;         // tiles of a piece, at least
+
+// A request's tiles of keys (all that some row of it sees, at most), its tiles of rows.
+struct StreamRequest {
+  int row_lo, rows, n, len, nt, tiles;
+  long long units;
+};
+template <int RT>
+__device__ __forceinline__ StreamRequest stream_request(const PrefixAttnParams& p, int b, int np) {
+  StreamRequest r;
+  int hi;
+  request_rows(p, b, r.row_lo, hi, r.n);
+  r.rows = (hi - r.row_lo) * p.G;
+  r.len = request_len(p, b);
+  r.nt = np + (int)(((long long)r.len + FQ_KEYS - 1) / FQ_KEYS);
+  r.tiles = (r.rows + RT - 1) / RT;
+  r.units = (long long)r.tiles * p.Hkv * (r.nt + FQ_UNIT);
+  return r;
+}
 
 __device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
   uint32_t y;
-  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+  asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
   return y;
 }
 __device__ __forceinline__ float min_keep_nan(float a, float b) {
@@ -80,19 +113,22 @@ __device__ __forceinline__ void lds_share(uint32_t at, uint32_t other, uint32_t 
 }
 
 template <typename QB, int NT, bool CLUSTER>
-__global__ void __launch_bounds__(FR_WARPS * 32, FewRowsQuant<QB, NT>::CTAS)
-few_rows_quant_kernel(const PrefixAttnParams p, const uint8_t* pages, int with_prefix, int splits, int row_groups, int slot0) {
+__global__ void __launch_bounds__(FR_WARPS * 32, CLUSTER ? FewRowsQuant<QB, NT>::CTAS_CLUSTER : FewRowsQuant<QB, NT>::CTAS)
+few_rows_quant_kernel(const PrefixAttnParams p, const uint8_t* pages, int with_prefix, int splits, int row_groups, int slot0,
+                      const StreamArgs stream) {
   using C = FewRowsQuant<QB, NT>;
-  constexpr int RT = C::RT, NST = C::NST, KT = 16, HD = QB::HD, NG = QB::NG, GS = QB::GS, WORDS = C::WORDS, PER = C::PER;
+  constexpr int RT = C::RT, NST = C::NST, KT = FQ_KEYS, HD = QB::HD, NG = QB::NG, GS = QB::GS, WORDS = C::WORDS, PER = C::PER;
   extern __shared__ __align__(128) unsigned char fq_smem[];
   __shared__ __align__(8) uint64_t full[FR_WARPS][NST];
   __shared__ float s_m[FR_WARPS][RT], s_l[FR_WARPS][RT];
+  __shared__ float s_cq[RT], s_qsum[NG][RT];
   __shared__ float2 s_ml[CLUSTER ? RT : 1];
-  __shared__ int s_abort;
-  unsigned char* base = fq_smem;
+  __shared__ long long s_sum[FR_WARPS], s_at;
+  __shared__ int s_abort, s_b;
+  unsigned char* base = fq_smem + C::QBYTES;
+  const uint32_t q_u = smem_u32(fq_smem);
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   const int q4 = lane & 3, r8 = lane >> 2;
-  const int split = blockIdx.x % splits, group = blockIdx.x / splits, h = blockIdx.y, b = blockIdx.z;
   if (threadIdx.x == 0) {
     for (int w = 0; w < FR_WARPS; ++w)
       for (int s = 0; s < NST; ++s) mbar_init(&full[w][s], 1);
@@ -103,131 +139,101 @@ few_rows_quant_kernel(const PrefixAttnParams p, const uint8_t* pages, int with_p
   pdl_trigger();
   // Without the prefix this kernel runs beside the prefix's, as few_rows_kernel does (sc_prefix_attn.cu).
   if (with_prefix) pdl_wait();
-  const int P = with_prefix ? prefix_keys(p) : 0, np = (P + KT - 1) / KT;
-  const int t0 = split * FR_WARPS + warp, step = splits * FR_WARPS;
-  // the pool's blocks of this warp's tiles first .. first + 31, one per lane; -1: no such page
-  auto blocks_of = [&](int first) {
-    const long long t = t0 + (long long)step * (first + lane);
+  const int P = with_prefix ? prefix_keys(p) : 0, np = (int)(((long long)P + KT - 1) / KT);
+  unsigned char* ring = base + (size_t)warp * C::RING;
+  const uint32_t ring_u = smem_u32(ring);
+  int s_in = 0, s_out = 0;            // the stage that the next tile goes to, that it comes from
+  uint32_t phase = 0, in_flight = 0;  // of s_out's barrier; tiles asked for and not yet waited for
+
+  // The pool's blocks of tiles t0 + step (first .. first + 15) of request b and head h, two lanes a tile; -1: no such page.
+  auto blocks_of = [&](int b, int h, int t0, int step, int first) {
+    const long long t = t0 + (long long)step * (first + (lane >> 1));
     const bool pre = t < np;
-    const long long key = (pre ? t : t - np) * KT;
+    const long long key = (pre ? t : t - np) * KT + (lane & 1) * 16;
     const int blk = (int)min(key >> p.lg_page, (long long)INT32_MAX);
     if (blk >= (pre ? p.max_prefix_blocks : p.max_blocks)) return -1;
     const int id = pre ? p.prefix_table[blk] : p.block_table[(size_t)b * p.max_blocks + blk];
     if (id < 0 || id >= p.n_pages) return -1;
-    return ((id * p.Hkv + h) << (p.lg_page - 4)) + (((int)key & ((1 << p.lg_page) - 1)) >> 4);
+    return ((id * p.Hkv + h) << (p.lg_page - 4)) + (int)((key & ((1 << p.lg_page) - 1)) >> 4);
   };
-  const int blocks0 = blocks_of(0);
-  int row_lo, row_hi, n;
-  request_rows(p, b, row_lo, row_hi, n);
-  const int rows_b = (row_hi - row_lo) * p.G, len = request_len(p, b);
-  unsigned char* ring = base + (size_t)warp * C::RING;
-  const uint32_t ring_u = smem_u32(ring);
-  uint32_t issued = 0, used = 0;  // tiles of this warp's ring, over all row tiles
 
-  for (int r0 = group * RT; r0 < rows_b; r0 += row_groups * RT) {
-    const int nr = min(RT, rows_b - r0);
-    // own keys that the tile's last row sees
-    const int own = max(0, min(len, len - n + (r0 + nr - 1) / p.G + 1));
-    const int nt = np + (own + KT - 1) / KT;
-    const int cnt = max(0, (nt - t0 + step - 1) / step);
-
-    int blocks = blocks0;
-    uint32_t absent = 0;  // stages whose tile has no page
+  // Rows r0 .. r0 + nr of request b under this warp's tiles t0 + step i, i < cnt; `own`: own keys that the last of the rows sees.
+  // The warps' results go to their rings, (m, l) to s_m and s_l.  False after a wait that ran out.
+  auto attend = [&](int b, int h, int row_lo, int n, int len, int r0, int nr, int own, int t0, int step, int cnt, int blocks) {
+    uint32_t absent = 0;  // blocks without a page, two bits per stage
     auto issue = [&](int i) {
-      if (i && (i & 31) == 0) blocks = blocks_of(i);
-      const int blk = __shfl_sync(0xffffffffu, blocks, i & 31);
-      const int s = issued % NST;
-      absent = (absent & ~(1u << s)) | ((blk < 0 ? 1u : 0u) << s);
+      if (i && (i & 15) == 0) blocks = blocks_of(b, h, t0, step, i);
+      const int blk = __shfl_sync(0xffffffffu, blocks, 2 * (i & 15) + (lane & 1));
+      const uint32_t there = __ballot_sync(0xffffffffu, blk >= 0) & 3u;
+      absent = (absent & ~(3u << (2 * s_in))) | ((there ^ 3u) << (2 * s_in));
       if (lane == 0) {
-        if (blk < 0) {
-          mbar_arrive(&full[warp][s]);
-        } else {
-          mbar_arrive_expect_tx(&full[warp][s], QB::BYTES);
-          bulk_load(ring + s * QB::BYTES, pages + (size_t)blk * QB::BYTES, QB::BYTES, &full[warp][s]);
-        }
+        if (there)
+          mbar_arrive_expect_tx(&full[warp][s_in], (there == 3u ? 2 : 1) * QB::BYTES);
+        else
+          mbar_arrive(&full[warp][s_in]);
       }
       __syncwarp();
-      ++issued;
+      if (lane < 2 && blk >= 0)
+        bulk_load(ring + s_in * C::STAGE + lane * QB::BYTES, pages + (size_t)blk * QB::BYTES, QB::BYTES, &full[warp][s_in]);
+      s_in = s_in + 1 == NST ? 0 : s_in + 1;
+      ++in_flight;
     };
     for (int i = 0; i < min(NST, cnt); ++i) issue(i);
 
-    // ---- q fragments: this lane's column of a tile of 8 rows, its dims those of its share of K
-    uint32_t qb[NT][C::KSTEPS][2];
-    float qsum[NT][NG][2], cq[NT][2];  // of the columns 2 q4 and 2 q4 + 1
+    // ---- q's fragments, by all warps: eight dims of a row a lane, those of a word (8 bits: two) of a thread's share of K
 #pragma unroll
-    for (int j = 0; j < NT; ++j) {
-      const int r = j * 8 + r8;
-      const __half* src = nullptr;
-      if (r < nr) src = reinterpret_cast<const __half*>(p.q) + ((size_t)(row_lo + (r0 + r) / p.G) * p.Hq + h * p.G + (r0 + r) % p.G) * HD;
-      float x[WORDS][PER], big = 0.f, sum[NG];
+    for (int r1 = 0; r1 < RT; r1 += FR_WARPS * 256 / HD) {
+      constexpr int LPR = HD / 8, SH = GS / 4;
+      const int r = r1 + (int)threadIdx.x / LPR, c = threadIdx.x % LPR, t = c & 3, w = c >> 2;
+      const int d = w * 8 / SH * GS + t * SH + w * 8 % SH;
+      uint4 u = make_uint4(0u, 0u, 0u, 0u);
+      if (r < nr) {
+        const int tok = (r0 + r) / p.G;
+        u = *reinterpret_cast<const uint4*>(reinterpret_cast<const __half*>(p.q) + ((size_t)(row_lo + tok) * p.Hq + h * p.G + (r0 + r - tok * p.G)) * HD + d);
+      }
+      float x[8];
+      const uint32_t uu[4] = {u.x, u.y, u.z, u.w};
+      float big = 0.f, sum = 0.f;
 #pragma unroll
-      for (int g = 0; g < NG; ++g) sum[g] = 0.f;
-#pragma unroll
-      for (int w = 0; w < WORDS; ++w) {
-        constexpr int SH = GS / 4;
-        const int d = w * PER / SH * GS + q4 * SH + w * PER % SH;
-        uint32_t u[PER / 2];
-#pragma unroll
-        for (int k = 0; k < PER / 2; ++k) u[k] = 0u;
-        if (src) {
-          if constexpr (PER == 8) {
-            const uint4 v = *reinterpret_cast<const uint4*>(src + d);
-            u[0] = v.x; u[1] = v.y; u[2] = v.z; u[3] = v.w;
-          } else {
-            const uint2 v = *reinterpret_cast<const uint2*>(src + d);
-            u[0] = v.x; u[1] = v.y;
-          }
-        }
-#pragma unroll
-        for (int k = 0; k < PER / 2; ++k) {
-          const float2 f = __half22float2(u32_as_h2(u[k]));
-          x[w][2 * k] = f.x;
-          x[w][2 * k + 1] = f.y;
-          big = fmaxf(big, fmaxf(fabsf(f.x), fabsf(f.y)));
-          sum[w * PER / SH] += f.x + f.y;
-        }
+      for (int k = 0; k < 4; ++k) {
+        const float2 f = __half22float2(u32_as_h2(uu[k]));
+        x[2 * k] = f.x;
+        x[2 * k + 1] = f.y;
+        big = fmaxf(big, fmaxf(fabsf(f.x), fabsf(f.y)));
+        sum += f.x + f.y;
       }
 #pragma unroll
-      for (int d = 1; d <= 2; d <<= 1) {
-        big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, d));
+      for (int z = 1; z < LPR; z <<= 1) big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, z));
 #pragma unroll
-        for (int g = 0; g < NG; ++g) sum[g] += __shfl_xor_sync(0xffffffffu, sum[g], d);
-      }
+      for (int z = 1; z < SH / 2; z <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, z);  // four shares, SH / 8 words of each
       // 2^k: the row's largest value to [2^11, 2^12) (an infinity, or no value at all: 1)
       const int e = (int)(__float_as_uint(big) >> 23) - 127, k = big > 0.f && e < 128 ? 11 - e : 0;
-      const float up = __uint_as_float((uint32_t)(127 + k) << 23), down = __uint_as_float((uint32_t)(127 + 24 - k) << 23);
-#pragma unroll
-      for (int w = 0; w < WORDS; ++w) {
-        auto pair = [&](int a, int c, float f) { return h2_as_u32(__floats2half2_rn(x[w][a] * f, x[w][c] * f)); };
-        if constexpr (PER == 8) {
-          qb[j][2 * w][0] = pair(0, 4, up);
-          qb[j][2 * w][1] = pair(2, 6, up);
-          qb[j][2 * w + 1][0] = pair(1, 5, up * 0.0625f);
-          qb[j][2 * w + 1][1] = pair(3, 7, up * 0.0625f);
-        } else {
-          qb[j][w][0] = pair(0, 2, up);
-          qb[j][w][1] = pair(1, 3, up);
-        }
-      }
-#pragma unroll
-      for (int c = 0; c < 2; ++c) {
-        const int from = (2 * q4 + c) * 4;
-        const float back = __shfl_sync(0xffffffffu, down, from);  // 2^(24 - k)
-        cq[j][c] = p.c * back;
-#pragma unroll
-        for (int g = 0; g < NG; ++g) qsum[j][g][c] = __shfl_sync(0xffffffffu, sum[g], from) / back;
-      }
+      const float up = __uint_as_float((uint32_t)(127 + k) << 23), back = __uint_as_float((uint32_t)(127 + 24 - k) << 23);  // 2^(24 - k)
+      auto pair = [&](int a, int b2, float f) { return h2_as_u32(__floats2half2_rn(x[a] * f, x[b2] * f)); };
+      // the fragment of two steps of k, 16 bytes a lane
+      const uint32_t to = q_u + (((r >> 3) * (C::KSTEPS / 2) + w) * 32 + (r & 7) * 4 + t) * 16;
+      if (r >= RT) continue;  // heads of 64 and eight rows: half of the threads
+      if constexpr (PER == 8)
+        asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(to), "r"(pair(0, 4, up)), "r"(pair(2, 6, up)),
+                     "r"(pair(1, 5, up * 0.0625f)), "r"(pair(3, 7, up * 0.0625f)) : "memory");
+      else
+        asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(to), "r"(pair(0, 2, up)), "r"(pair(1, 3, up)), "r"(pair(4, 6, up)),
+                     "r"(pair(5, 7, up)) : "memory");
+      if (c == 0) s_cq[r] = p.c * back;
+      if (w * 8 % SH == 0 && t == 0) s_qsum[w * 8 / SH][r] = sum / back;
     }
-    // own keys that the first row sees, and each of this thread's columns (rows past the last: as the last)
-    const int see_first = max(0, min(len, len - n + r0 / p.G + 1));
-    int see[NT][2];
+    __syncthreads();
+    float qsum[NT][NG][2], cq[NT][2];  // of the columns 2 q4 and 2 q4 + 1
 #pragma unroll
     for (int j = 0; j < NT; ++j)
 #pragma unroll
       for (int c = 0; c < 2; ++c) {
-        const int r = j * 8 + 2 * q4 + c;
-        see[j][c] = r < nr ? max(0, len - n + (r0 + r) / p.G + 1) : own;
+        cq[j][c] = s_cq[j * 8 + 2 * q4 + c];
+#pragma unroll
+        for (int g = 0; g < NG; ++g) qsum[j][g][c] = s_qsum[g][j * 8 + 2 * q4 + c];
       }
+    // own keys that the first row sees
+    const int see_first = max(0, min(len, len - n + r0 / p.G + 1));
 
     float o[C::MT][NT][4], bias[NT][NG][2], m[NT][2], l[NT][2];
 #pragma unroll
@@ -246,91 +252,104 @@ few_rows_quant_kernel(const PrefixAttnParams p, const uint8_t* pages, int with_p
     const uint32_t v_lane = QB::V + q4 * 2 * QB::ROW + QB::piece_v(q4, r8, 0);
     const uint32_t meta_lane = r8 * 4 * NG;
 
-    for (int i = 0; i < cnt; ++i, ++used) {
-      const int s = used % NST;
-      if (!mbar_wait_warp(&full[warp][s], (used / NST) & 1u, &s_abort, PA_WAIT_NS)) break;
-      const int t = t0 + step * i;
-      if ((absent >> s) & 1u) {  // nothing to see
-        __syncwarp();
-        if (i + NST < cnt) issue(i + NST);
-        continue;
+    for (int i = 0; i < cnt; ++i) {
+      if (!mbar_wait_warp(&full[warp][s_out], phase, &s_abort, PA_WAIT_NS)) return false;
+      const uint32_t tile = ring_u + s_out * C::STAGE;
+      const uint32_t gone = (absent >> (2 * s_out)) & 3u;
+      --in_flight;
+      if (++s_out == NST) {
+        s_out = 0;
+        phase ^= 1u;
       }
-      const uint32_t tile = ring_u + s * QB::BYTES;
+      const int t = t0 + step * i;
       const int first = (t < np ? t : t - np) * KT;
-      const bool part = (t < np ? P : see_first) - first < KT;  // not every row sees every key
-      // ---- S = K Q^T
-      float sc[NT][4];
+      const bool part = gone || (t < np ? P : see_first) - first < KT;  // not every row sees every key
+      // ---- S = K Q^T: tokens r8, r8 + 8, r8 + 16, r8 + 24 of the tile by columns 2 q4, 2 q4 + 1
+      float sc[NT][8];
 #pragma unroll
-      for (int j = 0; j < NT; ++j) sc[j][0] = sc[j][1] = sc[j][2] = sc[j][3] = 0.f;
+      for (int j = 0; j < NT; ++j)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) sc[j][e] = 0.f;
       {
-        uint32_t ka[WORDS], kb[WORDS], ma[NG], mb[NG];  // tokens r8 and r8 + 8
-        lds_share<WORDS>(tile + k_lane, tile + (k_lane ^ 64), ka);
-        lds_share<WORDS>(tile + k_lane + 8 * QB::ROW, tile + (k_lane ^ 64) + 8 * QB::ROW, kb);
-        lds_words<NG>(tile + QB::KM + meta_lane, ma);
-        lds_words<NG>(tile + QB::KM + meta_lane + 32 * NG, mb);
+        uint32_t ka[2][WORDS], kb[2][WORDS];
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+          const uint32_t block = tile + k * QB::BYTES;
+          lds_share<WORDS>(block + k_lane, block + (k_lane ^ 64), ka[k]);
+          lds_share<WORDS>(block + k_lane + 8 * QB::ROW, block + (k_lane ^ 64) + 8 * QB::ROW, kb[k]);
+        }
 #pragma unroll
         for (int g = 0; g < NG; ++g) {
-          float y[NT][4];
+          float y[NT][8];
 #pragma unroll
-          for (int j = 0; j < NT; ++j) y[j][0] = y[j][1] = y[j][2] = y[j][3] = 0.f;
+          for (int j = 0; j < NT; ++j)
 #pragma unroll
-          for (int w = g * WORDS / NG; w < (g + 1) * WORDS / NG; ++w) {
-            const uint32_t a = ka[w], c = kb[w];
+            for (int e = 0; e < 8; ++e) y[j][e] = 0.f;
+#pragma unroll
+          for (int w = g * C::KSTEPS / 2 / NG; w < (g + 1) * C::KSTEPS / 2 / NG; ++w)  // two steps of k
 #pragma unroll
             for (int j = 0; j < NT; ++j) {
-              if constexpr (PER == 8) {
-                mma_16816(y[j], a & 0x000f000fu, c & 0x000f000fu, (a >> 8) & 0x000f000fu, (c >> 8) & 0x000f000fu, qb[j][2 * w][0], qb[j][2 * w][1]);
-                mma_16816(y[j], a & 0x00f000f0u, c & 0x00f000f0u, (a >> 8) & 0x00f000f0u, (c >> 8) & 0x00f000f0u, qb[j][2 * w + 1][0],
-                          qb[j][2 * w + 1][1]);
-              } else {
-                mma_16816(y[j], a & 0x00ff00ffu, c & 0x00ff00ffu, (a >> 8) & 0x00ff00ffu, (c >> 8) & 0x00ff00ffu, qb[j][w][0], qb[j][w][1]);
+              const uint4 q = lds_v4(q_u + ((j * (C::KSTEPS / 2) + w) * 32 + lane) * 16);
+#pragma unroll
+              for (int k = 0; k < 2; ++k) {
+                float(&z)[4] = *reinterpret_cast<float(*)[4]>(&y[j][4 * k]);
+                if constexpr (PER == 8) {
+                  const uint32_t a = ka[k][w], c = kb[k][w];
+                  mma_16816(z, a & 0x000f000fu, c & 0x000f000fu, (a >> 8) & 0x000f000fu, (c >> 8) & 0x000f000fu, q.x, q.y);
+                  mma_16816(z, a & 0x00f000f0u, c & 0x00f000f0u, (a >> 8) & 0x00f000f0u, (c >> 8) & 0x00f000f0u, q.z, q.w);
+                } else {
+#pragma unroll
+                  for (int i = 0; i < 2; ++i) {
+                    const uint32_t a = ka[k][2 * w + i], c = kb[k][2 * w + i];
+                    mma_16816(z, a & 0x00ff00ffu, c & 0x00ff00ffu, (a >> 8) & 0x00ff00ffu, (c >> 8) & 0x00ff00ffu, i ? q.z : q.x, i ? q.w : q.y);
+                  }
+                }
               }
             }
-          }
-          const float2 x0 = __half22float2(u32_as_h2(ma[g])), x1 = __half22float2(u32_as_h2(mb[g]));
 #pragma unroll
-          for (int j = 0; j < NT; ++j) {
-            sc[j][0] = fmaf(x0.x, y[j][0], fmaf(x0.y, qsum[j][g][0], sc[j][0]));
-            sc[j][1] = fmaf(x0.x, y[j][1], fmaf(x0.y, qsum[j][g][1], sc[j][1]));
-            sc[j][2] = fmaf(x1.x, y[j][2], fmaf(x1.y, qsum[j][g][0], sc[j][2]));
-            sc[j][3] = fmaf(x1.x, y[j][3], fmaf(x1.y, qsum[j][g][1], sc[j][3]));
+          for (int k = 0; k < 2; ++k) {
+            const float2 x0 = __half22float2(u32_as_h2(lds_u32(tile + k * QB::BYTES + QB::KM + meta_lane + 4 * g)));
+            const float2 x1 = __half22float2(u32_as_h2(lds_u32(tile + k * QB::BYTES + QB::KM + meta_lane + 32 * NG + 4 * g)));
+#pragma unroll
+            for (int j = 0; j < NT; ++j)
+#pragma unroll
+              for (int c = 0; c < 2; ++c) {
+                sc[j][4 * k + c] = fmaf(x0.x, y[j][4 * k + c], fmaf(x0.y, qsum[j][g][c], sc[j][4 * k + c]));
+                sc[j][4 * k + 2 + c] = fmaf(x1.x, y[j][4 * k + 2 + c], fmaf(x1.y, qsum[j][g][c], sc[j][4 * k + 2 + c]));
+              }
           }
         }
       }
 #pragma unroll
       for (int j = 0; j < NT; ++j)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) sc[j][e] *= cq[j][e & 1];
-      uint32_t hidden = 0;  // bit 4 j + e
+        for (int e = 0; e < 8; ++e) sc[j][e] *= cq[j][e & 1];
+      uint32_t hidden = 0;  // bit 8 j + e
       if (part) {
 #pragma unroll
         for (int j = 0; j < NT; ++j)
 #pragma unroll
-          for (int e = 0; e < 4; ++e)
-            if (r8 + (e >> 1) * 8 >= (t < np ? P : see[j][e & 1]) - first) {
-              hidden |= 1u << (4 * j + e);
-              sc[j][e] = -INFINITY;
-            }
-      }
-      // ---- V's scales and biases; log2 of a bound of the largest scale
-      float2 v0[NG], v1[NG];
-      float lg[2], cap[2];
-      {
-        uint32_t ma[NG], mb[NG];
-        lds_words<NG>(tile + QB::VM + meta_lane, ma);
-        lds_words<NG>(tile + QB::VM + meta_lane + 32 * NG, mb);
-        float big0 = 0x1p-24f, big1 = 0x1p-24f;
+          for (int c = 0; c < 2; ++c) {
+            const int r = j * 8 + 2 * q4 + c;  // rows past the last see what the last does
+            const int lim = (t < np ? P : r < nr ? max(0, min(len, len - n + (r0 + r) / p.G + 1)) : own) - first;
 #pragma unroll
-        for (int g = 0; g < NG; ++g) {
-          v0[g] = __half22float2(u32_as_h2(ma[g]));
-          v1[g] = __half22float2(u32_as_h2(mb[g]));
-          big0 = fmaxf(big0, v0[g].x);
-          big1 = fmaxf(big1, v1[g].x);
-        }
-        lg[0] = (float)((int)(__float_as_uint(big0) >> 23) - 126);
-        lg[1] = (float)((int)(__float_as_uint(big1) >> 23) - 126);
-        cap[0] = PA_LIFT + PA_RAISE - lg[0];
-        cap[1] = PA_LIFT + PA_RAISE - lg[1];
+            for (int e = c; e < 8; e += 2)
+              if (r8 + (e >> 1) * 8 >= lim || (gone >> (e >> 2)) & 1u) {
+                hidden |= 1u << (8 * j + e);
+                sc[j][e] = -INFINITY;
+              }
+          }
+      }
+      // ---- V's scales and biases; log2 of a bound of each token's largest scale
+      uint32_t mv[4][NG];
+      float lg[4];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        lds_words<NG>(tile + (k >> 1) * QB::BYTES + QB::VM + meta_lane + (k & 1) * 32 * NG, mv[k]);
+        float big = 0x1p-24f;
+#pragma unroll
+        for (int g = 0; g < NG; ++g) big = fmaxf(big, __low2float(u32_as_h2(mv[k][g])));
+        lg[k] = (float)((int)(__float_as_uint(big) >> 23) - 126);
       }
       // ---- running softmax: a column's m, the same in its eight lanes, is raised (and o rescaled) only when some p s may pass
       // 2^(PA_LIFT + PA_RAISE)
@@ -340,7 +359,7 @@ few_rows_quant_kernel(const PrefixAttnParams p, const uint8_t* pages, int with_p
       for (int j = 0; j < NT; ++j)
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
-          x[j][c] = fmaxf(sc[j][c] + lg[0], sc[j][2 + c] + lg[1]) - PA_LIFT;
+          x[j][c] = fmaxf(fmaxf(sc[j][c] + lg[0], sc[j][2 + c] + lg[1]), fmaxf(sc[j][4 + c] + lg[2], sc[j][6 + c] + lg[3])) - PA_LIFT;
           up |= x[j][c] > m[j][c] + PA_RAISE;
         }
       if (__any_sync(0xffffffffu, up)) {
@@ -367,46 +386,53 @@ few_rows_quant_kernel(const PrefixAttnParams p, const uint8_t* pages, int with_p
 #pragma unroll
       for (int j = 0; j < NT; ++j)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
+        for (int e = 0; e < 8; ++e) {
           const float mm = m[j][e & 1] == -INFINITY ? 0.f : m[j][e & 1];
-          sc[j][e] = ex2(min_keep_nan(sc[j][e] - mm, cap[e >> 1]));
+          sc[j][e] = ex2(min_keep_nan(sc[j][e] - mm, PA_LIFT + PA_RAISE - lg[e >> 1]));
           l[j][e & 1] += sc[j][e];
         }
       // ---- O += V^T (P s)^T, and the biases' part
-      uint32_t va[WORDS], vb[WORDS];  // pairs of tokens q4 and q4 + 4
-      lds_share<WORDS>(tile + v_lane, tile + v_lane + 128, va);
-      lds_share<WORDS>(tile + v_lane + 8 * QB::ROW, tile + v_lane + 8 * QB::ROW + 128, vb);
 #pragma unroll
-      for (int g = 0; g < NG; ++g) {
-        uint32_t pb[NT][2];
+      for (int k = 0; k < 2; ++k) {
+        const uint32_t block = tile + k * QB::BYTES + v_lane;
+        uint32_t va[WORDS], vb[WORDS];  // pairs of tokens q4 and q4 + 4
+        lds_share<WORDS>(block, block + 128, va);
+        lds_share<WORDS>(block + 8 * QB::ROW, block + 8 * QB::ROW + 128, vb);
 #pragma unroll
-        for (int j = 0; j < NT; ++j) {
-          float ps[4], pz[4];
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            ps[e] = sc[j][e] * (e < 2 ? v0[g].x : v1[g].x);
-            pz[e] = sc[j][e] * (e < 2 ? v0[g].y : v1[g].y);
-          }
-          if (part) {  // what is hidden may be an infinity or NaN
-#pragma unroll
-            for (int e = 0; e < 4; ++e)
-              if (hidden >> (4 * j + e) & 1u) ps[e] = pz[e] = 0.f;
-          }
-          bias[j][g][0] += pz[0] + pz[2];
-          bias[j][g][1] += pz[1] + pz[3];
-          pb[j][0] = transpose8x8(h2_as_u32(__floats2half2_rn(ps[0], ps[1])));
-          pb[j][1] = transpose8x8(h2_as_u32(__floats2half2_rn(ps[2], ps[3])));
-        }
-#pragma unroll
-        for (int w = g * WORDS / NG; w < (g + 1) * WORDS / NG; ++w) {
-          const uint32_t a = va[w], c = vb[w];
+        for (int g = 0; g < NG; ++g) {
+          const float2 v0 = __half22float2(u32_as_h2(mv[2 * k][g])), v1 = __half22float2(u32_as_h2(mv[2 * k + 1][g]));
+          uint32_t pb[NT][2];
 #pragma unroll
           for (int j = 0; j < NT; ++j) {
-            if constexpr (PER == 8) {
-              mma_16816(o[2 * w][j], a & 0x000f000fu, (a >> 8) & 0x000f000fu, c & 0x000f000fu, (c >> 8) & 0x000f000fu, pb[j][0], pb[j][1]);
-              mma_16816(o[2 * w + 1][j], a & 0x00f000f0u, (a >> 8) & 0x00f000f0u, c & 0x00f000f0u, (c >> 8) & 0x00f000f0u, pb[j][0], pb[j][1]);
+            float ps[4];
+            if (part) {  // what is hidden may be an infinity or NaN
+#pragma unroll
+              for (int e = 0; e < 4; ++e) {
+                const bool out = hidden >> (8 * j + 4 * k + e) & 1u;
+                ps[e] = out ? 0.f : sc[j][4 * k + e] * (e < 2 ? v0.x : v1.x);
+                bias[j][g][e & 1] += out ? 0.f : sc[j][4 * k + e] * (e < 2 ? v0.y : v1.y);
+              }
             } else {
-              mma_16816(o[w][j], a & 0x00ff00ffu, (a >> 8) & 0x00ff00ffu, c & 0x00ff00ffu, (c >> 8) & 0x00ff00ffu, pb[j][0], pb[j][1]);
+#pragma unroll
+              for (int e = 0; e < 4; ++e) {
+                ps[e] = sc[j][4 * k + e] * (e < 2 ? v0.x : v1.x);
+                bias[j][g][e & 1] = fmaf(sc[j][4 * k + e], e < 2 ? v0.y : v1.y, bias[j][g][e & 1]);
+              }
+            }
+            pb[j][0] = transpose8x8(h2_as_u32(__floats2half2_rn(ps[0], ps[1])));
+            pb[j][1] = transpose8x8(h2_as_u32(__floats2half2_rn(ps[2], ps[3])));
+          }
+#pragma unroll
+          for (int w = g * WORDS / NG; w < (g + 1) * WORDS / NG; ++w) {
+            const uint32_t a = va[w], c = vb[w];
+#pragma unroll
+            for (int j = 0; j < NT; ++j) {
+              if constexpr (PER == 8) {
+                mma_16816(o[2 * w][j], a & 0x000f000fu, (a >> 8) & 0x000f000fu, c & 0x000f000fu, (c >> 8) & 0x000f000fu, pb[j][0], pb[j][1]);
+                mma_16816(o[2 * w + 1][j], a & 0x00f000f0u, (a >> 8) & 0x00f000f0u, c & 0x00f000f0u, (c >> 8) & 0x00f000f0u, pb[j][0], pb[j][1]);
+              } else {
+                mma_16816(o[w][j], a & 0x00ff00ffu, (a >> 8) & 0x00ff00ffu, c & 0x00ff00ffu, (c >> 8) & 0x00ff00ffu, pb[j][0], pb[j][1]);
+              }
             }
           }
         }
@@ -414,17 +440,8 @@ few_rows_quant_kernel(const PrefixAttnParams p, const uint8_t* pages, int with_p
       __syncwarp();
       if (i + NST < cnt) issue(i + NST);
     }
-    // ---- join the warps
-    const bool failed = __syncthreads_or(issued != used);  // a wait ran out (also: every ring is free)
-    if (failed) {
-      if (CLUSTER)  // the others' barriers: two for this tile of rows and for each that follows
-        for (int r = r0; r < rows_b; r += row_groups * RT) {
-          cluster_sync();
-          cluster_sync();
-        }
-      break;
-    }
-    float* so = reinterpret_cast<float*>(ring);  // [RT][HD], this warp's ring
+    // ---- this warp's sums, [RT][HD], over its ring, whose tiles it is done with
+    float* so = reinterpret_cast<float*>(ring);
 #pragma unroll
     for (int j = 0; j < NT; ++j)
 #pragma unroll
@@ -441,16 +458,23 @@ few_rows_quant_kernel(const PrefixAttnParams p, const uint8_t* pages, int with_p
           s_l[warp][r] = l[j][c];
         }
 #pragma unroll
-        for (int k = 0; k < C::MT; ++k)
-#pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            // the place in this thread's eighth of the groups of tile k's rows r8 (e = 0) and r8 + 8
-            const int at = PER == 8 ? (k >> 1) * 4 + 2 * e + (k & 1) : 2 * k + e, g = at / (GS / 8);
-            so[r * HD + g * GS + r8 * (GS / 8) + at % (GS / 8)] =
-                fmaf(o[k][j][2 * e + c], PER == 8 && (k & 1) ? 0x1p20f : 0x1p24f, bias[j][g][c]);
-          }
+        for (int k = 0; k < C::MT; k += 2) {  // four dims in a row: of two tiles of 16, this thread's two rows each
+          const int at = 2 * k, g = at / (GS / 8);
+          const float z = bias[j][g][c];
+          float4 v;
+          if constexpr (PER == 8)
+            v = make_float4(fmaf(o[k][j][c], 0x1p24f, z), fmaf(o[k + 1][j][c], 0x1p20f, z), fmaf(o[k][j][2 + c], 0x1p24f, z),
+                            fmaf(o[k + 1][j][2 + c], 0x1p20f, z));
+          else
+            v = make_float4(fmaf(o[k][j][c], 0x1p24f, z), fmaf(o[k][j][2 + c], 0x1p24f, z), fmaf(o[k + 1][j][c], 0x1p24f, z),
+                            fmaf(o[k + 1][j][2 + c], 0x1p24f, z));
+          *reinterpret_cast<float4*>(so + r * HD + g * GS + r8 * (GS / 8) + at % (GS / 8)) = v;
+        }
       }
-    __syncthreads();
+    return true;
+  };
+  // The warps' results joined, four values a thread at a time: sink(row, dim, sum, reference, sum of weights).
+  auto join_warps = [&](int nr, auto sink) {
     for (int e = threadIdx.x; e < nr * (HD / 4); e += FR_WARPS * 32) {
       const int r = e / (HD / 4), d = (e % (HD / 4)) * 4;
       float M = -INFINITY;
@@ -469,38 +493,246 @@ few_rows_quant_kernel(const PrefixAttnParams p, const uint8_t* pages, int with_p
         acc.w += f * v.w;
         L += f * s_l[w][r];
       }
-      const int tok = row_lo + (r0 + r) / p.G, g = (r0 + r) % p.G;
-      const size_t row = (size_t)tok * p.Hq + h * p.G + g;
-      if (CLUSTER) {
-        *reinterpret_cast<float4*>(base + ((size_t)(RT + r) * HD + d) * 4) = acc;  // behind warp 0's result
-        if (d == 0) s_ml[CLUSTER ? r : 0] = make_float2(M, L);
-      } else if (p.nslots == 1) {
-        store_out<__half>(reinterpret_cast<__half*>(p.out) + row * HD + d, acc, L);
-      } else {
-        const size_t at = (size_t)(slot0 + split) * p.T * p.Hq + row;
-        *reinterpret_cast<float4*>(p.part_o + at * HD + d) = acc;
-        if (d == 0) p.part_ml[at] = make_float2(M, L);
-      }
+      sink(r, d, acc, M, L);
     }
-    if (CLUSTER) {  // join the CTAs, each a part of the outputs
+  };
+  auto out_row = [&](int row_lo, int r, int h) { return (size_t)(row_lo + r / p.G) * p.Hq + h * p.G + r % p.G; };
+
+  if constexpr (CLUSTER) {
+    const int split = blockIdx.x % splits, group = blockIdx.x / splits, h = blockIdx.y, b = blockIdx.z;
+    const int t0 = split * FR_WARPS + warp, step = splits * FR_WARPS;
+    const int blocks0 = blocks_of(b, h, t0, step, 0);  // asked for before the lengths are there
+    int row_lo, row_hi, n;
+    request_rows(p, b, row_lo, row_hi, n);
+    const int rows_b = (row_hi - row_lo) * p.G, len = request_len(p, b);
+    for (int r0 = group * RT; r0 < rows_b; r0 += row_groups * RT) {
+      const int nr = min(RT, rows_b - r0);
+      const int own = max(0, min(len, len - n + (r0 + nr - 1) / p.G + 1));
+      const int nt = np + (own + KT - 1) / KT;
+      const bool ok = attend(b, h, row_lo, n, len, r0, nr, own, t0, step, max(0, (nt - t0 + step - 1) / step), blocks0);
+      if (__syncthreads_or(!ok)) {  // (also: every ring is free)
+        for (int r = r0; r < rows_b; r += row_groups * RT) {  // the others' barriers: two for this tile and for each that follows
+          cluster_sync();
+          cluster_sync();
+        }
+        break;
+      }
+      join_warps(nr, [&](int r, int d, const float4& acc, float M, float L) {
+        *reinterpret_cast<float4*>(base + ((size_t)(RT + r) * HD + d) * 4) = acc;  // behind warp 0's result
+        if (d == 0) s_ml[r] = make_float2(M, L);
+      });
       __syncthreads();
       cluster_sync();
       join_cluster<__half, HD>(p, smem_u32(s_ml), smem_u32(base) + RT * HD * 4, split, splits, nr, row_lo, r0, h);
       __syncthreads();
       cluster_sync();  // before a result is written over, or its CTA exits
+      // the rings hold the joined results: written by threads, next by copies
+      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+      __syncthreads();
     }
-    // the rings hold the joined results: written by threads, next by copies
-    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+  } else {
+    // ---- where the requests lie on the line: each thread a run of them, then a scan
+    const int per = (p.B + FR_WARPS * 32 - 1) / (FR_WARPS * 32), b0 = min(p.B, (int)threadIdx.x * per), b1 = min(p.B, b0 + per);
+    long long sum = 0;
+    for (int b = b0; b < b1; ++b) sum += stream_request<RT>(p, b, np).units;
+    long long upto = sum;
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+      const long long u = __shfl_up_sync(0xffffffffu, upto, d);
+      if (lane >= d) upto += u;
+    }
+    if (lane == 31) s_sum[warp] = upto;
     __syncthreads();
+    long long all = 0, at = upto - sum;
+    for (int w = 0; w < FR_WARPS; ++w) {
+      if (w < warp) at += s_sum[w];
+      all += s_sum[w];
+    }
+    const long long quantum = max((all + gridDim.x - 1) / gridDim.x, (long long)FQ_LEAST);
+    const long long lo = blockIdx.x * quantum, hi = min(all, lo + quantum);
+    if (blockIdx.x == 0) {
+      long long x = at;
+      for (int b = b0; b < b1; ++b) {
+        stream.offsets[b] = x;
+        x += stream_request<RT>(p, b, np).units;
+      }
+      if (threadIdx.x == 0) stream.offsets[p.B] = quantum;
+    }
+    if (lo >= at && lo < at + sum) {
+      int b = b0;
+      for (; b < b1; ++b) {
+        const long long u = stream_request<RT>(p, b, np).units;
+        if (lo < at + u) break;
+        at += u;
+      }
+      s_b = b;
+      s_at = at;
+    }
+    __syncthreads();
+    // ---- the CTA's piece of the line, unit by unit
+    long long pos = lo, off = lo < hi ? s_at : 0;
+    int b = lo < hi ? s_b : 0;
+    StreamRequest q = stream_request<RT>(p, b, np);
+    int unit = 0;
+    bool fresh = true;
+    while (pos < hi) {
+      if (pos >= off + q.units) {
+        off += q.units;
+        q = stream_request<RT>(p, ++b, np);
+        unit = 0;
+        continue;
+      }
+      const int u = q.nt + FQ_UNIT;
+      if (fresh) {  // the first unit
+        unit = (int)((pos - off) / u);
+        fresh = false;
+      }
+      const int ta = (int)(pos - off - (long long)unit * u), tb = (int)min((long long)u, ta + (hi - pos));
+      pos += tb - ta;
+      const int at = unit;
+      if (tb == u) ++unit;
+      if (ta > 0 && ta >= q.nt) continue;  // nothing left of it
+      const int h = at / q.tiles, r0 = (at - h * q.tiles) * RT, nr = min(RT, q.rows - r0);
+      const int own = max(0, min(q.len, q.len - q.n + (r0 + nr - 1) / p.G + 1));
+      const int end = min(tb, np + (own + KT - 1) / KT), t0 = ta + warp;
+      const int cnt = max(0, (end - t0 + FR_WARPS - 1) / FR_WARPS);
+      const bool ok = attend(b, h, q.row_lo, q.n, q.len, r0, nr, own, t0, FR_WARPS, cnt, blocks_of(b, h, t0, FR_WARPS, 0));
+      if (__syncthreads_or(!ok)) break;
+      const bool whole = ta == 0 && tb >= q.nt;
+      const size_t place = (size_t)(2 * blockIdx.x + (ta == 0 ? 1 : 0)) * RT;
+      join_warps(nr, [&](int r, int d, const float4& acc, float M, float L) {
+        const size_t row = out_row(q.row_lo, r0 + r, h);
+        if (!whole) {
+          *reinterpret_cast<float4*>(stream.o + (place + r) * HD + d) = acc;
+          if (d == 0) stream.ml[place + r] = make_float2(M, L);
+        } else if (slot0 < 0) {
+          store_out<__half>(reinterpret_cast<__half*>(p.out) + row * HD + d, acc, L);
+        } else {
+          const size_t to = (size_t)slot0 * p.T * p.Hq + row;
+          *reinterpret_cast<float4*>(p.part_o + to * HD + d) = acc;
+          if (d == 0) p.part_ml[to] = make_float2(M, L);
+        }
+      });
+      // the rings hold the results: written by threads, next by copies
+      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+      __syncthreads();
+    }
   }
   // copies in flight land before the CTA may exit (after a wait that ran out)
   if (lane == 0)
-    for (; used < issued; ++used) {
+    for (; in_flight; --in_flight) {
       int ignore = 0;
-      mbar_wait_bounded(&full[warp][used % NST], (used / NST) & 1u, &ignore, PA_WAIT_NS);
+      mbar_wait_bounded(&full[warp][s_out], phase, &ignore, PA_WAIT_NS);
+      if (++s_out == NST) {
+        s_out = 0;
+        phase ^= 1u;
+      }
     }
   if (threadIdx.x == 0 && s_abort) atomicExch(&g_prefix_attn_error, 1);
   if (!with_prefix && blockIdx.x == gridDim.x - 1 && blockIdx.y == gridDim.y - 1 && blockIdx.z == gridDim.z - 1) pdl_wait();
+}
+
+// ---------------------------------------------------------------- join
+
+// A row's partial results: the many-rows kernel's (slots 0 .. tc - 1, a value for every row), and of the CTAs that share the row's
+// unit on the line.  WPR warps to a (row, head), which read every WPR-th of them (few rows have many), eight of them in flight; a
+// block's rows are of one request.
+template <int HD, int RT, int WPR>
+__global__ void __launch_bounds__(256) join_stream_kernel(const PrefixAttnParams p, const StreamArgs stream, int with_prefix, int tc) {
+  constexpr int V = HD / 32, ROWS = 8 / WPR;
+  __shared__ float s_o[WPR > 1 ? 8 : 1][HD];
+  __shared__ float2 s_ml[WPR > 1 ? 8 : 1];
+  pdl_trigger();
+  pdl_wait();
+  const int b = blockIdx.x, warp = threadIdx.x >> 5, lane = threadIdx.x & 31, part = warp % WPR, P = with_prefix ? prefix_keys(p) : 0;
+  const StreamRequest q = stream_request<RT>(p, b, (int)(((long long)P + FQ_KEYS - 1) / FQ_KEYS));
+  const long long off = stream.offsets[b], quantum = stream.offsets[p.B];
+  const size_t stride = (size_t)p.T * p.Hq;
+  for (int i0 = blockIdx.y * ROWS; i0 < q.rows * p.Hkv; i0 += gridDim.y * ROWS) {
+    const int i = i0 + warp / WPR;
+    const bool live = i < q.rows * p.Hkv;
+    const int h = live ? i / q.rows : 0, r = live ? i % q.rows : 0;
+    const size_t row = (size_t)(q.row_lo + r / p.G) * p.Hq + h * p.G + r % p.G;
+    const long long start = off + ((long long)h * q.tiles + r / RT) * (q.nt + FQ_UNIT);
+    const int c0 = (int)(start / quantum), shares = q.nt ? (int)((start + q.nt - 1) / quantum) - c0 + 1 : 1;
+    // a unit that one CTA had lies in slot tc, or was written already
+    const int all = live ? tc + (shares > 1 ? shares : tc > 0 ? 1 : 0) : 0;
+    float acc[V], L = 0.f, M = -INFINITY;
+#pragma unroll
+    for (int k = 0; k < V; ++k) acc[k] = 0.f;
+    for (int s0 = part; s0 < all; s0 += 32 * WPR) {  // a lane's slot: s0 + WPR lane
+      const int s = s0 + WPR * lane, c = s - tc;
+      size_t at = 0;  // in rows of o
+      bool line = false;
+      float2 ml = make_float2(-INFINITY, 0.f);
+      if (s < all) {
+        line = c >= 0 && shares > 1;
+        at = line ? (size_t)(2 * (c0 + c) + (c == 0 ? 1 : 0)) * RT + r % RT : s * stride + row;
+        ml = line ? stream.ml[at] : p.part_ml[at];
+      }
+      float top = ml.x;
+#pragma unroll
+      for (int d = 16; d; d >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
+      top = fmaxf(M, top);
+      const float back = M == -INFINITY ? 0.f : ex2(M - top);
+      M = top;
+      L *= back;
+#pragma unroll
+      for (int k = 0; k < V; ++k) acc[k] *= back;
+      const float f = ml.x == -INFINITY && ml.y == 0.f ? 0.f : ex2(ml.x - M);  // 0: no key, nothing was written
+      L += f * ml.y;
+      const int n = min(32, (all - s0 + WPR - 1) / WPR);
+      for (int k0 = 0; k0 < n; k0 += 8) {
+        float fs[8], v[8][V];
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+          fs[k] = __shfl_sync(0xffffffffu, f, (k0 + k) & 31);
+          const unsigned long long src = __shfl_sync(0xffffffffu, (unsigned long long)(at * 2 + (line ? 1 : 0)), (k0 + k) & 31);
+          if (k0 + k >= n) fs[k] = 0.f;
+          const float* from = ((src & 1) ? stream.o : p.part_o) + (src >> 1) * HD + lane * V;
+#pragma unroll
+          for (int e = 0; e < V; ++e) v[k][e] = 0.f;
+          if (fs[k] != 0.f) {
+            if constexpr (V == 4)
+              *reinterpret_cast<float4*>(v[k]) = *reinterpret_cast<const float4*>(from);
+            else
+              *reinterpret_cast<float2*>(v[k]) = *reinterpret_cast<const float2*>(from);
+          }
+        }
+#pragma unroll
+        for (int k = 0; k < 8; ++k)
+#pragma unroll
+          for (int e = 0; e < V; ++e) acc[e] += fs[k] * v[k][e];
+      }
+    }
+#pragma unroll
+    for (int d = 16; d; d >>= 1) L += __shfl_xor_sync(0xffffffffu, L, d);
+    if constexpr (WPR > 1) {
+#pragma unroll
+      for (int e = 0; e < V; ++e) s_o[warp][lane * V + e] = acc[e];
+      if (lane == 0) s_ml[warp] = make_float2(M, L);
+      __syncthreads();
+      if (part == 0) {
+        for (int w = warp + 1; w < warp + WPR; ++w) M = fmaxf(M, s_ml[w].x);
+        L = 0.f;
+#pragma unroll
+        for (int e = 0; e < V; ++e) acc[e] = 0.f;
+        for (int w = warp; w < warp + WPR; ++w) {
+          if (s_ml[w].x == -INFINITY && s_ml[w].y == 0.f) continue;
+          const float f = ex2(s_ml[w].x - M);
+          L += f * s_ml[w].y;
+#pragma unroll
+          for (int e = 0; e < V; ++e) acc[e] += f * s_o[w][lane * V + e];
+        }
+      }
+      __syncthreads();
+    }
+    if (all == 0 || part != 0) continue;
+    const float inv = L == 0.f ? 0.f : 1.f / L;
+    __half* dst = reinterpret_cast<__half*>(p.out) + row * HD + lane * V;
+#pragma unroll
+    for (int k = 0; k < V; k += 2) *reinterpret_cast<__half2*>(dst + k) = __floats2half2_rn(acc[k] * inv, acc[k + 1] * inv);
+  }
 }
 
 // ---------------------------------------------------------------- host side
@@ -515,59 +747,165 @@ int quant_attn_device_error(int reset) {
   return v;
 }
 
-static AttnPlan plan_quant_attn(int T, int B, int Hkv, int G, long long own_keys, long long prefix_keys, int sms) {
-  AttnPlan a{};
+struct QuantPlan {
+  AttnPlan::Kind kind;
+  bool two;                // tiles of 16 rows in the few-rows kernel
+  int splits, row_groups;  // its clusters; 0: its CTAs take pieces of the line
+  int ctas;
+  long long units;          // of the line, if every request has the mean number of rows
+  int tc_splits, tc_items;  // many_rows_kernel
+  int nslots;               // partial results that every row has
+  size_t o_rows, ml_rows;   // rows of partial results in scratch: of values, with those of the line
+  size_t bytes;
+};
+
+// How a call is cut, as plan_attn (sc_prefix_attn.cu) does, by what the tables hold.  `resident`: CTAs of the few-rows kernel that an
+// SM takes, for tiles of 8 rows and of 16.
+static QuantPlan plan_quant_attn(int T, int B, int Hq, int Hkv, int hd, long long own_keys, long long prefix_keys, int sms,
+                                 const int (&resident)[2]) {
+  QuantPlan a{};
+  const int G = Hq / Hkv;
   const long long rows = (long long)T * G;
   const auto ceil_div = [](long long x, long long y) { return (x + y - 1) / y; };
-  const long long groups = ceil_div(rows, (long long)B * 8), slots = 4ll * sms;
-  a.kind = AttnPlan::FEW;
-  const long long keys = own_keys + prefix_keys;
-  const long long want = ceil_div(8ll * sms, (long long)B * Hkv);
-  a.row_groups = (int)std::max(1ll, std::min(want, groups > 1 ? 2 * groups : 1));
-  const long long most = ceil_div(keys, 64);
-  const long long once = std::max(1ll, std::min({slots / ((long long)B * Hkv * a.row_groups), most, (long long)FR_CLUSTER}));
-  const bool few_keys = (double)keys * std::max(ceil_div(slots, once), (long long)B * Hkv * a.row_groups) <= slots * 1536.0;
-  a.splits = (int)(few_keys ? once : std::max(1ll, std::min({ceil_div(want, a.row_groups), most, 64ll})));
-  a.cluster = few_keys && a.splits > 1;
-  a.nslots = a.cluster ? 1 : a.splits;
+  a.two = rows > 8ll * B;
+  const long long groups = ceil_div(rows, (long long)B * (a.two ? 16 : 8)), slots = (long long)resident[a.two] * sms;
+  a.units = (long long)B * Hkv * groups;
+  // Few rows a request: the prefix is taken apart (SHARED) once the keys of it that a CTA slot of the few-rows kernel would stream
+  // for its requests pass 1000 (us in a graph, 4 bits, few | shared: 8 kv heads of 128, 16 requests behind 2000 tokens 18 | 20, 8000 39 | 30,
+  // 64 behind 700 19 | 19, 2000 38 | 23; 4 of 64, 16 behind 8000 18 | 20, 16000 30 | 26, 64 behind 2000 18 | 18).  64 rows and more:
+  // the many-rows kernel over all keys, but for a few keys and tiles of rows, which clusters do with less of a start (cluster | chunks: one
+  // request of 64 new tokens over 600 11 | 15, behind 6000 82 | 34; 3 of 32 over 600 16 | 17, behind 1000 23 | 20; 8 of 32 alone
+  // 19 | 11), or where the prefix is most of what they see and a request has less than half a tile of rows (shared | chunks: 8 of 16 behind 6000
+  // 52 | 93, of 32 78 | 80, of 64 138 | 97).
+  const bool many = rows >= 64ll * B, shares = prefix_keys > 0 && B > 1;
+  const double load = (double)(own_keys + prefix_keys) * std::max(slots / FR_CLUSTER, a.units) / slots;
+  if (many ? a.units < 0.6 * slots && load <= 400 : !shares || (double)prefix_keys * a.units <= 1000.0 * slots)
+    a.kind = AttnPlan::FEW;
+  else if (!many || (shares && rows < 112ll * B && prefix_keys >= 4 * own_keys))
+    a.kind = AttnPlan::SHARED;
+  else
+    a.kind = AttnPlan::CHUNKS;
+  int line_sms = sms;
+  if (a.kind == AttnPlan::CHUNKS) {
+    // shares of the keys until there is a CTA for every SM, as in plan_attn; a request has a tile of rows of its own at least
+    const long long tiles = ceil_div(prefix_keys + own_keys, TC_N), items = B * ceil_div(rows, (long long)B * 2 * TC_M);
+    a.tc_items = (int)(ceil_div(rows, 2 * TC_M) + B);
+    a.tc_splits = (int)std::max(1ll, std::min({(sms + items * Hkv / 2) / (items * Hkv), tiles, 32ll}));
+    a.tc_splits = (int)ceil_div(tiles, ceil_div(tiles, a.tc_splits));
+    if (tiles - ceil_div(tiles, a.tc_splits) < 3) a.tc_splits = 1;
+    a.tc_splits = std::max(a.tc_splits, (int)std::min(32ll, ceil_div(tiles, 131072 / TC_N)));  // as in plan_attn
+    a.nslots = a.tc_splits;
+  } else if (a.kind == AttnPlan::SHARED) {
+    // Shares of the prefix: the ones that end soonest with the own keys' kernel beside them, by a tile of 256 rows and 128 keys in 2.3 us
+    // (heads of 64: 1.9) and 8 us for a CTA's start and end, own keys (half of what the tables hold) at 128 (230) a us and SM, and as much
+    // again for those that are left when the last of the prefix's CTAs has ended (their SMs fill late).  64 requests behind 8197 tokens,
+    // us with 4, 5, 6, 8, 10 shares: 57, 48, 45, 49, 52 (taken: 6); 256 behind 32768, 4, 6, 8, 10: 278, 256, 244, 243 (10).
+    const long long tiles = ceil_div(prefix_keys, TC_N), items = ceil_div(rows, 2 * TC_M);
+    const double tile = hd == 128 ? 2.3 : 1.9, few = (double)B * own_keys / 2 * Hkv * groups / (hd == 128 ? 128 : 230);
+    double best = INFINITY;
+    for (int s = 1; s <= 32 && s <= tiles; ++s) {
+      if (ceil_div(tiles, ceil_div(tiles, s)) != s) continue;  // no more shares than their longest one needs
+      const long long n = items * Hkv * s, waves = ceil_div(n, sms);
+      const double one = tile * ceil_div(tiles, s) + 8, beside = (double)(waves * sms - n) * one;
+      const double t = waves * one + 2 * std::max(0.0, few - beside) / sms;
+      if (t < best) {
+        best = t;
+        a.tc_splits = s;
+      }
+    }
+    a.tc_splits = std::max(a.tc_splits, (int)std::min(32ll, ceil_div(tiles, 131072 / TC_N)));
+    a.tc_items = (int)items;
+    a.nslots = a.tc_splits + 1;
+    // as many CTAs as the SMs that the prefix's kernel leaves take at once
+    const long long n = items * Hkv * a.tc_splits;
+    if (n < sms) line_sms = std::max(sms / 4, sms - (int)n);
+  } else {
+    // Clusters of up to eight CTAs, which join their shares in place, while a share is short: up to 1600 keys (heads of 64: 2200) of the longest
+    // request there may be, or, with more requests than CTA slots, 4500 keys a slot; past that pieces of the line and a join (us in a graph,
+    // requests of any length up to the longest, cluster | line: 8 kv heads of 128, one of 5000 9 | 14, of 20000 22 | 17, 16 of 5000 22 | 23,
+    // of 20000 71 | 54, 64 of 1200 22 | 25, of 5000 72 | 57, 128 of 5000 105 | 101; 4 of 64, 16 of 20000 23 | 24, of 60000 75 | 56).
+    a.nslots = 1;
+    const long long keys = own_keys + prefix_keys;
+    a.row_groups = (int)std::max(1ll, std::min(ceil_div(2 * slots, (long long)B * Hkv), groups > 1 ? 2 * groups : 1));
+    const long long ctas = (long long)B * Hkv * a.row_groups;
+    const long long once = std::max(1ll, std::min({slots / ctas, ceil_div(keys, 128), (long long)FR_CLUSTER}));
+    if (ctas >= slots ? keys * ctas <= 4500 * slots : keys <= (hd == 128 ? 1600 : 2200) * once) a.splits = (int)once;
+  }
+  size_t rows_all = a.nslots > 1 ? (size_t)a.nslots * T * Hq : 0;
+  a.o_rows = rows_all;
+  if (a.kind != AttnPlan::CHUNKS && !a.splits) {
+    a.ctas = resident[a.two] * line_sms;
+    rows_all += 2 * (size_t)a.ctas * (a.two ? 16 : 8);
+  }
+  a.ml_rows = rows_all;
+  a.bytes = rows_all * (hd + 2) * sizeof(float) + (a.ctas ? (size_t)(B + 1) * 8 : 0);
+  return a;
+}
+static QuantPlan plan_quant_attn(int T, int B, int Hq, int Hkv, int hd, int bits, int group, int max_blocks, int max_prefix_blocks, int page_size) {
+  QuantPlan a;
+  with_quant_block(hd, bits, group, [&](auto block) {
+    using QB = decltype(block);
+    a = plan_quant_attn(T, B, Hq, Hkv, hd, (long long)max_blocks * page_size, (long long)max_prefix_blocks * page_size, sm_count(),
+                        {FewRowsQuant<QB, 1>::CTAS, FewRowsQuant<QB, 2>::CTAS});
+    return 0;
+  });
   return a;
 }
 
 template <typename QB, int NT, bool CLUSTER>
-static int run_few_rows_quant(const PrefixAttnParams& p, const uint8_t* pages, const AttnPlan& a, cudaStream_t stream) {
+static int run_few_rows_quant(const PrefixAttnParams& p, const uint8_t* pages, const QuantPlan& a, const StreamArgs& line, cudaStream_t stream) {
   constexpr auto kern = few_rows_quant_kernel<QB, NT, CLUSTER>;
   constexpr int smem = FewRowsQuant<QB, NT>::SMEM;
   const cudaError_t e = opt_in<kern>(smem);
   if (e != cudaSuccess) return check_launch("prefix_attn_q", e);
-  launch_clusters(CLUSTER ? a.splits : 1, kern, dim3(a.splits * a.row_groups, p.Hkv, p.B), dim3(FR_WARPS * 32), smem, stream, p, pages,
-                  a.kind == AttnPlan::FEW ? 1 : 0, a.splits, a.row_groups, a.kind == AttnPlan::SHARED ? a.tc_splits : 0);
-  return check_launch("prefix_attn_q");
+  launch_clusters(CLUSTER ? a.splits : 1, kern, CLUSTER ? dim3(a.splits * a.row_groups, p.Hkv, p.B) : dim3(a.ctas), dim3(FR_WARPS * 32), smem,
+                  stream, p, pages, a.kind == AttnPlan::FEW ? 1 : 0, a.splits, a.row_groups, a.kind == AttnPlan::SHARED ? a.tc_splits : -1, line);
+  const int st = check_launch("prefix_attn_q");
+  if (CLUSTER || st != SC_OK) return st;
+  const long long rows = (long long)p.T * p.Hq;
+  const bool wide = a.ctas >= 8 * a.units;  // each unit in eight pieces or more, if all are alike
+  const long long y = std::min(std::max(16ll * sm_count() / p.B, 64ll), ((wide ? rows : rows / 8) * 2 + p.B - 1) / p.B);  // twice the mean: requests differ
+  launch(wide ? join_stream_kernel<QB::HD, 8 * NT, 8> : join_stream_kernel<QB::HD, 8 * NT, 1>, dim3(p.B, (unsigned)std::max(1ll, y)), dim3(256), 0, stream, p, line,
+         a.kind == AttnPlan::FEW ? 1 : 0, a.kind == AttnPlan::SHARED ? a.tc_splits : 0);
+  return check_launch("prefix_attn_q_join");
+}
+
+template <typename QB, bool PACKED>
+static int run_many_rows_quant(const PrefixAttnParams& p, const uint8_t* pages, const QuantPlan& a, cudaStream_t stream) {
+  using C = ManyRows<QB::HD, QuantSource<QB>>;
+  constexpr auto kern = many_rows_kernel<QB::HD, PACKED, QuantSource<QB>>;
+  const cudaError_t e = opt_in<kern>(C::SMEM);
+  if (e != cudaSuccess) return check_launch("prefix_attn_q", e);
+  launch(kern, dim3((unsigned)(a.tc_splits * a.tc_items), p.Hkv), dim3(C::THREADS), C::SMEM, stream, p, QuantSource<QB>{pages}, a.tc_splits, 0);
+  return check_launch("prefix_attn_q_many_rows");
 }
 
 template <typename QB>
-static int run_quant_attn(const PrefixAttnParams& p, const uint8_t* pages, const AttnPlan& a, cudaStream_t stream) {
-  const bool two = (long long)p.T * p.G > 8ll * p.B;
-  int st;
-  if (two)
-    st = a.cluster ? run_few_rows_quant<QB, 2, true>(p, pages, a, stream) : run_few_rows_quant<QB, 2, false>(p, pages, a, stream);
-  else
-    st = a.cluster ? run_few_rows_quant<QB, 1, true>(p, pages, a, stream) : run_few_rows_quant<QB, 1, false>(p, pages, a, stream);
-  if (st != SC_OK || p.nslots == 1) return st;
-  launch(join_slots_kernel<__half, QB::HD>, dim3((unsigned)(((size_t)p.T * p.Hq + 7) / 8)), dim3(256), 0, stream, p);
-  return check_launch("prefix_attn_q_join");
+static int run_quant_attn(const PrefixAttnParams& p, const uint8_t* pages, const QuantPlan& a, const StreamArgs& line, cudaStream_t stream) {
+  if (a.kind == AttnPlan::CHUNKS) {
+    const int st = run_many_rows_quant<QB, false>(p, pages, a, stream);
+    if (st != SC_OK || a.nslots == 1) return st;
+    launch(join_slots_kernel<__half, QB::HD>, dim3((unsigned)(((size_t)p.T * p.Hq + 7) / 8)), dim3(256), 0, stream, p);
+    return check_launch("prefix_attn_q_join");
+  }
+  if (a.kind == AttnPlan::SHARED) {
+    const int st = run_many_rows_quant<QB, true>(p, pages, a, stream);
+    if (st != SC_OK) return st;
+  }
+  if (a.splits)
+    return a.two ? run_few_rows_quant<QB, 2, true>(p, pages, a, line, stream) : run_few_rows_quant<QB, 1, true>(p, pages, a, line, stream);
+  return a.two ? run_few_rows_quant<QB, 2, false>(p, pages, a, line, stream) : run_few_rows_quant<QB, 1, false>(p, pages, a, line, stream);
 }
 
 }  // namespace sc
 
 extern "C" {
 
-size_t sc_prefix_attn_q_workspace_bytes(int T, int B, int Hq, int Hkv, int hd, int max_blocks, int max_prefix_blocks,
-                                        int page_size) {
-  if (T < 1 || B < 1 || Hq < 1 || Hkv < 1 || hd < 1 || max_blocks < 0 || max_prefix_blocks < 0 || page_size < 1) return 0;
-  if (Hq % Hkv) return 0;
-  const sc::AttnPlan a = sc::plan_quant_attn(T, B, Hkv, Hq / Hkv, (long long)max_blocks * page_size, (long long)max_prefix_blocks * page_size,
-                                             sc::sm_count());
-  return a.nslots <= 1 ? 0 : (size_t)a.nslots * T * Hq * (hd + 2) * sizeof(float);
+size_t sc_prefix_attn_q_workspace_bytes(int T, int B, int Hq, int Hkv, int hd, int bits, int group, int max_blocks,
+                                        int max_prefix_blocks, int page_size) {
+  if (T < 1 || B < 1 || Hq < 1 || Hkv < 1 || max_blocks < 0 || max_prefix_blocks < 0 || page_size < 1) return 0;
+  if (Hq % Hkv || !sc::quant_kind_ok(hd, bits, group)) return 0;
+  return sc::plan_quant_attn(T, B, Hq, Hkv, hd, bits, group, max_blocks, max_prefix_blocks, page_size).bytes;
 }
 
 int sc_prefix_attn_q(const void* q, const void* pages, int bits, int group, int T, const int32_t* q_start,
@@ -592,8 +930,8 @@ int sc_prefix_attn_q(const void* q, const void* pages, int bits, int group, int 
   SC_REQUIRE((((uintptr_t)q | (uintptr_t)pages | (uintptr_t)out) & 15) == 0, SC_ERR_ARG,
              "prefix_attn_q: tensors must start on 16-byte boundaries");
   if (!prefix_len) max_prefix_blocks = 0;
-  const AttnPlan a = plan_quant_attn(T, B, Hkv, Hq / Hkv, (long long)max_blocks * page_size, (long long)max_prefix_blocks * page_size, sm_count());
-  const size_t need = sc_prefix_attn_q_workspace_bytes(T, B, Hq, Hkv, hd, max_blocks, max_prefix_blocks, page_size);
+  const QuantPlan a = plan_quant_attn(T, B, Hq, Hkv, hd, bits, group, max_blocks, max_prefix_blocks, page_size);
+  const size_t need = a.bytes;
   SC_REQUIRE(workspace_bytes >= need && (need == 0 || workspace), SC_ERR_WORKSPACE,
              "prefix_attn_q: workspace of %zu bytes needed (got %zu)", need, workspace_bytes);
   SC_REQUIRE(((uintptr_t)workspace & 15) == 0, SC_ERR_ARG, "prefix_attn_q: the workspace must start on a 16-byte boundary");
@@ -601,7 +939,9 @@ int sc_prefix_attn_q(const void* q, const void* pages, int bits, int group, int 
   p.q = q;
   p.out = out;
   p.part_o = static_cast<float*>(workspace);
-  p.part_ml = reinterpret_cast<float2*>(p.part_o + (size_t)a.nslots * T * Hq * hd);
+  // values of all rows, of the line; then (m, l) of both; then the line's offsets
+  p.part_ml = reinterpret_cast<float2*>(p.part_o + a.ml_rows * hd);
+  const StreamArgs line = {reinterpret_cast<long long*>(p.part_ml + a.ml_rows), p.part_o + a.o_rows * hd, p.part_ml + a.o_rows};
   p.q_start = q_start;
   p.kv_lens = kv_lens;
   p.block_table = block_table;
@@ -619,7 +959,7 @@ int sc_prefix_attn_q(const void* q, const void* pages, int bits, int group, int 
   p.c = c;
   p.nslots = a.nslots;
   return with_quant_block(hd, bits, group, [&](auto block) {
-    return run_quant_attn<decltype(block)>(p, static_cast<const uint8_t*>(pages), a, stream);
+    return run_quant_attn<decltype(block)>(p, static_cast<const uint8_t*>(pages), a, line, stream);
   });
 }
 

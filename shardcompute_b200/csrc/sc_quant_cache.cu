@@ -4,7 +4,8 @@
 // a scale s and a bias b (fp16):
 //   b = min x rounded down, s = the smallest fp16 value with MOST s >= max x - b,
 //   c = rint((x - b) / s) in 0..MOST (0 where s is 0), and stands for s c + b
-// so that b <= x <= b + MOST s, and x is at most s / 2 off.
+// so that b <= x <= b + MOST s, and x is at most s / 2 off.  s and c are the ones that
+// exact arithmetic gives: next to a border, fp32's roundings would decide.
 #include <algorithm>
 
 #include "sc_quant.cuh"
@@ -17,7 +18,8 @@ struct AppendQuantParams {
   const float *cos_tab, *sin_tab;
   __half* q_out;
   uint8_t* pages;
-  int row0, items, Hq, Hkv, max_pos, n_pages, page;
+  int row0, items, Hq, Hkv, max_pos, n_pages;
+  PageDiv page, per_row;  // items of a row
 };
 
 __device__ __forceinline__ void load4(const float* p, float (&v)[4]) {
@@ -42,8 +44,9 @@ __device__ __forceinline__ float max_nan(float a, float b) {
   return d;
 }
 
-// (scale, bias) of a group with these extremes.  Where either is not finite the bias is NaN: the group stands for NaN, and
-// no score of it is an infinity that would take the token out of the attention unseen.
+// (scale, bias) of a group with these extremes.  Where either is not finite, or the largest code would stand for more than
+// fp16 holds, the bias is NaN: the group stands for NaN, and no score of it is an infinity that would take the token out of the
+// attention unseen.
 template <int MOST>
 __device__ __forceinline__ __half2 scale_bias(float lo, float hi) {
   const __half b = __float2half_rd(lo);
@@ -55,14 +58,20 @@ __device__ __forceinline__ __half2 scale_bias(float lo, float hi) {
     s = __ushort_as_half(u + 1);
   else if (u > 0 && u <= 0x7c00 && (double)(__half2float(__ushort_as_half(u - 1)) * MOST) >= need)
     s = __ushort_as_half(u - 1);
-  const bool finite = (__half_as_ushort(s) & 0x7c00) != 0x7c00 && (__half_as_ushort(b) & 0x7c00) != 0x7c00;
-  return __halves2half2(s, finite ? b : __ushort_as_half(0x7e00));
+  const float top = fmaf(__half2float(s), (float)MOST, __half2float(b));
+  return __halves2half2(s, __half2float(b) >= -65504.f && top <= 65504.f ? b : __ushort_as_half(0x7e00));
 }
 
+// rint((x - b) / s), `inv` about 1 / s.  The quotient in fp32 finds it or a neighbour; which, what is left over says exactly: x - b as
+// a sum of two fp32 values t + e, and t - c s, which near the border of two codes needs no rounding, against half a step.
 template <int MOST>
-__device__ __forceinline__ uint32_t code_of(float x, float s, float b) {
-  const float c = rintf(__fdiv_rn(x - b, s));
-  return s > 0.f ? (uint32_t)fminf(fmaxf(c, 0.f), (float)MOST) : 0u;  // NaN: 0
+__device__ __forceinline__ uint32_t code_of(float x, float s, float b, float inv) {
+  const float t = __fsub_rn(x, b), z = __fsub_rn(t, x), e = __fsub_rn(__fsub_rn(x, __fsub_rn(t, z)), __fadd_rn(b, z));
+  const float c = rintf(__fmul_rn(t, inv)), r = __fmaf_rn(-c, s, t), h = 0.5f * s;
+  const float over = __fsub_rn(r, h), under = __fadd_rn(r, h);  // beside -e: zero or more, zero or less
+  const bool odd = (int)c & 1;
+  const float up = over > -e || (over == -e && odd) ? 1.f : 0.f, down = under < -e || (under == -e && odd) ? 1.f : 0.f;
+  return s > 0.f ? (uint32_t)fminf(fmaxf(c + up - down, 0.f), (float)MOST) : 0u;  // NaN: 0
 }
 
 // Four codes as the bytes that hold them.
@@ -83,41 +92,60 @@ __global__ void __launch_bounds__(256) append_quant_kernel(const AppendQuantPara
   constexpr int HD = QB::HD, HALF = HD / 2, LPH = HD / 8, NG = QB::NG, GS = QB::GS;
   pdl_trigger();
   pdl_wait();
-  const int end = *p.rows_end, per_row = (p.Hq + 2 * p.Hkv) * LPH;
+  const int end = *p.rows_end;
+  int row[AQ_ITEMS], h[AQ_ITEMS], d[AQ_ITEMS], pos[AQ_ITEMS], slot[AQ_ITEMS];
+  bool live[AQ_ITEMS];
+  float a[AQ_ITEMS][4], b[AQ_ITEMS][4], c[AQ_ITEMS][4], s[AQ_ITEMS][4];
 #pragma unroll
   for (int i = 0; i < AQ_ITEMS; ++i) {
     const int it = (blockIdx.x * AQ_ITEMS + i) * 256 + threadIdx.x;
-    const int r = it / per_row, e = it - r * per_row, row = p.row0 + r, h = e / LPH, l = e % LPH, d = l * 4;
-    const bool live = it < p.items && row < end, is_kv = h >= p.Hq, is_v = h >= p.Hq + p.Hkv;
-    float a[4] = {0.f, 0.f, 0.f, 0.f}, b[4] = {0.f, 0.f, 0.f, 0.f};
-    int pos = -1, slot = -1;
-    if (live) {
-      pos = p.positions[row];
-      slot = p.slots[row];
-      const ST* src = reinterpret_cast<const ST*>(p.qkv) + ((size_t)row * (p.Hq + 2 * p.Hkv) + h) * HD + d;
-      load4(src, a);
-      load4(src + HALF, b);
-      if (!is_v && pos >= 0 && pos < p.max_pos) {
-        float c[4], s[4];
-        load4(p.cos_tab + (size_t)pos * HALF + d, c);
-        load4(p.sin_tab + (size_t)pos * HALF + d, s);
+    live[i] = it < p.items;
+    const int r = live[i] ? p.per_row.div(it) : 0, e = it - r * p.per_row.d;
+    row[i] = p.row0 + r;
+    live[i] = live[i] && row[i] < end;
+    h[i] = e / LPH;
+    d[i] = e % LPH * 4;
+    pos[i] = slot[i] = -1;
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          const float x = __fadd_rn(__fmul_rn(a[k], c[k]), __fmul_rn(-b[k], s[k]));
-          b[k] = __fadd_rn(__fmul_rn(b[k], c[k]), __fmul_rn(a[k], s[k]));
-          a[k] = x;
-        }
+    for (int k = 0; k < 4; ++k) {
+      a[i][k] = b[i][k] = s[i][k] = 0.f;
+      c[i][k] = 1.f;
+    }
+    if (live[i]) {
+      pos[i] = p.positions[row[i]];
+      slot[i] = p.slots[row[i]];
+      const ST* src = reinterpret_cast<const ST*>(p.qkv) + ((size_t)row[i] * (p.Hq + 2 * p.Hkv) + h[i]) * HD + d[i];
+      load4(src, a[i]);
+      load4(src + HALF, b[i]);
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < AQ_ITEMS; ++i)
+    if (live[i] && h[i] < p.Hq + p.Hkv && pos[i] >= 0 && pos[i] < p.max_pos) {
+      load4(p.cos_tab + (size_t)pos[i] * HALF + d[i], c[i]);
+      load4(p.sin_tab + (size_t)pos[i] * HALF + d[i], s[i]);
+    }
+#pragma unroll
+  for (int i = 0; i < AQ_ITEMS; ++i) {
+    const bool is_kv = h[i] >= p.Hq, is_v = h[i] >= p.Hq + p.Hkv;
+    if (!is_v) {
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const float x = __fadd_rn(__fmul_rn(a[i][k], c[i][k]), __fmul_rn(-b[i][k], s[i][k]));
+        b[i][k] = __fadd_rn(__fmul_rn(b[i][k], c[i][k]), __fmul_rn(a[i][k], s[i][k]));
+        a[i][k] = x;
       }
     }
-    if (live && !is_kv) {
-      __half* dst = p.q_out + ((size_t)row * p.Hq + h) * HD + d;
-      *reinterpret_cast<uint2*>(dst) = make_uint2(h2_as_u32(__floats2half2_rn(a[0], a[1])), h2_as_u32(__floats2half2_rn(a[2], a[3])));
-      *reinterpret_cast<uint2*>(dst + HALF) = make_uint2(h2_as_u32(__floats2half2_rn(b[0], b[1])), h2_as_u32(__floats2half2_rn(b[2], b[3])));
+    if (live[i] && !is_kv) {
+      __half* dst = p.q_out + ((size_t)row[i] * p.Hq + h[i]) * HD + d[i];
+      *reinterpret_cast<uint2*>(dst) = make_uint2(h2_as_u32(__floats2half2_rn(a[i][0], a[i][1])), h2_as_u32(__floats2half2_rn(a[i][2], a[i][3])));
+      *reinterpret_cast<uint2*>(dst + HALF) =
+          make_uint2(h2_as_u32(__floats2half2_rn(b[i][0], b[i][1])), h2_as_u32(__floats2half2_rn(b[i][2], b[i][3])));
     }
-    if (!__any_sync(0xffffffffu, live && is_kv)) continue;
+    if (!__any_sync(0xffffffffu, live[i] && is_kv)) continue;
     // ---- the groups of a's and of b's dims (one and the same where a head is a single group)
-    float lo[2] = {min_nan(min_nan(a[0], a[1]), min_nan(a[2], a[3])), min_nan(min_nan(b[0], b[1]), min_nan(b[2], b[3]))};
-    float hi[2] = {max_nan(max_nan(a[0], a[1]), max_nan(a[2], a[3])), max_nan(max_nan(b[0], b[1]), max_nan(b[2], b[3]))};
+    float lo[2] = {min_nan(min_nan(a[i][0], a[i][1]), min_nan(a[i][2], a[i][3])), min_nan(min_nan(b[i][0], b[i][1]), min_nan(b[i][2], b[i][3]))};
+    float hi[2] = {max_nan(max_nan(a[i][0], a[i][1]), max_nan(a[i][2], a[i][3])), max_nan(max_nan(b[i][0], b[i][1]), max_nan(b[i][2], b[i][3]))};
     if (NG == 1) {
       lo[0] = lo[1] = min_nan(lo[0], lo[1]);
       hi[0] = hi[1] = max_nan(hi[0], hi[1]);
@@ -130,20 +158,19 @@ __global__ void __launch_bounds__(256) append_quant_kernel(const AppendQuantPara
         lo[k] = min_nan(lo[k], __shfl_xor_sync(0xffffffffu, lo[k], x));
         hi[k] = max_nan(hi[k], __shfl_xor_sync(0xffffffffu, hi[k], x));
       }
-    const int id = slot >= 0 ? slot / p.page : p.n_pages;
-    if (!live || !is_kv || pos < 0 || pos >= p.max_pos || id >= p.n_pages) continue;
-    const int off = slot - id * p.page, tok = off & 15, head = h - p.Hq - (is_v ? p.Hkv : 0);
-    uint8_t* block = p.pages + (((size_t)id * p.Hkv + head) * (p.page >> 4) + (off >> 4)) * QB::BYTES;
+    const int id = slot[i] >= 0 ? p.page.div(slot[i]) : p.n_pages;
+    if (!live[i] || !is_kv || pos[i] < 0 || pos[i] >= p.max_pos || id >= p.n_pages) continue;
+    const int off = slot[i] - id * p.page.d, tok = off & 15, head = h[i] - p.Hq - (is_v ? p.Hkv : 0);
+    uint8_t* block = p.pages + (((size_t)id * p.Hkv + head) * (p.page.d >> 4) + (off >> 4)) * QB::BYTES;
 #pragma unroll
     for (int k = 0; k < 2; ++k) {
       const __half2 sb = scale_bias<QB::MOST>(lo[k], hi[k]);
-      const float s = __low2float(sb), bias = __high2float(sb);
-      const float(&x)[4] = k ? b : a;
-      const int dim = d + k * HALF;
-      uint32_t c[4];
+      const float scale = __low2float(sb), bias = __high2float(sb), inv = __frcp_rn(scale);
+      const int dim = d[i] + k * HALF;
+      uint32_t code[4];
 #pragma unroll
-      for (int j = 0; j < 4; ++j) c[j] = code_of<QB::MOST>(x[j], s, bias);
-      const uint32_t w = pack4<QB::BITS>(c);
+      for (int j = 0; j < 4; ++j) code[j] = code_of<QB::MOST>(k ? b[i][j] : a[i][j], scale, bias, inv);
+      const uint32_t w = pack4<QB::BITS>(code);
       if (is_v) {
         uint8_t* dst = block + QB::v_at(tok, dim);
         *reinterpret_cast<uint16_t*>(dst) = (uint16_t)w;
@@ -162,47 +189,65 @@ struct ReadQuantParams {
   const uint8_t* pages;
   const int32_t *slots, *rows_end;  // rows_end: NULL: every row
   void *k_out, *v_out;
-  int row0, items, Hkv, n_pages, page;
+  int row0, items, Hkv, n_pages;
+  PageDiv page, per_row;  // items of a row
 };
 
-// An item is eight consecutive values of a head of a row's K or V: s c + b in
-// fp32, rounded once.  Bound by the writes.
+// A code as fp32: 2^23 + c is its bit pattern.
+__device__ __forceinline__ float code_f32(uint32_t c) { return __uint_as_float(0x4b000000u | c) - 8388608.f; }
+
+// An item is sixteen values of a head of a row's K or V, four times four 32
+// apart, so that the items of a head store whole sectors together: s c + b in fp32,
+// rounded once.  With one group of four an item, finding its place was most of
+// the instructions (40000 rows of 8 heads of 128 in 8 bits to fp32 114 us).
 template <typename OT, typename QB>
 __global__ void __launch_bounds__(256) read_quant_kernel(const ReadQuantParams p) {
-  constexpr int HD = QB::HD, LPH = HD / 8;
+  constexpr int HD = QB::HD, LPH = 8, Q = HD / 32, NG = QB::NG;
   pdl_trigger();
   pdl_wait();
-  const int it = blockIdx.x * 256 + threadIdx.x, per_row = 2 * p.Hkv * LPH;
+  const int it = blockIdx.x * 256 + threadIdx.x;
   if (it >= p.items) return;
-  const int r = it / per_row, e = it - r * per_row, row = p.row0 + r, side = e / (p.Hkv * LPH), h = e / LPH - side * p.Hkv, d = e % LPH * 8;
-  if (p.rows_end && row >= *p.rows_end) return;
-  const int slot = p.slots[row], id = slot >= 0 ? slot / p.page : p.n_pages;
-  float v[8];
+  const int r = p.per_row.div(it), e = it - r * p.per_row.d, row = p.row0 + r;
+  const int slot = p.slots[row], end = p.rows_end ? *p.rows_end : INT32_MAX;
+  if (row >= end) return;
+  const int hh = e / LPH, side = hh >= p.Hkv, h = hh - (side ? p.Hkv : 0), d0 = e % LPH * 4;
+  const int id = slot >= 0 ? p.page.div(slot) : p.n_pages;
+  uint32_t w[Q], sb[NG];
+#pragma unroll
+  for (int k = 0; k < Q; ++k) w[k] = 0u;
+#pragma unroll
+  for (int g = 0; g < NG; ++g) sb[g] = 0u;
   if (id < p.n_pages) {
-    const int off = slot - id * p.page, tok = off & 15;
-    const uint8_t* block = p.pages + (((size_t)id * p.Hkv + h) * (p.page >> 4) + (off >> 4)) * QB::BYTES;
-    const __half2 sb = *reinterpret_cast<const __half2*>(block + (side ? QB::VM : QB::KM) + (tok * QB::NG + d / QB::GS) * 4);
-    const float s = __low2float(sb), b = __high2float(sb);
-    uint32_t w[2];
+    const int off = slot - id * p.page.d, tok = off & 15;
+    const uint8_t* block = p.pages + (((size_t)id * p.Hkv + h) * (p.page.d >> 4) + (off >> 4)) * QB::BYTES;
 #pragma unroll
-    for (int k = 0; k < 2; ++k) {
-      const uint8_t* src = block + (side ? QB::v_at(tok, d + 4 * k) : QB::k_at(tok, d + 4 * k));
-      w[k] = *reinterpret_cast<const uint16_t*>(src);
-      if (QB::BITS == 8) w[k] |= (uint32_t)*reinterpret_cast<const uint16_t*>(src + (side ? 4 : 2)) << 16;
+    for (int g = 0; g < NG; ++g) sb[g] = *reinterpret_cast<const uint32_t*>(block + (side ? QB::VM : QB::KM) + (tok * NG + g) * 4);
+#pragma unroll
+    for (int k = 0; k < Q; ++k) {
+      const int d = d0 + 32 * k;
+      if (side) {
+        const uint8_t* src = block + QB::v_at(tok, d);
+        w[k] = *reinterpret_cast<const uint16_t*>(src);
+        if (QB::BITS == 8) w[k] |= (uint32_t)*reinterpret_cast<const uint16_t*>(src + 4) << 16;
+      } else if (QB::BITS == 8) {
+        w[k] = *reinterpret_cast<const uint32_t*>(block + QB::k_at(tok, d));
+      } else {
+        w[k] = *reinterpret_cast<const uint16_t*>(block + QB::k_at(tok, d));
+      }
     }
-#pragma unroll
-    for (int j = 0; j < 8; ++j) v[j] = fmaf((float)((w[j >> 2] >> ((j & 3) * QB::BITS)) & QB::MOST), s, b);
-  } else {
-#pragma unroll
-    for (int j = 0; j < 8; ++j) v[j] = 0.f;
   }
-  OT* dst = reinterpret_cast<OT*>(side ? p.v_out : p.k_out) + ((size_t)row * p.Hkv + h) * HD + d;
-  if constexpr (sizeof(OT) == 2) {
-    *reinterpret_cast<uint4*>(dst) = make_uint4(h2_as_u32(__floats2half2_rn(v[0], v[1])), h2_as_u32(__floats2half2_rn(v[2], v[3])),
-                                                h2_as_u32(__floats2half2_rn(v[4], v[5])), h2_as_u32(__floats2half2_rn(v[6], v[7])));
-  } else {
-    *reinterpret_cast<float4*>(dst) = make_float4(v[0], v[1], v[2], v[3]);
-    *reinterpret_cast<float4*>(dst + 4) = make_float4(v[4], v[5], v[6], v[7]);
+  OT* dst = reinterpret_cast<OT*>(side ? p.v_out : p.k_out) + ((size_t)row * p.Hkv + h) * HD + d0;
+#pragma unroll
+  for (int k = 0; k < Q; ++k) {
+    const float2 f = __half22float2(u32_as_h2(sb[k * 32 / QB::GS]));
+    float v[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      v[j] = fmaf(code_f32(QB::BITS == 8 ? __byte_perm(w[k], 0u, 0x4440 + j) : (w[k] >> (4 * j)) & 15u), f.x, f.y);
+    if constexpr (sizeof(OT) == 2)
+      *reinterpret_cast<uint2*>(dst + 32 * k) = make_uint2(h2_as_u32(__floats2half2_rn(v[0], v[1])), h2_as_u32(__floats2half2_rn(v[2], v[3])));
+    else
+      *reinterpret_cast<float4*>(dst + 32 * k) = make_float4(v[0], v[1], v[2], v[3]);
   }
 }
 
@@ -244,7 +289,7 @@ int sc_paged_rope_append_q(const void* qkv, int qkv_dtype, int rows, const int32
              "paged_rope_append_q: tensors must start on 16-byte boundaries");
   SC_REQUIRE(((long long)Hq + 2ll * Hkv) * (hd / 8) <= (1 << 24), SC_ERR_SHAPE, "paged_rope_append_q: rows of %d + 2 * %d heads are too wide", Hq, Hkv);
   const AppendQuantParams p = {qkv, rows_end, slots, positions, cos_tab, sin_tab, static_cast<__half*>(q_out), static_cast<uint8_t*>(pages),
-                               0, 0, Hq, Hkv, max_pos, n_pages, page_size};
+                               0, 0, Hq, Hkv, max_pos, n_pages, page_div(page_size), page_div((Hq + 2 * Hkv) * (hd / 8))};
   return with_quant_block(hd, bits, group, [&](auto block) {
     using QB = decltype(block);
     return over_rows(p, rows, (Hq + 2 * Hkv) * (hd / 8), [&](const AppendQuantParams& a) {
@@ -268,11 +313,12 @@ int sc_paged_read_q(const void* pages, int bits, int group, int n_pages, int pag
   SC_REQUIRE(out_dtype == SC_F16 || out_dtype == SC_F32, SC_ERR_ARG, "paged_read_q: dtype");
   SC_REQUIRE((((uintptr_t)pages | (uintptr_t)k_out | (uintptr_t)v_out) & 15) == 0, SC_ERR_ARG,
              "paged_read_q: tensors must start on 16-byte boundaries");
-  SC_REQUIRE(2ll * Hkv * (hd / 8) <= (1 << 24), SC_ERR_SHAPE, "paged_read_q: rows of 2 * %d heads are too wide", Hkv);
-  const ReadQuantParams p = {static_cast<const uint8_t*>(pages), slots, rows_end, k_out, v_out, 0, 0, Hkv, n_pages, page_size};
+  SC_REQUIRE(2ll * Hkv * 8 <= (1 << 24), SC_ERR_SHAPE, "paged_read_q: rows of 2 * %d heads are too wide", Hkv);
+  const ReadQuantParams p = {static_cast<const uint8_t*>(pages), slots, rows_end, k_out, v_out, 0, 0, Hkv, n_pages,
+                             page_div(page_size), page_div(2 * Hkv * 8)};
   return with_quant_block(hd, bits, group, [&](auto block) {
     using QB = decltype(block);
-    return over_rows(p, rows, 2 * Hkv * (hd / 8), [&](const ReadQuantParams& a) {
+    return over_rows(p, rows, 2 * Hkv * 8, [&](const ReadQuantParams& a) {
       auto kern = out_dtype == SC_F32 ? read_quant_kernel<float, QB> : read_quant_kernel<__half, QB>;
       launch(kern, dim3((unsigned)((a.items + 255) / 256)), dim3(256), 0, stream, a);
       return check_launch("paged_read_q");

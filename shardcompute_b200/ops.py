@@ -596,8 +596,10 @@ def paged_read_q(pages: QuantPages, slots: torch.Tensor, q_start: Optional[torch
     """The tokens that ``slots`` [T] hold, as ``(k, v)`` [T, Hkv, hd] of ``dtype`` (float16 or float32; that of ``k_out`` and
     ``v_out`` where they are given): what the cache stands for, rounded once.  Zeros for a slot outside the pool.  With
     ``q_start`` rows from ``q_start[-1]`` on are left as they were."""
-    n_pages, Hkv = _quant_pool("paged_read_q", pages)
     data, hd, page, bits, group = pages
+    if k_out is not None and v_out is not None and _native().paged_read_q(slots, data, hd, page, bits, group, q_start, k_out, v_out) == 0:
+        return k_out, v_out
+    n_pages, Hkv = _quant_pool("paged_read_q", pages)
     T, dev = slots.numel(), slots.get_device()
     if (k_out is None) != (v_out is None):
         raise ValueError("paged_read_q: k_out and v_out go together")
@@ -624,8 +626,8 @@ def paged_read_q(pages: QuantPages, slots: torch.Tensor, q_start: Optional[torch
 
 @functools.lru_cache(maxsize=1024)
 def prefix_attn_q_workspace_bytes(T: int, B: int, Hq: int, Hkv: int, hd: int, max_blocks: int, max_prefix_blocks: int,
-                                  page_size: int) -> int:
-    return int(L.load().sc_prefix_attn_q_workspace_bytes(T, B, Hq, Hkv, hd, max_blocks, max_prefix_blocks, page_size))
+                                  page_size: int, bits: int = 4, group_size: int = 64) -> int:
+    return int(L.load().sc_prefix_attn_q_workspace_bytes(T, B, Hq, Hkv, hd, bits, group_size, max_blocks, max_prefix_blocks, page_size))
 
 
 def prefix_attn_q(q: torch.Tensor, pages: QuantPages, q_start: torch.Tensor, kv_lens: torch.Tensor, block_table: torch.Tensor,
@@ -668,7 +670,7 @@ def prefix_attn_q(q: torch.Tensor, pages: QuantPages, q_start: torch.Tensor, kv_
     _sized("prefix_attn_q", B + 1, q_start=q_start)
     if not T or not B:
         return out
-    nbytes = prefix_attn_q_workspace_bytes(T, B, Hq, Hkv, hd, tab[1], nbp, page)
+    nbytes = prefix_attn_q_workspace_bytes(T, B, Hq, Hkv, hd, tab[1], nbp, page, bits, group)
     wp, wb = None, 0
     if workspace is not None:
         _check("prefix_attn_q", dev, (workspace,))

@@ -83,9 +83,11 @@ def test_attn_refuses(kw, code):
 
 def test_attn_workspace_is_bounded():
     for T, B in [(1, 1), (1, 4096), (256, 256), (16384, 1), (16384, 64), (100000, 1000)]:
-        n = ops.prefix_attn_q_workspace_bytes(T, B, 32, 8, 128, 4096, 4096, 16)
-        assert 0 <= n <= 64 * max(T, 148) * 32 * 130 * 4
-    assert L.load().sc_prefix_attn_q_workspace_bytes(4, 4, 7, 2, 128, 8, 8, 16) == 0
+        for bits, group in [(4, 64), (8, 32)]:
+            n = ops.prefix_attn_q_workspace_bytes(T, B, 32, 8, 128, 4096, 4096, 16, bits, group)
+            assert 0 <= n <= 64 * max(T, 148) * 32 * 130 * 4
+    assert L.load().sc_prefix_attn_q_workspace_bytes(4, 4, 7, 2, 128, 4, 64, 8, 8, 16) == 0
+    assert L.load().sc_prefix_attn_q_workspace_bytes(4, 4, 8, 2, 96, 4, 64, 8, 8, 16) == 0
 
 
 def test_tensors_are_checked():
