@@ -31,6 +31,7 @@ struct FewRowsQuant {
   static constexpr int RT = 8 * NT;            // rows of a tile
   static constexpr int WORDS = QB::KSH / 4;    // of codes in a thread's share of a token
   static constexpr int PER = 32 / QB::BITS;    // codes of a word
+  static constexpr float MID = QB::BITS == 4 ? 8.f : 128.f;
   static constexpr int KSTEPS = QB::HD / 16, MT = QB::HD / 16;
   static constexpr int STAGE = 2 * QB::BYTES;  // two blocks: 32 tokens
   static constexpr int NST = STAGE > 4000 ? 2 : STAGE > 2400 ? 3 : 4;
@@ -136,9 +137,9 @@ few_rows_quant_kernel(const PrefixAttnParams p, const uint8_t* pages, int with_p
     fence_mbar_init();
   }
   __syncthreads();
-  pdl_trigger();
   // Without the prefix this kernel runs beside the prefix's, as few_rows_kernel does (sc_prefix_attn.cu).
   if (with_prefix) pdl_wait();
+  pdl_trigger();  // after the wait: the join relies on it
   const int P = with_prefix ? prefix_keys(p) : 0, np = (int)(((long long)P + KT - 1) / KT);
   unsigned char* ring = base + (size_t)warp * C::RING;
   const uint32_t ring_u = smem_u32(ring);
@@ -178,19 +179,24 @@ few_rows_quant_kernel(const PrefixAttnParams p, const uint8_t* pages, int with_p
       s_in = s_in + 1 == NST ? 0 : s_in + 1;
       ++in_flight;
     };
-    for (int i = 0; i < min(NST, cnt); ++i) issue(i);
-
-    // ---- q's fragments, by all warps: eight dims of a row a lane, those of a word (8 bits: two) of a thread's share of K
+    // ---- q's fragments, by all warps: eight dims of a row a lane, those of a word (8 bits: two) of a thread's share of K; asked for
+    // ahead of the copies, which wait for the page ids
+    constexpr int LPR = HD / 8, SH = GS / 4, QR = FR_WARPS * 256 / HD, PASSES = (RT + QR - 1) / QR;
+    const int qc = threadIdx.x % LPR, t = qc & 3, w = qc >> 2;
+    uint4 qv[PASSES];
 #pragma unroll
-    for (int r1 = 0; r1 < RT; r1 += FR_WARPS * 256 / HD) {
-      constexpr int LPR = HD / 8, SH = GS / 4;
-      const int r = r1 + (int)threadIdx.x / LPR, c = threadIdx.x % LPR, t = c & 3, w = c >> 2;
-      const int d = w * 8 / SH * GS + t * SH + w * 8 % SH;
-      uint4 u = make_uint4(0u, 0u, 0u, 0u);
-      if (r < nr) {
-        const int tok = (r0 + r) / p.G;
-        u = *reinterpret_cast<const uint4*>(reinterpret_cast<const __half*>(p.q) + ((size_t)(row_lo + tok) * p.Hq + h * p.G + (r0 + r - tok * p.G)) * HD + d);
-      }
+    for (int k = 0; k < PASSES; ++k) {
+      const int r = k * QR + (int)threadIdx.x / LPR, tok = (r0 + r) / p.G;
+      qv[k] = make_uint4(0u, 0u, 0u, 0u);
+      if (r < nr)
+        qv[k] = *reinterpret_cast<const uint4*>(reinterpret_cast<const __half*>(p.q) + ((size_t)(row_lo + tok) * p.Hq + h * p.G + (r0 + r - tok * p.G)) * HD +
+                                                w * 8 / SH * GS + t * SH + w * 8 % SH);
+    }
+    for (int i = 0; i < min(NST, cnt); ++i) issue(i);
+#pragma unroll
+    for (int k1 = 0; k1 < PASSES; ++k1) {
+      const int r = k1 * QR + (int)threadIdx.x / LPR;
+      const uint4 u = qv[k1];
       float x[8];
       const uint32_t uu[4] = {u.x, u.y, u.z, u.w};
       float big = 0.f, sum = 0.f;
@@ -219,7 +225,7 @@ few_rows_quant_kernel(const PrefixAttnParams p, const uint8_t* pages, int with_p
       else
         asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(to), "r"(pair(0, 2, up)), "r"(pair(1, 3, up)), "r"(pair(4, 6, up)),
                      "r"(pair(5, 7, up)) : "memory");
-      if (c == 0) s_cq[r] = p.c * back;
+      if (qc == 0) s_cq[r] = p.c * back;
       if (w * 8 % SH == 0 && t == 0) s_qsum[w * 8 / SH][r] = sum / back;
     }
     __syncthreads();
@@ -235,11 +241,14 @@ few_rows_quant_kernel(const PrefixAttnParams p, const uint8_t* pages, int with_p
     // own keys that the first row sees
     const int see_first = max(0, min(len, len - n + r0 / p.G + 1));
 
-    float o[C::MT][NT][4], bias[NT][NG][2], m[NT][2], l[NT][2];
+    float o[C::MT][NT][4], z[NG][NT][4], bias[NT][NG][2], m[NT][2], l[NT][2];
+    bool far = false;  // m of some column
 #pragma unroll
     for (int j = 0; j < NT; ++j) {
 #pragma unroll
       for (int i = 0; i < C::MT; ++i) o[i][j][0] = o[i][j][1] = o[i][j][2] = o[i][j][3] = 0.f;
+#pragma unroll
+      for (int g = 0; g < NG; ++g) z[g][j][0] = z[g][j][1] = z[g][j][2] = z[g][j][3] = 0.f;
 #pragma unroll
       for (int c = 0; c < 2; ++c) {
         m[j][c] = -INFINITY;
@@ -320,10 +329,6 @@ few_rows_quant_kernel(const PrefixAttnParams p, const uint8_t* pages, int with_p
           }
         }
       }
-#pragma unroll
-      for (int j = 0; j < NT; ++j)
-#pragma unroll
-        for (int e = 0; e < 8; ++e) sc[j][e] *= cq[j][e & 1];
       uint32_t hidden = 0;  // bit 8 j + e
       if (part) {
 #pragma unroll
@@ -359,8 +364,9 @@ few_rows_quant_kernel(const PrefixAttnParams p, const uint8_t* pages, int with_p
       for (int j = 0; j < NT; ++j)
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
-          x[j][c] = fmaxf(fmaxf(sc[j][c] + lg[0], sc[j][2 + c] + lg[1]), fmaxf(sc[j][4 + c] + lg[2], sc[j][6 + c] + lg[3])) - PA_LIFT;
-          up |= x[j][c] > m[j][c] + PA_RAISE;
+          x[j][c] = fmaxf(fmaxf(fmaf(sc[j][c], cq[j][c], lg[0]), fmaf(sc[j][2 + c], cq[j][c], lg[1])),
+                          fmaxf(fmaf(sc[j][4 + c], cq[j][c], lg[2]), fmaf(sc[j][6 + c], cq[j][c], lg[3])));
+          up |= x[j][c] > m[j][c] + (PA_LIFT + PA_RAISE);
         }
       if (__any_sync(0xffffffffu, up)) {
 #pragma unroll
@@ -369,7 +375,8 @@ few_rows_quant_kernel(const PrefixAttnParams p, const uint8_t* pages, int with_p
           for (int c = 0; c < 2; ++c) {
 #pragma unroll
             for (int d = 4; d <= 16; d <<= 1) x[j][c] = fmaxf(x[j][c], __shfl_xor_sync(0xffffffffu, x[j][c], d));
-            const float mn = fmaxf(m[j][c], x[j][c]), f = m[j][c] == -INFINITY ? 0.f : ex2(m[j][c] - mn);
+            // (a column that did not pass keeps its m: what the others see has no influence on it, not even on its roundings)
+            const float mn = x[j][c] > m[j][c] + (PA_LIFT + PA_RAISE) ? x[j][c] - PA_LIFT : m[j][c], f = m[j][c] == -INFINITY ? 0.f : ex2(m[j][c] - mn);
             m[j][c] = mn;
             l[j][c] *= f;
 #pragma unroll
@@ -379,18 +386,37 @@ few_rows_quant_kernel(const PrefixAttnParams p, const uint8_t* pages, int with_p
               o[k][j][c] *= f;
               o[k][j][2 + c] *= f;
             }
+            z[0][j][c] *= f;
+            if constexpr (NG > 1) z[NG - 1][j][c] *= f;
+            if constexpr (NG > 2) {
+              z[1][j][c] *= f;
+              z[2][j][c] *= f;
+            }
           }
+        bool any = false;
+#pragma unroll
+        for (int j = 0; j < NT; ++j) any |= (fabsf(m[j][0]) >= PA_FAR && m[j][0] != -INFINITY) || (fabsf(m[j][1]) >= PA_FAR && m[j][1] != -INFINITY);
+        far = __any_sync(0xffffffffu, any);
       }
-      // (the difference is rounded apart from c s, and the exponent kept to what m was chosen for: m far from zero is itself
-      // rounded by more than a little)
+      // p = 2^(c s - m).  Where m is far from zero it is itself rounded by more than a little: there the difference is rounded apart
+      // from c s, and the exponent kept to what m was chosen for.
+      auto weights = [&](auto is_far) {
 #pragma unroll
-      for (int j = 0; j < NT; ++j)
+        for (int j = 0; j < NT; ++j)
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          const float mm = m[j][e & 1] == -INFINITY ? 0.f : m[j][e & 1];
-          sc[j][e] = ex2(min_keep_nan(sc[j][e] - mm, PA_LIFT + PA_RAISE - lg[e >> 1]));
-          l[j][e & 1] += sc[j][e];
-        }
+          for (int e = 0; e < 8; ++e) {
+            const float mm = m[j][e & 1] == -INFINITY ? 0.f : m[j][e & 1];
+            float d = fmaf(sc[j][e], cq[j][e & 1], -mm);
+            if constexpr (is_far)
+              if (fabsf(mm) >= PA_FAR) d = min_keep_nan(__fsub_rn(__fmul_rn(sc[j][e], cq[j][e & 1]), mm), PA_LIFT + PA_RAISE - lg[e >> 1]);
+            sc[j][e] = ex2(d);
+            l[j][e & 1] += sc[j][e];
+          }
+      };
+      if (far)
+        weights(std::true_type{});
+      else
+        weights(std::false_type{});
       // ---- O += V^T (P s)^T, and the biases' part
 #pragma unroll
       for (int k = 0; k < 2; ++k) {
@@ -400,7 +426,9 @@ few_rows_quant_kernel(const PrefixAttnParams p, const uint8_t* pages, int with_p
         lds_share<WORDS>(block + 8 * QB::ROW, block + 8 * QB::ROW + 128, vb);
 #pragma unroll
         for (int g = 0; g < NG; ++g) {
-          const float2 v0 = __half22float2(u32_as_h2(mv[2 * k][g])), v1 = __half22float2(u32_as_h2(mv[2 * k + 1][g]));
+          float2 v0 = __half22float2(u32_as_h2(mv[2 * k][g])), v1 = __half22float2(u32_as_h2(mv[2 * k + 1][g]));
+          v0.y = fmaf(v0.x, C::MID, v0.y);
+          v1.y = fmaf(v1.x, C::MID, v1.y);
           uint32_t pb[NT][2];
 #pragma unroll
           for (int j = 0; j < NT; ++j) {
@@ -421,6 +449,7 @@ few_rows_quant_kernel(const PrefixAttnParams p, const uint8_t* pages, int with_p
             }
             pb[j][0] = transpose8x8(h2_as_u32(__floats2half2_rn(ps[0], ps[1])));
             pb[j][1] = transpose8x8(h2_as_u32(__floats2half2_rn(ps[2], ps[3])));
+            mma_16816(z[g][j], 0x00010001u, 0x00010001u, 0x00010001u, 0x00010001u, pb[j][0], pb[j][1]);
           }
 #pragma unroll
           for (int w = g * WORDS / NG; w < (g + 1) * WORDS / NG; ++w) {
@@ -428,8 +457,9 @@ few_rows_quant_kernel(const PrefixAttnParams p, const uint8_t* pages, int with_p
 #pragma unroll
             for (int j = 0; j < NT; ++j) {
               if constexpr (PER == 8) {
-                mma_16816(o[2 * w][j], a & 0x000f000fu, (a >> 8) & 0x000f000fu, c & 0x000f000fu, (c >> 8) & 0x000f000fu, pb[j][0], pb[j][1]);
-                mma_16816(o[2 * w + 1][j], a & 0x00f000f0u, (a >> 8) & 0x00f000f0u, c & 0x00f000f0u, (c >> 8) & 0x00f000f0u, pb[j][0], pb[j][1]);
+                const uint32_t a0 = a & 0x00ff00ffu, a1 = __byte_perm(a, 0u, 0x4341), c0 = c & 0x00ff00ffu, c1 = __byte_perm(c, 0u, 0x4341);
+                mma_16816(o[2 * w][j], a0 & 0x000f000fu, a1 & 0x000f000fu, c0 & 0x000f000fu, c1 & 0x000f000fu, pb[j][0], pb[j][1]);
+                mma_16816(o[2 * w + 1][j], a0, a1, c0, c1, pb[j][0], pb[j][1]);  // n0 + 16 n1
               } else {
                 mma_16816(o[w][j], a & 0x00ff00ffu, (a >> 8) & 0x00ff00ffu, c & 0x00ff00ffu, (c >> 8) & 0x00ff00ffu, pb[j][0], pb[j][1]);
               }
@@ -460,14 +490,14 @@ few_rows_quant_kernel(const PrefixAttnParams p, const uint8_t* pages, int with_p
 #pragma unroll
         for (int k = 0; k < C::MT; k += 2) {  // four dims in a row: of two tiles of 16, this thread's two rows each
           const int at = 2 * k, g = at / (GS / 8);
-          const float z = bias[j][g][c];
+          const float add = fmaf(z[g][j][c], -C::MID * 0x1p24f, bias[j][g][c]);
           float4 v;
           if constexpr (PER == 8)
-            v = make_float4(fmaf(o[k][j][c], 0x1p24f, z), fmaf(o[k + 1][j][c], 0x1p20f, z), fmaf(o[k][j][2 + c], 0x1p24f, z),
-                            fmaf(o[k + 1][j][2 + c], 0x1p20f, z));
+            v = make_float4(fmaf(o[k][j][c], 0x1p24f, add), fmaf(o[k + 1][j][c] - o[k][j][c], 0x1p20f, add), fmaf(o[k][j][2 + c], 0x1p24f, add),
+                            fmaf(o[k + 1][j][2 + c] - o[k][j][2 + c], 0x1p20f, add));
           else
-            v = make_float4(fmaf(o[k][j][c], 0x1p24f, z), fmaf(o[k][j][2 + c], 0x1p24f, z), fmaf(o[k + 1][j][c], 0x1p24f, z),
-                            fmaf(o[k + 1][j][2 + c], 0x1p24f, z));
+            v = make_float4(fmaf(o[k][j][c], 0x1p24f, add), fmaf(o[k][j][2 + c], 0x1p24f, add), fmaf(o[k + 1][j][c], 0x1p24f, add),
+                            fmaf(o[k + 1][j][2 + c], 0x1p24f, add));
           *reinterpret_cast<float4*>(so + r * HD + g * GS + r8 * (GS / 8) + at % (GS / 8)) = v;
         }
       }
@@ -635,23 +665,24 @@ few_rows_quant_kernel(const PrefixAttnParams p, const uint8_t* pages, int with_p
 // ---------------------------------------------------------------- join
 
 // A row's partial results: the many-rows kernel's (slots 0 .. tc - 1, a value for every row), and of the CTAs that share the row's
-// unit on the line.  WPR warps to a (row, head), which read every WPR-th of them (few rows have many), eight of them in flight; a
-// block's rows are of one request.
+// unit on the line.  WPR warps to a (row, head), which read every WPR-th of them (few rows have many), eight of them in flight,
+// each with its (m, l); a block's rows are of one request.  Bound by latency: what does not hang on the results is asked for
+// while the kernel before still runs.
 template <int HD, int RT, int WPR>
 __global__ void __launch_bounds__(256) join_stream_kernel(const PrefixAttnParams p, const StreamArgs stream, int with_prefix, int tc) {
-  constexpr int V = HD / 32, ROWS = 8 / WPR;
+  constexpr int V = HD / 32, ROWS = 8 / WPR, N = 8;
   __shared__ float s_o[WPR > 1 ? 8 : 1][HD];
   __shared__ float2 s_ml[WPR > 1 ? 8 : 1];
-  pdl_trigger();
-  pdl_wait();
   const int b = blockIdx.x, warp = threadIdx.x >> 5, lane = threadIdx.x & 31, part = warp % WPR, P = with_prefix ? prefix_keys(p) : 0;
   const StreamRequest q = stream_request<RT>(p, b, (int)(((long long)P + FQ_KEYS - 1) / FQ_KEYS));
+  pdl_wait();
+  pdl_trigger();
   const long long off = stream.offsets[b], quantum = stream.offsets[p.B];
   const size_t stride = (size_t)p.T * p.Hq;
   for (int i0 = blockIdx.y * ROWS; i0 < q.rows * p.Hkv; i0 += gridDim.y * ROWS) {
     const int i = i0 + warp / WPR;
     const bool live = i < q.rows * p.Hkv;
-    const int h = live ? i / q.rows : 0, r = live ? i % q.rows : 0;
+    const int h = live ? i / q.rows : 0, r = live ? i - h * q.rows : 0;
     const size_t row = (size_t)(q.row_lo + r / p.G) * p.Hq + h * p.G + r % p.G;
     const long long start = off + ((long long)h * q.tiles + r / RT) * (q.nt + FQ_UNIT);
     const int c0 = (int)(start / quantum), shares = q.nt ? (int)((start + q.nt - 1) / quantum) - c0 + 1 : 1;
@@ -660,53 +691,43 @@ __global__ void __launch_bounds__(256) join_stream_kernel(const PrefixAttnParams
     float acc[V], L = 0.f, M = -INFINITY;
 #pragma unroll
     for (int k = 0; k < V; ++k) acc[k] = 0.f;
-    for (int s0 = part; s0 < all; s0 += 32 * WPR) {  // a lane's slot: s0 + WPR lane
-      const int s = s0 + WPR * lane, c = s - tc;
-      size_t at = 0;  // in rows of o
-      bool line = false;
-      float2 ml = make_float2(-INFINITY, 0.f);
-      if (s < all) {
-        line = c >= 0 && shares > 1;
-        at = line ? (size_t)(2 * (c0 + c) + (c == 0 ? 1 : 0)) * RT + r % RT : s * stride + row;
-        ml = line ? stream.ml[at] : p.part_ml[at];
-      }
-      float top = ml.x;
+    for (int s0 = part; s0 < all; s0 += N * WPR) {
+      float2 ml[N];
+      float v[N][V];
 #pragma unroll
-      for (int d = 16; d; d >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
-      top = fmaxf(M, top);
+      for (int k = 0; k < N; ++k) {
+        const int s = s0 + k * WPR, c = s - tc;
+        ml[k] = make_float2(-INFINITY, 0.f);
+#pragma unroll
+        for (int e = 0; e < V; ++e) v[k][e] = 0.f;
+        if (s < all) {
+          const bool line = c >= 0 && shares > 1;
+          const size_t at = line ? (size_t)(2 * (c0 + c) + (c == 0 ? 1 : 0)) * RT + r % RT : s * stride + row;
+          ml[k] = line ? stream.ml[at] : p.part_ml[at];
+          const float* from = (line ? stream.o : p.part_o) + at * HD + lane * V;
+          if constexpr (V == 4)
+            *reinterpret_cast<float4*>(v[k]) = *reinterpret_cast<const float4*>(from);
+          else
+            *reinterpret_cast<float2*>(v[k]) = *reinterpret_cast<const float2*>(from);
+        }
+      }
+      float top = M;
+#pragma unroll
+      for (int k = 0; k < N; ++k) top = fmaxf(top, ml[k].x);
       const float back = M == -INFINITY ? 0.f : ex2(M - top);
       M = top;
       L *= back;
 #pragma unroll
-      for (int k = 0; k < V; ++k) acc[k] *= back;
-      const float f = ml.x == -INFINITY && ml.y == 0.f ? 0.f : ex2(ml.x - M);  // 0: no key, nothing was written
-      L += f * ml.y;
-      const int n = min(32, (all - s0 + WPR - 1) / WPR);
-      for (int k0 = 0; k0 < n; k0 += 8) {
-        float fs[8], v[8][V];
+      for (int e = 0; e < V; ++e) acc[e] *= back;
 #pragma unroll
-        for (int k = 0; k < 8; ++k) {
-          fs[k] = __shfl_sync(0xffffffffu, f, (k0 + k) & 31);
-          const unsigned long long src = __shfl_sync(0xffffffffu, (unsigned long long)(at * 2 + (line ? 1 : 0)), (k0 + k) & 31);
-          if (k0 + k >= n) fs[k] = 0.f;
-          const float* from = ((src & 1) ? stream.o : p.part_o) + (src >> 1) * HD + lane * V;
+      for (int k = 0; k < N; ++k) {
+        if (ml[k].x == -INFINITY && ml[k].y == 0.f) continue;  // no key: there may be no values either
+        const float f = ex2(ml[k].x - M);
+        L += f * ml[k].y;
 #pragma unroll
-          for (int e = 0; e < V; ++e) v[k][e] = 0.f;
-          if (fs[k] != 0.f) {
-            if constexpr (V == 4)
-              *reinterpret_cast<float4*>(v[k]) = *reinterpret_cast<const float4*>(from);
-            else
-              *reinterpret_cast<float2*>(v[k]) = *reinterpret_cast<const float2*>(from);
-          }
-        }
-#pragma unroll
-        for (int k = 0; k < 8; ++k)
-#pragma unroll
-          for (int e = 0; e < V; ++e) acc[e] += fs[k] * v[k][e];
+        for (int e = 0; e < V; ++e) acc[e] += f * v[k][e];
       }
     }
-#pragma unroll
-    for (int d = 16; d; d >>= 1) L += __shfl_xor_sync(0xffffffffu, L, d);
     if constexpr (WPR > 1) {
 #pragma unroll
       for (int e = 0; e < V; ++e) s_o[warp][lane * V + e] = acc[e];
@@ -760,9 +781,9 @@ struct QuantPlan {
 };
 
 // How a call is cut, as plan_attn (sc_prefix_attn.cu) does, by what the tables hold.  `resident`: CTAs of the few-rows kernel that an
-// SM takes, for tiles of 8 rows and of 16.
+// SM takes, for tiles of 8 rows and of 16; `clusters`: of those that work in clusters.
 static QuantPlan plan_quant_attn(int T, int B, int Hq, int Hkv, int hd, long long own_keys, long long prefix_keys, int sms,
-                                 const int (&resident)[2]) {
+                                 const int (&resident)[2], const int (&clusters)[2]) {
   QuantPlan a{};
   const int G = Hq / Hkv;
   const long long rows = (long long)T * G;
@@ -826,10 +847,15 @@ static QuantPlan plan_quant_attn(int T, int B, int Hq, int Hkv, int hd, long lon
     // of 20000 71 | 54, 64 of 1200 22 | 25, of 5000 72 | 57, 128 of 5000 105 | 101; 4 of 64, 16 of 20000 23 | 24, of 60000 75 | 56).
     a.nslots = 1;
     const long long keys = own_keys + prefix_keys;
-    a.row_groups = (int)std::max(1ll, std::min(ceil_div(2 * slots, (long long)B * Hkv), groups > 1 ? 2 * groups : 1));
-    const long long ctas = (long long)B * Hkv * a.row_groups;
-    const long long once = std::max(1ll, std::min({slots / ctas, ceil_div(keys, 128), (long long)FR_CLUSTER}));
-    if (ctas >= slots ? keys * ctas <= 4500 * slots : keys <= (hd == 128 ? 1600 : 2200) * once) a.splits = (int)once;
+    // Sizes a power of two: 16 requests of up to 800 tokens, 8 kv heads of 128, 1 to 6 and 8 CTAs a cluster: 12.2, 9.9, 11.0, 9.8, 13.9,
+    // 15.2, 16.2 us; as many as run at once, and up to a third more (drafts of up to five tokens, 16 requests behind 1000, 4 kv heads of 64, three tiles
+    // of rows each, 1 to 4: 20.5, 14.1, 19.6, 19.6; 384 CTAs in clusters of two on 296 places).
+    // (CTAs for tiles of rows: those of requests with half as many rows again as the mean)
+    a.row_groups = (int)(a.two ? ceil_div(3 * rows, 2ll * B * 16) : 1);
+    const long long ctas = (long long)B * Hkv * a.row_groups, places = clusters[a.two] * sms;
+    long long once = 1;
+    while (once < FR_CLUSTER && 2 * once * ctas * 3 <= 4 * places && 2 * once <= ceil_div(keys, 64)) once *= 2;
+    if (ctas >= places ? keys * ctas <= 4500 * places : keys <= (hd == 128 ? 1600 : 2200) * once) a.splits = (int)once;
   }
   size_t rows_all = a.nslots > 1 ? (size_t)a.nslots * T * Hq : 0;
   a.o_rows = rows_all;
@@ -846,7 +872,7 @@ static QuantPlan plan_quant_attn(int T, int B, int Hq, int Hkv, int hd, int bits
   with_quant_block(hd, bits, group, [&](auto block) {
     using QB = decltype(block);
     a = plan_quant_attn(T, B, Hq, Hkv, hd, (long long)max_blocks * page_size, (long long)max_prefix_blocks * page_size, sm_count(),
-                        {FewRowsQuant<QB, 1>::CTAS, FewRowsQuant<QB, 2>::CTAS});
+                        {FewRowsQuant<QB, 1>::CTAS, FewRowsQuant<QB, 2>::CTAS}, {FewRowsQuant<QB, 1>::CTAS_CLUSTER, FewRowsQuant<QB, 2>::CTAS_CLUSTER});
     return 0;
   });
   return a;
