@@ -85,8 +85,8 @@ struct ManyRows<HD, QuantSource<QB>> {
   static constexpr bool QUANT = true;
   static constexpr int THREADS = TC_THREADS_QUANT, REGS_CTL = TC_REGS_CTL_QUANT, REGS_SM = TC_REGS_SM_QUANT;
   static constexpr int TILE = TC_N * HD * 2;
-  static constexpr int NBUF = HD == 128 ? 4 : 8;
-  static constexpr int RB = HD == 128 && QB::BITS == 8 ? 2 : 4;  // blocks of 16 tokens to a stage of codes
+  static constexpr int NBUF = HD == 128 ? (QB::BITS == 4 ? 4 : 3) : 8;
+  static constexpr int RB = 4;  // blocks of 16 tokens to a stage of codes
   static constexpr int RAW = RB * QB::BYTES, NRAW = 3, STAGES = 8 / RB;  // stages of a tile
   static constexpr int SMEM = 2 * TILE + NBUF * TILE + NRAW * RAW + 1024;
 };
@@ -349,7 +349,7 @@ struct QuantValues {
   // K at `raw` to the tile's rows from row0 on.
   static __device__ __forceinline__ void keys(uint32_t raw, uint32_t tile, int row0) {
     const int tid = threadIdx.x & 127;
-#pragma unroll
+#pragma unroll 1
     for (int u = 0; u < RB / 2; ++u) {
       const int token = u * 32 + (tid >> 2), t = tid & 3, tok = token & 15, row = row0 + token;
       const uint32_t block = raw + (token >> 4) * QB::BYTES, at = block + tok * QB::ROW + QB::piece_k(tok, t, 0);
@@ -390,7 +390,7 @@ struct QuantValues {
   // V; blocks whose bit in `gone` is set are zero.
   static __device__ __forceinline__ void values(uint32_t raw, uint32_t tile, int row0, uint32_t gone) {
     const int tid = threadIdx.x & 127;
-#pragma unroll
+#pragma unroll 1
     for (int u = 0; u < RB / 2; ++u) {
       const int pair = u * 16 + (tid >> 3), t = tid & 7, pr = pair & 7, row = row0 + 2 * pair;
       const uint32_t block = raw + (pair >> 3) * QB::BYTES, at = block + QB::V + pr * 2 * QB::ROW + QB::piece_v(pr, t, 0);
@@ -455,7 +455,7 @@ __device__ __forceinline__ void quant_writer(int cnt, uint32_t ring_u, uint32_t 
   for (int i = 0; i < cnt; ++i) {
     const uint32_t ki = 2 * i, vi = 2 * i + 1;
     const uint32_t kt = ring_u + (ki % NBUF) * C::TILE, vt = ring_u + (vi % NBUF) * C::TILE;
-    if (!wait(&empty[ki % NBUF], ((ki / NBUF) & 1u) ^ 1u) || !wait(&empty[vi % NBUF], ((vi / NBUF) & 1u) ^ 1u)) return;
+    if (!wait(&empty[ki % NBUF], ((ki / NBUF) & 1u) ^ 1u)) return;
 #pragma unroll 1
     for (int st = 0; st < C::STAGES; ++st, ++it) {
       const int s = it % NRAW, row0 = st * C::RB * 16;
@@ -466,6 +466,7 @@ __device__ __forceinline__ void quant_writer(int cnt, uint32_t ring_u, uint32_t 
         __syncwarp();
         if (lane == 0) mbar_arrive(&full[ki % NBUF]);
       }
+      if (st == 0 && !wait(&empty[vi % NBUF], ((vi / NBUF) & 1u) ^ 1u)) return;
       V::values(raw_u + s * C::RAW, vt, row0, s_absent[i & 15] >> (C::RB * st));
       fence_async_smem();
       __syncwarp();

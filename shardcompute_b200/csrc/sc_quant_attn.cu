@@ -449,7 +449,9 @@ few_rows_quant_kernel(const PrefixAttnParams p, const uint8_t* pages, int with_p
             }
             pb[j][0] = transpose8x8(h2_as_u32(__floats2half2_rn(ps[0], ps[1])));
             pb[j][1] = transpose8x8(h2_as_u32(__floats2half2_rn(ps[2], ps[3])));
-            mma_16816(z[g][j], 0x00010001u, 0x00010001u, 0x00010001u, 0x00010001u, pb[j][0], pb[j][1]);
+            // (1, not 2^-24 as in the codes: the tensor cores cut their sums off 24 bits below what the largest product's exponents
+            // allow, and a subnormal counts as 2^-14 there: of 2^-24 ten bits are left, 2.8e-4 of the output; of the codes 16 and more)
+            mma_16816(z[g][j], 0x3c003c00u, 0x3c003c00u, 0x3c003c00u, 0x3c003c00u, pb[j][0], pb[j][1]);
           }
 #pragma unroll
           for (int w = g * WORDS / NG; w < (g + 1) * WORDS / NG; ++w) {
@@ -490,7 +492,7 @@ few_rows_quant_kernel(const PrefixAttnParams p, const uint8_t* pages, int with_p
 #pragma unroll
         for (int k = 0; k < C::MT; k += 2) {  // four dims in a row: of two tiles of 16, this thread's two rows each
           const int at = 2 * k, g = at / (GS / 8);
-          const float add = fmaf(z[g][j][c], -C::MID * 0x1p24f, bias[j][g][c]);
+          const float add = fmaf(z[g][j][c], -C::MID, bias[j][g][c]);
           float4 v;
           if constexpr (PER == 8)
             v = make_float4(fmaf(o[k][j][c], 0x1p24f, add), fmaf(o[k + 1][j][c] - o[k][j][c], 0x1p20f, add), fmaf(o[k][j][2 + c], 0x1p24f, add),

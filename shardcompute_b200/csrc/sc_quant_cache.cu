@@ -50,16 +50,19 @@ __device__ __forceinline__ float max_nan(float a, float b) {
 template <int MOST>
 __device__ __forceinline__ __half2 scale_bias(float lo, float hi) {
   const __half b = __float2half_rd(lo);
-  const double need = fmax((double)hi - (double)__half2float(b), 0.0);
-  __half s = __float2half_ru((float)need * (1.f / MOST));
-  // the estimate is within a few roundings of fp32: at most one fp16 value off
+  const float fb = __half2float(b);
+  // max x - b as a sum of two fp32 values t + e
+  const float t = __fsub_rn(hi, fb), z = __fsub_rn(t, hi), e = __fsub_rn(__fsub_rn(hi, __fsub_rn(t, z)), __fadd_rn(fb, z));
+  __half s = __float2half_ru(fmaxf(t, 0.f) * (1.f / MOST));
+  // The estimate is within a few roundings of fp32, at most one fp16 value off.  MOST s needs no rounding, nor does its difference to t
+  // where that is near.
   const unsigned short u = __half_as_ushort(s);
-  if ((double)(__half2float(s) * MOST) < need)
+  if (__fsub_rn(__half2float(s) * MOST, t) < e)
     s = __ushort_as_half(u + 1);
-  else if (u > 0 && u <= 0x7c00 && (double)(__half2float(__ushort_as_half(u - 1)) * MOST) >= need)
+  else if (u > 0 && u <= 0x7c00 && __fsub_rn(__half2float(__ushort_as_half(u - 1)) * MOST, t) >= e)
     s = __ushort_as_half(u - 1);
-  const float top = fmaf(__half2float(s), (float)MOST, __half2float(b));
-  return __halves2half2(s, __half2float(b) >= -65504.f && top <= 65504.f ? b : __ushort_as_half(0x7e00));
+  const float top = fmaf(__half2float(s), (float)MOST, fb);
+  return __halves2half2(s, fb >= -65504.f && top <= 65504.f ? b : __ushort_as_half(0x7e00));
 }
 
 // rint((x - b) / s), `inv` about 1 / s.  The quotient in fp32 finds it or a neighbour; which, what is left over says exactly: x - b as
@@ -92,7 +95,7 @@ __global__ void __launch_bounds__(256) append_quant_kernel(const AppendQuantPara
   constexpr int HD = QB::HD, HALF = HD / 2, LPH = HD / 8, NG = QB::NG, GS = QB::GS;
   pdl_trigger();
   pdl_wait();
-  const int end = *p.rows_end;
+  const int end = *p.rows_end;  // on its way together with the rows
   int row[AQ_ITEMS], h[AQ_ITEMS], d[AQ_ITEMS], pos[AQ_ITEMS], slot[AQ_ITEMS];
   bool live[AQ_ITEMS];
   float a[AQ_ITEMS][4], b[AQ_ITEMS][4], c[AQ_ITEMS][4], s[AQ_ITEMS][4];
@@ -102,7 +105,6 @@ __global__ void __launch_bounds__(256) append_quant_kernel(const AppendQuantPara
     live[i] = it < p.items;
     const int r = live[i] ? p.per_row.div(it) : 0, e = it - r * p.per_row.d;
     row[i] = p.row0 + r;
-    live[i] = live[i] && row[i] < end;
     h[i] = e / LPH;
     d[i] = e % LPH * 4;
     pos[i] = slot[i] = -1;
@@ -120,11 +122,13 @@ __global__ void __launch_bounds__(256) append_quant_kernel(const AppendQuantPara
     }
   }
 #pragma unroll
-  for (int i = 0; i < AQ_ITEMS; ++i)
+  for (int i = 0; i < AQ_ITEMS; ++i) {
+    live[i] = live[i] && row[i] < end;
     if (live[i] && h[i] < p.Hq + p.Hkv && pos[i] >= 0 && pos[i] < p.max_pos) {
       load4(p.cos_tab + (size_t)pos[i] * HALF + d[i], c[i]);
       load4(p.sin_tab + (size_t)pos[i] * HALF + d[i], s[i]);
     }
+  }
 #pragma unroll
   for (int i = 0; i < AQ_ITEMS; ++i) {
     const bool is_kv = h[i] >= p.Hq, is_v = h[i] >= p.Hq + p.Hkv;
