@@ -33,8 +33,12 @@ struct FewRowsQuant {
   static constexpr int PER = 32 / QB::BITS;    // codes of a word
   static constexpr float MID = QB::BITS == 4 ? 8.f : 128.f;
   static constexpr int KSTEPS = QB::HD / 16, MT = QB::HD / 16;
-  static constexpr int STAGE = 2 * QB::BYTES;  // two blocks: 32 tokens
-  static constexpr int NST = STAGE > 4000 ? 2 : STAGE > 2400 ? 3 : 4;
+  // Blocks of 16 tokens to a step: two, which share the step's fixed costs; one of the largest blocks, so that four CTAs fit an SM
+  // in place of three (32 requests of up to 3500 tokens, 16 heads of 128, 8 bits: groups of 32 66 -> 52 us; of 64 47 -> 44, but of up to
+  // 1000 tokens 19 -> 22, which is why those stay with two)
+  static constexpr int NBK = QB::BYTES > 4500 ? 1 : 2, KEYS = 16 * NBK;
+  static constexpr int STAGE = NBK * QB::BYTES;
+  static constexpr int NST = NBK == 1 ? 2 : STAGE > 4000 ? 2 : STAGE > 2400 ? 3 : 4;
   static constexpr int OUT = 2 * RT * QB::HD * 4;  // a warp's result, and the CTA's behind it
   static constexpr int RING = NST * STAGE > OUT ? NST * STAGE : OUT;
   static constexpr int QBYTES = NT * KSTEPS * 256;  // q's fragments
@@ -52,25 +56,24 @@ struct StreamArgs {
   float* o;            // [2 CTAs, RT, HD]
   float2* ml;          // [2 CTAs, RT]
 };
-constexpr int FQ_KEYS = 32;         // of a tile
-constexpr int FQ_UNIT = 4;          // tiles that a unit's start and end are worth
-constexpr int FQ_LEAST = 8;         // tiles of a piece, at least
+constexpr int FQ_UNIT = 128;   // keys that a unit's start and end are worth
+constexpr int FQ_LEAST = 256;  // keys of a piece, at least
 
 // A request's tiles of keys (all that some row of it sees, at most), its tiles of rows.
 struct StreamRequest {
   int row_lo, rows, n, len, nt, tiles;
   long long units;
 };
-template <int RT>
+template <int RT, int KEYS>
 __device__ __forceinline__ StreamRequest stream_request(const PrefixAttnParams& p, int b, int np) {
   StreamRequest r;
   int hi;
   request_rows(p, b, r.row_lo, hi, r.n);
   r.rows = (hi - r.row_lo) * p.G;
   r.len = request_len(p, b);
-  r.nt = np + (int)(((long long)r.len + FQ_KEYS - 1) / FQ_KEYS);
+  r.nt = np + (int)(((long long)r.len + KEYS - 1) / KEYS);
   r.tiles = (r.rows + RT - 1) / RT;
-  r.units = (long long)r.tiles * p.Hkv * (r.nt + FQ_UNIT);
+  r.units = (long long)r.tiles * p.Hkv * (r.nt + FQ_UNIT / KEYS);
   return r;
 }
 
@@ -118,7 +121,7 @@ __global__ void __launch_bounds__(FR_WARPS * 32, CLUSTER ? FewRowsQuant<QB, NT>:
 few_rows_quant_kernel(const PrefixAttnParams p, const uint8_t* pages, int with_prefix, int splits, int row_groups, int slot0,
                       const StreamArgs stream) {
   using C = FewRowsQuant<QB, NT>;
-  constexpr int RT = C::RT, NST = C::NST, KT = FQ_KEYS, HD = QB::HD, NG = QB::NG, GS = QB::GS, WORDS = C::WORDS, PER = C::PER;
+  constexpr int RT = C::RT, NST = C::NST, KT = C::KEYS, NBK = C::NBK, HD = QB::HD, NG = QB::NG, GS = QB::GS, WORDS = C::WORDS, PER = C::PER;
   extern __shared__ __align__(128) unsigned char fq_smem[];
   __shared__ __align__(8) uint64_t full[FR_WARPS][NST];
   __shared__ float s_m[FR_WARPS][RT], s_l[FR_WARPS][RT];
@@ -146,11 +149,11 @@ few_rows_quant_kernel(const PrefixAttnParams p, const uint8_t* pages, int with_p
   int s_in = 0, s_out = 0;            // the stage that the next tile goes to, that it comes from
   uint32_t phase = 0, in_flight = 0;  // of s_out's barrier; tiles asked for and not yet waited for
 
-  // The pool's blocks of tiles t0 + step (first .. first + 15) of request b and head h, two lanes a tile; -1: no such page.
+  // The pool's blocks of tiles t0 + step (first .. first + 32 / NBK - 1) of request b and head h, NBK lanes a tile; -1: no such page.
   auto blocks_of = [&](int b, int h, int t0, int step, int first) {
-    const long long t = t0 + (long long)step * (first + (lane >> 1));
+    const long long t = t0 + (long long)step * (first + lane / NBK);
     const bool pre = t < np;
-    const long long key = (pre ? t : t - np) * KT + (lane & 1) * 16;
+    const long long key = (pre ? t : t - np) * KT + lane % NBK * 16;
     const int blk = (int)min(key >> p.lg_page, (long long)INT32_MAX);
     if (blk >= (pre ? p.max_prefix_blocks : p.max_blocks)) return -1;
     const int id = pre ? p.prefix_table[blk] : p.block_table[(size_t)b * p.max_blocks + blk];
@@ -161,12 +164,13 @@ few_rows_quant_kernel(const PrefixAttnParams p, const uint8_t* pages, int with_p
   // Rows r0 .. r0 + nr of request b under this warp's tiles t0 + step i, i < cnt; `own`: own keys that the last of the rows sees.
   // The warps' results go to their rings, (m, l) to s_m and s_l.  False after a wait that ran out.
   auto attend = [&](int b, int h, int row_lo, int n, int len, int r0, int nr, int own, int t0, int step, int cnt, int blocks) {
-    uint32_t absent = 0;  // blocks without a page, two bits per stage
+    constexpr uint32_t ALL = (1u << NBK) - 1;
+    uint32_t absent = 0;  // blocks without a page, NBK bits per stage
     auto issue = [&](int i) {
-      if (i && (i & 15) == 0) blocks = blocks_of(b, h, t0, step, i);
-      const int blk = __shfl_sync(0xffffffffu, blocks, 2 * (i & 15) + (lane & 1));
-      const uint32_t there = __ballot_sync(0xffffffffu, blk >= 0) & 3u;
-      absent = (absent & ~(3u << (2 * s_in))) | ((there ^ 3u) << (2 * s_in));
+      if (i && i % (32 / NBK) == 0) blocks = blocks_of(b, h, t0, step, i);
+      const int blk = __shfl_sync(0xffffffffu, blocks, NBK * (i % (32 / NBK)) + lane % NBK);
+      const uint32_t there = __ballot_sync(0xffffffffu, blk >= 0) & ALL;
+      absent = (absent & ~(ALL << (NBK * s_in))) | ((there ^ ALL) << (NBK * s_in));
       if (lane == 0) {
         if (there)
           mbar_arrive_expect_tx(&full[warp][s_in], (there == 3u ? 2 : 1) * QB::BYTES);
@@ -174,7 +178,7 @@ few_rows_quant_kernel(const PrefixAttnParams p, const uint8_t* pages, int with_p
           mbar_arrive(&full[warp][s_in]);
       }
       __syncwarp();
-      if (lane < 2 && blk >= 0)
+      if (lane < NBK && blk >= 0)
         bulk_load(ring + s_in * C::STAGE + lane * QB::BYTES, pages + (size_t)blk * QB::BYTES, QB::BYTES, &full[warp][s_in]);
       s_in = s_in + 1 == NST ? 0 : s_in + 1;
       ++in_flight;
@@ -264,7 +268,7 @@ few_rows_quant_kernel(const PrefixAttnParams p, const uint8_t* pages, int with_p
     for (int i = 0; i < cnt; ++i) {
       if (!mbar_wait_warp(&full[warp][s_out], phase, &s_abort, PA_WAIT_NS)) return false;
       const uint32_t tile = ring_u + s_out * C::STAGE;
-      const uint32_t gone = (absent >> (2 * s_out)) & 3u;
+      const uint32_t gone = (absent >> (NBK * s_out)) & ALL;
       --in_flight;
       if (++s_out == NST) {
         s_out = 0;
@@ -273,34 +277,34 @@ few_rows_quant_kernel(const PrefixAttnParams p, const uint8_t* pages, int with_p
       const int t = t0 + step * i;
       const int first = (t < np ? t : t - np) * KT;
       const bool part = gone || (t < np ? P : see_first) - first < KT;  // not every row sees every key
-      // ---- S = K Q^T: tokens r8, r8 + 8, r8 + 16, r8 + 24 of the tile by columns 2 q4, 2 q4 + 1
-      float sc[NT][8];
+      // ---- S = K Q^T: tokens r8, r8 + 8 of each block by columns 2 q4, 2 q4 + 1
+      float sc[NT][4 * NBK];
 #pragma unroll
       for (int j = 0; j < NT; ++j)
 #pragma unroll
-        for (int e = 0; e < 8; ++e) sc[j][e] = 0.f;
+        for (int e = 0; e < 4 * NBK; ++e) sc[j][e] = 0.f;
       {
-        uint32_t ka[2][WORDS], kb[2][WORDS];
+        uint32_t ka[NBK][WORDS], kb[NBK][WORDS];
 #pragma unroll
-        for (int k = 0; k < 2; ++k) {
+        for (int k = 0; k < NBK; ++k) {
           const uint32_t block = tile + k * QB::BYTES;
           lds_share<WORDS>(block + k_lane, block + (k_lane ^ 64), ka[k]);
           lds_share<WORDS>(block + k_lane + 8 * QB::ROW, block + (k_lane ^ 64) + 8 * QB::ROW, kb[k]);
         }
 #pragma unroll
         for (int g = 0; g < NG; ++g) {
-          float y[NT][8];
+          float y[NT][4 * NBK];
 #pragma unroll
           for (int j = 0; j < NT; ++j)
 #pragma unroll
-            for (int e = 0; e < 8; ++e) y[j][e] = 0.f;
+            for (int e = 0; e < 4 * NBK; ++e) y[j][e] = 0.f;
 #pragma unroll
           for (int w = g * C::KSTEPS / 2 / NG; w < (g + 1) * C::KSTEPS / 2 / NG; ++w)  // two steps of k
 #pragma unroll
             for (int j = 0; j < NT; ++j) {
               const uint4 q = lds_v4(q_u + ((j * (C::KSTEPS / 2) + w) * 32 + lane) * 16);
 #pragma unroll
-              for (int k = 0; k < 2; ++k) {
+              for (int k = 0; k < NBK; ++k) {
                 float(&z)[4] = *reinterpret_cast<float(*)[4]>(&y[j][4 * k]);
                 if constexpr (PER == 8) {
                   const uint32_t a = ka[k][w], c = kb[k][w];
@@ -316,7 +320,7 @@ few_rows_quant_kernel(const PrefixAttnParams p, const uint8_t* pages, int with_p
               }
             }
 #pragma unroll
-          for (int k = 0; k < 2; ++k) {
+          for (int k = 0; k < NBK; ++k) {
             const float2 x0 = __half22float2(u32_as_h2(lds_u32(tile + k * QB::BYTES + QB::KM + meta_lane + 4 * g)));
             const float2 x1 = __half22float2(u32_as_h2(lds_u32(tile + k * QB::BYTES + QB::KM + meta_lane + 32 * NG + 4 * g)));
 #pragma unroll
@@ -329,7 +333,7 @@ few_rows_quant_kernel(const PrefixAttnParams p, const uint8_t* pages, int with_p
           }
         }
       }
-      uint32_t hidden = 0;  // bit 8 j + e
+      uint32_t hidden = 0;  // bit 4 NBK j + e
       if (part) {
 #pragma unroll
         for (int j = 0; j < NT; ++j)
@@ -338,18 +342,18 @@ few_rows_quant_kernel(const PrefixAttnParams p, const uint8_t* pages, int with_p
             const int r = j * 8 + 2 * q4 + c;  // rows past the last see what the last does
             const int lim = (t < np ? P : r < nr ? max(0, min(len, len - n + (r0 + r) / p.G + 1)) : own) - first;
 #pragma unroll
-            for (int e = c; e < 8; e += 2)
+            for (int e = c; e < 4 * NBK; e += 2)
               if (r8 + (e >> 1) * 8 >= lim || (gone >> (e >> 2)) & 1u) {
-                hidden |= 1u << (8 * j + e);
+                hidden |= 1u << (4 * NBK * j + e);
                 sc[j][e] = -INFINITY;
               }
           }
       }
       // ---- V's scales and biases; log2 of a bound of each token's largest scale
-      uint32_t mv[4][NG];
-      float lg[4];
+      uint32_t mv[2 * NBK][NG];
+      float lg[2 * NBK];
 #pragma unroll
-      for (int k = 0; k < 4; ++k) {
+      for (int k = 0; k < 2 * NBK; ++k) {
         lds_words<NG>(tile + (k >> 1) * QB::BYTES + QB::VM + meta_lane + (k & 1) * 32 * NG, mv[k]);
         float big = 0x1p-24f;
 #pragma unroll
@@ -364,8 +368,9 @@ few_rows_quant_kernel(const PrefixAttnParams p, const uint8_t* pages, int with_p
       for (int j = 0; j < NT; ++j)
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
-          x[j][c] = fmaxf(fmaxf(fmaf(sc[j][c], cq[j][c], lg[0]), fmaf(sc[j][2 + c], cq[j][c], lg[1])),
-                          fmaxf(fmaf(sc[j][4 + c], cq[j][c], lg[2]), fmaf(sc[j][6 + c], cq[j][c], lg[3])));
+          x[j][c] = fmaxf(fmaf(sc[j][c], cq[j][c], lg[0]), fmaf(sc[j][2 + c], cq[j][c], lg[1]));
+          if constexpr (NBK == 2)
+            x[j][c] = fmaxf(x[j][c], fmaxf(fmaf(sc[j][4 * NBK - 4 + c], cq[j][c], lg[2 * NBK - 2]), fmaf(sc[j][4 * NBK - 2 + c], cq[j][c], lg[2 * NBK - 1])));
           up |= x[j][c] > m[j][c] + (PA_LIFT + PA_RAISE);
         }
       if (__any_sync(0xffffffffu, up)) {
@@ -404,7 +409,7 @@ few_rows_quant_kernel(const PrefixAttnParams p, const uint8_t* pages, int with_p
 #pragma unroll
         for (int j = 0; j < NT; ++j)
 #pragma unroll
-          for (int e = 0; e < 8; ++e) {
+          for (int e = 0; e < 4 * NBK; ++e) {
             const float mm = m[j][e & 1] == -INFINITY ? 0.f : m[j][e & 1];
             float d = fmaf(sc[j][e], cq[j][e & 1], -mm);
             if constexpr (is_far)
@@ -419,7 +424,7 @@ few_rows_quant_kernel(const PrefixAttnParams p, const uint8_t* pages, int with_p
         weights(std::false_type{});
       // ---- O += V^T (P s)^T, and the biases' part
 #pragma unroll
-      for (int k = 0; k < 2; ++k) {
+      for (int k = 0; k < NBK; ++k) {
         const uint32_t block = tile + k * QB::BYTES + v_lane;
         uint32_t va[WORDS], vb[WORDS];  // pairs of tokens q4 and q4 + 4
         lds_share<WORDS>(block, block + 128, va);
@@ -436,7 +441,7 @@ few_rows_quant_kernel(const PrefixAttnParams p, const uint8_t* pages, int with_p
             if (part) {  // what is hidden may be an infinity or NaN
 #pragma unroll
               for (int e = 0; e < 4; ++e) {
-                const bool out = hidden >> (8 * j + 4 * k + e) & 1u;
+                const bool out = hidden >> (4 * (NBK * j + k) + e) & 1u;
                 ps[e] = out ? 0.f : sc[j][4 * k + e] * (e < 2 ? v0.x : v1.x);
                 bias[j][g][e & 1] += out ? 0.f : sc[j][4 * k + e] * (e < 2 ? v0.y : v1.y);
               }
@@ -566,7 +571,7 @@ few_rows_quant_kernel(const PrefixAttnParams p, const uint8_t* pages, int with_p
     // ---- where the requests lie on the line: each thread a run of them, then a scan
     const int per = (p.B + FR_WARPS * 32 - 1) / (FR_WARPS * 32), b0 = min(p.B, (int)threadIdx.x * per), b1 = min(p.B, b0 + per);
     long long sum = 0;
-    for (int b = b0; b < b1; ++b) sum += stream_request<RT>(p, b, np).units;
+    for (int b = b0; b < b1; ++b) sum += stream_request<RT, KT>(p, b, np).units;
     long long upto = sum;
 #pragma unroll
     for (int d = 1; d < 32; d <<= 1) {
@@ -580,20 +585,20 @@ few_rows_quant_kernel(const PrefixAttnParams p, const uint8_t* pages, int with_p
       if (w < warp) at += s_sum[w];
       all += s_sum[w];
     }
-    const long long quantum = max((all + gridDim.x - 1) / gridDim.x, (long long)FQ_LEAST);
+    const long long quantum = max((all + gridDim.x - 1) / gridDim.x, (long long)(FQ_LEAST / KT));
     const long long lo = blockIdx.x * quantum, hi = min(all, lo + quantum);
     if (blockIdx.x == 0) {
       long long x = at;
       for (int b = b0; b < b1; ++b) {
         stream.offsets[b] = x;
-        x += stream_request<RT>(p, b, np).units;
+        x += stream_request<RT, KT>(p, b, np).units;
       }
       if (threadIdx.x == 0) stream.offsets[p.B] = quantum;
     }
     if (lo >= at && lo < at + sum) {
       int b = b0;
       for (; b < b1; ++b) {
-        const long long u = stream_request<RT>(p, b, np).units;
+        const long long u = stream_request<RT, KT>(p, b, np).units;
         if (lo < at + u) break;
         at += u;
       }
@@ -604,17 +609,17 @@ few_rows_quant_kernel(const PrefixAttnParams p, const uint8_t* pages, int with_p
     // ---- the CTA's piece of the line, unit by unit
     long long pos = lo, off = lo < hi ? s_at : 0;
     int b = lo < hi ? s_b : 0;
-    StreamRequest q = stream_request<RT>(p, b, np);
+    StreamRequest q = stream_request<RT, KT>(p, b, np);
     int unit = 0;
     bool fresh = true;
     while (pos < hi) {
       if (pos >= off + q.units) {
         off += q.units;
-        q = stream_request<RT>(p, ++b, np);
+        q = stream_request<RT, KT>(p, ++b, np);
         unit = 0;
         continue;
       }
-      const int u = q.nt + FQ_UNIT;
+      const int u = q.nt + FQ_UNIT / KT;
       if (fresh) {  // the first unit
         unit = (int)((pos - off) / u);
         fresh = false;
@@ -670,13 +675,13 @@ few_rows_quant_kernel(const PrefixAttnParams p, const uint8_t* pages, int with_p
 // unit on the line.  WPR warps to a (row, head), which read every WPR-th of them (few rows have many), eight of them in flight,
 // each with its (m, l); a block's rows are of one request.  Bound by latency: what does not hang on the results is asked for
 // while the kernel before still runs.
-template <int HD, int RT, int WPR>
+template <int HD, int RT, int KT, int WPR>
 __global__ void __launch_bounds__(256) join_stream_kernel(const PrefixAttnParams p, const StreamArgs stream, int with_prefix, int tc) {
   constexpr int V = HD / 32, ROWS = 8 / WPR, N = 8;
   __shared__ float s_o[WPR > 1 ? 8 : 1][HD];
   __shared__ float2 s_ml[WPR > 1 ? 8 : 1];
   const int b = blockIdx.x, warp = threadIdx.x >> 5, lane = threadIdx.x & 31, part = warp % WPR, P = with_prefix ? prefix_keys(p) : 0;
-  const StreamRequest q = stream_request<RT>(p, b, (int)(((long long)P + FQ_KEYS - 1) / FQ_KEYS));
+  const StreamRequest q = stream_request<RT, KT>(p, b, (int)(((long long)P + KT - 1) / KT));
   pdl_wait();
   pdl_trigger();
   const long long off = stream.offsets[b], quantum = stream.offsets[p.B];
@@ -686,7 +691,7 @@ __global__ void __launch_bounds__(256) join_stream_kernel(const PrefixAttnParams
     const bool live = i < q.rows * p.Hkv;
     const int h = live ? i / q.rows : 0, r = live ? i - h * q.rows : 0;
     const size_t row = (size_t)(q.row_lo + r / p.G) * p.Hq + h * p.G + r % p.G;
-    const long long start = off + ((long long)h * q.tiles + r / RT) * (q.nt + FQ_UNIT);
+    const long long start = off + ((long long)h * q.tiles + r / RT) * (q.nt + FQ_UNIT / KT);
     const int c0 = (int)(start / quantum), shares = q.nt ? (int)((start + q.nt - 1) / quantum) - c0 + 1 : 1;
     // a unit that one CTA had lies in slot tc, or was written already
     const int all = live ? tc + (shares > 1 ? shares : tc > 0 ? 1 : 0) : 0;
@@ -784,7 +789,7 @@ struct QuantPlan {
 
 // How a call is cut, as plan_attn (sc_prefix_attn.cu) does, by what the tables hold.  `resident`: CTAs of the few-rows kernel that an
 // SM takes, for tiles of 8 rows and of 16; `clusters`: of those that work in clusters.
-static QuantPlan plan_quant_attn(int T, int B, int Hq, int Hkv, int hd, long long own_keys, long long prefix_keys, int sms,
+static QuantPlan plan_quant_attn(int T, int B, int Hq, int Hkv, int hd, int bits, long long own_keys, long long prefix_keys, int sms,
                                  const int (&resident)[2], const int (&clusters)[2]) {
   QuantPlan a{};
   const int G = Hq / Hkv;
@@ -843,8 +848,8 @@ static QuantPlan plan_quant_attn(int T, int B, int Hq, int Hkv, int hd, long lon
     const long long n = items * Hkv * a.tc_splits;
     if (n < sms) line_sms = std::max(sms / 4, sms - (int)n);
   } else {
-    // Clusters of up to eight CTAs, which join their shares in place, while a share is short: up to 1600 keys (heads of 64: 2200) of the longest
-    // request there may be, or, with more requests than CTA slots, 4500 keys a slot; past that pieces of the line and a join (us in a graph,
+    // Clusters of up to eight CTAs, which join their shares in place, while a share is short: up to 1800 keys (heads of 64: 2200) of the longest
+    // request there may be, or, with more requests than CTA slots, 4500 keys a slot (8 bits: 2700); past that pieces of the line and a join (us in a graph,
     // requests of any length up to the longest, cluster | line: 8 kv heads of 128, one of 5000 9 | 14, of 20000 22 | 17, 16 of 5000 22 | 23,
     // of 20000 71 | 54, 64 of 1200 22 | 25, of 5000 72 | 57, 128 of 5000 105 | 101; 4 of 64, 16 of 20000 23 | 24, of 60000 75 | 56).
     a.nslots = 1;
@@ -857,7 +862,7 @@ static QuantPlan plan_quant_attn(int T, int B, int Hq, int Hkv, int hd, long lon
     const long long ctas = (long long)B * Hkv * a.row_groups, places = clusters[a.two] * sms;
     long long once = 1;
     while (once < FR_CLUSTER && 2 * once * ctas * 3 <= 4 * places && 2 * once <= ceil_div(keys, 64)) once *= 2;
-    if (ctas >= places ? keys * ctas <= 4500 * places : keys <= (hd == 128 ? 1600 : 2200) * once) a.splits = (int)once;
+    if (ctas >= places ? keys * ctas <= (bits == 4 ? 4500 : 2700) * places : keys <= (hd == 128 ? 1800 : 2200) * once) a.splits = (int)once;
   }
   size_t rows_all = a.nslots > 1 ? (size_t)a.nslots * T * Hq : 0;
   a.o_rows = rows_all;
@@ -873,7 +878,7 @@ static QuantPlan plan_quant_attn(int T, int B, int Hq, int Hkv, int hd, int bits
   QuantPlan a;
   with_quant_block(hd, bits, group, [&](auto block) {
     using QB = decltype(block);
-    a = plan_quant_attn(T, B, Hq, Hkv, hd, (long long)max_blocks * page_size, (long long)max_prefix_blocks * page_size, sm_count(),
+    a = plan_quant_attn(T, B, Hq, Hkv, hd, bits, (long long)max_blocks * page_size, (long long)max_prefix_blocks * page_size, sm_count(),
                         {FewRowsQuant<QB, 1>::CTAS, FewRowsQuant<QB, 2>::CTAS}, {FewRowsQuant<QB, 1>::CTAS_CLUSTER, FewRowsQuant<QB, 2>::CTAS_CLUSTER});
     return 0;
   });
@@ -883,7 +888,7 @@ static QuantPlan plan_quant_attn(int T, int B, int Hq, int Hkv, int hd, int bits
 template <typename QB, int NT, bool CLUSTER>
 static int run_few_rows_quant(const PrefixAttnParams& p, const uint8_t* pages, const QuantPlan& a, const StreamArgs& line, cudaStream_t stream) {
   constexpr auto kern = few_rows_quant_kernel<QB, NT, CLUSTER>;
-  constexpr int smem = FewRowsQuant<QB, NT>::SMEM;
+  constexpr int smem = FewRowsQuant<QB, NT>::SMEM, KEYS = FewRowsQuant<QB, NT>::KEYS;
   const cudaError_t e = opt_in<kern>(smem);
   if (e != cudaSuccess) return check_launch("prefix_attn_q", e);
   launch_clusters(CLUSTER ? a.splits : 1, kern, CLUSTER ? dim3(a.splits * a.row_groups, p.Hkv, p.B) : dim3(a.ctas), dim3(FR_WARPS * 32), smem,
@@ -893,7 +898,7 @@ static int run_few_rows_quant(const PrefixAttnParams& p, const uint8_t* pages, c
   const long long rows = (long long)p.T * p.Hq;
   const bool wide = a.ctas >= 8 * a.units;  // each unit in eight pieces or more, if all are alike
   const long long y = std::min(std::max(16ll * sm_count() / p.B, 64ll), ((wide ? rows : rows / 8) * 2 + p.B - 1) / p.B);  // twice the mean: requests differ
-  launch(wide ? join_stream_kernel<QB::HD, 8 * NT, 8> : join_stream_kernel<QB::HD, 8 * NT, 1>, dim3(p.B, (unsigned)std::max(1ll, y)), dim3(256), 0, stream, p, line,
+  launch(wide ? join_stream_kernel<QB::HD, 8 * NT, KEYS, 8> : join_stream_kernel<QB::HD, 8 * NT, KEYS, 1>, dim3(p.B, (unsigned)std::max(1ll, y)), dim3(256), 0, stream, p, line,
          a.kind == AttnPlan::FEW ? 1 : 0, a.kind == AttnPlan::SHARED ? a.tc_splits : 0);
   return check_launch("prefix_attn_q_join");
 }
