@@ -45,7 +45,7 @@ struct FewRowsQuant {
   static constexpr int SMEM = FR_WARPS * RING + QBYTES;
   // CTAs of an SM, by shared memory and by the registers that they need without spills
   static constexpr int CTAS = NT == 1 ? (SMEM > 56000 ? 3 : SMEM > 44000 || QB::NG == 4 ? 4 : 5) : QB::NG == 4 || SMEM > 75000 ? 2 : 3;
-  static constexpr int CTAS_CLUSTER = NT == 1 ? (CTAS < 4 ? CTAS : 4) : 2;
+  static constexpr int CTAS_CLUSTER = NT == 1 ? (CTAS < 4 ? CTAS : QB::NG == 4 ? 3 : 4) : 2;
 };
 
 // Work of the CTAs where a grid of requests would leave them uneven: the (request, kv head, tile of rows) follow one another on
@@ -55,6 +55,7 @@ struct StreamArgs {
   long long* offsets;  // [B + 1]: where each request's units begin, and the quantum behind them: written by CTA 0, for the join
   float* o;            // [2 CTAs, RT, HD]
   float2* ml;          // [2 CTAs, RT]
+  int ctas;
 };
 constexpr int FQ_UNIT = 128;   // keys that a unit's start and end are worth
 constexpr int FQ_LEAST = 256;  // keys of a piece, at least
@@ -136,7 +137,8 @@ few_rows_quant_kernel(const PrefixAttnParams p, const uint8_t* pages, int with_p
   if (threadIdx.x == 0) {
     for (int w = 0; w < FR_WARPS; ++w)
       for (int s = 0; s < NST; ++s) mbar_init(&full[w][s], 1);
-    s_abort = 0;
+    s_abort = s_b = 0;
+    s_at = 0;
     fence_mbar_init();
   }
   __syncthreads();
@@ -615,7 +617,8 @@ few_rows_quant_kernel(const PrefixAttnParams p, const uint8_t* pages, int with_p
     while (pos < hi) {
       if (pos >= off + q.units) {
         off += q.units;
-        q = stream_request<RT, KT>(p, ++b, np);
+        if (++b >= p.B) break;  // (offsets in q_start that cannot be, and their sums, lead nowhere)
+        q = stream_request<RT, KT>(p, b, np);
         unit = 0;
         continue;
       }
@@ -629,6 +632,7 @@ few_rows_quant_kernel(const PrefixAttnParams p, const uint8_t* pages, int with_p
       const int at = unit;
       if (tb == u) ++unit;
       if (ta > 0 && ta >= q.nt) continue;  // nothing left of it
+      if (at < 0 || at >= q.tiles * p.Hkv) break;
       const int h = at / q.tiles, r0 = (at - h * q.tiles) * RT, nr = min(RT, q.rows - r0);
       const int own = max(0, min(q.len, q.len - q.n + (r0 + nr - 1) / p.G + 1));
       const int end = min(tb, np + (own + KT - 1) / KT), t0 = ta + warp;
@@ -692,7 +696,8 @@ __global__ void __launch_bounds__(256) join_stream_kernel(const PrefixAttnParams
     const int h = live ? i / q.rows : 0, r = live ? i - h * q.rows : 0;
     const size_t row = (size_t)(q.row_lo + r / p.G) * p.Hq + h * p.G + r % p.G;
     const long long start = off + ((long long)h * q.tiles + r / RT) * (q.nt + FQ_UNIT / KT);
-    const int c0 = (int)(start / quantum), shares = q.nt ? (int)((start + q.nt - 1) / quantum) - c0 + 1 : 1;
+    const int c0 = (int)(start / quantum), last = q.nt ? (int)((start + q.nt - 1) / quantum) : c0, shares = last - c0 + 1;
+    if (c0 < 0 || last < c0 || last >= stream.ctas) break;  // as there
     // a unit that one CTA had lies in slot tc, or was written already
     const int all = live ? tc + (shares > 1 ? shares : tc > 0 ? 1 : 0) : 0;
     float acc[V], L = 0.f, M = -INFINITY;
@@ -848,7 +853,7 @@ static QuantPlan plan_quant_attn(int T, int B, int Hq, int Hkv, int hd, int bits
     const long long n = items * Hkv * a.tc_splits;
     if (n < sms) line_sms = std::max(sms / 4, sms - (int)n);
   } else {
-    // Clusters of up to eight CTAs, which join their shares in place, while a share is short: up to 1800 keys (heads of 64: 2200) of the longest
+    // Clusters of up to eight CTAs, which join their shares in place, while a share is short: up to 1800 keys (8 bits: 1600, heads of 64: 2200) of the longest
     // request there may be, or, with more requests than CTA slots, 4500 keys a slot (8 bits: 2700); past that pieces of the line and a join (us in a graph,
     // requests of any length up to the longest, cluster | line: 8 kv heads of 128, one of 5000 9 | 14, of 20000 22 | 17, 16 of 5000 22 | 23,
     // of 20000 71 | 54, 64 of 1200 22 | 25, of 5000 72 | 57, 128 of 5000 105 | 101; 4 of 64, 16 of 20000 23 | 24, of 60000 75 | 56).
@@ -862,7 +867,7 @@ static QuantPlan plan_quant_attn(int T, int B, int Hq, int Hkv, int hd, int bits
     const long long ctas = (long long)B * Hkv * a.row_groups, places = clusters[a.two] * sms;
     long long once = 1;
     while (once < FR_CLUSTER && 2 * once * ctas * 3 <= 4 * places && 2 * once <= ceil_div(keys, 64)) once *= 2;
-    if (ctas >= places ? keys * ctas <= (bits == 4 ? 4500 : 2700) * places : keys <= (hd == 128 ? 1800 : 2200) * once) a.splits = (int)once;
+    if (ctas >= places ? keys * ctas <= (bits == 4 ? 4500 : 2700) * places : keys <= (hd == 64 ? 2200 : bits == 4 ? 1800 : 1600) * once) a.splits = (int)once;
   }
   size_t rows_all = a.nslots > 1 ? (size_t)a.nslots * T * Hq : 0;
   a.o_rows = rows_all;
@@ -974,7 +979,7 @@ int sc_prefix_attn_q(const void* q, const void* pages, int bits, int group, int 
   p.part_o = static_cast<float*>(workspace);
   // values of all rows, of the line; then (m, l) of both; then the line's offsets
   p.part_ml = reinterpret_cast<float2*>(p.part_o + a.ml_rows * hd);
-  const StreamArgs line = {reinterpret_cast<long long*>(p.part_ml + a.ml_rows), p.part_o + a.o_rows * hd, p.part_ml + a.o_rows};
+  const StreamArgs line = {reinterpret_cast<long long*>(p.part_ml + a.ml_rows), p.part_o + a.o_rows * hd, p.part_ml + a.o_rows, a.ctas};
   p.q_start = q_start;
   p.kv_lens = kv_lens;
   p.block_table = block_table;

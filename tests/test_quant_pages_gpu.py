@@ -530,3 +530,115 @@ def test_attn_pages_of_any_size(cuda, rng):
         for lens, new, prefix in (([200, 33], [1, 1], 100), ([200, 133], [150, 130], 100)):
             d = make_attn(rng, 8, 2, 64, page, 8, 64, prefix, lens, new, dirty=page < 1000)
             check_attn(cuda, d, 8, rounded=True)
+
+
+# ------------------------------------------------------------------------------------------------ cut otherwise than usual
+
+@pytest.mark.parametrize("hd,bits,group", [(64, 4, 64), (64, 8, 32), (128, 4, 64), (128, 8, 64), (128, 8, 32)])
+@pytest.mark.parametrize("drafts", [False, True])
+def test_attn_pieces_of_long_requests(cuda, rng, hd, bits, group, drafts):
+    """Lengths from nothing to thousands: CTAs that take the end of one request, all of others, and the start of one more; the
+    same bits every time."""
+    B, hq, hkv = (24, 8, 2) if drafts else (26, 8, 8)
+    new = [int(x) for x in rng.integers(0, 9, B)] if drafts else [int(x) for x in rng.integers(0, 2, B)]
+    lens = [n + int(x) for n, x in zip(new, np.where(rng.random(B) < 0.5, rng.integers(0, 40, B), rng.integers(0, 1500, B)))]
+    new[3], lens[3], new[5], lens[5] = 1, 0, 1, 1  # a row that sees nothing, a row that sees one token
+    lens[0], new[0] = 9000, 1
+    for prefix in (0, 60):
+        d = make_attn(rng, hq, hkv, hd, 32, bits, group, prefix, lens, new, dirty=False)
+        out = check_attn(cuda, d, hq)
+        for _ in range(3):
+            assert torch.equal(out, run_attn(cuda, d))
+
+
+@pytest.mark.parametrize("prefix,new,rows", [(0, [3, 5, 2], 7), (77, [1, 1, 1], 2), (0, [9, 150, 70], 100), (300, [150, 150], 299),
+                                             (9000, [1] * 40 + [4], 42), (40, [20, 0, 7], 20), (0, [4, 4], 1), (0, [1] * 30, 17)])
+def test_q_ends_before_the_last_request(cuda, rng, prefix, new, rows):
+    """Fewer rows of q than were reserved: the rows that are there see what they see in the whole call."""
+    hq, hkv, hd = 8, 2, 64
+    d = make_attn(rng, hq, hkv, hd, 16, 4, 32, prefix, [n + (5000 if len(new) == 30 else 30) for n in new], new, pad=0, dirty=len(new) < 30)
+    want, mass, dot, keys, tail = (x[:rows] for x in oq.attention(d["q"].double().numpy(), d["data"], d["start"], d["lens"], d["table"], d["ptab"],
+                                                                  prefix, hq, hd, 16, 4, 32, 1 / math.sqrt(hd)))
+    d["q"] = d["q"][:rows].contiguous()
+    got = run_attn(cuda, d).double().cpu().numpy().reshape(want.shape)
+    assert (np.abs(got - want) <= attn_bound(want, mass, dot, keys, tail, hd, rounded=True)).all()
+    assert L.load().sc_prefix_attn_device_error(1) == 0
+
+
+def test_offsets_that_cannot_be(cuda, rng):
+    """Rows and lengths on the device that no reservation writes: whatever comes out, nothing is read or written out of bounds
+    (offsets that fall and pass the rows, lengths below zero and past the tables, pages that are none) and the next call is as
+    before."""
+    for lens, new, prefix in (([30, 25, 9, 40], [1, 1, 1, 1], 20), ([6000] * 4, [1, 1, 1, 1], 20), ([300, 200, 150, 90], [150, 100, 100, 64], 20),
+                              ([30] * 4, [1, 1, 1, 1], 40000)):
+        d = make_attn(rng, 8, 2, 64, 16, 4, 32, prefix, lens, new, dirty=False)
+        clean = run_attn(cuda, d)
+        guard = torch.full((clean.numel() + 4096,), 5.0, dtype=torch.float16, device=cuda)
+        out = guard[:clean.numel()].view(clean.shape)
+        odd = dict(d, start=np.array([0, 10**6, -5, 2**31 - 1, 3]), lens=np.array([-7, 2**31 - 1, 0, -(2**31)]), table=d["table"].copy())
+        odd["table"][:, 0] = [-1, 2**31 - 1, -(2**31), 10**6]
+        run_attn(cuda, odd, out=out)
+        run_attn(cuda, dict(odd, prefix=2**31 - 1), out=out)
+        run_attn(cuda, dict(odd, prefix=-4), out=out)
+        torch.cuda.synchronize()
+        assert (guard[clean.numel():] == 5.0).all()
+        assert torch.equal(run_attn(cuda, d), clean)
+
+
+def test_two_graphs_share_a_workspace(cuda, rng):
+    """Captured calls of other shapes and plans with one workspace, replayed in turn on one stream."""
+    ds = [make_attn(rng, 8, 2, 128, 16, 4, 64, 900, [40, 90, 33], [1, 1, 1]), make_attn(rng, 4, 1, 64, 32, 8, 32, 3000, [700], [2]),
+          make_attn(rng, 8, 4, 64, 32, 4, 64, 0, [20000] + [50] * 20, [1] * 21, dirty=False),
+          make_attn(rng, 32, 4, 64, 32, 4, 32, 2900, [20] * 48, [1] * 48, dirty=False)]
+    ws, calls = torch.empty(64 << 20, dtype=torch.uint8, device=cuda), []
+    for d in ds:
+        t = [d["q"].to(cuda), pool(d, cuda), i32(d["start"], cuda), i32(d["lens"], cuda), i32(d["table"], cuda)]
+        pre = dict(prefix_table=i32(d["ptab"], cuda), prefix_len=i32([d["prefix"]], cuda))
+        want, out = ops.prefix_attn_q(*t, **pre), torch.zeros_like(t[0])
+        graph = torch.cuda.CUDAGraph()
+        torch.cuda.synchronize()
+        with torch.cuda.graph(graph):
+            ops.prefix_attn_q(*t, out=out, workspace=ws, **pre)
+        calls.append((graph, out, want, (t, pre)))
+    for _ in range(3):
+        for graph, out, _, _ in calls:
+            out.zero_()
+            graph.replay()
+        for _, out, want, _ in calls:
+            assert torch.equal(out, want)
+
+
+def test_workspace_that_is_too_small(cuda, rng):
+    d = make_attn(rng, 8, 4, 64, 32, 4, 64, 0, [20000] + [50] * 20, [1] * 21, dirty=False)
+    need = ops.prefix_attn_q_workspace_bytes(23, 21, 8, 4, 64, d["table"].shape[1], 1, 32)
+    assert need > 0
+    with pytest.raises(ValueError, match="workspace"):
+        run_attn(cuda, d, workspace=torch.empty(need - 16, dtype=torch.uint8, device=cuda))
+    assert torch.equal(run_attn(cuda, d), run_attn(cuda, d, workspace=torch.empty(need, dtype=torch.uint8, device=cuda)))
+
+
+def test_many_requests(cuda):
+    """More requests than threads of a CTA, most without a row, a few long: against the same requests alone."""
+    B, hd, page, hq, hkv = 1000, 64, 16, 4, 2
+    g = torch.Generator(device=cuda).manual_seed(5)
+    lens = torch.full((B,), 16, dtype=torch.int32, device=cuda)
+    lens[::97] = 4000
+    blocks = 250
+    n_pages = B // 97 * blocks + 2 * blocks
+    pages = ops.quant_pages(n_pages, hkv, page, hd, 4, 64, cuda)
+    one = torch.ones(n_pages * page, hd // 2, device=cuda)
+    at = torch.arange(n_pages * page, dtype=torch.int32, device=cuda)
+    x = torch.randn(n_pages * page, (1 + 2 * hkv) * hd, device=cuda, generator=g)
+    ops.paged_rope_append_q(x, i32([0, len(at)], cuda), at, at, one, one * 0, torch.empty(len(at), hd, dtype=torch.float16, device=cuda), pages)
+    table = torch.randint(0, n_pages, (B, blocks), dtype=torch.int32, device=cuda, generator=g)
+    new = torch.zeros(B, dtype=torch.int32, device=cuda)
+    new[::97] = 1
+    new[5::50] = 1
+    start = torch.cat([new.new_zeros(1), new.cumsum(0).int()])
+    rows = int(start[-1])
+    q = torch.randn(rows, hq * hd, device=cuda, generator=g).half()
+    out = ops.prefix_attn_q(q, pages, start, lens, table)
+    for r, b in enumerate(new.nonzero().flatten().tolist()):
+        alone = ops.prefix_attn_q(q[r:r + 1].contiguous(), pages, i32([0, 1], cuda), lens[b:b + 1].contiguous(), table[b:b + 1].contiguous())
+        # two ways to cut the same sums: weights rounded by up to 2^-11 of each about another reference, outputs by 2^-11
+        assert (out[r] - alone[0]).abs().max() <= 2.0**-9 * 4
