@@ -359,8 +359,8 @@ int sc_prefix_attn(const void* q, const void* k_pages, const void* v_pages, int 
  * a bias b (fp16) that stand for s c + b:
  *   b = min x rounded down, s = the smallest fp16 value with (2^bits - 1) s >=
  *   max x - b, c = rint((x - b) / s), 0 where s is 0: at most s / 2 off x.
- * A group that holds a value that is not finite, below -65504 or too far above
- * 65504 for s stands for NaN.
+ * A group that holds a value that is not finite or below -65504, or whose
+ * largest code would stand for more than 65504, stands for NaN.
  *   hd 64 or 128; bits 4 or 8; group 32 or 64.
  * Pages [n_pages, Hkv, sc_quant_page_bytes] of bytes, in blocks of 16 tokens
  * whose order is the kernels' own (csrc/sc_quant.cuh); sc_paged_reserve and
@@ -384,7 +384,9 @@ int sc_paged_read_q(const void* pages, int bits, int group, int n_pages, int pag
  * power of two, 16 to 32768; 0 < scale < 5e28.  The products take the codes
  * as they are; scores, softmax statistics and sums are fp32; weights times
  * scales are rounded to fp16 before their product with v's codes: 2^-11 of each,
- * down to 2^-25 of the row's largest.  A group that stands for NaN makes the
+ * down to 2^-25 of the row's largest.  Where many rows share keys (a prefix, a
+ * long chunk) what k and v stand for is rounded to fp16 instead, 2^-11 of each,
+ * and the rest is as for a cache in fp16.  A group that stands for NaN makes the
  * rows that see it NaN (of v: its dims), and no others. */
 size_t sc_prefix_attn_q_workspace_bytes(int T, int B, int Hq, int Hkv, int hd, int bits, int group, int max_blocks,
                                         int max_prefix_blocks, int page_size);

@@ -27,8 +27,8 @@ namespace sc {
 // n0, which saves the masks of n1.
 //
 // q is scaled per row by a power of two so that its largest value is in
-// [2^11, 2^12): exact, and the 1/16 that the codes at 2^-20 need loses nothing.  Its
-// fragments lie in shared memory: in registers they kept a fifth CTA from the SM.
+// [2^11, 2^12): exact, with the 1/16 that the codes at 2^-20 need, but for what is below 2^-32
+// of that largest.  Its fragments lie in shared memory: in registers they kept a fifth CTA from the SM.
 // The weights p s are rounded to fp16, 2^11 to 2^15 high at the row's largest p s
 // (PA_LIFT over c s + log2 of the token's largest scale): 2^-11 of each, the
 // output's own rounding, down to 2^-25 of that largest.  Their error meets c - MID, not c,
@@ -36,9 +36,9 @@ namespace sc {
 // and bias are two large numbers of different signs (3.2e-4 of the output for one key, now
 // 2.1e-4, 2.07e-4 of it the output's rounding).
 //
-// Two requests of 140000 tokens together, 8 kv heads of 128, 4 bits: 161 MB in 39 us, with the
-// join 43: the loop at 5.9 TB/s, and 15 us of starts (lengths, page ids, first blocks, one after
-// another) and ends.  Four requests behind 700 tokens 7.5 us, latency.
+// Two requests of 140000 tokens together, 8 kv heads of 128, 4 bits: 161 MB in 43 us with the
+// join; twice the tokens take 30 us more (5.9 TB/s), so 15 us are starts (lengths, page ids,
+// first blocks, one after another) and ends.  Four requests behind 700 tokens 7.5 us, latency.
 template <typename QB, int NT>
 struct FewRowsQuant {
   static constexpr int RT = 8 * NT;            // rows of a tile
@@ -244,7 +244,7 @@ few_rows_quant_kernel(const PrefixAttnParams p, const uint8_t* pages, int with_p
       else
         asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(to), "r"(pair(0, 2, up)), "r"(pair(1, 3, up)), "r"(pair(4, 6, up)),
                      "r"(pair(5, 7, up)) : "memory");
-      if (qc == 0) s_cq[r] = p.c * back;
+      if (qc == 0) s_cq[r] = fmaxf(p.c * back, 0x1p-149f);  // not zero: -inf times it stays -inf
       if (w * 8 % SH == 0 && t == 0) s_qsum[w * 8 / SH][r] = sum / back;
     }
     __syncthreads();

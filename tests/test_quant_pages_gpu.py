@@ -287,6 +287,13 @@ def test_attn_no_prefix_and_scale(cuda, rng, new):
     check_attn(cuda, d, 8, with_prefix=False, scale=0.3)
 
 
+def test_attn_scale_next_to_zero(cuda, rng):
+    """Scores that vanish: every key that a row sees weighs the same, and what it does not see stays out."""
+    d = make_attn(rng, 4, 2, 64, 16, 4, 64, 33, [5, 100, 40], [1, 4, 1])
+    d["q"] = torch.full_like(d["q"], 2.0**-24)
+    check_attn(cuda, d, 4, scale=1e-44)
+
+
 @pytest.mark.parametrize("prefix", [0, 50])
 def test_attn_rows_that_see_nothing(cuda, rng, prefix):
     """More rows than tokens: the first ones see the prefix only, or nothing at all, and are zero."""
