@@ -39,7 +39,7 @@ namespace sc {
 // Two requests of 140000 tokens together, 8 kv heads of 128, 4 bits: 161 MB in 43 us with the
 // join; twice the tokens take 30 us more (5.9 TB/s), so 15 us are starts (lengths, page ids,
 // first blocks, one after another) and ends.  Four requests behind 700 tokens 7.5 us, latency.
-template <typename QB, int NT>
+template <typename QB, int NT, bool CLUSTER>
 struct FewRowsQuant {
   static constexpr int RT = 8 * NT;            // rows of a tile
   static constexpr int WORDS = QB::KSH / 4;    // of codes in a thread's share of a token
@@ -47,9 +47,10 @@ struct FewRowsQuant {
   static constexpr float MID = QB::BITS == 4 ? 8.f : 128.f;
   static constexpr int KSTEPS = QB::HD / 16, MT = QB::HD / 16;
   // Blocks of 16 tokens to a step: two, which share the step's fixed costs; one of the largest blocks, so that four CTAs fit an SM
-  // in place of three (32 requests of up to 3500 tokens, 16 heads of 128, 8 bits: groups of 32 66 -> 52 us; of 64 47 -> 44, but of up to
-  // 1000 tokens 19 -> 22, which is why those stay with two)
-  static constexpr int NBK = QB::BYTES > 4500 ? 1 : 2, KEYS = 16 * NBK;
+  // in place of three (16 heads of 128, 8 bits, groups of 32, 32 requests of up to 3500 tokens: 66 -> 52 us).  In groups of 64 so on the line
+  // alone, whose requests are long (of up to 3500 tokens 48 -> 43 us, 64 of them 101 -> 88, five CTAs 91; 128 behind a prefix of 8197 with up to
+  // 300 of their own 77 -> 68): in clusters, up to 1000 tokens, it took 22 us in place of 19.
+  static constexpr int NBK = QB::BYTES > 4500 || (!CLUSTER && NT == 1 && QB::BYTES > 4300) ? 1 : 2, KEYS = 16 * NBK;
   static constexpr int STAGE = NBK * QB::BYTES;
   static constexpr int NST = NBK == 1 ? 2 : STAGE > 4000 ? 2 : STAGE > 2400 ? 3 : 4;
   static constexpr int OUT = 2 * RT * QB::HD * 4;  // a warp's result, and the CTA's behind it
@@ -57,7 +58,7 @@ struct FewRowsQuant {
   static constexpr int QBYTES = NT * KSTEPS * 256;  // q's fragments
   static constexpr int SMEM = FR_WARPS * RING + QBYTES;
   // CTAs of an SM, by shared memory and by the registers that they need without spills
-  static constexpr int CTAS = NT == 1 ? (SMEM > 56000 ? 3 : SMEM > 44000 || QB::NG == 4 ? 4 : 5) : QB::NG == 4 || SMEM > 75000 ? 2 : 3;
+  static constexpr int CTAS = NT == 1 ? (SMEM > 56000 ? 3 : SMEM > 44000 || QB::NG == 4 || QB::BYTES > 4300 ? 4 : 5) : QB::NG == 4 || SMEM > 75000 ? 2 : 3;
   static constexpr int CTAS_CLUSTER = NT == 1 ? (CTAS < 4 ? CTAS : QB::NG == 4 ? 3 : 4) : 2;
 };
 
@@ -131,10 +132,10 @@ __device__ __forceinline__ void lds_share(uint32_t at, uint32_t other, uint32_t 
 }
 
 template <typename QB, int NT, bool CLUSTER>
-__global__ void __launch_bounds__(FR_WARPS * 32, CLUSTER ? FewRowsQuant<QB, NT>::CTAS_CLUSTER : FewRowsQuant<QB, NT>::CTAS)
+__global__ void __launch_bounds__(FR_WARPS * 32, CLUSTER ? FewRowsQuant<QB, NT, CLUSTER>::CTAS_CLUSTER : FewRowsQuant<QB, NT, CLUSTER>::CTAS)
 few_rows_quant_kernel(const PrefixAttnParams p, const uint8_t* pages, int with_prefix, int splits, int row_groups, int slot0,
                       const StreamArgs stream) {
-  using C = FewRowsQuant<QB, NT>;
+  using C = FewRowsQuant<QB, NT, CLUSTER>;
   constexpr int RT = C::RT, NST = C::NST, KT = C::KEYS, NBK = C::NBK, HD = QB::HD, NG = QB::NG, GS = QB::GS, WORDS = C::WORDS, PER = C::PER;
   extern __shared__ __align__(128) unsigned char fq_smem[];
   __shared__ __align__(8) uint64_t full[FR_WARPS][NST];
@@ -897,7 +898,7 @@ static QuantPlan plan_quant_attn(int T, int B, int Hq, int Hkv, int hd, int bits
   with_quant_block(hd, bits, group, [&](auto block) {
     using QB = decltype(block);
     a = plan_quant_attn(T, B, Hq, Hkv, hd, bits, (long long)max_blocks * page_size, (long long)max_prefix_blocks * page_size, sm_count(),
-                        {FewRowsQuant<QB, 1>::CTAS, FewRowsQuant<QB, 2>::CTAS}, {FewRowsQuant<QB, 1>::CTAS_CLUSTER, FewRowsQuant<QB, 2>::CTAS_CLUSTER});
+                        {FewRowsQuant<QB, 1, false>::CTAS, FewRowsQuant<QB, 2, false>::CTAS}, {FewRowsQuant<QB, 1, true>::CTAS_CLUSTER, FewRowsQuant<QB, 2, true>::CTAS_CLUSTER});
     return 0;
   });
   return a;
@@ -906,7 +907,7 @@ static QuantPlan plan_quant_attn(int T, int B, int Hq, int Hkv, int hd, int bits
 template <typename QB, int NT, bool CLUSTER>
 static int run_few_rows_quant(const PrefixAttnParams& p, const uint8_t* pages, const QuantPlan& a, const StreamArgs& line, cudaStream_t stream) {
   constexpr auto kern = few_rows_quant_kernel<QB, NT, CLUSTER>;
-  constexpr int smem = FewRowsQuant<QB, NT>::SMEM, KEYS = FewRowsQuant<QB, NT>::KEYS;
+  constexpr int smem = FewRowsQuant<QB, NT, CLUSTER>::SMEM, KEYS = FewRowsQuant<QB, NT, CLUSTER>::KEYS;
   const cudaError_t e = opt_in<kern>(smem);
   if (e != cudaSuccess) return check_launch("prefix_attn_q", e);
   launch_clusters(CLUSTER ? a.splits : 1, kern, CLUSTER ? dim3(a.splits * a.row_groups, p.Hkv, p.B) : dim3(a.ctas), dim3(FR_WARPS * 32), smem,
