@@ -874,13 +874,16 @@ static QuantPlan plan_quant_attn(int T, int B, int Hq, int Hkv, int hd, int bits
     a.nslots = 1;
     const long long keys = own_keys + prefix_keys;
     // Sizes a power of two: 16 requests of up to 800 tokens, 8 kv heads of 128, 1 to 6 and 8 CTAs a cluster: 12.2, 9.9, 11.0, 9.8, 13.9,
-    // 15.2, 16.2 us; as many as run at once, and up to a third more (drafts of up to five tokens, 16 requests behind 1000, 4 kv heads of 64, three tiles
-    // of rows each, 1 to 4: 20.5, 14.1, 19.6, 19.6; 384 CTAs in clusters of two on 296 places).
+    // 15.2, 16.2 us; as many as run at once, since a cluster of the next wave waits for one to end whole (8 kv heads of 128, 4 bits, 40 requests of up
+    // to 100 tokens, 1 CTA a cluster | 2, a tenth too many: 7.3 | 13.4 us, to 300 10 | 14, 48 to 1000, a third too many, 18.6 | 20.3); up to a tenth more where
+    // shares are long (40 of up to 2300: 27 | 25; 4 of 64, 8 bits, 80 of up to 2300: 23 | 19), and of tiles of 16 rows, some of whose CTAs have no rows, a
+    // third (drafts of up to five tokens, 16 requests behind 1000, 4 kv heads of 64, three tiles of rows each, 1 to 4: 20.5, 14.1, 19.6, 19.6; 384 CTAs
+    // in clusters of two on 296 places).
     // (CTAs for tiles of rows: those of requests with half as many rows again as the mean)
     a.row_groups = (int)(a.two ? ceil_div(3 * rows, 2ll * B * 16) : 1);
     const long long ctas = (long long)B * Hkv * a.row_groups, places = clusters[a.two] * sms;
     long long once = 1;
-    while (once < FR_CLUSTER && 2 * once * ctas * 3 <= 4 * places && 2 * once <= ceil_div(keys, 64)) once *= 2;
+    while (once < FR_CLUSTER && 2 * once * ctas * 30 <= (a.two ? 40 : keys > 900 * once ? 33 : 30) * places && 2 * once <= ceil_div(keys, 64)) once *= 2;
     if (ctas >= places ? keys * ctas <= (bits == 4 ? 4500 : 2700) * places : keys <= (hd == 64 ? 2200 : bits == 4 ? 1800 : 1600) * once) a.splits = (int)once;
   }
   size_t rows_all = a.nslots > 1 ? (size_t)a.nslots * T * Hq : 0;
