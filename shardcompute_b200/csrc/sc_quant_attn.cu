@@ -365,7 +365,8 @@ few_rows_quant_kernel(const PrefixAttnParams p, const uint8_t* pages, int with_p
               }
           }
       }
-      // ---- V's scales and biases; log2 of a bound of each token's largest scale
+      // ---- V's scales and biases; log2 of a bound of each token's largest scale.  A group that stands for NaN, by its bias, has no part
+      // in it: an infinite scale would press the weights of every key to nothing, for the other groups too.
       uint32_t mv[2 * NBK][NG];
       float lg[2 * NBK];
 #pragma unroll
@@ -373,8 +374,11 @@ few_rows_quant_kernel(const PrefixAttnParams p, const uint8_t* pages, int with_p
         lds_words<NG>(tile + (k >> 1) * QB::BYTES + QB::VM + meta_lane + (k & 1) * 32 * NG, mv[k]);
         float big = 0x1p-24f;
 #pragma unroll
-        for (int g = 0; g < NG; ++g) big = fmaxf(big, __low2float(u32_as_h2(mv[k][g])));
-        lg[k] = (float)((int)(__float_as_uint(big) >> 23) - 126);
+        for (int g = 0; g < NG; ++g) {
+          const float2 sb = __half22float2(u32_as_h2(mv[k][g]));
+          big = fmaxf(big, fmaf(sb.y, 0.f, sb.x));  // NaN: the other one
+        }
+        lg[k] = (float)((int)(__float_as_uint(fminf(big, 65504.f)) >> 23) - 126);
       }
       // ---- running softmax: a column's m, the same in its eight lanes, is raised (and o rescaled) only when some p s may pass
       // 2^(PA_LIFT + PA_RAISE)

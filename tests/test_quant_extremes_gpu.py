@@ -1,0 +1,54 @@
+"""The paged cache in 8 or 4 bits where values, queries and scales stand out, against oracle/quant_pages.py."""
+
+import math
+
+import numpy as np
+import pytest
+import torch
+
+from oracle import quant_pages as oq
+from shardcompute_b200 import _lib as L
+from shardcompute_b200 import ops
+from tests.test_quant_pages_gpu import attn_bound, i32, make_attn, pool, run_attn
+
+pytestmark = pytest.mark.gpu
+
+
+# ------------------------------------------------------------------------------------------------ values that are not finite
+
+@pytest.mark.parametrize("bad", [np.inf, -np.inf, 1e7], ids=["inf", "-inf", "1e7"])
+@pytest.mark.parametrize("hd,bits,group", [(128, 4, 64), (128, 8, 32), (64, 4, 32)])
+@pytest.mark.parametrize("longest", [700, 20000], ids=["clusters", "line"])
+def test_a_group_that_is_not_finite_leaves_the_others(cuda, rng, longest, hd, bits, group, bad):
+    """A value of v that is not finite (or past what a group can hold) makes its group's dims NaN in the rows that see it; the other
+    groups' dims of these rows, and all of the others, are what they are without it, within the bound of finite values."""
+    hq, hkv, lens, new = 4, 2, [longest, 90, 50], [1, 4, 1]
+    d = make_attn(rng, hq, hkv, hd, 16, bits, group, 0, lens, new, dirty=False)
+    assert (ops.prefix_attn_q_workspace_bytes(8, 3, hq, hkv, hd, d["table"].shape[1], 0, 16, bits, group) == 0) == (longest == 700)
+    # through the append: token 333 of the first request, the last but one of the second, in head 1, dim 5
+    pages, at = pool(d, cuda), [(0, 333), (1, 88)]
+    slots = [int(d["table"][b, t // 16]) * 16 + t % 16 for b, t in at]
+    x = np.zeros((2, 1 + 2 * hkv, hd), np.float32)
+    x[:, 1:] = rng.standard_normal((2, 2 * hkv, hd))
+    x[:, 1 + hkv + 1, 5] = bad
+    one = torch.ones(4, hd // 2, device=cuda)
+    ops.paged_rope_append_q(torch.from_numpy(x.reshape(2, -1)).to(cuda), i32([0, 2], cuda), i32(slots, cuda), i32([0, 0], cuda), one, one * 0,
+                            torch.empty(2, hd, dtype=torch.float16, device=cuda), pages)
+    d["data"] = pages.data.cpu().numpy()
+    got = run_attn(cuda, d, with_prefix=False)[:6].double().cpu().numpy().reshape(6, hq, hd)
+    # the oracle on the same bytes with zeros in that group: the other dims do not depend on it
+    finite = d["data"].copy()
+    for s in slots:
+        m = s % 16
+        base = oq.meta_place(1, m, 0, hd, bits, group)
+        held = finite[s // 16, 1, base:base + 4].view(np.float16)
+        assert np.isnan(held[1])  # what the append writes of such a group
+        finite[s // 16, 1, base:base + 4] = 0
+    want, mass, dot, keys, tail = oq.attention(d["q"].double().numpy(), finite, d["start"], d["lens"], d["table"], d["ptab"], 0, hq, hd, 16, bits,
+                                               group, 1 / math.sqrt(hd))
+    sees = np.zeros(got.shape, bool)
+    sees[[0, 3, 4], 2:, :group] = True  # heads 2, 3 are of kv head 1; of the second request's rows the last two see token 88
+    assert np.array_equal(np.isnan(got), sees)
+    err, bound = np.abs(got - want), attn_bound(want, mass, dot, keys, tail, hd)
+    assert (err[~sees] <= bound[~sees]).all(), np.nanmax(np.where(sees, 0, err / bound))
+    assert L.load().sc_prefix_attn_device_error(1) == 0
