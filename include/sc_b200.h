@@ -382,8 +382,9 @@ int sc_paged_read_q(const void* pages, int bits, int group, int n_pages, int pag
                     cudaStream_t stream);
 /* sc_prefix_attn over such pages, in all else as above: q, out fp16; page_size a
  * power of two, 16 to 32768; 0 < scale < 5e28.  The products take the codes
- * as they are; scores, softmax statistics and sums are fp32; weights times
- * scales are rounded to fp16 before their product with v's codes: 2^-11 of each,
+ * as they are; scores, softmax statistics and sums are fp32 (q.c is added up 16
+ * dims at a time, each step off by less than 2^-23 of the row's largest |q| times
+ * 2^bits); weights times scales are rounded to fp16 before their product with v's codes: 2^-11 of each,
  * down to 2^-25 of the row's largest.  Where many rows share keys (a prefix, a
  * long chunk) what k and v stand for is rounded to fp16 instead, 2^-11 of each,
  * and the rest is as for a cache in fp16.  A group that stands for NaN makes the

@@ -17,8 +17,9 @@
 //      holds an eighth of every group; the threads' pieces are exchanged by the
 //      pair's number, against bank conflicts.
 // Codes are taken as fp16 bit patterns: `w & 0x000f000f` is a pair of fp16
-// subnormals code 2^-24, exact in the tensor cores, so that no conversion stands
-// between memory and the products (0x00f000f0: code 2^-20).
+// subnormals code 2^-24 (0x00f000f0: code 2^-20), exact as operands of the tensor
+// cores, so that no conversion stands between memory and the products.  A sum of
+// products keeps the fewer bits, the lower a code lies (sc_quant_attn.cu, at q).
 #pragma once
 
 #include "sc_common.cuh"

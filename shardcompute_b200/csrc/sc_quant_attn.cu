@@ -20,15 +20,19 @@ namespace sc {
 // mma.sync m16n8k16 with the tokens (S = K Q^T), then the dims (O = V^T P^T) as
 // its 16 rows, the queries as its 8 columns: a decoded token of four heads
 // fills half of them, where queries as rows would fill a quarter, and tcgen05's 128 rows
-// of queries a thirtieth.  A register of an operand is an AND of a word of codes (fp16
-// subnormals), so a value costs 0.6 instructions; scales and biases are applied in
+// of queries a thirtieth.  A register of an operand is a shift and an AND of a word of codes
+// (fp16 subnormals), of V an AND alone, so a value costs 0.7 instructions; scales and biases are applied in
 // fp32, to S per group and to the weights before their product.  S passes to the second
 // product's operand through movmatrix; of V's nibbles the pair n0 + 16 n1 goes in beside
 // n0, which saves the masks of n1.
 //
 // q is scaled per row by a power of two so that its largest value is in
-// [2^11, 2^12): exact, with the 1/16 that the codes at 2^-20 need, but for what is below 2^-32
-// of that largest.  Its fragments lie in shared memory: in registers they kept a fifth CTA from the SM.
+// [2^11, 2^12): exact, but for what is below 2^-36 of that largest.  K's codes are moved up to the top of the subnormals (4 bits: code
+// 2^-18, 8 bits: 2^-22), since the tensor cores cut their sums below what an operand's exponent allows, and a subnormal's is that
+// of 2^-14: a product with q is then off as one of fp32 with the largest code would be.  As they lie (2^-24, 2^-20) q.c beside a dim of
+// q 2000 times the rest was up to 16 steps of fp32 off (of 16 times that dim), now 0.4; the shifts take 2 us of the 44 below, and codes
+// made whole (1024 + c, less 1024), which keep the exponents of small codes too, 6 us.
+// q's fragments lie in shared memory: in registers they kept a fifth CTA from the SM.
 // The weights p s are rounded to fp16, 2^11 to 2^15 high at the row's largest p s
 // (PA_LIFT over c s + log2 of the token's largest scale): 2^-11 of each, the
 // output's own rounding, down to 2^-25 of that largest.  Their error meets c - MID, not c,
@@ -36,8 +40,8 @@ namespace sc {
 // and bias are two large numbers of different signs (3.2e-4 of the output for one key, now
 // 2.1e-4, 2.07e-4 of it the output's rounding).
 //
-// Two requests of 140000 tokens together, 8 kv heads of 128, 4 bits: 161 MB in 43 us with the
-// join; twice the tokens take 30 us more (5.9 TB/s), so 15 us are starts (lengths, page ids,
+// Two requests of 140000 tokens together, 8 kv heads of 128, 4 bits: 161 MB in 44 us with the
+// join; twice the tokens take 29 us more (5.6 TB/s), so 15 us are starts (lengths, page ids,
 // first blocks, one after another) and ends.  Four requests behind 700 tokens 7.5 us, latency.
 template <typename QB, int NT, bool CLUSTER>
 struct FewRowsQuant {
@@ -45,6 +49,7 @@ struct FewRowsQuant {
   static constexpr int WORDS = QB::KSH / 4;    // of codes in a thread's share of a token
   static constexpr int PER = 32 / QB::BITS;    // codes of a word
   static constexpr float MID = QB::BITS == 4 ? 8.f : 128.f;
+  static constexpr int UNIT = QB::BITS == 4 ? 18 : 22;  // a code of K is taken as 2^-UNIT of itself
   static constexpr int KSTEPS = QB::HD / 16, MT = QB::HD / 16;
   // Blocks of 16 tokens to a step: two, which share the step's fixed costs; one of the largest blocks, so that four CTAs fit an SM
   // in place of three (16 heads of 128, 8 bits, groups of 32, 32 requests of up to 3500 tokens: 66 -> 52 us).  In groups of 64 so on the line
@@ -136,7 +141,7 @@ __global__ void __launch_bounds__(FR_WARPS * 32, CLUSTER ? FewRowsQuant<QB, NT, 
 few_rows_quant_kernel(const PrefixAttnParams p, const uint8_t* pages, int with_prefix, int splits, int row_groups, int slot0,
                       const StreamArgs stream) {
   using C = FewRowsQuant<QB, NT, CLUSTER>;
-  constexpr int RT = C::RT, NST = C::NST, KT = C::KEYS, NBK = C::NBK, HD = QB::HD, NG = QB::NG, GS = QB::GS, WORDS = C::WORDS, PER = C::PER;
+  constexpr int RT = C::RT, NST = C::NST, KT = C::KEYS, NBK = C::NBK, HD = QB::HD, NG = QB::NG, GS = QB::GS, WORDS = C::WORDS, PER = C::PER, UNIT = C::UNIT;
   extern __shared__ __align__(128) unsigned char fq_smem[];
   __shared__ __align__(8) uint64_t full[FR_WARPS][NST];
   __shared__ float s_m[FR_WARPS][RT], s_l[FR_WARPS][RT];
@@ -234,17 +239,17 @@ few_rows_quant_kernel(const PrefixAttnParams p, const uint8_t* pages, int with_p
       for (int z = 1; z < SH / 2; z <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, z);  // four shares, SH / 8 words of each
       // 2^k: the row's largest value to [2^11, 2^12) (an infinity, or no value at all: 1)
       const int e = (int)(__float_as_uint(big) >> 23) - 127, k = big > 0.f && e < 128 ? 11 - e : 0;
-      const float up = __uint_as_float((uint32_t)(127 + k) << 23), back = __uint_as_float((uint32_t)(127 + 24 - k) << 23);  // 2^(24 - k)
-      auto pair = [&](int a, int b2, float f) { return h2_as_u32(__floats2half2_rn(x[a] * f, x[b2] * f)); };
+      const float up = __uint_as_float((uint32_t)(127 + k) << 23), back = __uint_as_float((uint32_t)(127 + UNIT - k) << 23);
+      auto pair = [&](int a, int b2) { return h2_as_u32(__floats2half2_rn(x[a] * up, x[b2] * up)); };
       // the fragment of two steps of k, 16 bytes a lane
       const uint32_t to = q_u + (((r >> 3) * (C::KSTEPS / 2) + w) * 32 + (r & 7) * 4 + t) * 16;
       if (r >= RT) continue;  // heads of 64 and eight rows: half of the threads
       if constexpr (PER == 8)
-        asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(to), "r"(pair(0, 4, up)), "r"(pair(2, 6, up)),
-                     "r"(pair(1, 5, up * 0.0625f)), "r"(pair(3, 7, up * 0.0625f)) : "memory");
+        asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(to), "r"(pair(0, 4)), "r"(pair(2, 6)), "r"(pair(1, 5)),
+                     "r"(pair(3, 7)) : "memory");
       else
-        asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(to), "r"(pair(0, 2, up)), "r"(pair(1, 3, up)), "r"(pair(4, 6, up)),
-                     "r"(pair(5, 7, up)) : "memory");
+        asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(to), "r"(pair(0, 2)), "r"(pair(1, 3)), "r"(pair(4, 6)),
+                     "r"(pair(5, 7)) : "memory");
       if (qc == 0) s_cq[r] = fmaxf(p.c * back, 0x1p-149f);  // not zero: -inf times it stays -inf
       if (w * 8 % SH == 0 && t == 0) s_qsum[w * 8 / SH][r] = sum / back;
     }
@@ -323,14 +328,14 @@ few_rows_quant_kernel(const PrefixAttnParams p, const uint8_t* pages, int with_p
               for (int k = 0; k < NBK; ++k) {
                 float(&z)[4] = *reinterpret_cast<float(*)[4]>(&y[j][4 * k]);
                 if constexpr (PER == 8) {
-                  const uint32_t a = ka[k][w], c = kb[k][w];
-                  mma_16816(z, a & 0x000f000fu, c & 0x000f000fu, (a >> 8) & 0x000f000fu, (c >> 8) & 0x000f000fu, q.x, q.y);
-                  mma_16816(z, a & 0x00f000f0u, c & 0x00f000f0u, (a >> 8) & 0x00f000f0u, (c >> 8) & 0x00f000f0u, q.z, q.w);
+                  const uint32_t a = ka[k][w], c = kb[k][w], M = 0x03c003c0u;  // code 2^-18
+                  mma_16816(z, (a << 6) & M, (c << 6) & M, (a >> 2) & M, (c >> 2) & M, q.x, q.y);
+                  mma_16816(z, (a << 2) & M, (c << 2) & M, (a >> 6) & M, (c >> 6) & M, q.z, q.w);
                 } else {
 #pragma unroll
                   for (int i = 0; i < 2; ++i) {
-                    const uint32_t a = ka[k][2 * w + i], c = kb[k][2 * w + i];
-                    mma_16816(z, a & 0x00ff00ffu, c & 0x00ff00ffu, (a >> 8) & 0x00ff00ffu, (c >> 8) & 0x00ff00ffu, i ? q.z : q.x, i ? q.w : q.y);
+                    const uint32_t a = ka[k][2 * w + i], c = kb[k][2 * w + i], M = 0x03fc03fcu;  // code 2^-22
+                    mma_16816(z, (a << 2) & M, (c << 2) & M, (a >> 6) & M, (c >> 6) & M, i ? q.z : q.x, i ? q.w : q.y);
                   }
                 }
               }

@@ -52,3 +52,41 @@ def test_a_group_that_is_not_finite_leaves_the_others(cuda, rng, longest, hd, bi
     err, bound = np.abs(got - want), attn_bound(want, mass, dot, keys, tail, hd)
     assert (err[~sees] <= bound[~sees]).all(), np.nanmax(np.where(sees, 0, err / bound))
     assert L.load().sc_prefix_attn_device_error(1) == 0
+
+
+# ------------------------------------------------------------------------------------------------ queries with a dim that stands out
+
+@pytest.mark.parametrize("bits,hd,group", [(4, 128, 64), (4, 128, 32), (4, 64, 64), (8, 128, 64), (8, 64, 32)])
+@pytest.mark.parametrize("large", [2000.0, 20000.0])
+@pytest.mark.parametrize("drafts", [False, True])
+def test_scores_beside_a_dim_that_stands_out(cuda, rng, drafts, large, bits, hd, group):
+    """Two tokens a request whose scores are equal, though their codes differ: q is the same over eight dims, over which both tokens'
+    codes have one sum.  One dim of q is far larger than the rest, over a code of 1 in both; each head has another such dim, so that every
+    place of a code in its word is met.  The second token's value is 1, the first one's 0, so that the output is 1 / (1 + exp(-x)), x the
+    difference of the scores.  S adds 16 dims at a time to an fp32 sum, off by less than 2^-23 of the largest product that may stand there,
+    2^bits max |q|: hd / 16 of that, which the scale makes 2 here."""
+    B, hq, most = 32, 8, 2**bits - 1
+    limit = hd / 16 * 2.0**-23 * 2**bits * large
+    codes = rng.integers(1, most + 1, (B, 2, hd // 8, 8))
+    for a, c in ((codes[b, 0, g], codes[b, 1, g]) for b in range(B) for g in range(hd // 8)):
+        while a.sum() != c.sum():
+            i = rng.integers(0, 8)
+            c[i] = min(max(c[i] + np.sign(a.sum() - c.sum()), 1), most)
+    codes[:, :, 0] = 1
+    assert (codes[:, 0].sum(-1) == codes[:, 1].sum(-1)).all() and (codes[:, 0] != codes[:, 1]).any()
+    data, n = np.zeros((B, 1, oq.block_bytes(hd, bits, group)), np.uint8), hd // group
+    one, zero = np.ones((1, n), np.float16), np.zeros((1, n), np.float16)
+    for b in range(B):
+        for t in (0, 1):
+            oq.put(data, 16 * b + t, 16, 0, codes[b, t].reshape(1, hd), one, zero, bits, group)
+            oq.put(data, 16 * b + t, 16, 1, np.full((1, hd), t), one, zero, bits, group)
+    T = 3 * B if drafts else B  # tiles of 16 rows; the first two of a draft's three tokens see one token or none
+    q = np.repeat(rng.standard_normal((T, hq, hd // 8)), 8, -1)
+    q[..., :8] = 0.0
+    q[:, np.arange(hq), np.arange(hq)] = large
+    pages = ops.QuantPages(torch.from_numpy(data).to(cuda), hd, 16, bits, group)
+    out = ops.prefix_attn_q(torch.from_numpy(q.reshape(T, -1)).half().to(cuda), pages, i32(np.arange(B + 1) * (T // B), cuda), i32([2] * B, cuda),
+                            i32(np.arange(B)[:, None], cuda), scale=2.0 / limit)
+    got = out.double().cpu().numpy().reshape(B, -1, hq, hd)[:, -1]
+    # the weights' rounding to fp16 and the output's: 3 2^-11 of a value, 8e-3 of x
+    assert (np.abs(np.log(got / (1 - got))) <= 2.008).all(), (got.min(), got.max())
