@@ -358,9 +358,9 @@ int sc_prefix_attn(const void* q, const void* k_pages, const void* v_pages, int 
  * groups of `group` consecutive dims, are codes c of `bits` bits, a scale s and
  * a bias b (fp16) that stand for s c + b:
  *   b = min x rounded down, s = the smallest fp16 value with (2^bits - 1) s >=
- *   max x - b, c = rint((x - b) / s), 0 where s is 0: at most s / 2 off x.
- * A group that holds a value that is not finite or below -65504, or whose
- * largest code would stand for more than 65504, stands for NaN.
+ *   max x - b (the one below where (2^bits - 1) s + b passes 65504), c =
+ *   rint((x - b) / s), 0 where s is 0: at most s / 2 off x.
+ * A group that holds a value that is not finite or past +-65504 stands for NaN.
  *   hd 64 or 128; bits 4 or 8; group 32 or 64.
  * Pages [n_pages, Hkv, sc_quant_page_bytes] of bytes, in blocks of 16 tokens
  * whose order is the kernels' own (csrc/sc_quant.cuh); sc_paged_reserve and

@@ -21,6 +21,8 @@ def quantise(x, bits, group):
     most = 2**bits - 1
     b = floor16(x.min(-1))
     s = -floor16(-(x.max(-1) - b.astype(np.float64)) / most)
+    over = (s.astype(np.float64) * most + b.astype(np.float64) > 65504) & (x.max(-1) <= 65504)  # fp16 holds the group: the scale below
+    s = np.where(over, np.nextafter(s, np.float16(0)), s)
     c = np.zeros(x.shape, np.int64)
     some = s > 0
     c[some] = np.clip(np.rint((x - b.astype(np.float64)[..., None])[some] / s.astype(np.float64)[..., None][some]), 0, most)

@@ -4,7 +4,8 @@
 // a scale s and a bias b (fp16):
 //   b = min x rounded down, s = the smallest fp16 value with MOST s >= max x - b,
 //   c = rint((x - b) / s) in 0..MOST (0 where s is 0), and stands for s c + b
-// so that b <= x <= b + MOST s, and x is at most s / 2 off.  s and c are the ones that
+// so that b <= x <= b + MOST s, and x is at most s / 2 off.  Where b + MOST s would pass what fp16 holds, s is the
+// fp16 value below: b + MOST s is then less than max x by no more than MOST 2^-10 s, and x still at most s / 2 off.  s and c are the ones that
 // exact arithmetic gives: next to a border, fp32's roundings would decide.
 #include <algorithm>
 
@@ -44,8 +45,7 @@ __device__ __forceinline__ float max_nan(float a, float b) {
   return d;
 }
 
-// (scale, bias) of a group with these extremes.  Where either is not finite, or the largest code would stand for more than
-// fp16 holds, the bias is NaN: the group stands for NaN, and no score of it is an infinity that would take the token out of the
+// (scale, bias) of a group with these extremes.  Where either is not a finite value of fp16's range, the bias is NaN: the group stands for NaN, and no score of it is an infinity that would take the token out of the
 // attention unseen.
 template <int MOST>
 __device__ __forceinline__ __half2 scale_bias(float lo, float hi) {
@@ -61,8 +61,10 @@ __device__ __forceinline__ __half2 scale_bias(float lo, float hi) {
     s = __ushort_as_half(u + 1);
   else if (u > 0 && u <= 0x7c00 && __fsub_rn(__half2float(__ushort_as_half(u - 1)) * MOST, t) >= e)
     s = __ushort_as_half(u - 1);
-  const float top = fmaf(__half2float(s), (float)MOST, fb);
-  return __halves2half2(s, fb >= -65504.f && top <= 65504.f ? b : __ushort_as_half(0x7e00));
+  const bool holds = fb >= -65504.f && hi <= 65504.f;
+  // (fp32 may take a top next to 65504 for it: so does fp16)
+  if (holds && fmaf(__half2float(s), (float)MOST, fb) > 65504.f) s = __ushort_as_half(__half_as_ushort(s) - 1);
+  return __halves2half2(s, holds ? b : __ushort_as_half(0x7e00));
 }
 
 // rint((x - b) / s), `inv` about 1 / s.  The quotient in fp32 finds it or a neighbour; which, what is left over says exactly: x - b as

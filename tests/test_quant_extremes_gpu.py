@@ -90,3 +90,50 @@ def test_scores_beside_a_dim_that_stands_out(cuda, rng, drafts, large, bits, hd,
     got = out.double().cpu().numpy().reshape(B, -1, hq, hd)[:, -1]
     # the weights' rounding to fp16 and the output's: 3 2^-11 of a value, 8e-3 of x
     assert (np.abs(np.log(got / (1 - got))) <= 2.008).all(), (got.min(), got.max())
+
+
+# ------------------------------------------------------------------------------------------------ the ends of fp16's range
+
+@pytest.mark.parametrize("src", [torch.float16, torch.float32])
+@pytest.mark.parametrize("hd,bits,group", [(128, 4, 64), (128, 8, 64), (64, 4, 32), (64, 8, 32)])
+def test_what_fp16_holds_is_held(cuda, rng, hd, bits, group, src):
+    """Groups up to +-65504: codes, scales and biases as the oracle's, every value at most half a step off, and finite as fp16."""
+    ends = [(0, 65504), (-65504, 65504), (1, 65504), (-65504, 0), (65504, 65504), (-65504, -65504), (65472, 65504), (-3, 65504), (30000, 65504),
+            (-65504, 65472), (1e-3, 65504), (-40000, 60000)]
+    rows, hkv = len(ends), 2
+    x = np.stack([lo + (hi - lo) * rng.random((hkv, hd // group, group)) for lo, hi in ends])
+    x[..., 0], x[..., 1] = np.array(ends)[:, :1, None], np.array(ends)[:, 1:, None]
+    x = torch.from_numpy(x.reshape(rows, hkv, hd)).float().clamp(-65504, 65504).to(src)
+    pages, one, at = ops.quant_pages(1, hkv, 16, hd, bits, group, cuda), torch.ones(16, hd // 2, device=cuda), i32(np.arange(rows), cuda)
+    qkv = torch.cat([x.new_zeros(rows, 1, hd), x, x], 1).reshape(rows, -1).to(cuda)
+    ops.paged_rope_append_q(qkv, i32([0, rows], cuda), at, at, one, one * 0, torch.empty(rows, hd, dtype=torch.float16, device=cuda), pages)
+    want, s, b = oq.quantise(x.float().numpy(), bits, group)
+    assert np.isfinite(b).all()
+    for codes, scales, biases in oq.take(pages.data.cpu().numpy(), hd, 16, bits, group):
+        assert np.array_equal(codes[0, :, :rows].swapaxes(0, 1), want)
+        assert np.array_equal(scales[0, :, :rows].swapaxes(0, 1), s) and np.array_equal(biases[0, :, :rows].swapaxes(0, 1), b)
+    for v in ops.paged_read_q(pages, at, dtype=torch.float32):
+        # s / 2, and the rounding of s c + b to fp32
+        limit = np.repeat(s.astype(np.float64), group, -1) / 2 + 2.0**-24 * 65536
+        assert (np.abs(v.double().cpu().numpy() - x.double().numpy()) <= limit).all()
+    assert all(bool(torch.isfinite(v).all()) for v in ops.paged_read_q(pages, at))
+    # a row that sees all of it, by few rows and by many
+    for new in (1, 80):
+        q = torch.from_numpy(rng.standard_normal((new, 2 * hkv * hd)) * 1e-4).half()
+        table, start, lens = np.zeros((1, 1), np.int32), [0, new], [rows]
+        out = ops.prefix_attn_q(q.to(cuda), pages, i32(start, cuda), i32(lens, cuda), i32(table, cuda))
+        assert torch.isfinite(out[-1]).all()
+
+
+def test_append_past_fp16s_range(cuda):
+    """A value past +-65504 in fp32 makes its group NaN, the last one within it does not."""
+    hd, values = 64, [65504.0, 65505.0, -65504.0, -65505.0, 1e6]
+    x = torch.zeros(len(values), 3, hd)
+    x[:, 2, 7] = torch.tensor(values)
+    for bits in (4, 8):
+        pages, one, at = ops.quant_pages(1, 1, 16, hd, bits, 32, cuda), torch.ones(16, hd // 2, device=cuda), i32(np.arange(len(values)), cuda)
+        ops.paged_rope_append_q(x.reshape(len(values), -1).to(cuda), i32([0, len(values)], cuda), at, at, one, one * 0,
+                                torch.empty(len(values), hd, dtype=torch.float16, device=cuda), pages)
+        k, v = ops.paged_read_q(pages, at)
+        assert torch.isfinite(k).all() and torch.isfinite(v[..., 32:]).all()
+        assert v[:, 0, :32].isnan().all(-1).tolist() == [False, True, False, True, True] == v[:, 0, :32].isnan().any(-1).tolist()
