@@ -148,15 +148,19 @@ class PagedKVCache:
             return [PagedLayer(self, None, None, p) for p in self.pages]
         return [PagedLayer(self, k, v) for k, v in zip(self.k, self.v)]
 
-    def read(self, layer: int, request: int, dtype: torch.dtype = torch.float16):
-        """The request's tokens in one layer, as ``(k, v)`` ``[len, Hkv/TP, hd]``: to look at, or to move to another cache.
-        Waits for the device (a request's length lives there).  The shared prefix is not among them."""
+    def read(self, layer: int, request: int, dtype: Optional[torch.dtype] = None):
+        """The request's tokens in one layer, as ``(k, v)`` ``[len, Hkv/TP, hd]`` of ``dtype`` (default: that of the pages; of pages
+        in 8 or 4 bits float16): what the cache holds, keys as they were rotated, to look at or to compare.  Zeros where the
+        block table has no page.  Waits for the device (a request's length lives there).  The shared prefix is not among
+        them, and no call writes them back: an append takes keys before their rotation."""
         if not 0 <= request < self.max_batch:
             raise IndexError(f"request {request} out of range [0, {self.max_batch})")
         n = int(self.lens[request])
         at = torch.arange(n, device=self.lens.device)
         slots = self.block_table[request, at // self.page_size] * self.page_size + at.int() % self.page_size
         if self.pages is not None:
-            return ops.paged_read_q(self.pages[layer], slots, dtype=dtype)
+            return ops.paged_read_q(self.pages[layer], slots, dtype=dtype or torch.float16)
         page, off = slots.long() // self.page_size, slots.long() % self.page_size
-        return self.k[layer][page, :, off].to(dtype), self.v[layer][page, :, off].to(dtype)
+        there = (page >= 0) & (page < self.k.shape[1])
+        page = page.where(there, 0)
+        return tuple(x[layer][page, :, off].masked_fill(~there[:, None, None], 0).to(dtype or x.dtype) for x in (self.k, self.v))

@@ -9,6 +9,7 @@ import torch
 from oracle import quant_pages as oq
 from shardcompute_b200 import _lib as L
 from shardcompute_b200 import ops
+from shardcompute_b200.parallel import PagedKVCache
 from tests.test_quant_pages_gpu import attn_bound, i32, make_attn, pool, run_attn
 
 pytestmark = pytest.mark.gpu
@@ -137,3 +138,19 @@ def test_append_past_fp16s_range(cuda):
         k, v = ops.paged_read_q(pages, at)
         assert torch.isfinite(k).all() and torch.isfinite(v[..., 32:]).all()
         assert v[:, 0, :32].isnan().all(-1).tolist() == [False, True, False, True, True] == v[:, 0, :32].isnan().any(-1).tolist()
+
+
+# ------------------------------------------------------------------------------------------------ PagedKVCache.read
+
+@pytest.mark.parametrize("kind", [dict(bits=8), dict(bits=4, group_size=32), dict(dtype=torch.float16), dict(dtype=torch.float32)],
+                         ids=["8", "4", "f16", "f32"])
+def test_read_without_a_page(cuda, kind):
+    """In codes and in full alike: zeros where the table has no page, the pages' own type unless another is asked for."""
+    c = PagedKVCache(num_layers=1, kv_heads=2, head_dim=64, n_pages=4, max_batch=2, max_len=64, max_tokens=40, device=cuda, **kind)
+    c.reserve([40, 0])
+    for pool_ in ([p.data for p in c.pages] if c.pages else [c.k, c.v]):
+        pool_.fill_(60 if c.pages else 3.0)
+    c.block_table[0, 1] = -1
+    for x in c.read(0, 0):
+        assert x.dtype is kind.get("dtype", torch.float16) and x.shape == (40, 2, 64)
+        assert (x[16:32] == 0).all() and (x[:16] != 0).all() and (x[32:] != 0).all()
