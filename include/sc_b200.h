@@ -391,6 +391,14 @@ int sc_paged_read_q(const void* pages, int bits, int group, int n_pages, int pag
  * rows that see it NaN (of v: its dims), and no others. */
 size_t sc_prefix_attn_q_workspace_bytes(int T, int B, int Hq, int Hkv, int hd, int bits, int group, int max_blocks,
                                         int max_prefix_blocks, int page_size);
+/* How sc_prefix_attn_q cuts such a call on the current device: by what the tables could hold, not by the lengths in them.
+ *   plan[0]  0 few rows (its codes go into the products), 1 shared (the prefix's keys through fp16, the others as codes),
+ *            2 chunks (all keys through fp16)
+ *   plan[1]  CTAs of a cluster in the few-rows kernel; 0: its CTAs take pieces of a line
+ *   plan[2]  CTAs on that line
+ *   plan[3]  CTAs of the many-rows kernel */
+int sc_prefix_attn_q_plan(int T, int B, int Hq, int Hkv, int hd, int bits, int group, int max_blocks,
+                          int max_prefix_blocks, int page_size, int32_t plan[4]);
 int sc_prefix_attn_q(const void* q, const void* pages, int bits, int group, int T, const int32_t* q_start,
                      const int32_t* kv_lens, const int32_t* block_table, int B, int max_blocks,
                      const int32_t* prefix_table, const int32_t* prefix_len, int max_prefix_blocks, int Hq, int Hkv,

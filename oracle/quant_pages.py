@@ -125,19 +125,26 @@ def fill(k, v, bits, group):
     return data.reshape(n_pages, Hkv, -1)
 
 
-def attention(q, data, q_start, kv_lens, table, prefix_table, prefix_len, Hq, hd, page, bits, group, scale):
+def attention(q, data, q_start, kv_lens, table, prefix_table, prefix_len, Hq, hd, page, bits, group, scale, fp16=None):
     """out [rows, Hq, hd] float64, and per output a bound's parts (as oracle.paged.attention's): sum_j w_j (s c + |b|), the row's
-    largest scale * sum |q| (s c + |b|), its number of keys, and max_j (w_j s_j) * sum_j c_j / sum_j w_j."""
+    largest scale * sum |q| (s c + |b|), its number of keys, and max_j (w_j s_j) * sum_j c_j / sum_j w_j.
+
+    fp16: which tokens' s c + b is rounded once to fp16 on its way, "none", "prefix" or "all": for those the parts hold |k| and |v| in
+    place of s c + |b|, and the last one max_j w_j * sum_j |v_j| / sum_j w_j, added to the others'.  A sixth part comes with it:
+    sqrt(sum_j (w_j (s c + |b|))^2) / sum_j w_j."""
     n_pages, Hkv, _ = data.shape
     (kc, ks, kb), (vc, vs, vb) = take(data, hd, page, bits, group)
     spread = lambda x: np.repeat(x.astype(np.float64), group, -1)  # noqa: E731
     with np.errstate(invalid="ignore", over="ignore"):
         pools = dict(k=value(kc, ks, kb), v=value(vc, vs, vb), ka=value(kc, ks, np.abs(kb)), va=value(vc, vs, np.abs(vb)), c=vc.astype(float),
                      s=spread(vs))
+        k16, v16 = (pools[name].astype(np.float16).astype(np.float64) for name in "kv")
+    through = dict(k=k16, v=v16, ka=np.abs(k16), va=np.abs(v16))
     rows, G = int(q_start[-1]), Hq // Hkv
     q = np.asarray(q, np.float64).reshape(-1, Hq, hd)
     out = np.zeros((rows, Hq, hd))
     mass, dot, keys, tail = np.zeros_like(out), np.zeros((rows, Hq)), np.zeros((rows, Hq)), np.zeros_like(out)
+    spread_of = np.zeros_like(out)
 
     def where(ids, n):
         i = np.arange(n)
@@ -154,6 +161,10 @@ def attention(q, data, q_start, kv_lens, table, prefix_table, prefix_len, Hq, hd
         place_of = np.concatenate([np.full(len(pp), -1), np.flatnonzero(there)])  # a token's place in the request; -1: the prefix
         for h in range(Hkv if hi > lo else 0):
             x = {name: pool[pid, h, off] for name, pool in pools.items()}
+            r = np.full(len(pid), fp16 == "all") | ((place_of == -1) if fp16 == "prefix" else False)
+            for name, pool in through.items():
+                x[name][r] = pool[pid, h, off][r]
+            x["s"][r], x["c"][r] = 0.0, 0.0
             heads = slice(h * G, (h + 1) * G)
             for i in range(hi - lo):
                 n = int(np.searchsorted(place_of, max(-1, L - (hi - lo) + i), side="right"))  # tokens that the row sees
@@ -168,4 +179,7 @@ def attention(q, data, q_start, kv_lens, table, prefix_table, prefix_len, Hq, hd
                 tail[lo + i, heads] = (w * x["s"][:n].max(-1)).max(-1, keepdims=True) * x["c"][:n].sum(0) / total
                 dot[lo + i, heads] = scale * (np.abs(qs) @ x["ka"][:n].T).max(-1)
                 keys[lo + i, heads] = n
-    return out, mass, dot, keys, tail
+                spread_of[lo + i, heads] = np.sqrt((w * w) @ (x["va"][:n] ** 2)) / total
+                if r[:n].any():
+                    tail[lo + i, heads] += (w * r[:n]).max(-1, keepdims=True) * x["va"][:n][r[:n]].sum(0) / total
+    return (out, mass, dot, keys, tail) if fp16 is None else (out, mass, dot, keys, tail, spread_of)

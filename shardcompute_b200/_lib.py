@@ -66,6 +66,7 @@ SIGNATURES = {
     "sc_paged_rope_append_q": (_i, [_vp, _i, _i, _vp, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _vp, _vp, _i, _i, _i, _i, _vp]),
     "sc_paged_read_q": (_i, [_vp, _i, _i, _i, _i, _i, _i, _vp, _i, _vp, _vp, _vp, _i, _vp]),
     "sc_prefix_attn_q_workspace_bytes": (_sz, [_i, _i, _i, _i, _i, _i, _i, _i, _i, _i]),
+    "sc_prefix_attn_q_plan": (_i, [_i, _i, _i, _i, _i, _i, _i, _i, _i, _i, _vp]),
     "sc_prefix_attn_q": (_i, [_vp, _vp, _i, _i, _i, _vp, _vp, _vp, _i, _i, _vp, _vp, _i, _i, _i, _i, _i, _i, _f, _vp,
                               _vp, _sz, _vp]),
     "sc_rmsnorm": (_i, [_vp, _i, _i, _i, _vp, _f, _vp, _i, _vp]),

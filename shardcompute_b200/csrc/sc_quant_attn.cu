@@ -972,6 +972,23 @@ size_t sc_prefix_attn_q_workspace_bytes(int T, int B, int Hq, int Hkv, int hd, i
   return sc::plan_quant_attn(T, B, Hq, Hkv, hd, bits, group, max_blocks, max_prefix_blocks, page_size).bytes;
 }
 
+int sc_prefix_attn_q_plan(int T, int B, int Hq, int Hkv, int hd, int bits, int group, int max_blocks, int max_prefix_blocks, int page_size,
+                          int32_t plan[4]) {
+  using namespace sc;
+  SC_REQUIRE(plan, SC_ERR_ARG, "prefix_attn_q_plan: null pointer");
+  SC_REQUIRE(quant_kind_ok(hd, bits, group), SC_ERR_UNSUPPORTED,
+             "prefix_attn_q_plan: head_dim %d in %d bits by groups of %d unsupported (64 or 128; 4 or 8; 32 or 64)", hd, bits, group);
+  SC_REQUIRE(T >= 1 && B >= 1 && max_blocks >= 0 && max_prefix_blocks >= 0 && page_size >= 1 && Hkv >= 1 && Hq >= Hkv && Hq % Hkv == 0 &&
+                 (long long)T * Hq <= (1 << 30),
+             SC_ERR_SHAPE, "prefix_attn_q_plan: bad shape");
+  const QuantPlan a = plan_quant_attn(T, B, Hq, Hkv, hd, bits, group, max_blocks, max_prefix_blocks, page_size);
+  plan[0] = a.kind == AttnPlan::FEW ? 0 : a.kind == AttnPlan::SHARED ? 1 : 2;
+  plan[1] = a.splits;
+  plan[2] = a.ctas;
+  plan[3] = a.tc_splits * a.tc_items * Hkv;
+  return SC_OK;
+}
+
 int sc_prefix_attn_q(const void* q, const void* pages, int bits, int group, int T, const int32_t* q_start,
                      const int32_t* kv_lens, const int32_t* block_table, int B, int max_blocks,
                      const int32_t* prefix_table, const int32_t* prefix_len, int max_prefix_blocks, int Hq, int Hkv,

@@ -630,6 +630,25 @@ def prefix_attn_q_workspace_bytes(T: int, B: int, Hq: int, Hkv: int, hd: int, ma
     return int(L.load().sc_prefix_attn_q_workspace_bytes(T, B, Hq, Hkv, hd, bits, group_size, max_blocks, max_prefix_blocks, page_size))
 
 
+class QuantAttnPlan(NamedTuple):
+    """How ``prefix_attn_q`` cuts a call: ``kind`` "few", "shared" or "chunks", CTAs of a cluster (0: pieces of a line), CTAs on the
+    line, CTAs of the many-rows kernel."""
+
+    kind: str
+    cluster: int
+    line: int
+    many: int
+
+
+def prefix_attn_q_plan(T: int, B: int, Hq: int, Hkv: int, hd: int, max_blocks: int, max_prefix_blocks: int, page_size: int, bits: int = 4,
+                       group_size: int = 64) -> QuantAttnPlan:
+    """The plan of such a call on the current device.  It goes by what the tables could hold (``max_blocks`` and
+    ``max_prefix_blocks`` pages), since the lengths live on the device: tables cut to what is held are planned best."""
+    plan = (C.c_int32 * 4)()
+    L.check(L.load().sc_prefix_attn_q_plan(T, B, Hq, Hkv, hd, bits, group_size, max_blocks, max_prefix_blocks, page_size, plan), "sc_prefix_attn_q_plan")
+    return QuantAttnPlan(("few", "shared", "chunks")[plan[0]], *plan[1:])
+
+
 def prefix_attn_q(q: torch.Tensor, pages: QuantPages, q_start: torch.Tensor, kv_lens: torch.Tensor, block_table: torch.Tensor,
                   prefix_table: Optional[torch.Tensor] = None, prefix_len: Optional[torch.Tensor] = None,
                   out: Optional[torch.Tensor] = None, scale: Optional[float] = None,

@@ -1,0 +1,134 @@
+"""prefix_attn_q where the many-rows kernel takes part (shared prefixes, chunks): the plan is asserted, and the outputs are compared with
+float64 attention over the very fp16 values that the kernel makes of the codes, in a bound that a lost block of keys breaks."""
+
+import math
+
+import numpy as np
+import pytest
+import torch
+
+from oracle import quant_pages as oq
+from shardcompute_b200 import _lib as L
+from shardcompute_b200 import ops
+from tests.test_quant_pages_gpu import KINDS, make_attn, run_attn
+
+pytestmark = pytest.mark.gpu
+FP16 = {"few": "none", "shared": "prefix", "chunks": "all"}
+
+
+def plan_of(d, hq):
+    hd, page, bits, group = d["kind"]
+    return ops.prefix_attn_q_plan(len(d["q"]), len(d["lens"]), hq, d["data"].shape[1], hd, d["table"].shape[1], len(d["ptab"]), page, bits, group)
+
+
+def oracle(d, hq, kind, scale=None):
+    hd, page, bits, group = d["kind"]
+    return oq.attention(d["q"].double().numpy(), d["data"], d["start"], d["lens"], d["table"], d["ptab"], d["prefix"], hq, hd, page, bits, group,
+                        1 / math.sqrt(hd) if scale is None else scale, fp16=FP16[kind])
+
+
+def bounds(want, mass, dot, keys, tail, spread, hd):
+    """How far an output, and the norm of a (row, head), may be off.  With e = 2^-24, p = 2^-11:
+      score   S adds 16 dims at a time to an fp32 sum, each time off by at most 2 e of the largest sum; scales, biases and the difference
+              to the maximum are a few roundings more: ds = dot (hd / 16 + 6) 2 e
+      weight  w (1 + 2 ds + 8 e), rounded to fp16 (p; steps of 2^-36 of the largest weight: tail), codes' times s before
+      output  mass (2 ds + 16 e + 2 p + 2 e (keys / 8 + 64)) for numerator and denominator, then its rounding to fp16
+    In the norm the keys' roundings, up to p each whichever way, are independent of one another: six standard deviations of their sum,
+    p / sqrt(3) spread, in place of p mass."""
+    e, p = 2.0**-24, 2.0**-11
+    ds = (dot * (hd / 16 + 6) * 2 * e)[..., None]
+    sums = mass * (2 * ds + 16 * e + 2 * e * (keys[..., None] / 8 + 64)) + 2.0**-36 * 1.01 * tail + 2.0**-25
+    last = p * 1.01 * np.abs(want)
+    norm = lambda x: np.linalg.norm(x, axis=-1)  # noqa: E731
+    return sums + 2 * p * mass + last, norm(sums) + 6 * p / math.sqrt(3) * norm(spread) + norm(last)
+
+
+def check(cuda, d, hq, kind, scale=None, prepared=None):
+    assert plan_of(d, hq).kind == kind
+    out = run_attn(cuda, d, scale=scale)
+    want, *parts = prepared or oracle(d, hq, kind, scale)
+    rows = int(d["start"][-1])
+    got = out[:rows].double().cpu().numpy().reshape(want.shape)
+    each, whole = bounds(want, *parts, d["kind"][0])
+    err = np.abs(got - want)
+    worst = np.unravel_index(np.argmax(err / each), err.shape)
+    assert np.isfinite(got).all() and (err <= each).all(), (worst, got[worst], want[worst], each[worst])
+    off = np.linalg.norm(err, axis=-1)
+    worst = np.unravel_index(np.argmax(off / whole), off.shape)
+    assert (off <= whole).all(), (worst, off[worst], whole[worst])
+    assert (out[rows:] == 5.0).all()
+    assert L.load().sc_prefix_attn_device_error(1) == 0
+    for _ in range(3):
+        assert torch.equal(out, run_attn(cuda, d, scale=scale))
+    return out
+
+
+def chunks(rng, hq, hkv, hd, page, bits, group, prefix):
+    """Prompt chunks, some over tokens that were there before, beside requests with one row and with none."""
+    return make_attn(rng, hq, hkv, hd, page, bits, group, prefix, [20, 1, 5, 160, 0, 100, 40, 3300], [0, 1, 5, 137, 0, 100, 3, 170])
+
+
+def shared(rng, hd, bits, group, prefix, longest):
+    hq, hkv, page = (32, 4, 32) if hd == 64 else (24, 8, 16)
+    new = [int(x) for x in rng.integers(0, 6, 48)]
+    lens = [n + int(rng.integers(0, longest)) for n in new]
+    lens[5], new[5], lens[6], new[6] = 0, 2, longest, 1  # rows that see the prefix alone
+    return hq, make_attn(rng, hq, hkv, hd, page, bits, group, prefix, lens, new)
+
+
+@pytest.mark.parametrize("hd,bits,group", KINDS)
+@pytest.mark.parametrize("hq,hkv,page,prefix", [(8, 1, 16, 0), (6, 2, 64, 333), (8, 2, 256, 1)])
+def test_chunks(cuda, rng, hd, bits, group, hq, hkv, page, prefix):
+    check(cuda, chunks(rng, hq, hkv, hd, page, bits, group, prefix), hq, "chunks")
+
+
+@pytest.mark.parametrize("hd,bits,group", KINDS)
+@pytest.mark.parametrize("lens,new,prefix", [([900, 700], [600, 300], 0), ([300], [300], 5000), ([2600, 10], [80, 2], 1500)], ids=["own", "prefix", "both"])
+def test_chunk_of_many_tiles(cuda, rng, hd, bits, group, lens, new, prefix):
+    check(cuda, make_attn(rng, 8, 2, hd, 32, bits, group, prefix, lens, new), 8, "chunks")
+
+
+@pytest.mark.parametrize("hd,bits,group", KINDS)
+@pytest.mark.parametrize("prefix,longest", [(2900, 40), (4000, 300)])
+def test_shared_by_many_requests(cuda, rng, hd, bits, group, prefix, longest):
+    """The prefix once for all, then with absent pages in it and in a request."""
+    hq, d = shared(rng, hd, bits, group, prefix, longest)
+    check(cuda, d, hq, "shared")
+    d["ptab"][[0, 3, len(d["ptab"]) - 1]] = [-1, -2, len(d["data"]) + 5]
+    d["table"][6, 0] = -3
+    check(cuda, d, hq, "shared")
+
+
+def test_absent_pages_in_chunks(cuda, rng):
+    d = chunks(rng, 8, 2, 128, 16, 4, 64, 333)
+    d["ptab"][[0, 5, len(d["ptab"]) - 1]] = [-1, -7, len(d["data"]) + 5]
+    d["table"][7, [0, 3, 100]], d["table"][5, :] = -1, -1
+    check(cuda, d, 8, "chunks")
+
+
+@pytest.mark.parametrize("hd,bits,group", [(128, 4, 64), (64, 8, 32)])
+def test_values_of_any_size_in_chunks(cuda, rng, hd, bits, group):
+    """Biases large beside their groups' ranges, subnormal values and large ones: what fp16 makes of s c + b."""
+    for kv, shift in ((1.0, 30.0), (1e-6, 0.0), (2e3, -500.0)):
+        d = make_attn(rng, 8, 2, hd, 32, bits, group, 100, [900, 700], [600, 300], dirty=False, scale_q=0.05 / kv if kv > 1 else 0.5)
+        k, v = (rng.standard_normal((len(d["data"]), 2, 32, hd)) * kv + shift for _ in range(2))
+        d["data"] = oq.fill(k.astype(np.float32), v.astype(np.float32), bits, group)
+        check(cuda, d, 8, "chunks")
+
+
+def test_hidden_groups_in_chunks(cuda, rng):
+    """A chunk's later token that is not finite shows in the rows that see it: of k everywhere, of v in its group's dims, whatever the
+    scale that stands beside the bias of NaN; the other rows and dims are what they were, bit for bit."""
+    d = make_attn(rng, 8, 1, 64, 16, 4, 32, 20, [3400, 250], [300, 200], dirty=False)
+    assert plan_of(d, 8).kind == "chunks"
+    clean = run_attn(cuda, d)
+    first = 3350 - 3100  # the row that first sees token 3350
+    for side in (0, 1):
+        for scale in (np.inf, 1.0):
+            e = dict(d, data=d["data"].copy())
+            at = oq.meta_place(side, 3350 % 16, 1, 64, 4, 32)
+            e["data"][d["table"][0, 3350 // 16], :, at:at + 4] = np.array([scale, np.nan], np.float16).view(np.uint8)
+            out = run_attn(cuda, e)
+            assert torch.equal(out[:first], clean[:first]) and torch.equal(out[300:500], clean[300:500])
+            sees, was = out[first:300].view(-1, 8, 64), clean[first:300].view(-1, 8, 64)
+            assert sees[..., 32:].isnan().all() and (side == 0 or torch.equal(sees[..., :32], was[..., :32]))
