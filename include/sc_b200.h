@@ -386,8 +386,10 @@ int sc_paged_read_q(const void* pages, int bits, int group, int n_pages, int pag
  * dims at a time, each step off by less than 2^-23 of the row's largest |q| times
  * 2^bits); weights times scales are rounded to fp16 before their product with v's codes: 2^-11 of each,
  * down to 2^-25 of the row's largest.  Where many rows share keys (a prefix, a
- * long chunk) what k and v stand for is rounded to fp16 instead, 2^-11 of each,
- * and the rest is as for a cache in fp16.  A group that stands for NaN makes the
+ * long chunk) what v stands for is rounded to fp16 instead, as a cache in fp16
+ * would hold it, and what k stands for too, in one term where the rows see 1024 keys,
+ * in the sum of two where they see fewer (2^-15 of half its group's range; 2^-11 of it
+ * for a group whose middle is further than that from zero).  A group that stands for NaN makes the
  * rows that see it NaN (of v: its dims), and no others. */
 size_t sc_prefix_attn_q_workspace_bytes(int T, int B, int Hq, int Hkv, int hd, int bits, int group, int max_blocks,
                                         int max_prefix_blocks, int page_size);

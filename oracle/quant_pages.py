@@ -129,22 +129,29 @@ def attention(q, data, q_start, kv_lens, table, prefix_table, prefix_len, Hq, hd
     """out [rows, Hq, hd] float64, and per output a bound's parts (as oracle.paged.attention's): sum_j w_j (s c + |b|), the row's
     largest scale * sum |q| (s c + |b|), its number of keys, and max_j (w_j s_j) * sum_j c_j / sum_j w_j.
 
-    fp16: which tokens' s c + b is rounded once to fp16 on its way, "none", "prefix" or "all": for those the parts hold |k| and |v| in
-    place of s c + |b|, and the last one max_j w_j * sum_j |v_j| / sum_j w_j, added to the others'.  A sixth part comes with it:
-    sqrt(sum_j (w_j (s c + |b|))^2) / sum_j w_j."""
+    fp16: of which tokens s c + b goes through fp16, "none", "prefix" (of 1024 tokens at least, else none) or "all": v, and k in one term for
+    rows in whose tile of 256 (token, head) rows all see 1024 keys, in two for the others.  For those tokens the parts hold |k| and |v| in
+    place of s c + |b|, and the last one max_j w_j * sum_j |v_j| / sum_j w_j, added to the others'.  Two more parts come with it:
+    sqrt(sum_j (w_j (s c + |b|))^2) / sum_j w_j, and the largest scale * sum |q| e of those tokens, e what the two terms may be off a k:
+    2^-15 of half its group's range, 2^-11 where the group's middle is further than that from zero, and of all of it next to fp16's
+    limits."""
     n_pages, Hkv, _ = data.shape
     (kc, ks, kb), (vc, vs, vb) = take(data, hd, page, bits, group)
     spread = lambda x: np.repeat(x.astype(np.float64), group, -1)  # noqa: E731
     with np.errstate(invalid="ignore", over="ignore"):
         pools = dict(k=value(kc, ks, kb), v=value(vc, vs, vb), ka=value(kc, ks, np.abs(kb)), va=value(vc, vs, np.abs(vb)), c=vc.astype(float),
                      s=spread(vs))
-        k16, v16 = (pools[name].astype(np.float16).astype(np.float64) for name in "kv")
-    through = dict(k=k16, v=v16, ka=np.abs(k16), va=np.abs(v16))
+        v16 = pools["v"].astype(np.float16).astype(np.float64)
+        pools["k16"] = pools["k"].astype(np.float16).astype(np.float64)
+        half = spread(ks) * 2.0 ** (bits - 1)
+        middle = np.abs(spread(kb) + half)
+        pools["e"] = np.where(middle <= half, 2.0**-15 * half, 2.0**-11 * np.where(middle + half < 30000, half, middle + half))
+    through = dict(ka=np.abs(pools["k"]), v=v16, va=np.abs(v16))
     rows, G = int(q_start[-1]), Hq // Hkv
     q = np.asarray(q, np.float64).reshape(-1, Hq, hd)
     out = np.zeros((rows, Hq, hd))
     mass, dot, keys, tail = np.zeros_like(out), np.zeros((rows, Hq)), np.zeros((rows, Hq)), np.zeros_like(out)
-    spread_of = np.zeros_like(out)
+    spread_of, split = np.zeros_like(out), np.zeros((rows, Hq))
 
     def where(ids, n):
         i = np.arange(n)
@@ -161,7 +168,7 @@ def attention(q, data, q_start, kv_lens, table, prefix_table, prefix_len, Hq, hd
         place_of = np.concatenate([np.full(len(pp), -1), np.flatnonzero(there)])  # a token's place in the request; -1: the prefix
         for h in range(Hkv if hi > lo else 0):
             x = {name: pool[pid, h, off] for name, pool in pools.items()}
-            r = np.full(len(pid), fp16 == "all") | ((place_of == -1) if fp16 == "prefix" else False)
+            r = np.full(len(pid), fp16 == "all") | ((place_of == -1) if fp16 == "prefix" and prefix_len >= 1024 else False)
             for name, pool in through.items():
                 x[name][r] = pool[pid, h, off][r]
             x["s"][r], x["c"][r] = 0.0, 0.0
@@ -171,7 +178,10 @@ def attention(q, data, q_start, kv_lens, table, prefix_table, prefix_len, Hq, hd
                 if n == 0:
                     continue
                 qs = q[lo + i, heads]
-                sc = scale * (qs @ x["k"][:n].T)
+                first = (i * G + np.arange(G)) // 256 * 256 // G  # of each head's tile of rows
+                deep = prefix_len + np.clip(L - (hi - lo) + first + 1, 0, max(L, 0)) >= 1024
+                one = r[:n] & (deep[:, None] if fp16 == "all" else np.full((G, 1), True))
+                sc = scale * np.where(one, qs @ x["k16"][:n].T, qs @ x["k"][:n].T) if one.any() else scale * (qs @ x["k"][:n].T)
                 w = np.exp(sc - sc.max(-1, keepdims=True))
                 total = w.sum(-1, keepdims=True)
                 out[lo + i, heads] = w @ x["v"][:n] / total
@@ -181,5 +191,6 @@ def attention(q, data, q_start, kv_lens, table, prefix_table, prefix_len, Hq, hd
                 keys[lo + i, heads] = n
                 spread_of[lo + i, heads] = np.sqrt((w * w) @ (x["va"][:n] ** 2)) / total
                 if r[:n].any():
+                    split[lo + i, heads] = scale * np.where(r[:n] & ~one, np.abs(qs) @ x["e"][:n].T, 0.0).max(-1)
                     tail[lo + i, heads] += (w * r[:n]).max(-1, keepdims=True) * x["va"][:n][r[:n]].sum(0) / total
-    return (out, mass, dot, keys, tail) if fp16 is None else (out, mass, dot, keys, tail, spread_of)
+    return (out, mass, dot, keys, tail) if fp16 is None else (out, mass, dot, keys, tail, spread_of, split)

@@ -52,7 +52,8 @@ __device__ __forceinline__ bool not_finite(const uint4& v) {
 //              (0 x NaN is NaN), before the MMA issuers use the tile
 //   warps 12-15, over codes (sc_quant_attn.cu): the producer's copies are blocks
 //              of codes, K and V of 64 tokens a stage; these warps write the values
-//              s c + b, rounded to fp16 once, into the ring that TMA fills otherwise.
+//              s c + b, rounded to fp16 once (K for rows of few keys in two terms, a
+//              tile of the ring each), into the ring that TMA fills otherwise.
 //              Their loops are rolled: unrolled, the SM's instruction cache no longer
 //              held what its warps run (the chunks below, 4 bits, 336 us; 300 so)
 //   warps 4-7, 8-11: softmax of tile 0 and of tile 1, a thread per row, which
@@ -71,6 +72,13 @@ constexpr int TC_THREADS = 12 * 32;
 constexpr int TC_REGS_CTL = 88, TC_REGS_SM = 208;  // 128 x 88 + 256 x 208: what the block starts with, 384 x 168
 constexpr int TC_THREADS_QUANT = 16 * 32;
 constexpr int TC_REGS_CTL_QUANT = 56, TC_REGS_SM_QUANT = 200;  // 256 x 56 + 256 x 200 = 512 x 128
+// Over codes: rows that all see this many keys take k rounded once to fp16, as a cache in fp16 would hold it; the others as the sum of two
+// fp16 terms (QuantValues::two_terms).  The rounding's errors, 2^-12 of each k, are independent of one another and even out over many keys;
+// over few they do not: the output's error against float64, over that of the output's own rounding, rows that see 32, 128, 512, 1024, 2048
+// keys, heads of 64, channels that stand out: 2.0, 1.9, 1.5, 1.35, 1.2 with one term, 1.35, 1.26, 1.12, 1.09, 1.05 with two (v and the weights
+// are rounded in both).  The second term costs half as many products again: 12 prompts of up to 700 tokens alone, heads of 128, 4 bits, 105
+// -> 126 us; the two kernels side by side 304 -> 310 us for 12 chunks behind 2050, 243 -> 269 for a prompt of 4000.
+constexpr int TC_TWO_TERMS = 1024;
 constexpr int TC_HAND = 3;  // quarter of a tile before which its softmax lets the other one start
 
 template <int HD, typename Src = PoolMaps>
@@ -389,6 +397,86 @@ struct QuantValues {
       }
     }
   }
+  // (s, b) of a group taken apart for its codes' distances d = c - MID from their middle: x.x = (s1, b1), x.y = (s2, b2), with
+  // s c + b = (s1 d + b1) + (s2 d + b2).  With b' = b + MID s, the middle's value:
+  //   s1 the s of 11 - BITS significant bits, b1 the multiple of its last one next to b': s1 d + b1 has 11 bits, so fp16 holds it exactly
+  //     (4 bits: s2 d + b2 too; 8 bits: to 2^-15 of MID s);
+  //   where b' is too large beside s for that, s1 = 0: b' alone, and s d to fp16's 2^-12;
+  //   next to fp16's limits s2 = 0, one term, as an fp16 cache would hold the value.
+  static __device__ __forceinline__ uint2 two_terms(uint32_t sb) {
+    constexpr float MID = QB::BITS == 4 ? 8.f : 128.f;
+    constexpr uint32_t DROP = QB::BITS == 4 ? 17 : 21, UP = QB::BITS == 4 ? 4 : 8;
+    const float2 x = __half22float2(u32_as_h2(sb));
+    const float mid = fmaf(MID, x.x, x.y);
+    const uint32_t u = __float_as_uint(x.x), e = u & 0xff800000u;
+    const float grid = __uint_as_float(e + ((17u + UP - 4u) << 23) + 0x400000u);  // 1.5 2^23 of the last bits of s1
+    const bool far = fabsf(mid) > __uint_as_float(e + (UP << 23)), end = fabsf(mid) + (MID + 1.f) * x.x >= 32768.f;
+    const float s1 = end ? x.x : far ? 0.f : __uint_as_float((u + (1u << (DROP - 1))) & ~((1u << DROP) - 1u));
+    const __half b1 = __float2half_rz(end || far ? mid : __fsub_rn(__fadd_rn(mid, grid), grid));  // (rz: a sum next to the limit stays below it)
+    const float b2 = end ? 0.f : mid - __half2float(b1);
+    return make_uint2(h2_as_u32(__halves2half2(__float2half_rn(s1), b1)), h2_as_u32(__floats2half2_rn(end ? 0.f : x.x - s1, b2)));
+  }
+  // Codes of a word less MID: four (two) half2 in the order of unpack_u4 (unpack_u8), exact.
+  static __device__ __forceinline__ void distances(uint32_t w, __half2 (&x)[QB::BITS == 4 ? 4 : 2]) {
+    if constexpr (QB::BITS == 4) {
+      const __half2 low = u32_as_h2(0x64086408u), k16th = u32_as_h2(0x2c002c00u), high = u32_as_h2(0xd480d480u);  // 1032, 1/16, -72
+      const uint32_t w8 = w >> 8;
+      x[0] = __hsub2(u32_as_h2((w & 0x000f000fu) | 0x64006400u), low);
+      x[1] = hfma2_rn(u32_as_h2((w & 0x00f000f0u) | 0x64006400u), k16th, high);
+      x[2] = __hsub2(u32_as_h2((w8 & 0x000f000fu) | 0x64006400u), low);
+      x[3] = hfma2_rn(u32_as_h2((w8 & 0x00f000f0u) | 0x64006400u), k16th, high);
+    } else {
+      const __half2 low = u32_as_h2(0x64806480u);  // 1152
+      x[0] = __hsub2(u32_as_h2((w & 0x00ff00ffu) | 0x64006400u), low);
+      x[1] = __hsub2(u32_as_h2(((w >> 8) & 0x00ff00ffu) | 0x64006400u), low);
+    }
+  }
+  // K as two terms, each to its tile.  A warp's eight tokens of a step have 8 NG groups, of which each lane takes one apart.
+  static __device__ __forceinline__ void keys_two(uint32_t raw, uint32_t tile, uint32_t tile2, int row0) {
+    const int tid = threadIdx.x & 127, lane = threadIdx.x & 31;
+#pragma unroll 1
+    for (int u = 0; u < RB / 2; ++u) {
+      const int token = u * 32 + (tid >> 2), t = tid & 3, tok = token & 15, row = row0 + token;
+      const uint32_t block = raw + (token >> 4) * QB::BYTES, at = block + tok * QB::ROW + QB::piece_k(tok, t, 0);
+      uint32_t w[WORDS];
+      load(at, block + tok * QB::ROW + (QB::piece_k(tok, t, 0) ^ 64), w);
+      const int mine = (token & ~7) + (lane & 7);  // eight tokens in a row: of one block
+      const uint2 terms = two_terms(lds_u32(block + QB::KM + ((mine & 15) * NG + (lane >> 3) % NG) * 4));
+      uint32_t sb1 = 0u, sb2 = 0u;
+#pragma unroll
+      for (int c = 0; c < HD / 32; ++c) {  // eight dims
+        const int l = c * 8, g = l / (GS / 4), d = g * GS + t * (GS / 4) + l % (GS / 4);
+        if (l % (GS / 4) == 0) {
+          sb1 = __shfl_sync(0xffffffffu, terms.x, g * 8 + (lane >> 2));
+          sb2 = __shfl_sync(0xffffffffu, terms.y, g * 8 + (lane >> 2));
+        }
+        __half2 x[4];  // dims i and i + 4 (8 bits: 0 and 2, 1 and 3, and four on)
+        if constexpr (QB::BITS == 4) {
+          distances(w[c], x);
+        } else {
+          __half2 lo[2], hi[2];
+          distances(w[2 * c], lo);
+          distances(w[2 * c + 1], hi);
+          x[0] = lo[0]; x[1] = lo[1]; x[2] = hi[0]; x[3] = hi[1];
+        }
+        const uint32_t to = (d >> 6) * (TC_N * 128) + sw128(row, (d >> 3) & 7);
+#pragma unroll
+        for (int term = 0; term < 2; ++term) {
+          const __half2 s = __low2half2(u32_as_h2(term ? sb2 : sb1)), b = __high2half2(u32_as_h2(term ? sb2 : sb1));
+          uint32_t z[4], y[4];
+#pragma unroll
+          for (int k = 0; k < 4; ++k) z[k] = h2_as_u32(hfma2_rn(x[k], s, b));
+#pragma unroll
+          for (int k = 0; k < 2; ++k) {
+            // 4 bits: dims 0 1 | 2 3 | 4 5 | 6 7 of pairs (0, 4) .. (3, 7); 8 bits: of (0, 2), (1, 3), (4, 6), (5, 7)
+            y[QB::BITS == 4 ? k : 2 * k] = __byte_perm(z[2 * k], z[2 * k + 1], 0x5410);
+            y[QB::BITS == 4 ? 2 + k : 2 * k + 1] = __byte_perm(z[2 * k], z[2 * k + 1], 0x7632);
+          }
+          sts_v4((term ? tile2 : tile) + to, y[0], y[1], y[2], y[3]);
+        }
+      }
+    }
+  }
   // V; blocks whose bit in `gone` is set are zero.
   static __device__ __forceinline__ void values(uint32_t raw, uint32_t tile, int row0, uint32_t gone) {
     const int tid = threadIdx.x & 127;
@@ -480,13 +568,57 @@ __device__ __forceinline__ void quant_writer(int cnt, uint32_t ring_u, uint32_t 
   }
 }
 
+// K as two terms, all of a tile's K ahead of its V, whose place may be free only when the products of the tile before are done: S waits for
+// K, and three tiles may be the whole ring.
+template <int HD, typename Src>
+__device__ __forceinline__ void quant_writer_two(int cnt, uint32_t ring_u, uint32_t raw_u, uint64_t* full, uint64_t* empty, uint64_t* raw_full,
+                                                 uint64_t* raw_empty, const uint32_t* s_absent, volatile int* abort) {
+  using C = ManyRows<HD, Src>;
+  using V = QuantValues<HD, typename QuantBlockOf<HD, Src>::type, C::RB>;
+  constexpr int NBUF = C::NBUF, NRAW = C::NRAW;
+  const int lane = threadIdx.x & 31;
+  auto wait = [&](uint64_t* bar, uint32_t parity) { return __all_sync(0xffffffffu, pa_wait(bar, parity, abort)); };
+  auto place = [&](uint32_t t) { return wait(&empty[t % NBUF], ((t / NBUF) & 1u) ^ 1u); };
+  for (int i = 0; i < cnt; ++i) {
+    const uint32_t ki = 3 * i, li = ki + 1, vi = ki + 2, it = C::STAGES * i;
+    const uint32_t kt = ring_u + (ki % NBUF) * C::TILE, lt = ring_u + (li % NBUF) * C::TILE, vt = ring_u + (vi % NBUF) * C::TILE;
+    if (!place(ki) || !place(li)) return;
+#pragma unroll 1
+    for (int st = 0; st < C::STAGES; ++st) {
+      const int s = (it + st) % NRAW;
+      if (!wait(&raw_full[s], ((it + st) / NRAW) & 1u)) return;
+      V::keys_two(raw_u + s * C::RAW, kt, lt, st * C::RB * 16);
+    }
+    fence_async_smem();
+    __syncwarp();
+    if (lane == 0) {
+      mbar_arrive(&full[ki % NBUF]);
+      mbar_arrive(&full[li % NBUF]);
+    }
+    if (!place(vi)) return;
+#pragma unroll 1
+    for (int st = 0; st < C::STAGES; ++st) {
+      const int s = (it + st) % NRAW;
+      V::values(raw_u + s * C::RAW, vt, st * C::RB * 16, s_absent[i & 15] >> (C::RB * st));
+      fence_async_smem();
+      __syncwarp();
+      if (lane == 0) {
+        mbar_arrive(&raw_empty[s]);
+        if (st == C::STAGES - 1) mbar_arrive(&full[vi % NBUF]);
+      }
+    }
+  }
+}
+
 // PACKED: rows of all requests, keys of the prefix.  Otherwise: rows of one
-// request, keys of the prefix and its own.
-template <int HD, bool PACKED, typename Src>
+// request, keys of the prefix and its own.  Over codes rows of which some sees
+// fewer than TC_TWO_TERMS keys are those of the kernel with TWO, k in two terms, the others those of the one
+// without, which it runs beside (p.beside: no wait for that one until the end).
+template <int HD, bool PACKED, typename Src, bool TWO = false>
 __global__ void __launch_bounds__(ManyRows<HD, Src>::THREADS, 1)
 many_rows_kernel(const PrefixAttnParams p, const __grid_constant__ Src src, int splits, int slot0) {
   using C = ManyRows<HD, Src>;
-  constexpr int NBUF = C::NBUF, NCH = HD / 64;  // NCH: 64-wide columns
+  constexpr int NBUF = C::NBUF, NCH = HD / 64, TPK = TWO ? 3 : 2;  // NCH: 64-wide columns; TPK: ring tiles to a tile of keys, K (or its two terms) and V
   extern __shared__ __align__(1024) unsigned char mr_smem[];
   __shared__ __align__(8) uint64_t full[NBUF], empty[NBUF], q_full[2], s_full[2], p_full[2][2], o_full[2], v_clean[NBUF], drained[2], turn[2][4];
   __shared__ uint32_t s_tmem, s_absent[16];
@@ -529,12 +661,23 @@ many_rows_kernel(const PrefixAttnParams p, const __grid_constant__ Src src, int 
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  pdl_wait();
+  const bool beside = TWO && p.beside;
+  if (!beside) pdl_wait();
   pdl_trigger();  // after the wait: few_rows_kernel relies on it
   volatile int* abort = &s_abort;
   const uint32_t tmem = s_tmem;
 
-  const RowShare w = row_share<PACKED, 2 * TC_M, TC_N, C::THREADS>(p, item, split, splits, s_req, s_row0, s_sum);
+  RowShare w = row_share<PACKED, 2 * TC_M, TC_N, C::THREADS>(p, item, split, splits, s_req, s_row0, s_sum);
+  if (C::QUANT && PACKED && w.P < TC_TWO_TERMS) w.P = w.np = w.cnt = 0;  // few_rows_quant_kernel's
+  const bool last_cta = blockIdx.x == gridDim.x - 1 && blockIdx.y == gridDim.y - 1;
+  if (C::QUANT && !PACKED && (w.P + w.all < TC_TWO_TERMS) != TWO) {  // the other kernel's
+    if (warp == 1) {
+      tmem_dealloc_cols(tmem, 512);
+      tmem_relinquish();
+    }
+    if (beside && last_cta) pdl_wait();
+    return;
+  }
   const int b = w.b, r0 = w.r0, row_lo = w.row_lo, rows = w.rows, n = w.n, len = w.len, P = w.P, np = w.np, own = w.own;
   const int cnt = w.cnt;
   const bool work = w.work;
@@ -550,7 +693,10 @@ many_rows_kernel(const PrefixAttnParams p, const __grid_constant__ Src src, int 
     if constexpr (C::QUANT) quant_producer<HD, PACKED, Src>(p, src, w, b, h, base + (2 + NBUF) * C::TILE, raw_full, raw_empty, s_absent, abort);
   } else if (C::QUANT && warp >= 12) {
     if constexpr (C::QUANT)
-      quant_writer<HD, Src>(w.cnt, ring_u, ring_u + NBUF * C::TILE, full, empty, raw_full, raw_empty, s_absent, abort);
+      if constexpr (TWO)
+        quant_writer_two<HD, Src>(w.cnt, ring_u, ring_u + NBUF * C::TILE, full, empty, raw_full, raw_empty, s_absent, abort);
+      else
+        quant_writer<HD, Src>(w.cnt, ring_u, ring_u + NBUF * C::TILE, full, empty, raw_full, raw_empty, s_absent, abort);
   } else if (warp == 0) {
    if constexpr (!C::QUANT) {
     // ================================ TMA producer ================================
@@ -603,13 +749,24 @@ many_rows_kernel(const PrefixAttnParams p, const __grid_constant__ Src src, int 
       const uint32_t ts = tmem + x * TC_N, to = tmem + 2 * TC_N + x * HD;
       const uint64_t dq = umma_desc_sw128(q_u + x * C::TILE), dk = umma_desc_sw128(ring_u), dv = umma_desc_sw128_mn(ring_u, TC_N * 128);
       auto at = [](uint32_t it) { return (uint64_t)((it % NBUF) * (C::TILE >> 4)); };  // a ring tile, in descriptor units
-      auto wait_full = [&](uint32_t it) { return pa_spin(&full[it % NBUF], (it / NBUF) & 1u, abort); };
+      auto wait_full = [&](uint32_t it) {
+        return pa_spin(&full[it % NBUF], (it / NBUF) & 1u, abort) && (!TWO || pa_spin(&full[(it + 1) % NBUF], ((it + 1) / NBUF) & 1u, abort));
+      };
       auto issue_s = [&](uint32_t it) {  // S = Q K^T
         const uint64_t k = dk + at(it);
 #pragma unroll
         for (int kk = 0; kk < HD / 16; ++kk) {
           const uint32_t off = ((kk >> 2) * (TC_N * 128) + (kk & 3) * 32) >> 4;
           umma_f16(ts, dq + off, k + off, idesc_s, kk != 0);
+        }
+        if constexpr (TWO) {
+          const uint64_t k2 = dk + at(it + 1);
+#pragma unroll
+          for (int kk = 0; kk < HD / 16; ++kk) {
+            const uint32_t off = ((kk >> 2) * (TC_N * 128) + (kk & 3) * 32) >> 4;
+            umma_f16(ts, dq + off, k2 + off, idesc_s, 1);
+          }
+          tc_commit(&empty[(it + 1) % NBUF]);
         }
         tc_commit(&s_full[x]);
         tc_commit(&empty[it % NBUF]);
@@ -620,7 +777,7 @@ many_rows_kernel(const PrefixAttnParams p, const __grid_constant__ Src src, int 
         issue_s(0);
       }
       for (int i = 0; i < cnt && ok; ++i) {
-        const uint32_t vi = 2 * i + 1, ki = 2 * i + 2;
+        const uint32_t vi = TPK * i + TPK - 1, ki = vi + 1;
         ok = pa_spin(&v_clean[vi % NBUF], (vi / NBUF) & 1u, abort);
         const uint64_t v = dv + at(vi);
 #pragma unroll
@@ -646,13 +803,13 @@ many_rows_kernel(const PrefixAttnParams p, const __grid_constant__ Src src, int 
     // ================================ V looked over ================================
     // Every tile passes here before the MMA issuers take it, and is freed as by them: a barrier's parity says which of
     // two phases is over, not which of many.
-    for (uint32_t it = 0; it < 2u * cnt; ++it) {
-      const int s = it % NBUF, t = tile_of((int)(it / 2)), keys = min(TC_N, keys_of(t));
+    for (uint32_t it = 0; it < (uint32_t)TPK * cnt; ++it) {
+      const int s = it % NBUF, t = tile_of((int)(it / TPK)), keys = min(TC_N, keys_of(t));
       if (!__all_sync(0xffffffffu, pa_wait(&full[s], (it / NBUF) & 1u, abort))) break;
       const uint32_t v = ring_u + s * C::TILE;
       // keys from here on are hidden from some row
       const int shown = PACKED || t < np ? keys : max(0, min(keys, w.all - (t - np) * TC_N));
-      if ((it & 1) && shown < TC_N) {
+      if (it % TPK == TPK - 1 && shown < TC_N) {
         for (int e = lane; e < (keys - shown) * 8 * NCH; e += 32) {
           const int r = shown + e / (8 * NCH), c = e % (8 * NCH);
           const uint32_t at = v + (c >> 3) * (TC_N * 128) + r * 128 + ((c & 7) << 4);
@@ -897,6 +1054,7 @@ many_rows_kernel(const PrefixAttnParams p, const __grid_constant__ Src src, int 
     tmem_relinquish();
   }
   if (threadIdx.x == 0 && failed) atomicExch(&g_prefix_attn_error, 1);
+  if (beside && last_cta) pdl_wait();
 }
 
 }  // namespace sc

@@ -42,6 +42,7 @@ struct PrefixAttnParams {
   int pool_rows;       // n_pages * Hkv * page: one past the last row of the pools' tensor maps
   float c;             // scale * log2(e)
   int nslots;          // partial results per row, all kernels of the call together
+  int beside;          // many_rows_kernel with TWO: runs beside the one without
 };
 
 __device__ __forceinline__ float ex2(float x) {

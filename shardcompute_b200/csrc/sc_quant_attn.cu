@@ -136,6 +136,14 @@ __device__ __forceinline__ void lds_share(uint32_t at, uint32_t other, uint32_t 
   }
 }
 
+// Keys of the prefix that the few-rows kernel takes.  PREFIX_SHORT: those of a prefix too short for the many-rows kernel, which then leaves
+// it alone: for its precision (TC_TWO_TERMS), and since a table may hold far more than it does.
+enum { PREFIX_NONE, PREFIX_ALL, PREFIX_SHORT };
+__device__ __forceinline__ int few_rows_prefix(const PrefixAttnParams& p, int with_prefix) {
+  const int P = with_prefix == PREFIX_NONE ? 0 : prefix_keys(p);
+  return with_prefix == PREFIX_SHORT && P >= TC_TWO_TERMS ? 0 : P;
+}
+
 template <typename QB, int NT, bool CLUSTER>
 __global__ void __launch_bounds__(FR_WARPS * 32, CLUSTER ? FewRowsQuant<QB, NT, CLUSTER>::CTAS_CLUSTER : FewRowsQuant<QB, NT, CLUSTER>::CTAS)
 few_rows_quant_kernel(const PrefixAttnParams p, const uint8_t* pages, int with_prefix, int splits, int row_groups, int slot0,
@@ -162,9 +170,9 @@ few_rows_quant_kernel(const PrefixAttnParams p, const uint8_t* pages, int with_p
   }
   __syncthreads();
   // Without the prefix this kernel runs beside the prefix's, as few_rows_kernel does (sc_prefix_attn.cu).
-  if (with_prefix) pdl_wait();
+  if (with_prefix == PREFIX_ALL) pdl_wait();
   pdl_trigger();  // after the wait: the join relies on it
-  const int P = with_prefix ? prefix_keys(p) : 0, np = (int)(((long long)P + KT - 1) / KT);
+  const int P = few_rows_prefix(p, with_prefix), np = (int)(((long long)P + KT - 1) / KT);
   unsigned char* ring = base + (size_t)warp * C::RING;
   const uint32_t ring_u = smem_u32(ring);
   int s_in = 0, s_out = 0;            // the stage that the next tile goes to, that it comes from
@@ -693,7 +701,7 @@ few_rows_quant_kernel(const PrefixAttnParams p, const uint8_t* pages, int with_p
       }
     }
   if (threadIdx.x == 0 && s_abort) atomicExch(&g_prefix_attn_error, 1);
-  if (!with_prefix && blockIdx.x == gridDim.x - 1 && blockIdx.y == gridDim.y - 1 && blockIdx.z == gridDim.z - 1) pdl_wait();
+  if (with_prefix != PREFIX_ALL && blockIdx.x == gridDim.x - 1 && blockIdx.y == gridDim.y - 1 && blockIdx.z == gridDim.z - 1) pdl_wait();
 }
 
 // ---------------------------------------------------------------- join
@@ -707,7 +715,7 @@ __global__ void __launch_bounds__(256) join_stream_kernel(const PrefixAttnParams
   constexpr int V = HD / 32, ROWS = 8 / WPR, N = 8;
   __shared__ float s_o[WPR > 1 ? 8 : 1][HD];
   __shared__ float2 s_ml[WPR > 1 ? 8 : 1];
-  const int b = blockIdx.x, warp = threadIdx.x >> 5, lane = threadIdx.x & 31, part = warp % WPR, P = with_prefix ? prefix_keys(p) : 0;
+  const int b = blockIdx.x, warp = threadIdx.x >> 5, lane = threadIdx.x & 31, part = warp % WPR, P = few_rows_prefix(p, with_prefix);
   const StreamRequest q = stream_request<RT, KT>(p, b, (int)(((long long)P + KT - 1) / KT));
   pdl_wait();
   pdl_trigger();
@@ -923,21 +931,21 @@ static int run_few_rows_quant(const PrefixAttnParams& p, const uint8_t* pages, c
   const cudaError_t e = opt_in<kern>(smem);
   if (e != cudaSuccess) return check_launch("prefix_attn_q", e);
   launch_clusters(CLUSTER ? a.splits : 1, kern, CLUSTER ? dim3(a.splits * a.row_groups, p.Hkv, p.B) : dim3(a.ctas), dim3(FR_WARPS * 32), smem,
-                  stream, p, pages, a.kind == AttnPlan::FEW ? 1 : 0, a.splits, a.row_groups, a.kind == AttnPlan::SHARED ? a.tc_splits : -1, line);
+                  stream, p, pages, a.kind == AttnPlan::FEW ? PREFIX_ALL : PREFIX_SHORT, a.splits, a.row_groups, a.kind == AttnPlan::SHARED ? a.tc_splits : -1, line);
   const int st = check_launch("prefix_attn_q");
   if (CLUSTER || st != SC_OK) return st;
   const long long rows = (long long)p.T * p.Hq;
   const bool wide = a.ctas >= 8 * a.units;  // each unit in eight pieces or more, if all are alike
   const long long y = std::min(std::max(16ll * sm_count() / p.B, 64ll), ((wide ? rows : rows / 8) * 2 + p.B - 1) / p.B);  // twice the mean: requests differ
   launch(wide ? join_stream_kernel<QB::HD, 8 * NT, KEYS, 8> : join_stream_kernel<QB::HD, 8 * NT, KEYS, 1>, dim3(p.B, (unsigned)std::max(1ll, y)), dim3(256), 0, stream, p, line,
-         a.kind == AttnPlan::FEW ? 1 : 0, a.kind == AttnPlan::SHARED ? a.tc_splits : 0);
+         a.kind == AttnPlan::FEW ? PREFIX_ALL : PREFIX_SHORT, a.kind == AttnPlan::SHARED ? a.tc_splits : 0);
   return check_launch("prefix_attn_q_join");
 }
 
-template <typename QB, bool PACKED>
+template <typename QB, bool PACKED, bool TWO>
 static int run_many_rows_quant(const PrefixAttnParams& p, const uint8_t* pages, const QuantPlan& a, cudaStream_t stream) {
   using C = ManyRows<QB::HD, QuantSource<QB>>;
-  constexpr auto kern = many_rows_kernel<QB::HD, PACKED, QuantSource<QB>>;
+  constexpr auto kern = many_rows_kernel<QB::HD, PACKED, QuantSource<QB>, TWO>;
   const cudaError_t e = opt_in<kern>(C::SMEM);
   if (e != cudaSuccess) return check_launch("prefix_attn_q", e);
   launch(kern, dim3((unsigned)(a.tc_splits * a.tc_items), p.Hkv), dim3(C::THREADS), C::SMEM, stream, p, QuantSource<QB>{pages}, a.tc_splits, 0);
@@ -947,13 +955,17 @@ static int run_many_rows_quant(const PrefixAttnParams& p, const uint8_t* pages, 
 template <typename QB>
 static int run_quant_attn(const PrefixAttnParams& p, const uint8_t* pages, const QuantPlan& a, const StreamArgs& line, cudaStream_t stream) {
   if (a.kind == AttnPlan::CHUNKS) {
-    const int st = run_many_rows_quant<QB, false>(p, pages, a, stream);
+    const bool deep = ((long long)(p.max_prefix_blocks + p.max_blocks) << p.lg_page) >= TC_TWO_TERMS;
+    int st = deep ? run_many_rows_quant<QB, false, false>(p, pages, a, stream) : SC_OK;
+    PrefixAttnParams p2 = p;
+    p2.beside = deep;
+    if (st == SC_OK) st = run_many_rows_quant<QB, false, true>(p2, pages, a, stream);
     if (st != SC_OK || a.nslots == 1) return st;
     launch(join_slots_kernel<__half, QB::HD>, dim3((unsigned)(((size_t)p.T * p.Hq + 7) / 8)), dim3(256), 0, stream, p);
     return check_launch("prefix_attn_q_join");
   }
   if (a.kind == AttnPlan::SHARED) {
-    const int st = run_many_rows_quant<QB, true>(p, pages, a, stream);
+    const int st = run_many_rows_quant<QB, true, false>(p, pages, a, stream);
     if (st != SC_OK) return st;
   }
   if (a.splits)

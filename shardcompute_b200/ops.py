@@ -655,8 +655,8 @@ def prefix_attn_q(q: torch.Tensor, pages: QuantPages, q_start: torch.Tensor, kv_
                   workspace: Optional[torch.Tensor] = None) -> torch.Tensor:
     """``prefix_attn`` over pages in 8 or 4 bits: the same rows, tables and lengths; ``q`` and ``out`` [T, Hq hd] are float16.
     The attention is that of what the cache stands for (``paged_read_q``); weights are rounded to float16 before the
-    second product, and so is what k and v stand for where many rows share keys (a prefix, a long chunk); everything else is
-    kept in float32.  ``workspace``: uint8, at least ``prefix_attn_q_workspace_bytes``;
+    second product, and so is what v stands for where many rows share keys (a prefix, a long chunk), and what k does where these
+    rows see 1024 keys or more; everything else is kept in float32.  ``workspace``: uint8, at least ``prefix_attn_q_workspace_bytes``;
     without it scratch is allocated per call, so calls on two streams do not meet."""
     if out is None:
         out = torch.zeros_like(q)

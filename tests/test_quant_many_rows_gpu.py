@@ -1,5 +1,6 @@
 """prefix_attn_q where the many-rows kernel takes part (shared prefixes, chunks): the plan is asserted, and the outputs are compared with
-float64 attention over the very fp16 values that the kernel makes of the codes, in a bound that a lost block of keys breaks."""
+float64 attention over the very fp16 values that the kernel makes of k and v (k in two terms for rows that see few keys), in a bound that a
+lost block of keys breaks."""
 
 import math
 
@@ -27,16 +28,16 @@ def oracle(d, hq, kind, scale=None):
                         1 / math.sqrt(hd) if scale is None else scale, fp16=FP16[kind])
 
 
-def bounds(want, mass, dot, keys, tail, spread, hd):
+def bounds(want, mass, dot, keys, tail, spread, split, hd):
     """How far an output, and the norm of a (row, head), may be off.  With e = 2^-24, p = 2^-11:
       score   S adds 16 dims at a time to an fp32 sum, each time off by at most 2 e of the largest sum; scales, biases and the difference
-              to the maximum are a few roundings more: ds = dot (hd / 16 + 6) 2 e
+              to the maximum are a few roundings more: ds = dot (hd / 16 + 6) 2 e; and split, what two terms of fp16 are off k
       weight  w (1 + 2 ds + 8 e), rounded to fp16 (p; steps of 2^-36 of the largest weight: tail), codes' times s before
       output  mass (2 ds + 16 e + 2 p + 2 e (keys / 8 + 64)) for numerator and denominator, then its rounding to fp16
     In the norm the keys' roundings, up to p each whichever way, are independent of one another: six standard deviations of their sum,
     p / sqrt(3) spread, in place of p mass."""
     e, p = 2.0**-24, 2.0**-11
-    ds = (dot * (hd / 16 + 6) * 2 * e)[..., None]
+    ds = (dot * (hd / 16 + 6) * 2 * e + split)[..., None]
     sums = mass * (2 * ds + 16 * e + 2 * e * (keys[..., None] / 8 + 64)) + 2.0**-36 * 1.01 * tail + 2.0**-25
     last = p * 1.01 * np.abs(want)
     norm = lambda x: np.linalg.norm(x, axis=-1)  # noqa: E731
@@ -132,3 +133,58 @@ def test_hidden_groups_in_chunks(cuda, rng):
             assert torch.equal(out[:first], clean[:first]) and torch.equal(out[300:500], clean[300:500])
             sees, was = out[first:300].view(-1, 8, 64), clean[first:300].view(-1, 8, 64)
             assert sees[..., 32:].isnan().all() and (side == 0 or torch.equal(sees[..., :32], was[..., :32]))
+
+
+@pytest.mark.parametrize("hd,bits,group", KINDS)
+@pytest.mark.parametrize("middle", [0.0, 0.4, 30.0, -1000.0])
+def test_scores_of_codes_beside_a_large_bias(cuda, rng, middle, hd, bits, group):
+    """Keys whose codes the rounding of s c + b to fp16 would lose: two tokens of a prefix with equal scores, though their codes differ (q is
+    the same over eight dims, over which both have one sum), of values 1 and 0.  The output is 1 / (1 + exp(-x)), x the difference of the
+    scores, which two terms of fp16 leave off by no more than the oracle's bound of them and fp32's steps: the scale makes that 2."""
+    hq, T, most = 8, 200, 2**bits - 1
+    codes = rng.integers(0, most + 1, (2, hd // 8, 8))
+    for a, c in ((codes[0, g], codes[1, g]) for g in range(hd // 8)):
+        while a.sum() != c.sum():
+            i = rng.integers(0, 8)
+            c[i] = min(max(c[i] + np.sign(a.sum() - c.sum()), 0), most)
+    n, s = hd // group, np.float16(1.37 / 2**bits)
+    data = np.zeros((1, 1, oq.block_bytes(hd, bits, group)), np.uint8)
+    half = float(s) * 2.0 ** (bits - 1)
+    scales, biases = np.full((1, n), s, np.float16), np.full((1, n), middle - half, np.float16)
+    for t in (0, 1):
+        oq.put(data, t, 16, 0, codes[t].reshape(1, hd), scales, biases, bits, group)
+        oq.put(data, t, 16, 1, np.full((1, hd), t), np.ones((1, n), np.float16), np.zeros((1, n), np.float16), bits, group)
+    q = torch.from_numpy(np.repeat(rng.standard_normal((T, hq, hd // 8)), 8, -1).reshape(T, -1)).half()
+    size = q.double().abs().view(T, hq, hd).sum(-1).max().item()
+    # as in bounds(): split, and (hd / 16 + 6) 2^-23 of sum |q| |k|
+    off = 2.0**-15 * half if abs(middle) < 0.9 * half else 2.0**-11 * half
+    limit = 2 * size * (off + (hd / 16 + 6) * 2.0**-23 * (abs(middle) + half))
+    pages = ops.QuantPages(torch.from_numpy(data).to(cuda), hd, 16, bits, group)
+    i = lambda x: torch.tensor(x, dtype=torch.int32, device=cuda)  # noqa: E731
+    table = torch.full((1, 2048), -1, dtype=torch.int32, device=cuda)  # room for many tokens, none there
+    assert ops.prefix_attn_q_plan(T, 1, hq, 1, hd, 2048, 1, 16, bits, group).kind == "chunks"
+    out = ops.prefix_attn_q(q.to(cuda), pages, i([0, T]), i([0]), table, prefix_table=i([0]), prefix_len=i([2]), scale=2.0 / limit)
+    got = out.double().cpu().numpy()
+    assert (np.abs(np.log(got / (1 - got))) <= 2.008).all(), (got.min(), got.max())
+
+
+@pytest.mark.parametrize("hd,bits,group", [(128, 4, 64), (64, 8, 32)])
+@pytest.mark.parametrize("prefix", [0, 1, 100, 1023, 1024, 2000])
+def test_a_table_for_a_longer_prefix(cuda, rng, prefix, hd, bits, group):
+    """A call planned for a prefix of 4096 that holds less: a short one is the few-rows kernel's, as codes; the same bits every time."""
+    hq, d = shared(rng, hd, bits, group, prefix, 40)
+    page = d["kind"][1]
+    ptab = np.full(4096 // page, -1, np.int32)
+    ptab[:len(d["ptab"])] = d["ptab"]
+    check(cuda, dict(d, ptab=ptab), hq, "shared", prepared=oracle(d, hq, "shared"))
+
+
+@pytest.mark.parametrize("hd,bits,group", [(128, 4, 64), (128, 8, 32), (64, 4, 32), (64, 8, 64)])
+@pytest.mark.parametrize("lens,new,prefix", [([1500], [1500], 0), ([300, 1300, 90], [300, 700, 80], 700), ([3400, 20], [900, 20], 0)])
+def test_rows_that_see_few_keys_beside_rows_that_see_many(cuda, rng, lens, new, prefix, hd, bits, group):
+    """Tiles of rows on both sides of 1024 keys in one call."""
+    d = make_attn(rng, 8, 2, hd, 16, bits, group, prefix, lens, new)
+    page = d["kind"][1]
+    table = np.full((len(lens), 8192 // page), -1, np.int32)
+    table[:, :d["table"].shape[1]] = d["table"]
+    check(cuda, dict(d, table=table), 8, "chunks", prepared=oracle(d, 8, "chunks"))
