@@ -374,8 +374,8 @@ int sc_paged_rope_append_q(const void* qkv, int qkv_dtype, int rows, const int32
                            int Hkv, int hd, void* q_out, void* pages, int bits, int group, int n_pages, int page_size,
                            cudaStream_t stream);
 /* The tokens in `slots`, read back: k_out, v_out [rows, Hkv, hd] in out_dtype
- * (fp16 or fp32): s c + b in fp32, rounded once.  Zeros for a slot outside the
- * pool.  Rows from *rows_end on are left as they were (NULL: none).  A slot may
+ * (fp16 or fp32): s c + b in fp32, then rounded to fp16 where that is asked for.
+ * Zeros for a slot outside the pool.  Rows from *rows_end on are left as they were (NULL: none).  A slot may
  * be named more than once. */
 int sc_paged_read_q(const void* pages, int bits, int group, int n_pages, int page_size, int Hkv, int hd,
                     const int32_t* slots, int rows, const int32_t* rows_end, void* k_out, void* v_out, int out_dtype,

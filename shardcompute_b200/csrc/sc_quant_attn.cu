@@ -62,7 +62,9 @@ struct FewRowsQuant {
   static constexpr int RING = NST * STAGE > OUT ? NST * STAGE : OUT;
   static constexpr int QBYTES = NT * KSTEPS * 256;  // q's fragments
   static constexpr int SMEM = FR_WARPS * RING + QBYTES;
-  // CTAs of an SM, by shared memory and by the registers that they need without spills
+  // CTAs of an SM, by shared memory and by registers, of which they leave too few in some instances: 4 bits, heads of 128, groups of 64, 92 bytes
+  // are spilled on the line and 112 in clusters; groups of 32, 124 and, tiles of 16 rows in clusters, 220; 8 bits, groups of 64, 120 with
+  // such tiles on the line.
   static constexpr int CTAS = NT == 1 ? (SMEM > 56000 ? 3 : SMEM > 44000 || QB::NG == 4 || QB::BYTES > 4300 ? 4 : 5) : QB::NG == 4 || SMEM > 75000 ? 2 : 3;
   static constexpr int CTAS_CLUSTER = NT == 1 ? (CTAS < 4 ? CTAS : QB::NG == 4 ? 3 : 4) : 2;
 };

@@ -90,8 +90,8 @@ __device__ __forceinline__ uint32_t pack4(const uint32_t (&c)[4]) {
 // quantise), and q is rounded once.  The HD/8 items of a k or v head lie in
 // neighbouring lanes, which find their groups' extremes by shuffles and write
 // the codes.  Moves its bytes once; bound by the loads' latency, three in a row (8150
-// rows of 40 heads of 64, fp32, in 8 bits: 122 MB in 24.6 us, 5.0 TB/s; with 40 registers in place of 32 26.4, with two items a
-// thread 28.1, with four 35.5; 32 rows of 48 heads of 128: 2.6 us).
+// rows of 40 heads of 64, fp32, in 8 bits: 122 MB in 25.3 us, 4.8 TB/s, from fp16 23.1; 32 rows of 48 heads of 128: 2.6 us).  The 32 registers
+// that eight CTAs an SM leave spill 16 to 24 bytes: with 40 it took 26.4 us for 24.6 then, with two items a thread 28.1, with four 35.5.
 template <typename ST, typename QB>
 __global__ void __launch_bounds__(256, 8) append_quant_kernel(const AppendQuantParams p) {
   constexpr int HD = QB::HD, HALF = HD / 2, LPH = HD / 8, NG = QB::NG, GS = QB::GS;
@@ -183,8 +183,8 @@ struct ReadQuantParams {
 __device__ __forceinline__ float code_f32(uint32_t c) { return __uint_as_float(0x4b000000u | c) - 8388608.f; }
 
 // An item is sixteen values of a head of a row's K or V, four times four 32
-// apart, so that the items of a head store whole sectors together: s c + b in fp32,
-// rounded once.  With one group of four an item, finding its place was most of
+// apart, so that the items of a head store whole sectors together: s c + b in fp32
+// (one rounding, where a bias is far from its scale), then in the output's type.  With one group of four an item, finding its place was most of
 // the instructions (40000 rows of 8 heads of 128 in 8 bits to fp32 114 us).
 template <typename OT, typename QB>
 __global__ void __launch_bounds__(256) read_quant_kernel(const ReadQuantParams p) {

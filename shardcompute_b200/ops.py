@@ -594,7 +594,7 @@ def paged_rope_append_q(qkv: torch.Tensor, q_start: torch.Tensor, slots: torch.T
 def paged_read_q(pages: QuantPages, slots: torch.Tensor, q_start: Optional[torch.Tensor] = None, k_out: Optional[torch.Tensor] = None,
                  v_out: Optional[torch.Tensor] = None, dtype: torch.dtype = _F16):
     """The tokens that ``slots`` [T] hold, as ``(k, v)`` [T, Hkv, hd] of ``dtype`` (float16 or float32; that of ``k_out`` and
-    ``v_out`` where they are given): what the cache stands for, rounded once.  Zeros for a slot outside the pool.  With
+    ``v_out`` where they are given): what the cache stands for in float32, and that rounded to float16.  Zeros for a slot outside the pool.  With
     ``q_start`` rows from ``q_start[-1]`` on are left as they were."""
     data, hd, page, bits, group = pages
     if k_out is not None and v_out is not None and _native().paged_read_q(slots, data, hd, page, bits, group, q_start, k_out, v_out) == 0:

@@ -11,6 +11,10 @@ are held once and attended to once for the whole batch.
 With ``bits`` 8 or 4 the pages hold codes (``ops.QuantPages``): a quarter to a half of float16's room, 72 bytes in place of
 256 for a token's key or value of a head of 128.  Keys and values are quantised as they are written and attended to as they
 lie; ``read`` gives back what the cache stands for.
+
+The attention is cut by what the tables have room for, since the lengths live on the device: ``max_len`` and ``max_prefix`` far
+past what is held cost time (64 requests behind 8197 tokens with room for 32768: the prefix's kernel runs as 8 CTAs, not 48), not
+correctness.  ``ops.prefix_attn_q_plan`` says how a call is cut.
 """
 
 from __future__ import annotations
