@@ -10,7 +10,7 @@ def floor16(x):
     x = np.asarray(x, np.float64)
     with np.errstate(over="ignore"):
         h = x.astype(np.float16)
-    h = np.where(h.astype(np.float64) > x, np.nextafter(h, np.float16(-np.inf)), h)
+        h = np.where(h.astype(np.float64) > x, np.nextafter(h, np.float16(-np.inf)), h)
     return h.astype(np.float16)
 
 

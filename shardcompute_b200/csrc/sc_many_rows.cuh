@@ -670,7 +670,7 @@ many_rows_kernel(const PrefixAttnParams p, const __grid_constant__ Src src, int 
   RowShare w = row_share<PACKED, 2 * TC_M, TC_N, C::THREADS>(p, item, split, splits, s_req, s_row0, s_sum);
   if (C::QUANT && PACKED && w.P < TC_TWO_TERMS) w.P = w.np = w.cnt = 0;  // few_rows_quant_kernel's
   const bool last_cta = blockIdx.x == gridDim.x - 1 && blockIdx.y == gridDim.y - 1;
-  if (C::QUANT && !PACKED && (w.P + w.all < TC_TWO_TERMS) != TWO) {  // the other kernel's
+  if (C::QUANT && !PACKED && (w.P < TC_TWO_TERMS && w.all < TC_TWO_TERMS - w.P) != TWO) {  // the other kernel's
     if (warp == 1) {
       tmem_dealloc_cols(tmem, 512);
       tmem_relinquish();

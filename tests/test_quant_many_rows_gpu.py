@@ -188,3 +188,74 @@ def test_rows_that_see_few_keys_beside_rows_that_see_many(cuda, rng, lens, new, 
     table = np.full((len(lens), 8192 // page), -1, np.int32)
     table[:, :d["table"].shape[1]] = d["table"]
     check(cuda, dict(d, table=table), 8, "chunks", prepared=oracle(d, 8, "chunks"))
+
+
+def wide(d, tokens=8192):
+    """The same call with a block table that could hold `tokens` a request."""
+    table = np.full((len(d["lens"]), tokens // d["kind"][1]), -1, np.int32)
+    table[:, :d["table"].shape[1]] = d["table"]
+    return dict(d, table=table)
+
+
+def test_hidden_groups_in_chunks_of_few_keys(cuda, rng):
+    """As test_hidden_groups_in_chunks, where k is taken as two terms."""
+    d = wide(make_attn(rng, 8, 1, 64, 16, 4, 32, 20, [400, 250], [300, 200], dirty=False))
+    assert plan_of(d, 8).kind == "chunks"
+    clean = run_attn(cuda, d)
+    first = 350 - 100  # the row that first sees token 350
+    for side in (0, 1):
+        for scale in (np.inf, 1.0):
+            e = dict(d, data=d["data"].copy())
+            at = oq.meta_place(side, 350 % 16, 1, 64, 4, 32)
+            e["data"][d["table"][0, 350 // 16], :, at:at + 4] = np.array([scale, np.nan], np.float16).view(np.uint8)
+            out = run_attn(cuda, e)
+            assert torch.equal(out[:first], clean[:first]) and torch.equal(out[300:500], clean[300:500])
+            sees, was = out[first:300].view(-1, 8, 64), clean[first:300].view(-1, 8, 64)
+            assert sees[..., 32:].isnan().all() and (side == 0 or torch.equal(sees[..., :32], was[..., :32]))
+
+
+@pytest.mark.parametrize("hd,bits,group", [(128, 4, 64), (128, 8, 64), (64, 8, 32)])
+def test_keys_at_the_ends_of_fp16s_range_in_chunks(cuda, rng, hd, bits, group):
+    """Groups of k that reach +-65504: neither term of theirs, nor the one, becomes an infinity."""
+    for lens, new in (([300, 90], [200, 80]), ([1500], [300])):
+        d = wide(make_attn(rng, 8, 2, hd, 16, bits, group, 0, lens, new, dirty=False))
+        k = rng.uniform(-1, 1, (len(d["data"]), 2, 16, hd // group, group)) * 65504 * rng.choice([1.0, 0.6, 0.3], (len(d["data"]), 2, 16, hd // group, 1))
+        k[..., 0], k[..., 1] = 65504 * rng.choice([1, 0.9, -0.5], k.shape[:-1]), -65504 * rng.choice([1, 0.8, -0.7], k.shape[:-1])
+        v = rng.standard_normal((len(d["data"]), 2, 16, hd)) + 0.3
+        d["data"] = oq.fill(k.reshape(v.shape).astype(np.float32), v.astype(np.float32), bits, group)
+        d["q"] = (d["q"] * 2e-5).half()
+        check(cuda, d, 8, "chunks")
+
+
+def test_captured_chunks(cuda, rng):
+    """Chunks on both sides of 1024 keys and a shared prefix, captured with one workspace and replayed in turn, and on two streams at once."""
+    i = lambda a: torch.from_numpy(np.ascontiguousarray(np.asarray(a, np.int32))).to(cuda)  # noqa: E731
+    ds = [(8, wide(make_attn(rng, 8, 2, 128, 16, 4, 64, 0, [1500, 90], [1200, 80]))), (8, wide(make_attn(rng, 8, 2, 64, 16, 8, 32, 1100, [500], [400]))),
+          shared(rng, 64, 4, 32, 2900, 40), (32, wide(make_attn(rng, 32, 8, 128, 16, 4, 64, 40, [300] * 12, [290] * 12)))]
+    ws, calls = torch.empty(256 << 20, dtype=torch.uint8, device=cuda), []
+    for hq, d in ds:
+        t = [d["q"].to(cuda), ops.QuantPages(torch.from_numpy(d["data"]).to(cuda), *d["kind"]), i(d["start"]), i(d["lens"]), i(d["table"])]
+        pre = dict(prefix_table=i(d["ptab"]), prefix_len=i([d["prefix"]]))
+        want, out = ops.prefix_attn_q(*t, **pre), torch.zeros_like(t[0])
+        graph = torch.cuda.CUDAGraph()
+        torch.cuda.synchronize()
+        with torch.cuda.graph(graph):
+            ops.prefix_attn_q(*t, out=out, workspace=ws, **pre)
+        calls.append((graph, out, want, t, pre))
+    assert {plan_of(d, hq).kind for hq, d in ds} == {"chunks", "shared"}
+    for _ in range(5):
+        for graph, out, *_ in calls:
+            out.zero_()
+            graph.replay()
+        for _, out, want, *_ in calls:
+            assert torch.equal(out, want)
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    torch.cuda.synchronize()
+    for _ in range(5):
+        outs = []
+        for n, (_, _, want, t, pre) in enumerate(calls):
+            with torch.cuda.stream(streams[n % 2]):
+                outs.append(ops.prefix_attn_q(*t, **pre))
+        torch.cuda.synchronize()
+        for o, (_, _, want, *_) in zip(outs, calls):
+            assert torch.equal(o, want)
